@@ -308,6 +308,120 @@ int32_t nca_b200_run_steps_static(const NcaModelDesc* m, const NcaBatchDesc* b,
                                   int32_t n_steps, const NcaFireDesc* fire, int32_t timeout_ms,
                                   void* stream);
 
+/* ---- cell-training operators -------------------------------------------------------------- */
+/* Group norm with an activation (channels last), the gated feed-forward block, and distillation
+ * from a teacher's top logits, each with its gradient: what a normalised, gated cell
+ * (NCAConfig.norm_groups, update "swiglu") and its training need beside the rollout.
+ *
+ * Strides are in elements and may be any size_t-addressable value; every product of indexes and
+ * strides is formed in 64 bits.  Outputs are contiguous.  Zero sizes are valid: nothing is read,
+ * and gradients of parameters are written as zeros.  Results do not depend on the launch order of
+ * blocks: no floating-point atomics.  `workspace` is device scratch of the size that the
+ * operator's *_workspace query returns (256-byte aligned); it carries nothing between calls. */
+typedef enum NcaDtype { NCA_F32 = 0, NCA_BF16 = 1, NCA_F16 = 2 } NcaDtype;
+
+typedef enum NcaAct {
+  NCA_ACT_NONE = 0,
+  NCA_ACT_RELU = 1,
+  NCA_ACT_SILU = 2,     /* z / (1 + exp(-z)) */
+  NCA_ACT_GELU = 3,     /* z / 2 (1 + erf(z / sqrt 2)) */
+  NCA_ACT_SIGMOID = 4
+} NcaAct;
+
+/* y = act((x - mean) / sqrt(var + eps) * weight + bias), mean and (biased) variance over the cells
+ * of a sample and the channels / groups channels of a group.  With a mask, only cells whose mask
+ * is non-zero count; the others are not read, and their y and dx are zero (a sample without any
+ * such cell gives zeros). */
+typedef struct NcaNormDesc {
+  int64_t n, cells;             /* samples, cells per sample */
+  int32_t channels, groups;     /* groups divides channels */
+  int32_t dtype;                /* NcaDtype of x, y, dy, dx */
+  int32_t param_dtype;          /* NcaDtype of weight, bias and their gradients: NCA_F32 or dtype */
+  int32_t act;                  /* NcaAct */
+  float eps;
+  int64_t x_stride_n, x_stride_cell;    /* channels are adjacent */
+  int64_t dy_stride_n, dy_stride_cell;
+  int64_t mask_stride_n, mask_stride_cell;
+} NcaNormDesc;
+
+int32_t nca_b200_group_norm_workspace(const NcaNormDesc* d, int32_t backward, size_t* bytes);
+/* stats: device [n][groups][2] fp32, receives each group's mean and 1 / sqrt(var + eps) (the
+ * backward call reads it).  weight, bias, mask (uint8) may be NULL. */
+int32_t nca_b200_group_norm(const NcaNormDesc* d, const void* x, const void* weight,
+                            const void* bias, const uint8_t* mask, void* y, float* stats,
+                            void* workspace, size_t workspace_bytes, void* stream);
+/* dx, dweight, dbias may be NULL. */
+int32_t nca_b200_group_norm_backward(const NcaNormDesc* d, const void* x, const void* weight,
+                                     const void* bias, const uint8_t* mask, const float* stats,
+                                     const void* dy, void* dx, void* dweight, void* dbias,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = (act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down, weights as (out, in).
+ * One matrix type (bf16 or fp16) for x, the weights, y and all gradients; products are summed in
+ * fp32.  h = act(gate) * up, dgate and dup are rounded to that type in between. */
+typedef struct NcaGatedDesc {
+  int64_t rows;
+  int64_t d_in, hidden, d_out;
+  int32_t dtype;                 /* NCA_BF16 or NCA_F16 */
+  int32_t bias_dtype;            /* NCA_F32 or dtype, for the biases and their gradients */
+  int32_t act;                   /* NCA_ACT_RELU, _SILU, _GELU or _SIGMOID */
+  int32_t unaligned;             /* bit i set: pointer i (x, w_gate, w_up, w_down, dy) is not a
+                                    multiple of 16 bytes */
+  int64_t x_stride[2];           /* (row, column) strides */
+  int64_t w_gate_stride[2], w_up_stride[2], w_down_stride[2];
+  int64_t dy_stride[2];
+} NcaGatedDesc;
+
+/* Bytes of the buffer `saved` that a training forward fills for the backward call: gate and up
+ * (the upper 24 bits of their fp32 values) and h, 8 bytes an element of [rows][hidden up to 8]. */
+int32_t nca_b200_gated_saved_bytes(const NcaGatedDesc* d, size_t* bytes);
+/* The workspace holds copies of the operands that the tensor-memory accelerator cannot read as they
+ * lie (columns not adjacent, rows or pointer not on 16-byte boundaries), h of an inference call,
+ * and the backward's intermediates. */
+int32_t nca_b200_gated_workspace(const NcaGatedDesc* d, int32_t backward, size_t* bytes);
+/* saved: NULL for inference (h then lives in the workspace).  Biases may be NULL.  ctrl: 4 x int32
+ * control words as for nca_b200_run_steps; a wait that exceeds timeout_ms gives up and sets them. */
+int32_t nca_b200_gated_ffn(const NcaGatedDesc* d, const void* x, const void* w_gate,
+                           const void* w_up, const void* w_down, const void* b_gate,
+                           const void* b_up, const void* b_down, void* y, void* saved,
+                           void* workspace, size_t workspace_bytes, int32_t* ctrl,
+                           int32_t timeout_ms, void* stream);
+/* Any gradient may be NULL and is then not computed. */
+int32_t nca_b200_gated_ffn_backward(const NcaGatedDesc* d, const void* x, const void* w_gate,
+                                    const void* w_up, const void* w_down, const void* saved,
+                                    const void* dy, void* dx, void* dw_gate, void* dw_up,
+                                    void* dw_down, void* db_gate, void* db_up, void* db_down,
+                                    void* workspace, size_t workspace_bytes, int32_t* ctrl,
+                                    int32_t timeout_ms, void* stream);
+
+/* loss[r] = weight[r] tau^2 sum_k p_k (log p_k - log q[index_k]), p = softmax(teacher[r] / tau)
+ * over the row's entries, q = softmax(logits[r] / tau) over all classes.  An entry whose index is
+ * outside [0, classes) is no entry; entries with teacher -inf have p = 0.  Entries of one class
+ * add up.  A row without entries, or with weight 0, gives loss 0 and gradient 0, whatever its
+ * logits hold; otherwise a row whose logits hold NaN or +inf, or -inf only, gives NaN. */
+typedef struct NcaDistillDesc {
+  int64_t rows;
+  int64_t classes;               /* < 2^31 */
+  int64_t top;
+  int32_t dtype, teacher_dtype;  /* NcaDtype */
+  int32_t index_bits;            /* 32 or 64 */
+  float temperature;             /* tau > 0 */
+  int64_t logits_stride, teacher_stride, index_stride;   /* row strides; classes are adjacent */
+} NcaDistillDesc;
+
+int32_t nca_b200_distill_workspace(const NcaDistillDesc* d, size_t* bytes);
+/* loss: device [rows] fp32.  dlogits (may be NULL): the gradient of sum(loss), in the logits' type.
+ * stats (may be NULL): device [rows][2] fp32, the largest logit and sum exp((logit - largest) / tau),
+ * for the backward call. */
+int32_t nca_b200_distill(const NcaDistillDesc* d, const void* logits, const void* teacher,
+                         const void* index, const float* weight, float* loss, float* stats,
+                         void* dlogits, void* workspace, size_t workspace_bytes, void* stream);
+/* dlogits[r] = grad[r * grad_stride] * d loss[r] / d logits[r]; grad_stride 0 broadcasts one value. */
+int32_t nca_b200_distill_backward(const NcaDistillDesc* d, const void* logits, const void* teacher,
+                                  const void* index, const float* weight, const float* stats,
+                                  const float* grad, int64_t grad_stride, void* dlogits,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -114,6 +114,58 @@ class NcaFireDesc(C.Structure):
     ]
 
 
+class NcaNormDesc(C.Structure):
+    _fields_ = [
+        ("n", C.c_int64),
+        ("cells", C.c_int64),
+        ("channels", C.c_int32),
+        ("groups", C.c_int32),
+        ("dtype", C.c_int32),
+        ("param_dtype", C.c_int32),
+        ("act", C.c_int32),
+        ("eps", C.c_float),
+        ("x_stride_n", C.c_int64),
+        ("x_stride_cell", C.c_int64),
+        ("dy_stride_n", C.c_int64),
+        ("dy_stride_cell", C.c_int64),
+        ("mask_stride_n", C.c_int64),
+        ("mask_stride_cell", C.c_int64),
+    ]
+
+
+class NcaGatedDesc(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64),
+        ("d_in", C.c_int64),
+        ("hidden", C.c_int64),
+        ("d_out", C.c_int64),
+        ("dtype", C.c_int32),
+        ("bias_dtype", C.c_int32),
+        ("act", C.c_int32),
+        ("unaligned", C.c_int32),
+        ("x_stride", C.c_int64 * 2),
+        ("w_gate_stride", C.c_int64 * 2),
+        ("w_up_stride", C.c_int64 * 2),
+        ("w_down_stride", C.c_int64 * 2),
+        ("dy_stride", C.c_int64 * 2),
+    ]
+
+
+class NcaDistillDesc(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64),
+        ("classes", C.c_int64),
+        ("top", C.c_int64),
+        ("dtype", C.c_int32),
+        ("teacher_dtype", C.c_int32),
+        ("index_bits", C.c_int32),
+        ("temperature", C.c_float),
+        ("logits_stride", C.c_int64),
+        ("teacher_stride", C.c_int64),
+        ("index_stride", C.c_int64),
+    ]
+
+
 # name -> (restype, argtypes); must match include/nca_b200.h
 _P = C.c_void_p
 _I = C.c_int32
@@ -173,6 +225,16 @@ SIGNATURES = {
         _I,
         [C.POINTER(NcaModelDesc), C.POINTER(NcaBatchDesc), _I, _P, _P, _I, C.POINTER(NcaFireDesc), _I, _P],
     ),
+    "nca_b200_group_norm_workspace": (_I, [C.POINTER(NcaNormDesc), _I, C.POINTER(C.c_size_t)]),
+    "nca_b200_group_norm": (_I, [C.POINTER(NcaNormDesc), *[_P] * 7, C.c_size_t, _P]),
+    "nca_b200_group_norm_backward": (_I, [C.POINTER(NcaNormDesc), *[_P] * 10, C.c_size_t, _P]),
+    "nca_b200_gated_saved_bytes": (_I, [C.POINTER(NcaGatedDesc), C.POINTER(C.c_size_t)]),
+    "nca_b200_gated_workspace": (_I, [C.POINTER(NcaGatedDesc), _I, C.POINTER(C.c_size_t)]),
+    "nca_b200_gated_ffn": (_I, [C.POINTER(NcaGatedDesc), *[_P] * 10, C.c_size_t, _P, _I, _P]),
+    "nca_b200_gated_ffn_backward": (_I, [C.POINTER(NcaGatedDesc), *[_P] * 14, C.c_size_t, _P, _I, _P]),
+    "nca_b200_distill_workspace": (_I, [C.POINTER(NcaDistillDesc), C.POINTER(C.c_size_t)]),
+    "nca_b200_distill": (_I, [C.POINTER(NcaDistillDesc), *[_P] * 8, C.c_size_t, _P]),
+    "nca_b200_distill_backward": (_I, [C.POINTER(NcaDistillDesc), *[_P] * 6, C.c_int64, _P, _P]),
 }
 
 _lib: C.CDLL | None = None

@@ -17,12 +17,14 @@ OUT = ROOT / "_lib" / "libnca_b200.so"
 # api.cu holds the entry points and small kernels; each steps_<C>_<HD>.cu the step-kernel
 # instances of one model shape (compiled in parallel, then linked into one library)
 SOURCES = [CSRC / "api.cu", CSRC / "steps_64_256.cu", CSRC / "steps_32_128.cu",
-           CSRC / "steps_16_128.cu", CSRC / "steps_32_256.cu"]
-HEADERS = [CSRC / "ptx.cuh", CSRC / "step_kernel.cuh", CSRC / "launch.cuh",
+           CSRC / "steps_16_128.cu", CSRC / "steps_32_256.cu",
+           CSRC / "norm.cu", CSRC / "gated.cu", CSRC / "distill.cu"]  # the cell-training operators
+HEADERS = [CSRC / "ptx.cuh", CSRC / "step_kernel.cuh", CSRC / "launch.cuh", CSRC / "cell_ops.cuh",
+           CSRC / "gemm.cuh",
            ROOT.parent / "include" / "nca_b200.h"]
 DEPS = SOURCES + HEADERS
 # the torch operators over the C ABI (ncas_b200._ops), linked against libnca_b200.so
-OPS_SOURCE = CSRC / "torch_ops.cpp"
+OPS_SOURCES = [CSRC / "torch_ops.cpp", CSRC / "operators_torch.cpp"]
 OPS_OUT = ROOT / "_lib" / "libnca_b200_ops.so"
 
 ARCH_FLAGS = [
@@ -48,7 +50,7 @@ def up_to_date() -> bool:
     if not OUT.exists() or not OPS_OUT.exists():
         return False
     t = min(OUT.stat().st_mtime, OPS_OUT.stat().st_mtime)
-    return all(p.stat().st_mtime <= t for p in DEPS + [OPS_SOURCE] if p.exists())
+    return all(p.stat().st_mtime <= t for p in DEPS + OPS_SOURCES if p.exists())
 
 
 def _torch_flags() -> tuple[list[str], list[str]]:
@@ -80,9 +82,12 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         procs.append((cmd, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE,
                                                  text=True)))
     cflags, libs = _torch_flags()
-    ops_obj = objdir / "torch_ops.o"
-    ops_cmd = ["g++", "-O2", "-std=c++17", "-fPIC", *cflags, "-c", "-o", str(ops_obj), str(OPS_SOURCE)]
-    ops_proc = subprocess.Popen(ops_cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+    ops_procs = []
+    for src in OPS_SOURCES:
+        obj = objdir / (src.stem + ".o")
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", *cflags, "-c", "-o", str(obj), str(src)]
+        ops_procs.append((cmd, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE,
+                                                     text=True)))
     objs = []
     for cmd, obj, p in procs:
         out, err = p.communicate()
@@ -97,11 +102,14 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"nvcc link failed ({' '.join(cmd)}):\n{res.stdout}\n{res.stderr}")
     tmp.replace(OUT)
-    out, err = ops_proc.communicate()
-    if ops_proc.returncode != 0:
-        raise RuntimeError(f"g++ failed ({' '.join(ops_cmd)}):\n{out}\n{err}")
+    ops_objs = []
+    for cmd, obj, p in ops_procs:
+        out, err = p.communicate()
+        if p.returncode != 0:
+            raise RuntimeError(f"g++ failed ({' '.join(cmd)}):\n{out}\n{err}")
+        ops_objs.append(str(obj))
     tmp = OPS_OUT.with_suffix(".so.tmp")
-    cmd = ["g++", "-shared", "-o", str(tmp), str(ops_obj), f"-L{OUT.parent}", "-lnca_b200",
+    cmd = ["g++", "-shared", "-o", str(tmp), *ops_objs, f"-L{OUT.parent}", "-lnca_b200",
            "-Wl,-rpath,$ORIGIN", *libs]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:

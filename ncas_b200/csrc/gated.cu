@@ -1,0 +1,557 @@
+// gated.cu -- the gated feed-forward block, forward and backward (nca_b200_gated_*), on the tcgen05
+// product kernel of gemm.cuh.  With T rows, D inputs, F hidden, O outputs:
+//
+//   forward   gate = x Wg^T + bg, up = x Wu^T + bu, h = act(gate) up       one product, fused epilogue
+//             y = h Wd^T + bd                                              one product
+//   backward  dh = dy Wd;  dgate = dh up act'(gate), dup = dh act(gate)    one product, fused epilogue
+//             dx = dgate Wg + dup Wu                                       one product, k axis 2 F
+//             dWd = dy^T h;  dWg = dgate^T x, dWu = dup^T x                products over the T rows
+//             db = column sums of dgate, dup, dy
+//
+// Roundings: h, dgate and dup are rounded once to the matrix type, since they are operands of the
+// next 16-bit product; gate and up are kept for the backward with 24 bits; sums stay in fp32.
+//
+// The products over T rows have small outputs and a long k axis in a cell model: the axis is then
+// cut into pieces whose fp32 sums are added in a fixed order by a second kernel.
+#include "gemm.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+using namespace nca;
+
+namespace {
+
+inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+inline long long pad8(long long v) { return (v + 7) / 8 * 8; }
+
+constexpr int kMaxDevices = 64;
+
+int sm_count() {
+  static std::atomic<int> kept[kMaxDevices];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  n = kept[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    kept[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static std::atomic<EncodeFn> kept{nullptr};
+  EncodeFn f = kept.load(std::memory_order_acquire);
+  if (!f) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    f = reinterpret_cast<EncodeFn>(p);
+    kept.store(f, std::memory_order_release);
+  }
+  return f;
+}
+
+// A 16-bit matrix that TMA can read: `cols` adjacent values a row, rows `ld` values apart.
+struct Matrix {
+  const void* p;
+  long long rows, cols, ld;
+};
+
+// Boxes of 64 columns (128 bytes, swizzled) x box_rows rows; outside reads as zero.
+bool encode(CUtensorMap* map, const Matrix& m, int dtype, int box_rows) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)m.ld * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  const cuuint32_t one[2] = {1, 1};
+  return fn(map, dtype == NCA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+            const_cast<void*>(m.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// ------------------------------------------------------------------------------- small kernels
+// dst[r][c] = src[r * sr + c * sc]: an operand that TMA cannot read, copied to padded rows.  32 x 32
+// tiles through shared memory, read along whichever stride is 1.
+__global__ void pack_kernel(const uint16_t* src, long long rows, long long cols, long long sr, long long sc,
+                            uint16_t* dst, long long ld) {
+  __shared__ uint16_t tile[32][34];
+  const long long ct = (cols + 31) / 32, tiles = ct * ((rows + 31) / 32);
+  for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const long long r0 = t / ct * 32, c0 = t % ct * 32;
+    __syncthreads();
+    for (int i = threadIdx.y; i < 32; i += 8) {
+      const int r = sr == 1 ? threadIdx.x : i, c = sr == 1 ? i : threadIdx.x;
+      if (r0 + r < rows && c0 + c < cols) tile[r][c] = src[(r0 + r) * sr + (c0 + c) * sc];
+    }
+    __syncthreads();
+    for (int i = threadIdx.y; i < 32; i += 8)
+      if (r0 + i < rows && c0 + threadIdx.x < cols) dst[(r0 + i) * ld + c0 + threadIdx.x] = tile[i][threadIdx.x];
+  }
+}
+
+// c[z][m][n] = sum over the pieces of part[s * batch + z][m][n], in the order of s.
+template <class T>
+__global__ void join_kernel(const float* part, int splits, int batch, long long m, long long n, long long ldp,
+                            T* c0, T* c1) {
+  const long long total = batch * m * n;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
+       i += (long long)gridDim.x * blockDim.x) {
+    const long long z = i / (m * n), r = (i - z * m * n) / n, c = i - z * m * n - r * n;
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += part[((long long)(k * batch + z) * m + r) * ldp + c];
+    (z ? c1 : c0)[r * n + c] = from_f32<T>(s);
+  }
+}
+
+// Column sums of a [rows][cols] matrix in two steps of a fixed order.
+template <class T>
+__global__ void column_sums_kernel(const T* a, long long rows, long long cols, long long ld, int splits, float* part) {
+  __shared__ float red[8][33];
+  const long long c = (long long)blockIdx.x * 32 + threadIdx.x;
+  const long long per = (rows + splits - 1) / splits, r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
+  float s = 0.f;
+  if (c < cols)
+    for (long long r = r0 + threadIdx.y; r < r1; r += 8) s += to_f32(a[r * ld + c]);
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < cols) {
+    for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x];
+    part[(long long)blockIdx.y * cols + c] = s;
+  }
+}
+__global__ void column_store_kernel(const float* part, int splits, long long cols, void* out, int dtype) {
+  const long long c = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.f;
+  for (int k = 0; k < splits; ++k) s += part[(long long)k * cols + c];
+  store_param(out, dtype, c, s);
+}
+constexpr int kSumSplits = 64;
+
+// --------------------------------------------------------------------------------- the products
+template <class T, int CG, int BN, bool A_MN, bool B_MN, int EPI, int ACT>
+int32_t launch(GemmParams& p, cudaStream_t s) {
+  using S = GemmShape<CG, BN>;
+  constexpr int kTN = EPI == EPI_GATE ? BN / 2 : BN;
+  auto* kernel = gemm_kernel<T, CG, BN, A_MN, B_MN, EPI, ACT>;
+  static std::atomic<uint64_t> ready{0};  // a bit for each device whose shared-memory limit is set
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
+  if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
+      return launch_status() == NCA_OK ? NCA_ERR_CUDA : NCA_ERR_DEVICE;
+    ready.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  p.m_tiles = (int)ceil_div(p.m, kBM * CG);
+  p.n_tiles = (int)ceil_div(p.n, kTN);
+  const long long tiles = (long long)p.m_tiles * p.n_tiles * p.batch * p.splits;
+  if (tiles > (1ll << 31) - 1024) return NCA_ERR_UNSUPPORTED;
+  const long long room = sm_count() / CG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((tiles < room ? tiles : room) * CG));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+    cudaGetLastError();
+    return NCA_ERR_CUDA;
+  }
+  return launch_status();
+}
+
+// Pairs of multiprocessors (256 x 256 tiles) when their tiles occupy the GPU, single ones
+// (128 x 128 tiles) otherwise.
+struct Shape {
+  bool pair;
+  int splits;
+};
+Shape shape_of(long long m, long long n, int batch, long long kb, bool may_split, bool gate) {
+  const long long sms = sm_count();
+  const long long big = ceil_div(m, 256) * ceil_div(n, gate ? 128 : 256) * batch;
+  if (big >= sms / 2) return {true, 1};
+  if (may_split && kb >= 64 && big * kb >= sms / 2 * 16) {
+    const long long s = std::max(1ll, std::min(sms / 2 / big, kb / 16));
+    return {true, (int)s};
+  }
+  const long long small = ceil_div(m, 128) * ceil_div(n, gate ? 64 : 128) * batch;
+  long long s = 1;
+  if (may_split) s = std::max(1ll, std::min(sms / small, kb / 8));
+  return {false, (int)s};
+}
+
+struct Product {
+  Matrix a[2], b[2];
+  bool two_a, two_b;     // a[1] / b[1] present
+  long long m, n, k;     // k: one source's length
+  bool k_sources;        // a[1], b[1] continue the k axis
+  int batch;
+};
+
+int32_t set_up(GemmParams& p, const Product& g, int dtype, bool a_mn, bool b_mn, int cg, int bn, bool gate) {
+  const int bnc = gate ? bn / 2 : bn / cg;
+  for (int i = 0; i < 2; ++i) {
+    const Matrix& a = i && g.two_a ? g.a[1] : g.a[0];
+    const Matrix& b = i && g.two_b ? g.b[1] : g.b[0];
+    if (!encode(&p.a[i], a, dtype, a_mn ? 64 : kBM) || !encode(&p.b[i], b, dtype, b_mn ? 64 : bnc))
+      return NCA_ERR_CUDA;
+  }
+  p.m = (int)g.m;
+  p.n = (int)g.n;
+  p.batch = g.batch;
+  p.splits = 1;
+  const int kb = (int)ceil_div(g.k, kBK);
+  p.kb = g.k_sources ? 2 * kb : kb;
+  p.kb_second = kb;
+  return NCA_OK;
+}
+
+template <class T, bool A_MN, bool B_MN, int EPI, int ACT>
+int32_t product(GemmParams& p, const Product& g, int dtype, const Shape& sh, cudaStream_t s) {
+  const int32_t st = set_up(p, g, dtype, A_MN, B_MN, sh.pair ? 2 : 1, sh.pair ? 256 : 128, EPI == EPI_GATE);
+  if (st != NCA_OK) return st;
+  p.splits = sh.splits;
+  return sh.pair ? launch<T, 2, 256, A_MN, B_MN, EPI, ACT>(p, s) : launch<T, 1, 128, A_MN, B_MN, EPI, ACT>(p, s);
+}
+
+// The weight gradient dW[batch] (m x n) = A^T B over the rows, through partial sums when split.
+template <class T>
+int32_t weight_product(GemmParams& p, const Product& g, int dtype, void* c0, void* c1, float* part, cudaStream_t s) {
+  const Shape sh = shape_of(g.m, g.n, g.batch, ceil_div(g.k, kBK), true, false);
+  p.c[0] = c0;
+  p.c[1] = c1;
+  p.ldc = g.n;
+  p.vec_c = g.n % 8 == 0 && reinterpret_cast<uintptr_t>(c0) % 16 == 0 && reinterpret_cast<uintptr_t>(c1) % 16 == 0;
+  if (sh.splits == 1) return product<T, true, true, EPI_STORE, NCA_ACT_NONE>(p, g, dtype, sh, s);
+  p.part = part;
+  p.ldp = (g.n + 3) / 4 * 4;
+  const int32_t st = product<T, true, true, EPI_PARTIAL, NCA_ACT_NONE>(p, g, dtype, sh, s);
+  if (st != NCA_OK) return st;
+  const long long total = g.batch * g.m * g.n;
+  join_kernel<T><<<(unsigned)std::min(ceil_div(total, 256), 4096ll), 256, 0, s>>>(
+      part, sh.splits, g.batch, g.m, g.n, p.ldp, static_cast<T*>(c0), static_cast<T*>(c1));
+  return launch_status();
+}
+size_t weight_part_bytes(long long m, long long n, int batch, long long rows) {
+  const Shape sh = shape_of(m, n, batch, ceil_div(rows, kBK), true, false);
+  return sh.splits == 1 ? 0 : (size_t)sh.splits * batch * m * ((n + 3) / 4 * 4) * sizeof(float);
+}
+
+// --------------------------------------------------------------------------------- arguments
+int32_t check_desc(const NcaGatedDesc* d) {
+  if (!d || d->rows < 0 || d->d_in <= 0 || d->hidden <= 0 || d->d_out <= 0) return NCA_ERR_INVALID;
+  if (d->dtype != NCA_BF16 && d->dtype != NCA_F16) return NCA_ERR_UNSUPPORTED;
+  if (d->bias_dtype != NCA_F32 && d->bias_dtype != d->dtype) return NCA_ERR_INVALID;
+  if (d->act < NCA_ACT_RELU || d->act > NCA_ACT_SIGMOID) return NCA_ERR_INVALID;
+  const long long most = (1ll << 31) - 1024;
+  if (d->rows > most || d->d_in > most || d->hidden > most || d->d_out > most) return NCA_ERR_UNSUPPORTED;
+  return NCA_OK;
+}
+
+enum { OP_X, OP_WG, OP_WU, OP_WD, OP_DY, OPS };
+struct Operand {
+  long long rows, cols, sr, sc;
+  bool packed;
+  size_t at;  // offset of the copy in the workspace
+};
+struct Plan {
+  Operand op[OPS];
+  size_t h, dgate, dup, part, sums, total;
+  long long fp;  // padded hidden
+};
+
+Plan plan_of(const NcaGatedDesc& d, bool backward) {
+  Plan p{};
+  const long long rows[OPS] = {d.rows, d.hidden, d.hidden, d.d_out, d.rows};
+  const long long cols[OPS] = {d.d_in, d.d_in, d.d_in, d.hidden, d.d_out};
+  const int64_t* stride[OPS] = {d.x_stride, d.w_gate_stride, d.w_up_stride, d.w_down_stride, d.dy_stride};
+  size_t at = 0;
+  for (int i = 0; i < OPS; ++i) {
+    Operand& o = p.op[i];
+    o.rows = rows[i];
+    o.cols = cols[i];
+    o.sr = o.rows == 1 ? pad8(o.cols) : stride[i][0];  // the stride of a single row or column means nothing
+    o.sc = o.cols == 1 ? 1 : stride[i][1];
+    o.packed = o.sc != 1 || o.sr % 8 != 0 || o.sr < o.cols || o.sr >= (1ll << 38) || (d.unaligned >> i & 1);
+    if (i == OP_DY && !backward) o.packed = false;
+    if (o.packed) {
+      if (o.rows == 1) o.sr = 0;
+      o.at = at;
+      at += align256((size_t)o.rows * pad8(o.cols) * 2);
+    }
+  }
+  p.fp = pad8(d.hidden);
+  const size_t tf = align256((size_t)d.rows * p.fp * 2);
+  if (!backward) {
+    p.h = at;
+    at += tf;
+  } else {
+    p.dgate = at;
+    at += tf;
+    p.dup = at;
+    at += tf;
+    p.part = at;
+    at += align256(std::max({weight_part_bytes(d.hidden, d.d_in, 2, d.rows),
+                             weight_part_bytes(d.hidden, d.d_in, 1, d.rows),
+                             weight_part_bytes(d.d_out, d.hidden, 1, d.rows)}));
+    p.sums = at;
+    at += align256((size_t)kSumSplits * std::max(d.hidden, d.d_out) * sizeof(float));
+  }
+  p.total = at + 256;
+  return p;
+}
+
+// The operand as TMA reads it: in place, or copied into the workspace first.
+int32_t matrix_of(const Operand& o, const void* src, uint8_t* ws, cudaStream_t s, Matrix* out) {
+  if (!src) return NCA_ERR_INVALID;
+  if (!o.packed) {
+    if (reinterpret_cast<uintptr_t>(src) % 16) return NCA_ERR_INVALID;  // `unaligned` did not say so
+    *out = {src, o.rows, o.cols, o.sr};
+    return NCA_OK;
+  }
+  const long long ld = pad8(o.cols);
+  const long long tiles = ceil_div(o.rows, 32) * ceil_div(o.cols, 32);
+  pack_kernel<<<(unsigned)std::min(tiles, 148ll * 16), dim3(32, 8), 0, s>>>(
+      static_cast<const uint16_t*>(src), o.rows, o.cols, o.sr, o.sc, reinterpret_cast<uint16_t*>(ws + o.at), ld);
+  *out = {ws + o.at, o.rows, o.cols, ld};
+  return launch_status();
+}
+
+#define NCA_TRY(call)                    \
+  do {                                   \
+    const int32_t st_ = (call);          \
+    if (st_ != NCA_OK) return st_;       \
+  } while (0)
+
+template <class T, int ACT>
+int32_t forward(const NcaGatedDesc& d, const void* x, const void* w_gate, const void* w_up, const void* w_down,
+                const void* b_gate, const void* b_up, const void* b_down, void* y, void* saved, uint8_t* ws,
+                GemmParams& base, cudaStream_t s) {
+  const Plan pl = plan_of(d, false);
+  Matrix mx, mg, mu, md;
+  NCA_TRY(matrix_of(pl.op[OP_X], x, ws, s, &mx));
+  NCA_TRY(matrix_of(pl.op[OP_WG], w_gate, ws, s, &mg));
+  NCA_TRY(matrix_of(pl.op[OP_WU], w_up, ws, s, &mu));
+  NCA_TRY(matrix_of(pl.op[OP_WD], w_down, ws, s, &md));
+  const size_t tf = align256((size_t)d.rows * pl.fp * 2);
+  uint8_t* keep = static_cast<uint8_t*>(saved);
+  void* h = keep ? keep + 3 * tf : ws + pl.h;
+  {
+    GemmParams p = base;
+    Product g{{mx, mx}, {mg, mu}, false, true, d.rows, d.hidden, d.d_in, false, 1};
+    p.c[0] = h;
+    p.ldc = pl.fp;
+    p.bias[0] = b_gate;
+    p.bias[1] = b_up;
+    p.saved = reinterpret_cast<uint16_t*>(keep);
+    p.plane = (long long)(tf / 2);
+    NCA_TRY((product<T, false, false, EPI_GATE, ACT>(
+        p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, true), s)));
+  }
+  GemmParams p = base;
+  const Matrix mh{h, d.rows, d.hidden, pl.fp};
+  Product g{{mh, mh}, {md, md}, false, false, d.rows, d.d_out, d.hidden, false, 1};
+  p.c[0] = y;
+  p.ldc = d.d_out;
+  p.vec_c = d.d_out % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  p.bias[0] = b_down;
+  return product<T, false, false, EPI_STORE, NCA_ACT_NONE>(
+      p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s);
+}
+
+template <class T>
+int32_t column_sums(const void* a, long long rows, long long cols, long long ld, float* part, void* out, int dtype,
+                    cudaStream_t s) {
+  const int splits = (int)std::max(1ll, std::min((long long)kSumSplits, rows / 32));
+  column_sums_kernel<T><<<dim3((unsigned)ceil_div(cols, 32), splits), dim3(32, 8), 0, s>>>(
+      static_cast<const T*>(a), rows, cols, ld, splits, part);
+  column_store_kernel<<<(unsigned)ceil_div(cols, 128), 128, 0, s>>>(part, splits, cols, out, dtype);
+  return launch_status();
+}
+
+template <class T, int ACT>
+int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const void* w_up, const void* w_down,
+                 const void* saved, const void* dy, void* dx, void* dw_gate, void* dw_up, void* dw_down,
+                 void* db_gate, void* db_up, void* db_down, uint8_t* ws, GemmParams& base, cudaStream_t s) {
+  const Plan pl = plan_of(d, true);
+  const size_t tf = align256((size_t)d.rows * pl.fp * 2);
+  const uint8_t* keep = static_cast<const uint8_t*>(saved);
+  Matrix mx, mg, mu, md, mdy;
+  NCA_TRY(matrix_of(pl.op[OP_DY], dy, ws, s, &mdy));
+  const Matrix mh{keep + 3 * tf, d.rows, d.hidden, pl.fp};
+  const Matrix mdg{ws + pl.dgate, d.rows, d.hidden, pl.fp}, mdu{ws + pl.dup, d.rows, d.hidden, pl.fp};
+  float* part = reinterpret_cast<float*>(ws + pl.part);
+  float* sums = reinterpret_cast<float*>(ws + pl.sums);
+  if (dx || dw_gate || dw_up || db_gate || db_up) {
+    NCA_TRY(matrix_of(pl.op[OP_WD], w_down, ws, s, &md));
+    GemmParams p = base;
+    Product g{{mdy, mdy}, {md, md}, false, false, d.rows, d.hidden, d.d_out, false, 1};
+    p.c[0] = ws + pl.dgate;
+    p.c[1] = ws + pl.dup;
+    p.ldc = pl.fp;
+    p.saved = reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(keep));
+    p.plane = (long long)(tf / 2);
+    NCA_TRY((product<T, false, true, EPI_DGATE, ACT>(
+        p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s)));
+  }
+  if (dx) {
+    NCA_TRY(matrix_of(pl.op[OP_WG], w_gate, ws, s, &mg));
+    NCA_TRY(matrix_of(pl.op[OP_WU], w_up, ws, s, &mu));
+    GemmParams p = base;
+    Product g{{mdg, mdu}, {mg, mu}, true, true, d.rows, d.d_in, d.hidden, true, 1};
+    p.c[0] = dx;
+    p.ldc = d.d_in;
+    p.vec_c = d.d_in % 8 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0;
+    NCA_TRY((product<T, false, true, EPI_STORE, NCA_ACT_NONE>(
+        p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s)));
+  }
+  if (dw_gate || dw_up) {
+    NCA_TRY(matrix_of(pl.op[OP_X], x, ws, s, &mx));
+    GemmParams p = base;
+    if (dw_gate && dw_up) {
+      Product g{{mdg, mdu}, {mx, mx}, true, false, d.hidden, d.d_in, d.rows, false, 2};
+      NCA_TRY(weight_product<T>(p, g, d.dtype, dw_gate, dw_up, part, s));
+    } else {
+      const Matrix& m = dw_gate ? mdg : mdu;
+      void* out = dw_gate ? dw_gate : dw_up;
+      Product g{{m, m}, {mx, mx}, false, false, d.hidden, d.d_in, d.rows, false, 1};
+      NCA_TRY(weight_product<T>(p, g, d.dtype, out, out, part, s));
+    }
+  }
+  if (dw_down) {
+    GemmParams p = base;
+    Product g{{mdy, mdy}, {mh, mh}, false, false, d.d_out, d.hidden, d.rows, false, 1};
+    NCA_TRY(weight_product<T>(p, g, d.dtype, dw_down, dw_down, part, s));
+  }
+  if (db_gate) NCA_TRY(column_sums<T>(mdg.p, d.rows, d.hidden, pl.fp, sums, db_gate, d.bias_dtype, s));
+  if (db_up) NCA_TRY(column_sums<T>(mdu.p, d.rows, d.hidden, pl.fp, sums, db_up, d.bias_dtype, s));
+  if (db_down) NCA_TRY(column_sums<T>(mdy.p, d.rows, d.d_out, mdy.ld, sums, db_down, d.bias_dtype, s));
+  return NCA_OK;
+}
+
+template <class F>
+int32_t dispatch(const NcaGatedDesc& d, F fn) {
+  auto by_act = [&](auto t) {
+    using T = decltype(t);
+    switch (d.act) {
+      case NCA_ACT_RELU: return fn.template operator()<T, NCA_ACT_RELU>();
+      case NCA_ACT_SILU: return fn.template operator()<T, NCA_ACT_SILU>();
+      case NCA_ACT_GELU: return fn.template operator()<T, NCA_ACT_GELU>();
+      default: return fn.template operator()<T, NCA_ACT_SIGMOID>();
+    }
+  };
+  return d.dtype == NCA_BF16 ? by_act(__nv_bfloat16{}) : by_act(__half{});
+}
+
+struct ForwardCall {
+  const NcaGatedDesc& d;
+  const void *x, *wg, *wu, *wd, *bg, *bu, *bd;
+  void *y, *saved;
+  uint8_t* ws;
+  GemmParams& base;
+  cudaStream_t s;
+  template <class T, int A>
+  int32_t operator()() const { return forward<T, A>(d, x, wg, wu, wd, bg, bu, bd, y, saved, ws, base, s); }
+};
+struct BackwardCall {
+  const NcaGatedDesc& d;
+  const void *x, *wg, *wu, *wd, *saved, *dy;
+  void *dx, *dwg, *dwu, *dwd, *dbg, *dbu, *dbd;
+  uint8_t* ws;
+  GemmParams& base;
+  cudaStream_t s;
+  template <class T, int A>
+  int32_t operator()() const {
+    return backward<T, A>(d, x, wg, wu, wd, saved, dy, dx, dwg, dwu, dwd, dbg, dbu, dbd, ws, base, s);
+  }
+};
+
+// Makes the current device's context current on this thread: the tensor-map encoder is a driver
+// call, which a thread without one (autograd's, before its first runtime call) would fail.
+int32_t bind_context() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess ? NCA_OK : NCA_ERR_DEVICE;
+}
+
+GemmParams base_params(const NcaGatedDesc& d, int32_t* ctrl, int32_t timeout_ms) {
+  GemmParams p{};
+  p.bias_dtype = d.bias_dtype;
+  p.ctrl = ctrl;
+  p.timeout_ns = (unsigned long long)(timeout_ms > 0 ? timeout_ms : 20000) * 1000000ull;
+  return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t nca_b200_gated_saved_bytes(const NcaGatedDesc* d, size_t* bytes) {
+  const int32_t st = check_desc(d);
+  if (st != NCA_OK || !bytes) return st != NCA_OK ? st : NCA_ERR_INVALID;
+  *bytes = 4 * align256((size_t)d->rows * pad8(d->hidden) * 2);
+  return NCA_OK;
+}
+
+int32_t nca_b200_gated_workspace(const NcaGatedDesc* d, int32_t backward, size_t* bytes) {
+  const int32_t st = check_desc(d);
+  if (st != NCA_OK || !bytes) return st != NCA_OK ? st : NCA_ERR_INVALID;
+  *bytes = plan_of(*d, backward != 0).total;
+  return NCA_OK;
+}
+
+int32_t nca_b200_gated_ffn(const NcaGatedDesc* d, const void* x, const void* w_gate, const void* w_up,
+                           const void* w_down, const void* b_gate, const void* b_up, const void* b_down, void* y,
+                           void* saved, void* workspace, size_t workspace_bytes, int32_t* ctrl, int32_t timeout_ms,
+                           void* stream) {
+  const int32_t st = check_desc(d);
+  if (st != NCA_OK) return st;
+  if (d->rows == 0) return NCA_OK;
+  if (!y || !workspace || !ctrl || workspace_bytes < plan_of(*d, false).total) return NCA_ERR_INVALID;
+  NCA_TRY(bind_context());
+  GemmParams base = base_params(*d, ctrl, timeout_ms);
+  return dispatch(*d, ForwardCall{*d, x, w_gate, w_up, w_down, b_gate, b_up, b_down, y, saved,
+                                  static_cast<uint8_t*>(workspace), base, static_cast<cudaStream_t>(stream)});
+}
+
+int32_t nca_b200_gated_ffn_backward(const NcaGatedDesc* d, const void* x, const void* w_gate, const void* w_up,
+                                    const void* w_down, const void* saved, const void* dy, void* dx, void* dw_gate,
+                                    void* dw_up, void* dw_down, void* db_gate, void* db_up, void* db_down,
+                                    void* workspace, size_t workspace_bytes, int32_t* ctrl, int32_t timeout_ms,
+                                    void* stream) {
+  const int32_t st = check_desc(d);
+  if (st != NCA_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (d->rows == 0) {
+    const size_t b = dtype_size(d->bias_dtype);
+    const struct {
+      void* p;
+      size_t bytes;
+    } outs[] = {{dw_gate, (size_t)d->hidden * d->d_in * 2}, {dw_up, (size_t)d->hidden * d->d_in * 2},
+                {dw_down, (size_t)d->d_out * d->hidden * 2}, {db_gate, d->hidden * b}, {db_up, d->hidden * b},
+                {db_down, d->d_out * b}};
+    for (const auto& o : outs)
+      if (o.p && cudaMemsetAsync(o.p, 0, o.bytes, s) != cudaSuccess) return NCA_ERR_CUDA;
+    return NCA_OK;
+  }
+  if (!saved || !dy || !workspace || !ctrl || workspace_bytes < plan_of(*d, true).total) return NCA_ERR_INVALID;
+  NCA_TRY(bind_context());
+  GemmParams base = base_params(*d, ctrl, timeout_ms);
+  return dispatch(*d, BackwardCall{*d, x, w_gate, w_up, w_down, saved, dy, dx, dw_gate, dw_up, dw_down, db_gate, db_up,
+                                   db_down, static_cast<uint8_t*>(workspace), base, s});
+}
+
+}  // extern "C"

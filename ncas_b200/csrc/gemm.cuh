@@ -1,0 +1,497 @@
+// gemm.cuh -- the tcgen05 matrix-product kernel behind the gated feed-forward block (gated.cu).
+//
+// D[M, N] = sum_k A[m, k] B[n, k] with 16-bit operands and fp32 sums in tensor memory.  Either
+// operand may be stored with k adjacent ("K-major") or with its rows adjacent ("MN-major": the
+// transposed operand of a backward product is read as it lies, nothing is transposed in memory).
+//
+// One persistent CTA (CG = 1) or CTA pair (CG = 2, cta_group::2: one 256-row tile over two
+// multiprocessors, each loading half of B) per multiprocessor.  Warp 0 loads tiles by TMA into a
+// ring of shared-memory stages, warp 1 issues the MMAs, warp 2 owns the tensor memory, warps 4-7
+// take finished accumulators out and apply the epilogue.  Two accumulators in tensor memory let
+// the epilogue of one tile run under the MMAs of the next.
+#pragma once
+#include <cuda.h>
+
+#include "cell_ops.cuh"
+#include "ptx.cuh"
+
+namespace nca {
+
+enum GemmEpilogue {
+  EPI_STORE = 0,    // c = D (+ bias), rounded to the matrix type
+  EPI_PARTIAL = 1,  // fp32 partial sums of one piece of a long k axis
+  EPI_GATE = 2,     // columns are gate | up halves: h = act(gate) up (and gate, up when saved)
+  EPI_DGATE = 3     // D = dh: dgate = dh up act'(gate), dup = dh act(gate)
+};
+
+struct GemmParams {
+  CUtensorMap a[2], b[2];
+  int m, n;            // logical rows and columns of D (columns of one half for EPI_GATE)
+  int m_tiles, n_tiles;
+  int batch;           // independent products: a[z], c[z] (1 or 2)
+  int splits;          // pieces of the k axis (EPI_PARTIAL)
+  int kb;              // k blocks of 64
+  int kb_second;       // first k block that reads a[1], b[1] (kb when there is one source)
+  void* c[2];          // EPI_STORE: outputs; EPI_GATE: h, -; EPI_DGATE: dgate, dup
+  long long ldc;
+  int vec_c;           // 16-byte stores allowed
+  const void* bias[2];
+  int bias_dtype;
+  uint16_t* saved;     // pre-activations (SavedPlanes): EPI_GATE writes (may be null), EPI_DGATE reads
+  long long plane;     // distance of the three planes
+  float* part;         // [batch * splits][m][ldp]
+  long long ldp;
+  int* ctrl;
+  unsigned long long timeout_ns;
+};
+
+constexpr int kGemmThreads = 256;
+constexpr int kBM = 128, kBK = 64;
+
+// ------------------------------------------------------------------------------- PTX wrappers
+__device__ __forceinline__ uint32_t cta_rank_in_cluster() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tc_alloc(uint32_t* dst, uint32_t cols) {
+  if constexpr (CG == 1) {
+    tmem_alloc(dst, cols);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void tc_dealloc(uint32_t addr, uint32_t cols) {
+  if constexpr (CG == 1) tmem_dealloc(addr, cols);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem]^T, 16-bit inputs of one type, fp32 accumulators.
+template <int CG>
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives on `bar` (of both CTAs of a pair) when the MMAs issued so far have finished.
+template <int CG>
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  if constexpr (CG == 1) {
+    umma_commit(bar);
+  } else {
+    const uint16_t both = 3;
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(both)
+        : "memory");
+  }
+}
+
+// The same on a barrier of this CTA alone.
+template <int CG>
+__device__ __forceinline__ void umma_commit_local(uint64_t* bar) {
+  if constexpr (CG == 1)
+    umma_commit(bar);
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+
+// Shared-memory descriptor of a 128-byte-swizzled operand tile.  K-major: rows of 64 values (128
+// bytes), 8 rows a swizzle atom, `sbo` the distance of atoms along the rows (lbo unused).
+// MN-major: k lines of 64 adjacent rows (128 bytes), 8 lines an atom; `sbo` the distance of atoms
+// along k, `lbo` the distance of blocks of 64 rows.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  uint64_t d = (uint64_t)((addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)(lbo >> 4) << 16;
+  d |= (uint64_t)(sbo >> 4) << 32;
+  d |= (uint64_t)1 << 46;  // descriptor version of sm_100
+  d |= (uint64_t)2 << 61;  // 128-byte swizzle
+  return d;
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Stores n <= 32 adjacent values of one row (16 bytes at a time when the rows allow it).
+template <class T>
+__device__ __forceinline__ void store_row(T* dst, const float (&v)[32], int n, bool vec) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+      if (i < n)
+        *reinterpret_cast<uint4*>(dst + i) =
+            make_uint4(pack2<T>(v[i], v[i + 1]), pack2<T>(v[i + 2], v[i + 3]), pack2<T>(v[i + 4], v[i + 5]),
+                       pack2<T>(v[i + 6], v[i + 7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < n) dst[i] = from_f32<T>(v[i]);
+  }
+}
+// The pre-activations kept for the backward pass: the upper 24 bits of their fp32 values (relative
+// error below 2^-15, the full fp32 range).  In the matrix type, bf16 would put 2^-8 more noise into
+// every gradient, and fp16 would overflow where the fp32 sum does not; the third plane costs 2 of
+// 8 bytes.  Three planes of 16-bit values: gate bits 31-16, up bits 31-16, and bits 15-8 of both
+// (gate low byte, up high byte).
+struct SavedPlanes {
+  static __device__ __forceinline__ void store(uint16_t* at, long long plane, const float (&g)[32],
+                                               const float (&u)[32], int n) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      uint32_t hg[4], hu[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t g0 = __float_as_uint(g[i + 2 * j]), g1 = __float_as_uint(g[i + 2 * j + 1]);
+        const uint32_t u0 = __float_as_uint(u[i + 2 * j]), u1 = __float_as_uint(u[i + 2 * j + 1]);
+        hg[j] = __byte_perm(g0, g1, 0x7632);
+        hu[j] = __byte_perm(u0, u1, 0x7632);
+        lo[j] = __byte_perm(__byte_perm(g0, u0, 0x0051), __byte_perm(g1, u1, 0x0051), 0x5410);
+      }
+      if (i < n) {
+        *reinterpret_cast<uint4*>(at + i) = make_uint4(hg[0], hg[1], hg[2], hg[3]);
+        *reinterpret_cast<uint4*>(at + plane + i) = make_uint4(hu[0], hu[1], hu[2], hu[3]);
+        *reinterpret_cast<uint4*>(at + 2 * plane + i) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+    }
+  }
+  static __device__ __forceinline__ void load(const uint16_t* at, long long plane, float (&g)[32], float (&u)[32],
+                                              int n) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      uint4 a = make_uint4(0, 0, 0, 0), b = a, c = a;
+      if (i < n) {
+        a = *reinterpret_cast<const uint4*>(at + i);
+        b = *reinterpret_cast<const uint4*>(at + plane + i);
+        c = *reinterpret_cast<const uint4*>(at + 2 * plane + i);
+      }
+      const uint32_t hg[4] = {a.x, a.y, a.z, a.w}, hu[4] = {b.x, b.y, b.z, b.w}, lo[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        g[i + 2 * j] = __uint_as_float((hg[j] << 16) | (lo[j] << 8 & 0xFF00u));
+        g[i + 2 * j + 1] = __uint_as_float((hg[j] & 0xFFFF0000u) | (lo[j] >> 8 & 0xFF00u));
+        u[i + 2 * j] = __uint_as_float((hu[j] << 16) | (lo[j] & 0xFF00u));
+        u[i + 2 * j + 1] = __uint_as_float((hu[j] & 0xFFFF0000u) | (lo[j] >> 16 & 0xFF00u));
+      }
+    }
+  }
+};
+
+template <int CG, int BN>
+struct GemmShape {
+  static constexpr int kBNc = BN / CG;  // rows of B in one CTA
+  static constexpr int kABytes = kBM * kBK * 2;
+  static constexpr int kBBytes = kBNc * kBK * 2;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = (196 * 1024) / kStageBytes;
+  static constexpr int kSmem = kStages * kStageBytes + 1024 + 1024;  // alignment, barriers
+  static constexpr int kTmemCols = 2 * BN;
+};
+
+struct GemmTile {
+  int m0, n0, batch, split, kb0, kb1;
+};
+
+// Tiles in groups of 8 tile rows, columns within, so that tiles that run together share operands
+// in L2.  TN: columns of D that one tile covers.
+template <int TM, int TN>
+__device__ __forceinline__ GemmTile tile_of(const GemmParams& p, int t) {
+  GemmTile r;
+  const int per = p.m_tiles * p.n_tiles;
+  const int z = t / per;
+  int i = t - z * per;
+  r.batch = z % p.batch;
+  r.split = z / p.batch;
+  const int group = 8 * p.n_tiles;
+  const int g = i / group;
+  const int rows = min(8, p.m_tiles - g * 8);
+  i -= g * group;
+  r.m0 = (g * 8 + i % rows) * TM;
+  r.n0 = (i / rows) * TN;
+  r.kb0 = (int)((long long)p.kb * r.split / p.splits);
+  r.kb1 = (int)((long long)p.kb * (r.split + 1) / p.splits);
+  return r;
+}
+
+template <class T, int CG, int BN, bool A_MN, bool B_MN, int EPI, int ACT>
+__global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
+  using S = GemmShape<CG, BN>;
+  constexpr int kTN = EPI == EPI_GATE ? BN / 2 : BN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStageBytes);
+  uint64_t* empty = full + S::kStages;
+  uint64_t* acc_full = empty + S::kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drained = acc_empty + 2;
+  uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_base_s + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 1 ? 0 : cta_rank_in_cluster();
+  const FailState fs{p.ctrl, abort_s, 0, p.timeout_ns};
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4 * CG);
+    }
+    mbar_init(drained, 1);
+    *abort_s = 0;
+    fence_mbar_init();
+  }
+  if (warp == 2) tc_alloc<CG>(tmem_base_s, S::kTmemCols);
+  tc_fence_before();
+  if constexpr (CG == 2) cluster_sync_all();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_base_s;
+
+  const int tiles = p.m_tiles * p.n_tiles * p.batch * p.splits;
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      long long issued = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        const GemmTile tl = tile_of<kBM * CG, kTN>(p, t);
+        const int am = tl.m0 + (int)rank * kBM;
+        for (int kb = tl.kb0; kb < tl.kb1; ++kb) {
+          if (!mbar_wait(&empty[s], ph ^ 1, fs, 101)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], S::kStageBytes * CG);
+          const uint32_t bar = CG == 1 ? smem_u32(&full[s]) : map_to_rank(smem_u32(&full[s]), 0);
+          const uint32_t sa = smem_u32(smem + s * S::kStageBytes), sb = sa + S::kABytes;
+          const int second = kb >= p.kb_second;
+          const int k0 = (second ? kb - p.kb_second : kb) * kBK;
+          const CUtensorMap* ma = &p.a[p.batch == 2 ? tl.batch : second];
+          if constexpr (A_MN) {
+#pragma unroll
+            for (int i = 0; i < kBM / 64; ++i) tma_load_2d<CG>(sa + i * 8192, ma, bar, am + 64 * i, k0);
+          } else {
+            tma_load_2d<CG>(sa, ma, bar, k0, am);
+          }
+          if constexpr (EPI == EPI_GATE) {
+            if constexpr (CG == 2) {
+              tma_load_2d<CG>(sb, &p.b[rank], bar, k0, tl.n0);
+            } else {
+              tma_load_2d<CG>(sb, &p.b[0], bar, k0, tl.n0);
+              tma_load_2d<CG>(sb + S::kBBytes / 2, &p.b[1], bar, k0, tl.n0);
+            }
+          } else {
+            const CUtensorMap* mb = &p.b[second];
+            const int bn = tl.n0 + (int)rank * S::kBNc;
+            if constexpr (B_MN) {
+#pragma unroll
+              for (int i = 0; i < S::kBNc / 64; ++i) tma_load_2d<CG>(sb + i * 8192, mb, bar, bn + 64 * i, k0);
+            } else {
+              tma_load_2d<CG>(sb, mb, bar, k0, bn);
+            }
+          }
+          ++issued;
+          if (++s == S::kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      if (!ok && rank == 0) {  // loads in flight land before this CTA leaves (bounded)
+        for (long long i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
+          for (int tries = 0; tries < 64 && !mbar_try_wait(&full[i % S::kStages], (i / S::kStages) & 1); ++tries) {
+          }
+      }
+    }
+  } else if (warp == 1 && rank == 0) {
+    if (lane == 0) {
+      constexpr bool is_bf16 = __is_same(T, __nv_bfloat16);
+      constexpr uint32_t idesc = (1u << 4) | ((is_bf16 ? 1u : 0u) << 7) | ((is_bf16 ? 1u : 0u) << 10) |
+                                 ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) |
+                                 ((uint32_t)(kBM * CG >> 4) << 24);
+      // one MMA takes 16 k: 32 bytes along a K-major row, 16 lines of 128 bytes MN-major
+      constexpr uint32_t a_step = (A_MN ? 2048 : 32) >> 4, b_step = (B_MN ? 2048 : 32) >> 4;
+      int s = 0, buf = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        const GemmTile tl = tile_of<kBM * CG, kTN>(p, t);
+        if (!mbar_wait(&acc_empty[buf], acc_ph ^ 1, fs, 102)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + buf * BN;
+        for (int kb = tl.kb0; kb < tl.kb1; ++kb) {
+          if (!mbar_wait(&full[s], ph, fs, 103)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * S::kStageBytes), sb = sa + S::kABytes;
+          const uint64_t da = smem_desc(sa, A_MN ? 8192 : 16, 1024);
+          const uint64_t db = smem_desc(sb, B_MN ? 8192 : 16, 1024);
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k)
+            umma_ss<CG>(d, da + k * a_step, db + k * b_step, idesc, kb > tl.kb0 || k > 0);
+          tc_commit<CG>(&empty[s]);
+          if (++s == S::kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (!ok) break;
+        tc_commit<CG>(&acc_full[buf]);
+        buf ^= 1;
+        if (buf == 0) acc_ph ^= 1;
+      }
+      if (!ok) {  // the MMAs in flight end before the tensor memory is freed (bounded)
+        umma_commit_local<CG>(drained);
+        for (int tries = 0; tries < 64 && !mbar_try_wait(drained, 0); ++tries) {
+        }
+      }
+    }
+  } else if (warp >= 4) {
+    const int q = warp - 4;  // tensor memory lanes 32 q .. 32 q + 31
+    int buf = 0;
+    uint32_t ph = 0;
+    for (int t = first; t < tiles; t += step) {
+      const GemmTile tl = tile_of<kBM * CG, kTN>(p, t);
+      if (!mbar_wait(&acc_full[buf], ph, fs, 104)) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * BN + ((uint32_t)(32 * q) << 16);
+      const int row = tl.m0 + (int)rank * kBM + 32 * q + lane;
+      const bool live = row < p.m;
+      for (int c = 0; c < kTN; c += 32) {
+        const int col = tl.n0 + c;
+        const int n = min(32, p.n - col);
+        uint32_t r0[32];
+        tmem_ld32(acc + c, r0);
+        if constexpr (EPI == EPI_GATE) {
+          uint32_t r1[32];
+          tmem_ld32(acc + kTN + c, r1);
+          tc_wait_ld_regs(r0);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r1[i]));
+          if (live && n > 0) {
+            float g[32], u[32], h[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const int cc = min(col + i, p.n - 1);
+              g[i] = __uint_as_float(r0[i]) + (p.bias[0] ? load_param(p.bias[0], p.bias_dtype, cc) : 0.f);
+              u[i] = __uint_as_float(r1[i]) + (p.bias[1] ? load_param(p.bias[1], p.bias_dtype, cc) : 0.f);
+              h[i] = act_f<ACT>(g[i]) * u[i];
+            }
+            const long long at = (long long)row * p.ldc + col;
+            store_row<T>(static_cast<T*>(p.c[0]) + at, h, n, true);
+            if (p.saved) SavedPlanes::store(p.saved + at, p.plane, g, u, n);
+          }
+        } else if constexpr (EPI == EPI_DGATE) {
+          tc_wait_ld_regs(r0);
+          if (live && n > 0) {
+            const long long at = (long long)row * p.ldc + col;
+            float g[32], u[32];
+            SavedPlanes::load(p.saved + at, p.plane, g, u, n);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float dh = __uint_as_float(r0[i]);
+              float a;
+              const float slope = act_slope_f<ACT>(g[i], a);
+              g[i] = dh * u[i] * slope;
+              u[i] = dh * a;
+            }
+            store_row<T>(static_cast<T*>(p.c[0]) + at, g, n, true);
+            store_row<T>(static_cast<T*>(p.c[1]) + at, u, n, true);
+          }
+        } else if constexpr (EPI == EPI_PARTIAL) {
+          tc_wait_ld_regs(r0);
+          if (live && n > 0) {
+            float* dst = p.part + ((long long)(tl.split * p.batch + tl.batch) * p.m + row) * p.ldp + col;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (i < n)
+                *reinterpret_cast<uint4*>(dst + i) = make_uint4(r0[i], r0[i + 1], r0[i + 2], r0[i + 3]);
+          }
+        } else {
+          tc_wait_ld_regs(r0);
+          if (live && n > 0) {
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              v[i] = __uint_as_float(r0[i]);
+              if (p.bias[0]) v[i] += load_param(p.bias[0], p.bias_dtype, min(col + i, p.n - 1));
+            }
+            store_row<T>(static_cast<T*>(p.c[tl.batch]) + (long long)row * p.ldc + col, v, n, p.vec_c);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[buf]), 0));
+        else mbar_arrive(&acc_empty[buf]);
+      }
+      buf ^= 1;
+      if (buf == 0) ph ^= 1;
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  if constexpr (CG == 2) cluster_sync_all();
+  else __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tc_dealloc<CG>(tmem, S::kTmemCols);
+}
+
+}  // namespace nca
