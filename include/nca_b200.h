@@ -402,7 +402,7 @@ int32_t nca_b200_gated_ffn_backward(const NcaGatedDesc* d, const void* x, const 
 typedef struct NcaDistillDesc {
   int64_t rows;
   int64_t classes;               /* < 2^31 */
-  int64_t top;
+  int64_t top;                   /* <= 4096 */
   int32_t dtype, teacher_dtype;  /* NcaDtype */
   int32_t index_bits;            /* 32 or 64 */
   float temperature;             /* tau > 0 */

@@ -440,6 +440,7 @@ Distill distill_args(const Tensor& logits, const Tensor& teacher, const Tensor& 
                     ", not ", teacher.sizes());
   TORCH_CHECK_VALUE(index.sizes() == teacher.sizes(), op, ": teacher_index must be ", teacher.sizes(), ", not ",
                     index.sizes());
+  TORCH_CHECK_VALUE(teacher.size(-1) <= 4096, op, ": at most 4096 entries a row, not ", teacher.size(-1));
   TORCH_CHECK_VALUE(temperature > 0 && temperature <= 1e30, op, ": temperature must be positive and finite");
   TORCH_CHECK_VALUE(!teacher.requires_grad() || !at::GradMode::is_enabled(), op,
                     ": teacher_logits gets no gradient: detach it");
