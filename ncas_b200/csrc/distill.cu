@@ -4,8 +4,11 @@
 //   p = softmax(t / tau) over the entries, q = softmax(s / tau) over the classes
 //   loss = w tau^2 sum_k p_k (log p_k - log q_{i_k}),  dloss/ds_j = w tau (q_j - sum_{k: i_k = j} p_k)
 // exp runs as exp2((s - m) log2(e) / tau), m the row's maximum: the difference first, so that the
-// rounding is relative to the distance from the maximum.
+// rounding is relative to the distance from the maximum, and a row of the type's lowest values, whose
+// product with the scale would overflow, still gives differences of 0.
 #include "cell_ops.cuh"
+#include <atomic>
+#include <type_traits>
 
 using namespace nca;
 
@@ -239,6 +242,17 @@ __device__ __forceinline__ uint4 pack(const float (&f)[16 / sizeof(T)]) {
   return q;
 }
 
+// (a - m) c2 of two values.
+__device__ __forceinline__ float2 scaled2(float a0, float a1, float m, float c2) {
+  float2 d;
+  const float2 a = make_float2(a0, a1), n = make_float2(-m, -m), c = make_float2(c2, c2);
+  asm("{\n\t.reg .b64 t;\n\tadd.rn.f32x2 t, %1, %2;\n\tmul.rn.f32x2 %0, t, %3;\n\t}"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(n)),
+        "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+
 // The running maximum and sum of exp2((v - m) c2).
 struct Running {
   float m = -kInf, sum = 0.f;
@@ -248,28 +262,60 @@ struct Running {
 #pragma unroll
     for (int i = 1; i < N; ++i) top = fmaxf(top, f[i]);
     if (top > m) {
-      sum *= ex2((m - top) * c2);  // 0 times it at first; a NaN stays
+      sum *= ex2((m - top) * c2);  // 0 times 0 at first; a NaN stays
       m = top;
     }
-    const float base = m == -kInf ? 0.f : m;  // only -inf so far: exp2(-inf) = 0
+    const float from = m == -kInf ? 0.f : m;  // only -inf so far: exp2(-inf) = 0
+    if constexpr (N % 2 == 0) {
+      float2 part = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum += ex2((f[i] - base) * c2);
+      for (int i = 0; i < N; i += 2) {
+        const float2 d = scaled2(f[i], f[i + 1], from, c2);
+        part.x += ex2(d.x);
+        part.y += ex2(d.y);
+      }
+      sum += part.x + part.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum += ex2((f[i] - from) * c2);
+    }
   }
 };
+// `sum` counted from maximum m, as counted from `to` >= m.
+__device__ __forceinline__ float rebase(float sum, float m, float to, float c2) {
+  return m == -kInf ? sum : sum * ex2((m - to) * c2);  // nothing, only -inf (0), or NaN
+}
 
 struct Entry {
   int index;
   float teacher;
 };
 
-// G lanes a row.  One pass over the row keeps the running maximum and sum, a second, which finds the
-// row in L1 or L2, writes q; then the classes that have an entry are written again with q - p.
-// `entries` (index, probability) of the row are staged in shared memory.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Writes two values into the shared memory of CTA `rank` of the cluster, at the place that `p` is here.
+__device__ __forceinline__ void put_remote(float2* p, uint32_t rank, float2 v) {
+  uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(r), "f"(v.x), "f"(v.y) : "memory");
+}
+constexpr int kMostSlices = 8;
+
+// G lanes a row, or a cluster of `slices` blocks.  One pass keeps the running maximum and sum, a
+// second, which finds the row in L1 or L2, writes q; then the classes that have an entry are written
+// again with q - p.  The row's entries are staged in shared memory.
 template <class T, int G, int NT, bool FWD>
-__global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
+__global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slices) {
   constexpr int kV = 16 / sizeof(T), kRows = NT / G, kWarps = G / 32;
   __shared__ float red_m[2][NT / 32], red_s[2][NT / 32];
-  __shared__ float red_t[NT / 32];
+  __shared__ float2 red_t[2];
+  __shared__ float2 red_c[2][kMostSlices];  // (maximum, sum) of each slice
   extern __shared__ Entry entries_all[];
   const int group = threadIdx.x / G, lane = threadIdx.x % G;
   Entry* entries = entries_all + (size_t)group * a.top;
@@ -277,22 +323,27 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
     if constexpr (G == 32) __syncwarp();
     else __syncthreads();
   };
+  const int slice = G > 32 && slices > 1 ? (int)cluster_rank() : 0;
   const float c2 = kLog2e / a.tau, inv_tau = 1.f / a.tau;
   const int top = (int)a.top;
   int flip = 0;
-  for (long long r = (long long)blockIdx.x * kRows + group; r < a.rows; r += (long long)gridDim.x * kRows) {
+  for (long long r = (long long)(blockIdx.x / slices) * kRows + group; r < a.rows;
+       r += (long long)(gridDim.x / slices) * kRows) {
     const T* s = static_cast<const T*>(a.logits) + r * a.s_stride;
     T* ds = a.dlogits ? static_cast<T*>(a.dlogits) + r * (long long)a.classes : nullptr;
     const float w = a.weight ? a.weight[r] : 1.f;
     const RowSpan<T> span(s, a.classes);
     const uint4* sv = reinterpret_cast<const uint4*>(s + span.head);
     const bool vec_out = ds && ((reinterpret_cast<uintptr_t>(ds) ^ reinterpret_cast<uintptr_t>(s)) & 15) == 0;
+    // this block's vectors; the ragged ends belong to the first slice
+    const int v0 = (int)((long long)span.vecs * slice / slices), v1 = (int)((long long)span.vecs * (slice + 1) / slices);
+    const int ragged = slice == 0 ? span.ragged() : 0;
     // the first warp of the row: the teacher's softmax over the entries
     float tmax = -kInf, tsum = 0.f;
     if (lane < 32 && w != 0.f) {
       for (int k = lane; k < top; k += 32) {
         const int i = index_of(a, r, k);
-        float t = i >= 0 ? teacher_of(a, r, k) : -kInf;
+        const float t = i >= 0 ? teacher_of(a, r, k) : -kInf;
         entries[k] = Entry{i, t};
         tmax = fmaxf(tmax, t != t ? kInf : t);  // NaN and +inf end in NaN
       }
@@ -308,8 +359,8 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
     if constexpr (FWD) {
       Running run;
       if (live) {
-        int j = lane;
-        for (; j + 3 * G < span.vecs; j += 4 * G) {
+        int j = v0 + lane;
+        for (; j + 3 * G < v1; j += 4 * G) {
           uint4 q[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) q[u] = __ldg(sv + j + u * G);
@@ -320,12 +371,12 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
             run.add(f, c2);
           }
         }
-        for (; j < span.vecs; j += G) {
+        for (; j < v1; j += G) {
           float f[kV];
           unpack<T>(__ldg(sv + j), f);
           run.add(f, c2);
         }
-        for (int i = lane; i < span.ragged(); i += G) {
+        for (int i = lane; i < ragged; i += G) {
           const float f[1] = {to_f32(s[span.ragged_at(i)])};
           run.add(f, c2);
         }
@@ -333,8 +384,7 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
       float wm = run.m;
 #pragma unroll
       for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-      float ws = run.sum * ex2((run.m - wm) * c2);
-      if (run.m == -kInf) ws = run.sum;  // nothing, or only -inf (0), or NaN
+      float ws = rebase(run.sum, run.m, wm, c2);
 #pragma unroll
       for (int o = 16; o; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
       if constexpr (G == 32) {
@@ -345,7 +395,7 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
           red_m[flip][threadIdx.x >> 5] = wm;
           red_s[flip][threadIdx.x >> 5] = ws;
         }
-        if (threadIdx.x == 0) red_t[flip] = tmax, red_t[2 + flip] = tsum;
+        if (threadIdx.x == 0) red_t[flip] = make_float2(tmax, tsum);
         __syncthreads();
         m = red_m[flip][0];
 #pragma unroll
@@ -353,7 +403,18 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) {
           const float e = red_m[flip][i];
-          sum += e == -kInf ? red_s[flip][i] : red_s[flip][i] * ex2((e - m) * c2);
+          sum += rebase(red_s[flip][i], e, m, c2);
+        }
+        if (slices > 1 && live) {  // `live` here is the weight's, the same in all slices
+          if (threadIdx.x < slices) put_remote(&red_c[flip][slice], threadIdx.x, make_float2(m, sum));
+          cluster_barrier();
+          m = red_c[flip][0].x;
+          for (int i = 1; i < slices; ++i) m = fmaxf(m, red_c[flip][i].x);
+          sum = 0.f;
+          for (int i = 0; i < slices; ++i) {
+            const float2 e = red_c[flip][i];
+            sum += rebase(e.y, e.x, m, c2);
+          }
         }
       }
       if (m == -kInf) sum = m - m;  // a row of -inf only: NaN
@@ -361,35 +422,35 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
       m = a.stats[2 * r];
       sum = a.stats[2 * r + 1];
       if constexpr (G > 32) {
-        if (threadIdx.x == 0) red_t[flip] = tmax, red_t[2 + flip] = tsum;
+        if (threadIdx.x == 0) red_t[flip] = make_float2(tmax, tsum);
         __syncthreads();
       }
     }
     if constexpr (G > 32) {
-      tmax = red_t[flip];
-      tsum = red_t[2 + flip];
+      tmax = red_t[flip].x;
+      tsum = red_t[flip].y;
       flip ^= 1;
     } else {
       __syncwarp();
     }
     live = live && tmax != -kInf;
     if (!live) {  // no weight, or no entry
-      if (FWD && lane == 0) {
+      if (FWD && lane == 0 && slice == 0) {
         a.loss[r] = 0.f;
         if (a.stats) a.stats[2 * r] = a.stats[2 * r + 1] = 0.f;
       }
       if (ds) {
         if (vec_out)
-          for (int j = lane; j < span.vecs; j += G)
+          for (int j = v0 + lane; j < v1; j += G)
             reinterpret_cast<uint4*>(ds + span.head)[j] = make_uint4(0, 0, 0, 0);
         else
-          for (int j = lane; j < span.vecs * kV; j += G) ds[span.head + j] = from_f32<T>(0.f);
-        for (int i = lane; i < span.ragged(); i += G) ds[span.ragged_at(i)] = from_f32<T>(0.f);
+          for (int j = v0 * kV + lane; j < v1 * kV; j += G) ds[span.head + j] = from_f32<T>(0.f);
+        for (int i = lane; i < ragged; i += G) ds[span.ragged_at(i)] = from_f32<T>(0.f);
       }
       sync();  // the entries have been read
       continue;
     }
-    if (FWD && lane < 32) {
+    if (FWD && lane < 32 && slice == 0) {
       const float lnt = logf(tsum), lns = logf(sum);
       float loss = 0.f;
       for (int k = lane; k < top; k += 32) {
@@ -412,40 +473,39 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
     if (ds) {
       const float coef = w * a.tau * (a.grad ? a.grad[r * a.grad_stride] : 1.f);
       const float cq = coef / sum;
-      const auto out = [&](float f) { return ex2((f - m) * c2) * cq; };
+      const auto write = [&](int j, const uint4& q) {
+        float f[kV];
+        unpack<T>(q, f);
+#pragma unroll
+        for (int i = 0; i < kV; i += 2) {
+          const float2 d = scaled2(f[i], f[i + 1], m, c2);
+          f[i] = ex2(d.x) * cq;
+          f[i + 1] = ex2(d.y) * cq;
+        }
+        __stcs(reinterpret_cast<uint4*>(ds + span.head) + j, pack<T>(f));
+      };
+      const auto write_one = [&](int j) { ds[j] = from_f32<T>(ex2((to_f32(s[j]) - m) * c2) * cq); };
       if (vec_out) {
-        uint4* dv = reinterpret_cast<uint4*>(ds + span.head);
-        int j = lane;
-        for (; j + 3 * G < span.vecs; j += 4 * G) {
+        int j = v0 + lane;
+        for (; j + 3 * G < v1; j += 4 * G) {
           uint4 q[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u) q[u] = __ldg(sv + j + u * G);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            float f[kV];
-            unpack<T>(q[u], f);
-#pragma unroll
-            for (int i = 0; i < kV; ++i) f[i] = out(f[i]);
-            __stcs(dv + j + u * G, pack<T>(f));
-          }
+          for (int u = 0; u < 4; ++u) write(j + u * G, q[u]);
         }
-        for (; j < span.vecs; j += G) {
-          float f[kV];
-          unpack<T>(__ldg(sv + j), f);
-#pragma unroll
-          for (int i = 0; i < kV; ++i) f[i] = out(f[i]);
-          __stcs(dv + j, pack<T>(f));
-        }
+        for (; j < v1; j += G) write(j, __ldg(sv + j));
       } else {
-        for (int j = lane; j < span.vecs * kV; j += G) ds[span.head + j] = from_f32<T>(out(to_f32(s[span.head + j])));
+        for (int j = v0 * kV + lane; j < v1 * kV; j += G) write_one(span.head + j);
       }
-      for (int i = lane; i < span.ragged(); i += G)
-        ds[span.ragged_at(i)] = from_f32<T>(out(to_f32(s[span.ragged_at(i)])));
+      for (int i = lane; i < ragged; i += G) write_one(span.ragged_at(i));
       sync();
-      // the classes with an entry, each by the lane of its first entry
+      // the classes with an entry in this slice, each by the lane of its first entry
+      const int c0 = span.head + v0 * kV, c1 = span.head + v1 * kV;
       for (int k = lane; k < top; k += G) {
         const int i = entries[k].index;
-        if (i < 0) continue;
+        if (i < 0 || (slices > 1 && (i < c0 || i >= c1) && !(slice == 0 && (i < span.head || i >= span.tail0))))
+          continue;
         float p = 0.f;
         bool first = true;
         for (int k2 = 0; k2 < top; ++k2) {
@@ -461,6 +521,352 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
   }
 }
 
+__device__ __forceinline__ void named_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+constexpr int kHeld = 8;       // 16-byte vectors of a row that a lane holds
+constexpr int kLaneTop = 4;    // entries of a row that a lane of the entry warp holds
+
+// The larger of m and a vector's values, 16-bit types two at a time (NaN is passed over: the sum finds it).
+template <class T>
+struct Largest {
+  using T2 = std::conditional_t<__is_same(T, __nv_bfloat16), __nv_bfloat162, __half2>;
+  T2 m;
+  __device__ __forceinline__ explicit Largest(uint32_t low) : m(reinterpret_cast<const T2&>(low)) {}
+  __device__ __forceinline__ void add(const uint4& q) {
+    m = __hmax2(__hmax2(m, reinterpret_cast<const T2&>(q.x)), reinterpret_cast<const T2&>(q.y));
+    m = __hmax2(__hmax2(m, reinterpret_cast<const T2&>(q.z)), reinterpret_cast<const T2&>(q.w));
+  }
+  __device__ __forceinline__ float get() const { return fmaxf(to_f32(m.x), to_f32(m.y)); }
+};
+template <>
+struct Largest<float> {
+  float m;
+  __device__ __forceinline__ explicit Largest(uint32_t low) : m(reinterpret_cast<const float&>(low)) {}
+  __device__ __forceinline__ void add(const uint4& q) {
+    m = fmaxf(fmaxf(m, fmaxf(reinterpret_cast<const float&>(q.x), reinterpret_cast<const float&>(q.y))),
+              fmaxf(reinterpret_cast<const float&>(q.z), reinterpret_cast<const float&>(q.w)));
+  }
+  __device__ __forceinline__ float get() const { return m; }
+};
+// A 16-byte read of shared memory that is done again at each use: kept values would not fit the registers.
+__device__ __forceinline__ uint4 ld_shared(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"((uint32_t)__cvta_generic_to_shared(p)));
+  return v;
+}
+template <class T>
+__device__ __forceinline__ float exp_sum(const uint4& q, float from, float c2) {
+  float f[16 / sizeof(T)], part = 0.f;
+  unpack<T>(q, f);
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); i += 2) {
+    const float2 d = scaled2(f[i], f[i + 1], from, c2);
+    part += ex2(d.x) + ex2(d.y);
+  }
+  return part;
+}
+
+// A block, or a cluster of `slices` blocks, goes through rows that it holds: NS lanes hold kHeld
+// 16-byte vectors each in registers and NSM in shared memory, loaded while the row before is written
+// (a place is reloaded as soon as it has been used), so a row is read once and reads stay in flight
+// through the reductions.  One
+// more warp does everything else a row ahead or behind: the entries, the loss, the ragged ends, the
+// weights, and after the others have written q, the classes that have an entry.
+// One block barrier a row (and one of the cluster when slices > 1).
+template <class T, int NS, int NSM, int BLOCKS, bool FWD>
+__global__ void __launch_bounds__(NS + 32, BLOCKS) distill_held_kernel(DistillArgs a, int slices) {
+  // vectors of a slice: the host's arithmetic, a row's `vecs` is classes / kV or one less
+  const int per = (a.classes / (16 / (int)sizeof(T)) + slices - 1) / slices;
+  constexpr int kV = 16 / sizeof(T), kWarps = NS / 32, NT = NS + 32;
+  constexpr int kWritten = 1;  // named barrier: the lanes have written a row's q
+  __shared__ float2 red[2][kWarps + 1];     // (maximum, sum) of each warp
+  __shared__ float2 red_c[2][kMostSlices];  // and of each slice
+  __shared__ float4 said[2];                // coef, live, next row has a weight, sum (backward: with red the maximum)
+  __shared__ Entry entries[32 * kLaneTop];
+  extern __shared__ uint4 held[];           // [NSM][NS]
+  const int slice = slices > 1 ? (int)cluster_rank() : 0;
+  const int lane = threadIdx.x & 31;
+  const bool entry_warp = threadIdx.x >= NS;
+  const float c2 = kLog2e / a.tau;
+  const long long step = gridDim.x / slices;
+  long long r = blockIdx.x / slices;
+  int flip = 0;
+  // the row's (maximum, sum) from the partial ones of all warps and slices
+  // (every lane of a warp gets them: one partial result a lane, then butterflies)
+  const auto butterfly = [&](float2 e, int n, float& m, float& sum) {
+    m = e.x;
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      if (o < n) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    sum = rebase(e.y, e.x, m, c2);
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+      if (o < n) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  };
+  const auto combine = [&](float& m, float& sum) {
+    constexpr int n = kWarps < 8 ? 8 : kWarps < 16 ? 16 : 32;  // partial results, rounded up
+    butterfly((lane & (n - 1)) <= kWarps ? red[flip][lane & (n - 1)] : make_float2(-kInf, 0.f), n, m, sum);
+    if (slices > 1) {
+      if (threadIdx.x < slices) put_remote(&red_c[flip][slice], threadIdx.x, make_float2(m, sum));
+      cluster_barrier();
+      butterfly((lane & 7) < slices ? red_c[flip][lane & 7] : make_float2(-kInf, 0.f), 8, m, sum);
+    }
+    if (m == -kInf) sum = m - m;  // a row of -inf only: NaN
+  };
+
+  if (!entry_warp) {
+    uint4 q[kHeld];
+    const uint32_t low = sizeof(T) == 4 ? 0xFF800000u : (__is_same(T, __nv_bfloat16) ? 0xFF80FF80u : 0xFC00FC00u);  // -inf
+    // this lane's vectors of row `at`: the first, and how many lie in the slice
+    const auto place = [&](long long at, const uint4*& p, int& first, int& count) {
+      const T* s = static_cast<const T*>(a.logits) + at * a.s_stride;
+      const RowSpan<T> span(s, a.classes);
+      const int v0 = min(span.vecs, slice * per), v1 = min(span.vecs, v0 + per);
+      first = v0 + (int)threadIdx.x;
+      p = reinterpret_cast<const uint4*>(s + span.head) + first;
+      count = v1 - first;  // vectors at first, first + NS, ... while u * NS < count
+    };
+    const uint4* p;
+    int first, count;
+    // vector u of the row at p: u < kHeld in a register, above in this lane's place of `held`
+    const auto fetch = [&](int u) {
+      const bool on = u * NS < count;
+      if (u < kHeld) {
+        q[u] = on ? __ldcs(p + u * NS) : make_uint4(low, low, low, low);
+      } else {
+        uint4* to = &held[(u - kHeld) * NS + threadIdx.x];
+        if (on)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)),
+                       "l"(p + u * NS)
+                       : "memory");
+        else
+          *to = make_uint4(low, low, low, low);
+      }
+    };
+    if (r < a.rows) {
+      place(r, p, first, count);
+#pragma unroll
+      for (int u = 0; u < kHeld + NSM; ++u) fetch(u);
+    }
+    for (; r < a.rows; r += step, flip ^= 1) {
+      float m = -kInf, sum = 0.f;
+      if constexpr (FWD) {
+        Largest<T> most(low);
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) most.add(q[u]);
+        if constexpr (NSM > 0) {
+          asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 3
+          for (int u = 0; u < NSM; ++u) most.add(ld_shared(&held[u * NS + threadIdx.x]));
+        }
+        m = most.get();
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float from = m == -kInf ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) asm volatile("" : "+r"(q[u].x), "+r"(q[u].y), "+r"(q[u].z), "+r"(q[u].w));
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u) sum += exp_sum<T>(q[u], from, c2);
+#pragma unroll 1
+        for (int u = 0; u < NSM; ++u) sum += exp_sum<T>(ld_shared(&held[u * NS + threadIdx.x]), from, c2);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) red[flip][threadIdx.x >> 5] = make_float2(m, sum);
+      }
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u)  // unpacked again below: the 32-bit values would not fit the registers
+        asm volatile("" : "+r"(q[u].x), "+r"(q[u].y), "+r"(q[u].z), "+r"(q[u].w));
+      __syncthreads();
+      if constexpr (FWD) combine(m, sum);
+      const float4 word = said[flip];
+      if constexpr (!FWD) {
+        m = red[flip][0].x;
+        sum = word.w;
+        if constexpr (NSM > 0) asm volatile("cp.async.wait_all;" ::: "memory");
+      }
+      const bool live = word.y != 0.f;
+      const float from = live ? m : 0.f, cq = live ? word.x / sum : 0.f;
+      const bool more = r + step < a.rows;
+      T* ds = static_cast<T*>(a.dlogits) + r * (long long)a.classes;
+      const int head = (int)(reinterpret_cast<const T*>(p) - (static_cast<const T*>(a.logits) + r * a.s_stride)) - first * kV;
+      T* out = a.dlogits ? ds + head + first * kV : nullptr;
+      const bool vec_out = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(p)) & 15) == 0;
+      const int now = a.dlogits ? count : 0;
+      if (more) place(r + step, p, first, count);
+      if (!more || word.z == 0.f) count = 0;
+#pragma unroll
+      for (int u = 0; u < kHeld + NSM; ++u) {
+        if (u * NS < now) {
+          float f[kV];
+          unpack<T>(u < kHeld ? q[u < kHeld ? u : 0] : ld_shared(&held[(u - kHeld) * NS + threadIdx.x]), f);
+#pragma unroll
+          for (int i = 0; i < kV; i += 2) {
+            const float2 d = scaled2(f[i], f[i + 1], from, c2);
+            f[i] = live ? ex2(d.x) * cq : 0.f;
+            f[i + 1] = live ? ex2(d.y) * cq : 0.f;
+          }
+          if (vec_out) {
+            __stcs(reinterpret_cast<uint4*>(out) + u * NS, pack<T>(f));
+          } else {
+#pragma unroll
+            for (int i = 0; i < kV; ++i) out[(size_t)u * NS * kV + i] = from_f32<T>(f[i]);
+          }
+        }
+        fetch(u);
+      }
+      if (more && word.z == 0.f) {  // nothing was loaded, but the row's zeros are to be written
+        place(r + step, p, first, count);
+      }
+      named_arrive(kWritten, NT);
+    }
+  } else {
+    const int top = (int)a.top;
+    const float inv_tau = 1.f / a.tau;
+    // raw words of the row ahead
+    long long index[kLaneTop];
+    float teach[kLaneTop];
+    float weight = 0.f, weight1 = 0.f, up = 1.f;
+    const auto weight_of = [&](long long at) { return at < a.rows ? (a.weight ? a.weight[at] : 1.f) : 0.f; };
+    const auto fetch = [&](long long at) {
+#pragma unroll
+      for (int k = 0; k < kLaneTop; ++k) {
+        const int e = k * 32 + lane;
+        index[k] = -1;
+        teach[k] = 0.f;
+        if (at < a.rows && e < top) {
+          index[k] = a.index_bits == 64 ? static_cast<const long long*>(a.index)[at * a.i_stride + e]
+                                        : (long long)static_cast<const int*>(a.index)[at * a.i_stride + e];
+          teach[k] = teacher_of(a, at, e);
+        }
+      }
+      if (at < a.rows && a.grad) up = a.grad[at * a.grad_stride];
+    };
+    weight = weight_of(r);
+    weight1 = weight_of(r + step);
+    fetch(r);
+    for (; r < a.rows; r += step, flip ^= 1) {
+      const T* s = static_cast<const T*>(a.logits) + r * a.s_stride;
+      const RowSpan<T> span(s, a.classes);
+      const int v0 = min(span.vecs, slice * per), v1 = min(span.vecs, v0 + per);
+      const int c0 = span.head + v0 * kV, c1 = span.head + v1 * kV;
+      const bool ragged = slice == 0 && lane < span.ragged();
+      const int ragged_at = ragged ? span.ragged_at(lane) : 0;
+      const float end = ragged ? to_f32(s[ragged_at]) : -kInf;
+      int i[kLaneTop];
+      T v[kLaneTop];
+      float t[kLaneTop], tmax = -kInf, tsum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kLaneTop; ++k) {
+        i[k] = index[k] >= 0 && index[k] < a.classes ? (int)index[k] : -1;
+        t[k] = i[k] >= 0 ? teach[k] : -kInf;
+        v[k] = s[i[k] >= 0 ? i[k] : 0];
+        tmax = fmaxf(tmax, t[k] != t[k] ? kInf : t[k]);  // NaN and +inf end in NaN
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, o));
+      const bool live = weight != 0.f && tmax != -kInf;
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < kLaneTop; ++k) {
+        t[k] -= tmax;
+        const float p = i[k] >= 0 ? ex2(t[k] * c2) : 0.f;
+        tsum += p;
+        if (k * 32 + lane < top) entries[k * 32 + lane] = Entry{i[k], p};  // p up to its sum
+      }
+      __syncwarp();
+#pragma unroll
+      for (int o = 16; o; o >>= 1) tsum += __shfl_xor_sync(0xffffffffu, tsum, o);
+      const float coef = live ? weight * a.tau * up : 0.f;
+      const float weight_now = weight;
+      float m = -kInf, sum = 0.f;
+      if constexpr (FWD) {
+        m = end;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        sum = ragged ? ex2((end - (m == -kInf ? 0.f : m)) * c2) : 0.f;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) {
+          red[flip][kWarps] = make_float2(m, sum);
+          said[flip] = make_float4(coef, live ? 1.f : 0.f, weight1, 0.f);
+        }
+      } else {
+        m = a.stats[2 * r];
+        sum = a.stats[2 * r + 1];
+        if (lane == 0) {
+          red[flip][0].x = m;
+          said[flip] = make_float4(coef, live ? 1.f : 0.f, weight1, sum);
+        }
+      }
+      __syncthreads();
+      // the row ahead, while the others write
+      weight = weight1;
+      weight1 = weight_of(r + 2 * step);
+      fetch(r + step);
+      if constexpr (FWD) combine(m, sum);
+      if (FWD && slice == 0) {
+        float loss = 0.f;
+        if (live) {
+          const float lnt = logf(tsum), lns = logf(sum);
+#pragma unroll
+          for (int k = 0; k < kLaneTop; ++k) {
+            const float p = i[k] >= 0 ? ex2(t[k] * c2) / tsum : 0.f;
+            if (!(p <= 0.f)) loss += p * ((t[k] * inv_tau - lnt) - ((to_f32(v[k]) - m) * inv_tau - lns));
+          }
+#pragma unroll
+          for (int o = 16; o; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+        }
+        if (lane == 0) {
+          a.loss[r] = live ? loss * weight_now * a.tau * a.tau : 0.f;
+          if (a.stats) {
+            a.stats[2 * r] = live ? m : 0.f;
+            a.stats[2 * r + 1] = live ? sum : 0.f;
+          }
+        }
+      }
+      // each class once, with the sum of its entries, by the lane of its first entry
+      float hit[kLaneTop];
+      unsigned mine = 0;
+#pragma unroll
+      for (int k = 0; k < kLaneTop; ++k) {
+        hit[k] = 0.f;
+        const bool here = (i[k] >= c0 && i[k] < c1) || (slice == 0 && (i[k] < span.head || i[k] >= span.tail0));
+        if (i[k] >= 0 && here) mine |= 1u << k;
+      }
+      if (a.dlogits && live) {
+#pragma unroll 4
+        for (int k2 = 0; k2 < top; ++k2) {
+          const Entry e = entries[k2];
+#pragma unroll
+          for (int k = 0; k < kLaneTop; ++k) {
+            if (k * 32 >= top) break;
+            if (e.index == i[k]) {
+              hit[k] += e.teacher;
+              if (k2 < k * 32 + lane) mine &= ~(1u << k);
+            }
+          }
+        }
+      }
+      __syncwarp();  // the entries have been read
+      T* ds = static_cast<T*>(a.dlogits) + r * (long long)a.classes;
+      if (a.dlogits && ragged) ds[ragged_at] = from_f32<T>(live ? ex2((end - m) * c2) * (coef / sum) : 0.f);
+      named_sync(kWritten, NT);
+      if (a.dlogits && live) {
+#pragma unroll
+        for (int k = 0; k < kLaneTop; ++k)
+          if (mine >> k & 1) ds[i[k]] = from_f32<T>(coef * (ex2((to_f32(v[k]) - m) * c2) / sum - hit[k] / tsum));
+      }
+    }
+  }
+}
+
 template <class T, int G, int K, bool FWD>
 int32_t launch_small(const DistillArgs& a, cudaStream_t s) {
   const long long blocks = (a.rows + kThreads / G - 1) / (kThreads / G);
@@ -470,12 +876,68 @@ int32_t launch_small(const DistillArgs& a, cudaStream_t s) {
 
 constexpr int kMostEntries = 4096;  // staged in shared memory: 8 bytes each
 
-template <class T, int G, int NT, bool FWD>
-int32_t launch_rows(const DistillArgs& a, cudaStream_t s) {
-  const long long blocks = (a.rows + NT / G - 1) / (NT / G);
-  const size_t smem = (size_t)(NT / G) * a.top * sizeof(Entry);
-  distill_row_kernel<T, G, NT, FWD><<<(unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), NT, smem, s>>>(a);
+// A launch in clusters of `slices` blocks that go through rows: `most` clusters, but no more than run
+// at once (a cluster that started after the others had ended would double the time).  `room` keeps
+// that number by device and cluster size.
+constexpr int kMaxDevices = 64;
+using Room = std::atomic<int>[kMaxDevices][kMostSlices + 1];
+
+int32_t launch_clusters(void (*kernel)(DistillArgs, int), Room& room, const DistillArgs& a, long long most, int slices,
+                        int threads, size_t smem, cudaStream_t s) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = slices;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3(slices);
+  int n = room[dev][slices].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (smem > 32 * 1024 &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) {
+      const int32_t st = launch_status();
+      return st == NCA_OK ? NCA_ERR_CUDA : st;
+    }
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      const int32_t st = launch_status();
+      return st == NCA_OK ? NCA_ERR_CUDA : st;
+    }
+    room[dev][slices].store(n, std::memory_order_relaxed);
+  }
+  cfg.gridDim = dim3((unsigned)((most < n ? most : n) * slices));
+  if (cudaLaunchKernelEx(&cfg, kernel, a, slices) != cudaSuccess) {
+    const int32_t st = launch_status();
+    return st == NCA_OK ? NCA_ERR_CUDA : st;
+  }
   return launch_status();
+}
+
+template <class T, int G, int NT, bool FWD>
+int32_t launch_rows(const DistillArgs& a, int slices, cudaStream_t s) {
+  static Room room;
+  return launch_clusters(distill_row_kernel<T, G, NT, FWD>, room, a, (a.rows + NT / G - 1) / (NT / G), slices, NT,
+                         (size_t)(NT / G) * a.top * sizeof(Entry), s);
+}
+
+template <class T, int NS, int NSM, int BLOCKS, bool FWD>
+int32_t launch_held(const DistillArgs& a, int slices, cudaStream_t s) {
+  static Room room;
+  return launch_clusters(distill_held_kernel<T, NS, NSM, BLOCKS, FWD>, room, a, a.rows, slices, NS + 32,
+                         (size_t)NSM * NS * 16, s);
+}
+
+// Blocks that share a row: as many as keep the rows in flight (two blocks a multiprocessor) small
+// enough for L2 to hold them until the second pass, more when there are few rows.
+int slices_of(const DistillArgs& a, size_t size) {
+  int n = 1;
+  while (n < kMostSlices && (a.classes * size / n > 131072 || a.rows * n < 148) && a.classes * size / n > 8192) n *= 2;
+  return n;
 }
 
 template <bool FWD>
@@ -485,8 +947,19 @@ int32_t dispatch(const NcaDistillDesc& d, const DistillArgs& a, cudaStream_t s) 
     if (a.classes <= 4 && a.top <= 4) return launch_small<T, 1, 4, FWD>(a, s);
     if (a.classes <= 16 && a.top <= 16) return launch_small<T, 4, 4, FWD>(a, s);
     if (a.classes <= 64 && a.top <= 64) return launch_small<T, 8, 8, FWD>(a, s);
-    if (a.classes <= 2048 && a.top <= 512) return launch_rows<T, 32, 256, FWD>(a, s);
-    return launch_rows<T, 512, 512, FWD>(a, s);
+    if (a.classes <= 2048 && a.top <= 512) return launch_rows<T, 32, 256, FWD>(a, 1, s);
+    const size_t bytes = a.classes * sizeof(T);
+    constexpr size_t kSmall = 96 * kHeld * 16, kMiddle = 256 * (kHeld + 8) * 16, kLarge = 992 * (kHeld + 9) * 16;
+    if (a.top <= 32 * kLaneTop && bytes <= kMostSlices * kLarge) {
+      if (bytes <= kSmall) return launch_held<T, 96, 0, 8, FWD>(a, 1, s);
+      int slices = 1;  // a row over several blocks where one cannot hold it, or where there are few rows
+      const bool middle = bytes <= kMiddle || (a.rows < 74 && bytes <= kMostSlices * kMiddle);
+      while (bytes > slices * (middle ? kMiddle : kLarge) ||
+             (slices * 2 <= kMostSlices && a.rows * slices < 148 && bytes > (size_t)slices * 8192))
+        slices *= 2;
+      return middle ? launch_held<T, 256, 8, 3, FWD>(a, slices, s) : launch_held<T, 992, 9, 1, FWD>(a, slices, s);
+    }
+    return launch_rows<T, 512, 512, FWD>(a, slices_of(a, sizeof(T)), s);
   });
 }
 

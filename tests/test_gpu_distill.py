@@ -72,6 +72,26 @@ def test_against_the_oracle(dtype, rows, classes, top):
     check(*inputs(rows, classes, top, dtype, seed=classes), temperature=1.5)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,classes,top,offset", [
+    (2600, 1500, 3, 0),    # more rows than blocks that run at once: a block goes through several
+    (1000, 7001, 2, 1),    # the same, rows on no 16-byte boundary
+    (150, 40003, 5, 3),    # up to a whole multiprocessor for a row
+    (2, 300007, 9, 0),     # a row over a cluster of blocks
+    (3, 20000, 200, 0),    # more entries than the entry warp holds
+])
+def test_rows_that_are_held(dtype, rows, classes, top, offset):
+    g = torch.Generator().manual_seed(rows)
+    wide = (torch.randn((rows, classes + offset), generator=g) * 2).to(DEV, dtype)
+    s = wide[:, offset:]  # with an offset, the gradient's rows are aligned unlike the logits'
+    _, t, i, w = inputs(rows, classes, top, dtype, seed=classes) if rows < 10 else inputs(rows, 50, top, dtype, seed=classes)
+    w[::7] = 0.0
+    i[::5, 0] = -1
+    i[1::5, :2] = classes - 1  # the last class, twice where top > 1
+    loss, grad = check(s, t, i, w, 1.5)
+    assert (loss[::7] == 0).all() and (grad[::7] == 0).all()
+
+
 @pytest.mark.parametrize("temperature", [0.25, 1.0, 8.0])
 @pytest.mark.parametrize("classes", [3, 40, 700, 3001])
 def test_temperatures_and_index_types(temperature, classes):
