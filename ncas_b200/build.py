@@ -18,9 +18,11 @@ OUT = ROOT / "_lib" / "libnca_b200.so"
 # instances of one model shape (compiled in parallel, then linked into one library)
 SOURCES = [CSRC / "api.cu", CSRC / "steps_64_256.cu", CSRC / "steps_32_128.cu",
            CSRC / "steps_16_128.cu", CSRC / "steps_32_256.cu",
-           CSRC / "norm.cu", CSRC / "gated.cu", CSRC / "distill.cu"]  # the cell-training operators
+           CSRC / "norm.cu", CSRC / "norm_held_forward.cu", CSRC / "norm_held_backward.cu",
+           CSRC / "gated.cu", CSRC / "distill.cu"]  # the cell-training operators
 HEADERS = [CSRC / "ptx.cuh", CSRC / "step_kernel.cuh", CSRC / "launch.cuh", CSRC / "cell_ops.cuh",
-           CSRC / "gemm.cuh",
+           CSRC / "gemm.cuh", CSRC / "norm.cuh",
+           CSRC / "norm_held.cuh",
            ROOT.parent / "include" / "nca_b200.h"]
 DEPS = SOURCES + HEADERS
 # the torch operators over the C ABI (ncas_b200._ops), linked against libnca_b200.so

@@ -46,43 +46,129 @@ __device__ __forceinline__ void store_param(void* p, int dtype, long long i, flo
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// ------------------------------------------------------------------------- packed fp32 arithmetic
+// Two fp32 operations in one instruction of sm_100.
+#define NCA_F32X2(name, op)                                                                        \
+  __device__ __forceinline__ float2 name(float2 a, float2 b) {                                     \
+    float2 d;                                                                                      \
+    asm(op " %0, %1, %2;"                                                                          \
+        : "=l"(reinterpret_cast<uint64_t&>(d))                                                     \
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));   \
+    return d;                                                                                      \
+  }
+NCA_F32X2(add2, "add.rn.f32x2")
+NCA_F32X2(mul2, "mul.rn.f32x2")
+#undef NCA_F32X2
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+        "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // ---------------------------------------------------------------------------------- activations
-// 1 / (1 + exp(-z)): exp overflows to inf for z < -88, whose quotient is the limit 0.
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+// Two values at a time.  1 / (1 + exp(-z)): exp overflows to inf for z < -88, whose reciprocal is the
+// limit 0.
+__device__ __forceinline__ float2 sigmoid2(float2 z) {
+  const float2 t = mul2(z, both(-1.4426950408889634f));
+  const float2 d = add2(make_float2(ex2(t.x), ex2(t.y)), both(1.f));
+  return make_float2(rcp(d.x), rcp(d.y));
+}
+__device__ __forceinline__ float2 normal_cdf2(float2 z) {
+  const float2 t = mul2(z, both(0.70710678118654752f));
+  return fma2(make_float2(erff(t.x), erff(t.y)), both(0.5f), both(0.5f));
+}
 
 template <int ACT>
-__device__ __forceinline__ float act_f(float z) {
-  if constexpr (ACT == NCA_ACT_RELU) return z < 0.f ? 0.f : z;  // keeps NaN
-  if constexpr (ACT == NCA_ACT_SILU) return z * sigmoid_f(z);
-  if constexpr (ACT == NCA_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-  if constexpr (ACT == NCA_ACT_SIGMOID) return sigmoid_f(z);
+__device__ __forceinline__ float2 act2(float2 z) {
+  if constexpr (ACT == NCA_ACT_RELU) return make_float2(z.x < 0.f ? 0.f : z.x, z.y < 0.f ? 0.f : z.y);  // keeps NaN
+  if constexpr (ACT == NCA_ACT_SILU) return mul2(z, sigmoid2(z));
+  if constexpr (ACT == NCA_ACT_GELU) return mul2(z, normal_cdf2(z));
+  if constexpr (ACT == NCA_ACT_SIGMOID) return sigmoid2(z);
   return z;
 }
 
-// act(z) and act'(z); relu'(0) = 0.
+// act'(z), and act(z) in `a`; relu'(0) = 0.
 template <int ACT>
-__device__ __forceinline__ float act_slope_f(float z, float& a) {
+__device__ __forceinline__ float2 act_slope2(float2 z, float2& a) {
   if constexpr (ACT == NCA_ACT_RELU) {
-    a = z < 0.f ? 0.f : z;
-    return z > 0.f ? 1.f : 0.f;
+    a = act2<ACT>(z);
+    return make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
   }
   if constexpr (ACT == NCA_ACT_SILU) {
-    const float s = sigmoid_f(z);
-    a = z * s;
-    return s * (1.f + z * (1.f - s));
+    const float2 s = sigmoid2(z);
+    a = mul2(z, s);
+    return fma2(s, mul2(z, fma2(s, both(-1.f), both(1.f))), s);  // s + s z (1 - s)
   }
   if constexpr (ACT == NCA_ACT_GELU) {
-    const float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-    a = z * cdf;
-    return cdf + z * 0.39894228040143268f * __expf(-0.5f * z * z);  // phi(z) = exp(-z^2/2)/sqrt(2 pi)
+    const float2 cdf = normal_cdf2(z);
+    a = mul2(z, cdf);
+    // the density exp(-z^2 / 2) / sqrt(2 pi)
+    const float2 t = mul2(mul2(z, z), both(-0.72134752044448170f));
+    return fma2(mul2(z, both(0.39894228040143268f)), make_float2(ex2(t.x), ex2(t.y)), cdf);
   }
   if constexpr (ACT == NCA_ACT_SIGMOID) {
-    const float s = sigmoid_f(z);
-    a = s;
-    return s * (1.f - s);
+    a = sigmoid2(z);
+    return mul2(a, fma2(a, both(-1.f), both(1.f)));
   }
   a = z;
-  return 1.f;
+  return both(1.f);
+}
+template <int ACT>
+__device__ __forceinline__ float act_f(float z) { return act2<ACT>(both(z)).x; }
+template <int ACT>
+__device__ __forceinline__ float act_slope_f(float z, float& a) {
+  float2 v;
+  const float2 d = act_slope2<ACT>(both(z), v);
+  a = v.x;
+  return d.x;
+}
+
+// V values of a vector as pairs (the pair of a single value repeats it).
+template <class T, int V>
+__device__ __forceinline__ void to_pairs(const Vec<T, V>& v, float2 (&f)[(V + 1) / 2]) {
+  if constexpr (V == 1) {
+    f[0] = both(to_f32(v.v[0]));
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) f[i] = make_float2(v.v[2 * i], v.v[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (__is_same(T, __nv_bfloat16)) f[i] = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162&>(v.v[2 * i]));
+      else f[i] = __half22float2(reinterpret_cast<const __half2&>(v.v[2 * i]));
+    }
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> from_pairs(const float2 (&f)[(V + 1) / 2]) {
+  Vec<T, V> v;
+  if constexpr (V == 1) {
+    v.v[0] = from_f32<T>(f[0].x);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) v.v[2 * i] = f[i].x, v.v[2 * i + 1] = f[i].y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (__is_same(T, __nv_bfloat16)) reinterpret_cast<__nv_bfloat162&>(v.v[2 * i]) = __float22bfloat162_rn(f[i]);
+      else reinterpret_cast<__half2&>(v.v[2 * i]) = __float22half2_rn(f[i]);
+    }
+  }
+  return v;
 }
 
 // ------------------------------------------------------------------------------------ host side

@@ -98,12 +98,6 @@ struct Lanes {
   }
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // -------------------------------------------------------------------------------- few classes
 // G lanes a row, K classes a lane in registers (class j of a row: lane j % G, register j / G), the
 // entries likewise: one read of everything, no second pass.  For top <= G K.

@@ -431,7 +431,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
               const int cc = min(col + i, p.n - 1);
               g[i] = __uint_as_float(r0[i]) + (p.bias[0] ? load_param(p.bias[0], p.bias_dtype, cc) : 0.f);
               u[i] = __uint_as_float(r1[i]) + (p.bias[1] ? load_param(p.bias[1], p.bias_dtype, cc) : 0.f);
-              h[i] = act_f<ACT>(g[i]) * u[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 a = mul2(act2<ACT>(make_float2(g[i], g[i + 1])), make_float2(u[i], u[i + 1]));
+              h[i] = a.x;
+              h[i + 1] = a.y;
             }
             const long long at = (long long)row * p.ldc + col;
             store_row<T>(static_cast<T*>(p.c[0]) + at, h, n, true);
@@ -444,12 +449,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             float g[32], u[32];
             SavedPlanes::load(p.saved + at, p.plane, g, u, n);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float dh = __uint_as_float(r0[i]);
-              float a;
-              const float slope = act_slope_f<ACT>(g[i], a);
-              g[i] = dh * u[i] * slope;
-              u[i] = dh * a;
+            for (int i = 0; i < 32; i += 2) {
+              const float2 dh = make_float2(__uint_as_float(r0[i]), __uint_as_float(r0[i + 1]));
+              float2 a;
+              const float2 slope = act_slope2<ACT>(make_float2(g[i], g[i + 1]), a);
+              const float2 dg = mul2(mul2(dh, make_float2(u[i], u[i + 1])), slope), du = mul2(dh, a);
+              g[i] = dg.x, g[i + 1] = dg.y;
+              u[i] = du.x, u[i + 1] = du.y;
             }
             store_row<T>(static_cast<T*>(p.c[0]) + at, g, n, true);
             store_row<T>(static_cast<T*>(p.c[1]) + at, u, n, true);

@@ -13,35 +13,15 @@
 // thread, however far the data lie from zero or K from the rest.  Partial results are (count, mean,
 // M2 = sum (x - mean)^2) and merge as mean = sum n_i mean_i / n,
 // M2 = sum M2_i + sum n_i (mean_i - mean)^2 (Chan, Golub, LeVeque 1979), in fp32 and in a fixed order.
-#include "cell_ops.cuh"
+#include <algorithm>
+
+#include "norm.cuh"
 
 using namespace nca;
 
 namespace {
 
 constexpr int kThreads = 256;
-
-struct NormArgs {
-  long long n, cells;
-  int channels, groups, per_group;
-  float eps;
-  long long x_sn, x_sl, dy_sn, dy_sl, m_sn, m_sl;
-  int tx, ty;                // threads over channel vectors, over cells
-  int ctiles;                // tiles of tx vectors over the channels
-  int chunks;                // pieces of a sample's cells, one per block at a time
-  long long chunk_cells;
-  int param_dtype;
-  const void* x;
-  const void* weight;
-  const void* bias;
-  const uint8_t* mask;
-  const void* dy;
-  void* y;                   // forward: y; backward: dx
-  float* stats;              // [n][groups][2] mean, rstd
-  float2* part;              // [n][chunks][channels]
-  int* counts;               // [n][chunks] kept cells
-  float2* ab;                // backward: [n][groups] (A / n, B / n)
-};
 
 struct Place {  // what a block works on
   long long sample, c0, c1;  // cells [c0, c1)
@@ -336,11 +316,8 @@ __global__ void norm_param_sums_kernel(const float2* part, long long rows, int c
   const long long r0 = split * per, r1 = min(rows, r0 + per);
   float2 s = make_float2(0.f, 0.f);
   if (ch < channels)
-    for (long long r = r0 + threadIdx.y; r < r1; r += 8) {
-      const float2 e = part[r * channels + ch];
-      s.x += e.x;
-      s.y += e.y;
-    }
+#pragma unroll 4
+    for (long long r = r0 + threadIdx.y; r < r1; r += 8) s = add2(s, part[r * channels + ch]);
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y == 0 && ch < channels) {
@@ -353,14 +330,15 @@ __global__ void norm_param_sums_kernel(const float2* part, long long rows, int c
 }
 __global__ void norm_param_store_kernel(const float2* part, int splits, int channels, void* dweight,
                                         void* dbias, int param_dtype) {
-  const int ch = blockIdx.x * blockDim.x + threadIdx.x;
-  if (ch >= channels) return;
+  __shared__ float2 red[16][32];
+  const int ch = blockIdx.x * 32 + threadIdx.x;
   float2 s = make_float2(0.f, 0.f);
-  for (int k = 0; k < splits; ++k) {
-    const float2 e = part[(long long)k * channels + ch];
-    s.x += e.x;
-    s.y += e.y;
-  }
+  if (ch < channels)
+    for (int k = threadIdx.y; k < splits; k += 16) s = add2(s, part[(long long)k * channels + ch]);
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y || ch >= channels) return;
+  for (int k = 1; k < 16; ++k) s = add2(s, red[k][threadIdx.x]);
   if (dweight) store_param(dweight, param_dtype, ch, s.y);
   if (dbias) store_param(dbias, param_dtype, ch, s.x);
 }
@@ -406,7 +384,7 @@ struct Layout {
   size_t part, counts, ab, params, total;
 };
 Layout layout_of(const NcaNormDesc& d) {
-  const size_t chunks = worst_chunks(d);
+  const size_t chunks = std::max(worst_chunks(d), 16);  // the held backward has up to 16 slices
   Layout l;
   l.part = 0;
   l.counts = l.part + align256((size_t)d.n * chunks * d.channels * sizeof(float2));
@@ -452,13 +430,19 @@ NormArgs args_of(const NcaNormDesc& d, const void* x, const void* weight, const 
 // Widest vector (16 bytes at most) that the channel count, the strides and the addresses allow.
 int vector_width(const NcaNormDesc& d, const NormArgs& a, bool backward) {
   const size_t size = dtype_size(d.dtype);
-  for (int v = (int)(16 / size); v > 1; v /= (size == 2 ? 4 : 4)) {
+  for (int v = (int)(16 / size); v > 1; v /= 2) {
     bool ok = d.channels % v == 0 && d.x_stride_n % v == 0 && d.x_stride_cell % v == 0 &&
               aligned(a.x, v * size) && aligned(a.y, v * size);
     if (backward) ok = ok && d.dy_stride_n % v == 0 && d.dy_stride_cell % v == 0 && aligned(a.dy, v * size);
     if (ok) return v;
   }
   return 1;
+}
+
+// The streaming kernels exist for 16-byte vectors, pairs of 16-bit values and single values.
+int streaming_width(int dtype, int v) {
+  const int w = (int)(16 / dtype_size(dtype));
+  return v == w ? v : (dtype != NCA_F32 && v >= 2 ? 2 : 1);
 }
 
 long long plan(const NcaNormDesc& d, NormArgs& a, int v) {
@@ -471,6 +455,14 @@ long long plan(const NcaNormDesc& d, NormArgs& a, int v) {
 }
 
 inline unsigned grid_of(long long items) { return (unsigned)(items < (1 << 20) ? items : (1 << 20)); }
+
+void param_grads(const float2* part, long long rows, int channels, void* dweight, void* dbias, int param_dtype,
+                 float2* params, cudaStream_t s) {
+  const int splits = (int)(rows < 8 * kParamSplits ? (rows + 7) / 8 : kParamSplits);
+  norm_param_sums_kernel<<<dim3((channels + 31) / 32, splits), dim3(32, 8), 0, s>>>(part, rows, channels, splits,
+                                                                                 params);
+  norm_param_store_kernel<<<(channels + 31) / 32, dim3(32, 16), 0, s>>>(params, splits, channels, dweight, dbias, param_dtype);
+}
 
 template <class T, int V, int ACT>
 int32_t forward(const NcaNormDesc& d, NormArgs a, cudaStream_t s) {
@@ -494,14 +486,7 @@ int32_t backward(const NcaNormDesc& d, NormArgs a, void* dweight, void* dbias, f
     norm_grad_merge_kernel<<<(unsigned)((a.n * a.groups + 7) / 8), 256, 0, s>>>(a);
     norm_grad_apply_kernel<T, V, ACT><<<grid_of(items), threads, 0, s>>>(a, items);
   }
-  if (dweight || dbias) {
-    const long long rows = a.n * a.chunks;
-    const int splits = (int)(rows < 8 * kParamSplits ? (rows + 7) / 8 : kParamSplits);
-    norm_param_sums_kernel<<<dim3((a.channels + 31) / 32, splits), dim3(32, 8), 0, s>>>(
-        a.part, rows, a.channels, splits, params);
-    norm_param_store_kernel<<<(a.channels + 127) / 128, 128, 0, s>>>(params, splits, a.channels, dweight,
-                                                                      dbias, a.param_dtype);
-  }
+  if (dweight || dbias) param_grads(a.part, a.n * a.chunks, a.channels, dweight, dbias, a.param_dtype, params, s);
   return launch_status();
 }
 
@@ -514,7 +499,8 @@ int32_t dispatch(const NcaNormDesc& d, int v, F fn) {
       constexpr int A = decltype(act)::value;
       constexpr int W = 16 / sizeof(T);
       if (v == W) return fn.template operator()<T, W, A>();
-      if (sizeof(T) == 2 && v == 2) return fn.template operator()<T, 2, A>();
+      if constexpr (sizeof(T) == 2)
+        if (v == 2) return fn.template operator()<T, 2, A>();
       return fn.template operator()<T, 1, A>();
     });
   });
@@ -556,7 +542,10 @@ int32_t nca_b200_group_norm(const NcaNormDesc* d, const void* x, const void* wei
   if (d->n == 0 || d->cells == 0) return NCA_OK;
   if (!x || !y || !stats || !workspace || workspace_bytes < layout_of(*d).total) return NCA_ERR_INVALID;
   const NormArgs a = args_of(*d, x, weight, bias, mask, nullptr, y, stats, workspace);
-  return dispatch(*d, vector_width(*d, a, false), ForwardCall{*d, a, static_cast<cudaStream_t>(stream)});
+  const int v = vector_width(*d, a, false);
+  if (norm_held_applies(a, d->dtype, v, false))
+    return norm_held_forward(a, d->dtype, d->act, v, static_cast<cudaStream_t>(stream));
+  return dispatch(*d, streaming_width(d->dtype, v), ForwardCall{*d, a, static_cast<cudaStream_t>(stream)});
 }
 
 int32_t nca_b200_group_norm_backward(const NcaNormDesc* d, const void* x, const void* weight,
@@ -575,7 +564,16 @@ int32_t nca_b200_group_norm_backward(const NcaNormDesc* d, const void* x, const 
   if (!x || !dy || !stats || !workspace || workspace_bytes < layout_of(*d).total) return NCA_ERR_INVALID;
   const NormArgs a = args_of(*d, x, weight, bias, mask, dy, dx, const_cast<float*>(stats), workspace);
   float2* params = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + layout_of(*d).params);
-  return dispatch(*d, vector_width(*d, a, true), BackwardCall{*d, a, dweight, dbias, params, s});
+  const int v = vector_width(*d, a, true);
+  if (norm_held_applies(a, d->dtype, v, true)) {
+    NormArgs b = a;
+    if (!dweight && !dbias) b.part = nullptr;
+    const int32_t r = norm_held_backward(b, d->dtype, d->act, v, s);
+    if (r != NCA_OK || !b.part) return r;
+    param_grads(a.part, a.n * norm_held_slices(a, d->dtype, v), a.channels, dweight, dbias, a.param_dtype, params, s);
+    return launch_status();
+  }
+  return dispatch(*d, streaming_width(d->dtype, v), BackwardCall{*d, a, dweight, dbias, params, s});
 }
 
 }  // extern "C"

@@ -1,0 +1,37 @@
+// norm.cuh -- arguments that the streaming (norm.cu) and the held (norm_held.cu) group norm share.
+#pragma once
+#include "cell_ops.cuh"
+
+namespace nca {
+
+struct NormArgs {
+  long long n, cells;
+  int channels, groups, per_group;
+  float eps;
+  long long x_sn, x_sl, dy_sn, dy_sl, m_sn, m_sl;
+  int tx, ty;                // threads over channel vectors, over cells
+  int ctiles;                // tiles of tx vectors over the channels
+  int chunks;                // pieces of a sample's cells, one per block at a time
+  long long chunk_cells;
+  int param_dtype;
+  const void* x;
+  const void* weight;
+  const void* bias;
+  const uint8_t* mask;
+  const void* dy;
+  void* y;                   // forward: y; backward: dx
+  float* stats;              // [n][groups][2] mean, rstd
+  float2* part;              // [n][chunks][channels]
+  int* counts;               // [n][chunks] kept cells
+  float2* ab;                // backward: [n][groups] (A / n, B / n)
+};
+
+// Runs the forward or backward kernel that holds samples in shared memory, when it applies: returns
+// false when it does not.  `v` is the vector width that channels, strides and addresses allow.  The
+// backward writes (sum dz, sum dz h) of every sample and slice to a.part as [n][slices][channels].
+int norm_held_slices(const NormArgs& a, int dtype, int v);  // of the backward, at most 16
+bool norm_held_applies(const NormArgs& a, int dtype, int v, bool backward);
+int32_t norm_held_forward(const NormArgs& a, int dtype, int act, int v, cudaStream_t s);
+int32_t norm_held_backward(const NormArgs& a, int dtype, int act, int v, cudaStream_t s);
+
+}  // namespace nca

@@ -1,0 +1,215 @@
+// norm_held.cuh -- group norm with an activation, samples held in shared memory: every value is read
+// from memory once (forward: x in, y out; backward: x and dy in, dx out).
+//
+// A block, or a cluster of `slices` blocks that split the cells, takes one sample, or a block of its
+// channels that ends on group borders.  A thread owns the same V adjacent channels (one group) of every
+// TY-th cell and copies its values asynchronously into places of its own in shared memory, so that no
+// thread waits for another's data (norm_held_forward.cu, norm_held_backward.cu); statistics are merged through shared memory, and over a cluster
+// through distributed shared memory.
+//
+// The mathematics and the treatment of sums are those of norm.cu.  Bound by HBM; the copies of the
+// blocks that share a multiprocessor overlap with each other's arithmetic and writes.
+#pragma once
+#include <atomic>
+
+#include "norm.cuh"
+
+namespace nca {
+namespace {
+
+constexpr int kMaxThreads = 512;
+constexpr int kMaxSlices = 16;
+constexpr int kMaxGroups = 64;  // of one block
+
+struct HeldArgs {
+  NormArgs a;
+  int cb;             // channels of a block
+  int cblocks;        // blocks of channels
+  int slices;
+  long long slice_cells;
+  int iters;          // places of a thread
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void put_remote(const float4* p, uint32_t rank, float4 v) {
+  uint32_t a = (uint32_t)__cvta_generic_to_shared(p), r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(r), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+               : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const uint32_t a = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(a), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// What a thread works on.
+struct Work {
+  long long sample;
+  int ch0, ch, group;  // first channel of the block, of the thread; group of the thread within the block
+  int col, row, rank;
+  long long c0;        // first cell of the slice
+  int cells;           // and how many
+  bool on;
+};
+template <int V>
+__device__ __forceinline__ Work work_of(const HeldArgs& h) {
+  Work w;
+  const long long id = blockIdx.x / h.slices;
+  w.rank = h.slices > 1 ? (int)cluster_rank() : 0;
+  w.sample = id / h.cblocks;
+  w.ch0 = (int)(id % h.cblocks) * h.cb;
+  w.col = threadIdx.x % h.a.tx;
+  w.row = threadIdx.x / h.a.tx;
+  w.ch = w.ch0 + w.col * V;
+  w.group = w.col * V / h.a.per_group;
+  w.c0 = w.rank * h.slice_cells;
+  w.cells = (int)min(h.a.cells - w.c0, h.slice_cells);
+  w.on = w.row < h.a.ty && w.ch < h.a.channels;
+  return w;
+}
+// Goes through the thread's cells: f(place in shared memory, cell of the slice) where the cell counts, g
+// where the mask leaves it out.
+template <bool MASK, class F, class G>
+__device__ __forceinline__ void each_cell(const NormArgs& a, const Work& w, F f, G g) {
+  int at = threadIdx.x;
+  const int first = w.on ? w.row : w.cells;
+  const uint8_t* m = MASK ? a.mask + w.sample * a.m_sn + (w.c0 + first) * a.m_sl : nullptr;
+  for (int c = first; c < w.cells; c += a.ty, at += blockDim.x) {
+    if (!MASK || *m != 0) f(at, c);
+    else g(at, c);
+    if (MASK) m += a.ty * a.m_sl;
+  }
+}
+
+// --------------------------------------------------------------------------------- host side
+struct HeldPlan {
+  bool ok;
+  int v, cb, cblocks, slices, tx, ty, iters, threads;
+  long long slice_cells;
+  size_t smem;
+};
+
+HeldPlan plan_of(const NormArgs& a, int dtype, int width, bool backward) {
+  HeldPlan p{};
+  const size_t size = dtype_size(dtype);
+  int v = width;
+  while (v > 1 && a.per_group % v) v /= 2;
+  if (v * size < 4) return p;  // an asynchronous copy moves 4 bytes at least
+  p.v = v;
+  const size_t tensors = backward ? 2 : 1;
+  // channels of a block: all of them, or as few groups as leave 64 adjacent bytes when a sample is large
+  const size_t sample = (size_t)a.cells * a.channels * size * tensors;
+  const size_t kFew = 72 * 1024, kTwo = 100 * 1024, kOne = 190 * 1024;
+  int groups = a.groups;
+  const auto fits = [&](int g) { return (size_t)a.cells * g * a.per_group * size * tensors <= kMaxSlices * kOne; };
+  (void)sample;
+  while (!fits(groups) || groups > kMaxGroups || groups * a.per_group / v > kMaxThreads) {
+    int next = groups - 1;
+    while (next > 0 && a.groups % next) --next;
+    if (next <= 0) return p;
+    groups = next;
+  }
+  if (groups < a.groups && groups * a.per_group * size < 32) return p;
+  // a large sample: fewer channels rather than the largest clusters
+  while (groups > 1 && (size_t)a.cells * groups * a.per_group * size * tensors > 8 * kTwo) {
+    int next = groups - 1;
+    while (next > 0 && a.groups % next) --next;
+    if (next <= 0 || next * a.per_group * size < 64) break;
+    groups = next;
+  }
+  p.cb = groups * a.per_group;
+  p.cblocks = a.groups / groups;
+  const size_t bytes = (size_t)a.cells * p.cb * size * tensors;
+  long long slices = (long long)((bytes + kFew - 1) / kFew);
+  if (slices > 8) slices = (long long)((bytes + kTwo - 1) / kTwo);
+  if (slices > kMaxSlices) slices = (long long)((bytes + kOne - 1) / kOne);
+  if (slices > kMaxSlices) return p;
+  // few samples: over more blocks, 8 KB each at least
+  while (slices < 8 && a.n * p.cblocks * slices < 148 && (long long)bytes / slices > 16384 && slices * 2 <= a.cells) slices *= 2;
+  if (slices > a.cells) slices = a.cells;
+  p.slice_cells = (a.cells + slices - 1) / slices;
+  p.slices = (int)((a.cells + p.slice_cells - 1) / p.slice_cells);
+  p.tx = p.cb / v;
+  const long long ty_max = kMaxThreads / p.tx;
+  long long iters = (p.slice_cells + ty_max - 1) / ty_max;
+  if (iters < 8) iters = p.slice_cells < 8 ? p.slice_cells : 8;
+  p.ty = (int)((p.slice_cells + iters - 1) / iters);
+  p.iters = (int)((p.slice_cells + p.ty - 1) / p.ty);
+  p.threads = (p.tx * p.ty + 31) / 32 * 32;
+  p.smem = (size_t)p.iters * p.threads * v * size * tensors;
+  p.smem += (size_t)p.slices * groups * sizeof(float4) + (size_t)p.ty * sizeof(int);
+  if (backward) p.smem += ((size_t)p.ty * p.tx * v + p.cb) * sizeof(float2);
+  else p.smem += (size_t)p.threads * sizeof(float2);
+  p.ok = p.smem <= 208 * 1024 && a.n * p.cblocks * p.slices < (1ll << 31);
+  return p;
+}
+
+constexpr int kMaxDevices = 64;
+
+int32_t launch(void (*kernel)(HeldArgs), std::atomic<uint64_t>& ready, const NormArgs& a, const HeldPlan& p,
+               cudaStream_t s) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
+  if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+      const int32_t st = launch_status();
+      return st == NCA_OK ? NCA_ERR_CUDA : st;
+    }
+    ready.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  HeldArgs h{a, p.cb, p.cblocks, p.slices, p.slice_cells, p.iters};
+  h.a.tx = p.tx;
+  h.a.ty = p.ty;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.n * p.cblocks * p.slices));
+  cfg.blockDim = dim3(p.threads);
+  cfg.dynamicSmemBytes = p.smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.slices;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.slices > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, h) != cudaSuccess) {
+    const int32_t st = launch_status();
+    return st == NCA_OK ? NCA_ERR_CUDA : st;
+  }
+  return launch_status();
+}
+
+
+// Instantiates fn(T, V, ACT, MASK) for the run-time choice.
+template <class F>
+int32_t dispatch_held(const NormArgs& a, int dtype, int act, int v, F fn) {
+  return with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    constexpr int W = 16 / sizeof(T);
+    return with_act(act, [&](auto tag) {
+      constexpr int A = decltype(tag)::value;
+      if (v == W) return a.mask ? fn.template operator()<T, W, A, true>() : fn.template operator()<T, W, A, false>();
+      if (v == W / 2) return a.mask ? fn.template operator()<T, W / 2, A, true>() : fn.template operator()<T, W / 2, A, false>();
+      return a.mask ? fn.template operator()<T, W / 4, A, true>() : fn.template operator()<T, W / 4, A, false>();
+    });
+  });
+}
+
+}  // namespace
+}  // namespace nca
