@@ -14,6 +14,7 @@
 // M2 = sum (x - mean)^2) and merge as mean = sum n_i mean_i / n,
 // M2 = sum M2_i + sum n_i (mean_i - mean)^2 (Chan, Golub, LeVeque 1979), in fp32 and in a fixed order.
 #include <algorithm>
+#include <atomic>
 
 #include "norm.cuh"
 
@@ -43,44 +44,132 @@ __device__ __forceinline__ Place place_of(const NormArgs& a, long long item) {
   return p;
 }
 
-__device__ __forceinline__ bool kept(const NormArgs& a, const Place& p, long long cell) {
-  return !a.mask || a.mask[p.sample * a.m_sn + cell * a.m_sl] != 0;
+// The cells of a thread that the mask keeps, a bit each (a block's piece has at most 32 a thread).
+template <bool MASK>
+__device__ __forceinline__ uint32_t kept_of(const NormArgs& a, const Place& p, int n) {
+  if constexpr (!MASK) return ~0u;
+  uint32_t bits = 0;
+  const long long step = a.ty * a.m_sl;
+  const uint8_t* m = a.mask + p.sample * a.m_sn + (p.c0 + threadIdx.x / a.tx) * a.m_sl;
+  for (int i = 0; i < n; i += 8, m += 8 * step) {
+    uint8_t v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = i + u < n ? m[u * step] : 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) bits |= (uint32_t)(v[u] != 0) << (i + u);
+  }
+  return bits;
+}
+
+// Goes through the thread's cells: use(cell of the piece, x vector, second vector) where the mask keeps the
+// cell, left_out(cell) elsewhere.  The vectors (one or two tensors) come through a ring of kRing
+// asynchronous copies in places of the thread's own, so that kRing cells are in flight all the time and
+// no thread waits for another; single 16-bit values, which such copies cannot move, are loaded directly.
+constexpr int kRing = 8;
+template <class T, int V>
+__host__ __device__ constexpr size_t ring_bytes(int tensors) {
+  return V * sizeof(T) >= 4 ? (size_t)kRing * tensors * kThreads * V * sizeof(T) : 0;
+}
+template <class T, int V, int TENSORS, bool MASK, class U, class O>
+__device__ __forceinline__ void each_cell(const NormArgs& a, const Place& p, void* ring, const T* x, long long x_step,
+                                          const T* g, long long g_step, U use, O left_out) {
+  using VecT = Vec<T, V>;
+  const int row = threadIdx.x / a.tx;
+  const int n = p.active ? (int)((p.c1 - p.c0 - row + a.ty - 1) / a.ty) : 0;  // cells of this thread
+  if (n <= 0) return;
+  uint32_t bits = kept_of<MASK>(a, p, n);
+  x += (p.c0 + row) * x_step;
+  x_step *= a.ty;
+  if (TENSORS > 1) {
+    g += (p.c0 + row) * g_step;
+    g_step *= a.ty;
+  }
+  if constexpr (V * sizeof(T) >= 4) {
+    VecT* place = static_cast<VecT*>(ring) + threadIdx.x;
+    uint32_t to_fetch = bits;
+    const auto fetch = [&](int slot, bool in) {
+      if (in && (to_fetch & 1)) {
+        copy_async<sizeof(VecT)>(place + slot * TENSORS * kThreads, x);
+        if (TENSORS > 1) copy_async<sizeof(VecT)>(place + (slot * TENSORS + 1) * kThreads, g);
+      }
+      to_fetch = MASK ? to_fetch >> 1 : to_fetch;
+      x += x_step;
+      if (TENSORS > 1) g += g_step;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) fetch(i, i < n);
+    int slot = 0;
+    for (int i = 0; i < n; ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+      if (bits & 1) {
+        const VecT xv = place[slot * TENSORS * kThreads];
+        use(row + i * a.ty, xv, TENSORS > 1 ? place[(slot * TENSORS + 1) * kThreads] : xv);
+      } else {
+        left_out(row + i * a.ty);
+      }
+      bits = MASK ? bits >> 1 : bits;
+      fetch(slot, i + kRing < n);
+      slot = slot + 1 == kRing ? 0 : slot + 1;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    for (int i = 0; i < n; ++i) {
+      if (bits & 1) {
+        const VecT xv = *reinterpret_cast<const VecT*>(x);
+        use(row + i * a.ty, xv, TENSORS > 1 ? *reinterpret_cast<const VecT*>(g) : xv);
+      } else {
+        left_out(row + i * a.ty);
+      }
+      bits = MASK ? bits >> 1 : bits;
+      x += x_step;
+      if (TENSORS > 1) g += g_step;
+    }
+  }
 }
 
 // ------------------------------------------------------------------------- forward: statistics
-template <class T, int V>
+template <class T, int V, bool MASK>
 __global__ void __launch_bounds__(kThreads) norm_stats_kernel(NormArgs a, long long items) {
-  extern __shared__ float2 red[];  // [ty][tx * V] (mean, M2), then [ty] counts
+  constexpr int P = (V + 1) / 2;
+  extern __shared__ float2 red[];  // the ring; after it [ty][tx * V] (mean, M2), then [ty] counts
   int* rc = reinterpret_cast<int*>(red + a.ty * a.tx * V);
   const int row = threadIdx.x / a.tx, col = (threadIdx.x % a.tx) * V;
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
     const Place p = place_of<V>(a, item);
-    float k[V], s1[V], s2[V];
+    float2 k[P], s1[P], s2[P];
 #pragma unroll
-    for (int v = 0; v < V; ++v) k[v] = s1[v] = s2[v] = 0.f;
+    for (int i = 0; i < P; ++i) k[i] = s1[i] = s2[i] = both(0.f);
     int cnt = 0;
     const T* x = static_cast<const T*>(a.x) + p.sample * a.x_sn + p.ch;
-    for (long long c = p.c0 + row; c < p.c1; c += a.ty) {
-      if (!kept(a, p, c)) continue;
-      if (p.active) {
-        const Vec<T, V> xv = *reinterpret_cast<const Vec<T, V>*>(x + c * a.x_sl);
+    each_cell<T, V, 1, MASK>(
+        a, p, red, x, a.x_sl, nullptr, 0,
+        [&](int, const Vec<T, V>& xv, const Vec<T, V>&) {
+          float2 f[P];
+          to_pairs<T, V>(xv, f);
+          if (cnt == 0) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float f = to_f32(xv.v[v]);
-          if (cnt == 0) k[v] = f;
-          const float d = f - k[v];
-          s1[v] += d;
-          s2[v] = fmaf(d, d, s2[v]);
-        }
-      }
-      ++cnt;
-    }
-    __syncthreads();  // the previous item's partials have been read
+            for (int i = 0; i < P; ++i) k[i] = f[i];
+          }
+          ++cnt;
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const float2 d = fma2(k[i], both(-1.f), f[i]);
+            s1[i] = add2(s1[i], d);
+            s2[i] = fma2(d, d, s2[i]);
+          }
+        },
+        [](int) {});
+    __syncthreads();  // the ring has been read
     const float inv = cnt ? 1.f / (float)cnt : 0.f;
+    const auto put = [&](int v, float k, float s1, float s2) {
+      const float m = s1 * inv, rest = s2 - s1 * m;
+      red[row * a.tx * V + col + v] = make_float2(k + m, rest < 0.f ? 0.f : rest);  // keeps NaN
+    };
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float m = s1[v] * inv;
-      red[row * a.tx * V + col + v] = make_float2(k[v] + m, fmaxf(s2[v] - s1[v] * m, 0.f));
+    for (int i = 0; i < P; ++i) {
+      put(2 * i, k[i].x, s1[i].x, s2[i].x);
+      if (V > 1) put(2 * i + 1, k[i].y, s1[i].y, s2[i].y);
     }
     if (col == 0) rc[row] = cnt;
     __syncthreads();
@@ -90,7 +179,7 @@ __global__ void __launch_bounds__(kThreads) norm_stats_kernel(NormArgs a, long l
       const int ch = (int)(item % a.ctiles) * a.tx * V + i;
       if (ch >= a.channels) break;
       float mean = 0.f, m2 = 0.f;
-      for (int r = 0; r < a.ty; ++r) mean += (float)rc[r] * red[r * a.tx * V + i].x;
+      for (int r = 0; r < a.ty; ++r) mean += rc[r] ? (float)rc[r] * red[r * a.tx * V + i].x : 0.f;
       mean = total ? mean / (float)total : 0.f;
       for (int r = 0; r < a.ty; ++r) {
         const float2 e = red[r * a.tx * V + i];
@@ -100,6 +189,7 @@ __global__ void __launch_bounds__(kThreads) norm_stats_kernel(NormArgs a, long l
       a.part[(p.sample * a.chunks + p.chunk) * a.channels + ch] = make_float2(mean, m2);
     }
     if (threadIdx.x == 0 && item % a.ctiles == 0) a.counts[p.sample * a.chunks + p.chunk] = total;
+    __syncthreads();  // the partial results have been read
   }
 }
 
@@ -109,129 +199,168 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// One warp per (sample, group): merges its chunks x per_group partials.
-__global__ void norm_stats_merge_kernel(NormArgs a) {
-  const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (w >= a.n * a.groups) return;
-  const long long sample = w / a.groups;
-  const int g = (int)(w % a.groups);
-  const int* cnt = a.counts + sample * a.chunks;
-  const float2* part = a.part + sample * a.chunks * a.channels + g * a.per_group;
-  const long long entries = (long long)a.chunks * a.per_group;
-  float n = 0.f, mean = 0.f, m2 = 0.f;
-  for (long long i = lane; i < entries; i += 32) {
-    const int k = (int)(i / a.per_group), c = (int)(i % a.per_group);
-    const float f = (float)cnt[k];
-    n += f;
-    mean = fmaf(f, part[(long long)k * a.channels + c].x, mean);
-  }
-  n = warp_sum(n);
-  mean = warp_sum(mean);
-  mean = n > 0.f ? mean / n : 0.f;
-  for (long long i = lane; i < entries; i += 32) {
-    const int k = (int)(i / a.per_group), c = (int)(i % a.per_group);
-    const float f = (float)cnt[k];
-    const float2 e = part[(long long)k * a.channels + c];
-    const float d = e.x - mean;
-    if (f > 0.f) m2 += fmaf(f * d, d, e.y);
-  }
-  m2 = warp_sum(m2);
-  if (lane == 0) {
-    a.stats[2 * w] = mean;
-    a.stats[2 * w + 1] = n > 0.f ? 1.f / sqrtf(m2 / n + a.eps) : 0.f;
+// A block per (sample, group) goes through its chunks x per_group partial results: f(chunk, channel).
+constexpr int kMergeThreads = 256;
+template <class F>
+__device__ __forceinline__ void each_partial(const NormArgs& a, F f) {
+  const int wide = min(a.per_group, kMergeThreads), high = kMergeThreads / wide;
+  const int k0 = threadIdx.x / wide, c0 = threadIdx.x % wide;
+  if (k0 >= high) return;
+  for (int c = c0; c < a.per_group; c += wide)
+#pragma unroll 8
+    for (int k = k0; k < a.chunks; k += high) f(k, c);
+}
+__device__ __forceinline__ float block_sum(float v, float* red) {  // in every thread, in a fixed order
+  v = warp_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int i = 1; i < kMergeThreads / 32; ++i) v += red[i];
+  return v;
+}
+
+__global__ void __launch_bounds__(kMergeThreads) norm_stats_merge_kernel(NormArgs a) {
+  __shared__ float red[kMergeThreads / 32];
+  for (long long w = blockIdx.x; w < a.n * a.groups; w += gridDim.x) {
+    const long long sample = w / a.groups;
+    const int* cnt = a.counts + sample * a.chunks;
+    const float2* part = a.part + sample * a.chunks * a.channels + (w % a.groups) * a.per_group;
+    float n = 0.f, mean = 0.f, m2 = 0.f;
+    each_partial(a, [&](int k, int c) {
+      const float f = (float)cnt[k];
+      n += f;
+      if (f > 0.f) mean = fmaf(f, part[(long long)k * a.channels + c].x, mean);
+    });
+    n = block_sum(n, red);
+    mean = block_sum(mean, red);
+    mean = n > 0.f ? mean / n : 0.f;
+    each_partial(a, [&](int k, int c) {
+      const float f = (float)cnt[k];
+      const float2 e = part[(long long)k * a.channels + c];
+      const float d = e.x - mean;
+      if (f > 0.f) m2 += fmaf(f * d, d, e.y);
+    });
+    m2 = block_sum(m2, red);
+    if (threadIdx.x == 0) {
+      a.stats[2 * w] = mean;
+      a.stats[2 * w + 1] = n > 0.f ? 1.f / sqrtf(m2 / n + a.eps) : 0.f;
+    }
   }
 }
 
-// The per-channel values of a thread: mean, rstd * weight and bias (rstd and weight apart in the
-// backward).  h uses x - mean: x a + b with b = -mean a would cancel for a large mean.
-template <int V>
+// The per-channel values of a thread.  h uses x - mean: x a + b with b = -mean a would cancel for a
+// large mean.
+// ONE: the V channels lie in one group.
+template <int V, bool ONE>
 struct ChannelValues {
-  float mean[V], rstd[V], w[V], b[V];
+  static constexpr int P = (V + 1) / 2, Q = ONE ? 1 : P;
+  float2 away[Q], rstd[Q];  // -mean, 1 / sqrt(var + eps)
+  float2 w[P], b[P];        // weight, bias
   __device__ __forceinline__ void load(const NormArgs& a, const Place& p) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const long long sg = p.sample * a.groups + (p.ch + v) / a.per_group;
-      mean[v] = a.stats[2 * sg];
-      rstd[v] = a.stats[2 * sg + 1];
-      w[v] = a.weight ? load_param(a.weight, a.param_dtype, p.ch + v) : 1.f;
-      b[v] = a.bias ? load_param(a.bias, a.param_dtype, p.ch + v) : 0.f;
+    for (int i = 0; i < Q; ++i) {
+      const int c0 = p.ch + 2 * i, c1 = ONE ? c0 : c0 + (V > 1);
+      const float* s0 = a.stats + 2 * (p.sample * a.groups + c0 / a.per_group);
+      const float* s1 = a.stats + 2 * (p.sample * a.groups + c1 / a.per_group);
+      away[i] = make_float2(-s0[0], -s1[0]);
+      rstd[i] = make_float2(s0[1], s1[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c0 = p.ch + 2 * i, c1 = c0 + (V > 1);
+      w[i] = a.weight ? make_float2(load_param(a.weight, a.param_dtype, c0), load_param(a.weight, a.param_dtype, c1)) : both(1.f);
+      b[i] = a.bias ? make_float2(load_param(a.bias, a.param_dtype, c0), load_param(a.bias, a.param_dtype, c1)) : both(0.f);
     }
   }
+  __device__ __forceinline__ float2 away_of(int i) const { return away[ONE ? 0 : i]; }
+  __device__ __forceinline__ float2 rstd_of(int i) const { return rstd[ONE ? 0 : i]; }
 };
 
-template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) norm_apply_kernel(NormArgs a, long long items) {
-  const int row = threadIdx.x / a.tx;
+template <class T, int V>
+__device__ __forceinline__ void write_zeros(T* to) {
+  Vec<T, V> v;
+#pragma unroll
+  for (int i = 0; i < V; ++i) v.v[i] = from_f32<T>(0.f);
+  *reinterpret_cast<Vec<T, V>*>(to) = v;
+}
+
+template <class T, int V, int ACT, bool MASK, bool ONE>
+__global__ void __launch_bounds__(kThreads, 4) norm_apply_kernel(NormArgs a, long long items) {
+  constexpr int P = (V + 1) / 2;
+  extern __shared__ uint4 ring[];
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-    const Place p = place_of<V>(a, item);
+    // from the end: L2 still holds what the pass before read last
+    const Place p = place_of<V>(a, items - 1 - item);
     if (!p.active) continue;
-    ChannelValues<V> cv;
+    ChannelValues<V, ONE> cv;
     cv.load(a, p);
+#pragma unroll
+    for (int i = 0; i < P; ++i) cv.w[i] = mul2(cv.w[i], cv.rstd_of(i));
     const T* x = static_cast<const T*>(a.x) + p.sample * a.x_sn + p.ch;
-    T* y = static_cast<T*>(a.y) + p.sample * a.cells * a.channels + p.ch;
-    for (long long c = p.c0 + row; c < p.c1; c += a.ty) {
-      Vec<T, V> yv;
-      if (kept(a, p, c)) {
-        const Vec<T, V> xv = *reinterpret_cast<const Vec<T, V>*>(x + c * a.x_sl);
+    T* y = static_cast<T*>(a.y) + (p.sample * a.cells + p.c0) * a.channels + p.ch;
+    each_cell<T, V, 1, MASK>(
+        a, p, ring, x, a.x_sl, nullptr, 0,
+        [&](int c, const Vec<T, V>& xv, const Vec<T, V>&) {
+          float2 f[P];
+          to_pairs<T, V>(xv, f);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float h = (to_f32(xv.v[v]) - cv.mean[v]) * cv.rstd[v];
-          yv.v[v] = from_f32<T>(act_f<ACT>(fmaf(h, cv.w[v], cv.b[v])));
-        }
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) yv.v[v] = from_f32<T>(0.f);
-      }
-      *reinterpret_cast<Vec<T, V>*>(y + c * a.channels) = yv;
-    }
+          for (int i = 0; i < P; ++i) f[i] = act2<ACT>(fma2(add2(f[i], cv.away_of(i)), cv.w[i], cv.b[i]));
+          *reinterpret_cast<Vec<T, V>*>(y + (long long)c * a.channels) = from_pairs<T, V>(f);
+        },
+        [&](int c) { write_zeros<T, V>(y + (long long)c * a.channels); });
   }
 }
 
 // ---------------------------------------------------------------------------------- backward
-template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) norm_grad_sums_kernel(NormArgs a, long long items) {
-  extern __shared__ float2 red[];  // [ty][tx * V] (sum dz, sum dz h), then [ty] counts
+template <class T, int V, int ACT, bool MASK, bool ONE>
+__global__ void __launch_bounds__(kThreads, 3) norm_grad_sums_kernel(NormArgs a, long long items) {
+  constexpr int P = (V + 1) / 2;
+  extern __shared__ float2 red[];  // the ring; after it [ty][tx * V] (sum dz, sum dz h), then [ty] counts
   int* rc = reinterpret_cast<int*>(red + a.ty * a.tx * V);
   const int row = threadIdx.x / a.tx, col = (threadIdx.x % a.tx) * V;
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
     const Place p = place_of<V>(a, item);
-    ChannelValues<V> cv;
+    ChannelValues<V, ONE> cv;
     if (p.active) cv.load(a, p);
-    float s1[V], s2[V];
+    float2 s1[P], s2[P];
 #pragma unroll
-    for (int v = 0; v < V; ++v) s1[v] = s2[v] = 0.f;
+    for (int i = 0; i < P; ++i) s1[i] = s2[i] = both(0.f);
     int cnt = 0;
     const T* x = static_cast<const T*>(a.x) + p.sample * a.x_sn + p.ch;
     const T* dy = static_cast<const T*>(a.dy) + p.sample * a.dy_sn + p.ch;
-    for (long long c = p.c0 + row; c < p.c1; c += a.ty) {
-      if (!kept(a, p, c)) continue;
-      ++cnt;
-      if (!p.active) continue;
-      const Vec<T, V> xv = *reinterpret_cast<const Vec<T, V>*>(x + c * a.x_sl);
-      const Vec<T, V> gv = *reinterpret_cast<const Vec<T, V>*>(dy + c * a.dy_sl);
+    each_cell<T, V, 2, MASK>(
+        a, p, red, x, a.x_sl, dy, a.dy_sl,
+        [&](int, const Vec<T, V>& xv, const Vec<T, V>& gv) {
+          ++cnt;
+          float2 f[P], g[P];
+          to_pairs<T, V>(xv, f);
+          to_pairs<T, V>(gv, g);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float h = (to_f32(xv.v[v]) - cv.mean[v]) * cv.rstd[v];
-        float unused;
-        const float dz = to_f32(gv.v[v]) * act_slope_f<ACT>(fmaf(h, cv.w[v], cv.b[v]), unused);
-        s1[v] += dz;
-        s2[v] = fmaf(dz, h, s2[v]);
-      }
+          for (int i = 0; i < P; ++i) {
+            const float2 h = mul2(add2(f[i], cv.away_of(i)), cv.rstd_of(i));
+            float2 unused;
+            const float2 dz = mul2(g[i], act_slope2<ACT>(fma2(h, cv.w[i], cv.b[i]), unused));
+            s1[i] = add2(s1[i], dz);
+            s2[i] = fma2(dz, h, s2[i]);
+          }
+        },
+        [](int) {});
+    __syncthreads();  // the ring has been read
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      float2* to = red + row * a.tx * V + col + 2 * i;
+      to[0] = make_float2(s1[i].x, s2[i].x);
+      if (V > 1) to[1] = make_float2(s1[i].y, s2[i].y);
     }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < V; ++v) red[row * a.tx * V + col + v] = make_float2(s1[v], s2[v]);
     if (col == 0) rc[row] = cnt;
     __syncthreads();
     for (int i = threadIdx.x; i < a.tx * V; i += blockDim.x) {
       const int ch = (int)(item % a.ctiles) * a.tx * V + i;
       if (ch >= a.channels) break;
-      float2 s = make_float2(0.f, 0.f);
-      for (int r = 0; r < a.ty; ++r) {
-        s.x += red[r * a.tx * V + i].x;
-        s.y += red[r * a.tx * V + i].y;
-      }
+      float2 s = both(0.f);
+      for (int r = 0; r < a.ty; ++r) s = add2(s, red[r * a.tx * V + i]);
       a.part[(p.sample * a.chunks + p.chunk) * a.channels + ch] = s;
     }
     if (threadIdx.x == 0 && item % a.ctiles == 0) {
@@ -239,69 +368,71 @@ __global__ void __launch_bounds__(kThreads) norm_grad_sums_kernel(NormArgs a, lo
       for (int r = 0; r < a.ty; ++r) total += rc[r];
       a.counts[p.sample * a.chunks + p.chunk] = total;
     }
+    __syncthreads();  // the partial results have been read
   }
 }
 
-// One warp per (sample, group): A / n and B / n.
-__global__ void norm_grad_merge_kernel(NormArgs a) {
-  const long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (w >= a.n * a.groups) return;
-  const long long sample = w / a.groups;
-  const int g = (int)(w % a.groups);
-  const float2* part = a.part + sample * a.chunks * a.channels + g * a.per_group;
-  const long long entries = (long long)a.chunks * a.per_group;
-  float n = 0.f, sa = 0.f, sb = 0.f;
-  for (long long i = lane; i < entries; i += 32) {
-    const int k = (int)(i / a.per_group), c = (int)(i % a.per_group);
-    const float wt = a.weight ? load_param(a.weight, a.param_dtype, g * a.per_group + c) : 1.f;
-    const float2 e = part[(long long)k * a.channels + c];
-    n += (float)a.counts[sample * a.chunks + k];
-    sa = fmaf(wt, e.x, sa);
-    sb = fmaf(wt, e.y, sb);
+// A / n and B / n of every (sample, group).
+__global__ void __launch_bounds__(kMergeThreads) norm_grad_merge_kernel(NormArgs a) {
+  __shared__ float red[kMergeThreads / 32];
+  for (long long w = blockIdx.x; w < a.n * a.groups; w += gridDim.x) {
+    const long long sample = w / a.groups;
+    const int g = (int)(w % a.groups);
+    const float2* part = a.part + sample * a.chunks * a.channels + g * a.per_group;
+    float n = 0.f, sa = 0.f, sb = 0.f;
+    each_partial(a, [&](int k, int c) {
+      const float wt = a.weight ? load_param(a.weight, a.param_dtype, g * a.per_group + c) : 1.f;
+      const float2 e = part[(long long)k * a.channels + c];
+      n += (float)a.counts[sample * a.chunks + k];
+      sa = fmaf(wt, e.x, sa);
+      sb = fmaf(wt, e.y, sb);
+    });
+    n = block_sum(n, red);
+    sa = block_sum(sa, red);
+    sb = block_sum(sb, red);
+    if (threadIdx.x == 0) a.ab[w] = n > 0.f ? make_float2(sa / n, sb / n) : make_float2(0.f, 0.f);
   }
-  n = warp_sum(n);
-  sa = warp_sum(sa);
-  sb = warp_sum(sb);
-  if (lane == 0) a.ab[w] = n > 0.f ? make_float2(sa / n, sb / n) : make_float2(0.f, 0.f);
 }
 
-template <class T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) norm_grad_apply_kernel(NormArgs a, long long items) {
-  const int row = threadIdx.x / a.tx;
+template <class T, int V, int ACT, bool MASK, bool ONE>
+__global__ void __launch_bounds__(kThreads, 3) norm_grad_apply_kernel(NormArgs a, long long items) {
+  constexpr int P = (V + 1) / 2;
+  extern __shared__ uint4 ring[];
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-    const Place p = place_of<V>(a, item);
+    // from the end: L2 still holds what the pass before read last
+    const Place p = place_of<V>(a, items - 1 - item);
     if (!p.active) continue;
-    ChannelValues<V> cv;
+    ChannelValues<V, ONE> cv;
     cv.load(a, p);
-    float ga[V], gb[V];
+    constexpr int Q = ONE ? 1 : P;
+    float2 ga[Q], gb[Q];  // -A / n, -B / n
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float2 e = a.ab[p.sample * a.groups + (p.ch + v) / a.per_group];
-      ga[v] = e.x;
-      gb[v] = e.y;
+    for (int i = 0; i < Q; ++i) {
+      const float2 e0 = a.ab[p.sample * a.groups + (p.ch + 2 * i) / a.per_group];
+      const float2 e1 = a.ab[p.sample * a.groups + (p.ch + (ONE ? 0 : 2 * i + (V > 1))) / a.per_group];
+      ga[i] = make_float2(-e0.x, -e1.x);
+      gb[i] = make_float2(-e0.y, -e1.y);
     }
     const T* x = static_cast<const T*>(a.x) + p.sample * a.x_sn + p.ch;
     const T* dy = static_cast<const T*>(a.dy) + p.sample * a.dy_sn + p.ch;
-    T* dx = static_cast<T*>(a.y) + p.sample * a.cells * a.channels + p.ch;
-    for (long long c = p.c0 + row; c < p.c1; c += a.ty) {
-      Vec<T, V> out;
-      if (kept(a, p, c)) {
-        const Vec<T, V> xv = *reinterpret_cast<const Vec<T, V>*>(x + c * a.x_sl);
-        const Vec<T, V> gv = *reinterpret_cast<const Vec<T, V>*>(dy + c * a.dy_sl);
+    T* dx = static_cast<T*>(a.y) + (p.sample * a.cells + p.c0) * a.channels + p.ch;
+    each_cell<T, V, 2, MASK>(
+        a, p, ring, x, a.x_sl, dy, a.dy_sl,
+        [&](int c, const Vec<T, V>& xv, const Vec<T, V>& gv) {
+          float2 f[P], g[P];
+          to_pairs<T, V>(xv, f);
+          to_pairs<T, V>(gv, g);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float h = (to_f32(xv.v[v]) - cv.mean[v]) * cv.rstd[v];
-          float unused;
-          const float dz = to_f32(gv.v[v]) * act_slope_f<ACT>(fmaf(h, cv.w[v], cv.b[v]), unused);
-          out.v[v] = from_f32<T>(cv.rstd[v] * (__fmul_rn(cv.w[v], dz) - fmaf(h, gb[v], ga[v])));
-        }
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) out.v[v] = from_f32<T>(0.f);
-      }
-      *reinterpret_cast<Vec<T, V>*>(dx + c * a.channels) = out;
-    }
+          for (int i = 0; i < P; ++i) {
+            const float2 h = mul2(add2(f[i], cv.away_of(i)), cv.rstd_of(i));
+            float2 unused;
+            const float2 dz = mul2(g[i], act_slope2<ACT>(fma2(h, cv.w[i], cv.b[i]), unused));
+            // rstd (w dz - (A + h B) / n), each product rounded: one value a group gives exactly 0
+            f[i] = mul2(add2(mul2(cv.w[i], dz), fma2(h, gb[ONE ? 0 : i], ga[ONE ? 0 : i])), cv.rstd_of(i));
+          }
+          *reinterpret_cast<Vec<T, V>*>(dx + (long long)c * a.channels) = from_pairs<T, V>(f);
+        },
+        [&](int c) { write_zeros<T, V>(dx + (long long)c * a.channels); });
   }
 }
 
@@ -384,7 +515,7 @@ struct Layout {
   size_t part, counts, ab, params, total;
 };
 Layout layout_of(const NcaNormDesc& d) {
-  const size_t chunks = std::max(worst_chunks(d), 16);  // the held backward has up to 16 slices
+  const size_t chunks = std::max(worst_chunks(d), 8);  // the held backward has up to 8 slices
   Layout l;
   l.part = 0;
   l.counts = l.part + align256((size_t)d.n * chunks * d.channels * sizeof(float2));
@@ -464,27 +595,51 @@ void param_grads(const float2* part, long long rows, int channels, void* dweight
   norm_param_store_kernel<<<(channels + 31) / 32, dim3(32, 16), 0, s>>>(params, splits, channels, dweight, dbias, param_dtype);
 }
 
-template <class T, int V, int ACT>
-int32_t forward(const NcaNormDesc& d, NormArgs a, cudaStream_t s) {
-  const long long items = plan(d, a, V);
-  const int threads = a.tx * a.ty;
-  const size_t smem = (size_t)a.ty * a.tx * V * sizeof(float2) + a.ty * sizeof(int);
-  norm_stats_kernel<T, V><<<grid_of(items), threads, smem, s>>>(a, items);
-  norm_stats_merge_kernel<<<(unsigned)((a.n * a.groups + 7) / 8), 256, 0, s>>>(a);
-  norm_apply_kernel<T, V, ACT><<<grid_of(items), threads, 0, s>>>(a, items);
+// Raises a kernel's shared-memory limit once a device, and launches it.
+constexpr int kMaxDevices = 64;
+int32_t launch(void (*kernel)(NormArgs, long long), std::atomic<uint64_t>& ready, const NormArgs& a, long long items,
+               size_t smem, cudaStream_t s) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
+  if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024) != cudaSuccess) {
+      const int32_t st = launch_status();
+      return st == NCA_OK ? NCA_ERR_CUDA : st;
+    }
+    ready.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  kernel<<<grid_of(items), a.tx * a.ty, smem, s>>>(a, items);
   return launch_status();
 }
+// Shared memory of a kernel that leaves partial results: the ring, or those where they are more.
+template <class T, int V>
+size_t sums_smem(const NormArgs& a, int tensors) {
+  return std::max(ring_bytes<T, V>(tensors), (size_t)a.ty * a.tx * V * sizeof(float2) + a.ty * sizeof(int));
+}
+#define NCA_TRY(call)              \
+  do {                             \
+    const int32_t st_ = (call);    \
+    if (st_ != NCA_OK) return st_; \
+  } while (0)
 
-template <class T, int V, int ACT>
+template <class T, int V, int ACT, bool MASK, bool ONE>
+int32_t forward(const NcaNormDesc& d, NormArgs a, cudaStream_t s) {
+  static std::atomic<uint64_t> ready[2];
+  const long long items = plan(d, a, V);
+  NCA_TRY(launch(norm_stats_kernel<T, V, MASK>, ready[0], a, items, sums_smem<T, V>(a, 1), s));
+  norm_stats_merge_kernel<<<grid_of(a.n * a.groups), kMergeThreads, 0, s>>>(a);
+  return launch(norm_apply_kernel<T, V, ACT, MASK, ONE>, ready[1], a, items, ring_bytes<T, V>(1), s);
+}
+
+template <class T, int V, int ACT, bool MASK, bool ONE>
 int32_t backward(const NcaNormDesc& d, NormArgs a, void* dweight, void* dbias, float2* params,
                  cudaStream_t s) {
+  static std::atomic<uint64_t> ready[2];
   const long long items = plan(d, a, V);
-  const int threads = a.tx * a.ty;
-  const size_t smem = (size_t)a.ty * a.tx * V * sizeof(float2) + a.ty * sizeof(int);
-  norm_grad_sums_kernel<T, V, ACT><<<grid_of(items), threads, smem, s>>>(a, items);
+  NCA_TRY(launch(norm_grad_sums_kernel<T, V, ACT, MASK, ONE>, ready[0], a, items, sums_smem<T, V>(a, 2), s));
   if (a.y) {
-    norm_grad_merge_kernel<<<(unsigned)((a.n * a.groups + 7) / 8), 256, 0, s>>>(a);
-    norm_grad_apply_kernel<T, V, ACT><<<grid_of(items), threads, 0, s>>>(a, items);
+    norm_grad_merge_kernel<<<grid_of(a.n * a.groups), kMergeThreads, 0, s>>>(a);
+    NCA_TRY(launch(norm_grad_apply_kernel<T, V, ACT, MASK, ONE>, ready[1], a, items, ring_bytes<T, V>(2), s));
   }
   if (dweight || dbias) param_grads(a.part, a.n * a.chunks, a.channels, dweight, dbias, a.param_dtype, params, s);
   return launch_status();
@@ -511,7 +666,13 @@ struct ForwardCall {
   const NormArgs& a;
   cudaStream_t s;
   template <class T, int V, int A>
-  int32_t operator()() const { return forward<T, V, A>(d, a, s); }
+  int32_t operator()() const { 
+    if constexpr (V * sizeof(T) == 16) {
+      if (a.per_group % V == 0)
+        return a.mask ? forward<T, V, A, true, true>(d, a, s) : forward<T, V, A, false, true>(d, a, s);
+    }
+    return a.mask ? forward<T, V, A, true, V == 1>(d, a, s) : forward<T, V, A, false, V == 1>(d, a, s);
+   }
 };
 struct BackwardCall {
   const NcaNormDesc& d;
@@ -520,7 +681,15 @@ struct BackwardCall {
   float2* params;
   cudaStream_t s;
   template <class T, int V, int A>
-  int32_t operator()() const { return backward<T, V, A>(d, a, dweight, dbias, params, s); }
+  int32_t operator()() const { 
+    if constexpr (V * sizeof(T) == 16) {
+      if (a.per_group % V == 0)
+        return a.mask ? backward<T, V, A, true, true>(d, a, dweight, dbias, params, s)
+                      : backward<T, V, A, false, true>(d, a, dweight, dbias, params, s);
+    }
+    return a.mask ? backward<T, V, A, true, V == 1>(d, a, dweight, dbias, params, s)
+                  : backward<T, V, A, false, V == 1>(d, a, dweight, dbias, params, s);
+   }
 };
 
 }  // namespace

@@ -4,6 +4,13 @@
 
 namespace nca {
 
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const uint32_t a = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(a), "l"(from), "n"(BYTES) : "memory");
+}
+
 struct NormArgs {
   long long n, cells;
   int channels, groups, per_group;
@@ -29,7 +36,7 @@ struct NormArgs {
 // Runs the forward or backward kernel that holds samples in shared memory, when it applies: returns
 // false when it does not.  `v` is the vector width that channels, strides and addresses allow.  The
 // backward writes (sum dz, sum dz h) of every sample and slice to a.part as [n][slices][channels].
-int norm_held_slices(const NormArgs& a, int dtype, int v);  // of the backward, at most 16
+int norm_held_slices(const NormArgs& a, int dtype, int v);  // of the backward, at most 8
 bool norm_held_applies(const NormArgs& a, int dtype, int v, bool backward);
 int32_t norm_held_forward(const NormArgs& a, int dtype, int act, int v, cudaStream_t s);
 int32_t norm_held_backward(const NormArgs& a, int dtype, int act, int v, cudaStream_t s);

@@ -10,6 +10,7 @@
 // The mathematics and the treatment of sums are those of norm.cu.  Bound by HBM; the copies of the
 // blocks that share a multiprocessor overlap with each other's arithmetic and writes.
 #pragma once
+#include <algorithm>
 #include <atomic>
 
 #include "norm.cuh"
@@ -18,7 +19,7 @@ namespace nca {
 namespace {
 
 constexpr int kMaxThreads = 512;
-constexpr int kMaxSlices = 16;
+constexpr int kMaxSlices = 8;
 constexpr int kMaxGroups = 64;  // of one block
 
 struct HeldArgs {
@@ -43,12 +44,6 @@ __device__ __forceinline__ void put_remote(const float4* p, uint32_t rank, float
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(r), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                : "memory");
-}
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const void* from) {
-  const uint32_t a = (uint32_t)__cvta_generic_to_shared(to);
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(a), "l"(from) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(a), "l"(from), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -83,17 +78,33 @@ __device__ __forceinline__ Work work_of(const HeldArgs& h) {
   w.on = w.row < h.a.ty && w.ch < h.a.channels;
   return w;
 }
+// The cells of a thread that the mask keeps, a bit for each of its places (32 at most).
+template <bool MASK>
+__device__ __forceinline__ uint32_t kept_of(const NormArgs& a, const Work& w) {
+  if (!w.on) return 0;
+  if constexpr (!MASK) return ~0u;
+  uint32_t bits = 0;
+  const uint8_t* m = a.mask + w.sample * a.m_sn + (w.c0 + w.row) * a.m_sl;
+  const long long step = a.ty * a.m_sl;
+  int i = 0;
+  for (int c = w.row; c < w.cells; c += 8 * a.ty, i += 8, m += 8 * step) {
+    uint8_t v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = c + u * a.ty < w.cells ? m[u * step] : 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) bits |= (uint32_t)(v[u] != 0) << (i + u);
+  }
+  return bits;
+}
 // Goes through the thread's cells: f(place in shared memory, cell of the slice) where the cell counts, g
 // where the mask leaves it out.
 template <bool MASK, class F, class G>
-__device__ __forceinline__ void each_cell(const NormArgs& a, const Work& w, F f, G g) {
+__device__ __forceinline__ void each_cell(const NormArgs& a, const Work& w, uint32_t bits, F f, G g) {
   int at = threadIdx.x;
-  const int first = w.on ? w.row : w.cells;
-  const uint8_t* m = MASK ? a.mask + w.sample * a.m_sn + (w.c0 + first) * a.m_sl : nullptr;
-  for (int c = first; c < w.cells; c += a.ty, at += blockDim.x) {
-    if (!MASK || *m != 0) f(at, c);
+  for (int c = w.on ? w.row : w.cells; c < w.cells; c += a.ty, at += blockDim.x) {
+    if (!MASK || (bits & 1)) f(at, c);
     else g(at, c);
-    if (MASK) m += a.ty * a.m_sl;
+    if (MASK) bits >>= 1;
   }
 }
 
@@ -113,42 +124,32 @@ HeldPlan plan_of(const NormArgs& a, int dtype, int width, bool backward) {
   if (v * size < 4) return p;  // an asynchronous copy moves 4 bytes at least
   p.v = v;
   const size_t tensors = backward ? 2 : 1;
-  // channels of a block: all of them, or as few groups as leave 64 adjacent bytes when a sample is large
-  const size_t sample = (size_t)a.cells * a.channels * size * tensors;
-  const size_t kFew = 72 * 1024, kTwo = 100 * 1024, kOne = 190 * 1024;
+  // channels of a block: all of them, or fewer whole groups (64 adjacent bytes at least) when a sample
+  // would need more than 8 blocks of 100 KB.  Beyond that the streaming kernels are faster: clusters of
+  // 16 blocks that fill a multiprocessor each read 16 x 16384 x 512 bf16 at half their rate.
+  const size_t kFew = 72 * 1024, kTwo = 100 * 1024;
+  const auto bytes_of = [&](int g) { return (size_t)a.cells * g * a.per_group * size * tensors; };
   int groups = a.groups;
-  const auto fits = [&](int g) { return (size_t)a.cells * g * a.per_group * size * tensors <= kMaxSlices * kOne; };
-  (void)sample;
-  while (!fits(groups) || groups > kMaxGroups || groups * a.per_group / v > kMaxThreads) {
+  while (bytes_of(groups) > kMaxSlices * kTwo || groups > kMaxGroups || groups * a.per_group / v > kMaxThreads) {
     int next = groups - 1;
     while (next > 0 && a.groups % next) --next;
-    if (next <= 0) return p;
-    groups = next;
-  }
-  if (groups < a.groups && groups * a.per_group * size < 32) return p;
-  // a large sample: fewer channels rather than the largest clusters
-  while (groups > 1 && (size_t)a.cells * groups * a.per_group * size * tensors > 8 * kTwo) {
-    int next = groups - 1;
-    while (next > 0 && a.groups % next) --next;
-    if (next <= 0 || next * a.per_group * size < 64) break;
+    if (next <= 0 || next * a.per_group * size < 64) return p;
     groups = next;
   }
   p.cb = groups * a.per_group;
   p.cblocks = a.groups / groups;
-  const size_t bytes = (size_t)a.cells * p.cb * size * tensors;
+  const size_t bytes = bytes_of(groups);
   long long slices = (long long)((bytes + kFew - 1) / kFew);
-  if (slices > 8) slices = (long long)((bytes + kTwo - 1) / kTwo);
-  if (slices > kMaxSlices) slices = (long long)((bytes + kOne - 1) / kOne);
-  if (slices > kMaxSlices) return p;
+  if (slices > kMaxSlices) slices = (long long)((bytes + kTwo - 1) / kTwo);
   // few samples: over more blocks, 8 KB each at least
-  while (slices < 8 && a.n * p.cblocks * slices < 148 && (long long)bytes / slices > 16384 && slices * 2 <= a.cells) slices *= 2;
-  if (slices > a.cells) slices = a.cells;
+  while (slices < kMaxSlices && a.n * p.cblocks * slices < 148 && (long long)bytes / slices > 16384) slices *= 2;
+  slices = std::min({slices, (long long)kMaxSlices, (long long)a.cells});
   p.slice_cells = (a.cells + slices - 1) / slices;
   p.slices = (int)((a.cells + p.slice_cells - 1) / p.slice_cells);
   p.tx = p.cb / v;
   const long long ty_max = kMaxThreads / p.tx;
   long long iters = (p.slice_cells + ty_max - 1) / ty_max;
-  if (iters < 8) iters = p.slice_cells < 8 ? p.slice_cells : 8;
+  if (iters < 12) iters = p.slice_cells < 12 ? p.slice_cells : 12;
   p.ty = (int)((p.slice_cells + iters - 1) / iters);
   p.iters = (int)((p.slice_cells + p.ty - 1) / p.ty);
   p.threads = (p.tx * p.ty + 31) / 32 * 32;
@@ -156,7 +157,7 @@ HeldPlan plan_of(const NormArgs& a, int dtype, int width, bool backward) {
   p.smem += (size_t)p.slices * groups * sizeof(float4) + (size_t)p.ty * sizeof(int);
   if (backward) p.smem += ((size_t)p.ty * p.tx * v + p.cb) * sizeof(float2);
   else p.smem += (size_t)p.threads * sizeof(float2);
-  p.ok = p.smem <= 208 * 1024 && a.n * p.cblocks * p.slices < (1ll << 31);
+  p.ok = p.smem <= 208 * 1024 && p.iters <= 32 && a.n * p.cblocks * p.slices < (1ll << 31);
   return p;
 }
 
@@ -167,8 +168,7 @@ int32_t launch(void (*kernel)(HeldArgs), std::atomic<uint64_t>& ready, const Nor
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
   if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024) != cudaSuccess ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024) != cudaSuccess) {
       const int32_t st = launch_status();
       return st == NCA_OK ? NCA_ERR_CUDA : st;
     }

@@ -24,11 +24,12 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(cons
   float2* chan = red + a.ty * a.tx * V;                             // [cb] totals of the block
   int* count = reinterpret_cast<int*>(chan + h.cb);                 // [ty] cells of a row of threads
   const Work w = work_of<V>(h);
+  const uint32_t kept = kept_of<MASK>(a, w);
   {
     const T* x = static_cast<const T*>(a.x) + w.sample * a.x_sn + w.ch + w.c0 * a.x_sl;
     const T* dy = static_cast<const T*>(a.dy) + w.sample * a.dy_sn + w.ch + w.c0 * a.dy_sl;
     each_cell<MASK>(
-        a, w,
+        a, w, kept,
         [&](int at, int c) {
           copy_async<sizeof(VecT)>(xs + at, x + c * a.x_sl);
           copy_async<sizeof(VecT)>(gs + at, dy + c * a.dy_sl);
@@ -52,7 +53,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(cons
   copy_wait();
   int cnt = 0;
   each_cell<MASK>(
-      a, w,
+      a, w, kept,
       [&](int at, int) {
         ++cnt;
         float2 f[P], g[P];
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(cons
   sb = n > 0.f ? sb / n : 0.f;
   T* dx = static_cast<T*>(a.y) + (w.sample * a.cells + w.c0) * a.channels + w.ch;
   each_cell<MASK>(
-      a, w,
+      a, w, kept,
       [&](int at, int c) {
         float2 f[P], g[P];
         to_pairs<T, V>(xs[at], f);

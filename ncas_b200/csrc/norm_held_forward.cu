@@ -11,6 +11,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_forward_kernel(const
   extern __shared__ uint4 smem_raw[];
   using VecT = Vec<T, V>;
   const Work w = work_of<V>(h);
+  const uint32_t kept = kept_of<MASK>(a, w);
   const int threads = blockDim.x, groups = h.cb / a.per_group;
   float4* all = reinterpret_cast<float4*>(smem_raw);            // [slices][groups] (n, mean, M2)
   VecT* xs = reinterpret_cast<VecT*>(all + h.slices * groups);  // [iters][threads]
@@ -18,7 +19,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_forward_kernel(const
   int* count = reinterpret_cast<int*>(part + threads);          // [ty] cells of a row of threads
   {
     const T* x = static_cast<const T*>(a.x) + w.sample * a.x_sn + w.ch + w.c0 * a.x_sl;
-    each_cell<MASK>(a, w, [&](int at, int c) { copy_async<sizeof(VecT)>(xs + at, x + c * a.x_sl); }, [](int, int) {});
+    each_cell<MASK>(a, w, kept, [&](int at, int c) { copy_async<sizeof(VecT)>(xs + at, x + c * a.x_sl); }, [](int, int) {});
   }
   float2 wt[P], b[P];
 #pragma unroll
@@ -33,7 +34,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_forward_kernel(const
     float2 s1 = both(0.f), s2 = both(0.f);
     int cnt = 0;
     each_cell<MASK>(
-        a, w,
+        a, w, kept,
         [&](int at, int) {
           float2 f[P];
           to_pairs<T, V>(xs[at], f);
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_forward_kernel(const
   for (int i = 0; i < P; ++i) wt[i] = mul2(wt[i], both(rstd));
   T* y = static_cast<T*>(a.y) + (w.sample * a.cells + w.c0) * a.channels + w.ch;
   each_cell<MASK>(
-      a, w,
+      a, w, kept,
       [&](int at, int c) {
         float2 f[P];
         to_pairs<T, V>(xs[at], f);
