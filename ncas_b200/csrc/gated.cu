@@ -102,40 +102,74 @@ __global__ void pack_kernel(const uint16_t* src, long long rows, long long cols,
 template <class T>
 __global__ void join_kernel(const float* part, int splits, int batch, long long m, long long n, long long ldp,
                             T* c0, T* c1) {
-  const long long total = batch * m * n;
+  const long long total = batch * m * ldp / 4, piece = batch * m * ldp;
   for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
        i += (long long)gridDim.x * blockDim.x) {
-    const long long z = i / (m * n), r = (i - z * m * n) / n, c = i - z * m * n - r * n;
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += part[((long long)(k * batch + z) * m + r) * ldp + c];
-    (z ? c1 : c0)[r * n + c] = from_f32<T>(s);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4* from = reinterpret_cast<const float4*>(part + 4 * i);
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) {
+      const float4 v = from[k * (piece / 4)];
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const long long zr = 4 * i / ldp, c = 4 * i - zr * ldp, z = zr / m, r = zr - z * m;
+    T* to = (z ? c1 : c0) + r * n + c;
+    const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < n) to[j] = from_f32<T>(f[j]);
   }
 }
 
-// Column sums of a [rows][cols] matrix in two steps of a fixed order.
+// Column sums of up to three [rows][cols] matrices (blockIdx.z) in two steps of a fixed order: the rows
+// of a piece by 8 lanes a column pair, then the pieces.  Pairs of columns: rows lie on 16-byte boundaries.
+struct ColumnSums {
+  const void* a[3];
+  long long cols[3], ld[3];
+  void* out[3];
+  float* part[3];  // [splits][cols]
+};
+constexpr int kSumSplits = 64;
 template <class T>
-__global__ void column_sums_kernel(const T* a, long long rows, long long cols, long long ld, int splits, float* part) {
-  __shared__ float red[8][33];
-  const long long c = (long long)blockIdx.x * 32 + threadIdx.x;
+__global__ void __launch_bounds__(256) column_sums_kernel(ColumnSums p, long long rows, int splits) {
+  __shared__ float2 red[8][33];
+  const int z = blockIdx.z;
+  const long long c = 2 * ((long long)blockIdx.x * 32 + threadIdx.x), cols = p.cols[z];
+  if (2ll * blockIdx.x * 32 >= cols) return;
   const long long per = (rows + splits - 1) / splits, r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
-  float s = 0.f;
-  if (c < cols)
-    for (long long r = r0 + threadIdx.y; r < r1; r += 8) s += to_f32(a[r * ld + c]);
+  float2 s = both(0.f);
+  if (c < cols) {
+    const T* from = static_cast<const T*>(p.a[z]) + c;
+#pragma unroll 8
+    for (long long r = r0 + threadIdx.y; r < r1; r += 8) {
+      float2 f[1];
+      to_pairs<T, 2>(*reinterpret_cast<const Vec<T, 2>*>(from + r * p.ld[z]), f);
+      s = add2(s, f[0]);
+    }
+  }
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y == 0 && c < cols) {
-    for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x];
-    part[(long long)blockIdx.y * cols + c] = s;
+    for (int i = 1; i < 8; ++i) s = add2(s, red[i][threadIdx.x]);
+    float* to = p.part[z] + (long long)blockIdx.y * cols + c;
+    to[0] = s.x;
+    if (c + 1 < cols) to[1] = s.y;
   }
 }
-__global__ void column_store_kernel(const float* part, int splits, long long cols, void* out, int dtype) {
-  const long long c = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= cols) return;
+__global__ void __launch_bounds__(256) column_store_kernel(ColumnSums p, int splits, int dtype) {
+  __shared__ float red[8][33];
+  const int z = blockIdx.z;
+  const long long c = (long long)blockIdx.x * 32 + threadIdx.x, cols = p.cols[z];
   float s = 0.f;
-  for (int k = 0; k < splits; ++k) s += part[(long long)k * cols + c];
-  store_param(out, dtype, c, s);
+  if (c < cols)
+#pragma unroll 8
+    for (int k = threadIdx.y; k < splits; k += 8) s += p.part[z][(long long)k * cols + c];
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y || c >= cols) return;
+  for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x];
+  store_param(p.out[z], dtype, c, s);
 }
-constexpr int kSumSplits = 64;
 
 // --------------------------------------------------------------------------------- the products
 template <class T, int CG, int BN, bool A_MN, bool B_MN, int EPI, int ACT>
@@ -241,7 +275,7 @@ int32_t weight_product(GemmParams& p, const Product& g, int dtype, void* c0, voi
   p.ldp = (g.n + 3) / 4 * 4;
   const int32_t st = product<T, true, true, EPI_PARTIAL, NCA_ACT_NONE>(p, g, dtype, sh, s);
   if (st != NCA_OK) return st;
-  const long long total = g.batch * g.m * g.n;
+  const long long total = g.batch * g.m * p.ldp / 4;
   join_kernel<T><<<(unsigned)std::min(ceil_div(total, 256), 4096ll), 256, 0, s>>>(
       part, sh.splits, g.batch, g.m, g.n, p.ldp, static_cast<T*>(c0), static_cast<T*>(c1));
   return launch_status();
@@ -309,7 +343,7 @@ Plan plan_of(const NcaGatedDesc& d, bool backward) {
                              weight_part_bytes(d.hidden, d.d_in, 1, d.rows),
                              weight_part_bytes(d.d_out, d.hidden, 1, d.rows)}));
     p.sums = at;
-    at += align256((size_t)kSumSplits * std::max(d.hidden, d.d_out) * sizeof(float));
+    at += align256((size_t)kSumSplits * (2 * d.hidden + d.d_out) * sizeof(float));
   }
   p.total = at + 256;
   return p;
@@ -373,16 +407,6 @@ int32_t forward(const NcaGatedDesc& d, const void* x, const void* w_gate, const 
       p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s);
 }
 
-template <class T>
-int32_t column_sums(const void* a, long long rows, long long cols, long long ld, float* part, void* out, int dtype,
-                    cudaStream_t s) {
-  const int splits = (int)std::max(1ll, std::min((long long)kSumSplits, rows / 32));
-  column_sums_kernel<T><<<dim3((unsigned)ceil_div(cols, 32), splits), dim3(32, 8), 0, s>>>(
-      static_cast<const T*>(a), rows, cols, ld, splits, part);
-  column_store_kernel<<<(unsigned)ceil_div(cols, 128), 128, 0, s>>>(part, splits, cols, out, dtype);
-  return launch_status();
-}
-
 template <class T, int ACT>
 int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const void* w_up, const void* w_down,
                  const void* saved, const void* dy, void* dx, void* dw_gate, void* dw_up, void* dw_down,
@@ -395,7 +419,7 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
   const Matrix mh{keep + 3 * tf, d.rows, d.hidden, pl.fp};
   const Matrix mdg{ws + pl.dgate, d.rows, d.hidden, pl.fp}, mdu{ws + pl.dup, d.rows, d.hidden, pl.fp};
   float* part = reinterpret_cast<float*>(ws + pl.part);
-  float* sums = reinterpret_cast<float*>(ws + pl.sums);
+  float* part_sums = reinterpret_cast<float*>(ws + pl.sums);
   if (dx || dw_gate || dw_up || db_gate || db_up) {
     NCA_TRY(matrix_of(pl.op[OP_WD], w_down, ws, s, &md));
     GemmParams p = base;
@@ -437,9 +461,30 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
     Product g{{mdy, mdy}, {mh, mh}, false, false, d.d_out, d.hidden, d.rows, false, 1};
     NCA_TRY(weight_product<T>(p, g, d.dtype, dw_down, dw_down, part, s));
   }
-  if (db_gate) NCA_TRY(column_sums<T>(mdg.p, d.rows, d.hidden, pl.fp, sums, db_gate, d.bias_dtype, s));
-  if (db_up) NCA_TRY(column_sums<T>(mdu.p, d.rows, d.hidden, pl.fp, sums, db_up, d.bias_dtype, s));
-  if (db_down) NCA_TRY(column_sums<T>(mdy.p, d.rows, d.d_out, mdy.ld, sums, db_down, d.bias_dtype, s));
+  ColumnSums sums{};
+  int count = 0;
+  long long widest = 0;
+  float* at = part_sums;
+  const int splits = (int)std::max<long long>(1, std::min<long long>(kSumSplits, d.rows / 64));
+  const auto add = [&](const Matrix& m, void* out) {
+    if (!out) return;
+    sums.a[count] = m.p;
+    sums.cols[count] = m.cols;
+    sums.ld[count] = m.ld;
+    sums.out[count] = out;
+    sums.part[count] = at;
+    at += (size_t)kSumSplits * m.cols;
+    widest = std::max(widest, m.cols);
+    ++count;
+  };
+  add(mdg, db_gate);
+  add(mdu, db_up);
+  add(mdy, db_down);
+  if (count) {
+    column_sums_kernel<T><<<dim3((unsigned)ceil_div(widest, 64), splits, count), dim3(32, 8), 0, s>>>(sums, d.rows, splits);
+    column_store_kernel<<<dim3((unsigned)ceil_div(widest, 32), 1, count), dim3(32, 8), 0, s>>>(sums, splits, d.bias_dtype);
+    return launch_status();
+  }
   return NCA_OK;
 }
 

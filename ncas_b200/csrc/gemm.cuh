@@ -6,8 +6,10 @@
 //
 // One persistent CTA (CG = 1) or CTA pair (CG = 2, cta_group::2: one 256-row tile over two
 // multiprocessors, each loading half of B) per multiprocessor.  Warp 0 loads tiles by TMA into a
-// ring of shared-memory stages, warp 1 issues the MMAs, warp 2 owns the tensor memory, warps 4-7
-// take finished accumulators out and apply the epilogue.  Two accumulators in tensor memory let
+// ring of shared-memory stages, warp 1 issues the MMAs, warp 2 owns the tensor memory, warps 4-11
+// take finished accumulators out and apply the epilogue (two warps a quarter of the lanes, in turn
+// over pieces of 32 columns).  They own rows of the accumulator, memory wants lines of columns: what
+// is stored and loaded passes through 2.5 KB of shared memory of the warp.  Two accumulators in tensor memory let
 // the epilogue of one tile run under the MMAs of the next.
 #pragma once
 #include <cuda.h>
@@ -45,7 +47,8 @@ struct GemmParams {
   unsigned long long timeout_ns;
 };
 
-constexpr int kGemmThreads = 256;
+constexpr int kGemmThreads = 384;
+constexpr int kEpilogueWarps = 8;
 constexpr int kBM = 128, kBK = 64;
 
 // ------------------------------------------------------------------------------- PTX wrappers
@@ -157,69 +160,101 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Stores n <= 32 adjacent values of one row (16 bytes at a time when the rows allow it).
-template <class T>
-__device__ __forceinline__ void store_row(T* dst, const float (&v)[32], int n, bool vec) {
-  if (vec) {
+// 32 rows of 64 bytes between a lane's row (registers) and lines of memory: the warp's staging place
+// has rows of 80 bytes, so that neither side meets a bank twice.
+constexpr int kStageRow = 80;
+struct Staging {
+  uint8_t* smem;  // [32][kStageRow]
+  int lane;
+  // Writes `bytes` of each of the first `rows` rows to to + row * ld (bytes).  vec: 16 bytes at a time
+  // (whole ones: the caller's rows are padded to that), else 2 at a time.
+  __device__ __forceinline__ void put(uint8_t* to, long long ld, int rows, int bytes, bool vec, const uint4 (&v)[4]) const {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8)
-      if (i < n)
-        *reinterpret_cast<uint4*>(dst + i) =
-            make_uint4(pack2<T>(v[i], v[i + 1]), pack2<T>(v[i + 2], v[i + 3]), pack2<T>(v[i + 4], v[i + 5]),
-                       pack2<T>(v[i + 6], v[i + 7]));
-  } else {
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(smem + lane * kStageRow + 16 * i) = v[i];
+    __syncwarp();
+    if (vec) {
+      const int piece = 16 * (lane & 3);
+      const uint8_t* from = smem + (lane >> 2) * kStageRow + piece;
+      to += (lane >> 2) * ld + piece;
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < n) dst[i] = from_f32<T>(v[i]);
+      for (int i = 0; i < 4; ++i)
+        if (8 * i + (lane >> 2) < rows && piece < bytes)
+          *reinterpret_cast<uint4*>(to + 8 * i * ld) = *reinterpret_cast<const uint4*>(from + 8 * i * kStageRow);
+    } else {
+      for (int r = 0; r < rows; ++r)
+        if (2 * lane < bytes)
+          *reinterpret_cast<uint16_t*>(to + r * ld + 2 * lane) = *reinterpret_cast<const uint16_t*>(smem + r * kStageRow + 2 * lane);
+    }
+    __syncwarp();
   }
+  // The loads of a `take` that comes later: this lane's pieces of the 32 rows.
+  static __device__ __forceinline__ void ask(const uint8_t* from, long long ld, int rows, int bytes, int lane, uint4 (&v)[4]) {
+    const int piece = 16 * (lane & 3);
+    from += (lane >> 2) * ld + piece;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = 8 * i + (lane >> 2) < rows && piece < bytes ? *reinterpret_cast<const uint4*>(from + 8 * i * ld)
+                                                         : make_uint4(0, 0, 0, 0);
+  }
+  // Turns them into the lane's row.
+  __device__ __forceinline__ void take(uint4 (&v)[4]) const {
+    uint8_t* at = smem + (lane >> 2) * kStageRow + 16 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(at + 8 * i * kStageRow) = v[i];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(smem + lane * kStageRow + 16 * i);
+    __syncwarp();
+  }
+};
+template <class T>
+__device__ __forceinline__ void pack_row(const float (&v)[32], uint4 (&q)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    q[i] = make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                      pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
 }
+
 // The pre-activations kept for the backward pass: the upper 24 bits of their fp32 values (relative
 // error below 2^-15, the full fp32 range).  In the matrix type, bf16 would put 2^-8 more noise into
 // every gradient, and fp16 would overflow where the fp32 sum does not; the third plane costs 2 of
 // 8 bytes.  Three planes of 16-bit values: gate bits 31-16, up bits 31-16, and bits 15-8 of both
 // (gate low byte, up high byte).
-struct SavedPlanes {
-  static __device__ __forceinline__ void store(uint16_t* at, long long plane, const float (&g)[32],
-                                               const float (&u)[32], int n) {
+__device__ __forceinline__ void split_planes(const float (&g)[32], const float (&u)[32], uint4 (&a)[4], uint4 (&b)[4],
+                                             uint4 (&c)[4]) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      uint32_t hg[4], hu[4], lo[4];
+  for (int i = 0; i < 4; ++i) {
+    uint32_t hg[4], hu[4], lo[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t g0 = __float_as_uint(g[i + 2 * j]), g1 = __float_as_uint(g[i + 2 * j + 1]);
-        const uint32_t u0 = __float_as_uint(u[i + 2 * j]), u1 = __float_as_uint(u[i + 2 * j + 1]);
-        hg[j] = __byte_perm(g0, g1, 0x7632);
-        hu[j] = __byte_perm(u0, u1, 0x7632);
-        lo[j] = __byte_perm(__byte_perm(g0, u0, 0x0051), __byte_perm(g1, u1, 0x0051), 0x5410);
-      }
-      if (i < n) {
-        *reinterpret_cast<uint4*>(at + i) = make_uint4(hg[0], hg[1], hg[2], hg[3]);
-        *reinterpret_cast<uint4*>(at + plane + i) = make_uint4(hu[0], hu[1], hu[2], hu[3]);
-        *reinterpret_cast<uint4*>(at + 2 * plane + i) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
+    for (int j = 0; j < 4; ++j) {
+      const int k = 8 * i + 2 * j;
+      const uint32_t g0 = __float_as_uint(g[k]), g1 = __float_as_uint(g[k + 1]);
+      const uint32_t u0 = __float_as_uint(u[k]), u1 = __float_as_uint(u[k + 1]);
+      hg[j] = __byte_perm(g0, g1, 0x7632);
+      hu[j] = __byte_perm(u0, u1, 0x7632);
+      lo[j] = __byte_perm(__byte_perm(g0, u0, 0x0051), __byte_perm(g1, u1, 0x0051), 0x5410);
+    }
+    a[i] = make_uint4(hg[0], hg[1], hg[2], hg[3]);
+    b[i] = make_uint4(hu[0], hu[1], hu[2], hu[3]);
+    c[i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+}
+__device__ __forceinline__ void join_planes(const uint4 (&a)[4], const uint4 (&b)[4], const uint4 (&c)[4], float (&g)[32],
+                                            float (&u)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t hg[4] = {a[i].x, a[i].y, a[i].z, a[i].w}, hu[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
+    const uint32_t lo[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = 8 * i + 2 * j;
+      g[k] = __uint_as_float((hg[j] << 16) | (lo[j] << 8 & 0xFF00u));
+      g[k + 1] = __uint_as_float((hg[j] & 0xFFFF0000u) | (lo[j] >> 8 & 0xFF00u));
+      u[k] = __uint_as_float((hu[j] << 16) | (lo[j] & 0xFF00u));
+      u[k + 1] = __uint_as_float((hu[j] & 0xFFFF0000u) | (lo[j] >> 16 & 0xFF00u));
     }
   }
-  static __device__ __forceinline__ void load(const uint16_t* at, long long plane, float (&g)[32], float (&u)[32],
-                                              int n) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      uint4 a = make_uint4(0, 0, 0, 0), b = a, c = a;
-      if (i < n) {
-        a = *reinterpret_cast<const uint4*>(at + i);
-        b = *reinterpret_cast<const uint4*>(at + plane + i);
-        c = *reinterpret_cast<const uint4*>(at + 2 * plane + i);
-      }
-      const uint32_t hg[4] = {a.x, a.y, a.z, a.w}, hu[4] = {b.x, b.y, b.z, b.w}, lo[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        g[i + 2 * j] = __uint_as_float((hg[j] << 16) | (lo[j] << 8 & 0xFF00u));
-        g[i + 2 * j + 1] = __uint_as_float((hg[j] & 0xFFFF0000u) | (lo[j] >> 8 & 0xFF00u));
-        u[i + 2 * j] = __uint_as_float((hu[j] << 16) | (lo[j] & 0xFF00u));
-        u[i + 2 * j + 1] = __uint_as_float((hu[j] & 0xFFFF0000u) | (lo[j] >> 16 & 0xFF00u));
-      }
-    }
-  }
-};
+}
 
 template <int CG, int BN>
 struct GemmShape {
@@ -228,7 +263,10 @@ struct GemmShape {
   static constexpr int kBBytes = kBNc * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kStages = (196 * 1024) / kStageBytes;
-  static constexpr int kSmem = kStages * kStageBytes + 1024 + 1024;  // alignment, barriers
+  static constexpr int kBars = kStages * kStageBytes;  // barriers, then biases, then the staging places
+  static constexpr int kBias = kBars + 256;
+  static constexpr int kStaging = kBias + 2 * 256 * (int)sizeof(float);
+  static constexpr int kSmem = kStaging + kEpilogueWarps * 32 * kStageRow + 1024;  // alignment
   static constexpr int kTmemCols = 2 * BN;
 };
 
@@ -263,7 +301,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   constexpr int kTN = EPI == EPI_GATE ? BN / 2 : BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStageBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
   uint64_t* empty = full + S::kStages;
   uint64_t* acc_full = empty + S::kStages;
   uint64_t* acc_empty = acc_full + 2;
@@ -282,7 +320,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 4 * CG);
+      mbar_init(&acc_empty[i], kEpilogueWarps * CG);
     }
     mbar_init(drained, 1);
     *abort_s = 0;
@@ -403,19 +441,39 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       }
     }
   } else if (warp >= 4) {
-    const int q = warp - 4;  // tensor memory lanes 32 q .. 32 q + 31
+    const int q = (warp - 4) & 3, turn = (warp - 4) >> 2;  // tensor memory lanes 32 q .. 32 q + 31
+    const Staging st{smem + S::kStaging + (warp - 4) * 32 * kStageRow, lane};
+    float* bias_s = reinterpret_cast<float*>(smem + S::kBias);  // [2][256]
+    const bool biased = (EPI == EPI_GATE || EPI == EPI_STORE) && (p.bias[0] || p.bias[1]);
     int buf = 0;
     uint32_t ph = 0;
     for (int t = first; t < tiles; t += step) {
       const GemmTile tl = tile_of<kBM * CG, kTN>(p, t);
+      const int row0 = tl.m0 + (int)rank * kBM + 32 * q, rows = min(32, p.m - row0);
+      const int cols = min(kTN, p.n - tl.n0);
+      if (biased) {  // the tile's biases, as floats
+        const int i = threadIdx.x - 128;
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the tile before has read its own
+        if (i < cols) {
+          bias_s[i] = p.bias[0] ? load_param(p.bias[0], p.bias_dtype, tl.n0 + i) : 0.f;
+          if (EPI == EPI_GATE) bias_s[256 + i] = p.bias[1] ? load_param(p.bias[1], p.bias_dtype, tl.n0 + i) : 0.f;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      uint4 k0[4], k1[4], k2[4];  // EPI_DGATE: the saved planes, asked for ahead of the accumulator
+      const auto ask = [&](int c) {
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(p.saved + (long long)row0 * p.ldc + tl.n0 + c);
+        const int bytes = 2 * min(32, cols - c);
+        Staging::ask(from, 2 * p.ldc, rows, bytes, lane, k0);
+        Staging::ask(from + 2 * p.plane, 2 * p.ldc, rows, bytes, lane, k1);
+        Staging::ask(from + 4 * p.plane, 2 * p.ldc, rows, bytes, lane, k2);
+      };
+      if (EPI == EPI_DGATE && 32 * turn < cols) ask(32 * turn);
       if (!mbar_wait(&acc_full[buf], ph, fs, 104)) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * BN + ((uint32_t)(32 * q) << 16);
-      const int row = tl.m0 + (int)rank * kBM + 32 * q + lane;
-      const bool live = row < p.m;
-      for (int c = 0; c < kTN; c += 32) {
-        const int col = tl.n0 + c;
-        const int n = min(32, p.n - col);
+      for (int c = 32 * turn; c < cols; c += 64) {
+        const int col = tl.n0 + c, n = min(32, cols - c);
         uint32_t r0[32];
         tmem_ld32(acc + c, r0);
         if constexpr (EPI == EPI_GATE) {
@@ -424,62 +482,82 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           tc_wait_ld_regs(r0);
 #pragma unroll
           for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r1[i]));
-          if (live && n > 0) {
-            float g[32], u[32], h[32];
+          float g[32], u[32], h[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            g[i] = __uint_as_float(r0[i]);
+            u[i] = __uint_as_float(r1[i]);
+          }
+          if (biased) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const int cc = min(col + i, p.n - 1);
-              g[i] = __uint_as_float(r0[i]) + (p.bias[0] ? load_param(p.bias[0], p.bias_dtype, cc) : 0.f);
-              u[i] = __uint_as_float(r1[i]) + (p.bias[1] ? load_param(p.bias[1], p.bias_dtype, cc) : 0.f);
+              g[i] += bias_s[c + i];
+              u[i] += bias_s[256 + c + i];
             }
+          }
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float2 a = mul2(act2<ACT>(make_float2(g[i], g[i + 1])), make_float2(u[i], u[i + 1]));
-              h[i] = a.x;
-              h[i + 1] = a.y;
-            }
-            const long long at = (long long)row * p.ldc + col;
-            store_row<T>(static_cast<T*>(p.c[0]) + at, h, n, true);
-            if (p.saved) SavedPlanes::store(p.saved + at, p.plane, g, u, n);
+          for (int i = 0; i < 32; i += 2) {
+            const float2 a = mul2(act2<ACT>(make_float2(g[i], g[i + 1])), make_float2(u[i], u[i + 1]));
+            h[i] = a.x;
+            h[i + 1] = a.y;
+          }
+          const long long at = (long long)row0 * p.ldc + col;
+          uint4 v[4];
+          pack_row<T>(h, v);
+          st.put(reinterpret_cast<uint8_t*>(static_cast<T*>(p.c[0]) + at), 2 * p.ldc, rows, 2 * n, true, v);
+          if (p.saved) {
+            uint4 v1[4], v2[4];
+            split_planes(g, u, v, v1, v2);
+            uint8_t* to = reinterpret_cast<uint8_t*>(p.saved + at);
+            st.put(to, 2 * p.ldc, rows, 2 * n, true, v);
+            st.put(to + 2 * p.plane, 2 * p.ldc, rows, 2 * n, true, v1);
+            st.put(to + 4 * p.plane, 2 * p.ldc, rows, 2 * n, true, v2);
           }
         } else if constexpr (EPI == EPI_DGATE) {
+          st.take(k0);
+          st.take(k1);
+          st.take(k2);
+          float g[32], u[32];
+          join_planes(k0, k1, k2, g, u);
+          if (c + 64 < cols) ask(c + 64);
           tc_wait_ld_regs(r0);
-          if (live && n > 0) {
-            const long long at = (long long)row * p.ldc + col;
-            float g[32], u[32];
-            SavedPlanes::load(p.saved + at, p.plane, g, u, n);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float2 dh = make_float2(__uint_as_float(r0[i]), __uint_as_float(r0[i + 1]));
-              float2 a;
-              const float2 slope = act_slope2<ACT>(make_float2(g[i], g[i + 1]), a);
-              const float2 dg = mul2(mul2(dh, make_float2(u[i], u[i + 1])), slope), du = mul2(dh, a);
-              g[i] = dg.x, g[i + 1] = dg.y;
-              u[i] = du.x, u[i + 1] = du.y;
-            }
-            store_row<T>(static_cast<T*>(p.c[0]) + at, g, n, true);
-            store_row<T>(static_cast<T*>(p.c[1]) + at, u, n, true);
+          for (int i = 0; i < 32; i += 2) {
+            const float2 dh = make_float2(__uint_as_float(r0[i]), __uint_as_float(r0[i + 1]));
+            float2 a;
+            const float2 slope = act_slope2<ACT>(make_float2(g[i], g[i + 1]), a);
+            const float2 dg = mul2(mul2(dh, make_float2(u[i], u[i + 1])), slope), du = mul2(dh, a);
+            g[i] = dg.x, g[i + 1] = dg.y;
+            u[i] = du.x, u[i + 1] = du.y;
           }
+          const long long at = (long long)row0 * p.ldc + col;
+          uint4 v[4];
+          pack_row<T>(g, v);
+          st.put(reinterpret_cast<uint8_t*>(static_cast<T*>(p.c[0]) + at), 2 * p.ldc, rows, 2 * n, true, v);
+          pack_row<T>(u, v);
+          st.put(reinterpret_cast<uint8_t*>(static_cast<T*>(p.c[1]) + at), 2 * p.ldc, rows, 2 * n, true, v);
         } else if constexpr (EPI == EPI_PARTIAL) {
           tc_wait_ld_regs(r0);
-          if (live && n > 0) {
-            float* dst = p.part + ((long long)(tl.split * p.batch + tl.batch) * p.m + row) * p.ldp + col;
+          uint8_t* to = reinterpret_cast<uint8_t*>(
+              p.part + ((long long)(tl.split * p.batch + tl.batch) * p.m + row0) * p.ldp + col);
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              if (i < n)
-                *reinterpret_cast<uint4*>(dst + i) = make_uint4(r0[i], r0[i + 1], r0[i + 2], r0[i + 3]);
+          for (int half = 0; half < 2; ++half) {
+            uint4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              v[i] = make_uint4(r0[16 * half + 4 * i], r0[16 * half + 4 * i + 1], r0[16 * half + 4 * i + 2],
+                                r0[16 * half + 4 * i + 3]);
+            st.put(to + 64 * half, 4 * p.ldp, rows, 4 * (n - 16 * half), true, v);
           }
         } else {
           tc_wait_ld_regs(r0);
-          if (live && n > 0) {
-            float v[32];
+          float f[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              v[i] = __uint_as_float(r0[i]);
-              if (p.bias[0]) v[i] += load_param(p.bias[0], p.bias_dtype, min(col + i, p.n - 1));
-            }
-            store_row<T>(static_cast<T*>(p.c[tl.batch]) + (long long)row * p.ldc + col, v, n, p.vec_c);
-          }
+          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r0[i]) + (biased ? bias_s[c + i] : 0.f);
+          uint4 v[4];
+          pack_row<T>(f, v);
+          st.put(reinterpret_cast<uint8_t*>(static_cast<T*>(p.c[tl.batch]) + (long long)row0 * p.ldc + col), 2 * p.ldc,
+                 rows, 2 * n, p.vec_c, v);
         }
       }
       tc_fence_before();
