@@ -78,6 +78,40 @@ bool encode(CUtensorMap* map, const Matrix& m, int dtype, int box_rows) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Boxes of 64 bytes x 32 rows, 64-byte swizzle, of `planes` matrices `plane` bytes apart: what the
+// epilogues store and load.
+bool encode_boxes(CUtensorMap* map, const void* p, CUtensorMapDataType type, int size, long long cols, long long rows,
+                  long long ld, int dims, long long planes, long long plane) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t d[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+  const cuuint64_t strides[2] = {(cuuint64_t)(ld * size), (cuuint64_t)plane};
+  const cuuint32_t box[3] = {(cuuint32_t)(64 / size), 32, 1};
+  const cuuint32_t one[3] = {1, 1, 1};
+  return fn(map, type, dims, const_cast<void*>(p), d, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+CUtensorMapDataType map_type(int dtype) {
+  return dtype == NCA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+// An output matrix of the matrix type with rows on 16-byte boundaries.
+bool encode_out(CUtensorMap* map, const void* p, int dtype, long long rows, long long cols, long long ld) {
+  return encode_boxes(map, p, map_type(dtype), 2, cols, rows, ld, 2, 1, 0);
+}
+// The three planes of the saved pre-activations.
+bool encode_planes(CUtensorMap* map, const void* p, long long rows, long long cols, long long ld, long long plane) {
+  return encode_boxes(map, p, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, cols, rows, ld, 3, 3, plane);
+}
+// The outputs of an EPI_STORE product (c[1] may repeat c[0]): by TMA where their rows allow it.
+bool set_out(GemmParams& p, int dtype, void* c0, void* c1, long long rows, long long cols) {
+  p.c[0] = c0;
+  p.c[1] = c1;
+  p.ldc = cols;
+  p.plain_c = cols % 8 != 0 || reinterpret_cast<uintptr_t>(c0) % 16 != 0 || reinterpret_cast<uintptr_t>(c1) % 16 != 0;
+  return p.plain_c || (encode_out(&p.out[0], c0, dtype, rows, cols, cols) && encode_out(&p.out[1], c1, dtype, rows, cols, cols));
+}
+
 // ------------------------------------------------------------------------------- small kernels
 // dst[r][c] = src[r * sr + c * sc]: an operand that TMA cannot read, copied to padded rows.  32 x 32
 // tiles through shared memory, read along whichever stride is 1.
@@ -98,83 +132,99 @@ __global__ void pack_kernel(const uint16_t* src, long long rows, long long cols,
   }
 }
 
-// c[z][m][n] = sum over the pieces of part[s * batch + z][m][n], in the order of s.
+// c[z][m][n] = sum over the pieces of part[s * batch + z][m][n]: 32 lanes of 4 columns by 8 groups of
+// pieces, which add up in the order of the groups.
 template <class T>
-__global__ void join_kernel(const float* part, int splits, int batch, long long m, long long n, long long ldp,
-                            T* c0, T* c1) {
-  const long long total = batch * m * ldp / 4, piece = batch * m * ldp;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (long long)gridDim.x * blockDim.x) {
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4* from = reinterpret_cast<const float4*>(part + 4 * i);
-#pragma unroll 8
-    for (int k = 0; k < splits; ++k) {
-      const float4 v = from[k * (piece / 4)];
+__global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int batch, long long m, long long n,
+                                                   long long ldp, T* c0, T* c1) {
+  __shared__ float4 red[8][32];
+  const long long total = batch * m * ldp / 4, i = (long long)blockIdx.x * 32 + threadIdx.x;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (i < total) {
+    const float4* from = reinterpret_cast<const float4*>(part) + i;
+#pragma unroll 4
+    for (int k = threadIdx.y; k < splits; k += 8) {
+      const float4 v = from[k * total];
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
-    const long long zr = 4 * i / ldp, c = 4 * i - zr * ldp, z = zr / m, r = zr - z * m;
-    T* to = (z ? c1 : c0) + r * n + c;
-    const float f[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + j < n) to[j] = from_f32<T>(f[j]);
   }
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y || i >= total) return;
+  for (int k = 1; k < 8; ++k) {
+    const float4 v = red[k][threadIdx.x];
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  const long long zr = 4 * i / ldp, c = 4 * i - zr * ldp, z = zr / m, r = zr - z * m;
+  T* to = (z ? c1 : c0) + r * n + c;
+  const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (c + j < n) to[j] = from_f32<T>(f[j]);
 }
 
 // Column sums of up to three [rows][cols] matrices (blockIdx.z) in two steps of a fixed order: the rows
-// of a piece by 8 lanes a column pair, then the pieces.  Pairs of columns: rows lie on 16-byte boundaries.
+// of a piece, 8 columns a lane (rows lie on 16-byte boundaries), then the pieces.
 struct ColumnSums {
   const void* a[3];
   long long cols[3], ld[3];
   void* out[3];
-  float* part[3];  // [splits][cols]
+  float* part[3];  // [splits][cols rounded up to 8]
 };
-constexpr int kSumSplits = 64;
+constexpr int kSumSplits = 256;
 template <class T>
 __global__ void __launch_bounds__(256) column_sums_kernel(ColumnSums p, long long rows, int splits) {
-  __shared__ float2 red[8][33];
+  __shared__ float2 red[8][32][4];
   const int z = blockIdx.z;
-  const long long c = 2 * ((long long)blockIdx.x * 32 + threadIdx.x), cols = p.cols[z];
-  if (2ll * blockIdx.x * 32 >= cols) return;
+  const long long c = 8 * ((long long)blockIdx.x * 32 + threadIdx.x), cols = p.cols[z], padded = (cols + 7) / 8 * 8;
+  if (256ll * blockIdx.x >= padded) return;
   const long long per = (rows + splits - 1) / splits, r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
-  float2 s = both(0.f);
-  if (c < cols) {
+  float2 s[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
+  if (c < padded) {
     const T* from = static_cast<const T*>(p.a[z]) + c;
-#pragma unroll 8
+#pragma unroll 4
     for (long long r = r0 + threadIdx.y; r < r1; r += 8) {
-      float2 f[1];
-      to_pairs<T, 2>(*reinterpret_cast<const Vec<T, 2>*>(from + r * p.ld[z]), f);
-      s = add2(s, f[0]);
+      Vec<T, 8> v;
+      if (c + 8 <= cols) {
+        v = *reinterpret_cast<const Vec<T, 8>*>(from + r * p.ld[z]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v.v[i] = c + i < cols ? from[r * p.ld[z] + i] : from_f32<T>(0.f);
+      }
+      float2 f[4];
+      to_pairs<T, 8>(v, f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = add2(s[i], f[i]);
     }
   }
-  red[threadIdx.y][threadIdx.x] = s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) red[threadIdx.y][threadIdx.x][i] = s[i];
   __syncthreads();
-  if (threadIdx.y == 0 && c < cols) {
-    for (int i = 1; i < 8; ++i) s = add2(s, red[i][threadIdx.x]);
-    float* to = p.part[z] + (long long)blockIdx.y * cols + c;
-    to[0] = s.x;
-    if (c + 1 < cols) to[1] = s.y;
+  if (threadIdx.y < 4 && c < padded) {
+    float2 t = red[0][threadIdx.x][threadIdx.y];
+    for (int i = 1; i < 8; ++i) t = add2(t, red[i][threadIdx.x][threadIdx.y]);
+    *reinterpret_cast<float2*>(p.part[z] + blockIdx.y * padded + c + 2 * threadIdx.y) = t;
   }
 }
-__global__ void __launch_bounds__(256) column_store_kernel(ColumnSums p, int splits, int dtype) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(512) column_store_kernel(ColumnSums p, int splits, int dtype) {
+  __shared__ float red[16][33];
   const int z = blockIdx.z;
-  const long long c = (long long)blockIdx.x * 32 + threadIdx.x, cols = p.cols[z];
+  const long long c = (long long)blockIdx.x * 32 + threadIdx.x, cols = p.cols[z], padded = (cols + 7) / 8 * 8;
   float s = 0.f;
   if (c < cols)
 #pragma unroll 8
-    for (int k = threadIdx.y; k < splits; k += 8) s += p.part[z][(long long)k * cols + c];
+    for (int k = threadIdx.y; k < splits; k += 16) s += p.part[z][k * padded + c];
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y || c >= cols) return;
-  for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x];
+  for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
   store_param(p.out[z], dtype, c, s);
 }
 
 // --------------------------------------------------------------------------------- the products
 template <class T, int CG, int BN, bool A_MN, bool B_MN, int EPI, int ACT>
 int32_t launch(GemmParams& p, cudaStream_t s) {
-  using S = GemmShape<CG, BN>;
+  using S = GemmShape<CG, BN, EPI>;
   constexpr int kTN = EPI == EPI_GATE ? BN / 2 : BN;
   auto* kernel = gemm_kernel<T, CG, BN, A_MN, B_MN, EPI, ACT>;
   static std::atomic<uint64_t> ready{0};  // a bit for each device whose shared-memory limit is set
@@ -266,18 +316,19 @@ int32_t product(GemmParams& p, const Product& g, int dtype, const Shape& sh, cud
 template <class T>
 int32_t weight_product(GemmParams& p, const Product& g, int dtype, void* c0, void* c1, float* part, cudaStream_t s) {
   const Shape sh = shape_of(g.m, g.n, g.batch, ceil_div(g.k, kBK), true, false);
-  p.c[0] = c0;
-  p.c[1] = c1;
-  p.ldc = g.n;
-  p.vec_c = g.n % 8 == 0 && reinterpret_cast<uintptr_t>(c0) % 16 == 0 && reinterpret_cast<uintptr_t>(c1) % 16 == 0;
-  if (sh.splits == 1) return product<T, true, true, EPI_STORE, NCA_ACT_NONE>(p, g, dtype, sh, s);
-  p.part = part;
-  p.ldp = (g.n + 3) / 4 * 4;
+  if (sh.splits == 1) {
+    if (!set_out(p, dtype, c0, c1, g.m, g.n)) return NCA_ERR_CUDA;
+    return product<T, true, true, EPI_STORE, NCA_ACT_NONE>(p, g, dtype, sh, s);
+  }
+  const long long ldp = (g.n + 3) / 4 * 4;
+  if (!encode_boxes(&p.out[0], part, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, g.n, g.m, ldp, 3, (long long)sh.splits * g.batch,
+                    g.m * ldp * 4))
+    return NCA_ERR_CUDA;
   const int32_t st = product<T, true, true, EPI_PARTIAL, NCA_ACT_NONE>(p, g, dtype, sh, s);
   if (st != NCA_OK) return st;
-  const long long total = g.batch * g.m * p.ldp / 4;
-  join_kernel<T><<<(unsigned)std::min(ceil_div(total, 256), 4096ll), 256, 0, s>>>(
-      part, sh.splits, g.batch, g.m, g.n, p.ldp, static_cast<T*>(c0), static_cast<T*>(c1));
+  const long long total = g.batch * g.m * ldp / 4;
+  join_kernel<T><<<(unsigned)ceil_div(total, 32), dim3(32, 8), 0, s>>>(
+      part, sh.splits, g.batch, g.m, g.n, ldp, static_cast<T*>(c0), static_cast<T*>(c1));
   return launch_status();
 }
 size_t weight_part_bytes(long long m, long long n, int batch, long long rows) {
@@ -343,7 +394,7 @@ Plan plan_of(const NcaGatedDesc& d, bool backward) {
                              weight_part_bytes(d.hidden, d.d_in, 1, d.rows),
                              weight_part_bytes(d.d_out, d.hidden, 1, d.rows)}));
     p.sums = at;
-    at += align256((size_t)kSumSplits * (2 * d.hidden + d.d_out) * sizeof(float));
+    at += align256((size_t)kSumSplits * (2 * p.fp + pad8(d.d_out)) * sizeof(float));
   }
   p.total = at + 256;
   return p;
@@ -387,21 +438,18 @@ int32_t forward(const NcaGatedDesc& d, const void* x, const void* w_gate, const 
   {
     GemmParams p = base;
     Product g{{mx, mx}, {mg, mu}, false, true, d.rows, d.hidden, d.d_in, false, 1};
-    p.c[0] = h;
-    p.ldc = pl.fp;
+    if (!encode_out(&p.out[0], h, d.dtype, d.rows, d.hidden, pl.fp)) return NCA_ERR_CUDA;
     p.bias[0] = b_gate;
     p.bias[1] = b_up;
-    p.saved = reinterpret_cast<uint16_t*>(keep);
-    p.plane = (long long)(tf / 2);
+    p.save = keep != nullptr;
+    if (keep && !encode_planes(&p.planes, keep, d.rows, d.hidden, pl.fp, (long long)tf)) return NCA_ERR_CUDA;
     NCA_TRY((product<T, false, false, EPI_GATE, ACT>(
         p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, true), s)));
   }
   GemmParams p = base;
   const Matrix mh{h, d.rows, d.hidden, pl.fp};
   Product g{{mh, mh}, {md, md}, false, false, d.rows, d.d_out, d.hidden, false, 1};
-  p.c[0] = y;
-  p.ldc = d.d_out;
-  p.vec_c = d.d_out % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  if (!set_out(p, d.dtype, y, y, d.rows, d.d_out)) return NCA_ERR_CUDA;
   p.bias[0] = b_down;
   return product<T, false, false, EPI_STORE, NCA_ACT_NONE>(
       p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s);
@@ -424,11 +472,10 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
     NCA_TRY(matrix_of(pl.op[OP_WD], w_down, ws, s, &md));
     GemmParams p = base;
     Product g{{mdy, mdy}, {md, md}, false, false, d.rows, d.hidden, d.d_out, false, 1};
-    p.c[0] = ws + pl.dgate;
-    p.c[1] = ws + pl.dup;
-    p.ldc = pl.fp;
-    p.saved = reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(keep));
-    p.plane = (long long)(tf / 2);
+    if (!encode_out(&p.out[0], ws + pl.dgate, d.dtype, d.rows, d.hidden, pl.fp) ||
+        !encode_out(&p.out[1], ws + pl.dup, d.dtype, d.rows, d.hidden, pl.fp) ||
+        !encode_planes(&p.planes, keep, d.rows, d.hidden, pl.fp, (long long)tf))
+      return NCA_ERR_CUDA;
     NCA_TRY((product<T, false, true, EPI_DGATE, ACT>(
         p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s)));
   }
@@ -437,9 +484,7 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
     NCA_TRY(matrix_of(pl.op[OP_WU], w_up, ws, s, &mu));
     GemmParams p = base;
     Product g{{mdg, mdu}, {mg, mu}, true, true, d.rows, d.d_in, d.hidden, true, 1};
-    p.c[0] = dx;
-    p.ldc = d.d_in;
-    p.vec_c = d.d_in % 8 == 0 && reinterpret_cast<uintptr_t>(dx) % 16 == 0;
+    if (!set_out(p, d.dtype, dx, dx, d.rows, d.d_in)) return NCA_ERR_CUDA;
     NCA_TRY((product<T, false, true, EPI_STORE, NCA_ACT_NONE>(
         p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s)));
   }
@@ -473,7 +518,7 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
     sums.ld[count] = m.ld;
     sums.out[count] = out;
     sums.part[count] = at;
-    at += (size_t)kSumSplits * m.cols;
+    at += (size_t)kSumSplits * pad8(m.cols);
     widest = std::max(widest, m.cols);
     ++count;
   };
@@ -481,8 +526,8 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
   add(mdu, db_up);
   add(mdy, db_down);
   if (count) {
-    column_sums_kernel<T><<<dim3((unsigned)ceil_div(widest, 64), splits, count), dim3(32, 8), 0, s>>>(sums, d.rows, splits);
-    column_store_kernel<<<dim3((unsigned)ceil_div(widest, 32), 1, count), dim3(32, 8), 0, s>>>(sums, splits, d.bias_dtype);
+    column_sums_kernel<T><<<dim3((unsigned)ceil_div(widest, 256), splits, count), dim3(32, 8), 0, s>>>(sums, d.rows, splits);
+    column_store_kernel<<<dim3((unsigned)ceil_div(widest, 32), 1, count), dim3(32, 16), 0, s>>>(sums, splits, d.bias_dtype);
     return launch_status();
   }
   return NCA_OK;

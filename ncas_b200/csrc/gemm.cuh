@@ -8,8 +8,9 @@
 // multiprocessors, each loading half of B) per multiprocessor.  Warp 0 loads tiles by TMA into a
 // ring of shared-memory stages, warp 1 issues the MMAs, warp 2 owns the tensor memory, warps 4-11
 // take finished accumulators out and apply the epilogue (two warps a quarter of the lanes, in turn
-// over pieces of 32 columns).  They own rows of the accumulator, memory wants lines of columns: what
-// is stored and loaded passes through 2.5 KB of shared memory of the warp.  Two accumulators in tensor memory let
+// over pieces of 32 columns).  What they store and load moves by TMA through 2 KB places of the warp's
+// own (32 rows of 64 bytes, swizzled so that lanes that write rows meet no bank twice): stores of 32
+// rows by lanes kept the load/store unit busy for 61% of the forward product of a cell model.  Two accumulators in tensor memory let
 // the epilogue of one tile run under the MMAs of the next.
 #pragma once
 #include <cuda.h>
@@ -28,6 +29,8 @@ enum GemmEpilogue {
 
 struct GemmParams {
   CUtensorMap a[2], b[2];
+  CUtensorMap out[2];  // c[0], c[1] (or, EPI_PARTIAL, the pieces) in boxes of 32 rows of 64 bytes
+  CUtensorMap planes;  // the saved pre-activations likewise
   int m, n;            // logical rows and columns of D (columns of one half for EPI_GATE)
   int m_tiles, n_tiles;
   int batch;           // independent products: a[z], c[z] (1 or 2)
@@ -36,13 +39,10 @@ struct GemmParams {
   int kb_second;       // first k block that reads a[1], b[1] (kb when there is one source)
   void* c[2];          // EPI_STORE: outputs; EPI_GATE: h, -; EPI_DGATE: dgate, dup
   long long ldc;
-  int vec_c;           // 16-byte stores allowed
+  int plain_c;         // EPI_STORE: rows of c on no 16-byte boundaries, stored by lanes
   const void* bias[2];
   int bias_dtype;
-  uint16_t* saved;     // pre-activations (SavedPlanes): EPI_GATE writes (may be null), EPI_DGATE reads
-  long long plane;     // distance of the three planes
-  float* part;         // [batch * splits][m][ldp]
-  long long ldp;
+  int save;            // EPI_GATE: write the planes
   int* ctrl;
   unsigned long long timeout_ns;
 };
@@ -65,8 +65,9 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+// Relaxed: hands over tensor memory, which the tcgen05 fences order.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
@@ -81,6 +82,30 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
         "l"(map), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
+// Stores of a 2 KB place of this CTA's shared memory; outside of the tensor nothing is written.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
+               "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+               "r"(src), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 template <int CG>
 __device__ __forceinline__ void tc_alloc(uint32_t* dst, uint32_t cols) {
   if constexpr (CG == 1) {
@@ -160,53 +185,34 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// 32 rows of 64 bytes between a lane's row (registers) and lines of memory: the warp's staging place
-// has rows of 80 bytes, so that neither side meets a bank twice.
-constexpr int kStageRow = 80;
-struct Staging {
-  uint8_t* smem;  // [32][kStageRow]
-  int lane;
-  // Writes `bytes` of each of the first `rows` rows to to + row * ld (bytes).  vec: 16 bytes at a time
-  // (whole ones: the caller's rows are padded to that), else 2 at a time.
-  __device__ __forceinline__ void put(uint8_t* to, long long ld, int rows, int bytes, bool vec, const uint4 (&v)[4]) const {
+// A place of 32 rows of 64 bytes, 16-byte pieces swizzled as TMA's 64-byte mode does it (piece j of row
+// r at j ^ (r / 2 % 4)): a lane's row, written or read.
+__device__ __forceinline__ void put_row(uint32_t place, int lane, const uint4 (&v)[4]) {
+  const uint32_t row = place + 64 * lane, x = 16 * ((lane >> 1) & 3);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(smem + lane * kStageRow + 16 * i) = v[i];
-    __syncwarp();
-    if (vec) {
-      const int piece = 16 * (lane & 3);
-      const uint8_t* from = smem + (lane >> 2) * kStageRow + piece;
-      to += (lane >> 2) * ld + piece;
+  for (int j = 0; j < 4; ++j)
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((16 * j) ^ x)), "r"(v[j].x), "r"(v[j].y),
+                 "r"(v[j].z), "r"(v[j].w)
+                 : "memory");
+}
+__device__ __forceinline__ void take_row(uint32_t place, int lane, uint4 (&v)[4]) {
+  const uint32_t row = place + 64 * lane, x = 16 * ((lane >> 1) & 3);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (8 * i + (lane >> 2) < rows && piece < bytes)
-          *reinterpret_cast<uint4*>(to + 8 * i * ld) = *reinterpret_cast<const uint4*>(from + 8 * i * kStageRow);
-    } else {
-      for (int r = 0; r < rows; ++r)
-        if (2 * lane < bytes)
-          *reinterpret_cast<uint16_t*>(to + r * ld + 2 * lane) = *reinterpret_cast<const uint16_t*>(smem + r * kStageRow + 2 * lane);
-    }
-    __syncwarp();
+  for (int j = 0; j < 4; ++j)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[j].x), "=r"(v[j].y), "=r"(v[j].z), "=r"(v[j].w)
+                 : "r"(row + ((16 * j) ^ x))
+                 : "memory");
+}
+// The first `rows` rows of a place to 16-bit rows that lie on no 16-byte boundaries, `cols` values each.
+__device__ __forceinline__ void store_plain(uint32_t place, int lane, uint16_t* to, long long ld, int rows, int cols) {
+  for (int r = 0; r < rows; ++r) {
+    const uint32_t at = place + 64 * r + ((16 * (lane >> 3)) ^ (16 * ((r >> 1) & 3))) + 2 * (lane & 7);
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+    if (lane < cols) to[r * ld + lane] = v;
   }
-  // The loads of a `take` that comes later: this lane's pieces of the 32 rows.
-  static __device__ __forceinline__ void ask(const uint8_t* from, long long ld, int rows, int bytes, int lane, uint4 (&v)[4]) {
-    const int piece = 16 * (lane & 3);
-    from += (lane >> 2) * ld + piece;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = 8 * i + (lane >> 2) < rows && piece < bytes ? *reinterpret_cast<const uint4*>(from + 8 * i * ld)
-                                                         : make_uint4(0, 0, 0, 0);
-  }
-  // Turns them into the lane's row.
-  __device__ __forceinline__ void take(uint4 (&v)[4]) const {
-    uint8_t* at = smem + (lane >> 2) * kStageRow + 16 * (lane & 3);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(at + 8 * i * kStageRow) = v[i];
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(smem + lane * kStageRow + 16 * i);
-    __syncwarp();
-  }
-};
+}
 template <class T>
 __device__ __forceinline__ void pack_row(const float (&v)[32], uint4 (&q)[4]) {
 #pragma unroll
@@ -256,17 +262,25 @@ __device__ __forceinline__ void join_planes(const uint4 (&a)[4], const uint4 (&b
   }
 }
 
-template <int CG, int BN>
+constexpr int kPlace = 2048;
+
+// Shared memory: the ring, the epilogue's places, biases, barriers.
+template <int CG, int BN, int EPI>
 struct GemmShape {
   static constexpr int kBNc = BN / CG;  // rows of B in one CTA
   static constexpr int kABytes = kBM * kBK * 2;
   static constexpr int kBBytes = kBNc * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = (196 * 1024) / kStageBytes;
-  static constexpr int kBars = kStages * kStageBytes;  // barriers, then biases, then the staging places
-  static constexpr int kBias = kBars + 256;
-  static constexpr int kStaging = kBias + 2 * 256 * (int)sizeof(float);
-  static constexpr int kSmem = kStaging + kEpilogueWarps * 32 * kStageRow + 1024;  // alignment
+  // places of an epilogue warp: h and the three planes; dgate, dup and the planes; else two in turn
+  static constexpr int kPlaces = EPI == EPI_GATE ? 4 : EPI == EPI_DGATE ? 5 : 2;
+  static constexpr int kPlaceBytes = kEpilogueWarps * kPlaces * kPlace;
+  static constexpr int kRest = 2 * 256 * (int)sizeof(float) + 512;
+  static constexpr int kMost = (227 * 1024 - 1024 - kPlaceBytes - kRest) / kStageBytes;
+  static constexpr int kStages = kMost > 6 ? 6 : kMost;
+  static constexpr int kPlacesAt = kStages * kStageBytes;
+  static constexpr int kBias = kPlacesAt + kPlaceBytes;
+  static constexpr int kBars = kBias + 2 * 256 * (int)sizeof(float);
+  static constexpr int kSmem = kBars + 512 + 1024;  // 1024: alignment
   static constexpr int kTmemCols = 2 * BN;
 };
 
@@ -297,7 +311,7 @@ __device__ __forceinline__ GemmTile tile_of(const GemmParams& p, int t) {
 
 template <class T, int CG, int BN, bool A_MN, bool B_MN, int EPI, int ACT>
 __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_constant__ GemmParams p) {
-  using S = GemmShape<CG, BN>;
+  using S = GemmShape<CG, BN, EPI>;
   constexpr int kTN = EPI == EPI_GATE ? BN / 2 : BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -306,7 +320,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
   uint64_t* acc_full = empty + S::kStages;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* drained = acc_empty + 2;
-  uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(drained + 1);
+  uint64_t* loaded = drained + 1;  // EPI_DGATE: the planes of each epilogue warp
+  uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(loaded + kEpilogueWarps);
   volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_base_s + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -323,6 +338,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       mbar_init(&acc_empty[i], kEpilogueWarps * CG);
     }
     mbar_init(drained, 1);
+    for (int i = 0; i < kEpilogueWarps; ++i) mbar_init(&loaded[i], 1);
     *abort_s = 0;
     fence_mbar_init();
   }
@@ -442,7 +458,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     }
   } else if (warp >= 4) {
     const int q = (warp - 4) & 3, turn = (warp - 4) >> 2;  // tensor memory lanes 32 q .. 32 q + 31
-    const Staging st{smem + S::kStaging + (warp - 4) * 32 * kStageRow, lane};
+    const uint32_t place = smem_u32(smem + S::kPlacesAt) + (warp - 4) * S::kPlaces * kPlace;
+    uint32_t load_ph = 0;
+    int flip = 0;
+    bool ok = true, pending = false;  // pending: planes asked for and not yet waited for
     float* bias_s = reinterpret_cast<float*>(smem + S::kBias);  // [2][256]
     const bool biased = (EPI == EPI_GATE || EPI == EPI_STORE) && (p.bias[0] || p.bias[1]);
     int buf = 0;
@@ -460,15 +479,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
-      uint4 k0[4], k1[4], k2[4];  // EPI_DGATE: the saved planes, asked for ahead of the accumulator
+      // EPI_DGATE: the saved planes of the piece at column c, asked for ahead of their use
       const auto ask = [&](int c) {
-        const uint8_t* from = reinterpret_cast<const uint8_t*>(p.saved + (long long)row0 * p.ldc + tl.n0 + c);
-        const int bytes = 2 * min(32, cols - c);
-        Staging::ask(from, 2 * p.ldc, rows, bytes, lane, k0);
-        Staging::ask(from + 2 * p.plane, 2 * p.ldc, rows, bytes, lane, k1);
-        Staging::ask(from + 4 * p.plane, 2 * p.ldc, rows, bytes, lane, k2);
+        pending = true;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&loaded[warp - 4], 3 * kPlace);
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            tma_load_3d(place + (2 + i) * kPlace, &p.planes, smem_u32(&loaded[warp - 4]), tl.n0 + c, row0, i);
+        }
       };
-      if (EPI == EPI_DGATE && 32 * turn < cols) ask(32 * turn);
+      if (EPI == EPI_DGATE && rows > 0 && 32 * turn < cols) ask(32 * turn);
       if (!mbar_wait(&acc_full[buf], ph, fs, 104)) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * BN + ((uint32_t)(32 * q) << 16);
@@ -501,25 +522,45 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             h[i] = a.x;
             h[i + 1] = a.y;
           }
-          const long long at = (long long)row0 * p.ldc + col;
-          uint4 v[4];
+          uint4 v[4], v1[4], v2[4];
+          if (lane == 0) bulk_wait_read<0>();  // the places have been read
+          __syncwarp();
           pack_row<T>(h, v);
-          st.put(reinterpret_cast<uint8_t*>(static_cast<T*>(p.c[0]) + at), 2 * p.ldc, rows, 2 * n, true, v);
-          if (p.saved) {
-            uint4 v1[4], v2[4];
+          put_row(place, lane, v);
+          if (p.save) {
             split_planes(g, u, v, v1, v2);
-            uint8_t* to = reinterpret_cast<uint8_t*>(p.saved + at);
-            st.put(to, 2 * p.ldc, rows, 2 * n, true, v);
-            st.put(to + 2 * p.plane, 2 * p.ldc, rows, 2 * n, true, v1);
-            st.put(to + 4 * p.plane, 2 * p.ldc, rows, 2 * n, true, v2);
+            put_row(place + kPlace, lane, v);
+            put_row(place + 2 * kPlace, lane, v1);
+            put_row(place + 3 * kPlace, lane, v2);
+          }
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0 && rows > 0) {
+            tma_store_2d(&p.out[0], place, col, row0);
+            if (p.save) {
+#pragma unroll
+              for (int i = 0; i < 3; ++i) tma_store_3d(&p.planes, place + (1 + i) * kPlace, col, row0, i);
+            }
+            bulk_commit();
           }
         } else if constexpr (EPI == EPI_DGATE) {
-          st.take(k0);
-          st.take(k1);
-          st.take(k2);
           float g[32], u[32];
-          join_planes(k0, k1, k2, g, u);
-          if (c + 64 < cols) ask(c + 64);
+          if (rows > 0) {
+            if (!mbar_wait(&loaded[warp - 4], load_ph, fs, 105)) {
+              ok = false;
+              break;
+            }
+            load_ph ^= 1;
+            pending = false;
+            uint4 k0[4], k1[4], k2[4];
+            take_row(place + 2 * kPlace, lane, k0);
+            take_row(place + 3 * kPlace, lane, k1);
+            take_row(place + 4 * kPlace, lane, k2);
+            __syncwarp();
+            if (c + 64 < cols) ask(c + 64);
+            join_planes(k0, k1, k2, g, u);
+          }
+          if (lane == 0) bulk_wait_read<0>();  // the places have been read
           tc_wait_ld_regs(r0);
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
@@ -530,16 +571,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             g[i] = dg.x, g[i + 1] = dg.y;
             u[i] = du.x, u[i + 1] = du.y;
           }
-          const long long at = (long long)row0 * p.ldc + col;
           uint4 v[4];
+          __syncwarp();
           pack_row<T>(g, v);
-          st.put(reinterpret_cast<uint8_t*>(static_cast<T*>(p.c[0]) + at), 2 * p.ldc, rows, 2 * n, true, v);
+          put_row(place, lane, v);
           pack_row<T>(u, v);
-          st.put(reinterpret_cast<uint8_t*>(static_cast<T*>(p.c[1]) + at), 2 * p.ldc, rows, 2 * n, true, v);
+          put_row(place + kPlace, lane, v);
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0 && rows > 0) {
+            tma_store_2d(&p.out[0], place, col, row0);
+            tma_store_2d(&p.out[1], place + kPlace, col, row0);
+            bulk_commit();
+          }
         } else if constexpr (EPI == EPI_PARTIAL) {
           tc_wait_ld_regs(r0);
-          uint8_t* to = reinterpret_cast<uint8_t*>(
-              p.part + ((long long)(tl.split * p.batch + tl.batch) * p.m + row0) * p.ldp + col);
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             uint4 v[4];
@@ -547,28 +595,59 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             for (int i = 0; i < 4; ++i)
               v[i] = make_uint4(r0[16 * half + 4 * i], r0[16 * half + 4 * i + 1], r0[16 * half + 4 * i + 2],
                                 r0[16 * half + 4 * i + 3]);
-            st.put(to + 64 * half, 4 * p.ldp, rows, 4 * (n - 16 * half), true, v);
+            put_row(place + half * kPlace, lane, v);
+          }
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0 && rows > 0) {
+            const int z = tl.split * p.batch + tl.batch;
+            tma_store_3d(&p.out[0], place, col, row0, z);
+            if (n > 16) tma_store_3d(&p.out[0], place + kPlace, col + 16, row0, z);
+            bulk_commit();
           }
         } else {
           tc_wait_ld_regs(r0);
           float f[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r0[i]) + (biased ? bias_s[c + i] : 0.f);
+          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r0[i]);
+          if (biased) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] += bias_s[c + i];
+          }
           uint4 v[4];
           pack_row<T>(f, v);
-          st.put(reinterpret_cast<uint8_t*>(static_cast<T*>(p.c[tl.batch]) + (long long)row0 * p.ldc + col), 2 * p.ldc,
-                 rows, 2 * n, p.vec_c, v);
+          const uint32_t here = place + flip * kPlace;
+          flip ^= 1;
+          if (lane == 0) bulk_wait_read<1>();  // the store before the last has read this place
+          __syncwarp();
+          put_row(here, lane, v);
+          if (p.plain_c) {
+            __syncwarp();
+            store_plain(here, lane, static_cast<uint16_t*>(p.c[tl.batch]) + (long long)row0 * p.ldc + col, p.ldc, rows, n);
+          } else {
+            fence_async_proxy();
+            __syncwarp();
+            if (lane == 0 && rows > 0) {
+              tma_store_2d(&p.out[tl.batch], here, col, row0);
+              bulk_commit();
+            }
+          }
         }
       }
+      if (!ok) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[buf]), 0));
-        else mbar_arrive(&acc_empty[buf]);
+        if constexpr (CG == 2) mbar_arrive_cluster_relaxed(map_to_rank(smem_u32(&acc_empty[buf]), 0));
+        else mbar_arrive_relaxed(&acc_empty[buf]);
       }
       buf ^= 1;
       if (buf == 0) ph ^= 1;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the stores are done
+    if (pending)  // after a wait that ran out: the load in flight lands before this CTA leaves (bounded)
+      for (int tries = 0; tries < 64 && !mbar_try_wait(&loaded[warp - 4], load_ph); ++tries) {
+      }
   }
   __syncwarp();
   tc_fence_before();
