@@ -13,14 +13,22 @@
 //
 // The products over T rows have small outputs and a long k axis in a cell model: the axis is then
 // cut into pieces whose fp32 sums are added in a fixed order by a second kernel.
-#include "gemm.cuh"
+#include "gemm_rows.cuh"
 
 #include <algorithm>
+#include <cstdio>
+#include <cstdlib>
 #include <atomic>
 
 using namespace nca;
 
 namespace {
+
+#define NCA_TRY(call)                    \
+  do {                                   \
+    const int32_t st_ = (call);          \
+    if (st_ != NCA_OK) return st_;       \
+  } while (0)
 
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
@@ -113,22 +121,65 @@ bool set_out(GemmParams& p, int dtype, void* c0, void* c1, long long rows, long 
 }
 
 // ------------------------------------------------------------------------------- small kernels
-// dst[r][c] = src[r * sr + c * sc]: an operand that TMA cannot read, copied to padded rows.  32 x 32
-// tiles through shared memory, read along whichever stride is 1.
-__global__ void pack_kernel(const uint16_t* src, long long rows, long long cols, long long sr, long long sc,
-                            uint16_t* dst, long long ld) {
+// dst[r][c] = src[r * sr + c * sc]: operands that TMA cannot read, copied to padded rows, all of a call in
+// one launch (blockIdx.y).
+struct Pack {
+  const uint16_t* src;
+  uint16_t* dst;
+  long long rows, cols, sr, sc, ld;
+};
+struct Packs {
+  Pack p[5];
+};
+// 16 bytes of a row that starts 2 m bytes after a 16-byte boundary, from the two aligned pieces that hold them.
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int m) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t v[5];
+#pragma unroll
+  for (int i = 0; i < 5; ++i)
+    v[i] = m < 2 ? w[i] : m < 4 ? w[i + 1] : m < 6 ? w[i + 2] : w[min(i + 3, 7)];
+  const int bits = 16 * (m & 1);
+  return make_uint4(__funnelshift_r(v[0], v[1], bits), __funnelshift_r(v[1], v[2], bits),
+                    __funnelshift_r(v[2], v[3], bits), __funnelshift_r(v[3], v[4], bits));
+}
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs all) {
   __shared__ uint16_t tile[32][34];
-  const long long ct = (cols + 31) / 32, tiles = ct * ((rows + 31) / 32);
+  const Pack& p = all.p[blockIdx.y];
+  if (p.sc == 1) {  // rows of adjacent values: 8 a lane
+    const long long vecs = p.ld / 8, total = p.rows * vecs;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.y * 32 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+      const long long r = i / vecs, c = (i - r * vecs) * 8;
+      const uint16_t* from = p.src + r * p.sr + c;
+      const int m = (int)(reinterpret_cast<uintptr_t>(from) & 15) / 2;
+      uint4 out;
+      if (c >= 8 && c + 16 <= p.cols) {  // both aligned pieces lie inside the row
+        const uint4* q = reinterpret_cast<const uint4*>(from - m);
+        out = shifted(q[0], q[1], m);
+      } else {
+        uint32_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t lo = c + 2 * j < p.cols ? from[2 * j] : 0, hi = c + 2 * j + 1 < p.cols ? from[2 * j + 1] : 0;
+          v[j] = lo | hi << 16;
+        }
+        out = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+      *reinterpret_cast<uint4*>(p.dst + r * p.ld + c) = out;
+    }
+    return;
+  }
+  // any strides: 32 x 32 tiles through shared memory, read along whichever stride is 1
+  const long long ct = (p.cols + 31) / 32, tiles = ct * ((p.rows + 31) / 32);
   for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
     const long long r0 = t / ct * 32, c0 = t % ct * 32;
     __syncthreads();
     for (int i = threadIdx.y; i < 32; i += 8) {
-      const int r = sr == 1 ? threadIdx.x : i, c = sr == 1 ? i : threadIdx.x;
-      if (r0 + r < rows && c0 + c < cols) tile[r][c] = src[(r0 + r) * sr + (c0 + c) * sc];
+      const int r = p.sr == 1 ? threadIdx.x : i, c = p.sr == 1 ? i : threadIdx.x;
+      if (r0 + r < p.rows && c0 + c < p.cols) tile[r][c] = p.src[(r0 + r) * p.sr + (c0 + c) * p.sc];
     }
     __syncthreads();
     for (int i = threadIdx.y; i < 32; i += 8)
-      if (r0 + i < rows && c0 + threadIdx.x < cols) dst[(r0 + i) * ld + c0 + threadIdx.x] = tile[i][threadIdx.x];
+      if (r0 + i < p.rows && c0 + threadIdx.x < p.cols) p.dst[(r0 + i) * p.ld + c0 + threadIdx.x] = tile[i][threadIdx.x];
   }
 }
 
@@ -182,19 +233,22 @@ __global__ void __launch_bounds__(256) column_sums_kernel(ColumnSums p, long lon
   float2 s[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
   if (c < padded) {
     const T* from = static_cast<const T*>(p.a[z]) + c;
-#pragma unroll 4
-    for (long long r = r0 + threadIdx.y; r < r1; r += 8) {
-      Vec<T, 8> v;
-      if (c + 8 <= cols) {
-        v = *reinterpret_cast<const Vec<T, 8>*>(from + r * p.ld[z]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v.v[i] = c + i < cols ? from[r * p.ld[z] + i] : from_f32<T>(0.f);
-      }
+    const auto add = [&](const Vec<T, 8>& v) {
       float2 f[4];
       to_pairs<T, 8>(v, f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[i] = add2(s[i], f[i]);
+    };
+    if (c + 8 <= cols) {
+#pragma unroll 8
+      for (long long r = r0 + threadIdx.y; r < r1; r += 8) add(*reinterpret_cast<const Vec<T, 8>*>(from + r * p.ld[z]));
+    } else {
+      for (long long r = r0 + threadIdx.y; r < r1; r += 8) {
+        Vec<T, 8> v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v.v[i] = c + i < cols ? from[r * p.ld[z] + i] : from_f32<T>(0.f);
+        add(v);
+      }
     }
   }
 #pragma unroll
@@ -261,21 +315,26 @@ int32_t launch(GemmParams& p, cudaStream_t s) {
 // Pairs of multiprocessors (256 x 256 tiles) when their tiles occupy the GPU, single ones
 // (128 x 128 tiles) otherwise.
 struct Shape {
-  bool pair;
+  int cg, bn;
   int splits;
 };
 Shape shape_of(long long m, long long n, int batch, long long kb, bool may_split, bool gate) {
+  if (getenv("GS")) {
+    int c = 2, w = 256, sp = 1;
+    sscanf(getenv("GS"), "%d,%d,%d", &c, &w, &sp);
+    return {c, w, may_split ? sp : 1};
+  }
   const long long sms = sm_count();
   const long long big = ceil_div(m, 256) * ceil_div(n, gate ? 128 : 256) * batch;
-  if (big >= sms / 2) return {true, 1};
+  if (big >= sms / 2) return {2, 256, 1};
   if (may_split && kb >= 64 && big * kb >= sms / 2 * 16) {
     const long long s = std::max(1ll, std::min(sms / 2 / big, kb / 16));
-    return {true, (int)s};
+    return {2, 256, (int)s};
   }
   const long long small = ceil_div(m, 128) * ceil_div(n, gate ? 64 : 128) * batch;
   long long s = 1;
   if (may_split) s = std::max(1ll, std::min(sms / small, kb / 8));
-  return {false, (int)s};
+  return {1, 128, (int)s};
 }
 
 struct Product {
@@ -306,10 +365,11 @@ int32_t set_up(GemmParams& p, const Product& g, int dtype, bool a_mn, bool b_mn,
 
 template <class T, bool A_MN, bool B_MN, int EPI, int ACT>
 int32_t product(GemmParams& p, const Product& g, int dtype, const Shape& sh, cudaStream_t s) {
-  const int32_t st = set_up(p, g, dtype, A_MN, B_MN, sh.pair ? 2 : 1, sh.pair ? 256 : 128, EPI == EPI_GATE);
+  const int32_t st = set_up(p, g, dtype, A_MN, B_MN, sh.cg, sh.bn, EPI == EPI_GATE);
   if (st != NCA_OK) return st;
   p.splits = sh.splits;
-  return sh.pair ? launch<T, 2, 256, A_MN, B_MN, EPI, ACT>(p, s) : launch<T, 1, 128, A_MN, B_MN, EPI, ACT>(p, s);
+  if (sh.cg == 1) return launch<T, 1, 128, A_MN, B_MN, EPI, ACT>(p, s);
+  return sh.bn == 128 ? launch<T, 2, 128, A_MN, B_MN, EPI, ACT>(p, s) : launch<T, 2, 256, A_MN, B_MN, EPI, ACT>(p, s);
 }
 
 // The weight gradient dW[batch] (m x n) = A^T B over the rows, through partial sums when split.
@@ -334,6 +394,65 @@ int32_t weight_product(GemmParams& p, const Product& g, int dtype, void* c0, voi
 size_t weight_part_bytes(long long m, long long n, int batch, long long rows) {
   const Shape sh = shape_of(m, n, batch, ceil_div(rows, kBK), true, false);
   return sh.splits == 1 ? 0 : (size_t)sh.splits * batch * m * ((n + 3) / 4 * 4) * sizeof(float);
+}
+
+// The products of few rows: out = act(x w0^T + b0) (x w1^T + b1), or x w0^T + b0.
+constexpr long long kFewRows = 64;
+template <class T, int N, bool GATE, int ACT>
+int32_t rows_launch(RowsParams& p, cudaStream_t s) {
+  using S = RowsShape<N, GATE>;
+  auto* kernel = gemm_rows_kernel<T, N, GATE, ACT>;
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
+  if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
+      return launch_status() == NCA_OK ? NCA_ERR_CUDA : NCA_ERR_DEVICE;
+    ready.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  const long long tiles = ceil_div(p.n, kBM);
+  if (tiles > (1ll << 27)) return NCA_ERR_UNSUPPORTED;
+  p.slices = 1;  // a power of two (it divides 128): two CTAs a multiprocessor, two k blocks a CTA at least
+  while (p.slices < 8 && tiles * p.slices * 2 <= 2 * sm_count() && p.kb >= 4 * p.slices) p.slices *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * p.slices));
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.slices;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.wait ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
+    cudaGetLastError();
+    return NCA_ERR_CUDA;
+  }
+  return launch_status();
+}
+template <class T, bool GATE, int ACT>
+int32_t rows_product(const GemmParams& base, const Matrix& x, const Matrix& w0, const Matrix& w1, const void* b0,
+                     const void* b1, void* out, long long ld, bool wait, int dtype, cudaStream_t s) {
+  RowsParams p{};
+  const int n = x.rows <= 16 ? 16 : x.rows <= 32 ? 32 : 64;
+  if (!encode(&p.x, x, dtype, n) || !encode(&p.w[0], w0, dtype, kBM) || (GATE && !encode(&p.w[1], w1, dtype, kBM)))
+    return NCA_ERR_CUDA;
+  p.rows = (int)x.rows;
+  p.n = (int)w0.rows;
+  p.kb = (int)ceil_div(x.cols, kBK);
+  p.wait = wait;
+  p.out = out;
+  p.ld = ld;
+  p.bias[0] = b0;
+  p.bias[1] = b1;
+  p.bias_dtype = base.bias_dtype;
+  p.ctrl = base.ctrl;
+  p.timeout_ns = base.timeout_ns;
+  if (n == 16) return rows_launch<T, 16, GATE, ACT>(p, s);
+  return n == 32 ? rows_launch<T, 32, GATE, ACT>(p, s) : rows_launch<T, 64, GATE, ACT>(p, s);
 }
 
 // --------------------------------------------------------------------------------- arguments
@@ -400,41 +519,54 @@ Plan plan_of(const NcaGatedDesc& d, bool backward) {
   return p;
 }
 
-// The operand as TMA reads it: in place, or copied into the workspace first.
-int32_t matrix_of(const Operand& o, const void* src, uint8_t* ws, cudaStream_t s, Matrix* out) {
-  if (!src) return NCA_ERR_INVALID;
-  if (!o.packed) {
-    if (reinterpret_cast<uintptr_t>(src) % 16) return NCA_ERR_INVALID;  // `unaligned` did not say so
-    *out = {src, o.rows, o.cols, o.sr};
+// The operands as TMA reads them: in place, or copied into the workspace by one launch.
+struct Operands {
+  Matrix m[OPS];
+  Packs packs;
+  int count = 0;
+  long long most = 0;  // 16-byte pieces of the largest copy
+  int32_t add(int i, const Operand& o, const void* src, uint8_t* ws) {
+    if (!src) return NCA_ERR_INVALID;
+    if (!o.packed) {
+      if (reinterpret_cast<uintptr_t>(src) % 16) return NCA_ERR_INVALID;  // `unaligned` did not say so
+      m[i] = {src, o.rows, o.cols, o.sr};
+      return NCA_OK;
+    }
+    uint16_t* dst = reinterpret_cast<uint16_t*>(ws + o.at);
+    const long long ld = pad8(o.cols);
+    packs.p[count++] = {static_cast<const uint16_t*>(src), dst, o.rows, o.cols, o.sr, o.sc, ld};
+    most = std::max(most, o.rows * ld / 8);
+    m[i] = {dst, o.rows, o.cols, ld};
     return NCA_OK;
   }
-  const long long ld = pad8(o.cols);
-  const long long tiles = ceil_div(o.rows, 32) * ceil_div(o.cols, 32);
-  pack_kernel<<<(unsigned)std::min(tiles, 148ll * 16), dim3(32, 8), 0, s>>>(
-      static_cast<const uint16_t*>(src), o.rows, o.cols, o.sr, o.sc, reinterpret_cast<uint16_t*>(ws + o.at), ld);
-  *out = {ws + o.at, o.rows, o.cols, ld};
-  return launch_status();
-}
+  int32_t copy(cudaStream_t s) const {
+    if (count == 0) return NCA_OK;
+    pack_kernel<<<dim3((unsigned)std::min<long long>(ceil_div(most, 256), 148 * 8), count), dim3(32, 8), 0, s>>>(packs);
+    return launch_status();
+  }
+};
 
-#define NCA_TRY(call)                    \
-  do {                                   \
-    const int32_t st_ = (call);          \
-    if (st_ != NCA_OK) return st_;       \
-  } while (0)
 
 template <class T, int ACT>
 int32_t forward(const NcaGatedDesc& d, const void* x, const void* w_gate, const void* w_up, const void* w_down,
                 const void* b_gate, const void* b_up, const void* b_down, void* y, void* saved, uint8_t* ws,
                 GemmParams& base, cudaStream_t s) {
   const Plan pl = plan_of(d, false);
-  Matrix mx, mg, mu, md;
-  NCA_TRY(matrix_of(pl.op[OP_X], x, ws, s, &mx));
-  NCA_TRY(matrix_of(pl.op[OP_WG], w_gate, ws, s, &mg));
-  NCA_TRY(matrix_of(pl.op[OP_WU], w_up, ws, s, &mu));
-  NCA_TRY(matrix_of(pl.op[OP_WD], w_down, ws, s, &md));
+  Operands in;
+  NCA_TRY(in.add(OP_X, pl.op[OP_X], x, ws));
+  NCA_TRY(in.add(OP_WG, pl.op[OP_WG], w_gate, ws));
+  NCA_TRY(in.add(OP_WU, pl.op[OP_WU], w_up, ws));
+  NCA_TRY(in.add(OP_WD, pl.op[OP_WD], w_down, ws));
+  NCA_TRY(in.copy(s));
+  const Matrix &mx = in.m[OP_X], &mg = in.m[OP_WG], &mu = in.m[OP_WU], &md = in.m[OP_WD];
   const size_t tf = align256((size_t)d.rows * pl.fp * 2);
   uint8_t* keep = static_cast<uint8_t*>(saved);
   void* h = keep ? keep + 3 * tf : ws + pl.h;
+  if (!keep && d.rows <= kFewRows) {
+    NCA_TRY((rows_product<T, true, ACT>(base, mx, mg, mu, b_gate, b_up, h, pl.fp, false, d.dtype, s)));
+    return rows_product<T, false, NCA_ACT_NONE>(base, {h, d.rows, d.hidden, pl.fp}, md, md, b_down, nullptr, y, d.d_out,
+                                                true, d.dtype, s);
+  }
   {
     GemmParams p = base;
     Product g{{mx, mx}, {mg, mu}, false, true, d.rows, d.hidden, d.d_in, false, 1};
@@ -462,14 +594,22 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
   const Plan pl = plan_of(d, true);
   const size_t tf = align256((size_t)d.rows * pl.fp * 2);
   const uint8_t* keep = static_cast<const uint8_t*>(saved);
-  Matrix mx, mg, mu, md, mdy;
-  NCA_TRY(matrix_of(pl.op[OP_DY], dy, ws, s, &mdy));
+  const bool hidden_grads = dx || dw_gate || dw_up || db_gate || db_up;
+  Operands in;
+  NCA_TRY(in.add(OP_DY, pl.op[OP_DY], dy, ws));
+  if (hidden_grads) NCA_TRY(in.add(OP_WD, pl.op[OP_WD], w_down, ws));
+  if (dx) {
+    NCA_TRY(in.add(OP_WG, pl.op[OP_WG], w_gate, ws));
+    NCA_TRY(in.add(OP_WU, pl.op[OP_WU], w_up, ws));
+  }
+  if (dw_gate || dw_up) NCA_TRY(in.add(OP_X, pl.op[OP_X], x, ws));
+  NCA_TRY(in.copy(s));
+  const Matrix &mx = in.m[OP_X], &mg = in.m[OP_WG], &mu = in.m[OP_WU], &md = in.m[OP_WD], &mdy = in.m[OP_DY];
   const Matrix mh{keep + 3 * tf, d.rows, d.hidden, pl.fp};
   const Matrix mdg{ws + pl.dgate, d.rows, d.hidden, pl.fp}, mdu{ws + pl.dup, d.rows, d.hidden, pl.fp};
   float* part = reinterpret_cast<float*>(ws + pl.part);
   float* part_sums = reinterpret_cast<float*>(ws + pl.sums);
-  if (dx || dw_gate || dw_up || db_gate || db_up) {
-    NCA_TRY(matrix_of(pl.op[OP_WD], w_down, ws, s, &md));
+  if (hidden_grads) {
     GemmParams p = base;
     Product g{{mdy, mdy}, {md, md}, false, false, d.rows, d.hidden, d.d_out, false, 1};
     if (!encode_out(&p.out[0], ws + pl.dgate, d.dtype, d.rows, d.hidden, pl.fp) ||
@@ -480,8 +620,6 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
         p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s)));
   }
   if (dx) {
-    NCA_TRY(matrix_of(pl.op[OP_WG], w_gate, ws, s, &mg));
-    NCA_TRY(matrix_of(pl.op[OP_WU], w_up, ws, s, &mu));
     GemmParams p = base;
     Product g{{mdg, mdu}, {mg, mu}, true, true, d.rows, d.d_in, d.hidden, true, 1};
     if (!set_out(p, d.dtype, dx, dx, d.rows, d.d_in)) return NCA_ERR_CUDA;
@@ -489,7 +627,6 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
         p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s)));
   }
   if (dw_gate || dw_up) {
-    NCA_TRY(matrix_of(pl.op[OP_X], x, ws, s, &mx));
     GemmParams p = base;
     if (dw_gate && dw_up) {
       Product g{{mdg, mdu}, {mx, mx}, true, false, d.hidden, d.d_in, d.rows, false, 2};

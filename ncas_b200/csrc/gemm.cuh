@@ -271,15 +271,15 @@ struct GemmShape {
   static constexpr int kABytes = kBM * kBK * 2;
   static constexpr int kBBytes = kBNc * kBK * 2;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  // places of an epilogue warp: h and the three planes; dgate, dup and the planes; else two in turn
-  static constexpr int kPlaces = EPI == EPI_GATE ? 4 : EPI == EPI_DGATE ? 5 : 2;
+  // places of an epilogue warp: h (or dgate, then dup) and the three planes; else two in turn
+  static constexpr int kPlaces = EPI == EPI_GATE || EPI == EPI_DGATE ? 4 : 2;
   static constexpr int kPlaceBytes = kEpilogueWarps * kPlaces * kPlace;
-  static constexpr int kRest = 2 * 256 * (int)sizeof(float) + 512;
+  static constexpr int kRest = BN * (int)sizeof(float) + 512;
   static constexpr int kMost = (227 * 1024 - 1024 - kPlaceBytes - kRest) / kStageBytes;
-  static constexpr int kStages = kMost > 6 ? 6 : kMost;
+  static constexpr int kStages = kMost > 10 ? 10 : kMost;
   static constexpr int kPlacesAt = kStages * kStageBytes;
   static constexpr int kBias = kPlacesAt + kPlaceBytes;
-  static constexpr int kBars = kBias + 2 * 256 * (int)sizeof(float);
+  static constexpr int kBars = kBias + BN * (int)sizeof(float);
   static constexpr int kSmem = kBars + 512 + 1024;  // 1024: alignment
   static constexpr int kTmemCols = 2 * BN;
 };
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     uint32_t load_ph = 0;
     int flip = 0;
     bool ok = true, pending = false;  // pending: planes asked for and not yet waited for
-    float* bias_s = reinterpret_cast<float*>(smem + S::kBias);  // [2][256]
+    float* bias_s = reinterpret_cast<float*>(smem + S::kBias);  // [BN]: EPI_GATE those of gate, then of up
     const bool biased = (EPI == EPI_GATE || EPI == EPI_STORE) && (p.bias[0] || p.bias[1]);
     int buf = 0;
     uint32_t ph = 0;
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         asm volatile("bar.sync 1, 256;" ::: "memory");  // the tile before has read its own
         if (i < cols) {
           bias_s[i] = p.bias[0] ? load_param(p.bias[0], p.bias_dtype, tl.n0 + i) : 0.f;
-          if (EPI == EPI_GATE) bias_s[256 + i] = p.bias[1] ? load_param(p.bias[1], p.bias_dtype, tl.n0 + i) : 0.f;
+          if (EPI == EPI_GATE) bias_s[kTN + i] = p.bias[1] ? load_param(p.bias[1], p.bias_dtype, tl.n0 + i) : 0.f;
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           mbar_arrive_expect_tx(&loaded[warp - 4], 3 * kPlace);
 #pragma unroll
           for (int i = 0; i < 3; ++i)
-            tma_load_3d(place + (2 + i) * kPlace, &p.planes, smem_u32(&loaded[warp - 4]), tl.n0 + c, row0, i);
+            tma_load_3d(place + (1 + i) * kPlace, &p.planes, smem_u32(&loaded[warp - 4]), tl.n0 + c, row0, i);
         }
       };
       if (EPI == EPI_DGATE && rows > 0 && 32 * turn < cols) ask(32 * turn);
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               g[i] += bias_s[c + i];
-              u[i] += bias_s[256 + c + i];
+              u[i] += bias_s[kTN + c + i];
             }
           }
 #pragma unroll
@@ -553,9 +553,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             load_ph ^= 1;
             pending = false;
             uint4 k0[4], k1[4], k2[4];
-            take_row(place + 2 * kPlace, lane, k0);
-            take_row(place + 3 * kPlace, lane, k1);
-            take_row(place + 4 * kPlace, lane, k2);
+            take_row(place + kPlace, lane, k0);
+            take_row(place + 2 * kPlace, lane, k1);
+            take_row(place + 3 * kPlace, lane, k2);
             __syncwarp();
             if (c + 64 < cols) ask(c + 64);
             join_planes(k0, k1, k2, g, u);
@@ -575,13 +575,22 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           __syncwarp();
           pack_row<T>(g, v);
           put_row(place, lane, v);
+          fence_async_proxy();
+          __syncwarp();
           pack_row<T>(u, v);
-          put_row(place + kPlace, lane, v);
+          if (lane == 0) {
+            if (rows > 0) {
+              tma_store_2d(&p.out[0], place, col, row0);
+              bulk_commit();
+            }
+            bulk_wait_read<0>();
+          }
+          __syncwarp();
+          put_row(place, lane, v);
           fence_async_proxy();
           __syncwarp();
           if (lane == 0 && rows > 0) {
-            tma_store_2d(&p.out[0], place, col, row0);
-            tma_store_2d(&p.out[1], place + kPlace, col, row0);
+            tma_store_2d(&p.out[1], place, col, row0);
             bulk_commit();
           }
         } else if constexpr (EPI == EPI_PARTIAL) {
