@@ -339,14 +339,16 @@ typedef struct NcaNormDesc {
   int32_t param_dtype;          /* NcaDtype of weight, bias and their gradients: NCA_F32 or dtype */
   int32_t act;                  /* NcaAct */
   float eps;
+  int32_t masked;               /* a mask is passed */
+  int32_t unaligned;            /* x, dy, y or dx is not on a 16-byte boundary */
   int64_t x_stride_n, x_stride_cell;    /* channels are adjacent */
   int64_t dy_stride_n, dy_stride_cell;
   int64_t mask_stride_n, mask_stride_cell;
 } NcaNormDesc;
 
 int32_t nca_b200_group_norm_workspace(const NcaNormDesc* d, int32_t backward, size_t* bytes);
-/* stats: device [n][groups][2] fp32, receives each group's mean and 1 / sqrt(var + eps) (the
- * backward call reads it).  weight, bias, mask (uint8) may be NULL. */
+/* stats: device [n][groups][2] fp32, receives each group's mean and 1 / sqrt(var + eps) for the
+ * backward call.  stats, weight, bias, mask (uint8) may be NULL, and the workspace when 0 bytes. */
 int32_t nca_b200_group_norm(const NcaNormDesc* d, const void* x, const void* weight,
                             const void* bias, const uint8_t* mask, void* y, float* stats,
                             void* workspace, size_t workspace_bytes, void* stream);

@@ -124,6 +124,8 @@ class NcaNormDesc(C.Structure):
         ("param_dtype", C.c_int32),
         ("act", C.c_int32),
         ("eps", C.c_float),
+        ("masked", C.c_int32),
+        ("unaligned", C.c_int32),
         ("x_stride_n", C.c_int64),
         ("x_stride_cell", C.c_int64),
         ("dy_stride_n", C.c_int64),

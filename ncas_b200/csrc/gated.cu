@@ -145,26 +145,27 @@ __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int m) 
 __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs all) {
   __shared__ uint16_t tile[32][34];
   const Pack& p = all.p[blockIdx.y];
-  if (p.sc == 1) {  // rows of adjacent values: 8 a lane
-    const long long vecs = p.ld / 8, total = p.rows * vecs;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.y * 32 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-      const long long r = i / vecs, c = (i - r * vecs) * 8;
-      const uint16_t* from = p.src + r * p.sr + c;
-      const int m = (int)(reinterpret_cast<uintptr_t>(from) & 15) / 2;
-      uint4 out;
-      if (c >= 8 && c + 16 <= p.cols) {  // both aligned pieces lie inside the row
-        const uint4* q = reinterpret_cast<const uint4*>(from - m);
-        out = shifted(q[0], q[1], m);
-      } else {
-        uint32_t v[4];
+  if (p.sc == 1) {  // rows of adjacent values: a warp a row, 8 a lane
+    for (long long r = (long long)blockIdx.x * 8 + threadIdx.y; r < p.rows; r += (long long)gridDim.x * 8) {
+      const uint16_t* row = p.src + r * p.sr;
+      const int m = (int)(reinterpret_cast<uintptr_t>(row) & 15) / 2;
+#pragma unroll 2
+      for (long long c = 8 * threadIdx.x; c < p.ld; c += 256) {
+        uint4 out;
+        if (c >= 8 && c + 16 <= p.cols) {  // both aligned pieces lie inside the row
+          const uint4* q = reinterpret_cast<const uint4*>(row + c - m);
+          out = shifted(q[0], q[1], m);
+        } else {
+          uint32_t v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t lo = c + 2 * j < p.cols ? from[2 * j] : 0, hi = c + 2 * j + 1 < p.cols ? from[2 * j + 1] : 0;
-          v[j] = lo | hi << 16;
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = c + 2 * j < p.cols ? row[c + 2 * j] : 0, hi = c + 2 * j + 1 < p.cols ? row[c + 2 * j + 1] : 0;
+            v[j] = lo | hi << 16;
+          }
+          out = make_uint4(v[0], v[1], v[2], v[3]);
         }
-        out = make_uint4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<uint4*>(p.dst + r * p.ld + c) = out;
       }
-      *reinterpret_cast<uint4*>(p.dst + r * p.ld + c) = out;
     }
     return;
   }
@@ -224,7 +225,8 @@ struct ColumnSums {
 };
 constexpr int kSumSplits = 256;
 template <class T>
-__global__ void __launch_bounds__(256) column_sums_kernel(ColumnSums p, long long rows, int splits) {
+__global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant__ ColumnSums p, long long rows,
+                                                          int splits) {
   __shared__ float2 red[8][32][4];
   const int z = blockIdx.z;
   const long long c = 8 * ((long long)blockIdx.x * 32 + threadIdx.x), cols = p.cols[z], padded = (cols + 7) / 8 * 8;
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(256) column_sums_kernel(ColumnSums p, long lon
     *reinterpret_cast<float2*>(p.part[z] + blockIdx.y * padded + c + 2 * threadIdx.y) = t;
   }
 }
-__global__ void __launch_bounds__(512) column_store_kernel(ColumnSums p, int splits, int dtype) {
+__global__ void __launch_bounds__(512) column_store_kernel(const __grid_constant__ ColumnSums p, int splits, int dtype) {
   __shared__ float red[16][33];
   const int z = blockIdx.z;
   const long long c = (long long)blockIdx.x * 32 + threadIdx.x, cols = p.cols[z], padded = (cols + 7) / 8 * 8;
@@ -524,7 +526,7 @@ struct Operands {
   Matrix m[OPS];
   Packs packs;
   int count = 0;
-  long long most = 0;  // 16-byte pieces of the largest copy
+  long long most = 0;  // blocks for the largest copy: 8 rows each, or tiles
   int32_t add(int i, const Operand& o, const void* src, uint8_t* ws) {
     if (!src) return NCA_ERR_INVALID;
     if (!o.packed) {
@@ -535,13 +537,13 @@ struct Operands {
     uint16_t* dst = reinterpret_cast<uint16_t*>(ws + o.at);
     const long long ld = pad8(o.cols);
     packs.p[count++] = {static_cast<const uint16_t*>(src), dst, o.rows, o.cols, o.sr, o.sc, ld};
-    most = std::max(most, o.rows * ld / 8);
+    most = std::max(most, o.sc == 1 ? ceil_div(o.rows, 8) : ceil_div(o.rows, 32) * ceil_div(o.cols, 32));
     m[i] = {dst, o.rows, o.cols, ld};
     return NCA_OK;
   }
   int32_t copy(cudaStream_t s) const {
     if (count == 0) return NCA_OK;
-    pack_kernel<<<dim3((unsigned)std::min<long long>(ceil_div(most, 256), 148 * 8), count), dim3(32, 8), 0, s>>>(packs);
+    pack_kernel<<<dim3((unsigned)std::min<long long>(most, 148 * 8), count), dim3(32, 8), 0, s>>>(packs);
     return launch_status();
   }
 };

@@ -512,23 +512,31 @@ int worst_chunks(const NcaNormDesc& d) {  // over every vector width: one vector
 }
 
 struct Layout {
-  size_t part, counts, ab, params, total;
+  size_t stats, part, counts, ab, params, total;
 };
-Layout layout_of(const NcaNormDesc& d) {
-  const size_t chunks = std::max(worst_chunks(d), 8);  // the held backward has up to 8 slices
-  Layout l;
-  l.part = 0;
-  l.counts = l.part + align256((size_t)d.n * chunks * d.channels * sizeof(float2));
-  l.ab = l.counts + align256((size_t)d.n * chunks * sizeof(int));
-  l.params = l.ab + align256((size_t)d.n * d.groups * sizeof(float2));
-  l.total = l.params + align256((size_t)kParamSplits * d.channels * sizeof(float2));
+// held: the slices of the kernel that holds samples, 0 when the streaming kernels run.
+Layout layout_of(const NcaNormDesc& d, bool backward, int held) {
+  const size_t chunks = held ? held : worst_chunks(d);
+  Layout l{};
+  size_t at = 0;
+  const auto take = [&](bool needed, size_t bytes) {
+    const size_t here = at;
+    if (needed) at += align256(bytes);
+    return here;
+  };
+  l.stats = take(!backward && !held, (size_t)d.n * d.groups * sizeof(float2));
+  l.part = take(backward || !held, (size_t)d.n * chunks * d.channels * sizeof(float2));
+  l.counts = take(!held, (size_t)d.n * chunks * sizeof(int));
+  l.ab = take(backward && !held, (size_t)d.n * d.groups * sizeof(float2));
+  l.params = take(backward, (size_t)kParamSplits * d.channels * sizeof(float2));
+  l.total = at;
   return l;
 }
 
 bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 
 NormArgs args_of(const NcaNormDesc& d, const void* x, const void* weight, const void* bias,
-                 const uint8_t* mask, const void* dy, void* y, float* stats, void* ws) {
+                 const uint8_t* mask, const void* dy, void* y, float* stats) {
   NormArgs a{};
   a.n = d.n;
   a.cells = d.cells;
@@ -550,21 +558,24 @@ NormArgs args_of(const NcaNormDesc& d, const void* x, const void* weight, const 
   a.dy = dy;
   a.y = y;
   a.stats = stats;
-  const Layout l = layout_of(d);
+  return a;
+}
+void place(NormArgs& a, const Layout& l, void* ws) {
   uint8_t* w = static_cast<uint8_t*>(ws);
+  if (!a.stats) a.stats = reinterpret_cast<float*>(w + l.stats);
   a.part = reinterpret_cast<float2*>(w + l.part);
   a.counts = reinterpret_cast<int*>(w + l.counts);
   a.ab = reinterpret_cast<float2*>(w + l.ab);
-  return a;
 }
 
-// Widest vector (16 bytes at most) that the channel count, the strides and the addresses allow.
-int vector_width(const NcaNormDesc& d, const NormArgs& a, bool backward) {
+// Widest vector (16 bytes at most) that the channel count, the strides and the addresses allow; single
+// values where an address is on no 16-byte boundary.
+int vector_width(const NcaNormDesc& d, bool backward) {
+  if (d.unaligned) return 1;
   const size_t size = dtype_size(d.dtype);
   for (int v = (int)(16 / size); v > 1; v /= 2) {
-    bool ok = d.channels % v == 0 && d.x_stride_n % v == 0 && d.x_stride_cell % v == 0 &&
-              aligned(a.x, v * size) && aligned(a.y, v * size);
-    if (backward) ok = ok && d.dy_stride_n % v == 0 && d.dy_stride_cell % v == 0 && aligned(a.dy, v * size);
+    bool ok = d.channels % v == 0 && d.x_stride_n % v == 0 && d.x_stride_cell % v == 0;
+    if (backward) ok = ok && d.dy_stride_n % v == 0 && d.dy_stride_cell % v == 0;
     if (ok) return v;
   }
   return 1;
@@ -694,12 +705,34 @@ struct BackwardCall {
 
 }  // namespace
 
+// What a call does and needs, from its descriptor alone.
+struct Choice {
+  int v, held;
+  Layout l;
+};
+Choice choose(const NcaNormDesc& d, bool backward) {
+  static const uint8_t some = 1;
+  Choice c;
+  c.v = vector_width(d, backward);
+  const NormArgs a = args_of(d, nullptr, nullptr, nullptr, d.masked ? &some : nullptr, nullptr, nullptr, nullptr);
+  c.held = norm_held_slices(a, d.dtype, c.v, backward);
+  c.l = layout_of(d, backward, c.held);
+  return c;
+}
+bool addresses_ok(const NcaNormDesc& d, const uint8_t* mask, std::initializer_list<const void*> ps) {
+  if ((mask != nullptr) != (d.masked != 0)) return false;
+  if (!d.unaligned)
+    for (const void* p : ps)
+      if (!aligned(p, 16)) return false;
+  return true;
+}
+
 extern "C" {
 
-int32_t nca_b200_group_norm_workspace(const NcaNormDesc* d, int32_t, size_t* bytes) {
+int32_t nca_b200_group_norm_workspace(const NcaNormDesc* d, int32_t backward, size_t* bytes) {
   const int32_t st = check_desc(d);
   if (st != NCA_OK || !bytes) return st != NCA_OK ? st : NCA_ERR_INVALID;
-  *bytes = layout_of(*d).total;
+  *bytes = d->n == 0 || d->cells == 0 ? 0 : choose(*d, backward != 0).l.total;
   return NCA_OK;
 }
 
@@ -709,12 +742,14 @@ int32_t nca_b200_group_norm(const NcaNormDesc* d, const void* x, const void* wei
   const int32_t st = check_desc(d);
   if (st != NCA_OK) return st;
   if (d->n == 0 || d->cells == 0) return NCA_OK;
-  if (!x || !y || !stats || !workspace || workspace_bytes < layout_of(*d).total) return NCA_ERR_INVALID;
-  const NormArgs a = args_of(*d, x, weight, bias, mask, nullptr, y, stats, workspace);
-  const int v = vector_width(*d, a, false);
-  if (norm_held_applies(a, d->dtype, v, false))
-    return norm_held_forward(a, d->dtype, d->act, v, static_cast<cudaStream_t>(stream));
-  return dispatch(*d, streaming_width(d->dtype, v), ForwardCall{*d, a, static_cast<cudaStream_t>(stream)});
+  const Choice c = choose(*d, false);
+  if (!x || !y || workspace_bytes < c.l.total || (c.l.total && !workspace) || !addresses_ok(*d, mask, {x, y}))
+    return NCA_ERR_INVALID;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  NormArgs a = args_of(*d, x, weight, bias, mask, nullptr, y, stats);
+  if (c.held) return norm_held_forward(a, d->dtype, d->act, c.v, s);
+  place(a, c.l, workspace);
+  return dispatch(*d, streaming_width(d->dtype, c.v), ForwardCall{*d, a, s});
 }
 
 int32_t nca_b200_group_norm_backward(const NcaNormDesc* d, const void* x, const void* weight,
@@ -730,19 +765,20 @@ int32_t nca_b200_group_norm_backward(const NcaNormDesc* d, const void* x, const 
     if (dbias && cudaMemsetAsync(dbias, 0, bytes, s) != cudaSuccess) return NCA_ERR_CUDA;
     return NCA_OK;
   }
-  if (!x || !dy || !stats || !workspace || workspace_bytes < layout_of(*d).total) return NCA_ERR_INVALID;
-  const NormArgs a = args_of(*d, x, weight, bias, mask, dy, dx, const_cast<float*>(stats), workspace);
-  float2* params = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + layout_of(*d).params);
-  const int v = vector_width(*d, a, true);
-  if (norm_held_applies(a, d->dtype, v, true)) {
-    NormArgs b = a;
-    if (!dweight && !dbias) b.part = nullptr;
-    const int32_t r = norm_held_backward(b, d->dtype, d->act, v, s);
-    if (r != NCA_OK || !b.part) return r;
-    param_grads(a.part, a.n * norm_held_slices(a, d->dtype, v), a.channels, dweight, dbias, a.param_dtype, params, s);
+  const Choice c = choose(*d, true);
+  if (!x || !dy || !stats || !workspace || workspace_bytes < c.l.total || !addresses_ok(*d, mask, {x, dy, dx}))
+    return NCA_ERR_INVALID;
+  NormArgs a = args_of(*d, x, weight, bias, mask, dy, dx, const_cast<float*>(stats));
+  place(a, c.l, workspace);
+  float2* params = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + c.l.params);
+  if (c.held) {
+    if (!dweight && !dbias) a.part = nullptr;
+    const int32_t r = norm_held_backward(a, d->dtype, d->act, c.v, s);
+    if (r != NCA_OK || !a.part) return r;
+    param_grads(a.part, a.n * c.held, a.channels, dweight, dbias, a.param_dtype, params, s);
     return launch_status();
   }
-  return dispatch(*d, streaming_width(d->dtype, v), BackwardCall{*d, a, dweight, dbias, params, s});
+  return dispatch(*d, streaming_width(d->dtype, c.v), BackwardCall{*d, a, dweight, dbias, params, s});
 }
 
 }  // extern "C"

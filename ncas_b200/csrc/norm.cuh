@@ -33,11 +33,10 @@ struct NormArgs {
   float2* ab;                // backward: [n][groups] (A / n, B / n)
 };
 
-// Runs the forward or backward kernel that holds samples in shared memory, when it applies: returns
-// false when it does not.  `v` is the vector width that channels, strides and addresses allow.  The
+// The kernels that hold samples in shared memory: the blocks that share a sample (8 at most), or 0 where
+// they do not apply.  `v` is the vector width that channels, strides and addresses allow.  The
 // backward writes (sum dz, sum dz h) of every sample and slice to a.part as [n][slices][channels].
-int norm_held_slices(const NormArgs& a, int dtype, int v);  // of the backward, at most 8
-bool norm_held_applies(const NormArgs& a, int dtype, int v, bool backward);
+int norm_held_slices(const NormArgs& a, int dtype, int v, bool backward);
 int32_t norm_held_forward(const NormArgs& a, int dtype, int act, int v, cudaStream_t s);
 int32_t norm_held_backward(const NormArgs& a, int dtype, int act, int v, cudaStream_t s);
 

@@ -158,8 +158,10 @@ struct Call {
 
 }  // namespace
 
-bool norm_held_applies(const NormArgs& a, int dtype, int v, bool backward) { return plan_of(a, dtype, v, backward).ok; }
-int norm_held_slices(const NormArgs& a, int dtype, int v) { return plan_of(a, dtype, v, true).slices; }
+int norm_held_slices(const NormArgs& a, int dtype, int v, bool backward) {
+  const HeldPlan p = plan_of(a, dtype, v, backward);
+  return p.ok ? p.slices : 0;
+}
 int32_t norm_held_backward(const NormArgs& a, int dtype, int act, int v, cudaStream_t s) {
   const HeldPlan p = plan_of(a, dtype, v, true);
   return dispatch_held(a, dtype, act, p.v, Call{a, p, s});

@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_forward_kernel(const
     }
   }
   const float rstd = n > 0.f ? 1.f / sqrtf(m2 / n + a.eps) : 0.f;
-  if (w.rank == 0 && w.row == 0 && w.ch % a.per_group == 0) {
+  if (a.stats && w.rank == 0 && w.row == 0 && w.ch % a.per_group == 0) {
     float* st = a.stats + 2 * (w.sample * a.groups + w.ch / a.per_group);
     st[0] = mean;
     st[1] = rstd;

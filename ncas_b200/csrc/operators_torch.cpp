@@ -91,8 +91,9 @@ struct Needs {
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 Tensor scratch(size_t bytes, const Tensor& like) {
-  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+  return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
+size_t bytes_of(const Tensor& t) { return t.defined() ? (size_t)t.numel() : 0; }
 
 // -------------------------------------------------------------------------------- group norm
 // (N, ..., C) seen as samples x cells x channels: a view when the dimensions between collapse to
@@ -129,6 +130,9 @@ Cells cells_of(const Tensor& x, bool channels) {
 
 struct Norm {
   NcaNormDesc d{};
+  static int unaligned(const Tensor& t) {
+    return t.defined() && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 ? 1 : 0;
+  }
   Cells x, mask, dy;
   Norm(const Tensor& xt, int64_t groups, const Tensor& weight, const Tensor& bias, double eps, int act,
        const Tensor& maskt) {
@@ -146,26 +150,28 @@ struct Norm {
     d.x_stride_cell = x.stride_cell;
     if (maskt.defined()) {
       mask = cells_of(maskt, false);
+      d.masked = 1;
       d.mask_stride_n = mask.stride_n;
       d.mask_stride_cell = mask.stride_cell;
     }
   }
-  Tensor workspace(bool backward) {
+  Tensor workspace(bool backward, const Tensor& out) {
     size_t bytes = 0;
+    d.unaligned = unaligned(x.t) | unaligned(out) | unaligned(dy.t);
     check(nca_b200_group_norm_workspace(&d, backward, &bytes), "nca_b200_group_norm_workspace");
     return scratch(bytes, x.t);
   }
 };
 
 std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, int64_t groups, const Tensor& weight, const Tensor& bias,
-                                        double eps, int act, const Tensor& mask) {
+                                        double eps, int act, const Tensor& mask, bool save) {
   const c10::cuda::CUDAGuard guard(x.device());
   Norm n(x, groups, weight, bias, eps, act, mask);
   Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-  Tensor stats = at::empty({n.d.n, groups, 2}, x.options().dtype(at::kFloat));
-  Tensor ws = n.workspace(false);
+  Tensor stats = save ? at::empty({n.d.n, groups, 2}, x.options().dtype(at::kFloat)) : Tensor();
+  Tensor ws = n.workspace(false, y);
   check(nca_b200_group_norm(&n.d, ptr(n.x.t), ptr(weight), ptr(bias), static_cast<const uint8_t*>(ptr(n.mask.t)),
-                            mptr(y), static_cast<float*>(mptr(stats)), mptr(ws), ws.numel(), stream_of(x)),
+                            mptr(y), static_cast<float*>(mptr(stats)), mptr(ws), bytes_of(ws), stream_of(x)),
         "nca_b200_group_norm");
   return {y, stats};
 }
@@ -175,7 +181,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
                         const OptTensor& bias_, double eps, int64_t act, const OptTensor& mask_) {
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor weight = or_none(weight_), bias = or_none(bias_), mask = or_none(mask_);
-    auto [y, stats] = norm_forward(x, groups, weight, bias, eps, (int)act, mask);
+    auto [y, stats] = norm_forward(x, groups, weight, bias, eps, (int)act, mask, true);
     ctx->save_for_backward({x, weight, bias, mask, stats});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["eps"] = eps;
@@ -197,11 +203,11 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     if (needs[0]) dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
     if (needs[1]) dw = at::empty_like(weight, at::MemoryFormat::Contiguous);
     if (needs[2]) db = at::empty_like(bias, at::MemoryFormat::Contiguous);
-    Tensor ws = n.workspace(true);
+    Tensor ws = n.workspace(true, dx);
     check(nca_b200_group_norm_backward(&n.d, ptr(n.x.t), ptr(weight), ptr(bias),
                                        static_cast<const uint8_t*>(ptr(n.mask.t)),
                                        static_cast<const float*>(ptr(stats)), ptr(n.dy.t), mptr(dx), mptr(dw),
-                                       mptr(db), mptr(ws), ws.numel(), stream_of(x)),
+                                       mptr(db), mptr(ws), bytes_of(ws), stream_of(x)),
           "nca_b200_group_norm_backward");
     return {dx, Tensor(), dw, db, Tensor(), Tensor(), Tensor()};
   }
@@ -237,7 +243,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight_,
   }
   if (any_grad({&x, &weight, &bias})) 
     return NormFunction::apply(x, groups, optional(weight), optional(bias), eps, (int64_t)act, optional(mask));
-  return std::get<0>(norm_forward(x, groups, weight, bias, eps, act, mask));
+  return std::get<0>(norm_forward(x, groups, weight, bias, eps, act, mask, false));
 }
 
 // -------------------------------------------------------------------------------- gated block
@@ -309,7 +315,7 @@ std::tuple<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& wg, cons
   check(nca_b200_gated_workspace(&g.d, 0, &bytes), "nca_b200_gated_workspace");
   Tensor ws = scratch(bytes, x), ctrl = control_words(x.device());
   check(nca_b200_gated_ffn(&g.d, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(bg), ptr(bu), ptr(bd), mptr(y), mptr(saved),
-                           mptr(ws), ws.numel(), static_cast<int32_t*>(mptr(ctrl)), timeout_ms(),
+                           mptr(ws), bytes_of(ws), static_cast<int32_t*>(mptr(ctrl)), timeout_ms(),
                            stream_of(x)),
         "nca_b200_gated_ffn");
   return {y, saved};
@@ -345,7 +351,7 @@ struct GatedFunction : torch::autograd::Function<GatedFunction> {
     Tensor ws = scratch(bytes, x), ctrl = control_words(x.device());
     check(nca_b200_gated_ffn_backward(&g.d, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(saved[7]), ptr(dy), mptr(out[0]),
                                       mptr(out[1]), mptr(out[2]), mptr(out[3]), mptr(out[4]), mptr(out[5]),
-                                      mptr(out[6]), mptr(ws), ws.numel(), static_cast<int32_t*>(mptr(ctrl)),
+                                      mptr(out[6]), mptr(ws), bytes_of(ws), static_cast<int32_t*>(mptr(ctrl)),
                                       timeout_ms(), stream_of(x)),
           "nca_b200_gated_ffn_backward");
     return {out[0], out[1], out[2], out[3], out[4], out[5], out[6], Tensor(), Tensor()};
@@ -477,7 +483,7 @@ Tensor distill_run(Distill& a, const Tensor& stats, const Tensor& dlogits) {
   Tensor ws = scratch(bytes, a.logits);
   check(nca_b200_distill(&a.d, ptr(a.logits), ptr(a.teacher), ptr(a.index), static_cast<const float*>(ptr(a.weight)),
                          static_cast<float*>(mptr(loss)), static_cast<float*>(mptr(stats)), mptr(dlogits), mptr(ws),
-                         ws.numel(), stream_of(a.logits)),
+                         bytes_of(ws), stream_of(a.logits)),
         "nca_b200_distill");
   return loss;
 }

@@ -19,6 +19,16 @@ import torch
 from ._lib import NcaError
 from ._ops import ops
 
+_overloads: dict = {}
+
+
+def _op(name):
+    """torch.ops.nca_b200.<name>.default, looked up once."""
+    op = _overloads.get(name)
+    if op is None:
+        op = _overloads[name] = getattr(ops(), name).default
+    return op
+
 
 def group_norm_act(x, groups, weight=None, bias=None, *, eps=1e-5, act="silu", mask=None):
     """act((x - mean) / sqrt(var + eps) * weight + bias) of x (N, ..., C), contiguous.
@@ -30,7 +40,7 @@ def group_norm_act(x, groups, weight=None, bias=None, *, eps=1e-5, act="silu", m
     zero are not read, count in no statistic, and have y and gradient 0; a sample without cells is 0.
     Differentiable in x, weight and bias.
     """
-    return ops().group_norm_act(x, groups, weight, bias, eps, act, mask)
+    return _op("group_norm_act")(x, groups, weight, bias, eps, act, mask)
 
 
 def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, *, act="silu"):
@@ -41,7 +51,7 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, *, a
     the hidden product and the gradients of its two factors are rounded to the type of x in between.  Matrices whose rows start on 16-byte boundaries are read in place, others are
     copied first.  Differentiable in every tensor.
     """
-    return ops().gated_ffn(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
+    return _op("gated_ffn")(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
 
 
 def distill_loss(logits, teacher_logits, teacher_index, *, temperature=1.0, weight=None, reduction="mean"):
@@ -53,19 +63,19 @@ def distill_loss(logits, teacher_logits, teacher_index, *, temperature=1.0, weig
     add up).  weight: float32 (...).  A row without entries or with weight 0 has loss and gradient 0.
     reduction: "none" (float32, (...)), "sum", or "mean" over all rows.  Differentiable in logits.
     """
-    return ops().distill_loss(logits, teacher_logits, teacher_index, temperature, weight, reduction)
+    return _op("distill_loss")(logits, teacher_logits, teacher_index, temperature, weight, reduction)
 
 
 def distill_loss_and_grad(logits, teacher_logits, teacher_index, *, temperature=1.0, weight=None,
                           reduction="mean"):
     """(distill_loss, gradient of its sum over rows, or of its mean, by the logits) with one read of the
     logits where a row fits on the chip; for training loops that call `logits.backward(grad)`."""
-    return ops().distill_loss_and_grad(logits, teacher_logits, teacher_index, temperature, weight, reduction)
+    return _op("distill_loss_and_grad")(logits, teacher_logits, teacher_index, temperature, weight, reduction)
 
 
 def check(device="cuda") -> None:
     """Synchronises the current stream and raises NcaError when a kernel's bounded wait ran out since
     the last call."""
-    status, site = ops().operators_status(torch.empty(0, device=device))
+    status, site = _op("operators_status")(torch.empty(0, device=device))
     if status != 0:
         raise NcaError(status, "cell-training operators", site)
