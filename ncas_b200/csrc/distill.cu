@@ -22,7 +22,7 @@ struct DistillArgs {
   long long rows, top;
   int classes;
   int teacher_dtype, index_bits;
-  float tau;
+  float tau, c2, inv_tau;  // temperature, log2(e) / tau, 1 / tau
   long long s_stride, t_stride, i_stride;
   const void* logits;
   const void* teacher;
@@ -99,28 +99,76 @@ struct Lanes {
 };
 
 // -------------------------------------------------------------------------------- few classes
+// A row of n <= K values into registers (one access when the row is K values wide and lies on its own
+// size).  n is the same for all threads.
+template <class E, int K>
+__device__ __forceinline__ void load_values(const E* from, int n, bool whole, E (&v)[K]) {
+  if (whole) {
+    const Vec<E, K> w = *reinterpret_cast<const Vec<E, K>*>(from);
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = w.v[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (k < n) v[k] = from[k];
+  }
+}
+template <class E, int K>
+__device__ __forceinline__ bool whole_rows(const void* p, long long stride, int n) {
+  return sizeof(E) * K <= 16 && n == K && stride % K == 0 && reinterpret_cast<uintptr_t>(p) % (sizeof(E) * K) == 0;
+}
+
 // G lanes a row, K classes a lane in registers (class j of a row: lane j % G, register j / G), the
-// entries likewise: one read of everything, no second pass.  For top <= G K.
-template <class T, int G, int K, bool FWD>
+// entries likewise: one read of everything, no second pass.  For top <= G K.  I: the index type; the
+// teacher has the logits' type (SAME) or one that is looked up at each load.
+template <class T, class I, int G, int K, bool SAME, bool FWD>
 __global__ void __launch_bounds__(kThreads) distill_small_kernel(DistillArgs a) {
   const Lanes<G> l(nullptr);
   constexpr int kRows = kThreads / G;
-  const float c2 = kLog2e / a.tau, inv_tau = 1.f / a.tau;
+  const float c2 = a.c2, inv_tau = a.inv_tau;
   const int top = (int)a.top;
+  const bool whole_s = G == 1 && whole_rows<T, K>(a.logits, a.s_stride, a.classes);
+  const bool whole_d = G == 1 && a.dlogits && whole_rows<T, K>(a.dlogits, a.classes, a.classes);
+  const bool whole_i = G == 1 && whole_rows<I, K>(a.index, a.i_stride, top);
+  const bool whole_t = G == 1 && SAME && whole_rows<T, K>(a.teacher, a.t_stride, top);
   for (long long r = (long long)blockIdx.x * kRows + threadIdx.x / G; r < a.rows;
        r += (long long)gridDim.x * kRows) {
     const T* s = static_cast<const T*>(a.logits) + r * a.s_stride;
+    const I* is = static_cast<const I*>(a.index) + r * a.i_stride;
     T* ds = static_cast<T*>(a.dlogits) + r * (long long)a.classes;
     const float w = a.weight ? a.weight[r] : 1.f;
     float v[K], t[K];
     int i[K];
     float m = -kInf, tmax = -kInf;
+    // everything is asked for before anything is used
+    T sv[K], tv[K];
+    I iv[K];
+    float tf[K];
+    if constexpr (G == 1) {
+      load_values<T, K>(s, a.classes, whole_s, sv);
+      load_values<I, K>(is, top, whole_i, iv);
+      if constexpr (SAME) load_values<T, K>(static_cast<const T*>(a.teacher) + r * a.t_stride, top, whole_t, tv);
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int j = k * G + l.lane;
+        if (j < a.classes) sv[k] = s[j];
+        if (j < top) iv[k] = is[j];
+        if (SAME && j < top) tv[k] = static_cast<const T*>(a.teacher)[r * a.t_stride + j];
+      }
+    }
+    if constexpr (!SAME) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (k * G + l.lane < top) tf[k] = teacher_of(a, r, k * G + l.lane);
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int j = k * G + l.lane;
-      v[k] = j < a.classes ? to_f32(s[j]) : -kInf;
-      i[k] = j < top ? index_of(a, r, j) : -1;
-      t[k] = i[k] >= 0 ? teacher_of(a, r, j) : -kInf;
+      v[k] = j < a.classes ? to_f32(sv[k]) : -kInf;
+      i[k] = j < top && iv[k] >= 0 && iv[k] < a.classes ? (int)iv[k] : -1;
+      if constexpr (SAME) t[k] = i[k] >= 0 ? to_f32(tv[k]) : -kInf;
+      else t[k] = i[k] >= 0 ? tf[k] : -kInf;
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -150,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) distill_small_kernel(DistillArgs a) 
     }
     sum = FWD ? l.sum(sum) : a.stats[2 * r + 1];
     tsum = l.sum(tsum);
-    const float ts = 1.f / tsum;
+    const float ts = rcp(tsum);
     float p[K], hit[K];  // each entry's p; each class's sum of them
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -196,10 +244,17 @@ __global__ void __launch_bounds__(kThreads) distill_small_kernel(DistillArgs a) 
       }
     }
     if (a.dlogits) {
-      const float coef = w * a.tau * (a.grad ? a.grad[r * a.grad_stride] : 1.f), qs = 1.f / sum;
+      const float coef = w * a.tau * (a.grad ? a.grad[r * a.grad_stride] : 1.f), qs = rcp(sum);
+      Vec<T, K> out;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (k * G + l.lane < a.classes) ds[k * G + l.lane] = from_f32<T>(coef * (q[k] * qs - hit[k]));
+      for (int k = 0; k < K; ++k) out.v[k] = from_f32<T>(coef * (q[k] * qs - hit[k]));
+      if (whole_d) {
+        *reinterpret_cast<Vec<T, K>*>(ds) = out;
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (k * G + l.lane < a.classes) ds[k * G + l.lane] = out.v[k];
+      }
     }
   }
 }
@@ -318,7 +373,7 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slic
     else __syncthreads();
   };
   const int slice = G > 32 && slices > 1 ? (int)cluster_rank() : 0;
-  const float c2 = kLog2e / a.tau, inv_tau = 1.f / a.tau;
+  const float c2 = a.c2, inv_tau = a.inv_tau;
   const int top = (int)a.top;
   int flip = 0;
   for (long long r = (long long)(blockIdx.x / slices) * kRows + group; r < a.rows;
@@ -588,7 +643,7 @@ __global__ void __launch_bounds__(NS + 32, BLOCKS) distill_held_kernel(DistillAr
   const int slice = slices > 1 ? (int)cluster_rank() : 0;
   const int lane = threadIdx.x & 31;
   const bool entry_warp = threadIdx.x >= NS;
-  const float c2 = kLog2e / a.tau;
+  const float c2 = a.c2;
   const long long step = gridDim.x / slices;
   long long r = blockIdx.x / slices;
   int flip = 0;
@@ -722,7 +777,7 @@ __global__ void __launch_bounds__(NS + 32, BLOCKS) distill_held_kernel(DistillAr
     }
   } else {
     const int top = (int)a.top;
-    const float inv_tau = 1.f / a.tau;
+    const float inv_tau = a.inv_tau;
     // raw words of the row ahead
     long long index[kLaneTop];
     float teach[kLaneTop];
@@ -862,9 +917,16 @@ __global__ void __launch_bounds__(NS + 32, BLOCKS) distill_held_kernel(DistillAr
 }
 
 template <class T, int G, int K, bool FWD>
-int32_t launch_small(const DistillArgs& a, cudaStream_t s) {
+int32_t launch_small(const DistillArgs& a, bool same, cudaStream_t s) {
   const long long blocks = (a.rows + kThreads / G - 1) / (kThreads / G);
-  distill_small_kernel<T, G, K, FWD><<<(unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)), kThreads, 0, s>>>(a);
+  const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);  // several rows a thread pay its set-up
+  const auto run = [&](auto index) {
+    using I = decltype(index);
+    if (same) distill_small_kernel<T, I, G, K, true, FWD><<<grid, kThreads, 0, s>>>(a);
+    else distill_small_kernel<T, I, G, K, false, FWD><<<grid, kThreads, 0, s>>>(a);
+  };
+  if (a.index_bits == 32) run(int{});
+  else run((long long){});
   return launch_status();
 }
 
@@ -938,9 +1000,11 @@ template <bool FWD>
 int32_t dispatch(const NcaDistillDesc& d, const DistillArgs& a, cudaStream_t s) {
   return with_dtype(d.dtype, [&](auto t) {
     using T = decltype(t);
-    if (a.classes <= 4 && a.top <= 4) return launch_small<T, 1, 4, FWD>(a, s);
-    if (a.classes <= 16 && a.top <= 16) return launch_small<T, 4, 4, FWD>(a, s);
-    if (a.classes <= 64 && a.top <= 64) return launch_small<T, 8, 8, FWD>(a, s);
+    const bool same = d.dtype == d.teacher_dtype;
+    if (a.classes <= 2 && a.top <= 2) return launch_small<T, 1, 2, FWD>(a, same, s);
+    if (a.classes <= 4 && a.top <= 4) return launch_small<T, 1, 4, FWD>(a, same, s);
+    if (a.classes <= 16 && a.top <= 16) return launch_small<T, 4, 4, FWD>(a, same, s);
+    if (a.classes <= 64 && a.top <= 64) return launch_small<T, 8, 8, FWD>(a, same, s);
     if (a.classes <= 2048 && a.top <= 512) return launch_rows<T, 32, 256, FWD>(a, 1, s);
     const size_t bytes = a.classes * sizeof(T);
     constexpr size_t kSmall = 96 * kHeld * 16, kMiddle = 256 * (kHeld + 8) * 16, kLarge = 992 * (kHeld + 9) * 16;
@@ -975,6 +1039,8 @@ DistillArgs args_of(const NcaDistillDesc& d, const void* logits, const void* tea
   a.teacher_dtype = d.teacher_dtype;
   a.index_bits = d.index_bits;
   a.tau = d.temperature;
+  a.c2 = kLog2e / d.temperature;
+  a.inv_tau = 1.f / d.temperature;
   a.s_stride = d.logits_stride;
   a.t_stride = d.teacher_stride;
   a.i_stride = d.index_stride;

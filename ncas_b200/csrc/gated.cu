@@ -16,8 +16,6 @@
 #include "gemm_rows.cuh"
 
 #include <algorithm>
-#include <cstdio>
-#include <cstdlib>
 #include <atomic>
 
 using namespace nca;
@@ -321,11 +319,6 @@ struct Shape {
   int splits;
 };
 Shape shape_of(long long m, long long n, int batch, long long kb, bool may_split, bool gate) {
-  if (getenv("GS")) {
-    int c = 2, w = 256, sp = 1;
-    sscanf(getenv("GS"), "%d,%d,%d", &c, &w, &sp);
-    return {c, w, may_split ? sp : 1};
-  }
   const long long sms = sm_count();
   const long long big = ceil_div(m, 256) * ceil_div(n, gate ? 128 : 256) * batch;
   if (big >= sms / 2) return {2, 256, 1};
@@ -414,8 +407,13 @@ int32_t rows_launch(RowsParams& p, cudaStream_t s) {
   }
   const long long tiles = ceil_div(p.n, kBM);
   if (tiles > (1ll << 27)) return NCA_ERR_UNSUPPORTED;
-  p.slices = 1;  // a power of two (it divides 128): two CTAs a multiprocessor, two k blocks a CTA at least
-  while (p.slices < 8 && tiles * p.slices * 2 <= 2 * sm_count() && p.kb >= 4 * p.slices) p.slices *= 2;
+  // a power of two (it divides 128): as many CTAs as run at once, two k blocks a CTA at least; clusters of
+  // 4 and 8 leave some multiprocessors of a processing cluster out
+  p.slices = 1;
+  const long long room = (long long)S::kBlocks * sm_count();
+  while (p.slices < 8 && p.kb >= 4 * p.slices &&
+         tiles * p.slices * 2 <= (p.slices == 1 ? room : p.slices == 2 ? room * 88 / 100 : room * 80 / 100))
+    p.slices *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * p.slices));
   cfg.blockDim = dim3(kRowsThreads);

@@ -8,7 +8,8 @@
 // shared memory, in the order of the pieces.  About 2 CTAs a multiprocessor, 100 KB of weights in flight
 // each: one output tile a CTA over the whole axis would leave most multiprocessors without work.
 // The second product is launched while the first runs (programmatic dependent launch) and loads its
-// weights before it waits for h.
+// weights before it waits for h.  (Prefetching them into L2 from the first took 2 us
+// longer in all: its own loads have the bandwidth.)
 #pragma once
 #include "gemm.cuh"
 
@@ -37,8 +38,9 @@ struct RowsShape {
   static constexpr int kWBytes = kAcc * kBM * kBK * 2;
   static constexpr int kXBytes = N * kBK * 2;
   static constexpr int kStageBytes = kWBytes + kXBytes;
-  static constexpr int kSums = kAcc * kBM * N * (int)sizeof(float);  // [slice][acc][rows of the share][N]
-  static constexpr int kBlocks = N == 64 ? 1 : 2;  // CTAs a multiprocessor
+  static constexpr int kRow = N + 4;  // floats: lanes that read a column meet few banks twice
+  static constexpr int kSums = kAcc * kBM * kRow * (int)sizeof(float);  // [slice][acc][rows of the share][kRow]
+  static constexpr int kBlocks = GATE && N == 64 ? 1 : 2;  // CTAs a multiprocessor
   static constexpr int kStages = (220 * 1024 / kBlocks - 2048 - kSums) / kStageBytes;
   static constexpr int kSumsAt = kStages * kStageBytes;
   static constexpr int kBars = kSumsAt + kSums;
@@ -143,7 +145,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
           uint32_t r[16];
           tmem_ld16(tmem + a * N + c + ((uint32_t)(32 * q) << 16), r);
           tc_wait_ld_regs(r);
-          float* mine = sums + ((rank * S::kAcc + a) * share + at) * N + c;
+          float* mine = sums + ((rank * S::kAcc + a) * share + at) * S::kRow + c;
           if (p.slices > 1) {
             const uint32_t far = map_to_rank(smem_u32(mine), to);
 #pragma unroll
@@ -174,7 +176,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
 #pragma unroll
     for (int a = 0; a < S::kAcc; ++a) {
       v[a] = 0.f;
-      for (int s = 0; s < p.slices; ++s) v[a] += sums[((s * S::kAcc + a) * share + at) * N + t];
+      for (int s = 0; s < p.slices; ++s) v[a] += sums[((s * S::kAcc + a) * share + at) * S::kRow + t];
       if (p.bias[a]) v[a] += load_param(p.bias[a], p.bias_dtype, f);
     }
     float r = v[0];

@@ -127,7 +127,7 @@ HeldPlan plan_of(const NormArgs& a, int dtype, int width, bool backward) {
   // channels of a block: all of them, or fewer whole groups (64 adjacent bytes at least) when a sample
   // would need more than 8 blocks of 100 KB.  Beyond that the streaming kernels are faster: clusters of
   // 16 blocks that fill a multiprocessor each read 16 x 16384 x 512 bf16 at half their rate.
-  const size_t kFew = 72 * 1024, kTwo = 100 * 1024;
+  const size_t kFew = (backward ? 56 : 32) * 1024, kTwo = 100 * 1024;
   const auto bytes_of = [&](int g) { return (size_t)a.cells * g * a.per_group * size * tensors; };
   int groups = a.groups;
   while (bytes_of(groups) > kMaxSlices * kTwo || groups > kMaxGroups || groups * a.per_group / v > kMaxThreads) {
@@ -149,7 +149,10 @@ HeldPlan plan_of(const NormArgs& a, int dtype, int width, bool backward) {
   p.tx = p.cb / v;
   const long long ty_max = kMaxThreads / p.tx;
   long long iters = (p.slice_cells + ty_max - 1) / ty_max;
-  if (iters < 12) iters = p.slice_cells < 12 ? p.slice_cells : 12;
+  // 8000 9 x 9 boards of 64 fp32 channels and padded 59 x 59 mazes: 16 places a thread forward, 8 backward
+  // (more threads hide the latency of a block's few steps, fewer share the cost of its sums)
+  const long long least = backward ? 8 : 16;
+  if (iters < least) iters = std::min<long long>(p.slice_cells, least);
   p.ty = (int)((p.slice_cells + iters - 1) / iters);
   p.iters = (int)((p.slice_cells + p.ty - 1) / p.ty);
   p.threads = (p.tx * p.ty + 31) / 32 * 32;
