@@ -171,12 +171,38 @@ __device__ __forceinline__ Vec<T, V> from_pairs(const float2 (&f)[(V + 1) / 2]) 
   return v;
 }
 
+// ------------------------------------------------------------------- programmatic dependent launch
+// A kernel launched by launch_after() may start while the kernel before it in the stream ends: it sets
+// itself up, and after after_previous() everything that ran before is complete and visible.  Every
+// such kernel calls both: may_start_next() early, after_previous() before its first access to memory.
+__device__ __forceinline__ void may_start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ------------------------------------------------------------------------------------ host side
 inline int32_t launch_status() {
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return NCA_OK;
   return e == cudaErrorNoKernelImageForDevice || e == cudaErrorInvalidDeviceFunction ? NCA_ERR_DEVICE
                                                                                     : NCA_ERR_CUDA;
+}
+template <class... P, class... A>
+int32_t launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, int cluster, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  const int32_t st = launch_status();
+  return e == cudaSuccess || st != NCA_OK ? st : NCA_ERR_CUDA;
 }
 inline size_t dtype_size(int dtype) { return dtype == NCA_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype >= NCA_F32 && dtype <= NCA_F16; }

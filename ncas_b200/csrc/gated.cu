@@ -141,6 +141,8 @@ __device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int m) 
                     __funnelshift_r(v[2], v[3], bits), __funnelshift_r(v[3], v[4], bits));
 }
 __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs all) {
+  may_start_next();
+  after_previous();
   __shared__ uint16_t tile[32][34];
   const Pack& p = all.p[blockIdx.y];
   if (p.sc == 1) {  // rows of adjacent values: a warp a row, 8 a lane
@@ -187,6 +189,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs
 template <class T>
 __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int batch, long long m, long long n,
                                                    long long ldp, T* c0, T* c1) {
+  may_start_next();
+  after_previous();
   __shared__ float4 red[8][32];
   const long long total = batch * m * ldp / 4, i = (long long)blockIdx.x * 32 + threadIdx.x;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -225,6 +229,8 @@ constexpr int kSumSplits = 256;
 template <class T>
 __global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant__ ColumnSums p, long long rows,
                                                           int splits) {
+  may_start_next();
+  after_previous();
   __shared__ float2 red[8][32][4];
   const int z = blockIdx.z;
   const long long c = 8 * ((long long)blockIdx.x * 32 + threadIdx.x), cols = p.cols[z], padded = (cols + 7) / 8 * 8;
@@ -261,6 +267,8 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant_
   }
 }
 __global__ void __launch_bounds__(512) column_store_kernel(const __grid_constant__ ColumnSums p, int splits, int dtype) {
+  may_start_next();
+  after_previous();
   __shared__ float red[16][33];
   const int z = blockIdx.z;
   const long long c = (long long)blockIdx.x * 32 + threadIdx.x, cols = p.cols[z], padded = (cols + 7) / 8 * 8;
@@ -294,22 +302,7 @@ int32_t launch(GemmParams& p, cudaStream_t s) {
   const long long tiles = (long long)p.m_tiles * p.n_tiles * p.batch * p.splits;
   if (tiles > (1ll << 31) - 1024) return NCA_ERR_UNSUPPORTED;
   const long long room = sm_count() / CG;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((tiles < room ? tiles : room) * CG));
-  cfg.blockDim = dim3(kGemmThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = CG > 1 ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
-    cudaGetLastError();
-    return NCA_ERR_CUDA;
-  }
-  return launch_status();
+  return launch_after(kernel, dim3((unsigned)((tiles < room ? tiles : room) * CG)), dim3(kGemmThreads), S::kSmem, s, CG, p);
 }
 
 // Pairs of multiprocessors (256 x 256 tiles) when their tiles occupy the GPU, single ones
@@ -382,9 +375,8 @@ int32_t weight_product(GemmParams& p, const Product& g, int dtype, void* c0, voi
   const int32_t st = product<T, true, true, EPI_PARTIAL, NCA_ACT_NONE>(p, g, dtype, sh, s);
   if (st != NCA_OK) return st;
   const long long total = g.batch * g.m * ldp / 4;
-  join_kernel<T><<<(unsigned)ceil_div(total, 32), dim3(32, 8), 0, s>>>(
-      part, sh.splits, g.batch, g.m, g.n, ldp, static_cast<T*>(c0), static_cast<T*>(c1));
-  return launch_status();
+  return launch_after(join_kernel<T>, dim3((unsigned)ceil_div(total, 32)), dim3(32, 8), 0, s, 1, part, sh.splits, g.batch,
+                      g.m, g.n, ldp, static_cast<T*>(c0), static_cast<T*>(c1));
 }
 size_t weight_part_bytes(long long m, long long n, int batch, long long rows) {
   const Shape sh = shape_of(m, n, batch, ceil_div(rows, kBK), true, false);
@@ -414,28 +406,11 @@ int32_t rows_launch(RowsParams& p, cudaStream_t s) {
   while (p.slices < 8 && p.kb >= 4 * p.slices &&
          tiles * p.slices * 2 <= (p.slices == 1 ? room : p.slices == 2 ? room * 88 / 100 : room * 80 / 100))
     p.slices *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * p.slices));
-  cfg.blockDim = dim3(kRowsThreads);
-  cfg.dynamicSmemBytes = S::kSmem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.slices;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.wait ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, p) != cudaSuccess) {
-    cudaGetLastError();
-    return NCA_ERR_CUDA;
-  }
-  return launch_status();
+  return launch_after(kernel, dim3((unsigned)(tiles * p.slices)), dim3(kRowsThreads), S::kSmem, s, p.slices, p);
 }
 template <class T, bool GATE, int ACT>
 int32_t rows_product(const GemmParams& base, const Matrix& x, const Matrix& w0, const Matrix& w1, const void* b0,
-                     const void* b1, void* out, long long ld, bool wait, int dtype, cudaStream_t s) {
+                     const void* b1, void* out, long long ld, bool weights_first, int dtype, cudaStream_t s) {
   RowsParams p{};
   const int n = x.rows <= 16 ? 16 : x.rows <= 32 ? 32 : 64;
   if (!encode(&p.x, x, dtype, n) || !encode(&p.w[0], w0, dtype, kBM) || (GATE && !encode(&p.w[1], w1, dtype, kBM)))
@@ -443,7 +418,7 @@ int32_t rows_product(const GemmParams& base, const Matrix& x, const Matrix& w0, 
   p.rows = (int)x.rows;
   p.n = (int)w0.rows;
   p.kb = (int)ceil_div(x.cols, kBK);
-  p.wait = wait;
+  p.weights_first = weights_first;
   p.out = out;
   p.ld = ld;
   p.bias[0] = b0;
@@ -541,8 +516,7 @@ struct Operands {
   }
   int32_t copy(cudaStream_t s) const {
     if (count == 0) return NCA_OK;
-    pack_kernel<<<dim3((unsigned)std::min<long long>(most, 148 * 8), count), dim3(32, 8), 0, s>>>(packs);
-    return launch_status();
+    return launch_after(pack_kernel, dim3((unsigned)std::min<long long>(most, 148 * 8), count), dim3(32, 8), 0, s, 1, packs);
   }
 };
 
@@ -663,9 +637,10 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
   add(mdu, db_up);
   add(mdy, db_down);
   if (count) {
-    column_sums_kernel<T><<<dim3((unsigned)ceil_div(widest, 256), splits, count), dim3(32, 8), 0, s>>>(sums, d.rows, splits);
-    column_store_kernel<<<dim3((unsigned)ceil_div(widest, 32), 1, count), dim3(32, 16), 0, s>>>(sums, splits, d.bias_dtype);
-    return launch_status();
+    NCA_TRY(launch_after(column_sums_kernel<T>, dim3((unsigned)ceil_div(widest, 256), splits, count), dim3(32, 8), 0, s, 1,
+                         sums, d.rows, splits));
+    return launch_after(column_store_kernel, dim3((unsigned)ceil_div(widest, 32), 1, count), dim3(32, 16), 0, s, 1, sums,
+                        splits, d.bias_dtype);
   }
   return NCA_OK;
 }

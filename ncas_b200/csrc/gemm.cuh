@@ -343,6 +343,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
     fence_mbar_init();
   }
   if (warp == 2) tc_alloc<CG>(tmem_base_s, S::kTmemCols);
+  may_start_next();
+  after_previous();
   tc_fence_before();
   if constexpr (CG == 2) cluster_sync_all();
   else __syncthreads();

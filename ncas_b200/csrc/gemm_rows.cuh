@@ -21,7 +21,7 @@ struct RowsParams {
   int rows, n;       // rows of x, outputs
   int kb;            // k blocks of 64
   int slices;
-  int wait;          // x is written by the launch before
+  int weights_first; // the launch before writes x alone: the weights need not wait for it
   void* out;         // [rows][ld]
   long long ld;
   const void* bias[2];
@@ -64,7 +64,6 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
   const int rank = p.slices > 1 ? (int)cta_rank_in_cluster() : 0;
   const int tile = blockIdx.x / p.slices;
   const FailState fs{p.ctrl, abort_s, 0, p.timeout_ns};
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
@@ -94,8 +93,17 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
         tma_load_2d<1>(smem_u32(smem + s * S::kStageBytes) + S::kWBytes, &p.x, smem_u32(&full[s]), kb * kBK, 0);
       };
       const int n = kb1 - kb0, ahead = n < S::kStages ? n : S::kStages;
+      // The next launch may load its weights before this one ends, so it must not start before all that
+      // ran ahead of this one (which may have written them) has ended: only after after_previous().
+      if (!p.weights_first) {
+        after_previous();
+        may_start_next();
+      }
       for (int i = 0; i < ahead; ++i) load_w(i, kb0 + i);
-      if (p.wait) asm volatile("griddepcontrol.wait;" ::: "memory");
+      if (p.weights_first) {
+        after_previous();
+        may_start_next();
+      }
       for (int i = 0; i < ahead; ++i) load_x(i, kb0 + i);
       int i = ahead;
       for (; i < n; ++i) {
@@ -167,6 +175,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
   else __syncthreads();
   tc_fence_after();
   if (warp == 1) tc_dealloc<1>(tmem, S::kTmemCols);
+  after_previous();  // every thread that writes
   // this CTA's share of the outputs, every row
   const int share = kBM / p.slices, first = tile * kBM + rank * share;
   for (int i = threadIdx.x; i < share * p.rows; i += kRowsThreads) {

@@ -131,6 +131,8 @@ __device__ __forceinline__ void each_cell(const NormArgs& a, const Place& p, voi
 // ------------------------------------------------------------------------- forward: statistics
 template <class T, int V, bool MASK>
 __global__ void __launch_bounds__(kThreads) norm_stats_kernel(NormArgs a, long long items) {
+  may_start_next();
+  after_previous();
   constexpr int P = (V + 1) / 2;
   extern __shared__ float2 red[];  // the ring; after it [ty][tx * V] (mean, M2), then [ty] counts
   int* rc = reinterpret_cast<int*>(red + a.ty * a.tx * V);
@@ -222,6 +224,8 @@ __device__ __forceinline__ float block_sum(float v, float* red) {  // in every t
 }
 
 __global__ void __launch_bounds__(kMergeThreads) norm_stats_merge_kernel(NormArgs a) {
+  may_start_next();
+  after_previous();
   __shared__ float red[kMergeThreads / 32];
   for (long long w = blockIdx.x; w < a.n * a.groups; w += gridDim.x) {
     const long long sample = w / a.groups;
@@ -288,6 +292,8 @@ __device__ __forceinline__ void write_zeros(T* to) {
 
 template <class T, int V, int ACT, bool MASK, bool ONE>
 __global__ void __launch_bounds__(kThreads, 4) norm_apply_kernel(NormArgs a, long long items) {
+  may_start_next();
+  after_previous();
   constexpr int P = (V + 1) / 2;
   extern __shared__ uint4 ring[];
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
@@ -316,6 +322,8 @@ __global__ void __launch_bounds__(kThreads, 4) norm_apply_kernel(NormArgs a, lon
 // ---------------------------------------------------------------------------------- backward
 template <class T, int V, int ACT, bool MASK, bool ONE>
 __global__ void __launch_bounds__(kThreads, 3) norm_grad_sums_kernel(NormArgs a, long long items) {
+  may_start_next();
+  after_previous();
   constexpr int P = (V + 1) / 2;
   extern __shared__ float2 red[];  // the ring; after it [ty][tx * V] (sum dz, sum dz h), then [ty] counts
   int* rc = reinterpret_cast<int*>(red + a.ty * a.tx * V);
@@ -374,6 +382,8 @@ __global__ void __launch_bounds__(kThreads, 3) norm_grad_sums_kernel(NormArgs a,
 
 // A / n and B / n of every (sample, group).
 __global__ void __launch_bounds__(kMergeThreads) norm_grad_merge_kernel(NormArgs a) {
+  may_start_next();
+  after_previous();
   __shared__ float red[kMergeThreads / 32];
   for (long long w = blockIdx.x; w < a.n * a.groups; w += gridDim.x) {
     const long long sample = w / a.groups;
@@ -396,6 +406,8 @@ __global__ void __launch_bounds__(kMergeThreads) norm_grad_merge_kernel(NormArgs
 
 template <class T, int V, int ACT, bool MASK, bool ONE>
 __global__ void __launch_bounds__(kThreads, 3) norm_grad_apply_kernel(NormArgs a, long long items) {
+  may_start_next();
+  after_previous();
   constexpr int P = (V + 1) / 2;
   extern __shared__ uint4 ring[];
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
@@ -440,6 +452,8 @@ __global__ void __launch_bounds__(kThreads, 3) norm_grad_apply_kernel(NormArgs a
 // x 8 rows) s sums the rows of its split, then one block a channel tile sums the splits.
 __global__ void norm_param_sums_kernel(const float2* part, long long rows, int channels, int splits,
                                        float2* out) {
+  may_start_next();
+  after_previous();
   __shared__ float2 red[8][32];
   const int ch = blockIdx.x * 32 + threadIdx.x;
   const int split = blockIdx.y;
@@ -461,6 +475,8 @@ __global__ void norm_param_sums_kernel(const float2* part, long long rows, int c
 }
 __global__ void norm_param_store_kernel(const float2* part, int splits, int channels, void* dweight,
                                         void* dbias, int param_dtype) {
+  may_start_next();
+  after_previous();
   __shared__ float2 red[16][32];
   const int ch = blockIdx.x * 32 + threadIdx.x;
   float2 s = make_float2(0.f, 0.f);
@@ -598,12 +614,14 @@ long long plan(const NcaNormDesc& d, NormArgs& a, int v) {
 
 inline unsigned grid_of(long long items) { return (unsigned)(items < (1 << 20) ? items : (1 << 20)); }
 
-void param_grads(const float2* part, long long rows, int channels, void* dweight, void* dbias, int param_dtype,
-                 float2* params, cudaStream_t s) {
+int32_t param_grads(const float2* part, long long rows, int channels, void* dweight, void* dbias, int param_dtype,
+                    float2* params, cudaStream_t s) {
   const int splits = (int)(rows < 8 * kParamSplits ? (rows + 7) / 8 : kParamSplits);
-  norm_param_sums_kernel<<<dim3((channels + 31) / 32, splits), dim3(32, 8), 0, s>>>(part, rows, channels, splits,
-                                                                                 params);
-  norm_param_store_kernel<<<(channels + 31) / 32, dim3(32, 16), 0, s>>>(params, splits, channels, dweight, dbias, param_dtype);
+  const int32_t st = launch_after(norm_param_sums_kernel, dim3((channels + 31) / 32, splits), dim3(32, 8), 0, s, 1, part,
+                                  rows, channels, splits, params);
+  if (st != NCA_OK) return st;
+  return launch_after(norm_param_store_kernel, dim3((channels + 31) / 32), dim3(32, 16), 0, s, 1, params, splits, channels,
+                      dweight, dbias, param_dtype);
 }
 
 // Raises a kernel's shared-memory limit once a device, and launches it.
@@ -619,8 +637,7 @@ int32_t launch(void (*kernel)(NormArgs, long long), std::atomic<uint64_t>& ready
     }
     ready.fetch_or(1ull << dev, std::memory_order_release);
   }
-  kernel<<<grid_of(items), a.tx * a.ty, smem, s>>>(a, items);
-  return launch_status();
+  return launch_after(kernel, dim3(grid_of(items)), dim3(a.tx * a.ty), smem, s, 1, a, items);
 }
 // Shared memory of a kernel that leaves partial results: the ring, or those where they are more.
 template <class T, int V>
@@ -638,7 +655,7 @@ int32_t forward(const NcaNormDesc& d, NormArgs a, cudaStream_t s) {
   static std::atomic<uint64_t> ready[2];
   const long long items = plan(d, a, V);
   NCA_TRY(launch(norm_stats_kernel<T, V, MASK>, ready[0], a, items, sums_smem<T, V>(a, 1), s));
-  norm_stats_merge_kernel<<<grid_of(a.n * a.groups), kMergeThreads, 0, s>>>(a);
+  NCA_TRY(launch_after(norm_stats_merge_kernel, dim3(grid_of(a.n * a.groups)), dim3(kMergeThreads), 0, s, 1, a));
   return launch(norm_apply_kernel<T, V, ACT, MASK, ONE>, ready[1], a, items, ring_bytes<T, V>(1), s);
 }
 
@@ -649,11 +666,11 @@ int32_t backward(const NcaNormDesc& d, NormArgs a, void* dweight, void* dbias, f
   const long long items = plan(d, a, V);
   NCA_TRY(launch(norm_grad_sums_kernel<T, V, ACT, MASK, ONE>, ready[0], a, items, sums_smem<T, V>(a, 2), s));
   if (a.y) {
-    norm_grad_merge_kernel<<<grid_of(a.n * a.groups), kMergeThreads, 0, s>>>(a);
+    NCA_TRY(launch_after(norm_grad_merge_kernel, dim3(grid_of(a.n * a.groups)), dim3(kMergeThreads), 0, s, 1, a));
     NCA_TRY(launch(norm_grad_apply_kernel<T, V, ACT, MASK, ONE>, ready[1], a, items, ring_bytes<T, V>(2), s));
   }
-  if (dweight || dbias) param_grads(a.part, a.n * a.chunks, a.channels, dweight, dbias, a.param_dtype, params, s);
-  return launch_status();
+  if (!dweight && !dbias) return NCA_OK;
+  return param_grads(a.part, a.n * a.chunks, a.channels, dweight, dbias, a.param_dtype, params, s);
 }
 
 // Instantiates fn(T, V, ACT) for the run-time choice.
@@ -775,8 +792,7 @@ int32_t nca_b200_group_norm_backward(const NcaNormDesc* d, const void* x, const 
     if (!dweight && !dbias) a.part = nullptr;
     const int32_t r = norm_held_backward(a, d->dtype, d->act, c.v, s);
     if (r != NCA_OK || !a.part) return r;
-    param_grads(a.part, a.n * c.held, a.channels, dweight, dbias, a.param_dtype, params, s);
-    return launch_status();
+    return param_grads(a.part, a.n * c.held, a.channels, dweight, dbias, a.param_dtype, params, s);
   }
   return dispatch(*d, streaming_width(d->dtype, c.v), BackwardCall{*d, a, dweight, dbias, params, s});
 }

@@ -180,22 +180,7 @@ int32_t launch(void (*kernel)(HeldArgs), std::atomic<uint64_t>& ready, const Nor
   HeldArgs h{a, p.cb, p.cblocks, p.slices, p.slice_cells, p.iters};
   h.a.tx = p.tx;
   h.a.ty = p.ty;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.n * p.cblocks * p.slices));
-  cfg.blockDim = dim3(p.threads);
-  cfg.dynamicSmemBytes = p.smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.slices;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.slices > 1 ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, kernel, h) != cudaSuccess) {
-    const int32_t st = launch_status();
-    return st == NCA_OK ? NCA_ERR_CUDA : st;
-  }
-  return launch_status();
+  return launch_after(kernel, dim3((unsigned)(a.n * p.cblocks * p.slices)), dim3(p.threads), p.smem, s, p.slices, h);
 }
 
 

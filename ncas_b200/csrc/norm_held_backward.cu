@@ -23,6 +23,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(cons
   float2* red = reinterpret_cast<float2*>(gs + h.iters * threads);  // [ty][tx * V] (sum dz, sum dz h)
   float2* chan = red + a.ty * a.tx * V;                             // [cb] totals of the block
   int* count = reinterpret_cast<int*>(chan + h.cb);                 // [ty] cells of a row of threads
+  may_start_next();
+  after_previous();
   const Work w = work_of<V>(h);
   const uint32_t kept = kept_of<MASK>(a, w);
   {

@@ -10,6 +10,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_forward_kernel(const
   const NormArgs& a = h.a;
   extern __shared__ uint4 smem_raw[];
   using VecT = Vec<T, V>;
+  may_start_next();
+  after_previous();
   const Work w = work_of<V>(h);
   const uint32_t kept = kept_of<MASK>(a, w);
   const int threads = blockDim.x, groups = h.cb / a.per_group;
