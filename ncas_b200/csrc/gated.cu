@@ -115,7 +115,8 @@ bool set_out(GemmParams& p, int dtype, void* c0, void* c1, long long rows, long 
   p.c[1] = c1;
   p.ldc = cols;
   p.plain_c = cols % 8 != 0 || reinterpret_cast<uintptr_t>(c0) % 16 != 0 || reinterpret_cast<uintptr_t>(c1) % 16 != 0;
-  return p.plain_c || (encode_out(&p.out[0], c0, dtype, rows, cols, cols) && encode_out(&p.out[1], c1, dtype, rows, cols, cols));
+  return p.plain_c || (encode_out(&p.out[0], c0, dtype, rows, cols, cols) &&
+                        (c1 == c0 || encode_out(&p.out[1], c1, dtype, rows, cols, cols)));
 }
 
 // ------------------------------------------------------------------------------- small kernels
@@ -184,11 +185,11 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packs
   }
 }
 
-// c[z][m][n] = sum over the pieces of part[s * batch + z][m][n]: 32 lanes of 4 columns by 8 groups of
+// c[z][m][n] = bias[n] + sum over the pieces of part[s * batch + z][m][n]: 32 lanes of 4 columns by 8 groups of
 // pieces, which add up in the order of the groups.
 template <class T>
 __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int batch, long long m, long long n,
-                                                   long long ldp, T* c0, T* c1) {
+                                                   long long ldp, T* c0, T* c1, const void* bias, int bias_dtype) {
   may_start_next();
   after_previous();
   __shared__ float4 red[8][32];
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits
   const float f[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    if (c + j < n) to[j] = from_f32<T>(f[j]);
+    if (c + j < n) to[j] = from_f32<T>(f[j] + (bias ? load_param(bias, bias_dtype, c + j) : 0.f));
 }
 
 // Column sums of up to three [rows][cols] matrices (blockIdx.z) in two steps of a fixed order: the rows
@@ -305,24 +306,39 @@ int32_t launch(GemmParams& p, cudaStream_t s) {
   return launch_after(kernel, dim3((unsigned)((tiles < room ? tiles : room) * CG)), dim3(kGemmThreads), S::kSmem, s, CG, p);
 }
 
-// Pairs of multiprocessors (256 x 256 tiles) when their tiles occupy the GPU, single ones
-// (128 x 128 tiles) otherwise.
+// Tiles and pieces of a product m x n over kb k blocks (`batch` of them).  A k block costs a 256 x 256 tile
+// of a pair of multiprocessors 0.28 us (the MMAs), a 256 x 128 tile 0.24 and a 128 x 128 tile of one
+// 0.25 (64 bytes a cycle from L2), a tile 5 us besides, and a product in pieces 3 us and 20 bytes of
+// traffic an output and piece more.  The smallest sum wins; measured on 2000 x 1008 x 5472: 33, 30 and
+// 32 us in one piece.
 struct Shape {
   int cg, bn;
   int splits;
 };
 Shape shape_of(long long m, long long n, int batch, long long kb, bool may_split, bool gate) {
+  static const struct {
+    int cg, bn;
+    double us;
+  } kinds[] = {{2, 256, 0.28}, {2, 128, 0.24}, {1, 128, 0.25}};
   const long long sms = sm_count();
-  const long long big = ceil_div(m, 256) * ceil_div(n, gate ? 128 : 256) * batch;
-  if (big >= sms / 2) return {2, 256, 1};
-  if (may_split && kb >= 64 && big * kb >= sms / 2 * 16) {
-    const long long s = std::max(1ll, std::min(sms / 2 / big, kb / 16));
-    return {2, 256, (int)s};
+  Shape best{2, 256, 1};
+  double least = 1e30;
+  for (const auto& k : kinds) {
+    const long long tiles = ceil_div(m, 128 * k.cg) * ceil_div(n, gate ? k.bn / 2 : k.bn) * batch;
+    const long long room = sms / k.cg;
+    if (tiles == 0) return best;  // no rows
+    const long long most = may_split ? std::max(1ll, std::min(room / tiles, kb / 8)) : 1;
+    for (long long s = 1; s <= most; s = s < most && 2 * s > most ? most : 2 * s) {
+      const double waves = (double)ceil_div(tiles * s, room);
+      double us = waves * ((double)ceil_div(kb, s) * k.us + 1.0) + 4.0;
+      if (s > 1) us += 3.0 + 1e6 * 20.0 * s * batch * m * n / 6.4e12;
+      if (us < least) {
+        least = us;
+        best = {k.cg, k.bn, (int)s};
+      }
+    }
   }
-  const long long small = ceil_div(m, 128) * ceil_div(n, gate ? 64 : 128) * batch;
-  long long s = 1;
-  if (may_split) s = std::max(1ll, std::min(sms / small, kb / 8));
-  return {1, 128, (int)s};
+  return best;
 }
 
 struct Product {
@@ -335,12 +351,12 @@ struct Product {
 
 int32_t set_up(GemmParams& p, const Product& g, int dtype, bool a_mn, bool b_mn, int cg, int bn, bool gate) {
   const int bnc = gate ? bn / 2 : bn / cg;
-  for (int i = 0; i < 2; ++i) {
-    const Matrix& a = i && g.two_a ? g.a[1] : g.a[0];
-    const Matrix& b = i && g.two_b ? g.b[1] : g.b[0];
-    if (!encode(&p.a[i], a, dtype, a_mn ? 64 : kBM) || !encode(&p.b[i], b, dtype, b_mn ? 64 : bnc))
-      return NCA_ERR_CUDA;
-  }
+  if (!encode(&p.a[0], g.a[0], dtype, a_mn ? 64 : kBM) || !encode(&p.b[0], g.b[0], dtype, b_mn ? 64 : bnc) ||
+      (g.two_a && !encode(&p.a[1], g.a[1], dtype, a_mn ? 64 : kBM)) ||
+      (g.two_b && !encode(&p.b[1], g.b[1], dtype, b_mn ? 64 : bnc)))
+    return NCA_ERR_CUDA;
+  if (!g.two_a) p.a[1] = p.a[0];
+  if (!g.two_b) p.b[1] = p.b[0];
   p.m = (int)g.m;
   p.n = (int)g.n;
   p.batch = g.batch;
@@ -360,26 +376,29 @@ int32_t product(GemmParams& p, const Product& g, int dtype, const Shape& sh, cud
   return sh.bn == 128 ? launch<T, 2, 128, A_MN, B_MN, EPI, ACT>(p, s) : launch<T, 2, 256, A_MN, B_MN, EPI, ACT>(p, s);
 }
 
-// The weight gradient dW[batch] (m x n) = A^T B over the rows, through partial sums when split.
-template <class T>
-int32_t weight_product(GemmParams& p, const Product& g, int dtype, void* c0, void* c1, float* part, cudaStream_t s) {
-  const Shape sh = shape_of(g.m, g.n, g.batch, ceil_div(g.k, kBK), true, false);
+// A product whose outputs are stored as they are (plus a bias), through partial sums when its k axis is cut.
+template <class T, bool A_MN, bool B_MN>
+int32_t stored_product(GemmParams& p, const Product& g, int dtype, void* c0, void* c1, const void* bias, float* part,
+                       cudaStream_t s) {
+  const long long kb = ceil_div(g.k, kBK) * (g.k_sources ? 2 : 1);
+  const Shape sh = shape_of(g.m, g.n, g.batch, kb, true, false);
   if (sh.splits == 1) {
+    p.bias[0] = bias;
     if (!set_out(p, dtype, c0, c1, g.m, g.n)) return NCA_ERR_CUDA;
-    return product<T, true, true, EPI_STORE, NCA_ACT_NONE>(p, g, dtype, sh, s);
+    return product<T, A_MN, B_MN, EPI_STORE, NCA_ACT_NONE>(p, g, dtype, sh, s);
   }
   const long long ldp = (g.n + 3) / 4 * 4;
   if (!encode_boxes(&p.out[0], part, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, g.n, g.m, ldp, 3, (long long)sh.splits * g.batch,
                     g.m * ldp * 4))
     return NCA_ERR_CUDA;
-  const int32_t st = product<T, true, true, EPI_PARTIAL, NCA_ACT_NONE>(p, g, dtype, sh, s);
+  const int32_t st = product<T, A_MN, B_MN, EPI_PARTIAL, NCA_ACT_NONE>(p, g, dtype, sh, s);
   if (st != NCA_OK) return st;
   const long long total = g.batch * g.m * ldp / 4;
   return launch_after(join_kernel<T>, dim3((unsigned)ceil_div(total, 32)), dim3(32, 8), 0, s, 1, part, sh.splits, g.batch,
-                      g.m, g.n, ldp, static_cast<T*>(c0), static_cast<T*>(c1));
+                      g.m, g.n, ldp, static_cast<T*>(c0), static_cast<T*>(c1), bias, p.bias_dtype);
 }
-size_t weight_part_bytes(long long m, long long n, int batch, long long rows) {
-  const Shape sh = shape_of(m, n, batch, ceil_div(rows, kBK), true, false);
+size_t part_bytes(long long m, long long n, int batch, long long k, int sources) {
+  const Shape sh = shape_of(m, n, batch, ceil_div(k, kBK) * sources, true, false);
   return sh.splits == 1 ? 0 : (size_t)sh.splits * batch * m * ((n + 3) / 4 * 4) * sizeof(float);
 }
 
@@ -478,15 +497,16 @@ Plan plan_of(const NcaGatedDesc& d, bool backward) {
   if (!backward) {
     p.h = at;
     at += tf;
+    p.part = at;
+    at += align256(part_bytes(d.rows, d.d_out, 1, d.hidden, 1));
   } else {
     p.dgate = at;
     at += tf;
     p.dup = at;
     at += tf;
     p.part = at;
-    at += align256(std::max({weight_part_bytes(d.hidden, d.d_in, 2, d.rows),
-                             weight_part_bytes(d.hidden, d.d_in, 1, d.rows),
-                             weight_part_bytes(d.d_out, d.hidden, 1, d.rows)}));
+    at += align256(std::max({part_bytes(d.rows, d.d_in, 1, d.hidden, 2), part_bytes(d.hidden, d.d_in, 2, d.rows, 1),
+                             part_bytes(d.hidden, d.d_in, 1, d.rows, 1), part_bytes(d.d_out, d.hidden, 1, d.rows, 1)}));
     p.sums = at;
     at += align256((size_t)kSumSplits * (2 * p.fp + pad8(d.d_out)) * sizeof(float));
   }
@@ -555,10 +575,7 @@ int32_t forward(const NcaGatedDesc& d, const void* x, const void* w_gate, const 
   GemmParams p = base;
   const Matrix mh{h, d.rows, d.hidden, pl.fp};
   Product g{{mh, mh}, {md, md}, false, false, d.rows, d.d_out, d.hidden, false, 1};
-  if (!set_out(p, d.dtype, y, y, d.rows, d.d_out)) return NCA_ERR_CUDA;
-  p.bias[0] = b_down;
-  return product<T, false, false, EPI_STORE, NCA_ACT_NONE>(
-      p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s);
+  return stored_product<T, false, false>(p, g, d.dtype, y, y, b_down, reinterpret_cast<float*>(ws + pl.part), s);
 }
 
 template <class T, int ACT>
@@ -596,26 +613,24 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
   if (dx) {
     GemmParams p = base;
     Product g{{mdg, mdu}, {mg, mu}, true, true, d.rows, d.d_in, d.hidden, true, 1};
-    if (!set_out(p, d.dtype, dx, dx, d.rows, d.d_in)) return NCA_ERR_CUDA;
-    NCA_TRY((product<T, false, true, EPI_STORE, NCA_ACT_NONE>(
-        p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s)));
+    NCA_TRY((stored_product<T, false, true>(p, g, d.dtype, dx, dx, nullptr, part, s)));
   }
   if (dw_gate || dw_up) {
     GemmParams p = base;
     if (dw_gate && dw_up) {
       Product g{{mdg, mdu}, {mx, mx}, true, false, d.hidden, d.d_in, d.rows, false, 2};
-      NCA_TRY(weight_product<T>(p, g, d.dtype, dw_gate, dw_up, part, s));
+      NCA_TRY((stored_product<T, true, true>(p, g, d.dtype, dw_gate, dw_up, nullptr, part, s)));
     } else {
       const Matrix& m = dw_gate ? mdg : mdu;
       void* out = dw_gate ? dw_gate : dw_up;
       Product g{{m, m}, {mx, mx}, false, false, d.hidden, d.d_in, d.rows, false, 1};
-      NCA_TRY(weight_product<T>(p, g, d.dtype, out, out, part, s));
+      NCA_TRY((stored_product<T, true, true>(p, g, d.dtype, out, out, nullptr, part, s)));
     }
   }
   if (dw_down) {
     GemmParams p = base;
     Product g{{mdy, mdy}, {mh, mh}, false, false, d.d_out, d.hidden, d.rows, false, 1};
-    NCA_TRY(weight_product<T>(p, g, d.dtype, dw_down, dw_down, part, s));
+    NCA_TRY((stored_product<T, true, true>(p, g, d.dtype, dw_down, dw_down, nullptr, part, s)));
   }
   ColumnSums sums{};
   int count = 0;

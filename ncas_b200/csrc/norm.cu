@@ -175,79 +175,94 @@ __global__ void __launch_bounds__(kThreads) norm_stats_kernel(NormArgs a, long l
     }
     if (col == 0) rc[row] = cnt;
     __syncthreads();
-    int total = 0;
-    for (int r = 0; r < a.ty; ++r) total += rc[r];
-    for (int i = threadIdx.x; i < a.tx * V; i += blockDim.x) {
-      const int ch = (int)(item % a.ctiles) * a.tx * V + i;
-      if (ch >= a.channels) break;
-      float mean = 0.f, m2 = 0.f;
-      for (int r = 0; r < a.ty; ++r) mean += rc[r] ? (float)rc[r] * red[r * a.tx * V + i].x : 0.f;
-      mean = total ? mean / (float)total : 0.f;
-      for (int r = 0; r < a.ty; ++r) {
+    // the rows of a channel: by one thread, or where there are many by the lanes of a warp
+    float2* part = a.part + (p.sample * a.chunks + p.chunk) * a.channels + (int)(item % a.ctiles) * a.tx * V;
+    const int width = min(a.tx * V, a.channels - (int)(item % a.ctiles) * a.tx * V);
+    const auto merged = [&](int i, int r0, int step, auto sum) {
+      float n = 0.f, mean = 0.f, m2 = 0.f;
+      for (int r = r0; r < a.ty; r += step) {
+        const float f = (float)rc[r];
+        n += f;
+        mean += rc[r] ? f * red[r * a.tx * V + i].x : 0.f;
+      }
+      n = sum(n);
+      mean = sum(mean);
+      mean = n > 0.f ? mean / n : 0.f;
+      for (int r = r0; r < a.ty; r += step) {
         const float2 e = red[r * a.tx * V + i];
         const float d = e.x - mean;
         m2 += rc[r] ? fmaf((float)rc[r] * d, d, e.y) : 0.f;
       }
-      a.part[(p.sample * a.chunks + p.chunk) * a.channels + ch] = make_float2(mean, m2);
+      m2 = sum(m2);
+      if (r0 == 0) {
+        part[i] = make_float2(mean, m2);
+        if (i == 0 && item % a.ctiles == 0) a.counts[p.sample * a.chunks + p.chunk] = (int)n;
+      }
+    };
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (a.ty > 16 && warps > 0) {
+      if ((int)threadIdx.x >> 5 < warps)
+        for (int i = threadIdx.x >> 5; i < width; i += warps) merged(i, lane, 32, [](float v) { return warp_sum(v); });
+    } else {
+      for (int i = threadIdx.x; i < width; i += blockDim.x) merged(i, 0, 1, [](float v) { return v; });
     }
-    if (threadIdx.x == 0 && item % a.ctiles == 0) a.counts[p.sample * a.chunks + p.chunk] = total;
     __syncthreads();  // the partial results have been read
   }
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// A block per (sample, group) goes through its chunks x per_group partial results: f(chunk, channel).
-constexpr int kMergeThreads = 256;
-template <class F>
+// L lanes (a warp, or a block of kMergeThreads) per (sample, group) go through its chunks x per_group partial
+// results: f(chunk, channel).
+constexpr int kMergeThreads = 512;
+template <int L, class F>
 __device__ __forceinline__ void each_partial(const NormArgs& a, F f) {
-  const int wide = min(a.per_group, kMergeThreads), high = kMergeThreads / wide;
-  const int k0 = threadIdx.x / wide, c0 = threadIdx.x % wide;
+  const int wide = min(a.per_group, L), high = L / wide, lane = threadIdx.x % L;
+  const int k0 = lane / wide, c0 = lane % wide;
   if (k0 >= high) return;
   for (int c = c0; c < a.per_group; c += wide)
 #pragma unroll 8
     for (int k = k0; k < a.chunks; k += high) f(k, c);
 }
-__device__ __forceinline__ float block_sum(float v, float* red) {  // in every thread, in a fixed order
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v, float* red) {  // in every lane, in a fixed order
   v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
+  if constexpr (L > 32) {
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = red[0];
 #pragma unroll
-  for (int i = 1; i < kMergeThreads / 32; ++i) v += red[i];
+    for (int i = 1; i < L / 32; ++i) v += red[i];
+  }
   return v;
 }
 
+template <int L>
 __global__ void __launch_bounds__(kMergeThreads) norm_stats_merge_kernel(NormArgs a) {
   may_start_next();
   after_previous();
   __shared__ float red[kMergeThreads / 32];
-  for (long long w = blockIdx.x; w < a.n * a.groups; w += gridDim.x) {
+  constexpr int kGroups = kMergeThreads / L;
+  for (long long w = (long long)blockIdx.x * kGroups + threadIdx.x / L; w < a.n * a.groups; w += (long long)gridDim.x * kGroups) {
     const long long sample = w / a.groups;
     const int* cnt = a.counts + sample * a.chunks;
     const float2* part = a.part + sample * a.chunks * a.channels + (w % a.groups) * a.per_group;
     float n = 0.f, mean = 0.f, m2 = 0.f;
-    each_partial(a, [&](int k, int c) {
+    each_partial<L>(a, [&](int k, int c) {
       const float f = (float)cnt[k];
       n += f;
       if (f > 0.f) mean = fmaf(f, part[(long long)k * a.channels + c].x, mean);
     });
-    n = block_sum(n, red);
-    mean = block_sum(mean, red);
+    n = lanes_sum<L>(n, red);
+    mean = lanes_sum<L>(mean, red);
     mean = n > 0.f ? mean / n : 0.f;
-    each_partial(a, [&](int k, int c) {
+    each_partial<L>(a, [&](int k, int c) {
       const float f = (float)cnt[k];
       const float2 e = part[(long long)k * a.channels + c];
       const float d = e.x - mean;
       if (f > 0.f) m2 += fmaf(f * d, d, e.y);
     });
-    m2 = block_sum(m2, red);
-    if (threadIdx.x == 0) {
+    m2 = lanes_sum<L>(m2, red);
+    if (threadIdx.x % L == 0) {
       a.stats[2 * w] = mean;
       a.stats[2 * w + 1] = n > 0.f ? 1.f / sqrtf(m2 / n + a.eps) : 0.f;
     }
@@ -364,43 +379,61 @@ __global__ void __launch_bounds__(kThreads, 3) norm_grad_sums_kernel(NormArgs a,
     }
     if (col == 0) rc[row] = cnt;
     __syncthreads();
-    for (int i = threadIdx.x; i < a.tx * V; i += blockDim.x) {
-      const int ch = (int)(item % a.ctiles) * a.tx * V + i;
-      if (ch >= a.channels) break;
-      float2 s = both(0.f);
-      for (int r = 0; r < a.ty; ++r) s = add2(s, red[r * a.tx * V + i]);
-      a.part[(p.sample * a.chunks + p.chunk) * a.channels + ch] = s;
+    float2* part = a.part + (p.sample * a.chunks + p.chunk) * a.channels + (int)(item % a.ctiles) * a.tx * V;
+    const int width = min(a.tx * V, a.channels - (int)(item % a.ctiles) * a.tx * V);
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (a.ty > 16 && warps > 0) {
+      if ((int)threadIdx.x >> 5 < warps)
+        for (int i = threadIdx.x >> 5; i < width; i += warps) {
+          float2 s = both(0.f);
+          for (int r = lane; r < a.ty; r += 32) s = add2(s, red[r * a.tx * V + i]);
+          s = make_float2(warp_sum(s.x), warp_sum(s.y));
+          if (lane == 0) part[i] = s;
+        }
+    } else {
+      for (int i = threadIdx.x; i < width; i += blockDim.x) {
+        float2 s = both(0.f);
+        for (int r = 0; r < a.ty; ++r) s = add2(s, red[r * a.tx * V + i]);
+        part[i] = s;
+      }
     }
-    if (threadIdx.x == 0 && item % a.ctiles == 0) {
+    if (threadIdx.x < 32 && item % a.ctiles == 0) {
       int total = 0;
-      for (int r = 0; r < a.ty; ++r) total += rc[r];
-      a.counts[p.sample * a.chunks + p.chunk] = total;
+      if (blockDim.x >= 32) {
+        for (int r = lane; r < a.ty; r += 32) total += rc[r];
+        total = __reduce_add_sync(0xffffffffu, total);
+      } else if (threadIdx.x == 0) {
+        for (int r = 0; r < a.ty; ++r) total += rc[r];
+      }
+      if (threadIdx.x == 0) a.counts[p.sample * a.chunks + p.chunk] = total;
     }
     __syncthreads();  // the partial results have been read
   }
 }
 
 // A / n and B / n of every (sample, group).
+template <int L>
 __global__ void __launch_bounds__(kMergeThreads) norm_grad_merge_kernel(NormArgs a) {
   may_start_next();
   after_previous();
   __shared__ float red[kMergeThreads / 32];
-  for (long long w = blockIdx.x; w < a.n * a.groups; w += gridDim.x) {
+  constexpr int kGroups = kMergeThreads / L;
+  for (long long w = (long long)blockIdx.x * kGroups + threadIdx.x / L; w < a.n * a.groups; w += (long long)gridDim.x * kGroups) {
     const long long sample = w / a.groups;
     const int g = (int)(w % a.groups);
     const float2* part = a.part + sample * a.chunks * a.channels + g * a.per_group;
     float n = 0.f, sa = 0.f, sb = 0.f;
-    each_partial(a, [&](int k, int c) {
+    each_partial<L>(a, [&](int k, int c) {
       const float wt = a.weight ? load_param(a.weight, a.param_dtype, g * a.per_group + c) : 1.f;
       const float2 e = part[(long long)k * a.channels + c];
       n += (float)a.counts[sample * a.chunks + k];
       sa = fmaf(wt, e.x, sa);
       sb = fmaf(wt, e.y, sb);
     });
-    n = block_sum(n, red);
-    sa = block_sum(sa, red);
-    sb = block_sum(sb, red);
-    if (threadIdx.x == 0) a.ab[w] = n > 0.f ? make_float2(sa / n, sb / n) : make_float2(0.f, 0.f);
+    n = lanes_sum<L>(n, red);
+    sa = lanes_sum<L>(sa, red);
+    sb = lanes_sum<L>(sb, red);
+    if (threadIdx.x % L == 0) a.ab[w] = n > 0.f ? make_float2(sa / n, sb / n) : make_float2(0.f, 0.f);
   }
 }
 
@@ -616,6 +649,9 @@ inline unsigned grid_of(long long items) { return (unsigned)(items < (1 << 20) ?
 
 int32_t param_grads(const float2* part, long long rows, int channels, void* dweight, void* dbias, int param_dtype,
                     float2* params, cudaStream_t s) {
+  if (rows <= 256)  // few: the second step alone
+    return launch_after(norm_param_store_kernel, dim3((channels + 31) / 32), dim3(32, 16), 0, s, 1, part, (int)rows, channels,
+                        dweight, dbias, param_dtype);
   const int splits = (int)(rows < 8 * kParamSplits ? (rows + 7) / 8 : kParamSplits);
   const int32_t st = launch_after(norm_param_sums_kernel, dim3((channels + 31) / 32, splits), dim3(32, 8), 0, s, 1, part,
                                   rows, channels, splits, params);
@@ -650,12 +686,20 @@ size_t sums_smem(const NormArgs& a, int tensors) {
     if (st_ != NCA_OK) return st_; \
   } while (0)
 
+// A warp a group for few partial results, a block for many.
+int32_t merge(void (*warp)(NormArgs), void (*block)(NormArgs), const NormArgs& a, cudaStream_t s) {
+  const long long groups = a.n * a.groups;
+  if ((long long)a.chunks * a.per_group <= 256 || groups >= 8192)
+    return launch_after(warp, dim3(grid_of((groups + kMergeThreads / 32 - 1) / (kMergeThreads / 32))), dim3(kMergeThreads), 0, s, 1, a);
+  return launch_after(block, dim3(grid_of(groups)), dim3(kMergeThreads), 0, s, 1, a);
+}
+
 template <class T, int V, int ACT, bool MASK, bool ONE>
 int32_t forward(const NcaNormDesc& d, NormArgs a, cudaStream_t s) {
   static std::atomic<uint64_t> ready[2];
   const long long items = plan(d, a, V);
   NCA_TRY(launch(norm_stats_kernel<T, V, MASK>, ready[0], a, items, sums_smem<T, V>(a, 1), s));
-  NCA_TRY(launch_after(norm_stats_merge_kernel, dim3(grid_of(a.n * a.groups)), dim3(kMergeThreads), 0, s, 1, a));
+  NCA_TRY(merge(norm_stats_merge_kernel<32>, norm_stats_merge_kernel<kMergeThreads>, a, s));
   return launch(norm_apply_kernel<T, V, ACT, MASK, ONE>, ready[1], a, items, ring_bytes<T, V>(1), s);
 }
 
@@ -666,7 +710,7 @@ int32_t backward(const NcaNormDesc& d, NormArgs a, void* dweight, void* dbias, f
   const long long items = plan(d, a, V);
   NCA_TRY(launch(norm_grad_sums_kernel<T, V, ACT, MASK, ONE>, ready[0], a, items, sums_smem<T, V>(a, 2), s));
   if (a.y) {
-    NCA_TRY(launch_after(norm_grad_merge_kernel, dim3(grid_of(a.n * a.groups)), dim3(kMergeThreads), 0, s, 1, a));
+    NCA_TRY(merge(norm_grad_merge_kernel<32>, norm_grad_merge_kernel<kMergeThreads>, a, s));
     NCA_TRY(launch(norm_grad_apply_kernel<T, V, ACT, MASK, ONE>, ready[1], a, items, ring_bytes<T, V>(2), s));
   }
   if (!dweight && !dbias) return NCA_OK;

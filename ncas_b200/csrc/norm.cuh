@@ -4,6 +4,12 @@
 
 namespace nca {
 
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 template <int BYTES>
 __device__ __forceinline__ void copy_async(void* to, const void* from) {
   const uint32_t a = (uint32_t)__cvta_generic_to_shared(to);

@@ -47,12 +47,6 @@ __device__ __forceinline__ void put_remote(const float4* p, uint32_t rank, float
 }
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 // What a thread works on.
 struct Work {
   long long sample;
