@@ -44,56 +44,23 @@ __device__ __forceinline__ float teacher_of(const DistillArgs& a, long long r, l
   return load_param(a.teacher, a.teacher_dtype, r * a.t_stride + k);
 }
 
-// The G lanes of one row: G <= 32 lanes of a warp, or the whole block of kThreads.
+// The G lanes of a warp that share a row.
 template <int G>
 struct Lanes {
   int lane;
   unsigned mask;
-  float* red;  // shared, for the block form
-  __device__ explicit Lanes(float* r) : red(r) {
-    if constexpr (G <= 32) {
-      lane = threadIdx.x % G;
-      const int first = (threadIdx.x & 31) / G * G;
-      mask = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << first;
-    } else {
-      lane = threadIdx.x;
-      mask = 0xffffffffu;
-    }
-  }
-  __device__ __forceinline__ void sync() const {
-    if constexpr (G <= 32) __syncwarp(mask);
-    else __syncthreads();
-  }
-  __device__ __forceinline__ float max_warp(float v) const {
-#pragma unroll
-    for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
-    return v;
-  }
-  __device__ __forceinline__ float sum_warp(float v) const {
-#pragma unroll
-    for (int o = (G < 32 ? G : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(mask, v, o);
-    return v;
+  __device__ Lanes() {
+    lane = threadIdx.x % G;
+    mask = G == 32 ? 0xffffffffu : ((1u << (G & 31)) - 1u) << ((threadIdx.x & 31) / G * G);
   }
   __device__ __forceinline__ float max(float v) const {
-    v = max_warp(v);
-    if constexpr (G > 32) {
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-      __syncthreads();
-      v = red[0];
-      for (int i = 1; i < G / 32; ++i) v = fmaxf(v, red[i]);
-    }
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(mask, v, o));
     return v;
   }
   __device__ __forceinline__ float sum(float v) const {
-    v = sum_warp(v);
-    if constexpr (G > 32) {
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-      __syncthreads();
-      v = red[0];
-      for (int i = 1; i < G / 32; ++i) v += red[i];
-    }
+#pragma unroll
+    for (int o = G / 2; o; o >>= 1) v += __shfl_xor_sync(mask, v, o);
     return v;
   }
 };
@@ -119,60 +86,65 @@ __device__ __forceinline__ bool whole_rows(const void* p, long long stride, int 
 }
 
 // G lanes a row, K classes a lane in registers (class j of a row: lane j % G, register j / G), the
-// entries likewise: one read of everything, no second pass.  For top <= G K.  I: the index type; the
-// teacher has the logits' type (SAME) or one that is looked up at each load.
-template <class T, class I, int G, int K, bool SAME, bool FWD>
+// entries likewise in KE registers: one read of everything, no second pass.  For top <= G KE.  I: the index
+// type; the teacher has the logits' type (SAME) or one that is looked up at each load.
+template <class T, class I, int G, int K, int KE, bool SAME, bool FWD>
 __global__ void __launch_bounds__(kThreads) distill_small_kernel(DistillArgs a) {
-  const Lanes<G> l(nullptr);
+  const Lanes<G> l;
   constexpr int kRows = kThreads / G;
   const float c2 = a.c2, inv_tau = a.inv_tau;
   const int top = (int)a.top;
   const bool whole_s = G == 1 && whole_rows<T, K>(a.logits, a.s_stride, a.classes);
   const bool whole_d = G == 1 && a.dlogits && whole_rows<T, K>(a.dlogits, a.classes, a.classes);
-  const bool whole_i = G == 1 && whole_rows<I, K>(a.index, a.i_stride, top);
-  const bool whole_t = G == 1 && SAME && whole_rows<T, K>(a.teacher, a.t_stride, top);
+  const bool whole_i = G == 1 && whole_rows<I, KE>(a.index, a.i_stride, top);
+  const bool whole_t = G == 1 && SAME && whole_rows<T, KE>(a.teacher, a.t_stride, top);
   for (long long r = (long long)blockIdx.x * kRows + threadIdx.x / G; r < a.rows;
        r += (long long)gridDim.x * kRows) {
     const T* s = static_cast<const T*>(a.logits) + r * a.s_stride;
     const I* is = static_cast<const I*>(a.index) + r * a.i_stride;
     T* ds = static_cast<T*>(a.dlogits) + r * (long long)a.classes;
     const float w = a.weight ? a.weight[r] : 1.f;
-    float v[K], t[K];
-    int i[K];
+    float v[K], t[KE];
+    int i[KE];
     float m = -kInf, tmax = -kInf;
     // everything is asked for before anything is used
-    T sv[K], tv[K];
-    I iv[K];
-    float tf[K];
+    T sv[K], tv[KE];
+    I iv[KE];
+    float tf[KE];
     if constexpr (G == 1) {
       load_values<T, K>(s, a.classes, whole_s, sv);
-      load_values<I, K>(is, top, whole_i, iv);
-      if constexpr (SAME) load_values<T, K>(static_cast<const T*>(a.teacher) + r * a.t_stride, top, whole_t, tv);
+      load_values<I, KE>(is, top, whole_i, iv);
+      if constexpr (SAME) load_values<T, KE>(static_cast<const T*>(a.teacher) + r * a.t_stride, top, whole_t, tv);
     } else {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int j = k * G + l.lane;
         if (j < a.classes) sv[k] = s[j];
+      }
+#pragma unroll
+      for (int k = 0; k < KE; ++k) {
+        const int j = k * G + l.lane;
         if (j < top) iv[k] = is[j];
         if (SAME && j < top) tv[k] = static_cast<const T*>(a.teacher)[r * a.t_stride + j];
       }
     }
     if constexpr (!SAME) {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int k = 0; k < KE; ++k)
         if (k * G + l.lane < top) tf[k] = teacher_of(a, r, k * G + l.lane);
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int j = k * G + l.lane;
       v[k] = j < a.classes ? to_f32(sv[k]) : -kInf;
+      m = fmaxf(m, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < KE; ++k) {
+      const int j = k * G + l.lane;
       i[k] = j < top && iv[k] >= 0 && iv[k] < a.classes ? (int)iv[k] : -1;
       if constexpr (SAME) t[k] = i[k] >= 0 ? to_f32(tv[k]) : -kInf;
       else t[k] = i[k] >= 0 ? tf[k] : -kInf;
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      m = fmaxf(m, v[k]);
       tmax = fmaxf(tmax, t[k] != t[k] ? kInf : t[k]);  // NaN and +inf end in NaN
     }
     tmax = l.max(tmax);
@@ -194,22 +166,25 @@ __global__ void __launch_bounds__(kThreads) distill_small_kernel(DistillArgs a) 
     for (int k = 0; k < K; ++k) {
       q[k] = k * G + l.lane < a.classes ? ex2((v[k] - m) * c2) : 0.f;
       sum += q[k];
+    }
+#pragma unroll
+    for (int k = 0; k < KE; ++k) {
       tsum += i[k] >= 0 ? ex2((t[k] - tmax) * c2) : 0.f;
     }
     sum = FWD ? l.sum(sum) : a.stats[2 * r + 1];
     tsum = l.sum(tsum);
     const float ts = rcp(tsum);
-    float p[K], hit[K];  // each entry's p; each class's sum of them
+    float p[KE], vi[KE];  // each entry's p and the logit of its class
+    float hit[K];         // each class's sum of p
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+    for (int k = 0; k < KE; ++k) {
       p[k] = i[k] >= 0 ? ex2((t[k] - tmax) * c2) * ts : 0.f;
-      hit[k] = 0.f;
+      vi[k] = 0.f;
     }
-    float vi[K];  // the logit of each entry's class
 #pragma unroll
-    for (int k = 0; k < K; ++k) vi[k] = 0.f;
+    for (int k = 0; k < K; ++k) hit[k] = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < KE; ++k)
 #pragma unroll
       for (int o = 0; o < G; ++o) {
         if (k * G + o >= top) break;
@@ -231,7 +206,7 @@ __global__ void __launch_bounds__(kThreads) distill_small_kernel(DistillArgs a) 
       const float lnt = logf(tsum), lns = logf(sum);
       float loss = 0.f;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int k = 0; k < KE; ++k)
         if (p[k] > 0.f) loss += p[k] * (((t[k] - tmax) * inv_tau - lnt) - ((vi[k] - m) * inv_tau - lns));
         else if (p[k] != p[k]) loss = p[k];
       loss = l.sum(loss);
@@ -356,28 +331,23 @@ __device__ __forceinline__ void put_remote(float2* p, uint32_t rank, float2 v) {
 }
 constexpr int kMostSlices = 8;
 
-// G lanes a row, or a cluster of `slices` blocks.  One pass keeps the running maximum and sum, a
+// A block a row, or a cluster of `slices` blocks: rows that no cluster holds, and more than 128 entries.
+// One pass keeps the running maximum and sum, a
 // second, which finds the row in L1 or L2, writes q; then the classes that have an entry are written
 // again with q - p.  The row's entries are staged in shared memory.
-template <class T, int G, int NT, bool FWD>
+template <class T, int NT, bool FWD>
 __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slices) {
-  constexpr int kV = 16 / sizeof(T), kRows = NT / G, kWarps = G / 32;
+  constexpr int kV = 16 / sizeof(T), G = NT, kWarps = NT / 32;
   __shared__ float red_m[2][NT / 32], red_s[2][NT / 32];
   __shared__ float2 red_t[2];
   __shared__ float2 red_c[2][kMostSlices];  // (maximum, sum) of each slice
-  extern __shared__ Entry entries_all[];
-  const int group = threadIdx.x / G, lane = threadIdx.x % G;
-  Entry* entries = entries_all + (size_t)group * a.top;
-  const auto sync = [] {
-    if constexpr (G == 32) __syncwarp();
-    else __syncthreads();
-  };
-  const int slice = G > 32 && slices > 1 ? (int)cluster_rank() : 0;
+  extern __shared__ Entry entries[];
+  const int lane = threadIdx.x;
+  const int slice = slices > 1 ? (int)cluster_rank() : 0;
   const float c2 = a.c2, inv_tau = a.inv_tau;
   const int top = (int)a.top;
   int flip = 0;
-  for (long long r = (long long)(blockIdx.x / slices) * kRows + group; r < a.rows;
-       r += (long long)(gridDim.x / slices) * kRows) {
+  for (long long r = blockIdx.x / slices; r < a.rows; r += gridDim.x / slices) {
     const T* s = static_cast<const T*>(a.logits) + r * a.s_stride;
     T* ds = a.dlogits ? static_cast<T*>(a.dlogits) + r * (long long)a.classes : nullptr;
     const float w = a.weight ? a.weight[r] : 1.f;
@@ -436,10 +406,7 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slic
       float ws = rebase(run.sum, run.m, wm, c2);
 #pragma unroll
       for (int o = 16; o; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
-      if constexpr (G == 32) {
-        m = wm;
-        sum = ws;
-      } else {
+      {
         if ((threadIdx.x & 31) == 0) {
           red_m[flip][threadIdx.x >> 5] = wm;
           red_s[flip][threadIdx.x >> 5] = ws;
@@ -470,18 +437,12 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slic
     } else {
       m = a.stats[2 * r];
       sum = a.stats[2 * r + 1];
-      if constexpr (G > 32) {
-        if (threadIdx.x == 0) red_t[flip] = make_float2(tmax, tsum);
-        __syncthreads();
-      }
+      if (threadIdx.x == 0) red_t[flip] = make_float2(tmax, tsum);
+      __syncthreads();
     }
-    if constexpr (G > 32) {
-      tmax = red_t[flip].x;
-      tsum = red_t[flip].y;
-      flip ^= 1;
-    } else {
-      __syncwarp();
-    }
+    tmax = red_t[flip].x;
+    tsum = red_t[flip].y;
+    flip ^= 1;
     live = live && tmax != -kInf;
     if (!live) {  // no weight, or no entry
       if (FWD && lane == 0 && slice == 0) {
@@ -496,7 +457,7 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slic
           for (int j = v0 * kV + lane; j < v1 * kV; j += G) ds[span.head + j] = from_f32<T>(0.f);
         for (int i = lane; i < ragged; i += G) ds[span.ragged_at(i)] = from_f32<T>(0.f);
       }
-      sync();  // the entries have been read
+      __syncthreads();  // the entries have been read
       continue;
     }
     if (FWD && lane < 32 && slice == 0) {
@@ -548,7 +509,7 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slic
         for (int j = v0 * kV + lane; j < v1 * kV; j += G) write_one(span.head + j);
       }
       for (int i = lane; i < ragged; i += G) write_one(span.ragged_at(i));
-      sync();
+      __syncthreads();
       // the classes with an entry in this slice, each by the lane of its first entry
       const int c0 = span.head + v0 * kV, c1 = span.head + v1 * kV;
       for (int k = lane; k < top; k += G) {
@@ -566,7 +527,7 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slic
         if (first) ds[i] = from_f32<T>(coef * (ex2((to_f32(s[i]) - m) * c2) / sum - p / tsum));
       }
     }
-    sync();  // the entries have been read
+    __syncthreads();  // the entries have been read
   }
 }
 
@@ -578,7 +539,7 @@ __device__ __forceinline__ void named_sync(int id, int threads) {
 }
 
 constexpr int kHeld = 8;       // 16-byte vectors of a row that a lane holds
-constexpr int kLaneTop = 4;    // entries of a row that a lane of the entry warp holds
+constexpr int kLaneTop = 4;    // entries of a row that a lane holds
 
 // The larger of m and a vector's values, 16-bit types two at a time (NaN is passed over: the sum finds it).
 template <class T>
@@ -916,14 +877,184 @@ __global__ void __launch_bounds__(NS + 32, BLOCKS) distill_held_kernel(DistillAr
   }
 }
 
-template <class T, int G, int K, bool FWD>
+// ------------------------------------------------------------------------- rows of up to 8 KB
+// A warp a row, which it holds in registers (NV vectors a lane); the gradient is put together in shared
+// memory in fp32: q, then minus p at the entries' classes, 32 entries at a time (equal classes among
+// them are found by a match over the lanes and added up by the first), then stored in lines.  Rows in
+// flight on other warps hide the latency of one row's steps.
+template <class T, int NV, int WARPS, bool FWD>
+__global__ void __launch_bounds__(32 * WARPS, 1024 / (4 * NV * WARPS)) distill_warp_kernel(DistillArgs a) {
+  constexpr int kV = 16 / sizeof(T), kWarps = WARPS;
+  extern __shared__ float4 warp_smem[];  // a warp: its gradient row, then its entries' probabilities
+  __shared__ float probs_all[kWarps][32 * kLaneTop];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* grad = reinterpret_cast<float*>(warp_smem) + warp * ((a.classes + 2 * kV + 3) / 4 * 4);
+  float* probs = probs_all[warp];
+  const float c2 = a.c2, inv_tau = a.inv_tau;
+  const int top = (int)a.top;
+  const uint32_t low = sizeof(T) == 4 ? 0xFF800000u : (__is_same(T, __nv_bfloat16) ? 0xFF80FF80u : 0xFC00FC00u);  // -inf
+  for (long long r = (long long)blockIdx.x * kWarps + warp; r < a.rows; r += (long long)gridDim.x * kWarps) {
+    const T* s = static_cast<const T*>(a.logits) + r * a.s_stride;
+    const RowSpan<T> span(s, a.classes);
+    const uint4* sv = reinterpret_cast<const uint4*>(s + span.head);
+    // everything is asked for before anything is used
+    const float w = a.weight ? a.weight[r] : 1.f;
+    int i[kLaneTop];
+    float t[kLaneTop];
+#pragma unroll
+    for (int k = 0; k < kLaneTop; ++k) {
+      i[k] = -1;
+      t[k] = -kInf;
+      if (k * 32 + lane < top) {
+        i[k] = index_of(a, r, k * 32 + lane);
+        t[k] = teacher_of(a, r, k * 32 + lane);
+      }
+    }
+    uint4 q[NV];
+#pragma unroll
+    for (int u = 0; u < NV; ++u) q[u] = u * 32 + lane < span.vecs ? __ldg(sv + u * 32 + lane) : make_uint4(low, low, low, low);
+    const bool ragged = lane < span.ragged();
+    const float end = ragged ? to_f32(s[span.ragged_at(lane)]) : -kInf;
+    T v[kLaneTop];
+    float tmax = -kInf, tsum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kLaneTop; ++k) {
+      if (k * 32 >= top) break;
+      v[k] = s[i[k] >= 0 ? i[k] : 0];
+      t[k] = i[k] >= 0 ? t[k] : -kInf;
+      tmax = fmaxf(tmax, t[k] != t[k] ? kInf : t[k]);  // NaN and +inf end in NaN
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, o));
+    T* ds = static_cast<T*>(a.dlogits) + r * (long long)a.classes;
+    const bool vec_out = ((reinterpret_cast<uintptr_t>(ds) ^ reinterpret_cast<uintptr_t>(s)) & 15) == 0;
+    if (w == 0.f || tmax == -kInf) {  // no weight, or no entry
+      if (FWD && lane == 0) {
+        a.loss[r] = 0.f;
+        if (a.stats) a.stats[2 * r] = a.stats[2 * r + 1] = 0.f;
+      }
+      if (a.dlogits) {
+        if (vec_out) {
+          for (int j = lane; j < span.vecs; j += 32) reinterpret_cast<uint4*>(ds + span.head)[j] = make_uint4(0, 0, 0, 0);
+          if (ragged) ds[span.ragged_at(lane)] = from_f32<T>(0.f);
+        } else {
+          for (int j = lane; j < a.classes; j += 32) ds[j] = from_f32<T>(0.f);
+        }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int k = 0; k < kLaneTop; ++k) {
+      if (k * 32 >= top) break;
+      t[k] -= tmax;
+      const float p = i[k] >= 0 ? ex2(t[k] * c2) : 0.f;
+      probs[k * 32 + lane] = p;
+      tsum += p;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) tsum += __shfl_xor_sync(0xffffffffu, tsum, o);
+    float m, sum;
+    if constexpr (FWD) {
+      Largest<T> most(low);
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+        if (u * 32 < span.vecs) most.add(q[u]);
+      m = fmaxf(most.get(), end);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float from = m == -kInf ? 0.f : m;
+      sum = ragged ? ex2((end - from) * c2) : 0.f;
+#pragma unroll
+      for (int u = 0; u < NV; ++u)
+        if (u * 32 < span.vecs) sum += exp_sum<T>(q[u], from, c2);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (m == -kInf) sum = m - m;  // a row of -inf only: NaN
+      const float lnt = logf(tsum), lns = logf(sum);
+      float loss = 0.f;
+#pragma unroll
+      for (int k = 0; k < kLaneTop; ++k) {
+        if (k * 32 >= top) break;
+        const float p = probs[k * 32 + lane] * rcp(tsum);
+        if (i[k] >= 0 && !(p <= 0.f)) loss += p * ((t[k] * inv_tau - lnt) - ((to_f32(v[k]) - m) * inv_tau - lns));
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+      if (lane == 0) {
+        a.loss[r] = loss * w * a.tau * a.tau;
+        if (a.stats) {
+          a.stats[2 * r] = m;
+          a.stats[2 * r + 1] = sum;
+        }
+      }
+    } else {
+      m = a.stats[2 * r];
+      sum = a.stats[2 * r + 1];
+    }
+    if (!a.dlogits) continue;
+    const float coef = w * a.tau * (a.grad ? a.grad[r * a.grad_stride] : 1.f);
+    const float cq = coef / sum, cp = coef / tsum;
+    const int off = (kV - span.head) % kV;  // class j lies at grad[j + off]: vectors on their boundaries
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      if (u * 32 >= span.vecs) break;
+      const int j = u * 32 + lane;
+      if (j < span.vecs) {
+        float f[kV];
+        unpack<T>(q[u], f);
+        float4* to = reinterpret_cast<float4*>(grad + span.head + off + j * kV);
+#pragma unroll
+        for (int e = 0; e < kV; e += 4) {
+          const float2 d0 = scaled2(f[e], f[e + 1], m, c2), d1 = scaled2(f[e + 2], f[e + 3], m, c2);
+          to[e / 4] = make_float4(ex2(d0.x) * cq, ex2(d0.y) * cq, ex2(d1.x) * cq, ex2(d1.y) * cq);
+        }
+      }
+    }
+    if (ragged) grad[span.ragged_at(lane) + off] = ex2((end - m) * c2) * cq;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kLaneTop; ++k) {
+      if (k * 32 >= top) break;
+      const unsigned peers = __match_any_sync(0xffffffffu, i[k]);
+      if (i[k] >= 0 && __ffs(peers) - 1 == lane) {
+        float p = 0.f;
+        for (unsigned b = peers; b; b &= b - 1) p += probs[k * 32 + __ffs(b) - 1];
+        grad[i[k] + off] -= cp * p;
+      }
+      __syncwarp();
+    }
+    if (vec_out) {
+#pragma unroll
+      for (int u = 0; u < NV; ++u) {
+        if (u * 32 >= span.vecs) break;
+        const int j = u * 32 + lane;
+        if (j < span.vecs) {
+          const float4* from = reinterpret_cast<const float4*>(grad + span.head + off + j * kV);
+          float f[kV];
+#pragma unroll
+          for (int e = 0; e < kV; e += 4) {
+            const float4 x = from[e / 4];
+            f[e] = x.x, f[e + 1] = x.y, f[e + 2] = x.z, f[e + 3] = x.w;
+          }
+          __stcs(reinterpret_cast<uint4*>(ds + span.head) + j, pack<T>(f));
+        }
+      }
+      if (ragged) ds[span.ragged_at(lane)] = from_f32<T>(grad[span.ragged_at(lane) + off]);
+    } else {
+      for (int j = lane; j < a.classes; j += 32) ds[j] = from_f32<T>(grad[j + off]);
+    }
+    __syncwarp();  // the row has been read
+  }
+}
+
+template <class T, int G, int K, int KE, bool FWD>
 int32_t launch_small(const DistillArgs& a, bool same, cudaStream_t s) {
   const long long blocks = (a.rows + kThreads / G - 1) / (kThreads / G);
   const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);  // several rows a thread pay its set-up
   const auto run = [&](auto index) {
     using I = decltype(index);
-    if (same) distill_small_kernel<T, I, G, K, true, FWD><<<grid, kThreads, 0, s>>>(a);
-    else distill_small_kernel<T, I, G, K, false, FWD><<<grid, kThreads, 0, s>>>(a);
+    if (same) distill_small_kernel<T, I, G, K, KE, true, FWD><<<grid, kThreads, 0, s>>>(a);
+    else distill_small_kernel<T, I, G, K, KE, false, FWD><<<grid, kThreads, 0, s>>>(a);
   };
   if (a.index_bits == 32) run(int{});
   else run((long long){});
@@ -974,11 +1105,30 @@ int32_t launch_clusters(void (*kernel)(DistillArgs, int), Room& room, const Dist
   return launch_status();
 }
 
-template <class T, int G, int NT, bool FWD>
+template <class T, int NT, bool FWD>
 int32_t launch_rows(const DistillArgs& a, int slices, cudaStream_t s) {
   static Room room;
-  return launch_clusters(distill_row_kernel<T, G, NT, FWD>, room, a, (a.rows + NT / G - 1) / (NT / G), slices, NT,
-                         (size_t)(NT / G) * a.top * sizeof(Entry), s);
+  return launch_clusters(distill_row_kernel<T, NT, FWD>, room, a, a.rows, slices, NT, a.top * sizeof(Entry), s);
+}
+
+template <class T, int NV, int WARPS, bool FWD>
+int32_t launch_warps(const DistillArgs& a, cudaStream_t s) {
+  static std::atomic<uint64_t> ready{0};
+  auto* kernel = distill_warp_kernel<T, NV, WARPS, FWD>;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
+  if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024) != cudaSuccess) {
+      const int32_t st = launch_status();
+      return st == NCA_OK ? NCA_ERR_CUDA : st;
+    }
+    ready.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  constexpr int kV = 16 / sizeof(T);
+  const size_t smem = a.dlogits ? (size_t)WARPS * ((a.classes + 2 * kV + 3) / 4 * 4) * sizeof(float) : 0;
+  const long long blocks = (a.rows + WARPS - 1) / WARPS;
+  kernel<<<(unsigned)(blocks < 148 * 16 ? blocks : 148 * 16), 32 * WARPS, smem, s>>>(a);
+  return launch_status();
 }
 
 template <class T, int NS, int NSM, int BLOCKS, bool FWD>
@@ -1001,12 +1151,18 @@ int32_t dispatch(const NcaDistillDesc& d, const DistillArgs& a, cudaStream_t s) 
   return with_dtype(d.dtype, [&](auto t) {
     using T = decltype(t);
     const bool same = d.dtype == d.teacher_dtype;
-    if (a.classes <= 2 && a.top <= 2) return launch_small<T, 1, 2, FWD>(a, same, s);
-    if (a.classes <= 4 && a.top <= 4) return launch_small<T, 1, 4, FWD>(a, same, s);
-    if (a.classes <= 16 && a.top <= 16) return launch_small<T, 4, 4, FWD>(a, same, s);
-    if (a.classes <= 64 && a.top <= 64) return launch_small<T, 8, 8, FWD>(a, same, s);
-    if (a.classes <= 2048 && a.top <= 512) return launch_rows<T, 32, 256, FWD>(a, 1, s);
+    if (a.classes <= 2 && a.top <= 2) return launch_small<T, 1, 2, 2, FWD>(a, same, s);
+    if (a.classes <= 4 && a.top <= 4) return launch_small<T, 1, 4, 4, FWD>(a, same, s);
+    if (a.classes <= 16 && a.top <= 4) return launch_small<T, 4, 4, 1, FWD>(a, same, s);
+    if (a.classes <= 16 && a.top <= 16) return launch_small<T, 4, 4, 4, FWD>(a, same, s);
+    if (a.classes <= 64 && a.top <= 8) return launch_small<T, 8, 8, 1, FWD>(a, same, s);
+    if (a.classes <= 128 && a.top <= 16) return launch_small<T, 16, 8, 1, FWD>(a, same, s);
+    if (a.classes <= 256 && a.top <= 32) return launch_small<T, 32, 8, 1, FWD>(a, same, s);
     const size_t bytes = a.classes * sizeof(T);
+    // many rows of up to 8 KB by warps; few ones go to blocks, whose lanes share a row's work
+    const bool many = a.rows >= 148 * 8 || bytes <= 2048;
+    if (many && bytes <= 32 * 8 * 16 && a.top <= 32 * kLaneTop) return launch_warps<T, 8, 8, FWD>(a, s);
+    if (many && bytes <= 32 * 16 * 16 && a.top <= 32 * kLaneTop) return launch_warps<T, 16, 4, FWD>(a, s);
     constexpr size_t kSmall = 96 * kHeld * 16, kMiddle = 256 * (kHeld + 8) * 16, kLarge = 992 * (kHeld + 9) * 16;
     if (a.top <= 32 * kLaneTop && bytes <= kMostSlices * kLarge) {
       if (bytes <= kSmall) return launch_held<T, 96, 0, 8, FWD>(a, 1, s);
@@ -1017,7 +1173,7 @@ int32_t dispatch(const NcaDistillDesc& d, const DistillArgs& a, cudaStream_t s) 
         slices *= 2;
       return middle ? launch_held<T, 256, 8, 3, FWD>(a, slices, s) : launch_held<T, 992, 9, 1, FWD>(a, slices, s);
     }
-    return launch_rows<T, 512, 512, FWD>(a, slices_of(a, sizeof(T)), s);
+    return launch_rows<T, 512, FWD>(a, slices_of(a, sizeof(T)), s);
   });
 }
 

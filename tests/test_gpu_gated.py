@@ -105,6 +105,8 @@ def check(a, dy, act="silu"):
     (1, 64, 64, 64), (1, 8, 8, 8), (1, 1, 1, 1), (2, 3, 5, 7), (17, 100, 36, 20), (64, 256, 256, 64), (81, 256, 256, 64),
     (129, 130, 131, 132), (200, 72, 520, 40), (300, 33, 65, 129), (777, 128, 96, 256), (1, 520, 1000, 264),
     (8, 1024, 640, 512), (16, 200, 1030, 17), (31, 264, 2048, 128), (33, 72, 136, 8), (1500, 16, 24, 9),
+    (130, 40, 9000, 24), (3, 700, 8200, 41), (70, 4100, 300, 40), (900, 33, 2100, 269),  # long k axes, few tiles
+    (16, 640, 256, 4100), (48, 96, 1300, 1000),
 ])
 def test_against_the_oracle(dtype, t, d, f, o):
     check(*make(t, d, f, o, dtype, seed=t + d))

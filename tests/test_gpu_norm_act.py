@@ -90,6 +90,9 @@ def check(x, groups, weight, bias, act="silu", mask=None, eps=1e-5, dy=None):
     (2, 40, 2304, 9),    # more 16-byte vectors than threads
     (1, 6000, 16, 2),    # a long sample, cut into pieces
     (700, 9, 8, 2),      # many small samples
+    (40, 500, 2, 1),     # two channels: all threads over the cells
+    (2, 30000, 64, 1),   # one group too large for a cluster of blocks
+    (1, 20000, 96, 32),  # the same with three channels a group
 ])
 def test_against_the_oracle(dtype, n, cells, channels, groups):
     x = normal(n, cells, channels, seed=cells, scale=1.5, shift=0.25).to(DEV, dtype)
@@ -138,6 +141,15 @@ def check_same_call(x, groups, w, b, mask, dy):
     leaves = [t.detach().requires_grad_() for t in (x, w, b)]
     y = ops.group_norm_act(leaves[0], groups, leaves[1], leaves[2], act="silu", mask=mask)
     return y, torch.autograd.grad(y, leaves, dy)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,cells,c,groups", [(5, 3481, 32, 4), (2, 20000, 64, 1), (3, 700, 6, 2), (9, 70, 40, 40)])
+def test_masks_of_padded_boards(dtype, n, cells, c, groups):
+    # a prefix of every sample's cells: whole pieces, and whole samples, without a cell
+    x = normal(n, cells, c, seed=6, shift=0.5).to(DEV, dtype)
+    keep = torch.arange(cells)[None] < torch.linspace(0, cells, n).round()[:, None]
+    check(x, groups, normal(c, seed=1, shift=1.0).to(DEV), normal(c, seed=2).to(DEV), act="relu", mask=keep.to(DEV))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
