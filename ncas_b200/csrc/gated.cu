@@ -218,28 +218,21 @@ __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits
     if (c + j < n) to[j] = from_f32<T>(f[j] + (bias ? load_param(bias, bias_dtype, c + j) : 0.f));
 }
 
-// Column sums of up to three [rows][cols] matrices (blockIdx.z) in two steps of a fixed order: the rows
-// of a piece, 8 columns a lane (rows lie on 16-byte boundaries), then the pieces.
-struct ColumnSums {
-  const void* a[3];
-  long long cols[3], ld[3];
-  void* out[3];
-  float* part[3];  // [splits][cols rounded up to 8]
-};
-constexpr int kSumSplits = 256;
+// Column sums of a [rows][cols] matrix, 8 columns a thread (rows lie on 16-byte boundaries): `wide` threads
+// side by side, 256 / wide rows at a time, a block the rows of its piece, in a fixed order.
+constexpr int kSumSplits = 256, kRowPieces = 32;
 template <class T>
-__global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant__ ColumnSums p, long long rows,
-                                                          int splits) {
+__global__ void __launch_bounds__(256) column_sums_kernel(const T* a, long long rows, long long cols, long long ld,
+                                                          int splits, int wide, float* part, long long padded) {
   may_start_next();
   after_previous();
-  __shared__ float2 red[8][32][4];
-  const int z = blockIdx.z;
-  const long long c = 8 * ((long long)blockIdx.x * 32 + threadIdx.x), cols = p.cols[z], padded = (cols + 7) / 8 * 8;
-  if (256ll * blockIdx.x >= padded) return;
+  __shared__ float2 red[256][4];
+  const int high = 256 / wide, row = threadIdx.x / wide;
+  const long long c = 8 * ((long long)blockIdx.x * wide + threadIdx.x % wide);
   const long long per = (rows + splits - 1) / splits, r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
   float2 s[4] = {both(0.f), both(0.f), both(0.f), both(0.f)};
-  if (c < padded) {
-    const T* from = static_cast<const T*>(p.a[z]) + c;
+  if (c < cols && row < high) {
+    const T* from = a + c;
     const auto add = [&](const Vec<T, 8>& v) {
       float2 f[4];
       to_pairs<T, 8>(v, f);
@@ -248,40 +241,56 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant_
     };
     if (c + 8 <= cols) {
 #pragma unroll 8
-      for (long long r = r0 + threadIdx.y; r < r1; r += 8) add(*reinterpret_cast<const Vec<T, 8>*>(from + r * p.ld[z]));
+      for (long long r = r0 + row; r < r1; r += high) add(*reinterpret_cast<const Vec<T, 8>*>(from + r * ld));
     } else {
-      for (long long r = r0 + threadIdx.y; r < r1; r += 8) {
+      for (long long r = r0 + row; r < r1; r += high) {
         Vec<T, 8> v;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.v[i] = c + i < cols ? from[r * p.ld[z] + i] : from_f32<T>(0.f);
+        for (int i = 0; i < 8; ++i) v.v[i] = c + i < cols ? from[r * ld + i] : from_f32<T>(0.f);
         add(v);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) red[threadIdx.y][threadIdx.x][i] = s[i];
+  for (int i = 0; i < 4; ++i) red[threadIdx.x][i] = s[i];
   __syncthreads();
-  if (threadIdx.y < 4 && c < padded) {
-    float2 t = red[0][threadIdx.x][threadIdx.y];
-    for (int i = 1; i < 8; ++i) t = add2(t, red[i][threadIdx.x][threadIdx.y]);
-    *reinterpret_cast<float2*>(p.part[z] + blockIdx.y * padded + c + 2 * threadIdx.y) = t;
+  for (int i = threadIdx.x; i < 4 * wide; i += 256) {  // a pair of columns each
+    const int v = i / 4;
+    const long long at = 8 * ((long long)blockIdx.x * wide + v) + 2 * (i % 4);
+    if (at >= padded) continue;
+    float2 t = red[v][i % 4];
+    for (int r = 1; r < high; ++r) t = add2(t, red[r * wide + v][i % 4]);
+    *reinterpret_cast<float2*>(part + blockIdx.y * padded + at) = t;
   }
 }
-__global__ void __launch_bounds__(512) column_store_kernel(const __grid_constant__ ColumnSums p, int splits, int dtype) {
+// Adds up the rows of up to three [rows][ld] fp32 matrices (blockIdx.z), a piece of them a block (blockIdx.y):
+// into the next matrix, or where there is one piece into the gradient.
+struct RowSums {
+  const float* part[3];
+  float* next[3];  // [pieces][ld], or null
+  void* out[3];
+  long long cols[3], ld[3];
+  int rows[3];
+};
+__global__ void __launch_bounds__(512) row_sums_kernel(const __grid_constant__ RowSums p, int dtype) {
   may_start_next();
   after_previous();
   __shared__ float red[16][33];
   const int z = blockIdx.z;
-  const long long c = (long long)blockIdx.x * 32 + threadIdx.x, cols = p.cols[z], padded = (cols + 7) / 8 * 8;
+  const long long c = (long long)blockIdx.x * 32 + threadIdx.x, ld = p.ld[z];
+  const int per = (p.rows[z] + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * per, r1 = min(p.rows[z], r0 + per);
   float s = 0.f;
-  if (c < cols)
+  if (c < p.cols[z]) {
+    const float* from = p.part[z] + c;
 #pragma unroll 8
-    for (int k = threadIdx.y; k < splits; k += 16) s += p.part[z][k * padded + c];
+    for (int r = r0 + threadIdx.y; r < r1; r += 16) s += from[r * ld];
+  }
   red[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y || c >= cols) return;
+  if (threadIdx.y || c >= p.cols[z]) return;
   for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
-  store_param(p.out[z], dtype, c, s);
+  if (gridDim.y > 1) p.next[z][blockIdx.y * ld + c] = s;
+  else store_param(p.out[z], dtype, c, s);
 }
 
 // --------------------------------------------------------------------------------- the products
@@ -468,7 +477,7 @@ struct Operand {
 };
 struct Plan {
   Operand op[OPS];
-  size_t h, dgate, dup, part, sums, total;
+  size_t h, dgate, dup, part, sums, cols, total;
   long long fp;  // padded hidden
 };
 
@@ -508,7 +517,9 @@ Plan plan_of(const NcaGatedDesc& d, bool backward) {
     at += align256(std::max({part_bytes(d.rows, d.d_in, 1, d.hidden, 2), part_bytes(d.hidden, d.d_in, 2, d.rows, 1),
                              part_bytes(d.hidden, d.d_in, 1, d.rows, 1), part_bytes(d.d_out, d.hidden, 1, d.rows, 1)}));
     p.sums = at;
-    at += align256((size_t)kSumSplits * (2 * p.fp + pad8(d.d_out)) * sizeof(float));
+    at += align256(((size_t)kRowPieces * 2 * p.fp + (size_t)(kSumSplits + kRowPieces) * pad8(d.d_out)) * sizeof(float));
+    p.cols = at;
+    at += align256((size_t)ceil_div(d.rows, 128) * 4 * 2 * p.fp * sizeof(float));
   }
   p.total = at + 256;
   return p;
@@ -600,6 +611,7 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
   const Matrix mdg{ws + pl.dgate, d.rows, d.hidden, pl.fp}, mdu{ws + pl.dup, d.rows, d.hidden, pl.fp};
   float* part = reinterpret_cast<float*>(ws + pl.part);
   float* part_sums = reinterpret_cast<float*>(ws + pl.sums);
+  float* col_sums = reinterpret_cast<float*>(ws + pl.cols);
   if (hidden_grads) {
     GemmParams p = base;
     Product g{{mdy, mdy}, {md, md}, false, false, d.rows, d.hidden, d.d_out, false, 1};
@@ -607,6 +619,8 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
         !encode_out(&p.out[1], ws + pl.dup, d.dtype, d.rows, d.hidden, pl.fp) ||
         !encode_planes(&p.planes, keep, d.rows, d.hidden, pl.fp, (long long)tf))
       return NCA_ERR_CUDA;
+    p.col_sums = db_gate || db_up ? col_sums : nullptr;
+    p.col_ld = pl.fp;
     NCA_TRY((product<T, false, true, EPI_DGATE, ACT>(
         p, g, d.dtype, shape_of(g.m, g.n, 1, ceil_div(g.k, kBK), false, false), s)));
   }
@@ -632,31 +646,44 @@ int32_t backward(const NcaGatedDesc& d, const void* x, const void* w_gate, const
     Product g{{mdy, mdy}, {mh, mh}, false, false, d.d_out, d.hidden, d.rows, false, 1};
     NCA_TRY((stored_product<T, true, true>(p, g, d.dtype, dw_down, dw_down, nullptr, part, s)));
   }
-  ColumnSums sums{};
-  int count = 0;
+  // the biases' gradients: sums of 32 rows each (or of pieces of dy), added up in one or two steps
+  RowSums sums{};
+  int count = 0, most = 0;
   long long widest = 0;
-  float* at = part_sums;
-  const int splits = (int)std::max<long long>(1, std::min<long long>(kSumSplits, d.rows / 64));
-  const auto add = [&](const Matrix& m, void* out) {
+  const auto add = [&](const float* part, int rows, long long cols, long long ld, float* next, void* out) {
     if (!out) return;
-    sums.a[count] = m.p;
-    sums.cols[count] = m.cols;
-    sums.ld[count] = m.ld;
+    sums.part[count] = part;
+    sums.next[count] = next;
     sums.out[count] = out;
-    sums.part[count] = at;
-    at += (size_t)kSumSplits * pad8(m.cols);
-    widest = std::max(widest, m.cols);
-    ++count;
+    sums.cols[count] = cols;
+    sums.ld[count] = ld;
+    sums.rows[count++] = rows;
+    most = std::max(most, rows);
+    widest = std::max(widest, cols);
   };
-  add(mdg, db_gate);
-  add(mdu, db_up);
-  add(mdy, db_down);
-  if (count) {
-    NCA_TRY(launch_after(column_sums_kernel<T>, dim3((unsigned)ceil_div(widest, 256), splits, count), dim3(32, 8), 0, s, 1,
-                         sums, d.rows, splits));
-    return launch_after(column_store_kernel, dim3((unsigned)ceil_div(widest, 32), 1, count), dim3(32, 16), 0, s, 1, sums,
-                        splits, d.bias_dtype);
+  const int blocks = (int)ceil_div(d.rows, 32);
+  add(col_sums, blocks, d.hidden, 2 * pl.fp, part_sums, db_gate);
+  add(col_sums + pl.fp, blocks, d.hidden, 2 * pl.fp, part_sums + pl.fp, db_up);
+  if (db_down) {
+    const long long padded = pad8(d.d_out);
+    const int splits = (int)std::max<long long>(1, std::min<long long>(kSumSplits, d.rows / 64));
+    float* part = part_sums + kRowPieces * 2 * pl.fp;
+    const int wide = (int)std::min<long long>(padded / 8, 32);
+    NCA_TRY(launch_after(column_sums_kernel<T>, dim3((unsigned)ceil_div(padded, 8 * wide), splits), dim3(256), 0, s, 1,
+                         static_cast<const T*>(mdy.p), d.rows, d.d_out, mdy.ld, splits, wide, part, padded));
+    add(part, splits, d.d_out, padded, part + kSumSplits * padded, db_down);
   }
+  if (count && most > 256) {
+    NCA_TRY(launch_after(row_sums_kernel, dim3((unsigned)ceil_div(widest, 32), kRowPieces, count), dim3(32, 16), 0, s, 1, sums,
+                         d.bias_dtype));
+    for (int i = 0; i < count; ++i) {
+      sums.part[i] = sums.next[i];
+      sums.rows[i] = kRowPieces;
+    }
+  }
+  if (count)
+    return launch_after(row_sums_kernel, dim3((unsigned)ceil_div(widest, 32), 1, count), dim3(32, 16), 0, s, 1, sums,
+                        d.bias_dtype);
   return NCA_OK;
 }
 

@@ -47,6 +47,8 @@ struct GemmParams {
   const void* bias[2];
   int bias_dtype;
   int save;            // EPI_GATE: write the planes
+  float* col_sums;     // EPI_DGATE: column sums of dgate, then dup, of every 32 rows [m / 32][2][col_ld] (may be null)
+  long long col_ld;
   int* ctrl;
   unsigned long long timeout_ns;
 };
@@ -264,6 +266,23 @@ __device__ __forceinline__ void join_planes(const uint4 (&a)[4], const uint4 (&b
       u[k + 1] = __uint_as_float((hu[j] & 0xFFFF0000u) | (lo[j] >> 16 & 0xFF00u));
     }
   }
+}
+
+// Adds up 32 columns over the lanes of a warp: lane l returns the sum of v[l].
+__device__ __forceinline__ float column_sum(const float (&x)[32], int lane) {
+  float v[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = x[i];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const bool high = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float send = high ? v[i] : v[i + o], keep = high ? v[i + o] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  return v[0];
 }
 
 constexpr int kPlace = 2048;
@@ -576,6 +595,14 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             const float2 dg = mul2(mul2(dh, make_float2(u[i], u[i + 1])), slope), du = mul2(dh, a);
             g[i] = dg.x, g[i + 1] = dg.y;
             u[i] = du.x, u[i + 1] = du.y;
+          }
+          if (p.col_sums && rows > 0) {  // of the biases' gradients, before the rounding; rows beyond m add 0
+            float* to = p.col_sums + (long long)(row0 >> 5) * 2 * p.col_ld + col + lane;
+            const float sg = column_sum(g, lane), su = column_sum(u, lane);
+            if (lane < n) {
+              to[0] = sg;
+              to[p.col_ld] = su;
+            }
           }
           uint4 v[4];
           __syncwarp();

@@ -251,7 +251,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight_,
 // reads and clears them).
 Tensor control_words(const c10::Device& dev) {
   static std::mutex m;
-  static std::array<Tensor, 64> kept;
+  static auto& kept = *new std::array<Tensor, 64>;  // never destroyed: CUDA may be gone by then
   const int i = dev.index();
   TORCH_CHECK(i >= 0 && i < 64, "device index ", i);
   std::lock_guard<std::mutex> lock(m);

@@ -49,7 +49,8 @@ def gated_ffn(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, *, a
     x and the weights (out, in): all bfloat16 or all float16; the biases float32 or of that type.  act:
     "relu", "silu", "gelu" (erf form) or "sigmoid".  Products are summed in fp32 on the tensor cores;
     the hidden product and the gradients of its two factors are rounded to the type of x in between.  Matrices whose rows start on 16-byte boundaries are read in place, others are
-    copied first.  Differentiable in every tensor.
+    copied first.  Differentiable in every tensor.  The first call on a device makes its control words:
+    it must precede a stream capture.
     """
     return _op("gated_ffn")(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
 
