@@ -212,6 +212,7 @@ __device__ __forceinline__ void take_row(uint32_t place, int lane, uint4 (&v)[4]
 }
 // The first `rows` rows of a place to 16-bit rows that lie on no 16-byte boundaries, `cols` values each.
 __device__ __forceinline__ void store_plain(uint32_t place, int lane, uint16_t* to, long long ld, int rows, int cols) {
+#pragma unroll 8
   for (int r = 0; r < rows; ++r) {
     const uint32_t at = place + 64 * r + ((16 * (lane >> 3)) ^ (16 * ((r >> 1) & 3))) + 2 * (lane & 7);
     uint16_t v;
