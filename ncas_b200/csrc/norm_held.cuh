@@ -2,8 +2,8 @@
 // from memory once (forward: x in, y out; backward: x and dy in, dx out).
 //
 // A block, or a cluster of `slices` blocks that split the cells, takes one sample, or a block of its
-// channels that ends on group borders.  A thread owns the same V adjacent channels (one group) of every
-// TY-th cell and copies its values asynchronously into places of its own in shared memory, so that no
+// channels that ends on group borders.  A thread owns the same V adjacent channels (of one group, or pairs
+// of one group each) of every TY-th cell and copies its values asynchronously into places of its own in shared memory, so that no
 // thread waits for another's data (norm_held_forward.cu, norm_held_backward.cu); statistics are merged through shared memory, and over a cluster
 // through distributed shared memory.
 //
@@ -52,7 +52,7 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_all;" 
 // What a thread works on.
 struct Work {
   long long sample;
-  int ch0, ch, group;  // first channel of the block, of the thread; group of the thread within the block
+  int ch0, ch;         // first channel of the block, of the thread
   int col, row, rank;
   long long c0;        // first cell of the slice
   int cells;           // and how many
@@ -68,7 +68,6 @@ __device__ __forceinline__ Work work_of(const HeldArgs& h) {
   w.col = threadIdx.x % h.a.tx;
   w.row = threadIdx.x / h.a.tx;
   w.ch = w.ch0 + w.col * V;
-  w.group = w.col * V / h.a.per_group;
   w.c0 = w.rank * h.slice_cells;
   w.cells = (int)min(h.a.cells - w.c0, h.slice_cells);
   w.on = w.row < h.a.ty && w.ch < h.a.channels;
@@ -106,7 +105,7 @@ __device__ __forceinline__ void each_cell(const NormArgs& a, const Work& w, uint
 
 // --------------------------------------------------------------------------------- host side
 struct HeldPlan {
-  bool ok;
+  bool ok, one;       // one: a thread's channels lie in one group
   int v, cb, cblocks, slices, tx, ty, iters, threads;
   long long slice_cells;
   size_t smem;
@@ -115,21 +114,27 @@ struct HeldPlan {
 HeldPlan plan_of(const NormArgs& a, int dtype, int width, bool backward) {
   HeldPlan p{};
   const size_t size = dtype_size(dtype);
+  // 16-byte vectors where groups hold whole ones, or pairs of channels; else what divides a group
   int v = width;
-  while (v > 1 && a.per_group % v) v /= 2;
+  p.one = !(v * size == 16 && a.per_group % v != 0 && a.per_group % 2 == 0);
+  while (p.one && v > 1 && a.per_group % v) v /= 2;
   if (v * size < 4) return p;  // an asynchronous copy moves 4 bytes at least
   p.v = v;
   const size_t tensors = backward ? 2 : 1;
-  // channels of a block: all of them, or fewer whole groups (64 adjacent bytes at least) when a sample
-  // would need more than 8 blocks of 100 KB.  Beyond that the streaming kernels are faster: clusters of
-  // 16 blocks that fill a multiprocessor each read 16 x 16384 x 512 bf16 at half their rate.
+  // channels of a block: all of them, or fewer whole groups when a sample would need more than 8 blocks of
+  // 100 KB, 256 adjacent bytes of them at least.  With shorter pieces the streaming kernels are faster on
+  // much data (64 x 4096 x 320 bf16 in 32 groups: forward 109 against 140 us, backward 189 against 480), but
+  // not on little, where their three launches cost more (4 x 4096 x 1024: 45 against 28 us).
+  const size_t all = (size_t)a.n * a.cells * a.channels * size;
+  const size_t narrowest = all < (48u << 20) ? 64 : 256;
   const size_t kFew = (backward ? 56 : 32) * 1024, kTwo = 100 * 1024;
   const auto bytes_of = [&](int g) { return (size_t)a.cells * g * a.per_group * size * tensors; };
   int groups = a.groups;
+  const auto whole = [&](int g) { return a.groups % g == 0 && g * a.per_group % v == 0; };
   while (bytes_of(groups) > kMaxSlices * kTwo || groups > kMaxGroups || groups * a.per_group / v > kMaxThreads) {
     int next = groups - 1;
-    while (next > 0 && a.groups % next) --next;
-    if (next <= 0 || next * a.per_group * size < 64) return p;
+    while (next > 0 && !whole(next)) --next;
+    if (next <= 0 || next * a.per_group * size < narrowest) return p;
     groups = next;
   }
   p.cb = groups * a.per_group;
@@ -155,7 +160,7 @@ HeldPlan plan_of(const NormArgs& a, int dtype, int width, bool backward) {
   p.smem = (size_t)p.iters * p.threads * v * size * tensors;
   p.smem += (size_t)p.slices * groups * sizeof(float4) + (size_t)p.ty * sizeof(int);
   if (backward) p.smem += ((size_t)p.ty * p.tx * v + p.cb) * sizeof(float2);
-  else p.smem += (size_t)p.threads * sizeof(float2);
+  else p.smem += (size_t)p.threads * (p.one ? 1 : v / 2) * sizeof(float2);
   p.ok = p.smem <= 208 * 1024 && p.iters <= 32 && a.n * p.cblocks * p.slices < (1ll << 31);
   return p;
 }
@@ -180,17 +185,19 @@ int32_t launch(void (*kernel)(HeldArgs), std::atomic<uint64_t>& ready, const Nor
 }
 
 
-// Instantiates fn(T, V, ACT, MASK) for the run-time choice.
+// Instantiates fn(T, V, ACT, MASK, ONE) for the run-time choice.
 template <class F>
-int32_t dispatch_held(const NormArgs& a, int dtype, int act, int v, F fn) {
+int32_t dispatch_held(const NormArgs& a, int dtype, int act, const HeldPlan& p, F fn) {
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int W = 16 / sizeof(T);
     return with_act(act, [&](auto tag) {
       constexpr int A = decltype(tag)::value;
-      if (v == W) return a.mask ? fn.template operator()<T, W, A, true>() : fn.template operator()<T, W, A, false>();
-      if (v == W / 2) return a.mask ? fn.template operator()<T, W / 2, A, true>() : fn.template operator()<T, W / 2, A, false>();
-      return a.mask ? fn.template operator()<T, W / 4, A, true>() : fn.template operator()<T, W / 4, A, false>();
+      if (!p.one) return a.mask ? fn.template operator()<T, W, A, true, false>() : fn.template operator()<T, W, A, false, false>();
+      if (p.v == W) return a.mask ? fn.template operator()<T, W, A, true, true>() : fn.template operator()<T, W, A, false, true>();
+      if (p.v == W / 2)
+        return a.mask ? fn.template operator()<T, W / 2, A, true, true>() : fn.template operator()<T, W / 2, A, false, true>();
+      return a.mask ? fn.template operator()<T, W / 4, A, true, true>() : fn.template operator()<T, W / 4, A, false, true>();
     });
   });
 }

@@ -8,9 +8,10 @@
 namespace nca {
 namespace {
 
-template <class T, int V, int ACT, bool MASK>
+template <class T, int V, int ACT, bool MASK, bool ONE>
 __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(const __grid_constant__ HeldArgs h) {
-  constexpr int P = (V + 1) / 2;
+  constexpr int P = (V + 1) / 2, U = ONE ? 1 : P;  // U: units of a thread, each in one group
+  constexpr int kUnit = ONE ? V : 2;               // channels of a unit
   constexpr bool kKeep = sizeof(T) == 4;
   const NormArgs& a = h.a;
   extern __shared__ uint4 smem_raw[];
@@ -38,12 +39,13 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(cons
         },
         [](int, int) {});
   }
-  float mean = 0.f, rstd = 0.f;
+  float mean[U], rstd[U];
   float2 wt[P], b[P], s1[P], s2[P];
-  if (w.on) {
-    const float* st = a.stats + 2 * (w.sample * a.groups + w.ch / a.per_group);
-    mean = st[0];
-    rstd = st[1];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float* st = a.stats + 2 * (w.sample * a.groups + (w.ch + u * kUnit) / a.per_group);
+    mean[u] = w.on ? st[0] : 0.f;
+    rstd[u] = w.on ? st[1] : 0.f;
   }
 #pragma unroll
   for (int i = 0; i < P; ++i) {
@@ -63,7 +65,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(cons
         to_pairs<T, V>(gs[at], g);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const float2 hh = mul2(add2(f[i], both(-mean)), both(rstd));
+          const float2 hh = mul2(add2(f[i], both(-mean[ONE ? 0 : i])), both(rstd[ONE ? 0 : i]));
           float2 unused;
           g[i] = mul2(g[i], act_slope2<ACT>(fma2(hh, wt[i], b[i]), unused));
           s1[i] = add2(s1[i], g[i]);
@@ -112,15 +114,20 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(cons
   if (h.slices > 1) cluster_barrier();
   else __syncthreads();
   if (!w.on || !a.y) return;
-  float sa = 0.f, sb = 0.f, n = 0.f;
-  for (int i = 0; i < h.slices; ++i) {
-    const float4 e = all[i * groups + w.group];
-    sa += e.x;
-    sb += e.y;
-    n += e.z;
+  float ga[U], gb[U];  // -A / n, -B / n
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int group = (w.col * V + u * kUnit) / a.per_group;  // within the block
+    float sa = 0.f, sb = 0.f, n = 0.f;
+    for (int i = 0; i < h.slices; ++i) {
+      const float4 e = all[i * groups + group];
+      sa += e.x;
+      sb += e.y;
+      n += e.z;
+    }
+    ga[u] = n > 0.f ? -sa / n : 0.f;
+    gb[u] = n > 0.f ? -sb / n : 0.f;
   }
-  sa = n > 0.f ? sa / n : 0.f;
-  sb = n > 0.f ? sb / n : 0.f;
   T* dx = static_cast<T*>(a.y) + (w.sample * a.cells + w.c0) * a.channels + w.ch;
   each_cell<MASK>(
       a, w, kept,
@@ -130,12 +137,12 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(cons
         to_pairs<T, V>(gs[at], g);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
-          const float2 hh = mul2(add2(f[i], both(-mean)), both(rstd));
+          const float2 hh = mul2(add2(f[i], both(-mean[ONE ? 0 : i])), both(rstd[ONE ? 0 : i]));
           float2 unused;
           if constexpr (!kKeep) g[i] = mul2(g[i], act_slope2<ACT>(fma2(hh, wt[i], b[i]), unused));
           // rstd (w dz - (A + h B) / n), each product rounded: one value a group gives exactly 0
-          const float2 away = fma2(hh, both(-sb), both(-sa));
-          f[i] = mul2(add2(mul2(wt[i], g[i]), away), both(rstd));
+          const int u = ONE ? 0 : i;
+          f[i] = mul2(add2(mul2(wt[i], g[i]), fma2(hh, both(gb[u]), both(ga[u]))), both(rstd[u]));
         }
         *reinterpret_cast<VecT*>(dx + (long long)c * a.channels) = from_pairs<T, V>(f);
       },
@@ -151,10 +158,10 @@ struct Call {
   const NormArgs& a;
   const HeldPlan& p;
   cudaStream_t s;
-  template <class T, int V, int ACT, bool MASK>
+  template <class T, int V, int ACT, bool MASK, bool ONE>
   int32_t operator()() const {
     static std::atomic<uint64_t> ready{0};
-    return launch(norm_held_backward_kernel<T, V, ACT, MASK>, ready, a, p, s);
+    return launch(norm_held_backward_kernel<T, V, ACT, MASK, ONE>, ready, a, p, s);
   }
 };
 
@@ -166,7 +173,7 @@ int norm_held_slices(const NormArgs& a, int dtype, int v, bool backward) {
 }
 int32_t norm_held_backward(const NormArgs& a, int dtype, int act, int v, cudaStream_t s) {
   const HeldPlan p = plan_of(a, dtype, v, true);
-  return dispatch_held(a, dtype, act, p.v, Call{a, p, s});
+  return dispatch_held(a, dtype, act, p, Call{a, p, s});
 }
 
 }  // namespace nca

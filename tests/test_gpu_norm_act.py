@@ -90,6 +90,10 @@ def check(x, groups, weight, bias, act="silu", mask=None, eps=1e-5, dy=None):
     (2, 40, 2304, 9),    # more 16-byte vectors than threads
     (1, 6000, 16, 2),    # a long sample, cut into pieces
     (700, 9, 8, 2),      # many small samples
+    (3, 100, 80, 8),     # ten channels a group: 16-byte loads that span groups
+    (2, 3000, 320, 32),  # the same over several blocks of channels and cells
+    (4, 33, 48, 8),      # six channels a group
+    (5, 19, 8, 4),       # pairs
     (40, 500, 2, 1),     # two channels: all threads over the cells
     (2, 30000, 64, 1),   # one group too large for a cluster of blocks
     (1, 20000, 96, 32),  # the same with three channels a group
@@ -144,7 +148,7 @@ def check_same_call(x, groups, w, b, mask, dy):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,cells,c,groups", [(5, 3481, 32, 4), (2, 20000, 64, 1), (3, 700, 6, 2), (9, 70, 40, 40)])
+@pytest.mark.parametrize("n,cells,c,groups", [(5, 3481, 32, 4), (4, 500, 40, 4), (2, 20000, 64, 1), (3, 700, 6, 2), (9, 70, 40, 40)])
 def test_masks_of_padded_boards(dtype, n, cells, c, groups):
     # a prefix of every sample's cells: whole pieces, and whole samples, without a cell
     x = normal(n, cells, c, seed=6, shift=0.5).to(DEV, dtype)
