@@ -133,6 +133,40 @@ __device__ __forceinline__ void each_cell(const NormArgs& a, const Place& p, voi
   }
 }
 
+// The channels of a block's tile, group by group: f(lanes, group, first channel of the tile, width) by as
+// many lanes for each group as let all groups be done at once, a warp at most.
+struct Lanes {
+  int count, lane;  // count a power of two
+  __device__ __forceinline__ float sum(float v) const {
+    for (int o = count >> 1; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+    return v;
+  }
+  // Through rows x width entries: f(row, column).
+  template <class F>
+  __device__ __forceinline__ void each(int rows, int width, F f) const {
+    const int wide = min(width, count), high = wide ? count / wide : 0;
+    const int r0 = wide ? lane / wide : 0, c0 = wide ? lane % wide : 0;
+    if (r0 >= high) return;
+    for (int r = r0; r < rows; r += high)
+      for (int c = c0; c < width; c += wide) f(r, c);
+  }
+};
+template <int V, class F>
+__device__ __forceinline__ void each_group(const NormArgs& a, long long item, F f) {
+  const int c_lo = (int)(item % a.ctiles) * a.tx * V, c_hi = min(a.channels, c_lo + a.tx * V);
+  const int first = c_lo / a.per_group, groups = (c_hi - 1) / a.per_group - first + 1;
+  const int threads = blockDim.x & ~31;
+  if ((int)threadIdx.x >= threads) return;  // an incomplete warp
+  Lanes l{32, 0};
+  while (l.count > 1 && groups * l.count > threads) l.count >>= 1;
+  l.lane = threadIdx.x & (l.count - 1);
+  for (int base = 0; base < groups; base += threads / l.count) {
+    const int g = first + base + threadIdx.x / l.count;
+    const int lo = max(g * a.per_group, c_lo) - c_lo;
+    f(l, g, lo, max(0, min((g + 1) * a.per_group, c_hi) - c_lo - lo));  // width 0 past the last group
+  }
+}
+
 // ------------------------------------------------------------------------- forward: statistics
 template <class T, int V, bool MASK>
 __global__ void __launch_bounds__(kThreads) norm_stats_kernel(NormArgs a, long long items) {
@@ -180,52 +214,40 @@ __global__ void __launch_bounds__(kThreads) norm_stats_kernel(NormArgs a, long l
     }
     if (col == 0) rc[row] = cnt;
     __syncthreads();
-    // the rows of a channel: by one thread, or where there are many by the lanes of a warp
-    float2* part = a.part + (p.sample * a.chunks + p.chunk) * a.channels + (int)(item % a.ctiles) * a.tx * V;
-    const int width = min(a.tx * V, a.channels - (int)(item % a.ctiles) * a.tx * V);
-    const auto merged = [&](int i, int r0, int step, auto sum) {
+    float4* to = a.gpart + (p.sample * a.chunks + p.chunk) * (a.groups + a.ctiles) + item % a.ctiles;
+    each_group<V>(a, item, [&](const Lanes& l, int g, int lo, int width) {
       float n = 0.f, mean = 0.f, m2 = 0.f;
-      for (int r = r0; r < a.ty; r += step) {
+      l.each(a.ty, width, [&](int r, int c) {
         const float f = (float)rc[r];
         n += f;
-        mean += rc[r] ? f * red[r * a.tx * V + i].x : 0.f;
-      }
-      n = sum(n);
-      mean = sum(mean);
+        if (f > 0.f) mean = fmaf(f, red[r * a.tx * V + lo + c].x, mean);
+      });
+      n = l.sum(n);
+      mean = l.sum(mean);
       mean = n > 0.f ? mean / n : 0.f;
-      for (int r = r0; r < a.ty; r += step) {
-        const float2 e = red[r * a.tx * V + i];
-        const float d = e.x - mean;
-        m2 += rc[r] ? fmaf((float)rc[r] * d, d, e.y) : 0.f;
-      }
-      m2 = sum(m2);
-      if (r0 == 0) {
-        part[i] = make_float2(mean, m2);
-        if (i == 0 && item % a.ctiles == 0) a.counts[p.sample * a.chunks + p.chunk] = (int)n;
-      }
-    };
-    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    if (a.ty > 16 && warps > 0) {
-      if ((int)threadIdx.x >> 5 < warps)
-        for (int i = threadIdx.x >> 5; i < width; i += warps) merged(i, lane, 32, [](float v) { return warp_sum(v); });
-    } else {
-      for (int i = threadIdx.x; i < width; i += blockDim.x) merged(i, 0, 1, [](float v) { return v; });
-    }
+      l.each(a.ty, width, [&](int r, int c) {
+        const float2 e = red[r * a.tx * V + lo + c];
+        const float f = (float)rc[r], d = e.x - mean;
+        if (f > 0.f) m2 += fmaf(f * d, d, e.y);
+      });
+      m2 = l.sum(m2);
+      if (l.lane == 0 && width) to[g] = make_float4(n, mean, m2, 0.f);
+    });
     __syncthreads();  // the partial results have been read
   }
 }
 
-// L lanes (a warp, or a block of kMergeThreads) per (sample, group) go through its chunks x per_group partial
-// results: f(chunk, channel).
-constexpr int kMergeThreads = 512;
+// L lanes (a warp, or a block of kMergeThreads) per (sample, group) go through its partial results, one for
+// every chunk and tile of channels that it reaches into.
+constexpr int kMergeThreads = 256;
 template <int L, class F>
-__device__ __forceinline__ void each_partial(const NormArgs& a, F f) {
-  const int wide = min(a.per_group, L), high = L / wide, lane = threadIdx.x % L;
-  const int k0 = lane / wide, c0 = lane % wide;
-  if (k0 >= high) return;
-  for (int c = c0; c < a.per_group; c += wide)
+__device__ __forceinline__ void each_partial(const NormArgs& a, long long w, int tile, F f) {
+  const int g = (int)(w % a.groups), t0 = g * a.per_group / tile, t1 = ((g + 1) * a.per_group - 1) / tile;
+  const long long step = a.groups + a.ctiles;
+  const float4* part = a.gpart + (w / a.groups) * a.chunks * step + g;
+  for (int t = t0; t <= t1; ++t)
 #pragma unroll 8
-    for (int k = k0; k < a.chunks; k += high) f(k, c);
+    for (int k = threadIdx.x % L; k < a.chunks; k += L) f(part[k * step + t]);
 }
 template <int L>
 __device__ __forceinline__ float lanes_sum(float v, float* red) {  // in every lane, in a fixed order
@@ -242,29 +264,23 @@ __device__ __forceinline__ float lanes_sum(float v, float* red) {  // in every l
 }
 
 template <int L>
-__global__ void __launch_bounds__(kMergeThreads) norm_stats_merge_kernel(NormArgs a) {
+__global__ void __launch_bounds__(kMergeThreads) norm_stats_merge_kernel(NormArgs a, int tile) {
   may_start_next();
   after_previous();
   __shared__ float red[kMergeThreads / 32];
   constexpr int kGroups = kMergeThreads / L;
   for (long long w = (long long)blockIdx.x * kGroups + threadIdx.x / L; w < a.n * a.groups; w += (long long)gridDim.x * kGroups) {
-    const long long sample = w / a.groups;
-    const int* cnt = a.counts + sample * a.chunks;
-    const float2* part = a.part + sample * a.chunks * a.channels + (w % a.groups) * a.per_group;
     float n = 0.f, mean = 0.f, m2 = 0.f;
-    each_partial<L>(a, [&](int k, int c) {
-      const float f = (float)cnt[k];
-      n += f;
-      if (f > 0.f) mean = fmaf(f, part[(long long)k * a.channels + c].x, mean);
+    each_partial<L>(a, w, tile, [&](const float4& e) {
+      n += e.x;
+      if (e.x > 0.f) mean = fmaf(e.x, e.y, mean);
     });
     n = lanes_sum<L>(n, red);
     mean = lanes_sum<L>(mean, red);
     mean = n > 0.f ? mean / n : 0.f;
-    each_partial<L>(a, [&](int k, int c) {
-      const float f = (float)cnt[k];
-      const float2 e = part[(long long)k * a.channels + c];
-      const float d = e.x - mean;
-      if (f > 0.f) m2 += fmaf(f * d, d, e.y);
+    each_partial<L>(a, w, tile, [&](const float4& e) {
+      const float d = e.y - mean;
+      if (e.x > 0.f) m2 += fmaf(e.x * d, d, e.z);
     });
     m2 = lanes_sum<L>(m2, red);
     if (threadIdx.x % L == 0) {
@@ -345,8 +361,10 @@ __global__ void __launch_bounds__(kThreads, 3) norm_grad_sums_kernel(NormArgs a,
   may_start_next();
   after_previous();
   constexpr int P = (V + 1) / 2;
-  extern __shared__ float2 red[];  // the ring; after it [ty][tx * V] (sum dz, sum dz h), then [ty] counts
+  // the ring; after it [ty][tx * V] (sum dz, sum dz h), then [ty] counts and [tx * V] weights
+  extern __shared__ float2 red[];
   int* rc = reinterpret_cast<int*>(red + a.ty * a.tx * V);
+  float* weights = reinterpret_cast<float*>(rc + a.ty);
   const int row = threadIdx.x / a.tx, col = (threadIdx.x % a.tx) * V;
   for (long long item = blockIdx.x; item < items; item += gridDim.x) {
     const Place p = place_of<V>(a, item);
@@ -381,59 +399,62 @@ __global__ void __launch_bounds__(kThreads, 3) norm_grad_sums_kernel(NormArgs a,
       float2* to = red + row * a.tx * V + col + 2 * i;
       to[0] = make_float2(s1[i].x, s2[i].x);
       if (V > 1) to[1] = make_float2(s1[i].y, s2[i].y);
+      if (row == 0) {
+        weights[col + 2 * i] = cv.w[i].x;
+        if (V > 1) weights[col + 2 * i + 1] = cv.w[i].y;
+      }
     }
     if (col == 0) rc[row] = cnt;
     __syncthreads();
     float2* part = a.part + (p.sample * a.chunks + p.chunk) * a.channels + (int)(item % a.ctiles) * a.tx * V;
     const int width = min(a.tx * V, a.channels - (int)(item % a.ctiles) * a.tx * V);
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    if (a.ty > 16 && warps > 0) {
+    if (a.ty > 16) {
       if ((int)threadIdx.x >> 5 < warps)
         for (int i = threadIdx.x >> 5; i < width; i += warps) {
           float2 s = both(0.f);
           for (int r = lane; r < a.ty; r += 32) s = add2(s, red[r * a.tx * V + i]);
           s = make_float2(warp_sum(s.x), warp_sum(s.y));
-          if (lane == 0) part[i] = s;
+          if (lane == 0) part[i] = red[i] = s;
         }
     } else {
       for (int i = threadIdx.x; i < width; i += blockDim.x) {
-        float2 s = both(0.f);
-        for (int r = 0; r < a.ty; ++r) s = add2(s, red[r * a.tx * V + i]);
-        part[i] = s;
+        float2 s = red[i];
+        for (int r = 1; r < a.ty; ++r) s = add2(s, red[r * a.tx * V + i]);
+        part[i] = red[i] = s;
       }
     }
-    if (threadIdx.x < 32 && item % a.ctiles == 0) {
-      int total = 0;
-      if (blockDim.x >= 32) {
-        for (int r = lane; r < a.ty; r += 32) total += rc[r];
-        total = __reduce_add_sync(0xffffffffu, total);
-      } else if (threadIdx.x == 0) {
-        for (int r = 0; r < a.ty; ++r) total += rc[r];
+    __syncthreads();
+    float4* to = a.gpart + (p.sample * a.chunks + p.chunk) * (a.groups + a.ctiles) + item % a.ctiles;
+    each_group<V>(a, item, [&](const Lanes& l, int g, int lo, int width) {
+      float n = 0.f, sa = 0.f, sb = 0.f;
+      for (int r = l.lane; r < a.ty; r += l.count) n += (float)rc[r];
+      for (int c = l.lane; c < width; c += l.count) {
+        sa = fmaf(weights[lo + c], red[lo + c].x, sa);
+        sb = fmaf(weights[lo + c], red[lo + c].y, sb);
       }
-      if (threadIdx.x == 0) a.counts[p.sample * a.chunks + p.chunk] = total;
-    }
+      n = l.sum(n) * (float)width;
+      sa = l.sum(sa);
+      sb = l.sum(sb);
+      if (l.lane == 0 && width) to[g] = make_float4(n, sa, sb, 0.f);
+    });
     __syncthreads();  // the partial results have been read
   }
 }
 
 // A / n and B / n of every (sample, group).
 template <int L>
-__global__ void __launch_bounds__(kMergeThreads) norm_grad_merge_kernel(NormArgs a) {
+__global__ void __launch_bounds__(kMergeThreads) norm_grad_merge_kernel(NormArgs a, int tile) {
   may_start_next();
   after_previous();
   __shared__ float red[kMergeThreads / 32];
   constexpr int kGroups = kMergeThreads / L;
   for (long long w = (long long)blockIdx.x * kGroups + threadIdx.x / L; w < a.n * a.groups; w += (long long)gridDim.x * kGroups) {
-    const long long sample = w / a.groups;
-    const int g = (int)(w % a.groups);
-    const float2* part = a.part + sample * a.chunks * a.channels + g * a.per_group;
     float n = 0.f, sa = 0.f, sb = 0.f;
-    each_partial<L>(a, [&](int k, int c) {
-      const float wt = a.weight ? load_param(a.weight, a.param_dtype, g * a.per_group + c) : 1.f;
-      const float2 e = part[(long long)k * a.channels + c];
-      n += (float)a.counts[sample * a.chunks + k];
-      sa = fmaf(wt, e.x, sa);
-      sb = fmaf(wt, e.y, sb);
+    each_partial<L>(a, w, tile, [&](const float4& e) {
+      n += e.x;
+      sa += e.y;
+      sb += e.z;
     });
     n = lanes_sum<L>(n, red);
     sa = lanes_sum<L>(sa, red);
@@ -552,25 +573,28 @@ void split_cells(const NcaNormDesc& d, int ty, int ctiles, int* chunks, long lon
   if (*chunks < 1) *chunks = 1;
 }
 
-int worst_chunks(const NcaNormDesc& d) {  // over every vector width: one vector a thread, 8 cells
-  int worst = 1;
+// The most chunks, and partial results of a sample's groups, over the vector widths.
+void worst_chunks(const NcaNormDesc& d, size_t* chunks, size_t* partials) {
+  *chunks = *partials = 1;
   for (int v = 1; v <= 8; v *= 2) {
     const int nv = (d.channels + v - 1) / v;
-    const int tx = nv < kThreads ? nv : kThreads, ty = kThreads / tx;
-    int chunks;
+    const int tx = nv < kThreads ? nv : kThreads, ty = kThreads / tx, ct = (nv + tx - 1) / tx;
+    int n;
     long long cc;
-    split_cells(d, ty, (nv + tx - 1) / tx, &chunks, &cc);
-    if (chunks > worst) worst = chunks;
+    split_cells(d, ty, ct, &n, &cc);
+    *chunks = std::max(*chunks, (size_t)n);
+    *partials = std::max(*partials, (size_t)n * (d.groups + ct));
   }
-  return worst;
 }
 
 struct Layout {
-  size_t stats, part, counts, ab, params, total;
+  size_t stats, part, gpart, ab, params, total;
 };
 // held: the slices of the kernel that holds samples, 0 when the streaming kernels run.
 Layout layout_of(const NcaNormDesc& d, bool backward, int held) {
-  const size_t chunks = held ? held : worst_chunks(d);
+  size_t chunks, partials;
+  worst_chunks(d, &chunks, &partials);
+  if (held) chunks = held;
   Layout l{};
   size_t at = 0;
   const auto take = [&](bool needed, size_t bytes) {
@@ -579,8 +603,8 @@ Layout layout_of(const NcaNormDesc& d, bool backward, int held) {
     return here;
   };
   l.stats = take(!backward && !held, (size_t)d.n * d.groups * sizeof(float2));
-  l.part = take(backward || !held, (size_t)d.n * chunks * d.channels * sizeof(float2));
-  l.counts = take(!held, (size_t)d.n * chunks * sizeof(int));
+  l.part = take(backward, (size_t)d.n * chunks * d.channels * sizeof(float2));
+  l.gpart = take(!held, (size_t)d.n * partials * sizeof(float4));
   l.ab = take(backward && !held, (size_t)d.n * d.groups * sizeof(float2));
   l.params = take(backward, (size_t)kParamSplits * d.channels * sizeof(float2));
   l.total = at;
@@ -618,7 +642,7 @@ void place(NormArgs& a, const Layout& l, void* ws) {
   uint8_t* w = static_cast<uint8_t*>(ws);
   if (!a.stats) a.stats = reinterpret_cast<float*>(w + l.stats);
   a.part = reinterpret_cast<float2*>(w + l.part);
-  a.counts = reinterpret_cast<int*>(w + l.counts);
+  a.gpart = reinterpret_cast<float4*>(w + l.gpart);
   a.ab = reinterpret_cast<float2*>(w + l.ab);
 }
 
@@ -683,7 +707,7 @@ int32_t launch(void (*kernel)(NormArgs, long long), std::atomic<uint64_t>& ready
 // Shared memory of a kernel that leaves partial results: the ring, or those where they are more.
 template <class T, int V>
 size_t sums_smem(const NormArgs& a, int tensors) {
-  return std::max(ring_bytes<T, V>(tensors), (size_t)a.ty * a.tx * V * sizeof(float2) + a.ty * sizeof(int));
+  return std::max(ring_bytes<T, V>(tensors), (size_t)a.ty * a.tx * V * sizeof(float2) + a.ty * sizeof(int) + a.tx * V * sizeof(float));
 }
 #define NCA_TRY(call)              \
   do {                             \
@@ -691,12 +715,13 @@ size_t sums_smem(const NormArgs& a, int tensors) {
     if (st_ != NCA_OK) return st_; \
   } while (0)
 
-// A warp a group for few partial results, a block for many.
-int32_t merge(void (*warp)(NormArgs), void (*block)(NormArgs), const NormArgs& a, cudaStream_t s) {
+// A warp a group for few partial results, a block for many.  tile: channels of a block.
+int32_t merge(void (*warp)(NormArgs, int), void (*block)(NormArgs, int), const NormArgs& a, int tile, cudaStream_t s) {
   const long long groups = a.n * a.groups;
-  if ((long long)a.chunks * a.per_group <= 256 || groups >= 8192)
-    return launch_after(warp, dim3(grid_of((groups + kMergeThreads / 32 - 1) / (kMergeThreads / 32))), dim3(kMergeThreads), 0, s, 1, a);
-  return launch_after(block, dim3(grid_of(groups)), dim3(kMergeThreads), 0, s, 1, a);
+  if ((long long)a.chunks * (a.ctiles / a.groups + 1) <= 64 || groups >= 8192)
+    return launch_after(warp, dim3(grid_of((groups + kMergeThreads / 32 - 1) / (kMergeThreads / 32))), dim3(kMergeThreads), 0,
+                        s, 1, a, tile);
+  return launch_after(block, dim3(grid_of(groups)), dim3(kMergeThreads), 0, s, 1, a, tile);
 }
 
 template <class T, int V, int ACT, bool MASK, bool ONE>
@@ -704,7 +729,7 @@ int32_t forward(const NcaNormDesc& d, NormArgs a, cudaStream_t s) {
   static std::atomic<uint64_t> ready[2];
   const long long items = plan(d, a, V);
   NCA_TRY(launch(norm_stats_kernel<T, V, MASK>, ready[0], a, items, sums_smem<T, V>(a, 1), s));
-  NCA_TRY(merge(norm_stats_merge_kernel<32>, norm_stats_merge_kernel<kMergeThreads>, a, s));
+  NCA_TRY(merge(norm_stats_merge_kernel<32>, norm_stats_merge_kernel<kMergeThreads>, a, a.tx * V, s));
   return launch(norm_apply_kernel<T, V, ACT, MASK, ONE>, ready[1], a, items, ring_bytes<T, V>(1), s);
 }
 
@@ -715,7 +740,7 @@ int32_t backward(const NcaNormDesc& d, NormArgs a, void* dweight, void* dbias, f
   const long long items = plan(d, a, V);
   NCA_TRY(launch(norm_grad_sums_kernel<T, V, ACT, MASK, ONE>, ready[0], a, items, sums_smem<T, V>(a, 2), s));
   if (a.y) {
-    NCA_TRY(merge(norm_grad_merge_kernel<32>, norm_grad_merge_kernel<kMergeThreads>, a, s));
+    NCA_TRY(merge(norm_grad_merge_kernel<32>, norm_grad_merge_kernel<kMergeThreads>, a, a.tx * V, s));
     NCA_TRY(launch(norm_grad_apply_kernel<T, V, ACT, MASK, ONE>, ready[1], a, items, ring_bytes<T, V>(2), s));
   }
   if (!dweight && !dbias) return NCA_OK;

@@ -34,8 +34,10 @@ struct NormArgs {
   const void* dy;
   void* y;                   // forward: y; backward: dx
   float* stats;              // [n][groups][2] mean, rstd
-  float2* part;              // [n][chunks][channels]
-  int* counts;               // [n][chunks] kept cells
+  float2* part;              // backward: [n][chunks][channels] (sum dz, sum dz h)
+  float4* gpart;             // [n][chunks][groups + ctiles]: (count, mean, M2) or (count, A, B) of a block's
+                             // channels of a group, at group + tile (no two pairs share a sum: along the
+                             // channels neither falls)
   float2* ab;                // backward: [n][groups] (A / n, B / n)
 };
 
