@@ -69,7 +69,8 @@ __device__ __forceinline__ uint32_t kept_of(const NormArgs& a, const Place& p, i
 // Goes through the thread's cells: use(cell of the piece, x vector, second vector) where the mask keeps the
 // cell, left_out(cell) elsewhere.  The vectors (one or two tensors) come through a ring of kRing
 // asynchronous copies in places of the thread's own, so that kRing cells are in flight all the time and
-// no thread waits for another; single 16-bit values, which such copies cannot move, are loaded directly.
+// no thread waits for another; single 16-bit values, which such copies cannot move, are loaded to registers,
+// kRing cells at a time (417 x 2009 x 69 fp16 backward: 332 us, one at a time 399).
 constexpr int kRing = 8;
 template <class T, int V>
 __host__ __device__ constexpr size_t ring_bytes(int tensors) {
@@ -119,16 +120,23 @@ __device__ __forceinline__ void each_cell(const NormArgs& a, const Place& p, voi
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
-    for (int i = 0; i < n; ++i) {
-      if (bits & 1) {
-        const VecT xv = *reinterpret_cast<const VecT*>(x);
-        use(row + i * a.ty, xv, TENSORS > 1 ? *reinterpret_cast<const VecT*>(g) : xv);
-      } else {
-        left_out(row + i * a.ty);
+    for (int i = 0; i < n; i += kRing) {
+      VecT xv[kRing], gv[TENSORS > 1 ? kRing : 1];
+      const uint32_t in = n - i < kRing ? bits & ((1u << (n - i)) - 1) : bits;
+#pragma unroll
+      for (int u = 0; u < kRing; ++u, x += x_step, g += TENSORS > 1 ? g_step : 0)
+        if (in >> u & 1) {
+          xv[u] = *reinterpret_cast<const VecT*>(x);
+          if (TENSORS > 1) gv[u] = *reinterpret_cast<const VecT*>(g);
+        }
+#pragma unroll
+      for (int u = 0; u < kRing; ++u) {
+        if (in >> u & 1)
+          use(row + (i + u) * a.ty, xv[u], gv[TENSORS > 1 ? u : 0]);
+        else if (MASK && i + u < n)
+          left_out(row + (i + u) * a.ty);
       }
-      bits = MASK ? bits >> 1 : bits;
-      x += x_step;
-      if (TENSORS > 1) g += g_step;
+      bits = MASK ? bits >> kRing : bits;
     }
   }
 }
