@@ -336,7 +336,8 @@ __device__ __forceinline__ void put_remote(float2* p, uint32_t rank, float2 v) {
 }
 constexpr int kMostSlices = 8;
 
-// A block a row, or a cluster of `slices` blocks: rows that no cluster holds, and more than 128 entries.
+// A block a row, or a cluster of `slices` blocks: rows that no cluster holds, more than 128 entries, and
+// the loss alone of many long rows.
 // One pass keeps the running maximum and sum, a
 // second, which finds the row in L1 or L2, writes q; then the classes that have an entry are written
 // again with q - p.  The row's entries are staged in shared memory.
@@ -887,11 +888,11 @@ __global__ void __launch_bounds__(NS + 32, BLOCKS) distill_held_kernel(DistillAr
 // memory in fp32: q, then minus p at the entries' classes, 32 entries at a time (equal classes among
 // them are found by a match over the lanes and added up by the first), then stored in lines.  Rows in
 // flight on other warps hide the latency of one row's steps.
-template <class T, int NV, int WARPS, bool FWD>
-__global__ void __launch_bounds__(32 * WARPS, 1024 / (4 * NV * WARPS)) distill_warp_kernel(DistillArgs a) {
+template <class T, int NV, int WARPS, int KT, int BLOCKS, bool FWD>
+__global__ void __launch_bounds__(32 * WARPS, BLOCKS) distill_warp_kernel(DistillArgs a) {
   constexpr int kV = 16 / sizeof(T), kWarps = WARPS;
   extern __shared__ float4 warp_smem[];  // a warp: its gradient row, then its entries' probabilities
-  __shared__ float probs_all[kWarps][32 * kLaneTop];
+  __shared__ float probs_all[kWarps][32 * KT];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float* grad = reinterpret_cast<float*>(warp_smem) + warp * ((a.classes + 2 * kV + 3) / 4 * 4);
   float* probs = probs_all[warp];
@@ -904,10 +905,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1024 / (4 * NV * WARPS)) distill_w
     const uint4* sv = reinterpret_cast<const uint4*>(s + span.head);
     // everything is asked for before anything is used
     const float w = a.weight ? a.weight[r] : 1.f;
-    int i[kLaneTop];
-    float t[kLaneTop];
+    int i[KT];
+    float t[KT];
 #pragma unroll
-    for (int k = 0; k < kLaneTop; ++k) {
+    for (int k = 0; k < KT; ++k) {
       i[k] = -1;
       t[k] = -kInf;
       if (k * 32 + lane < top) {
@@ -920,10 +921,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1024 / (4 * NV * WARPS)) distill_w
     for (int u = 0; u < NV; ++u) q[u] = u * 32 + lane < span.vecs ? __ldg(sv + u * 32 + lane) : make_uint4(low, low, low, low);
     const bool ragged = lane < span.ragged();
     const float end = ragged ? to_f32(s[span.ragged_at(lane)]) : -kInf;
-    T v[kLaneTop];
+    T v[KT];
     float tmax = -kInf, tsum = 0.f;
 #pragma unroll
-    for (int k = 0; k < kLaneTop; ++k) {
+    for (int k = 0; k < KT; ++k) {
       if (k * 32 >= top) break;
       v[k] = s[i[k] >= 0 ? i[k] : 0];
       t[k] = i[k] >= 0 ? t[k] : -kInf;
@@ -949,7 +950,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1024 / (4 * NV * WARPS)) distill_w
       continue;
     }
 #pragma unroll
-    for (int k = 0; k < kLaneTop; ++k) {
+    for (int k = 0; k < KT; ++k) {
       if (k * 32 >= top) break;
       t[k] -= tmax;
       const float p = i[k] >= 0 ? ex2(t[k] * c2) : 0.f;
@@ -978,7 +979,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1024 / (4 * NV * WARPS)) distill_w
       const float lnt = logf(tsum), lns = logf(sum);
       float loss = 0.f;
 #pragma unroll
-      for (int k = 0; k < kLaneTop; ++k) {
+      for (int k = 0; k < KT; ++k) {
         if (k * 32 >= top) break;
         const float p = probs[k * 32 + lane] * rcp(tsum);
         if (i[k] >= 0 && !(p <= 0.f)) loss += p * ((t[k] * inv_tau - lnt) - ((to_f32(v[k]) - m) * inv_tau - lns));
@@ -1018,7 +1019,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1024 / (4 * NV * WARPS)) distill_w
     if (ragged) grad[span.ragged_at(lane) + off] = ex2((end - m) * c2) * cq;
     __syncwarp();
 #pragma unroll
-    for (int k = 0; k < kLaneTop; ++k) {
+    for (int k = 0; k < KT; ++k) {
       if (k * 32 >= top) break;
       const unsigned peers = __match_any_sync(0xffffffffu, i[k]);
       if (i[k] >= 0 && __ffs(peers) - 1 == lane) {
@@ -1116,10 +1117,10 @@ int32_t launch_rows(const DistillArgs& a, int slices, cudaStream_t s) {
   return launch_clusters(distill_row_kernel<T, NT, FWD>, room, a, a.rows, slices, NT, a.top * sizeof(Entry), s);
 }
 
-template <class T, int NV, int WARPS, bool FWD>
+template <class T, int NV, int WARPS, int KT, int BLOCKS, bool FWD>
 int32_t launch_warps(const DistillArgs& a, cudaStream_t s) {
   static std::atomic<uint64_t> ready{0};
-  auto* kernel = distill_warp_kernel<T, NV, WARPS, FWD>;
+  auto* kernel = distill_warp_kernel<T, NV, WARPS, KT, BLOCKS, FWD>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
   if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
@@ -1164,13 +1165,33 @@ int32_t dispatch(const NcaDistillDesc& d, const DistillArgs& a, cudaStream_t s) 
     if (a.classes <= 128 && a.top <= 16) return launch_small<T, 16, 8, 1, FWD>(a, same, s);
     if (a.classes <= 256 && a.top <= 32) return launch_small<T, 32, 8, 1, FWD>(a, same, s);
     const size_t bytes = a.classes * sizeof(T);
-    // many rows of up to 8 KB by warps; few ones go to blocks, whose lanes share a row's work
+    // many rows of up to 8 KB by warps; few ones go to blocks, whose lanes share a row's work.  With no
+    // registers for more entries and vectors than there are, more warps fit (950,000 x 514 bf16, 2
+    // entries: 823 us, as 8 vectors and 128 entries 1080).
     const bool many = a.rows >= 148 * 8 || bytes <= 2048;
-    if (many && bytes <= 32 * 8 * 16 && a.top <= 32 * kLaneTop) return launch_warps<T, 8, 8, FWD>(a, s);
-    if (many && bytes <= 32 * 16 * 16 && a.top <= 32 * kLaneTop) return launch_warps<T, 16, 4, FWD>(a, s);
-    constexpr size_t kSmall = 96 * kHeld * 16, kMiddle = 256 * (kHeld + 8) * 16, kLarge = 992 * (kHeld + 9) * 16;
+    if (many && bytes <= 32 * 16 * 16 && a.top <= 32 * kLaneTop) {
+      if (bytes <= 32 * 4 * 16 && a.top <= 32) return launch_warps<T, 4, 8, 1, 6, FWD>(a, s);
+      if (bytes <= 32 * 8 * 16 && a.top <= 32) return launch_warps<T, 8, 8, 1, 4, FWD>(a, s);
+      if (bytes <= 32 * 8 * 16) return launch_warps<T, 8, 8, kLaneTop, 4, FWD>(a, s);
+      return launch_warps<T, 16, 4, kLaneTop, 4, FWD>(a, s);
+    }
+    constexpr auto held = [](int lanes, int in_smem) { return (size_t)lanes * (kHeld + in_smem) * 16; };
+    constexpr size_t kMiddle = held(256, 8), kLarge = held(992, 9);
     if (a.top <= 32 * kLaneTop && bytes <= kMostSlices * kLarge) {
-      if (bytes <= kSmall) return launch_held<T, 96, 0, 8, FWD>(a, 1, s);
+      if (bytes <= held(96, 0)) return launch_held<T, 96, 0, 8, FWD>(a, 1, s);
+      // Many rows: the smallest block that holds one, so that a multiprocessor has several, each at
+      // another row, and few places stay empty.  Measured, loss and gradient, against 256 x 16 vectors
+      // (to 64 KB) or 992 x 17: 25000 x 12000 bf16 263 (437) us, 14873 x 16384 200 (281), 14873 x 17000
+      // 252 (288), 7000 x 34528 217 (432), 4000 x 65536 211 (292).
+      if (a.rows >= 148 * 4) {
+        if (bytes <= held(192, 0)) return launch_held<T, 192, 0, 4, FWD>(a, 1, s);
+        if (bytes <= held(256, 0)) return launch_held<T, 256, 0, 3, FWD>(a, 1, s);
+        if (bytes <= held(384, 0)) return launch_held<T, 384, 0, 2, FWD>(a, 1, s);
+        // the loss alone needs no second look at a row: 4000 x 65536 bf16 123 us, held 210
+        if (FWD && !a.dlogits && bytes > kMiddle) return launch_rows<T, 256, FWD>(a, 1, s);
+        if (bytes > kMiddle && bytes <= held(256, 13)) return launch_held<T, 256, 13, 3, FWD>(a, 1, s);
+        if (bytes > kMiddle && bytes <= held(480, 10)) return launch_held<T, 480, 10, 2, FWD>(a, 1, s);
+      }
       int slices = 1;  // a row over several blocks where one cannot hold it, or where there are few rows
       const bool middle = bytes <= kMiddle || (a.rows < 74 && bytes <= kMostSlices * kMiddle);
       while (bytes > slices * (middle ? kMiddle : kLarge) ||
