@@ -63,6 +63,8 @@ def distill_loss(logits, teacher_logits, teacher_index, *, temperature=1.0, weig
     (int32 or int64; an index outside [0, classes), such as -1, marks no entry; entries of one class
     add up).  weight: float32 (...).  A row without entries or with weight 0 has loss and gradient 0.
     reduction: "none" (float32, (...)), "sum", or "mean" over all rows.  Differentiable in logits.
+    The same call gives the same bits; another number of rows, or distill_loss_and_grad, may run another
+    kernel, whose sums differ by rounding.
     """
     return _op("distill_loss")(logits, teacher_logits, teacher_index, temperature, weight, reduction)
 

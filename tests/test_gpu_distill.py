@@ -92,6 +92,46 @@ def test_rows_that_are_held(dtype, rows, classes, top, offset):
     assert (loss[::7] == 0).all() and (grad[::7] == 0).all()
 
 
+@pytest.mark.parametrize("dtype,classes,top,offset", [
+    (torch.bfloat16, 9001, 3, 0), (torch.float16, 15000, 40, 0), (torch.float16, 22001, 2, 1),
+    (torch.bfloat16, 24576, 128, 0), (torch.bfloat16, 40003, 5, 3), (torch.float16, 60008, 4, 0),
+    (torch.float32, 5000, 3, 0), (torch.float32, 20011, 7, 2), (torch.float32, 34560, 1, 0)])
+def test_many_long_rows(dtype, classes, top, offset):
+    """Enough rows that none is shared by blocks; a few of them are compared, with the tolerances of check()."""
+    g = torch.Generator().manual_seed(classes)
+    wide = (torch.randn((640, classes + offset), generator=g) * 2).to(DEV, dtype)
+    s = wide[:, offset:]
+    t = (torch.randn((640, top), generator=g) * 2).to(DEV, dtype)
+    i = torch.randint(0, classes, (640, top), generator=g).int().to(DEV)
+    w = (torch.rand((640,), generator=g) + 0.5).to(DEV)
+    w[::9] = 0.0
+    i[1::9] = -1
+    i[2::9, 0] = classes - 1
+    i[3::9, 0] = 0
+    s[4::9, 1] = -math.inf
+    loss, grad = ops.distill_loss_and_grad(s, t, i, temperature=1.5, weight=w, reduction="none")
+    with torch.no_grad():
+        alone = ops.distill_loss(s, t, i, temperature=1.5, weight=w, reduction="none")
+    leaf = s.detach().requires_grad_()
+    (later,) = torch.autograd.grad(ops.distill_loss(leaf, t, i, temperature=1.5, weight=w, reduction="sum"), leaf)
+    some = torch.arange(0, 640, 31)
+    ls, lg = O.distill(s[some].cpu(), t[some].cpu(), i[some].cpu(), 1.5, w[some].cpu())
+    f = torch.cat([s[some].double().flatten(), t[some].double().flatten()]).cpu()
+    f = f[torch.isfinite(f)]
+    spread = float(f.max() - f.min()) / 1.5
+    c = E * (spread + 80)
+    w64 = w[some].cpu().double()
+    for v in (loss, alone):
+        assert (v[:: 9] == 0).all() and (v[1::9] == 0).all()
+        fine = torch.isfinite(ls)  # an entry of a class that is ruled out: an infinite loss
+        got = v[some].cpu().double()
+        assert torch.equal(torch.isfinite(got), fine)
+        assert ((got - ls).abs() <= w64 * 1.5**2 * c * (1 + spread + 20))[fine].all()
+    for v in (grad, later):
+        assert (v[::9] == 0).all() and (v[1::9] == 0).all()
+        assert ((v[some].cpu().double() - lg).abs() <= UNIT[dtype] * lg.abs() + (w64 * 1.5 * c * 2)[:, None] + TINY[dtype]).all()
+
+
 @pytest.mark.parametrize("temperature", [0.25, 1.0, 8.0])
 @pytest.mark.parametrize("classes", [3, 40, 700, 3001])
 def test_temperatures_and_index_types(temperature, classes):
