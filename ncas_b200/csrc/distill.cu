@@ -8,7 +8,7 @@
 // product with the scale would overflow, still gives differences of 0.
 //
 // Which lanes share a row goes by its size (dispatch, below).  On a B200: 900,000 x 2 bf16 12.9 us in all
-// (2.0 TB/s; instructions bind), 150,022 x 662 fp16 with 90 entries 256 us (the entries' instructions),
+// (2.0 TB/s; instructions bind), 150,022 x 662 fp16 with 90 entries 261 us (the entries' instructions),
 // 2047 x 32003 fp16 55 us (4.7 TB/s), 8192 x 131072 bf16 with gradient 780 to 830 us (5.2 to 5.5 TB/s,
 // near HBM; the exponentials take 60% of their unit).
 #include "cell_ops.cuh"
@@ -1171,6 +1171,7 @@ int32_t dispatch(const NcaDistillDesc& d, const DistillArgs& a, cudaStream_t s) 
     const bool many = a.rows >= 148 * 8 || bytes <= 2048;
     if (many && bytes <= 32 * 16 * 16 && a.top <= 32 * kLaneTop) {
       if (bytes <= 32 * 4 * 16 && a.top <= 32) return launch_warps<T, 4, 8, 1, 6, FWD>(a, s);
+      if (bytes <= 32 * 4 * 16) return launch_warps<T, 4, 8, kLaneTop, 5, FWD>(a, s);
       if (bytes <= 32 * 8 * 16 && a.top <= 32) return launch_warps<T, 8, 8, 1, 4, FWD>(a, s);
       if (bytes <= 32 * 8 * 16) return launch_warps<T, 8, 8, kLaneTop, 4, FWD>(a, s);
       return launch_warps<T, 16, 4, kLaneTop, 4, FWD>(a, s);
