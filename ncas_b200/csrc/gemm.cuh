@@ -670,8 +670,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           } else {
             fence_async_proxy();
             __syncwarp();
-            if (lane == 0 && rows > 0) {
-              tma_store_2d(&p.out[tl.batch], here, col, row0);
+            if (lane == 0) {  // a group for every piece, also one without rows: the wait above counts groups
+              if (rows > 0) tma_store_2d(&p.out[tl.batch], here, col, row0);
               bulk_commit();
             }
           }

@@ -130,6 +130,26 @@ def test_tiles_on_multiprocessor_pairs(dtype):
     check(*make(2600, 280, 2072, 2064, dtype, seed=5))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,d,f,o", [
+    (5216, 2048, 64, 2048),  # y and dx: 21 x 8 tiles of 256 x 256, the last row of tiles with 96 rows
+    (72, 2048, 5216, 40),    # dWg, dWu
+    (72, 40, 2048, 5216),    # dWd
+])
+def test_tiles_without_rows_between_tiles_with_rows(dtype, t, d, f, o):
+    # several tiles for each pair of multiprocessors and a short k axis: the warps whose 32 rows of a tile
+    # lie beyond the matrix go on at once to the next tile while their stores of the tile before are read
+    a, dy = make(t, d, f, o, dtype, seed=16)
+    y, grads = check(a, dy)
+    for _ in range(10):
+        leaves = {k: v.detach().requires_grad_() for k, v in a.items()}
+        y2 = ops.gated_ffn(**leaves)
+        got = torch.autograd.grad(y2, list(leaves.values()), dy)
+        assert torch.equal(y2, y)
+        for k, g in zip(leaves, got):
+            assert torch.equal(g, grads[k]), k
+
+
 def test_long_row_axis_in_pieces():
     check(*make(20001, 64, 72, 24, torch.bfloat16, seed=6))
 
