@@ -178,6 +178,13 @@ __device__ __forceinline__ Vec<T, V> from_pairs(const float2 (&f)[(V + 1) / 2]) 
 __device__ __forceinline__ void may_start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// ------------------------------------------------------------------------------ blocks of a cluster
+// A block may write the shared memory of another of its cluster only once that one has started, which a
+// launch alone does not promise.  Every thread of a kernel that does so arrives at its start and waits
+// just before its block's first such write; what the kernel reads in between hides the wait.
+__device__ __forceinline__ void cluster_started_arrive() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_started_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 // ------------------------------------------------------------------------------------ host side
 inline int32_t launch_status() {
   const cudaError_t e = cudaGetLastError();

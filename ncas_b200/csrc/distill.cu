@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slic
   extern __shared__ Entry entries[];
   const int lane = threadIdx.x;
   const int slice = slices > 1 ? (int)cluster_rank() : 0;
+  if (FWD && slices > 1) cluster_started_arrive();
   const float c2 = a.c2, inv_tau = a.inv_tau;
   const int top = (int)a.top;
   int flip = 0;
@@ -427,6 +428,7 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slic
           const float e = red_m[flip][i];
           sum += rebase(red_s[flip][i], e, m, c2);
         }
+        if (slices > 1 && r < gridDim.x / slices) cluster_started_wait();  // the first row
         if (slices > 1 && live) {  // `live` here is the weight's, the same in all slices
           if (threadIdx.x < slices) put_remote(&red_c[flip][slice], threadIdx.x, make_float2(m, sum));
           cluster_barrier();
@@ -608,6 +610,7 @@ __global__ void __launch_bounds__(NS + 32, BLOCKS) distill_held_kernel(DistillAr
   __shared__ Entry entries[32 * kLaneTop];
   extern __shared__ uint4 held[];           // [NSM][NS]
   const int slice = slices > 1 ? (int)cluster_rank() : 0;
+  if (FWD && slices > 1) cluster_started_arrive();
   const int lane = threadIdx.x & 31;
   const bool entry_warp = threadIdx.x >= NS;
   const float c2 = a.c2;
@@ -630,6 +633,7 @@ __global__ void __launch_bounds__(NS + 32, BLOCKS) distill_held_kernel(DistillAr
     constexpr int n = kWarps < 8 ? 8 : kWarps < 16 ? 16 : 32;  // partial results, rounded up
     butterfly((lane & (n - 1)) <= kWarps ? red[flip][lane & (n - 1)] : make_float2(-kInf, 0.f), n, m, sum);
     if (slices > 1) {
+      if (r < step) cluster_started_wait();  // the first row
       if (threadIdx.x < slices) put_remote(&red_c[flip][slice], threadIdx.x, make_float2(m, sum));
       cluster_barrier();
       butterfly((lane & 7) < slices ? red_c[flip][lane & 7] : make_float2(-kInf, 0.f), 8, m, sum);

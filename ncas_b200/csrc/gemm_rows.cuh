@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
   const int tile = blockIdx.x / p.slices;
   const FailState fs{p.ctrl, abort_s, 0, p.timeout_ns};
 
+  if (p.slices > 1) cluster_started_arrive();
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(&full[i], 1);
@@ -145,6 +146,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
     const int q = warp & 3;  // tensor memory lanes 32 q .. 32 q + 31: an output each
     const bool ok = mbar_wait(done, 0, fs, 113);
     tc_fence_after();
+    if (p.slices > 1) cluster_started_wait();
     if (ok) {
       const int share = kBM / p.slices, row = 32 * q + lane;
       const int to = row / share, at = row % share;
@@ -173,6 +175,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
     tc_fence_before();
   }
   __syncwarp();
+  if (p.slices > 1 && warp < 2) cluster_started_wait();  // the others have waited
   if (p.slices > 1) cluster_sync_all();
   else __syncthreads();
   tc_fence_after();

@@ -24,6 +24,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(cons
   float2* red = reinterpret_cast<float2*>(gs + h.iters * threads);  // [ty][tx * V] (sum dz, sum dz h)
   float2* chan = red + a.ty * a.tx * V;                             // [cb] totals of the block
   int* count = reinterpret_cast<int*>(chan + h.cb);                 // [ty] cells of a row of threads
+  if (h.slices > 1) cluster_started_arrive();
   may_start_next();
   after_previous();
   const Work w = work_of<V>(h);
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_backward_kernel(cons
     if (a.part) a.part[(w.sample * h.slices + w.rank) * a.channels + w.ch0 + c] = s;  // of the parameters' gradients
   }
   __syncthreads();
+  if (h.slices > 1) cluster_started_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int g = warp; g < groups; g += threads >> 5) {
     float sa = 0.f, sb = 0.f, n = 0.f;

@@ -11,6 +11,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_forward_kernel(const
   const NormArgs& a = h.a;
   extern __shared__ uint4 smem_raw[];
   using VecT = Vec<T, V>;
+  if (h.slices > 1) cluster_started_arrive();
   may_start_next();
   after_previous();
   const Work w = work_of<V>(h);
@@ -67,6 +68,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) norm_held_forward_kernel(const
     if (w.on && w.col == 0) count[w.row] = cnt;
   }
   __syncthreads();
+  if (h.slices > 1) cluster_started_wait();
   // a warp a group: its ty x cols partial results, lanes over rows of threads
   const int cols = a.per_group / kUnit, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wide = cols < 32 ? cols : 32, high = 32 / wide, lrow = lane / wide, lcol = lane % wide;
