@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a, int slic
           const float e = red_m[flip][i];
           sum += rebase(red_s[flip][i], e, m, c2);
         }
-        if (slices > 1 && r < gridDim.x / slices) cluster_started_wait();  // the first row
-        if (slices > 1 && live) {  // `live` here is the weight's, the same in all slices
+        if (slices > 1) {  // for a row of weight 0 too: the barrier frees the places of the row before
+          if (r < gridDim.x / slices) cluster_started_wait();  // the first row
           if (threadIdx.x < slices) put_remote(&red_c[flip][slice], threadIdx.x, make_float2(m, sum));
           cluster_barrier();
           m = red_c[flip][0].x;

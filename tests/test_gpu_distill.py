@@ -132,6 +132,34 @@ def test_many_long_rows(dtype, classes, top, offset):
         assert ((v[some].cpu().double() - lg).abs() <= UNIT[dtype] * lg.abs() + (w64 * 1.5 * c * 2)[:, None] + TINY[dtype]).all()
 
 
+@pytest.mark.parametrize("dtype,classes,top,offset", [
+    (torch.bfloat16, 131072, 200, 0), (torch.float16, 100003, 131, 1), (torch.float32, 70001, 300, 2)])
+def test_clusters_that_go_through_rows_without_a_weight(dtype, classes, top, offset):
+    """More than 128 entries and rows that several blocks share, several rows a cluster, rows of weight 0
+    between the others; a few of them are compared, with the tolerances of check()."""
+    rows = 1500
+    g = torch.Generator(device=DEV).manual_seed(classes)
+    s = torch.randn((rows, classes + offset), generator=g, device=DEV).mul_(2).to(dtype)[:, offset:]
+    t = torch.randn((rows, top), generator=g, device=DEV).mul_(2).to(dtype)
+    i = torch.randint(0, classes, (rows, top), generator=g, device=DEV, dtype=torch.int32)
+    w = torch.rand((rows,), generator=g, device=DEV) + 0.5
+    w[rows // 2 :][torch.rand((rows - rows // 2,), generator=g, device=DEV) < 0.5] = 0.0
+    w[1 : rows // 2 : 2] = 0.0
+    loss, grad = ops.distill_loss_and_grad(s, t, i, temperature=1.5, weight=w, reduction="none")
+    off = w == 0
+    assert (loss[off] == 0).all() and (grad[off] == 0).all()
+    some = torch.arange(0, rows, 61)
+    ls, lg = O.distill(s[some].cpu(), t[some].cpu(), i[some].cpu(), 1.5, w[some].cpu())
+    spread = max(float(s[some].max() - s[some].min()), float(t[some].max() - t[some].min())) / 1.5
+    c = E * (spread + 80)
+    w64 = w[some].cpu().double()
+    assert ((loss[some].cpu().double() - ls).abs() <= w64 * 1.5**2 * c * (1 + spread + 20)).all()
+    assert ((grad[some].cpu().double() - lg).abs() <= UNIT[dtype] * lg.abs() + (w64 * 1.5 * c * 2)[:, None] + TINY[dtype]).all()
+    for _ in range(5):
+        again, again_grad = ops.distill_loss_and_grad(s, t, i, temperature=1.5, weight=w, reduction="none")
+        assert torch.equal(again, loss) and torch.equal(again_grad, grad)
+
+
 @pytest.mark.parametrize("temperature", [0.25, 1.0, 8.0])
 @pytest.mark.parametrize("classes", [3, 40, 700, 3001])
 def test_temperatures_and_index_types(temperature, classes):
