@@ -182,6 +182,11 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint3
   return d;
 }
 
+// A wait of a whole warp: it goes on only where no lane gave up, since loads from tensor memory take all lanes.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, const FailState& fs, int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, fs, where));
+}
+
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -505,6 +510,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
+      if (!ok) continue;  // after a wait that ran out: nothing but the barriers that the other warps wait at
       // EPI_DGATE: the saved planes of the piece at column c, asked for ahead of their use
       const auto ask = [&](int c) {
         pending = true;
@@ -516,7 +522,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         }
       };
       if (EPI == EPI_DGATE && rows > 0 && 32 * turn < cols) ask(32 * turn);
-      if (!mbar_wait(&acc_full[buf], ph, fs, 104)) break;
+      ok = mbar_wait_warp(&acc_full[buf], ph, fs, 104);
+      if (!ok) continue;
       tc_fence_after();
       const uint32_t acc = tmem + buf * BN + ((uint32_t)(32 * q) << 16);
       for (int c = 32 * turn; c < cols; c += 64) {
@@ -572,8 +579,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         } else if constexpr (EPI == EPI_DGATE) {
           float g[32], u[32];
           if (rows > 0) {
-            if (!mbar_wait(&loaded[warp - 4], load_ph, fs, 105)) {
-              ok = false;
+            ok = mbar_wait_warp(&loaded[warp - 4], load_ph, fs, 105);
+            if (!ok) {
+              tc_wait_ld();  // the accumulators that were asked for land first
               break;
             }
             load_ph ^= 1;
@@ -677,7 +685,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           }
         }
       }
-      if (!ok) break;
+      if (!ok) continue;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {

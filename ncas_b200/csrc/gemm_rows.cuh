@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
     __syncwarp();
   } else {
     const int q = warp & 3;  // tensor memory lanes 32 q .. 32 q + 31: an output each
-    const bool ok = mbar_wait(done, 0, fs, 113);
+    const bool ok = mbar_wait_warp(done, 0, fs, 113);
     tc_fence_after();
     if (p.slices > 1) cluster_started_wait();
     if (ok) {

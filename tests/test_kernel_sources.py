@@ -37,3 +37,23 @@ def test_remote_shared_memory_is_written_after_the_cluster_has_started(name, bod
     first = REMOTE_WRITE.search(body).start()
     arrive, wait = body.find("cluster_started_arrive()"), body.find("cluster_started_wait()")
     assert 0 <= arrive < wait < first, name
+
+
+def test_epilogue_warps_meet_at_the_named_barriers_after_a_failure():
+    # warps that leave the loop over tiles early would leave the others waiting at a barrier without a limit:
+    # after a wait that ran out, the loop goes on to the next tile's barriers
+    body = dict(kernels())["gemm.cuh:gemm_kernel"]
+    loop = body[body.index("} else if (warp >= 4) {") :]
+    barrier = loop.rindex('"bar.sync 1, 256;"')
+    tile = loop[loop.index("for (int t = first; t < tiles; t += step) {") : loop.index("cp.async.bulk.wait_group 0")]
+    leaves = [line for line in tile.splitlines() if "break;" in line]
+    assert [line.strip() for line in leaves] == ["break;"]  # of the pieces of a tile
+    assert "if (!ok) continue;" in loop[barrier:] and "return" not in tile
+
+
+def test_tensor_memory_is_read_by_whole_warps():
+    # tcgen05.ld takes all lanes: a wait before it may not let some lanes pass and others give up
+    for name in ("gemm.cuh:gemm_kernel", "gemm_rows.cuh:gemm_rows_kernel"):
+        body = dict(kernels())[name]
+        epilogue = body[body.index("    const int q = ") :]
+        assert "tmem_ld" in epilogue and "mbar_wait_warp(" in epilogue and "mbar_wait(" not in epilogue, name
