@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           }
         }
       }
-      if (!ok && rank == 0) {  // loads in flight land before this CTA leaves (bounded)
+      if (rank == 0) {  // loads in flight land before this CTA leaves, whichever warp gave up (bounded)
         for (long long i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
           for (int tries = 0; tries < 64 && !mbar_try_wait(&full[i % S::kStages], (i / S::kStages) & 1); ++tries) {
           }
@@ -481,10 +481,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
         buf ^= 1;
         if (buf == 0) acc_ph ^= 1;
       }
-      if (!ok) {  // the MMAs in flight end before the tensor memory is freed (bounded)
-        umma_commit_local<CG>(drained);
-        for (int tries = 0; tries < 64 && !mbar_try_wait(drained, 0); ++tries) {
-        }
+      // the MMAs in flight end before the tensor memory is freed, also when only the epilogue gave up (bounded)
+      umma_commit_local<CG>(drained);
+      for (int tries = 0; tries < 64 && !mbar_try_wait(drained, 0); ++tries) {
       }
     }
   } else if (warp >= 4) {

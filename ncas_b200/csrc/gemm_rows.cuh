@@ -115,10 +115,10 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
         load_w(s, kb0 + i);
         load_x(s, kb0 + i);
       }
-      if (i < n)  // loads in flight land before this CTA leaves (bounded)
-        for (int j = i > S::kStages ? i - S::kStages : 0; j < i; ++j)
-          for (int tries = 0; tries < 64 && !mbar_try_wait(&full[j % S::kStages], (j / S::kStages) & 1); ++tries) {
-          }
+      // loads in flight land before this CTA leaves, also when only another warp gave up (bounded)
+      for (int j = i > S::kStages ? i - S::kStages : 0; j < i; ++j)
+        for (int tries = 0; tries < 64 && !mbar_try_wait(&full[j % S::kStages], (j / S::kStages) & 1); ++tries) {
+        }
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -140,6 +140,9 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
         umma_commit(&empty[s]);
       }
       umma_commit(done);
+      // they end before the tensor memory is freed, also when only the epilogue gave up (bounded)
+      for (int tries = 0; tries < 64 && !mbar_try_wait(done, 0); ++tries) {
+      }
     }
     __syncwarp();
   } else {

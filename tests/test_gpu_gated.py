@@ -9,10 +9,13 @@ Tolerances follow the roundings, element by element (u the unit roundoff of the 
   dgate, dup      the same way from dh = dy Wd (|act''| <= 1.6), and u of themselves
   outputs         what their operands carry, e K sum |terms|, and u of themselves."""
 
+import ctypes as C
+
 import pytest
 import torch
 
 import oracle.cell_operators as O
+from ncas_b200 import _lib as L
 from ncas_b200 import operators as ops
 
 pytestmark = pytest.mark.gpu
@@ -312,6 +315,42 @@ def test_inside_a_cuda_graph():
         y.zero_()
         graph.replay()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("saved", [True, False])
+def test_a_wait_that_runs_out_is_reported(saved):
+    """The C ABI with a limit of 1 ms on products over 2^27 values a row: one tile, or the eighth of it that a
+    block of the few-row product takes, is at least 2^18 steps of 0.1 us, and a wait polls 64 times for at
+    most 0.5 ms before it looks at its limit.  The call ends with the status set, and the device goes on."""
+    lib = L.lib()
+    wide, out = 1 << 27, 8
+    x, w = (torch.zeros((1, wide), device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    down = torch.zeros((out, 1), device=DEV, dtype=torch.bfloat16)
+    bias = torch.ones(1, device=DEV)
+    y = torch.empty((1, out), device=DEV, dtype=torch.bfloat16)
+    ctrl = torch.zeros(4, device=DEV, dtype=torch.int32)
+    d = L.NcaGatedDesc(rows=1, d_in=wide, hidden=1, d_out=out, dtype=1, bias_dtype=0, act=2)
+    for name, t in (("x_stride", x), ("w_gate_stride", w), ("w_up_stride", w), ("w_down_stride", down)):
+        getattr(d, name)[0], getattr(d, name)[1] = t.stride()
+    size = C.c_size_t(0)
+    assert lib.nca_b200_gated_workspace(C.byref(d), 0, C.byref(size)) == 0
+    ws = torch.empty(size.value, device=DEV, dtype=torch.uint8)
+    assert lib.nca_b200_gated_saved_bytes(C.byref(d), C.byref(size)) == 0
+    kept = torch.empty(size.value, device=DEV, dtype=torch.uint8) if saved else None
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    p = lambda t: None if t is None else C.c_void_p(t.data_ptr())  # noqa: E731
+    detail = C.c_int32(0)
+    late = (104,) if saved else (112, 113)  # the second few-row product waits for the first
+    for limit, status, sites in ((1, 4, late), (20000, 0, (0,))):
+        st = lib.nca_b200_gated_ffn(C.byref(d), p(x), p(w), p(w), p(down), p(bias), p(bias), None, p(y), p(kept), p(ws),
+                                    ws.numel(), p(ctrl), limit, stream)
+        assert st == 0
+        assert lib.nca_b200_ctrl_status(p(ctrl), C.byref(detail), stream) == status
+        assert detail.value in sites
+        torch.cuda.synchronize()
+    assert (y == 0).all()
+    a, dy = make(70, 40, 56, 24, torch.bfloat16, seed=17)
+    check(a, dy)
 
 
 def test_refusals():

@@ -57,3 +57,13 @@ def test_tensor_memory_is_read_by_whole_warps():
         body = dict(kernels())[name]
         epilogue = body[body.index("    const int q = ") :]
         assert "tmem_ld" in epilogue and "mbar_wait_warp(" in epilogue and "mbar_wait(" not in epilogue, name
+
+
+def test_copies_and_products_in_flight_end_before_a_block_leaves():
+    # whichever warp gave up: the loads, and the MMAs before the tensor memory is freed
+    body = dict(kernels())["gemm.cuh:gemm_kernel"]
+    assert "\n      if (rank == 0) {  // loads in flight land" in body
+    assert "\n      umma_commit_local<CG>(drained);\n" in body
+    body = dict(kernels())["gemm_rows.cuh:gemm_rows_kernel"]
+    assert "\n      for (int j = i > S::kStages ? i - S::kStages : 0; j < i; ++j)" in body
+    assert body.count("mbar_try_wait(done, 0)") == 1
