@@ -382,7 +382,8 @@ int32_t nca_b200_gated_saved_bytes(const NcaGatedDesc* d, size_t* bytes);
  * and the backward's intermediates. */
 int32_t nca_b200_gated_workspace(const NcaGatedDesc* d, int32_t backward, size_t* bytes);
 /* saved: NULL for inference (h then lives in the workspace).  Biases may be NULL.  ctrl: 4 x int32
- * control words as for nca_b200_run_steps; a wait that exceeds timeout_ms gives up and sets them. */
+ * control words as for nca_b200_run_steps; a wait that exceeds timeout_ms gives up and sets them, and
+ * the outputs are then unfinished.  Words that an earlier call has set do not affect this one. */
 int32_t nca_b200_gated_ffn(const NcaGatedDesc* d, const void* x, const void* w_gate,
                            const void* w_up, const void* w_down, const void* b_gate,
                            const void* b_up, const void* b_down, void* y, void* saved,

@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 1 ? 0 : cta_rank_in_cluster();
-  const FailState fs{p.ctrl, abort_s, 0, p.timeout_ns};
+  const FailState fs{p.ctrl, abort_s, 0, p.timeout_ns, true};
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {

@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.slices > 1 ? (int)cta_rank_in_cluster() : 0;
   const int tile = blockIdx.x / p.slices;
-  const FailState fs{p.ctrl, abort_s, 0, p.timeout_ns};
+  const FailState fs{p.ctrl, abort_s, 0, p.timeout_ns, true};
 
   if (p.slices > 1) cluster_started_arrive();
   if (threadIdx.x == 0) {

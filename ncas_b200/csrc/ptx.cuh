@@ -67,6 +67,8 @@ struct FailState {
   volatile int* cta_abort;  // shared flag
   uint64_t deadline_ns;   // absolute globaltimer deadline for any single wait
   uint64_t timeout_ns;
+  bool alone = false;     // does not look at the abort word: its control words outlive the launch, and a failure of
+                          // another launch that nobody has read yet does not end this one
 };
 
 __device__ __forceinline__ void report_failure(const FailState& fs, int code, int where) {
@@ -76,7 +78,7 @@ __device__ __forceinline__ void report_failure(const FailState& fs, int code, in
 }
 
 __device__ __forceinline__ bool should_abort(const FailState& fs) {
-  return *fs.cta_abort != 0 || *((volatile int*)&fs.ctrl[3]) != 0;
+  return *fs.cta_abort != 0 || (!fs.alone && *((volatile int*)&fs.ctrl[3]) != 0);
 }
 
 // Bounded wait for the phase with `parity` to complete.  Returns false (after recording the

@@ -353,6 +353,35 @@ def test_a_wait_that_runs_out_is_reported(saved):
     check(a, dy)
 
 
+@pytest.mark.parametrize("saved", [True, False])
+def test_a_failure_that_nobody_has_read_does_not_end_later_calls(saved):
+    """The same products with control words that an earlier call has set: waits long enough to look at them
+    still end with the product, and the words stay for whoever asks."""
+    lib = L.lib()
+    wide, out = 1 << 27, 8
+    x, w = (torch.zeros((1, wide), device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    down = torch.ones((out, 1), device=DEV, dtype=torch.bfloat16)
+    bias = torch.ones(1, device=DEV)
+    y = torch.zeros((1, out), device=DEV, dtype=torch.bfloat16)
+    ctrl = torch.tensor([4, 77, 0, 1], device=DEV, dtype=torch.int32)
+    d = L.NcaGatedDesc(rows=1, d_in=wide, hidden=1, d_out=out, dtype=1, bias_dtype=0, act=1)
+    for name, t in (("x_stride", x), ("w_gate_stride", w), ("w_up_stride", w), ("w_down_stride", down)):
+        getattr(d, name)[0], getattr(d, name)[1] = t.stride()
+    size = C.c_size_t(0)
+    assert lib.nca_b200_gated_workspace(C.byref(d), 0, C.byref(size)) == 0
+    ws = torch.zeros(size.value, device=DEV, dtype=torch.uint8)
+    assert lib.nca_b200_gated_saved_bytes(C.byref(d), C.byref(size)) == 0
+    kept = torch.zeros(size.value, device=DEV, dtype=torch.uint8) if saved else None
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    p = lambda t: None if t is None else C.c_void_p(t.data_ptr())  # noqa: E731
+    st = lib.nca_b200_gated_ffn(C.byref(d), p(x), p(w), p(w), p(down), p(bias), p(bias), None, p(y), p(kept), p(ws),
+                                ws.numel(), p(ctrl), 20000, stream)
+    assert st == 0
+    detail = C.c_int32(0)
+    assert lib.nca_b200_ctrl_status(p(ctrl), C.byref(detail), stream) == 4 and detail.value == 77
+    assert (y == 1).all()  # relu(1) 1 through weights of 1
+
+
 def test_refusals():
     a, _ = make(4, 16, 24, 8, torch.bfloat16)
     for kw, exc, text in [
