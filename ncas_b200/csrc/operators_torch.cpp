@@ -247,19 +247,39 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight_,
 }
 
 // -------------------------------------------------------------------------------- gated block
-// Control words of the bounded waits, one set a device, kept for the process (operators.check()
-// reads and clears them).
+// Control words of the bounded waits, one set a device, kept for the process.  They record that a wait ran
+// out; whichever thread asks first (operators.check()) reads and clears them, and `count` tells the others.
+struct Failures {
+  std::mutex m, asking;
+  Tensor words;
+  int64_t count = 0;  // times that a failure was read
+  int32_t status = 0, detail = 0;  // the last
+};
+constexpr int kMostDevices = 64;
+Failures& failures(const c10::Device& dev) {
+  static auto& kept = *new std::array<Failures, kMostDevices>;  // never destroyed: CUDA may be gone by then
+  TORCH_CHECK(dev.index() >= 0 && dev.index() < kMostDevices, "device index ", (int)dev.index());
+  return kept[dev.index()];
+}
+// The failures that this thread knows of: those of its time, from its first call on.
+int64_t& known_failures(const c10::Device& dev) {
+  thread_local std::array<int64_t, kMostDevices> known = [] {
+    std::array<int64_t, kMostDevices> a;
+    a.fill(-1);
+    return a;
+  }();
+  return known[dev.index()];
+}
 Tensor control_words(const c10::Device& dev) {
-  static std::mutex m;
-  static auto& kept = *new std::array<Tensor, 64>;  // never destroyed: CUDA may be gone by then
-  const int i = dev.index();
-  TORCH_CHECK(i >= 0 && i < 64, "device index ", i);
-  std::lock_guard<std::mutex> lock(m);
-  if (!kept[i].defined()) {
-    kept[i] = at::zeros({4}, at::TensorOptions().device(dev).dtype(at::kInt));
-    at::cuda::getCurrentCUDAStream(i).synchronize();  // once: every stream finds them cleared
+  Failures& f = failures(dev);
+  std::lock_guard<std::mutex> lock(f.m);
+  if (!f.words.defined()) {
+    f.words = at::zeros({4}, at::TensorOptions().device(dev).dtype(at::kInt));
+    at::cuda::getCurrentCUDAStream(dev.index()).synchronize();  // once: every stream finds them cleared
   }
-  return kept[i];
+  int64_t& known = known_failures(dev);
+  if (known < 0) known = f.count;
+  return f.words;
 }
 // Limit of any single wait inside a kernel, as ncas_b200.engine reads it.
 int32_t timeout_ms() {
@@ -410,10 +430,22 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, cons
 std::vector<int64_t> operators_status(const Tensor& like) {
   on_cuda(like, "operators_status", "like");
   const c10::cuda::CUDAGuard guard(like.device());
+  const Tensor words = control_words(like.device());
+  Failures& f = failures(like.device());
+  std::lock_guard<std::mutex> one_at_a_time(f.asking);
   int32_t detail = 0;
-  const int32_t s =
-      nca_b200_ctrl_status(static_cast<int32_t*>(mptr(control_words(like.device()))), &detail, stream_of(like));
-  return {s, detail};
+  const int32_t s = nca_b200_ctrl_status(static_cast<int32_t*>(mptr(words)), &detail, stream_of(like));
+  if (s != NCA_OK && s != NCA_ERR_TIMEOUT) return {s, detail};
+  std::lock_guard<std::mutex> lock(f.m);
+  if (s != NCA_OK) {
+    ++f.count;
+    f.status = s;
+    f.detail = detail;
+  }
+  int64_t& known = known_failures(like.device());
+  if (known == f.count) return {NCA_OK, 0};
+  known = f.count;
+  return {f.status, f.detail};
 }
 
 // ------------------------------------------------------------------------------- distillation

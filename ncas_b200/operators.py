@@ -77,8 +77,12 @@ def distill_loss_and_grad(logits, teacher_logits, teacher_index, *, temperature=
 
 
 def check(device="cuda") -> None:
-    """Synchronises the current stream and raises NcaError when a kernel's bounded wait ran out since
-    the last call."""
+    """Synchronises the current stream and raises NcaError when a kernel's bounded wait ran out since this
+    thread's last call (at first: since it began to use the operators).
+
+    A gated_ffn whose wait ran out leaves its outputs unfinished; later calls are not affected.  The
+    record is the device's: every thread that uses the operators is told once, whichever of them ran
+    the call and whichever asks first."""
     status, site = _op("operators_status")(torch.empty(0, device=device))
     if status != 0:
         raise NcaError(status, "cell-training operators", site)

@@ -10,6 +10,10 @@ Tolerances follow the roundings, element by element (u the unit roundoff of the 
   outputs         what their operands carry, e K sum |terms|, and u of themselves."""
 
 import ctypes as C
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -380,6 +384,53 @@ def test_a_failure_that_nobody_has_read_does_not_end_later_calls(saved):
     detail = C.c_int32(0)
     assert lib.nca_b200_ctrl_status(p(ctrl), C.byref(detail), stream) == 4 and detail.value == 77
     assert (y == 1).all()  # relu(1) 1 through weights of 1
+
+
+THREADS = """
+import queue, threading
+import torch
+from ncas_b200 import operators as ops
+from ncas_b200._lib import NcaError
+
+def told():
+    try:
+        ops.check()
+    except NcaError:
+        return True
+    return False
+
+small = [torch.zeros(s, device="cuda", dtype=torch.bfloat16) for s in ((2, 8), (8, 8), (8, 8), (8, 8))]
+ask, answer = queue.Queue(), queue.Queue()
+def user():
+    torch.cuda.set_device(0)
+    ops.gated_ffn(*small)
+    answer.put(told())
+    while ask.get():
+        answer.put(told())
+other = threading.Thread(target=user)
+other.start()
+assert not answer.get() and not told()
+x, w = (torch.zeros((1, 1 << 27), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+ops.gated_ffn(x, w, w, small[0][:, :1])
+assert told() and not told()
+for first in (True, False):  # the other thread is told too, once
+    ask.put(True)
+    assert answer.get() == first
+ask.put(False)
+other.join()
+late = threading.Thread(target=lambda: answer.put(told()))  # began after the failure
+late.start()
+assert not answer.get()
+late.join()
+print("told")
+"""
+
+
+def test_every_thread_is_told_of_a_wait_that_ran_out():
+    env = {**os.environ, "NCA_B200_TIMEOUT_MS": "1"}
+    got = subprocess.run([sys.executable, "-c", THREADS], env=env, cwd=Path(__file__).parent.parent, capture_output=True,
+                         text=True, timeout=120)
+    assert got.returncode == 0 and got.stdout.split() == ["told"], got.stderr[-2000:]
 
 
 def test_refusals():
