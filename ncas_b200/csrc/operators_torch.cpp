@@ -100,10 +100,15 @@ size_t bytes_of(const Tensor& t) { return t.defined() ? (size_t)t.numel() : 0; }
 // one stride and the channels are adjacent, else a copy.
 struct Cells {
   Tensor t;
-  int64_t n, cells, stride_n, stride_cell;
+  int64_t n = 0, cells = 0, stride_n = 0, stride_cell = 0;
 };
 bool collapse(const Tensor& t, int64_t first, int64_t last, int64_t* size, int64_t* stride) {
   int64_t n = 1, s = 0;
+  for (int64_t i = first; i < last; ++i)
+    if (t.size(i) == 0) {  // no cells, whatever the strides
+      *size = *stride = 0;
+      return true;
+    }
   for (int64_t i = last - 1; i >= first; --i) {
     if (t.size(i) == 1) continue;
     if (n == 1) s = t.stride(i);

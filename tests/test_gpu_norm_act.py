@@ -216,6 +216,20 @@ def test_empty_batches():
         assert dx.shape == x.shape and (dw == 0).all() and (db == 0).all()
 
 
+@pytest.mark.parametrize("shape", [(2, 3, 0, 4), (2, 0, 3, 4), (3, 2, 0, 5, 4), (2, 5, 1, 0, 8), (0, 3, 0, 4)])
+def test_a_size_of_zero_among_the_cells(shape):
+    x = torch.empty(shape, device=DEV, requires_grad=True)
+    w = torch.ones(shape[-1], device=DEV, requires_grad=True)
+    for mask in (None, torch.ones(shape[:-1], device=DEV, dtype=torch.bool)):
+        with torch.no_grad():
+            assert ops.group_norm_act(x, 2, w, mask=mask).shape == shape
+        y = ops.group_norm_act(x, 2, w, mask=mask)
+        gx, gw = torch.autograd.grad(y.sum(), [x, w])
+        assert y.shape == shape and gx.shape == shape and (gw == 0).all()
+    view = torch.empty((2, 3, 6, 4), device=DEV)[:, :, 3:3]  # at an address, with strides of its own
+    assert ops.group_norm_act(view, 2).shape == (2, 3, 0, 4)
+
+
 def test_gradient_against_differences():
     # f(x + h v) - f(x - h v) over 2 h, in the kernel's own fp32: h = 2^-7 leaves h^2 / 6 f''' (about
     # 2^-16 of |f'|) and 2^-24 |f| 2^7 from rounding; f sums 2 * 20 * 12 terms of size about 1
