@@ -3,8 +3,9 @@
 //
 // Each operator checks its arguments (ValueError / TypeError with the argument's name), allocates
 // outputs and workspace from torch's caching allocator, and enqueues on torch's current stream of
-// the input's device.  The gradients are first-order: a backward pass under create_graph=True is
-// refused instead of giving a derivative that is silently constant.
+// the input's device.  The gradients are first-order and backward: a backward pass under
+// create_graph=True and forward-mode tangents are refused instead of giving a derivative that is
+// silently constant.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -68,6 +69,10 @@ void same_device(const Tensor& t, const Tensor& ref, const char* op, const char*
 }
 void first_order(const char* op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op, ": the backward pass is not differentiable (create_graph=True)");
+}
+void no_tangent(const Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK_VALUE(!t.defined() || !t._fw_grad(0).defined(), op, ": ", name,
+                    " carries a forward-mode tangent, and there is no forward-mode derivative");
 }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool any_grad(std::initializer_list<const Tensor*> ts) {
@@ -195,6 +200,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order("group_norm_act");
+    no_tangent(grads[0], "group_norm_act", "the gradient");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &mask = saved[3], &stats = saved[4];
     const c10::cuda::CUDAGuard guard(x.device());
@@ -222,6 +228,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight_,
                       std::string act_, const OptTensor& mask_) {
   constexpr const char* op = "group_norm_act";
   on_cuda(x, op, "x");
+  no_tangent(x, op, "x");
   dtype_of(x, op, "x");
   const int act = act_of(act_, false, op);
   TORCH_CHECK_VALUE(x.dim() >= 2, op, ": x must be (N, ..., C), not ", x.sizes());
@@ -232,6 +239,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight_,
   for (const auto& [t, name] : {std::pair<Tensor*, const char*>{&weight, "weight"}, {&bias, "bias"}}) {
     if (!t->defined()) continue;
     same_device(*t, x, op, name);
+    no_tangent(*t, op, name);
     TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == c, op, ": ", name, " must have shape (", c, "), not ", t->sizes());
     TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat || t->scalar_type() == x.scalar_type(), op, ": ", name,
                      " must be float32 or of x's type");
@@ -360,6 +368,7 @@ struct GatedFunction : torch::autograd::Function<GatedFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order("gated_ffn");
+    no_tangent(grads[0], "gated_ffn", "the gradient");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &wd = saved[3];
     const Tensor& dy = grads[0];
@@ -387,6 +396,7 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, cons
                  const OptTensor& b_gate, const OptTensor& b_up, const OptTensor& b_down, std::string act_) {
   constexpr const char* op = "gated_ffn";
   on_cuda(x, op, "x");
+  no_tangent(x, op, "x");
   const int act = act_of(act_, true, op);
   TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, op,
                    ": x must be bfloat16 or float16, not ", x.scalar_type());
@@ -394,6 +404,7 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, cons
   for (const auto& [t, name] : {std::pair<const Tensor*, const char*>{&w_gate, "w_gate"}, {&w_up, "w_up"},
                                 {&w_down, "w_down"}}) {
     same_device(*t, x, op, name);
+    no_tangent(*t, op, name);
     TORCH_CHECK_TYPE(t->scalar_type() == x.scalar_type(), op, ": ", name, " must be of x's type ", x.scalar_type(),
                      ", not ", t->scalar_type());
     TORCH_CHECK_VALUE(t->dim() == 2 && t->numel() > 0, op, ": ", name, " must be a non-empty matrix, not ", t->sizes());
@@ -410,6 +421,7 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, cons
   for (int i = 0; i < 3; ++i) {
     if (!b[i].defined()) continue;
     same_device(b[i], x, op, names[i]);
+    no_tangent(b[i], op, names[i]);
     TORCH_CHECK_VALUE(b[i].dim() == 1 && b[i].size(0) == sizes[i], op, ": ", names[i], " must have shape (", sizes[i],
                       "), not ", b[i].sizes());
     TORCH_CHECK_TYPE(b[i].scalar_type() == at::kFloat || b[i].scalar_type() == x.scalar_type(), op, ": ", names[i],
@@ -472,7 +484,9 @@ Distill distill_args(const Tensor& logits, const Tensor& teacher, const Tensor& 
   a.d.dtype = dtype_of(logits, op, "logits");
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0, op,
                     ": logits must be (..., classes) with classes > 0, not ", logits.sizes());
+  no_tangent(logits, op, "logits");
   same_device(teacher, logits, op, "teacher_logits");
+  no_tangent(teacher, op, "teacher_logits");
   same_device(index, logits, op, "teacher_index");
   a.d.teacher_dtype = dtype_of(teacher, op, "teacher_logits");
   TORCH_CHECK_TYPE(index.scalar_type() == at::kInt || index.scalar_type() == at::kLong, op,
@@ -495,6 +509,7 @@ Distill distill_args(const Tensor& logits, const Tensor& teacher, const Tensor& 
   a.index = rows && top ? rows_of(index, top) : index;
   if (weight.has_value() && weight->defined()) {
     same_device(*weight, logits, op, "weight");
+    no_tangent(*weight, op, "weight");
     TORCH_CHECK_TYPE(weight->scalar_type() == at::kFloat, op, ": weight must be float32");
     TORCH_CHECK_VALUE(weight->sizes() == logits.sizes().slice(0, logits.dim() - 1), op, ": weight must be ",
                       logits.sizes().slice(0, logits.dim() - 1), ", not ", weight->sizes());
@@ -539,6 +554,7 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order("distill_loss");
+    no_tangent(grads[0], "distill_loss", "the gradient");
     const auto saved = ctx->get_saved_variables();
     const Tensor& logits = saved[0];
     const c10::cuda::CUDAGuard guard(logits.device());
@@ -578,6 +594,7 @@ Tensor distill_loss(const Tensor& logits, const Tensor& teacher, const Tensor& i
 
 std::tuple<Tensor, Tensor> distill_loss_and_grad(const Tensor& logits_, const Tensor& teacher, const Tensor& index,
                                                  double temperature, const OptTensor& weight_, std::string reduction) {
+  no_tangent(logits_, "distill_loss_and_grad", "logits");
   const Tensor logits = logits_.detach();
   at::NoGradGuard no_grad;
   Distill a = distill_args(logits, teacher, index, temperature, weight_, "distill_loss_and_grad");

@@ -7,8 +7,10 @@
 
 The reference's cells have the first two as `norm_groups` and `update="swiglu"`
 (src/nca/model.py:48-137, 440-455), which the rollout kernels do not run.  The functions take CUDA
-tensors, run on torch's current stream, are differentiable (once) where a gradient is named, and
-raise ValueError or TypeError for arguments they do not take.  There is no CPU fallback.  Results do
+tensors, run on torch's current stream, are differentiable (once, backward) where a gradient is named,
+and raise ValueError or TypeError for arguments they do not take.  There is no CPU fallback, no
+forward-mode derivative and no form for torch.compile or vmap (a compiled or mapped function has to
+leave the calls out).  Results do
 not depend on the order in which blocks run.
 """
 

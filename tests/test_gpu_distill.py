@@ -10,6 +10,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import oracle.cell_operators as O
 from ncas_b200 import operators as ops
@@ -286,6 +287,21 @@ def test_repeatable_and_on_other_streams():
         got = ops.distill_loss_and_grad(s, t, i, weight=w)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_forward_mode_tangents_are_refused():
+    s, t, i, w = inputs(5, 9, 3, torch.float32)
+    with fwd.dual_level():
+        dual = lambda v: fwd.make_dual(v, torch.ones_like(v))  # noqa: E731
+        for call in (ops.distill_loss, ops.distill_loss_and_grad):
+            for name, args, kw in (("logits", (dual(s), t, i), {}), ("teacher_logits", (s, dual(t), i), {}),
+                                   ("weight", (s, t, i), dict(weight=dual(w)))):
+                with pytest.raises(ValueError, match=f"{name} carries a forward-mode tangent"):
+                    call(*args, **kw)
+        leaf = s.clone().requires_grad_()
+        loss = ops.distill_loss(leaf, t, i, reduction="none")
+        with pytest.raises(ValueError, match="tangent"):
+            torch.autograd.grad(loss, leaf, dual(torch.ones_like(loss)))
 
 
 def test_refusals():

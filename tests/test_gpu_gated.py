@@ -17,6 +17,7 @@ from pathlib import Path
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import oracle.cell_operators as O
 from ncas_b200 import _lib as L
@@ -431,6 +432,19 @@ def test_every_thread_is_told_of_a_wait_that_ran_out():
     got = subprocess.run([sys.executable, "-c", THREADS], env=env, cwd=Path(__file__).parent.parent, capture_output=True,
                          text=True, timeout=120)
     assert got.returncode == 0 and got.stdout.split() == ["told"], got.stderr[-2000:]
+
+
+def test_forward_mode_tangents_are_refused():
+    a, dy = make(4, 16, 24, 8, torch.bfloat16)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for k in NAMES:
+            with pytest.raises(ValueError, match=f"{k} carries a forward-mode tangent"):
+                ops.gated_ffn(**{**a, k: dual(a[k])})
+        leaf = a["x"].clone().requires_grad_()
+        y = ops.gated_ffn(**{**a, "x": leaf})
+        with pytest.raises(ValueError, match="tangent"):
+            torch.autograd.grad(y, leaf, dual(dy))
 
 
 def test_refusals():

@@ -9,6 +9,7 @@ the longest path of these sizes: 300 e sum |terms| (1 + max |x| rstd)."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import oracle.cell_operators as O
 from ncas_b200 import operators as ops
@@ -278,6 +279,19 @@ def test_inside_a_cuda_graph():
     y.zero_()
     graph.replay()
     assert torch.equal(y, want)
+
+
+def test_forward_mode_tangents_are_refused():
+    x, w = torch.ones((2, 3, 8), device=DEV), torch.ones(8, device=DEV)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for args in ((dual(x), 2, w, w), (x, 2, dual(w), w), (x, 2, w, dual(w))):
+            with pytest.raises(ValueError, match="tangent"):
+                ops.group_norm_act(*args)
+        leaf = x.clone().requires_grad_()
+        y = ops.group_norm_act(leaf, 2, w, w)
+        with pytest.raises(ValueError, match="tangent"):
+            torch.autograd.grad(y, leaf, dual(torch.ones_like(y)))
 
 
 def test_refusals():
