@@ -169,9 +169,10 @@ __device__ __forceinline__ void each_group(const NormArgs& a, long long item, F 
   while (l.count > 1 && groups * l.count > threads) l.count >>= 1;
   l.lane = threadIdx.x & (l.count - 1);
   for (int base = 0; base < groups; base += threads / l.count) {
-    const int g = first + base + threadIdx.x / l.count;
+    const bool in = base + (int)(threadIdx.x / l.count) < groups;  // past the last group a width of 0
+    const int g = first + (in ? base + (int)(threadIdx.x / l.count) : 0);  // (there g times per_group may pass 32 bits)
     const int lo = max(g * a.per_group, c_lo) - c_lo;
-    f(l, g, lo, max(0, min((g + 1) * a.per_group, c_hi) - c_lo - lo));  // width 0 past the last group
+    f(l, g, lo, in ? min((g + 1) * a.per_group, c_hi) - c_lo - lo : 0);
   }
 }
 
@@ -567,7 +568,7 @@ int32_t check_desc(const NcaNormDesc* d) {
   if (d->channels % d->groups) return NCA_ERR_INVALID;
   if (!dtype_ok(d->dtype) || (d->param_dtype != NCA_F32 && d->param_dtype != d->dtype)) return NCA_ERR_INVALID;
   if (d->act < NCA_ACT_NONE || d->act > NCA_ACT_SIGMOID || !(d->eps >= 0.f)) return NCA_ERR_INVALID;
-  if (d->cells > (1ll << 30) || d->n > (1ll << 40)) return NCA_ERR_UNSUPPORTED;
+  if (d->channels > (1 << 30) || d->cells > (1ll << 30) || d->n > (1ll << 40)) return NCA_ERR_UNSUPPORTED;
   return NCA_OK;
 }
 

@@ -138,6 +138,7 @@ Cells cells_of(const Tensor& x, bool channels) {
   return c;
 }
 
+constexpr int64_t kMostChannels = 1ll << 30;  // the kernels' channel numbers, and those of a tile beyond, fit 32 bits
 struct Norm {
   NcaNormDesc d{};
   static int unaligned(const Tensor& t) {
@@ -234,6 +235,7 @@ Tensor group_norm_act(const Tensor& x, int64_t groups, const OptTensor& weight_,
   TORCH_CHECK_VALUE(x.dim() >= 2, op, ": x must be (N, ..., C), not ", x.sizes());
   const int64_t c = x.size(-1);
   TORCH_CHECK_VALUE(c > 0 && groups > 0 && c % groups == 0, op, ": ", groups, " groups do not divide ", c, " channels");
+  TORCH_CHECK_VALUE(c <= kMostChannels, op, ": at most ", kMostChannels, " channels, not ", c);
   TORCH_CHECK_VALUE(eps >= 0, op, ": eps must not be negative");
   Tensor weight = or_none(weight_), bias = or_none(bias_), mask = or_none(mask_);
   for (const auto& [t, name] : {std::pair<Tensor*, const char*>{&weight, "weight"}, {&bias, "bias"}}) {

@@ -7,11 +7,14 @@ scale.  h = (x - mean) rstd carries e |x| rstd from the subtraction, so `scale` 
 times (1 + max |x| rstd).  A parameter's gradient adds at most 300 partial sums one after another on
 the longest path of these sizes: 300 e sum |terms| (1 + max |x| rstd)."""
 
+import ctypes as C
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
 import oracle.cell_operators as O
+from ncas_b200 import _lib as L
 from ncas_b200 import operators as ops
 
 pytestmark = pytest.mark.gpu
@@ -279,6 +282,31 @@ def test_inside_a_cuda_graph():
     y.zero_()
     graph.replay()
     assert torch.equal(y, want)
+
+
+def test_the_most_channels():
+    """2^30 channels in one group.  Tiles of 2048 channels hold +-k, k from 1 to 4: every sum is a whole
+    number below 2^24 times 2048, so mean and variance are exact and rstd carries its last roundings."""
+    c = 1 << 30
+    k = torch.randint(1, 5, (c // 2048, 1), generator=torch.Generator().manual_seed(8)).to(DEV, torch.float16)
+    x = (k * torch.tensor([1.0, -1.0], device=DEV, dtype=torch.float16).repeat(1024)).view(1, 1, c)
+    y = torch.empty_like(x)
+    stats = torch.zeros(2, device=DEV)
+    d = L.NcaNormDesc(n=1, cells=1, channels=c, groups=1, dtype=2, param_dtype=0, act=0, eps=0.0, x_stride_n=c, x_stride_cell=c)
+    lib, size, p = L.lib(), C.c_size_t(0), lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    assert lib.nca_b200_group_norm_workspace(C.byref(d), 0, C.byref(size)) == 0
+    ws = torch.empty(size.value, device=DEV, dtype=torch.uint8)
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert lib.nca_b200_group_norm(C.byref(d), p(x), None, None, None, p(y), p(stats), p(ws), ws.numel(), stream) == 0
+    rstd = 1 / float((k.double() ** 2).mean().sqrt())
+    assert stats[0].item() == 0 and abs(stats[1].item() - rstd) <= 4 * E * rstd
+    # y: one product and the rounding to fp16
+    want = x.double() * rstd
+    assert ((y.double() - want).abs() <= 2.0**-11 * want.abs() * 1.01).all()
+    with pytest.raises(ValueError, match="channels"):
+        ops.group_norm_act(torch.zeros((1, 1, 1), device=DEV).expand(1, 1, (1 << 30) + 8), 1)
+    with pytest.raises(ValueError, match="channels"):
+        ops.group_norm_act(torch.zeros((1, 1, 1), device=DEV).expand(1, 1, (1 << 32) + 8), 1)
 
 
 def test_forward_mode_tangents_are_refused():

@@ -101,6 +101,13 @@ def test_norm_descriptor_checks(lib):
     assert lib.nca_b200_group_norm(C.byref(d), *[None] * 7, 0, None) == 1
 
 
+def test_norm_channel_numbers_fit_32_bits(lib):
+    n = C.c_size_t(0)
+    ask = lambda c: lib.nca_b200_group_norm_workspace(  # noqa: E731
+        C.byref(norm_desc(n=1, cells=1, channels=c, groups=1)), 1, C.byref(n))
+    assert ask(1 << 30) == 0 and ask((1 << 30) + 1) == 2 and ask((1 << 31) - 1) == 2
+
+
 def gated_desc(**kw):
     d = L.NcaGatedDesc(rows=5, d_in=16, hidden=24, d_out=8, dtype=1, bias_dtype=0, act=2)
     for name, ld in (("x_stride", 16), ("w_gate_stride", 16), ("w_up_stride", 16), ("w_down_stride", 24),
