@@ -408,7 +408,7 @@ typedef struct NcaDistillDesc {
   int64_t top;                   /* <= 4096 */
   int32_t dtype, teacher_dtype;  /* NcaDtype */
   int32_t index_bits;            /* 32 or 64 */
-  float temperature;             /* tau > 0 */
+  float temperature;             /* tau, 1e-30 to 1e30 */
   int64_t logits_stride, teacher_stride, index_stride;   /* row strides; classes are adjacent */
 } NcaDistillDesc;
 

@@ -1212,7 +1212,8 @@ int32_t check_desc(const NcaDistillDesc* d) {
   if (!d || d->rows < 0 || d->classes <= 0 || d->top < 0) return NCA_ERR_INVALID;
   if (!dtype_ok(d->dtype) || !dtype_ok(d->teacher_dtype)) return NCA_ERR_INVALID;
   if (d->index_bits != 32 && d->index_bits != 64) return NCA_ERR_INVALID;
-  if (!(d->temperature > 0.f) || d->temperature > 1e30f) return NCA_ERR_INVALID;
+  // below, log2(e) / tau would overflow, and equal logits give 0 times infinity
+  if (!(d->temperature >= 1e-30f) || d->temperature > 1e30f) return NCA_ERR_INVALID;
   if (d->classes >= (1ll << 31) - 4096 || d->top > kMostEntries) return NCA_ERR_UNSUPPORTED;
   return NCA_OK;
 }

@@ -500,7 +500,8 @@ Distill distill_args(const Tensor& logits, const Tensor& teacher, const Tensor& 
   TORCH_CHECK_VALUE(index.sizes() == teacher.sizes(), op, ": teacher_index must be ", teacher.sizes(), ", not ",
                     index.sizes());
   TORCH_CHECK_VALUE(teacher.size(-1) <= 4096, op, ": at most 4096 entries a row, not ", teacher.size(-1));
-  TORCH_CHECK_VALUE(temperature > 0 && temperature <= 1e30, op, ": temperature must be positive and finite");
+  const float tau = (float)temperature;
+  TORCH_CHECK_VALUE(tau >= 1e-30f && tau <= 1e30f, op, ": temperature must lie between 1e-30 and 1e30, not ", temperature);
   TORCH_CHECK_VALUE(!teacher.requires_grad() || !at::GradMode::is_enabled(), op,
                     ": teacher_logits gets no gradient: detach it");
   int64_t rows = 1;
@@ -523,7 +524,7 @@ Distill distill_args(const Tensor& logits, const Tensor& teacher, const Tensor& 
   a.d.classes = logits.size(-1);
   a.d.top = top;
   a.d.index_bits = index.scalar_type() == at::kInt ? 32 : 64;
-  a.d.temperature = (float)temperature;
+  a.d.temperature = tau;
   a.d.logits_stride = rows > 1 ? a.logits.stride(0) : a.d.classes;
   a.d.teacher_stride = rows > 1 && top ? a.teacher.stride(0) : top;
   a.d.index_stride = rows > 1 && top ? a.index.stride(0) : top;

@@ -64,7 +64,7 @@ def distill_loss(logits, teacher_logits, teacher_index, *, temperature=1.0, weig
     logits (..., classes); teacher_logits (..., top) with the classes they belong to in teacher_index
     (int32 or int64; an index outside [0, classes), such as -1, marks no entry; entries of one class
     add up).  weight: float32 (...).  A row without entries or with weight 0 has loss and gradient 0.
-    reduction: "none" (float32, (...)), "sum", or "mean" over all rows.  Differentiable in logits.
+    temperature: 1e-30 to 1e30.  reduction: "none" (float32, (...)), "sum", or "mean" over all rows.  Differentiable in logits.
     The same call gives the same bits; another number of rows, or distill_loss_and_grad, may run another
     kernel, whose sums differ by rounding.
     """

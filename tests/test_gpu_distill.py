@@ -289,6 +289,23 @@ def test_repeatable_and_on_other_streams():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("classes", [2, 9, 300, 700, 5000])
+def test_temperatures_at_the_ends(classes):
+    # so small that the largest logit takes all of q, and p sits on another class: loss tau^2 (gap / tau) = tau gap
+    s = torch.zeros((3, classes), device=DEV)
+    s[:, 1] = 2.0
+    t, i = torch.tensor([[1.0, 0.0]] * 3, device=DEV), torch.tensor([[0, 1]] * 3, device=DEV)
+    tau = 1e-20
+    loss, grad = ops.distill_loss_and_grad(s, t, i, temperature=tau, reduction="none")
+    assert ((loss - tau * 2.0).abs() <= 2.0**-20 * tau * 2.0).all()
+    want = torch.zeros((3, classes), device=DEV)
+    want[:, 0], want[:, 1] = -tau, tau
+    assert ((grad - want).abs() <= 2.0**-20 * tau).all()
+    for bad in (1e-31, 1e-40, 1e-60, 1e31, 1e60, float("inf"), -1.0):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.distill_loss(s, t, i, temperature=bad)
+
+
 def test_forward_mode_tangents_are_refused():
     s, t, i, w = inputs(5, 9, 3, torch.float32)
     with fwd.dual_level():

@@ -159,6 +159,16 @@ def test_distill_descriptor_checks(lib):
     assert ask(classes=1 << 31) == 2
 
 
+def test_distill_temperatures_whose_reciprocal_overflows_are_refused(lib):
+    n = C.c_size_t(0)
+    ask = lambda t: lib.nca_b200_distill_workspace(C.byref(L.NcaDistillDesc(  # noqa: E731
+        rows=4, classes=9, top=3, dtype=0, teacher_dtype=0, index_bits=32, temperature=t, logits_stride=9,
+        teacher_stride=3, index_stride=3)), C.byref(n))
+    assert ask(1e-29) == 0 and ask(1e29) == 0
+    for t in (1e-39, 1e-44, 9e-31, 1.1e30):
+        assert ask(t) == 1, t
+
+
 def test_operators_are_registered_with_their_schemas(lib):
     from ncas_b200._ops import ops as torch_ops
 
