@@ -379,7 +379,8 @@ typedef struct NcaGatedDesc {
 int32_t nca_b200_gated_saved_bytes(const NcaGatedDesc* d, size_t* bytes);
 /* The workspace holds copies of the operands that the tensor-memory accelerator cannot read as they
  * lie (columns not adjacent, rows or pointer not on 16-byte boundaries), h of an inference call,
- * and the backward's intermediates. */
+ * and the backward's intermediates.  backward: 0 forward, 1 backward, 2 backward with db_gate and db_up
+ * NULL, which needs less. */
 int32_t nca_b200_gated_workspace(const NcaGatedDesc* d, int32_t backward, size_t* bytes);
 /* saved: NULL for inference (h then lives in the workspace).  Biases may be NULL.  ctrl: 4 x int32
  * control words as for nca_b200_run_steps; a wait that exceeds timeout_ms gives up and sets them, and

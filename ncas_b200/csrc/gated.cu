@@ -481,7 +481,8 @@ struct Plan {
   long long fp;  // padded hidden
 };
 
-Plan plan_of(const NcaGatedDesc& d, bool backward) {
+// bias_sums: room for the column sums that the gradients of b_gate and b_up are made of.
+Plan plan_of(const NcaGatedDesc& d, bool backward, bool bias_sums = true) {
   Plan p{};
   const long long rows[OPS] = {d.rows, d.hidden, d.hidden, d.d_out, d.rows};
   const long long cols[OPS] = {d.d_in, d.d_in, d.d_in, d.hidden, d.d_out};
@@ -519,7 +520,7 @@ Plan plan_of(const NcaGatedDesc& d, bool backward) {
     p.sums = at;
     at += align256(((size_t)kRowPieces * 2 * p.fp + (size_t)(kSumSplits + kRowPieces) * pad8(d.d_out)) * sizeof(float));
     p.cols = at;
-    at += align256((size_t)ceil_div(d.rows, 128) * 4 * 2 * p.fp * sizeof(float));
+    if (bias_sums) at += align256((size_t)ceil_div(d.rows, 128) * 4 * 2 * p.fp * sizeof(float));
   }
   p.total = at + 256;
   return p;
@@ -753,7 +754,7 @@ int32_t nca_b200_gated_saved_bytes(const NcaGatedDesc* d, size_t* bytes) {
 int32_t nca_b200_gated_workspace(const NcaGatedDesc* d, int32_t backward, size_t* bytes) {
   const int32_t st = check_desc(d);
   if (st != NCA_OK || !bytes) return st != NCA_OK ? st : NCA_ERR_INVALID;
-  *bytes = plan_of(*d, backward != 0).total;
+  *bytes = plan_of(*d, backward != 0, backward != 2).total;
   return NCA_OK;
 }
 
@@ -791,7 +792,8 @@ int32_t nca_b200_gated_ffn_backward(const NcaGatedDesc* d, const void* x, const 
       if (o.p && cudaMemsetAsync(o.p, 0, o.bytes, s) != cudaSuccess) return NCA_ERR_CUDA;
     return NCA_OK;
   }
-  if (!saved || !dy || !workspace || !ctrl || workspace_bytes < plan_of(*d, true).total) return NCA_ERR_INVALID;
+  if (!saved || !dy || !workspace || !ctrl || workspace_bytes < plan_of(*d, true, db_gate || db_up).total)
+    return NCA_ERR_INVALID;
   NCA_TRY(bind_context());
   GemmParams base = base_params(*d, ctrl, timeout_ms);
   return dispatch(*d, BackwardCall{*d, x, w_gate, w_up, w_down, saved, dy, dx, dw_gate, dw_up, dw_down, db_gate, db_up,

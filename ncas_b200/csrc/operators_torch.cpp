@@ -383,7 +383,7 @@ struct GatedFunction : torch::autograd::Function<GatedFunction> {
       if (needs[i])
         out[i] = at::empty(saved[i].sizes(), saved[i].options().memory_format(at::MemoryFormat::Contiguous));
     size_t bytes = 0;
-    check(nca_b200_gated_workspace(&g.d, 1, &bytes), "nca_b200_gated_workspace");
+    check(nca_b200_gated_workspace(&g.d, needs[4] || needs[5] ? 1 : 2, &bytes), "nca_b200_gated_workspace");
     Tensor ws = scratch(bytes, x), ctrl = control_words(x.device());
     check(nca_b200_gated_ffn_backward(&g.d, ptr(x), ptr(wg), ptr(wu), ptr(wd), ptr(saved[7]), ptr(dy), mptr(out[0]),
                                       mptr(out[1]), mptr(out[2]), mptr(out[3]), mptr(out[4]), mptr(out[5]),

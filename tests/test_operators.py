@@ -141,6 +141,16 @@ def test_gated_descriptor_checks(lib):
     assert lib.nca_b200_gated_ffn(C.byref(d), *[None] * 10, 0, None, 0, None) == 1
 
 
+def test_gated_backward_without_biases_needs_no_room_for_their_sums(lib):
+    def ask(bwd, rows):
+        n = C.c_size_t(0)
+        assert lib.nca_b200_gated_workspace(C.byref(gated_desc(rows=rows)), bwd, C.byref(n)) == 0
+        return n.value
+
+    for rows in (1, 5, 1000, 100000):  # a sum of every 32 rows of the tiles of 128, of both matrices, in fp32
+        assert ask(1, rows) - ask(2, rows) == 4 * -(-rows // 128) * 2 * 24 * 4
+
+
 def test_distill_descriptor_checks(lib):
     n = C.c_size_t(0)
 
