@@ -284,6 +284,56 @@ def test_inside_a_cuda_graph():
     assert torch.equal(y, want)
 
 
+@pytest.mark.parametrize("dtype,shift", [(torch.float32, 1e2), (torch.float32, 1e3), (torch.float32, 1e4), (torch.float16, 1e2)])
+@pytest.mark.parametrize("n,cells,c,groups", [
+    (3, 81, 64, 8), (4, 3481, 32, 4), (2, 20000, 64, 1), (3, 300, 33, 3), (2, 70, 1030, 2)])
+def test_means_far_from_zero(dtype, shift, n, cells, c, groups):
+    """Data of unit spread far from zero, with bounds that stay well below the outputs' spread.
+
+    far = max |x| rstd.  The mean is at most 64 roundings of |x| off: mean and h by 64 e far (and a rounding
+    of x - mean).  The sums of (x - K)^2 of a thread cancel to half on average and take at most 64 additions:
+    2 * 2 * 64 e of the variance, doubled for its spread over the threads; a thread's mean, rounded to e |x|,
+    enters the merged variance with its distance from the mean (below 1 in units of the spread): 2 e far;
+    and the variance about a mean that is off is larger by (64 e far)^2.  rstd takes half of these.
+    The gradients carry h's error through their sums, and 64 additions (300 over the samples)."""
+    x = normal(n, cells, c, seed=cells, shift=shift).to(DEV, dtype)
+    w, b = normal(c, seed=1, scale=0.3, shift=1.0).to(DEV), normal(c, seed=2, scale=0.3).to(DEV)
+    dy = normal(n, cells, c, seed=3).to(DEV, dtype)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = ops.group_norm_act(leaves[0], groups, leaves[1], leaves[2], act="none")
+    got = torch.autograd.grad(y, leaves, dy)
+    wy, wdx, wdw, wdb = O.group_norm_act(x.cpu(), groups, w.cpu(), b.cpu(), 1e-5, "none", None, dy.cpu())
+    u = UNIT[dtype]
+    xs = x.cpu().double().view(n, cells, groups, c // groups)
+    mean = xs.mean((1, 3), keepdim=True)
+    rstd = 1 / torch.sqrt(xs.var((1, 3), keepdim=True, unbiased=False) + 1e-5)
+    h = (xs - mean) * rstd
+    wv, bv = (t.cpu().double().view(groups, c // groups) for t in (w, b))
+    g = dy.cpu().double().view(xs.shape)
+    wg = wv * g
+    far = float((xs.abs() * rstd).max())
+    assert 0.5 * shift < far < 4 * shift
+    off = 65 * E * far                                    # of h
+    r = 256 * E + E * far + 0.5 * (64 * E * far) ** 2     # of rstd, relative
+    flat = lambda t: t.reshape(n, cells, c)  # noqa: E731
+    ty = flat(wv.abs() * (off + h.abs() * r) + 4 * E * ((wv * h).abs() + bv.abs())) + u * wy.abs()
+    assert float(ty.max()) < 0.25 * float(wy.std())
+    close(y, wy, ty, "y")
+    m = lambda t: t.mean((1, 3), keepdim=True)  # noqa: E731
+    bn = m(wg * h).abs()
+    tb = m(wg.abs()) * off + r * bn + 64 * E * m((wg * h).abs())
+    tx = rstd * (64 * E * m(wg.abs()) + h.abs() * tb + (off + h.abs() * r) * (bn + tb) + 4 * E * (wg.abs() + bn * h.abs()))
+    tx = flat(tx * (1 + r)) + (r + u) * wdx.abs()
+    assert float(tx.max()) < 0.25 * float(wdx.std())
+    close(got[0], wdx, tx, "dx")
+    s = lambda t: t.sum((0, 1)).reshape(c)  # noqa: E731
+    tw = s(g.abs() * (off + h.abs() * r)) + 300 * E * s((g * h).abs()) + UNIT[w.dtype] * wdw.abs()
+    if shift < 1e3:
+        assert float(tw.max()) < 0.5 * float(wdw.std())
+    close(got[1], wdw, tw, "dweight")
+    close(got[2], wdb, 300 * E * s(g.abs()) + UNIT[b.dtype] * wdb.abs(), "dbias")
+
+
 def test_the_most_channels():
     """2^30 channels in one group.  Tiles of 2048 channels hold +-k, k from 1 to 4: every sum is a whole
     number below 2^24 times 2048, so mean and variance are exact and rstd carries its last roundings."""
