@@ -129,13 +129,6 @@ __device__ __forceinline__ float2 act_slope2(float2 z, float2& a) {
 }
 template <int ACT>
 __device__ __forceinline__ float act_f(float z) { return act2<ACT>(both(z)).x; }
-template <int ACT>
-__device__ __forceinline__ float act_slope_f(float z, float& a) {
-  float2 v;
-  const float2 d = act_slope2<ACT>(both(z), v);
-  a = v.x;
-  return d.x;
-}
 
 // V values of a vector as pairs (the pair of a single value repeats it).
 template <class T, int V>

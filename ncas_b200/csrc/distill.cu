@@ -1193,7 +1193,9 @@ int32_t dispatch(const NcaDistillDesc& d, const DistillArgs& a, cudaStream_t s) 
         if (bytes <= held(256, 0)) return launch_held<T, 256, 0, 3, FWD>(a, 1, s);
         if (bytes <= held(384, 0)) return launch_held<T, 384, 0, 2, FWD>(a, 1, s);
         // the loss alone needs no second look at a row: 4000 x 65536 bf16 123 us, held 210
-        if (FWD && !a.dlogits && bytes > kMiddle) return launch_rows<T, 256, FWD>(a, 1, s);
+        if constexpr (FWD) {
+          if (!a.dlogits && bytes > kMiddle) return launch_rows<T, 256, FWD>(a, 1, s);
+        }
         if (bytes > kMiddle && bytes <= held(256, 13)) return launch_held<T, 256, 13, 3, FWD>(a, 1, s);
         if (bytes > kMiddle && bytes <= held(480, 10)) return launch_held<T, 480, 10, 2, FWD>(a, 1, s);
       }

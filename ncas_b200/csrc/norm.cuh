@@ -1,4 +1,4 @@
-// norm.cuh -- arguments that the streaming (norm.cu) and the held (norm_held.cu) group norm share.
+// norm.cuh -- arguments that the streaming (norm.cu) and the held (norm_held*.cu) group norm share.
 #pragma once
 #include "cell_ops.cuh"
 
