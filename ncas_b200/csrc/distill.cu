@@ -8,9 +8,9 @@
 // product with the scale would overflow, still gives differences of 0.
 //
 // Which lanes share a row goes by its size (dispatch, below).  On a B200: 900,000 x 2 bf16 12.9 us in all
-// (2.0 TB/s; instructions bind), 150,022 x 662 fp16 with 90 entries 261 us (the entries' instructions),
-// 2047 x 32003 fp16 55 us (4.7 TB/s), 8192 x 131072 bf16 with gradient 780 to 830 us (5.2 to 5.5 TB/s,
-// near HBM; the exponentials take 60% of their unit).
+// (2.0 TB/s; instructions bind, 74% of the issue slots), 150,022 x 662 fp16 with 90 entries 246 to 261 us,
+// 2047 x 32003 fp16 55 us (4.7 TB/s), 8192 x 131072 bf16 with gradient 770 to 840 us (5.1 to 5.6 TB/s,
+// near HBM; the exponentials take 58% of their unit).
 #include "cell_ops.cuh"
 #include <atomic>
 #include <type_traits>

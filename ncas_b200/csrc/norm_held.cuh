@@ -7,10 +7,11 @@
 // thread waits for another's data (norm_held_forward.cu, norm_held_backward.cu); statistics are merged through shared memory, and over a cluster
 // through distributed shared memory.
 //
-// The mathematics and the treatment of sums are those of norm.cu.  Bound by HBM; the copies of the
-// blocks that share a multiprocessor overlap with each other's arithmetic and writes.  On a B200, 8000
-// samples of 81 x 64 fp32, silu: forward 61 us (5.4 TB/s), backward 115 us (4.3 TB/s; its arithmetic
-// and 5 blocks a multiprocessor bind).
+// The mathematics and the treatment of sums are those of norm.cu.  Bound by HBM and, close behind, by
+// instructions; the copies of the blocks that share a multiprocessor overlap with each other's arithmetic
+// and writes.  On a B200, 8000 samples of 81 x 64 fp32, silu: forward 58 to 61 us (5.4 to 5.7 TB/s, 66% of
+// the issue slots), backward 109 to 115 us (4.3 to 4.6 TB/s; its arithmetic, 62% of the issue slots, and 4
+// blocks a multiprocessor bind).
 #pragma once
 #include <algorithm>
 #include <atomic>
