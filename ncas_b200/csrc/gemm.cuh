@@ -187,6 +187,58 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, c
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, fs, where));
 }
 
+// Accumulators out of tensor memory, n columns of the warp's lanes.  One statement loads them and waits: the
+// registers of a load in flight may not be touched, and between two statements the compiler may move them
+// (with the wait behind the planes' barrier, dgate and dup of the first tiles were wrong now and then).
+__device__ __forceinline__ void tmem_take16(uint32_t a, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15])
+      : "r"(a)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_take32(uint32_t a, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(a)
+      : "memory");
+}
+// (&: written before a1 is read)
+__device__ __forceinline__ void tmem_take32(uint32_t a0, uint32_t a1, uint32_t (&r0)[32], uint32_t (&r1)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=&r"(r0[0]), "=&r"(r0[1]), "=&r"(r0[2]), "=&r"(r0[3]), "=&r"(r0[4]), "=&r"(r0[5]), "=&r"(r0[6]),
+        "=&r"(r0[7]), "=&r"(r0[8]), "=&r"(r0[9]), "=&r"(r0[10]), "=&r"(r0[11]), "=&r"(r0[12]), "=&r"(r0[13]),
+        "=&r"(r0[14]), "=&r"(r0[15]), "=&r"(r0[16]), "=&r"(r0[17]), "=&r"(r0[18]), "=&r"(r0[19]), "=&r"(r0[20]),
+        "=&r"(r0[21]), "=&r"(r0[22]), "=&r"(r0[23]), "=&r"(r0[24]), "=&r"(r0[25]), "=&r"(r0[26]), "=&r"(r0[27]),
+        "=&r"(r0[28]), "=&r"(r0[29]), "=&r"(r0[30]), "=&r"(r0[31]), "=r"(r1[0]), "=r"(r1[1]), "=r"(r1[2]),
+        "=r"(r1[3]), "=r"(r1[4]), "=r"(r1[5]), "=r"(r1[6]), "=r"(r1[7]), "=r"(r1[8]), "=r"(r1[9]),
+        "=r"(r1[10]), "=r"(r1[11]), "=r"(r1[12]), "=r"(r1[13]), "=r"(r1[14]), "=r"(r1[15]), "=r"(r1[16]),
+        "=r"(r1[17]), "=r"(r1[18]), "=r"(r1[19]), "=r"(r1[20]), "=r"(r1[21]), "=r"(r1[22]), "=r"(r1[23]),
+        "=r"(r1[24]), "=r"(r1[25]), "=r"(r1[26]), "=r"(r1[27]), "=r"(r1[28]), "=r"(r1[29]), "=r"(r1[30]),
+        "=r"(r1[31])
+      : "r"(a0), "r"(a1)
+      : "memory");
+}
+
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <>
@@ -528,13 +580,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
       for (int c = 32 * turn; c < cols; c += 64) {
         const int col = tl.n0 + c, n = min(32, cols - c);
         uint32_t r0[32];
-        tmem_ld32(acc + c, r0);
         if constexpr (EPI == EPI_GATE) {
           uint32_t r1[32];
-          tmem_ld32(acc + kTN + c, r1);
-          tc_wait_ld_regs(r0);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r1[i]));
+          tmem_take32(acc + c, acc + kTN + c, r0, r1);
           float g[32], u[32], h[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
@@ -579,10 +627,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
           float g[32], u[32];
           if (rows > 0) {
             ok = mbar_wait_warp(&loaded[warp - 4], load_ph, fs, 105);
-            if (!ok) {
-              tc_wait_ld();  // the accumulators that were asked for land first
-              break;
-            }
+            if (!ok) break;
             load_ph ^= 1;
             pending = false;
             uint4 k0[4], k1[4], k2[4];
@@ -594,7 +639,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             join_planes(k0, k1, k2, g, u);
           }
           if (lane == 0) bulk_wait_read<0>();  // the places have been read
-          tc_wait_ld_regs(r0);
+          __syncwarp();
+          tmem_take32(acc + c, r0);
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             const float2 dh = make_float2(__uint_as_float(r0[i]), __uint_as_float(r0[i + 1]));
@@ -635,7 +681,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             bulk_commit();
           }
         } else if constexpr (EPI == EPI_PARTIAL) {
-          tc_wait_ld_regs(r0);
+          tmem_take32(acc + c, r0);
           if (lane == 0) bulk_wait_read<0>();
           __syncwarp();
 #pragma unroll
@@ -656,7 +702,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             bulk_commit();
           }
         } else {
-          tc_wait_ld_regs(r0);
+          tmem_take32(acc + c, r0);
           float f[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r0[i]);

@@ -158,8 +158,7 @@ __global__ void __launch_bounds__(kRowsThreads) gemm_rows_kernel(const __grid_co
 #pragma unroll
         for (int c = 0; c < N; c += 16) {
           uint32_t r[16];
-          tmem_ld16(tmem + a * N + c + ((uint32_t)(32 * q) << 16), r);
-          tc_wait_ld_regs(r);
+          tmem_take16(tmem + a * N + c + ((uint32_t)(32 * q) << 16), r);
           float* mine = sums + ((rank * S::kAcc + a) * share + at) * S::kRow + c;
           if (p.slices > 1) {
             const uint32_t far = map_to_rank(smem_u32(mine), to);

@@ -158,6 +158,20 @@ def test_tiles_without_rows_between_tiles_with_rows(dtype, t, d, f, o):
             assert torch.equal(g, grads[k]), k
 
 
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_first_tiles_of_many_repeat(dtype, act):
+    # the saved planes of a block's first tile are there before its accumulators: 12 x 8 tiles of 256 x 256
+    # of dh, each block's first piece against the oracle, and bit for bit in ten runs
+    a, dy = make(3001, 80, 2000, 208, dtype, seed=18)
+    _, grads = check(a, dy, act)
+    for _ in range(10):
+        leaves = {k: v.detach().requires_grad_() for k, v in a.items()}
+        got = torch.autograd.grad(ops.gated_ffn(**leaves, act=act), list(leaves.values()), dy)
+        for k, g in zip(leaves, got):
+            assert torch.equal(g, grads[k]), k
+
+
 def test_long_row_axis_in_pieces():
     check(*make(20001, 64, 72, 24, torch.bfloat16, seed=6))
 

@@ -47,7 +47,7 @@ def test_epilogue_warps_meet_at_the_named_barriers_after_a_failure():
     barrier = loop.rindex('"bar.sync 1, 256;"')
     tile = loop[loop.index("for (int t = first; t < tiles; t += step) {") : loop.index("cp.async.bulk.wait_group 0")]
     leaves = [line for line in tile.splitlines() if "break;" in line]
-    assert [line.strip() for line in leaves] == ["break;"]  # of the pieces of a tile
+    assert [line.strip() for line in leaves] == ["if (!ok) break;"]  # of the pieces of a tile
     assert "if (!ok) continue;" in loop[barrier:] and "return" not in tile
 
 
@@ -56,7 +56,17 @@ def test_tensor_memory_is_read_by_whole_warps():
     for name in ("gemm.cuh:gemm_kernel", "gemm_rows.cuh:gemm_rows_kernel"):
         body = dict(kernels())[name]
         epilogue = body[body.index("    const int q = ") :]
-        assert "tmem_ld" in epilogue and "mbar_wait_warp(" in epilogue and "mbar_wait(" not in epilogue, name
+        assert "tmem_take" in epilogue and "mbar_wait_warp(" in epilogue and "mbar_wait(" not in epilogue, name
+
+
+def test_accumulators_are_loaded_and_waited_for_in_one_statement():
+    # the registers of a load from tensor memory are its own until the wait: code between two statements can move them
+    files = {f: (CSRC / f).read_text() for f in ("gemm.cuh", "gemm_rows.cuh")}
+    statements = re.findall(r"asm volatile\((.*?)\);", files["gemm.cuh"], re.S)
+    loads = [s for s in statements if "tcgen05.ld." in s]
+    assert len(loads) == 3 and all(s.rindex("tcgen05.ld.") < s.index("tcgen05.wait::ld") for s in loads)
+    for text in files.values():
+        assert "tmem_ld" not in text and "tc_wait_ld" not in text
 
 
 def test_copies_and_products_in_flight_end_before_a_block_leaves():
