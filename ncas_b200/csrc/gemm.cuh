@@ -634,6 +634,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1) gemm_kernel(const __grid_cons
             take_row(place + kPlace, lane, k0);
             take_row(place + 2 * kPlace, lane, k1);
             take_row(place + 3 * kPlace, lane, k2);
+            // every lane's reads come before the copy that overwrites them: without the fence some may be moved
+            // behind it, and a warp that was then held up read the next piece's planes
+            fence_async_proxy();
             __syncwarp();
             if (c + 64 < cols) ask(c + 64);
             join_planes(k0, k1, k2, g, u);

@@ -172,6 +172,22 @@ def test_first_tiles_of_many_repeat(dtype, act):
             assert torch.equal(g, grads[k]), k
 
 
+@pytest.mark.parametrize("dtype,act", [(torch.float16, "sigmoid"), (torch.bfloat16, "sigmoid"), (torch.bfloat16, "silu")])
+def test_backward_of_many_pieces_repeats(dtype, act):
+    # 294 x 18 tiles of dh, 8 pieces of 32 columns each: a piece's planes are asked for as soon as those
+    # before have been read
+    g = torch.Generator(device=DEV).manual_seed(19)
+    r = lambda *s, k=1.0: torch.randn(s, generator=g, device=DEV).mul_(k).to(dtype)  # noqa: E731
+    t, d, f, o = 75243, 56, 4444, 639
+    leaves = [v.requires_grad_() for v in (r(t, d), r(f, d, k=d**-0.5), r(f, d, k=d**-0.5), r(o, f, k=f**-0.5),
+                                           r(f, k=0.1), r(f, k=0.1), r(o, k=0.1))]
+    y, dy = ops.gated_ffn(*leaves, act=act), r(t, o)
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    for _ in range(150):
+        got = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(first, got))
+
+
 def test_long_row_axis_in_pieces():
     check(*make(20001, 64, 72, 24, torch.bfloat16, seed=6))
 

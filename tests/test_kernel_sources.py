@@ -69,6 +69,13 @@ def test_accumulators_are_loaded_and_waited_for_in_one_statement():
         assert "tmem_ld" not in text and "tc_wait_ld" not in text
 
 
+def test_planes_are_read_before_they_are_asked_for_again():
+    body = dict(kernels())["gemm.cuh:gemm_kernel"]
+    read, fence = body.rindex("take_row("), body.index("fence_async_proxy();", body.rindex("take_row("))
+    assert read < fence < body.index("__syncwarp();", fence) < body.index("ask(c + 64);")
+    assert "put_row" not in body[read:fence] and "ask(" not in body[read:fence]
+
+
 def test_copies_and_products_in_flight_end_before_a_block_leaves():
     # whichever warp gave up: the loads, and the MMAs before the tensor memory is freed
     body = dict(kernels())["gemm.cuh:gemm_kernel"]
