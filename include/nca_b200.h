@@ -426,6 +426,38 @@ int32_t nca_b200_distill_backward(const NcaDistillDesc* d, const void* logits, c
                                   const float* grad, int64_t grad_stride, void* dlogits,
                                   void* stream);
 
+/* The gated scan along lines: h_t = a_t h_{t-1} + (1 - a_t) x_t with a = sigmoid(gate), y_t = h_t, over
+ * n x m lines of `steps` steps and `channels` channels.  A masked step (mask 0) leaves the state as
+ * it is; its y and gradients are 0, and what x, gate and dy hold there has no effect.  reverse: from
+ * the last step to the first. */
+typedef struct NcaScanDesc {
+  int64_t n, m, steps;
+  int32_t channels;
+  int32_t dtype;                 /* NcaDtype of x, gate, y, dy, dx, dgate */
+  int32_t reverse;
+  int32_t masked;                /* a mask is passed */
+  int32_t unaligned;             /* x, gate, y, dy, dx or dgate is not on a 4-byte boundary */
+  int32_t reserved;
+  int64_t x_stride[3];           /* of (n, m, step); channels are adjacent */
+  int64_t gate_stride[3], dy_stride[3];
+  int64_t y_stride[3];           /* of y, dx and dgate */
+  int64_t mask_stride[3];
+} NcaScanDesc;
+
+/* Bytes of the buffer `saved` that a training forward fills for the backward call: states along the line. */
+int32_t nca_b200_gated_scan_saved_bytes(const NcaScanDesc* d, size_t* bytes);
+int32_t nca_b200_gated_scan_workspace(const NcaScanDesc* d, int32_t backward, size_t* bytes);
+/* state (before the first step; NULL: zeros) and last (after the last): device [n][m][channels] fp32. */
+int32_t nca_b200_gated_scan(const NcaScanDesc* d, const void* x, const void* gate,
+                            const float* state, const uint8_t* mask, void* y, float* last,
+                            float* saved, void* workspace, size_t workspace_bytes, void* stream);
+/* dlast (the gradient of last) may be NULL; so may dx, dgate and dstate, which are then not written. */
+int32_t nca_b200_gated_scan_backward(const NcaScanDesc* d, const void* x, const void* gate,
+                                     const float* state, const uint8_t* mask, const float* saved,
+                                     const void* dy, const float* dlast, void* dx, void* dgate,
+                                     float* dstate, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -168,6 +168,25 @@ class NcaDistillDesc(C.Structure):
     ]
 
 
+class NcaScanDesc(C.Structure):
+    _fields_ = [
+        ("n", C.c_int64),
+        ("m", C.c_int64),
+        ("steps", C.c_int64),
+        ("channels", C.c_int32),
+        ("dtype", C.c_int32),
+        ("reverse", C.c_int32),
+        ("masked", C.c_int32),
+        ("unaligned", C.c_int32),
+        ("reserved", C.c_int32),
+        ("x_stride", C.c_int64 * 3),
+        ("gate_stride", C.c_int64 * 3),
+        ("dy_stride", C.c_int64 * 3),
+        ("y_stride", C.c_int64 * 3),
+        ("mask_stride", C.c_int64 * 3),
+    ]
+
+
 # name -> (restype, argtypes); must match include/nca_b200.h
 _P = C.c_void_p
 _I = C.c_int32
@@ -237,6 +256,10 @@ SIGNATURES = {
     "nca_b200_distill_workspace": (_I, [C.POINTER(NcaDistillDesc), C.POINTER(C.c_size_t)]),
     "nca_b200_distill": (_I, [C.POINTER(NcaDistillDesc), *[_P] * 8, C.c_size_t, _P]),
     "nca_b200_distill_backward": (_I, [C.POINTER(NcaDistillDesc), *[_P] * 6, C.c_int64, _P, _P]),
+    "nca_b200_gated_scan_saved_bytes": (_I, [C.POINTER(NcaScanDesc), C.POINTER(C.c_size_t)]),
+    "nca_b200_gated_scan_workspace": (_I, [C.POINTER(NcaScanDesc), _I, C.POINTER(C.c_size_t)]),
+    "nca_b200_gated_scan": (_I, [C.POINTER(NcaScanDesc), *[_P] * 8, C.c_size_t, _P]),
+    "nca_b200_gated_scan_backward": (_I, [C.POINTER(NcaScanDesc), *[_P] * 11, C.c_size_t, _P]),
 }
 
 _lib: C.CDLL | None = None

@@ -610,6 +610,171 @@ std::tuple<Tensor, Tensor> distill_loss_and_grad(const Tensor& logits_, const Te
   return {reduced(loss, reduction == "mean" && a.d.rows > 0 ? "sum" : reduction, logits, "distill_loss_and_grad"), grad};
 }
 
+// -------------------------------------------------------------------------------- gated scan
+// (n..., step, m..., C) seen as n x m lines: a view where the dimensions on each side of the step collapse to
+// one stride and the channels are adjacent, else a copy.
+struct Lines {
+  Tensor t;
+  int64_t n = 1, m = 1;
+  int64_t stride[3] = {0, 0, 0};
+  Lines() = default;
+  Lines(const Tensor& x, int64_t dim, bool channels) : t(x) {
+    const int64_t last = x.dim() - (channels ? 1 : 0);
+    const auto view = [&] {
+      return (!channels || t.size(-1) <= 1 || t.stride(-1) == 1) && collapse(t, 0, dim, &n, &stride[0]) &&
+             collapse(t, dim + 1, last, &m, &stride[1]);
+    };
+    if (!view()) {
+      t = x.contiguous();
+      view();
+    }
+    stride[2] = t.size(dim) > 1 ? t.stride(dim) : 0;
+  }
+};
+
+struct Scan {
+  NcaScanDesc d{};
+  Lines x, gate, dy, mask;
+  Tensor state;
+  static void put(int64_t (&to)[3], const Lines& l) {
+    for (int i = 0; i < 3; ++i) to[i] = l.stride[i];
+  }
+  static int unaligned(const Tensor& t) {
+    return t.defined() && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 4 ? 1 : 0;
+  }
+  Scan(const Tensor& xt, const Tensor& gt, const Tensor& st, int64_t dim, bool reverse, const Tensor& mt)
+      : x(xt, dim, true), gate(gt, dim, true) {
+    d.n = x.n;
+    d.m = x.m;
+    d.steps = xt.size(dim);
+    d.channels = (int32_t)xt.size(-1);
+    d.dtype = dtype_of(xt, "gated_scan", "x");
+    d.reverse = reverse;
+    put(d.x_stride, x);
+    put(d.gate_stride, gate);
+    // contiguous outputs
+    d.y_stride[2] = d.m * d.channels;
+    d.y_stride[1] = d.channels;
+    d.y_stride[0] = d.steps * d.m * d.channels;
+    if (mt.defined()) {
+      mask = Lines(mt, dim, false);
+      d.masked = 1;
+      put(d.mask_stride, mask);
+    }
+    if (st.defined()) state = st.contiguous();
+    d.unaligned = unaligned(x.t) | unaligned(gate.t);
+  }
+  void set_dy(const Tensor& t, int64_t dim) {
+    dy = Lines(t, dim, true);
+    put(d.dy_stride, dy);
+    d.unaligned |= unaligned(dy.t);
+  }
+  const uint8_t* mask_ptr() const { return static_cast<const uint8_t*>(ptr(mask.t)); }
+  const float* state_ptr() const { return static_cast<const float*>(ptr(state)); }
+};
+
+std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& x, const Tensor& gate, const Tensor& state, int64_t dim,
+                                                bool reverse, const Tensor& mask, bool save) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  Scan a(x, gate, state, dim, reverse, mask);
+  Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.erase(shape.begin() + dim);
+  Tensor last = at::empty(shape, x.options().dtype(at::kFloat)), saved;
+  size_t bytes = 0;
+  if (save) {
+    check(nca_b200_gated_scan_saved_bytes(&a.d, &bytes), "nca_b200_gated_scan_saved_bytes");
+    saved = scratch(bytes, x);
+  }
+  check(nca_b200_gated_scan_workspace(&a.d, 0, &bytes), "nca_b200_gated_scan_workspace");
+  Tensor ws = scratch(bytes, x);
+  check(nca_b200_gated_scan(&a.d, ptr(a.x.t), ptr(a.gate.t), a.state_ptr(), a.mask_ptr(), mptr(y),
+                            static_cast<float*>(mptr(last)), static_cast<float*>(mptr(saved)), mptr(ws), bytes_of(ws),
+                            stream_of(x)),
+        "nca_b200_gated_scan");
+  return {y, last, saved};
+}
+
+struct ScanFunction : torch::autograd::Function<ScanFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate, const OptTensor& state_,
+                               int64_t dim, bool reverse, const OptTensor& mask_) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor state = or_none(state_), mask = or_none(mask_);
+    auto [y, last, saved] = scan_forward(x, gate, state, dim, reverse, mask, true);
+    ctx->save_for_backward({x, gate, state, mask, saved});
+    ctx->saved_data["dim"] = dim;
+    ctx->saved_data["reverse"] = reverse;
+    ctx->set_materialize_grads(false);
+    return {y, last};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order("gated_scan");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &gate = saved[1], &state = saved[2];
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int64_t dim = ctx->saved_data["dim"].toInt();
+    for (const Tensor& g : grads) no_tangent(g, "gated_scan", "the gradient");
+    Scan a(x, gate, state, dim, ctx->saved_data["reverse"].toBool(), saved[3]);
+    const Tensor dy = grads[0].defined() ? grads[0] : at::zeros({1}, x.options()).expand(x.sizes());  // only `last` was used
+    a.set_dy(dy, dim);
+    const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Needs needs(ctx, {x, gate, state, saved[3]});
+    Tensor dx, dgate, dstate;
+    if (needs[0]) dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+    if (needs[1]) dgate = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+    if (needs[2]) dstate = at::empty_like(state, at::MemoryFormat::Contiguous);
+    size_t bytes = 0;
+    check(nca_b200_gated_scan_workspace(&a.d, 1, &bytes), "nca_b200_gated_scan_workspace");
+    Tensor ws = scratch(bytes, x);
+    check(nca_b200_gated_scan_backward(&a.d, ptr(a.x.t), ptr(a.gate.t), a.state_ptr(), a.mask_ptr(),
+                                       static_cast<const float*>(ptr(saved[4])), ptr(a.dy.t),
+                                       static_cast<const float*>(ptr(dlast)), mptr(dx), mptr(dgate),
+                                       static_cast<float*>(mptr(dstate)), mptr(ws), bytes_of(ws), stream_of(x)),
+          "nca_b200_gated_scan_backward");
+    return {dx, dgate, dstate, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const OptTensor& state_, int64_t dim_,
+                                      bool reverse, const OptTensor& mask_) {
+  constexpr const char* op = "gated_scan";
+  on_cuda(x, op, "x");
+  no_tangent(x, op, "x");
+  dtype_of(x, op, "x");
+  TORCH_CHECK_VALUE(x.dim() >= 2, op, ": x must have an axis to scan and channels, not ", x.sizes());
+  const int64_t dim = dim_ < 0 ? dim_ + x.dim() : dim_;
+  TORCH_CHECK_VALUE(dim >= 0 && dim < x.dim() - 1, op, ": dim must name an axis before the channels, not ", dim_);
+  TORCH_CHECK_VALUE(x.size(-1) <= kMostChannels, op, ": at most ", kMostChannels, " channels, not ", x.size(-1));
+  same_device(gate, x, op, "gate");
+  no_tangent(gate, op, "gate");
+  TORCH_CHECK_TYPE(gate.scalar_type() == x.scalar_type(), op, ": gate must be of x's type ", x.scalar_type(), ", not ",
+                   gate.scalar_type());
+  TORCH_CHECK_VALUE(gate.sizes() == x.sizes(), op, ": gate must be ", x.sizes(), ", not ", gate.sizes());
+  const Tensor state = or_none(state_), mask = or_none(mask_);
+  if (state.defined()) {
+    same_device(state, x, op, "state");
+    no_tangent(state, op, "state");
+    TORCH_CHECK_TYPE(state.scalar_type() == at::kFloat, op, ": state must be float32, not ", state.scalar_type());
+    std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+    shape.erase(shape.begin() + dim);
+    TORCH_CHECK_VALUE(state.sizes() == at::IntArrayRef(shape), op, ": state must be ", at::IntArrayRef(shape), ", not ",
+                      state.sizes());
+  }
+  if (mask.defined()) {
+    same_device(mask, x, op, "mask");
+    TORCH_CHECK_TYPE(mask.scalar_type() == at::kBool || mask.scalar_type() == at::kByte, op,
+                     ": mask must be bool or uint8");
+    TORCH_CHECK_VALUE(mask.sizes() == x.sizes().slice(0, x.dim() - 1), op, ": mask must have shape ",
+                      x.sizes().slice(0, x.dim() - 1), ", not ", mask.sizes());
+  }
+  if (any_grad({&x, &gate, &state})) {
+    const variable_list out = ScanFunction::apply(x, gate, optional(state), dim, reverse, optional(mask));
+    return {out[0], out[1]};
+  }
+  auto [y, last, saved] = scan_forward(x, gate, state, dim, reverse, mask, false);
+  return {y, last};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(nca_b200, m) {
@@ -624,5 +789,7 @@ TORCH_LIBRARY_FRAGMENT(nca_b200, m) {
   m.def("distill_loss_and_grad(Tensor logits, Tensor teacher_logits, Tensor teacher_index, float temperature, "
         "Tensor? weight, str reduction) -> (Tensor, Tensor)",
         &distill_loss_and_grad);
+  m.def("gated_scan(Tensor x, Tensor gate, Tensor? state, int dim, bool reverse, Tensor? mask) -> (Tensor, Tensor)",
+        &gated_scan);
   m.def("operators_status(Tensor like) -> int[]", &operators_status);
 }

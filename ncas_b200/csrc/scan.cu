@@ -1,0 +1,639 @@
+// scan.cu -- the gated scan h_t = a_t h_{t-1} + (1 - a_t) x_t, a = sigmoid(gate), along one axis, forward
+// and backward (nca_b200_gated_scan*).
+//
+// With e = exp(gate), 1 - a is 1 / (1 + e) and a is e / (1 + e): both with full relative precision.  States,
+// products and sums are fp32.
+//
+// Steps compose as maps h -> P h + H (P the product of the a), so a line can be cut anywhere.  A thread
+// owns two adjacent 16-bit channels (or one channel) of kSub adjacent steps, all of which it holds in
+// registers.  Where lines and channels fill the GPU, a thread walks along its line alone.  Else the
+// threads of a block's warps split a stretch of the line: each builds its steps' maps from the identity on, the
+// warps exchange the last through shared memory, and y_t = P_t h + H_t from the state h before the thread's
+// steps.  Blocks walk along the line and load the next stretch while they work on this one.  Where that does not fill
+// the GPU either, the line is cut into pieces for different blocks: a first kernel computes the
+// pieces' maps, at the price of a second read.  Backward: G_t = dy_t + a_{t+1} G_{t+1} is the same scan
+// from the end; the states come again from the inputs, from the state that the forward pass stored before
+// each kSub steps (4 bytes for kSub elements).
+#include "cell_ops.cuh"
+
+#include <algorithm>
+
+using namespace nca;
+
+namespace {
+
+constexpr int kSub = 16;             // steps of a thread
+constexpr int kLanes = 32;           // columns of a block whose warps split a line
+constexpr int kThreads = 256;        // forward
+constexpr int kThreadsBack = 128;    // backward: three times the registers
+constexpr int kMostPieces = 128;
+constexpr uint32_t kAll = (1u << kSub) - 1;
+
+struct ScanParams {
+  const void *x, *gate, *dy;
+  const float *state, *dlast;
+  const uint8_t* mask;
+  void *y, *dx, *dgate;
+  float *last, *dstate;
+  float* saved;        // states before steps kSub, 2 kSub, ... [lines][marks][channels]
+  float *agg_p, *agg_h;  // maps of the pieces [pieces][lines][channels]
+  long long m, steps, lines, columns, marks;
+  long long stretches, per;  // stretches of subs * kSub steps; those of a piece
+  int channels, per_line;    // columns of a line
+  int subs, pieces, block_columns;
+  long long xs[3], gs[3], ds[3], ys[3], ms[3];  // strides of (n, m, step); those of the step negative in a reversed scan
+};
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// The channels of a thread: one, or two whose operations go in pairs.
+template <int V>
+struct Ch;
+template <>
+struct Ch<1> {
+  using F = float;
+  static __device__ __forceinline__ F of(float v) { return v; }
+  static __device__ __forceinline__ F add(F a, F b) { return a + b; }
+  static __device__ __forceinline__ F mul(F a, F b) { return a * b; }
+  static __device__ __forceinline__ F fma(F a, F b, F c) { return fmaf(a, b, c); }
+  template <class O>
+  static __device__ __forceinline__ F each(F a, O o) { return o(a); }
+};
+template <>
+struct Ch<2> {
+  using F = float2;
+  static __device__ __forceinline__ F of(float v) { return both(v); }
+  static __device__ __forceinline__ F add(F a, F b) { return add2(a, b); }
+  static __device__ __forceinline__ F mul(F a, F b) { return mul2(a, b); }
+  static __device__ __forceinline__ F fma(F a, F b, F c) { return fma2(a, b, c); }
+  template <class O>
+  static __device__ __forceinline__ F each(F a, O o) { return make_float2(o(a.x), o(a.y)); }
+};
+
+// keep = 1 - a, and a.  Beyond 87, 1 - a is below 2^-125.  NaN stays NaN.  For fp32 data the product
+// gate log2(e) is taken with its rounding error, which would be worth 2^-24 |gate| of the exponential.
+template <class T, int V>
+__device__ __forceinline__ void coefficients(typename Ch<V>::F gate, typename Ch<V>::F& keep, typename Ch<V>::F& a) {
+  using C = Ch<V>;
+  typename C::F g = C::each(gate, [](float v) { return min_nan(v, 87.f); });
+  if constexpr (sizeof(T) == 4) g = C::each(g, [](float v) { return max_nan(v, -87.f); });
+  const typename C::F t = C::mul(g, C::of(1.4426950408889634f));
+  typename C::F e = C::each(t, [](float v) { return ex2(v); });
+  if constexpr (sizeof(T) == 4) {
+    const typename C::F rest = C::fma(g, C::of(1.925963033500011e-8f), C::fma(g, C::of(1.4426950408889634f), C::mul(t, C::of(-1.f))));
+    e = C::fma(e, C::mul(rest, C::of(0.6931471805599453f)), e);
+  }
+  keep = C::each(C::add(e, C::of(1.f)), [](float v) { return rcp(v); });
+  a = C::mul(e, keep);
+}
+
+// The 4 bytes (one fp32 or two 16-bit channels; one 16-bit channel: 2 bytes) of each of a thread's steps.
+struct Raw {
+  uint32_t v[kSub];
+};
+template <class T, int V>
+__device__ __forceinline__ uint32_t load_one(const T* at) {
+  if constexpr (sizeof(T) * V == 4) return *reinterpret_cast<const uint32_t*>(at);
+  else return *reinterpret_cast<const uint16_t*>(at);
+}
+template <class T, int V>
+__device__ __forceinline__ void load(Raw& r, const T* at, long long step, uint32_t on) {
+  if (on == kAll) {
+#pragma unroll
+    for (int i = 0; i < kSub; ++i) {
+      r.v[i] = load_one<T, V>(at);
+      at += step;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kSub; ++i) {
+      r.v[i] = 0;
+      if (on >> i & 1) r.v[i] = load_one<T, V>(at);
+      at += step;
+    }
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ typename Ch<V>::F take(uint32_t v) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(v);
+  } else {
+    float2 t;
+    if constexpr (__is_same(T, __nv_bfloat16)) t = make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+    else t = __half22float2(reinterpret_cast<const __half2&>(v));
+    if constexpr (V == 2) return t;
+    else return t.x;
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void put(T* at, typename Ch<V>::F f) {
+  if constexpr (V == 2) *reinterpret_cast<Vec<T, 2>*>(at) = from_pairs<T, 2>({f});
+  else *at = from_f32<T>(f);
+}
+template <int V>
+__device__ __forceinline__ typename Ch<V>::F load_f32(const float* p, long long at, bool on) {
+  if constexpr (V == 2) return on && p ? *reinterpret_cast<const float2*>(p + at) : both(0.f);
+  else return on && p ? p[at] : 0.f;
+}
+// (state, last and their gradients may start on any 4-byte boundary)
+template <int V>
+__device__ __forceinline__ typename Ch<V>::F load_edge(const float* p, long long at, bool on) {
+  if constexpr (V == 2) return on && p ? make_float2(p[at], p[at + 1]) : both(0.f);
+  else return on && p ? p[at] : 0.f;
+}
+template <int V>
+__device__ __forceinline__ void store_edge(float* p, long long at, typename Ch<V>::F f) {
+  if constexpr (V == 2) p[at] = f.x, p[at + 1] = f.y;
+  else p[at] = f;
+}
+template <int V>
+__device__ __forceinline__ void store_f32(float* p, long long at, typename Ch<V>::F f) {
+  if constexpr (V == 2) *reinterpret_cast<float2*>(p + at) = f;
+  else p[at] = f;
+}
+
+// One thread's place: its column (line and channels) and its place among the threads along the line.
+template <int V>
+struct Place {
+  long long line, n, m;
+  int c, sub, lane;
+  bool on;
+  __device__ __forceinline__ Place(const ScanParams& p) {
+    lane = p.subs > 1 ? threadIdx.x % kLanes : threadIdx.x;
+    sub = p.subs > 1 ? threadIdx.x / kLanes : 0;
+    const long long col = (long long)blockIdx.x * p.block_columns + lane;
+    on = col < p.columns;
+    line = on ? col / p.per_line : 0;
+    c = on ? (int)(col - line * p.per_line) * V : 0;
+    n = line / p.m;
+    m = line - n * p.m;
+  }
+  __device__ __forceinline__ long long at(const long long (&s)[3]) const { return n * s[0] + m * s[1]; }
+  // the steps of the kSub from t0 on that exist (bits), and those of them that the mask keeps
+  __device__ __forceinline__ uint32_t inside(const ScanParams& p, long long t0) const {
+    const long long left = p.steps - t0;
+    return !on || left <= 0 ? 0u : left >= kSub ? (1u << kSub) - 1 : (1u << left) - 1;
+  }
+  __device__ __forceinline__ uint32_t kept(const ScanParams& p, long long t0, uint32_t in) const {
+    if (!p.mask) return in;
+    const uint8_t* at_mask = p.mask + at(p.ms) + t0 * p.ms[2];
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < kSub; ++i)
+      if ((in >> i & 1) && at_mask[i * p.ms[2]]) bits |= 1u << i;
+    return bits;
+  }
+};
+
+// Maps of the warps along a line, two buffers in turn: one barrier an exchange.
+template <int V, int SUBS>
+struct Exchange {
+  using C = Ch<V>;
+  using F = typename C::F;
+  F p[2][SUBS][kLanes], h[2][SUBS][kLanes];
+  // In: this warp's map (P, H) and the state before (or, BACK, behind) the stretch in `run`.  Out: that of this
+  // warp's steps, and in `run` that of the next stretch.  Maps are applied in the order of the line.
+  template <bool BACK>
+  __device__ __forceinline__ F go(int buf, int sub, int lane, F P, F H, F& run) {
+    p[buf][sub][lane] = P;
+    h[buf][sub][lane] = H;
+    __syncthreads();
+    F start = run;
+#pragma unroll
+    for (int k = 0; k < SUBS; ++k) {
+      const int s = BACK ? SUBS - 1 - k : k;
+      if (s == sub) start = run;
+      run = C::fma(p[buf][s][lane], run, h[buf][s][lane]);
+    }
+    return start;
+  }
+};
+template <int V>
+struct Exchange<V, 1> {};
+
+// The state at the start (end) of this block's piece: through the maps of the pieces before (behind) it.
+template <int V, bool BACK>
+__device__ __forceinline__ typename Ch<V>::F enter(const ScanParams& p, const Place<V>& me) {
+  const long long at = me.line * p.channels + me.c, piece = p.lines * p.channels;
+  typename Ch<V>::F run = load_edge<V>(BACK ? p.dlast : p.state, at, me.on);
+  const int count = BACK ? p.pieces - 1 - (int)blockIdx.y : (int)blockIdx.y;
+#pragma unroll 8
+  for (int k = 0; k < count; ++k) {
+    const long long from = (BACK ? p.pieces - 1 - k : k) * piece + at;
+    run = Ch<V>::fma(load_f32<V>(p.agg_p, from, me.on), run, load_f32<V>(p.agg_h, from, me.on));
+  }
+  return run;
+}
+
+// SUBS: warps along a line (1: a thread walks along it alone, and there is one piece).
+template <class T, int V, int SUBS>
+__global__ void __launch_bounds__(kThreads, 2) scan_forward_kernel(const __grid_constant__ ScanParams p) {
+  using C = Ch<V>;
+  using F = typename C::F;
+  constexpr bool kSplit = SUBS > 1;
+  may_start_next();
+  after_previous();
+  __shared__ Exchange<V, SUBS> exchange;
+  const Place<V> me(p);
+  const T* x = static_cast<const T*>(p.x) + me.at(p.xs) + me.c;
+  const T* g = static_cast<const T*>(p.gate) + me.at(p.gs) + me.c;
+  T* y = static_cast<T*>(p.y) + me.at(p.ys) + me.c;
+  const long long k0 = blockIdx.y * p.per, k1 = min(k0 + p.per, p.stretches);
+  F run = enter<V, false>(p, me);
+
+  Raw rx, rg;
+  long long t0 = (k0 * SUBS + me.sub) * kSub;
+  uint32_t in = 0, on = 0;
+  const auto fetch = [&] {
+    in = me.inside(p, t0);
+    on = me.kept(p, t0, in);
+    load<T, V>(rx, x + t0 * p.xs[2], p.xs[2], on);
+    load<T, V>(rg, g + t0 * p.gs[2], p.gs[2], on);
+  };
+  if (k0 < k1) fetch();
+  for (long long k = k0; k < k1; ++k) {
+    const long long now = t0;
+    const uint32_t in_now = in, on_now = on;
+    F P[kSub], H[kSub];  // a thread alone: H is the state itself
+    {
+      F prod = C::of(1.f), h = kSplit ? C::of(0.f) : run;
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) {
+        F keep, a;
+        coefficients<T, V>(take<T, V>(rg.v[i]), keep, a);
+        const F b = C::mul(keep, take<T, V>(rx.v[i]));
+        if (on_now == kAll || (on_now >> i & 1)) {
+          h = C::fma(a, h, b);
+          if constexpr (kSplit) prod = C::mul(prod, a);
+        }
+        H[i] = h;
+        if constexpr (kSplit) P[i] = prod;
+      }
+    }
+    if (k + 1 < k1) {  // the next stretch, in flight from here on
+      t0 += SUBS * kSub;
+      fetch();
+    }
+    F start = run;
+    if constexpr (kSplit) start = exchange.template go<false>(k & 1, me.sub, me.lane, P[kSub - 1], H[kSub - 1], run);
+    const long long mark = now / kSub - 1;
+    if (p.saved && mark >= 0 && in_now) store_f32<V>(p.saved, (me.line * p.marks + mark) * p.channels + me.c, start);
+    T* to = y + now * p.ys[2];
+    if constexpr (kSplit) {
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) H[i] = C::fma(P[i], start, H[i]);
+    } else {
+      run = H[kSub - 1];
+    }
+    if (on_now == kAll) {
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) {
+        put<T, V>(to, H[i]);
+        to += p.ys[2];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) {
+        if (in_now >> i & 1) put<T, V>(to, on_now >> i & 1 ? H[i] : C::of(0.f));
+        to += p.ys[2];
+      }
+    }
+  }
+  if (me.on && me.sub == 0 && (int)blockIdx.y == p.pieces - 1) store_edge<V>(p.last, me.line * p.channels + me.c, run);
+}
+
+// The maps of the pieces.  Here a warp takes adjacent steps of the piece, so there is one exchange, at the end.
+// Backward: r -> P r + H with r = a G, built in the order of the line: a later step's dy passes the a before it.
+template <class T, int V, int SUBS, bool BACK>
+__global__ void __launch_bounds__(SUBS * kLanes, BACK ? 4 : 2) scan_pieces_kernel(const __grid_constant__ ScanParams p) {
+  using C = Ch<V>;
+  using F = typename C::F;
+  may_start_next();
+  after_previous();
+  __shared__ Exchange<V, SUBS> exchange;
+  const Place<V> me(p);
+  const long long z = BACK ? blockIdx.y + 1 : blockIdx.y;  // nothing enters the first piece, or behind the last
+  const T* v = static_cast<const T*>(BACK ? p.dy : p.x) + me.at(BACK ? p.ds : p.xs) + me.c;
+  const T* g = static_cast<const T*>(p.gate) + me.at(p.gs) + me.c;
+  const long long vs = BACK ? p.ds[2] : p.xs[2];
+  const long long count = min(p.per, p.stretches - z * p.per);
+  long long t0 = (z * p.per * SUBS + me.sub * count) * kSub;
+  F P = C::of(1.f), H = C::of(0.f);
+  Raw rv, rg;
+  uint32_t on = 0;
+  const auto fetch = [&] {
+    on = me.kept(p, t0, me.inside(p, t0));
+    load<T, V>(rv, v + t0 * vs, vs, on);
+    load<T, V>(rg, g + t0 * p.gs[2], p.gs[2], on);
+  };
+  if (count > 0) fetch();
+  for (long long k = 0; k < count; ++k) {
+    const Raw cv = rv, cg = rg;
+    const uint32_t on_now = on;
+    if (k + 1 < count) {  // the next steps, in flight while these are worked on
+      t0 += kSub;
+      fetch();
+    }
+#pragma unroll
+    for (int i = 0; i < kSub; ++i) {
+      F keep, a;
+      coefficients<T, V>(take<T, V>(cg.v[i]), keep, a);
+      if (on_now == kAll || (on_now >> i & 1)) {
+        P = C::mul(P, a);
+        if constexpr (BACK) H = C::fma(P, take<T, V>(cv.v[i]), H);
+        else H = C::fma(a, H, C::mul(keep, take<T, V>(cv.v[i])));
+      }
+    }
+  }
+  // the whole piece's map: its H from a state of 0, its P as the product over the warps
+  F run = C::of(0.f), all = C::of(1.f);
+  exchange.template go<BACK>(0, me.sub, me.lane, P, H, run);
+  if (!me.on || me.sub != 0) return;
+#pragma unroll
+  for (int s = 0; s < SUBS; ++s) all = C::mul(all, exchange.p[0][s][me.lane]);
+  const long long to = (z * p.lines + me.line) * p.channels + me.c;
+  store_f32<V>(p.agg_p, to, all);
+  store_f32<V>(p.agg_h, to, run);
+}
+
+template <class T, int V, int SUBS>
+__global__ void __launch_bounds__(kThreadsBack, 3) scan_backward_kernel(const __grid_constant__ ScanParams p) {
+  using C = Ch<V>;
+  using F = typename C::F;
+  constexpr bool kSplit = SUBS > 1;
+  may_start_next();
+  after_previous();
+  __shared__ Exchange<V, SUBS> exchange;
+  const Place<V> me(p);
+  const T* x = static_cast<const T*>(p.x) + me.at(p.xs) + me.c;
+  const T* g = static_cast<const T*>(p.gate) + me.at(p.gs) + me.c;
+  const T* dy = static_cast<const T*>(p.dy) + me.at(p.ds) + me.c;
+  T* dx = static_cast<T*>(p.dx) + me.at(p.ys) + me.c;
+  T* dg = static_cast<T*>(p.dgate) + me.at(p.ys) + me.c;
+  const long long k0 = blockIdx.y * p.per, k1 = min(k0 + p.per, p.stretches);
+  F run = enter<V, true>(p, me);
+
+  Raw rx, rg, rd;
+  F rh = C::of(0.f);
+  long long t0 = ((k1 - 1) * SUBS + me.sub) * kSub;
+  uint32_t in = 0, on = 0;
+  const auto fetch = [&] {
+    in = me.inside(p, t0);
+    on = me.kept(p, t0, in);
+    load<T, V>(rx, x + t0 * p.xs[2], p.xs[2], on);
+    load<T, V>(rg, g + t0 * p.gs[2], p.gs[2], on);
+    load<T, V>(rd, dy + t0 * p.ds[2], p.ds[2], on);
+    const long long mark = t0 / kSub - 1;  // the state before these steps
+    if (mark < 0) rh = load_edge<V>(p.state, me.line * p.channels + me.c, me.on);
+    else rh = load_f32<V>(p.saved, (me.line * p.marks + mark) * p.channels + me.c, in != 0);
+  };
+  if (k0 < k1) fetch();
+  for (long long k = k1 - 1; k >= k0; --k) {
+    const long long now = t0;
+    const uint32_t in_now = in, on_now = on;
+    F keeps[kSub], w[kSub], as[V == 1 ? kSub : 1];
+    F P = C::of(1.f), H = C::of(0.f);
+    // in the order of the line: the states again, w = a (h before - x), and the stretch's map of r = a G
+    {
+      F h = rh;
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) {
+        F keep, a;
+        coefficients<T, V>(take<T, V>(rg.v[i]), keep, a);
+        const F xi = take<T, V>(rx.v[i]);
+        w[i] = C::mul(a, C::fma(xi, C::of(-1.f), h));
+        if (on_now == kAll || (on_now >> i & 1)) {
+          h = C::fma(a, h, C::mul(keep, xi));
+          if constexpr (kSplit) {
+            P = C::mul(P, a);
+            H = C::fma(P, take<T, V>(rd.v[i]), H);
+          }
+        }
+        keeps[i] = keep;
+        if constexpr (V == 1) as[i] = a;
+      }
+    }
+    const Raw cd = rd;
+    if (k > k0) {  // the stretch before, in flight from here on
+      t0 -= SUBS * kSub;
+      fetch();
+    }
+    F r = run;
+    if constexpr (kSplit) r = exchange.template go<true>(k & 1, me.sub, me.lane, P, H, run);
+    // from its end: dx = (1 - a) G, dgate = w dx, r = a G.  Two channels: r = G - (1 - a) G in one rounding, since a third
+    // row of registers would halve the blocks; beside 16-bit outputs its error of 2^-24 G is nothing.
+    long long to = (now + kSub - 1) * p.ys[2];
+#pragma unroll
+    for (int i = kSub - 1; i >= 0; --i) {
+      const F G = C::add(take<T, V>(cd.v[i]), r);
+      F ox = C::mul(keeps[i], G), og = C::mul(w[i], ox);
+      if (on_now == kAll || (on_now >> i & 1)) {
+        if constexpr (V == 1) r = C::mul(as[i], G);
+        else r = C::fma(C::mul(keeps[i], C::of(-1.f)), G, G);
+      } else {
+        ox = og = C::of(0.f);
+      }
+      if (on_now == kAll || (in_now >> i & 1)) {
+        if (p.dx) put<T, V>(dx + to, ox);
+        if (p.dgate) put<T, V>(dg + to, og);
+      }
+      to -= p.ys[2];
+    }
+    if constexpr (!kSplit) run = r;
+  }
+  if (p.dstate && me.on && me.sub == 0 && blockIdx.y == 0) store_edge<V>(p.dstate, me.line * p.channels + me.c, run);
+}
+
+// --------------------------------------------------------------------------------------- host side
+inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+int32_t check_desc(const NcaScanDesc* d) {
+  if (!d || d->n < 0 || d->m < 0 || d->steps < 0 || d->channels < 0 || !dtype_ok(d->dtype)) return NCA_ERR_INVALID;
+  const long long most = 1ll << 40;  // products of sizes stay far inside 64 bits
+  if (d->n > most || d->m > most || d->steps > most || (d->n && d->m > most / d->n)) return NCA_ERR_UNSUPPORTED;
+  const long long lines = d->n * d->m;
+  if (lines && (d->channels > most / lines || (d->steps && d->steps > (1ll << 44) / (lines * std::max(d->channels, 1)))))
+    return NCA_ERR_UNSUPPORTED;
+  return NCA_OK;
+}
+bool strides_even(const int64_t (&s)[3]) { return ((s[0] | s[1] | s[2]) & 1) == 0; }
+
+// Two 16-bit channels a thread where every row starts on a 4-byte boundary, else one.  A thread a line where that gives
+// half the threads that run at once, or the line is short; else the warps of a block along a line, and pieces of
+// it for as many blocks as run at once.
+ScanParams plan_of(const NcaScanDesc& d, bool backward) {
+  ScanParams p{};
+  const bool pairs = d.dtype != NCA_F32 && d.channels % 2 == 0 && !d.unaligned && strides_even(d.x_stride) &&
+                     strides_even(d.gate_stride) && strides_even(d.y_stride) && (!backward || strides_even(d.dy_stride));
+  p.m = std::max<long long>(d.m, 1);
+  p.lines = d.n * d.m;
+  p.steps = d.steps;
+  p.channels = d.channels;
+  p.per_line = pairs ? d.channels / 2 : d.channels;
+  p.columns = p.lines * p.per_line;
+  p.marks = d.steps > kSub ? ceil_div(d.steps, kSub) - 1 : 0;
+  const int threads = backward ? kThreadsBack : kThreads, resident = 148 * (backward ? 3 : 2);
+  p.subs = d.steps > 2 * kSub && p.columns < (long long)resident * threads / 2 ? threads / kLanes : 1;
+  p.block_columns = threads / p.subs;
+  p.stretches = ceil_div(d.steps, (long long)p.subs * kSub);
+  const long long groups = ceil_div(p.columns, p.block_columns);
+  long long pieces = 1;
+  if (p.subs > 1 && groups > 0) pieces = std::min({(long long)kMostPieces, p.stretches / 4, resident / groups});
+  p.per = ceil_div(p.stretches, std::max(pieces, 1ll));
+  p.pieces = (int)std::max<long long>(1, ceil_div(p.stretches, std::max<long long>(p.per, 1)));
+  return p;
+}
+bool two_wide(const ScanParams& p) { return p.per_line != p.channels; }
+size_t workspace_of(const ScanParams& p) {
+  return p.pieces == 1 ? 0 : 2 * (size_t)p.pieces * p.lines * p.channels * sizeof(float);
+}
+
+void strides(long long (&to)[3], const int64_t (&from)[3], const NcaScanDesc& d) {
+  for (int i = 0; i < 3; ++i) to[i] = from[i];
+  if (d.reverse) to[2] = -to[2];
+}
+// The first step's element: in a reversed scan the last of the line.
+const void* first(const void* p, const int64_t (&s)[3], const NcaScanDesc& d, size_t size) {
+  return p && d.reverse && d.steps ? static_cast<const uint8_t*>(p) + (d.steps - 1) * s[2] * (int64_t)size : p;
+}
+bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 != 0; }
+
+template <class F>
+int32_t with_kind(int dtype, bool pairs, F fn) {
+  return with_dtype(dtype, [&](auto t) -> int32_t {
+    using T = decltype(t);
+    if constexpr (sizeof(T) == 2) {
+      if (pairs) return fn(t, ActTag<2>{});
+    }
+    return fn(t, ActTag<1>{});
+  });
+}
+
+template <class T, int V, int SUBS>
+int32_t run_forward(const ScanParams& p, long long groups, cudaStream_t s) {
+  if constexpr (SUBS > 1) {
+    if (p.pieces > 1) {
+      const int32_t e = launch_after(scan_pieces_kernel<T, V, SUBS, false>, dim3((unsigned)groups, p.pieces - 1),
+                                     dim3(kThreads), 0, s, 1, p);
+      if (e != NCA_OK) return e;
+    }
+  }
+  return launch_after(scan_forward_kernel<T, V, SUBS>, dim3((unsigned)groups, p.pieces), dim3(kThreads), 0, s, 1, p);
+}
+template <class T, int V, int SUBS>
+int32_t run_backward(const ScanParams& p, long long groups, cudaStream_t s) {
+  if constexpr (SUBS > 1) {
+    if (p.pieces > 1) {
+      const int32_t e = launch_after(scan_pieces_kernel<T, V, SUBS, true>, dim3((unsigned)groups, p.pieces - 1),
+                                     dim3(kThreadsBack), 0, s, 1, p);
+      if (e != NCA_OK) return e;
+    }
+  }
+  return launch_after(scan_backward_kernel<T, V, SUBS>, dim3((unsigned)groups, p.pieces), dim3(kThreadsBack), 0, s, 1, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t nca_b200_gated_scan_saved_bytes(const NcaScanDesc* d, size_t* bytes) {
+  const int32_t st = check_desc(d);
+  if (st != NCA_OK || !bytes) return st != NCA_OK ? st : NCA_ERR_INVALID;
+  const ScanParams p = plan_of(*d, false);
+  *bytes = (size_t)p.lines * p.marks * p.channels * sizeof(float);
+  return NCA_OK;
+}
+
+int32_t nca_b200_gated_scan_workspace(const NcaScanDesc* d, int32_t backward, size_t* bytes) {
+  const int32_t st = check_desc(d);
+  if (st != NCA_OK || !bytes) return st != NCA_OK ? st : NCA_ERR_INVALID;
+  *bytes = workspace_of(plan_of(*d, backward != 0));
+  return NCA_OK;
+}
+
+int32_t nca_b200_gated_scan(const NcaScanDesc* d, const void* x, const void* gate, const float* state,
+                            const uint8_t* mask, void* y, float* last, float* saved, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  const int32_t st = check_desc(d);
+  if (st != NCA_OK) return st;
+  ScanParams p = plan_of(*d, false);
+  if (p.columns == 0) return NCA_OK;
+  if (!last || (d->steps && (!x || !gate || !y)) || (d->masked && d->steps && !mask)) return NCA_ERR_INVALID;
+  if (two_wide(p) && (misaligned(x) || misaligned(gate) || misaligned(y))) return NCA_ERR_INVALID;
+  const size_t need = workspace_of(p);
+  if (need && (!workspace || workspace_bytes < need)) return NCA_ERR_SCRATCH;
+  const size_t size = dtype_size(d->dtype);
+  p.x = first(x, d->x_stride, *d, size);
+  p.gate = first(gate, d->gate_stride, *d, size);
+  p.y = const_cast<void*>(first(y, d->y_stride, *d, size));
+  p.mask = d->masked ? static_cast<const uint8_t*>(first(mask, d->mask_stride, *d, 1)) : nullptr;
+  strides(p.xs, d->x_stride, *d);
+  strides(p.gs, d->gate_stride, *d);
+  strides(p.ys, d->y_stride, *d);
+  strides(p.ms, d->mask_stride, *d);
+  p.state = state;
+  p.last = last;
+  p.saved = p.marks ? saved : nullptr;
+  p.agg_p = static_cast<float*>(workspace);
+  p.agg_h = p.agg_p + (size_t)p.pieces * p.lines * p.channels;
+  const long long groups = ceil_div(p.columns, p.block_columns);
+  if (groups > (1ll << 31) - 1) return NCA_ERR_UNSUPPORTED;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return with_kind(d->dtype, two_wide(p), [&](auto t, auto v) -> int32_t {
+    using T = decltype(t);
+    constexpr int V = decltype(v)::value;
+    return p.subs > 1 ? run_forward<T, V, kThreads / kLanes>(p, groups, s) : run_forward<T, V, 1>(p, groups, s);
+  });
+}
+
+int32_t nca_b200_gated_scan_backward(const NcaScanDesc* d, const void* x, const void* gate, const float* state,
+                                     const uint8_t* mask, const float* saved, const void* dy, const float* dlast,
+                                     void* dx, void* dgate, float* dstate, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
+  const int32_t st = check_desc(d);
+  if (st != NCA_OK) return st;
+  ScanParams p = plan_of(*d, true);
+  if (p.columns == 0) return NCA_OK;
+  if ((d->steps && (!x || !gate || !dy)) || (p.marks && !saved) || (d->masked && d->steps && !mask)) return NCA_ERR_INVALID;
+  if (two_wide(p) && (misaligned(x) || misaligned(gate) || misaligned(dy) || misaligned(dx) || misaligned(dgate)))
+    return NCA_ERR_INVALID;
+  const size_t need = workspace_of(p);
+  if (need && (!workspace || workspace_bytes < need)) return NCA_ERR_SCRATCH;
+  const size_t size = dtype_size(d->dtype);
+  p.x = first(x, d->x_stride, *d, size);
+  p.gate = first(gate, d->gate_stride, *d, size);
+  p.dy = first(dy, d->dy_stride, *d, size);
+  p.dx = const_cast<void*>(first(dx, d->y_stride, *d, size));
+  p.dgate = const_cast<void*>(first(dgate, d->y_stride, *d, size));
+  p.mask = d->masked ? static_cast<const uint8_t*>(first(mask, d->mask_stride, *d, 1)) : nullptr;
+  strides(p.xs, d->x_stride, *d);
+  strides(p.gs, d->gate_stride, *d);
+  strides(p.ds, d->dy_stride, *d);
+  strides(p.ys, d->y_stride, *d);
+  strides(p.ms, d->mask_stride, *d);
+  p.state = state;
+  p.dlast = dlast;
+  p.dstate = dstate;
+  p.saved = const_cast<float*>(saved);
+  p.agg_p = static_cast<float*>(workspace);
+  p.agg_h = p.agg_p + (size_t)p.pieces * p.lines * p.channels;
+  const long long groups = ceil_div(p.columns, p.block_columns);
+  if (groups > (1ll << 31) - 1) return NCA_ERR_UNSUPPORTED;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return with_kind(d->dtype, two_wide(p), [&](auto t, auto v) -> int32_t {
+    using T = decltype(t);
+    constexpr int V = decltype(v)::value;
+    return p.subs > 1 ? run_backward<T, V, kThreadsBack / kLanes>(p, groups, s) : run_backward<T, V, 1>(p, groups, s);
+  });
+}
+
+}  // extern "C"

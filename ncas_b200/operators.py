@@ -78,6 +78,20 @@ def distill_loss_and_grad(logits, teacher_logits, teacher_index, *, temperature=
     return _op("distill_loss_and_grad")(logits, teacher_logits, teacher_index, temperature, weight, reduction)
 
 
+def gated_scan(x, gate, state=None, *, dim=-2, reverse=False, mask=None):
+    """(y, last) of the recurrence y_t = a_t y_{t-1} + (1 - a_t) x_t, a = sigmoid(gate), along axis `dim` of x (..., C).
+
+    x, gate: float32, bfloat16 or float16, one type and shape, any strides (adjacent channels with collapsible axes
+    on either side of `dim` are read in place, others copied); y is contiguous, of that type, and rounded once: the
+    recurrence runs in fp32.  state: the value before the first step, float32, of x's shape without `dim` (absent:
+    zeros); last: the value after the last step, likewise, for the next call of a line that goes on.  reverse: from
+    the last step to the first.  mask: bool or uint8, x's shape without C: where it is zero the value stays as it
+    is, y and the gradients are 0, and what x and gate hold has no effect.  Differentiable in x, gate and state,
+    through y and last.
+    """
+    return _op("gated_scan")(x, gate, state, dim, reverse, mask)
+
+
 def check(device="cuda") -> None:
     """Synchronises the current stream and raises NcaError when a kernel's bounded wait ran out since this
     thread's last call (at first: since it began to use the operators).

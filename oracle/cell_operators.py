@@ -102,3 +102,32 @@ def distill(logits, teacher, index, temperature=1.0, weight=None):
             loss[r] += w * temperature**2 * p * (lp - logq[i])
         grad[r] = w * temperature * (logq.exp() - target)
     return loss, grad
+
+
+def gated_scan(x, gate, state=None, dim=-2, reverse=False, mask=None, dy=None, dlast=None):
+    """(y, last), or with dy a dict of y, last, x, gate, state.  A loop over the steps of axis `dim`."""
+    dim = dim % x.dim()
+    x, gate = x.double().movedim(dim, 0), gate.double().movedim(dim, 0)
+    steps = list(range(x.shape[0]))[:: -1 if reverse else 1]
+    on = torch.ones(x.shape[:-1], dtype=torch.bool) if mask is None else mask.movedim(dim, 0) != 0
+    h = torch.zeros(x.shape[1:], dtype=torch.float64) if state is None else state.double()
+    before, after, y = {}, {}, torch.zeros_like(x)
+    for t in steps:
+        a = torch.sigmoid(gate[t])
+        before[t] = h
+        h = torch.where(on[t][..., None], a * h + torch.sigmoid(-gate[t]) * x[t], h)
+        after[t] = h
+        y[t] = torch.where(on[t][..., None], h, 0.0)
+    if dy is None:
+        return y.movedim(0, dim), h
+    dy = dy.double().movedim(dim, 0)
+    g = torch.zeros_like(h) if dlast is None else dlast.double()
+    dx, dgate = torch.zeros_like(x), torch.zeros_like(x)
+    for t in reversed(steps):
+        live = on[t][..., None]
+        a, keep = torch.sigmoid(gate[t]), torch.sigmoid(-gate[t])
+        full = dy[t] + g
+        dx[t] = torch.where(live, keep * full, 0.0)
+        dgate[t] = torch.where(live, full * (before[t] - x[t]) * a * keep, 0.0)
+        g = torch.where(live, a * full, g)
+    return dict(y=y.movedim(0, dim), last=h, x=dx.movedim(0, dim), gate=dgate.movedim(0, dim), state=g)
