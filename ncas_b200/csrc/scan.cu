@@ -22,12 +22,11 @@ using namespace nca;
 
 namespace {
 
-constexpr int kSub = 16;             // steps of a thread
+constexpr int kSub = 8;             // steps of a thread
 constexpr int kLanes = 32;           // columns of a block whose warps split a line
-constexpr int kThreads = 256;        // forward
-constexpr int kThreadsBack = 128;    // backward: three times the registers
+constexpr int kThreads = 128;
+constexpr int kBlocksAlone = 8, kBlocks = 5, kBlocksBack = 4;  // of a multiprocessor, by their registers
 constexpr int kMostPieces = 128;
-constexpr uint32_t kAll = (1u << kSub) - 1;
 
 struct ScanParams {
   const void *x, *gate, *dy;
@@ -79,6 +78,18 @@ struct Ch<2> {
   static __device__ __forceinline__ F each(F a, O o) { return make_float2(o(a.x), o(a.y)); }
 };
 
+template <class T, int V>
+__device__ __forceinline__ typename Ch<V>::F take(uint32_t v) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(v);
+  } else {
+    float2 t;
+    if constexpr (__is_same(T, __nv_bfloat16)) t = make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+    else t = __half22float2(reinterpret_cast<const __half2&>(v));
+    if constexpr (V == 2) return t;
+    else return t.x;
+  }
+}
 // keep = 1 - a, and a.  Beyond 87, 1 - a is below 2^-125.  NaN stays NaN.  For fp32 data the product
 // gate log2(e) is taken with its rounding error, which would be worth 2^-24 |gate| of the exponential.
 template <class T, int V>
@@ -95,49 +106,106 @@ __device__ __forceinline__ void coefficients(typename Ch<V>::F gate, typename Ch
   keep = C::each(C::add(e, C::of(1.f)), [](float v) { return rcp(v); });
   a = C::mul(e, keep);
 }
+// Of a step that counts only where `live`: else a = 1, so that the state stays.
+template <class T, int V, bool WHOLE>
+__device__ __forceinline__ void coefficients(uint32_t gate, uint32_t live, typename Ch<V>::F& keep, typename Ch<V>::F& a) {
+  coefficients<T, V>(take<T, V>(gate), keep, a);
+  if (!WHOLE && !live) keep = Ch<V>::of(0.f), a = Ch<V>::of(1.f);
+}
 
-// The 4 bytes (one fp32 or two 16-bit channels; one 16-bit channel: 2 bytes) of each of a thread's steps.
+// The next row's place, from this one's: left to itself the compiler keeps 16 multiples of every stride in
+// registers, three times what the data takes.
+template <class P>
+__device__ __forceinline__ void advance(P& at, long long step) {
+  at += step;
+  asm volatile("" : "+l"(at));
+}
+
+// The 4 bytes (one fp32 or two 16-bit channels; one 16-bit channel: 2 bytes) of a thread's steps.
 struct Raw {
   uint32_t v[kSub];
 };
 template <class T, int V>
 __device__ __forceinline__ uint32_t load_one(const T* at) {
-  if constexpr (sizeof(T) * V == 4) return *reinterpret_cast<const uint32_t*>(at);
-  else return *reinterpret_cast<const uint16_t*>(at);
+  if constexpr (sizeof(T) * V == 4) {
+    uint32_t v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(at));
+    return v;
+  } else {
+    uint16_t v;
+    asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(at));
+    return v;
+  }
 }
+// 0 where the step does not count
 template <class T, int V>
-__device__ __forceinline__ void load(Raw& r, const T* at, long long step, uint32_t on) {
-  if (on == kAll) {
+__device__ __forceinline__ uint32_t load_one(const T* at, uint32_t live) {
+  if constexpr (sizeof(T) * V == 4) {
+    uint32_t v = 0;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "+r"(v) : "l"(at), "r"(live));
+    return v;
+  } else {
+    uint16_t v = 0;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p ld.global.b16 %0, [%1];\n\t}" : "+h"(v) : "l"(at), "r"(live));
+    return v;
+  }
+}
+// What a warp works on: all of its threads' steps, or (else) those of each thread's own bits, of which the last of the
+// warp comes before `end`.
+struct Steps {
+  uint32_t in, on;  // that exist; that exist and the mask keeps
+  int end;
+  bool whole;
+  __device__ __forceinline__ Steps(uint32_t in_, uint32_t on_) : in(in_), on(on_) {
+    whole = __all_sync(0xffffffffu, on == (1u << kSub) - 1);
+    end = whole ? kSub : __reduce_max_sync(0xffffffffu, 32 - __clz(in));
+  }
+};
+// The tensors' rows of the steps, N of them side by side.
+template <class T, int V, int N>
+__device__ __forceinline__ void load(Raw (&r)[N], const T* const (&from)[N], const long long (&step)[N], const Steps& st) {
+  const T* at[N];
 #pragma unroll
-    for (int i = 0; i < kSub; ++i) {
-      r.v[i] = load_one<T, V>(at);
-      at += step;
-    }
+  for (int n = 0; n < N; ++n) at[n] = from[n];
+  if (st.whole) {
+#pragma unroll
+    for (int i = 0; i < kSub; ++i)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        r[n].v[i] = load_one<T, V>(at[n]);
+        advance(at[n], step[n]);
+      }
   } else {
 #pragma unroll
     for (int i = 0; i < kSub; ++i) {
-      r.v[i] = 0;
-      if (on >> i & 1) r.v[i] = load_one<T, V>(at);
-      at += step;
+#pragma unroll
+      for (int n = 0; n < N; ++n) r[n].v[i] = 0;
+      if (i < st.end) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          r[n].v[i] = load_one<T, V>(at[n], st.on >> i & 1);
+          advance(at[n], step[n]);
+        }
+      }
     }
   }
 }
-template <class T, int V>
-__device__ __forceinline__ typename Ch<V>::F take(uint32_t v) {
-  if constexpr (sizeof(T) == 4) {
-    return __uint_as_float(v);
-  } else {
-    float2 t;
-    if constexpr (__is_same(T, __nv_bfloat16)) t = make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
-    else t = __half22float2(reinterpret_cast<const __half2&>(v));
-    if constexpr (V == 2) return t;
-    else return t.x;
-  }
+// Asks for the steps from t0 on in L2, a step a lane: the rows of a warp lie within a line of it.
+template <class T>
+__device__ __forceinline__ void ahead(const T* line, long long t0, long long step, long long steps, bool on) {
+  const long long t = t0 + threadIdx.x % kSub;
+  if (on && t < steps) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + t * step));
 }
 template <class T, int V>
 __device__ __forceinline__ void put(T* at, typename Ch<V>::F f) {
   if constexpr (V == 2) *reinterpret_cast<Vec<T, 2>*>(at) = from_pairs<T, 2>({f});
   else *at = from_f32<T>(f);
+}
+// Of a step in a stretch that is not whole: 0 where the mask is, nothing where there is no step.
+template <class T, int V, bool WHOLE>
+__device__ __forceinline__ void put(T* at, typename Ch<V>::F f, const Steps& st, int i) {
+  if (WHOLE || (st.on >> i & 1)) put<T, V>(at, f);
+  else if (st.in >> i & 1) put<T, V>(at, Ch<V>::of(0.f));
 }
 template <int V>
 __device__ __forceinline__ typename Ch<V>::F load_f32(const float* p, long long at, bool on) {
@@ -172,10 +240,18 @@ struct Place {
     sub = p.subs > 1 ? threadIdx.x / kLanes : 0;
     const long long col = (long long)blockIdx.x * p.block_columns + lane;
     on = col < p.columns;
-    line = on ? col / p.per_line : 0;
-    c = on ? (int)(col - line * p.per_line) * V : 0;
-    n = line / p.m;
-    m = line - n * p.m;
+    if (p.columns < 1ll << 31) {  // 64-bit divisions cost a short line more than its steps
+      const unsigned i = on ? (unsigned)col : 0u, l = i / (unsigned)p.per_line, k = l / (unsigned)p.m;
+      line = l;
+      c = (int)(i - l * (unsigned)p.per_line) * V;
+      n = k;
+      m = l - k * (unsigned)p.m;
+    } else {
+      line = on ? col / p.per_line : 0;
+      c = on ? (int)(col - line * p.per_line) * V : 0;
+      n = line / p.m;
+      m = line - n * p.m;
+    }
   }
   __device__ __forceinline__ long long at(const long long (&s)[3]) const { return n * s[0] + m * s[1]; }
   // the steps of the kSub from t0 on that exist (bits), and those of them that the mask keeps
@@ -188,8 +264,10 @@ struct Place {
     const uint8_t* at_mask = p.mask + at(p.ms) + t0 * p.ms[2];
     uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < kSub; ++i)
-      if ((in >> i & 1) && at_mask[i * p.ms[2]]) bits |= 1u << i;
+    for (int i = 0; i < kSub; ++i) {
+      if ((in >> i & 1) && *at_mask) bits |= 1u << i;
+      advance(at_mask, p.ms[2]);
+    }
     return bits;
   }
 };
@@ -234,12 +312,17 @@ __device__ __forceinline__ typename Ch<V>::F enter(const ScanParams& p, const Pl
   return run;
 }
 
+// Whether all steps of a stretch exist and count, for all columns of the block.
+template <int SUBS>
+__device__ __forceinline__ bool whole_stretch(const ScanParams& p, long long k) {
+  return !p.mask && (k + 1) * SUBS * kSub <= p.steps && ((long long)blockIdx.x + 1) * kLanes <= p.columns;
+}
+
 // SUBS: warps along a line (1: a thread walks along it alone, and there is one piece).
 template <class T, int V, int SUBS>
-__global__ void __launch_bounds__(kThreads, 2) scan_forward_kernel(const __grid_constant__ ScanParams p) {
+__global__ void __launch_bounds__(kThreads, SUBS == 1 ? kBlocksAlone : kBlocks) scan_forward_kernel(const __grid_constant__ ScanParams p) {
   using C = Ch<V>;
   using F = typename C::F;
-  constexpr bool kSplit = SUBS > 1;
   may_start_next();
   after_previous();
   __shared__ Exchange<V, SUBS> exchange;
@@ -250,63 +333,53 @@ __global__ void __launch_bounds__(kThreads, 2) scan_forward_kernel(const __grid_
   const long long k0 = blockIdx.y * p.per, k1 = min(k0 + p.per, p.stretches);
   F run = enter<V, false>(p, me);
 
-  Raw rx, rg;
-  long long t0 = (k0 * SUBS + me.sub) * kSub;
-  uint32_t in = 0, on = 0;
-  const auto fetch = [&] {
-    in = me.inside(p, t0);
-    on = me.kept(p, t0, in);
-    load<T, V>(rx, x + t0 * p.xs[2], p.xs[2], on);
-    load<T, V>(rg, g + t0 * p.gs[2], p.gs[2], on);
-  };
-  if (k0 < k1) fetch();
+  Raw r[2];
+  const long long step[2] = {p.xs[2], p.gs[2]}, ystep = p.ys[2];
   for (long long k = k0; k < k1; ++k) {
-    const long long now = t0;
-    const uint32_t in_now = in, on_now = on;
-    F P[kSub], H[kSub];  // a thread alone: H is the state itself
-    {
-      F prod = C::of(1.f), h = kSplit ? C::of(0.f) : run;
+    const long long t0 = (k * SUBS + me.sub) * kSub;
+    const uint32_t in = me.inside(p, t0);
+    const Steps st(in, me.kept(p, t0, in));
+    load<T, V, 2>(r, {x + t0 * step[0], g + t0 * step[1]}, step, st);
+    if (k + 1 < k1) {
+      ahead(x, t0 + SUBS * kSub, step[0], p.steps, me.on);
+      ahead(g, t0 + SUBS * kSub, step[1], p.steps, me.on);
+    }
+    const long long mark = t0 / kSub - 1;
+    float* to_mark = p.saved && mark >= 0 && in ? p.saved + (me.line * p.marks + mark) * p.channels + me.c : nullptr;
+    T* to = y + t0 * ystep;
+    const auto work = [&](auto all) {
+      constexpr bool W = decltype(all)::value != 0;
+      if constexpr (SUBS == 1) {
+        if (to_mark) store_f32<V>(to_mark, 0, run);
 #pragma unroll
-      for (int i = 0; i < kSub; ++i) {
-        F keep, a;
-        coefficients<T, V>(take<T, V>(rg.v[i]), keep, a);
-        const F b = C::mul(keep, take<T, V>(rx.v[i]));
-        if (on_now == kAll || (on_now >> i & 1)) {
-          h = C::fma(a, h, b);
-          if constexpr (kSplit) prod = C::mul(prod, a);
+        for (int i = 0; i < kSub; ++i) {
+          if (!W && i >= st.end) break;
+          F keep, a;
+          coefficients<T, V, W>(r[1].v[i], st.on >> i & 1, keep, a);
+          run = C::fma(a, run, C::mul(keep, take<T, V>(r[0].v[i])));
+          put<T, V, W>(to, run, st, i);
+          advance(to, ystep);
         }
-        H[i] = h;
-        if constexpr (kSplit) P[i] = prod;
-      }
-    }
-    if (k + 1 < k1) {  // the next stretch, in flight from here on
-      t0 += SUBS * kSub;
-      fetch();
-    }
-    F start = run;
-    if constexpr (kSplit) start = exchange.template go<false>(k & 1, me.sub, me.lane, P[kSub - 1], H[kSub - 1], run);
-    const long long mark = now / kSub - 1;
-    if (p.saved && mark >= 0 && in_now) store_f32<V>(p.saved, (me.line * p.marks + mark) * p.channels + me.c, start);
-    T* to = y + now * p.ys[2];
-    if constexpr (kSplit) {
+      } else {
+        F P[kSub], H[kSub], prod = C::of(1.f), h = C::of(0.f);
 #pragma unroll
-      for (int i = 0; i < kSub; ++i) H[i] = C::fma(P[i], start, H[i]);
-    } else {
-      run = H[kSub - 1];
-    }
-    if (on_now == kAll) {
+        for (int i = 0; i < kSub; ++i) {
+          F keep, a;
+          coefficients<T, V, W>(r[1].v[i], st.on >> i & 1, keep, a);
+          H[i] = h = C::fma(a, h, C::mul(keep, take<T, V>(r[0].v[i])));
+          P[i] = prod = C::mul(prod, a);
+        }
+        const F start = exchange.template go<false>(k & 1, me.sub, me.lane, prod, h, run);
+        if (to_mark) store_f32<V>(to_mark, 0, start);
 #pragma unroll
-      for (int i = 0; i < kSub; ++i) {
-        put<T, V>(to, H[i]);
-        to += p.ys[2];
+        for (int i = 0; i < kSub; ++i) {
+          put<T, V, W>(to, C::fma(P[i], start, H[i]), st, i);
+          advance(to, ystep);
+        }
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kSub; ++i) {
-        if (in_now >> i & 1) put<T, V>(to, on_now >> i & 1 ? H[i] : C::of(0.f));
-        to += p.ys[2];
-      }
-    }
+    };
+    if (SUBS == 1 ? st.whole : whole_stretch<SUBS>(p, k)) work(ActTag<1>{});
+    else work(ActTag<0>{});
   }
   if (me.on && me.sub == 0 && (int)blockIdx.y == p.pieces - 1) store_edge<V>(p.last, me.line * p.channels + me.c, run);
 }
@@ -314,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_forward_kernel(const __grid_
 // The maps of the pieces.  Here a warp takes adjacent steps of the piece, so there is one exchange, at the end.
 // Backward: r -> P r + H with r = a G, built in the order of the line: a later step's dy passes the a before it.
 template <class T, int V, int SUBS, bool BACK>
-__global__ void __launch_bounds__(SUBS * kLanes, BACK ? 4 : 2) scan_pieces_kernel(const __grid_constant__ ScanParams p) {
+__global__ void __launch_bounds__(kThreads, kBlocksAlone) scan_pieces_kernel(const __grid_constant__ ScanParams p) {
   using C = Ch<V>;
   using F = typename C::F;
   may_start_next();
@@ -328,31 +401,30 @@ __global__ void __launch_bounds__(SUBS * kLanes, BACK ? 4 : 2) scan_pieces_kerne
   const long long count = min(p.per, p.stretches - z * p.per);
   long long t0 = (z * p.per * SUBS + me.sub * count) * kSub;
   F P = C::of(1.f), H = C::of(0.f);
-  Raw rv, rg;
-  uint32_t on = 0;
-  const auto fetch = [&] {
-    on = me.kept(p, t0, me.inside(p, t0));
-    load<T, V>(rv, v + t0 * vs, vs, on);
-    load<T, V>(rg, g + t0 * p.gs[2], p.gs[2], on);
-  };
-  if (count > 0) fetch();
-  for (long long k = 0; k < count; ++k) {
-    const Raw cv = rv, cg = rg;
-    const uint32_t on_now = on;
-    if (k + 1 < count) {  // the next steps, in flight while these are worked on
-      t0 += kSub;
-      fetch();
+  Raw r[2];
+  const long long step[2] = {vs, p.gs[2]};
+  for (long long k = 0; k < count; ++k, t0 += kSub) {
+    const uint32_t in = me.inside(p, t0);
+    const Steps st(in, me.kept(p, t0, in));
+    load<T, V, 2>(r, {v + t0 * vs, g + t0 * step[1]}, step, st);
+    if (k + 1 < count) {
+      ahead(v, t0 + kSub, vs, p.steps, me.on);
+      ahead(g, t0 + kSub, step[1], p.steps, me.on);
     }
+    const auto work = [&](auto all) {
+      constexpr bool W = decltype(all)::value != 0;
 #pragma unroll
-    for (int i = 0; i < kSub; ++i) {
-      F keep, a;
-      coefficients<T, V>(take<T, V>(cg.v[i]), keep, a);
-      if (on_now == kAll || (on_now >> i & 1)) {
+      for (int i = 0; i < kSub; ++i) {
+        if (!W && i >= st.end) break;
+        F keep, a;
+        coefficients<T, V, W>(r[1].v[i], st.on >> i & 1, keep, a);
         P = C::mul(P, a);
-        if constexpr (BACK) H = C::fma(P, take<T, V>(cv.v[i]), H);
-        else H = C::fma(a, H, C::mul(keep, take<T, V>(cv.v[i])));
+        if constexpr (BACK) H = C::fma(P, take<T, V>(r[0].v[i]), H);
+        else H = C::fma(a, H, C::mul(keep, take<T, V>(r[0].v[i])));
       }
-    }
+    };
+    if (st.whole) work(ActTag<1>{});
+    else work(ActTag<0>{});
   }
   // the whole piece's map: its H from a state of 0, its P as the product over the warps
   F run = C::of(0.f), all = C::of(1.f);
@@ -366,10 +438,9 @@ __global__ void __launch_bounds__(SUBS * kLanes, BACK ? 4 : 2) scan_pieces_kerne
 }
 
 template <class T, int V, int SUBS>
-__global__ void __launch_bounds__(kThreadsBack, 3) scan_backward_kernel(const __grid_constant__ ScanParams p) {
+__global__ void __launch_bounds__(kThreads, kBlocksBack) scan_backward_kernel(const __grid_constant__ ScanParams p) {
   using C = Ch<V>;
   using F = typename C::F;
-  constexpr bool kSplit = SUBS > 1;
   may_start_next();
   after_previous();
   __shared__ Exchange<V, SUBS> exchange;
@@ -380,75 +451,62 @@ __global__ void __launch_bounds__(kThreadsBack, 3) scan_backward_kernel(const __
   T* dx = static_cast<T*>(p.dx) + me.at(p.ys) + me.c;
   T* dg = static_cast<T*>(p.dgate) + me.at(p.ys) + me.c;
   const long long k0 = blockIdx.y * p.per, k1 = min(k0 + p.per, p.stretches);
-  F run = enter<V, true>(p, me);
+  F run = enter<V, true>(p, me), r = run;
 
-  Raw rx, rg, rd;
-  F rh = C::of(0.f);
-  long long t0 = ((k1 - 1) * SUBS + me.sub) * kSub;
-  uint32_t in = 0, on = 0;
-  const auto fetch = [&] {
-    in = me.inside(p, t0);
-    on = me.kept(p, t0, in);
-    load<T, V>(rx, x + t0 * p.xs[2], p.xs[2], on);
-    load<T, V>(rg, g + t0 * p.gs[2], p.gs[2], on);
-    load<T, V>(rd, dy + t0 * p.ds[2], p.ds[2], on);
-    const long long mark = t0 / kSub - 1;  // the state before these steps
-    if (mark < 0) rh = load_edge<V>(p.state, me.line * p.channels + me.c, me.on);
-    else rh = load_f32<V>(p.saved, (me.line * p.marks + mark) * p.channels + me.c, in != 0);
-  };
-  if (k0 < k1) fetch();
+  Raw raw[3];
+  const long long step[3] = {p.xs[2], p.gs[2], p.ds[2]}, ystep = p.ys[2];
   for (long long k = k1 - 1; k >= k0; --k) {
-    const long long now = t0;
-    const uint32_t in_now = in, on_now = on;
-    F keeps[kSub], w[kSub], as[V == 1 ? kSub : 1];
-    F P = C::of(1.f), H = C::of(0.f);
-    // in the order of the line: the states again, w = a (h before - x), and the stretch's map of r = a G
-    {
-      F h = rh;
+    const long long t0 = (k * SUBS + me.sub) * kSub;
+    const uint32_t in = me.inside(p, t0);
+    const Steps st(in, me.kept(p, t0, in));
+    load<T, V, 3>(raw, {x + t0 * step[0], g + t0 * step[1], dy + t0 * step[2]}, step, st);
+    const long long mark = t0 / kSub - 1;  // the state before these steps
+    F h = mark < 0 ? load_edge<V>(p.state, me.line * p.channels + me.c, me.on)
+                   : load_f32<V>(p.saved, (me.line * p.marks + mark) * p.channels + me.c, in != 0);
+    if (k > k0) {
+      ahead(x, t0 - SUBS * kSub, step[0], p.steps, me.on);
+      ahead(g, t0 - SUBS * kSub, step[1], p.steps, me.on);
+      ahead(dy, t0 - SUBS * kSub, step[2], p.steps, me.on);
+    }
+    const auto work = [&](auto all) {
+      constexpr bool W = decltype(all)::value != 0;
+      F keeps[kSub], w[kSub], as[V == 1 ? kSub : 1];
+      F P = C::of(1.f), H = C::of(0.f);
+      // in the order of the line: the states again, w = a (h before - x), and the stretch's map of r = a G
 #pragma unroll
       for (int i = 0; i < kSub; ++i) {
+        if (SUBS == 1 && !W && i >= st.end) break;
         F keep, a;
-        coefficients<T, V>(take<T, V>(rg.v[i]), keep, a);
-        const F xi = take<T, V>(rx.v[i]);
+        coefficients<T, V, W>(raw[1].v[i], st.on >> i & 1, keep, a);
+        const F xi = take<T, V>(raw[0].v[i]);
         w[i] = C::mul(a, C::fma(xi, C::of(-1.f), h));
-        if (on_now == kAll || (on_now >> i & 1)) {
-          h = C::fma(a, h, C::mul(keep, xi));
-          if constexpr (kSplit) {
-            P = C::mul(P, a);
-            H = C::fma(P, take<T, V>(rd.v[i]), H);
-          }
+        h = C::fma(a, h, C::mul(keep, xi));
+        if constexpr (SUBS > 1) {
+          P = C::mul(P, a);
+          H = C::fma(P, take<T, V>(raw[2].v[i]), H);
         }
         keeps[i] = keep;
         if constexpr (V == 1) as[i] = a;
       }
-    }
-    const Raw cd = rd;
-    if (k > k0) {  // the stretch before, in flight from here on
-      t0 -= SUBS * kSub;
-      fetch();
-    }
-    F r = run;
-    if constexpr (kSplit) r = exchange.template go<true>(k & 1, me.sub, me.lane, P, H, run);
-    // from its end: dx = (1 - a) G, dgate = w dx, r = a G.  Two channels: r = G - (1 - a) G in one rounding, since a third
-    // row of registers would halve the blocks; beside 16-bit outputs its error of 2^-24 G is nothing.
-    long long to = (now + kSub - 1) * p.ys[2];
+      if constexpr (SUBS > 1) r = exchange.template go<true>(k & 1, me.sub, me.lane, P, H, run);
+      // from its end: dx = (1 - a) G, dgate = w dx, r = a G.  Two channels: r = G - (1 - a) G in one rounding, since a third
+      // row of registers would cost blocks; beside 16-bit outputs its error of 2^-24 G is nothing.
+      long long to = (t0 + kSub - 1) * ystep;
 #pragma unroll
-    for (int i = kSub - 1; i >= 0; --i) {
-      const F G = C::add(take<T, V>(cd.v[i]), r);
-      F ox = C::mul(keeps[i], G), og = C::mul(w[i], ox);
-      if (on_now == kAll || (on_now >> i & 1)) {
-        if constexpr (V == 1) r = C::mul(as[i], G);
-        else r = C::fma(C::mul(keeps[i], C::of(-1.f)), G, G);
-      } else {
-        ox = og = C::of(0.f);
+      for (int i = kSub - 1; i >= 0; --i) {
+        if (W || i < st.end) {
+          const F G = C::add(take<T, V>(raw[2].v[i]), r), ox = C::mul(keeps[i], G);
+          if constexpr (V == 1) r = C::mul(as[i], G);
+          else r = C::fma(C::mul(keeps[i], C::of(-1.f)), G, G);
+          if (p.dx) put<T, V, W>(dx + to, ox, st, i);
+          if (p.dgate) put<T, V, W>(dg + to, C::mul(w[i], ox), st, i);
+        }
+        advance(to, -ystep);
       }
-      if (on_now == kAll || (in_now >> i & 1)) {
-        if (p.dx) put<T, V>(dx + to, ox);
-        if (p.dgate) put<T, V>(dg + to, og);
-      }
-      to -= p.ys[2];
-    }
-    if constexpr (!kSplit) run = r;
+    };
+    if (SUBS == 1 ? st.whole : whole_stretch<SUBS>(p, k)) work(ActTag<1>{});
+    else work(ActTag<0>{});
+    if constexpr (SUBS == 1) run = r;
   }
   if (p.dstate && me.on && me.sub == 0 && blockIdx.y == 0) store_edge<V>(p.dstate, me.line * p.channels + me.c, run);
 }
@@ -481,7 +539,7 @@ ScanParams plan_of(const NcaScanDesc& d, bool backward) {
   p.per_line = pairs ? d.channels / 2 : d.channels;
   p.columns = p.lines * p.per_line;
   p.marks = d.steps > kSub ? ceil_div(d.steps, kSub) - 1 : 0;
-  const int threads = backward ? kThreadsBack : kThreads, resident = 148 * (backward ? 3 : 2);
+  const int threads = kThreads, resident = 148 * (backward ? kBlocksBack : kBlocks);
   p.subs = d.steps > 2 * kSub && p.columns < (long long)resident * threads / 2 ? threads / kLanes : 1;
   p.block_columns = threads / p.subs;
   p.stretches = ceil_div(d.steps, (long long)p.subs * kSub);
@@ -534,11 +592,11 @@ int32_t run_backward(const ScanParams& p, long long groups, cudaStream_t s) {
   if constexpr (SUBS > 1) {
     if (p.pieces > 1) {
       const int32_t e = launch_after(scan_pieces_kernel<T, V, SUBS, true>, dim3((unsigned)groups, p.pieces - 1),
-                                     dim3(kThreadsBack), 0, s, 1, p);
+                                     dim3(kThreads), 0, s, 1, p);
       if (e != NCA_OK) return e;
     }
   }
-  return launch_after(scan_backward_kernel<T, V, SUBS>, dim3((unsigned)groups, p.pieces), dim3(kThreadsBack), 0, s, 1, p);
+  return launch_after(scan_backward_kernel<T, V, SUBS>, dim3((unsigned)groups, p.pieces), dim3(kThreads), 0, s, 1, p);
 }
 
 }  // namespace
@@ -632,7 +690,7 @@ int32_t nca_b200_gated_scan_backward(const NcaScanDesc* d, const void* x, const 
   return with_kind(d->dtype, two_wide(p), [&](auto t, auto v) -> int32_t {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
-    return p.subs > 1 ? run_backward<T, V, kThreadsBack / kLanes>(p, groups, s) : run_backward<T, V, 1>(p, groups, s);
+    return p.subs > 1 ? run_backward<T, V, kThreads / kLanes>(p, groups, s) : run_backward<T, V, 1>(p, groups, s);
   });
 }
 
