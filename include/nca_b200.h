@@ -458,6 +458,25 @@ int32_t nca_b200_gated_scan_backward(const NcaScanDesc* d, const void* x, const 
                                      float* dstate, void* workspace, size_t workspace_bytes,
                                      void* stream);
 
+/* X = M / (|M|_F + eps), then `steps` times X = a X + (b A + c A^2) X with A = X X^T (of a tall matrix
+ * X = a X + X (b A + c A^2), A = X^T X), for every matrix of a batch: singular values towards 1.  Products of fp16
+ * operands with fp32 sums; X keeps 22 bits between the steps.  Coefficients that let a singular value of [0, 1] grow
+ * beyond 2 within the steps are NCA_ERR_UNSUPPORTED. */
+typedef struct NcaOrthoDesc {
+  int64_t batch, rows, cols;
+  int32_t dtype;               /* NCA_BF16 or NCA_F16, of the matrix and the result */
+  int32_t steps;               /* 1 to 1000 */
+  double coefficients[3];      /* a, b, c */
+  double eps;
+  int64_t stride[2];           /* of the input: (matrix, row); columns are adjacent */
+} NcaOrthoDesc;
+
+int32_t nca_b200_orthogonalize_workspace(const NcaOrthoDesc* d, size_t* bytes);
+/* out: contiguous [batch][rows][cols]; it may not overlap the input.  ctrl, timeout_ms: as nca_b200_gated_ffn. */
+int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* out,
+                               void* workspace, size_t workspace_bytes, int32_t* ctrl,
+                               int32_t timeout_ms, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -187,6 +187,19 @@ class NcaScanDesc(C.Structure):
     ]
 
 
+class NcaOrthoDesc(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int64),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("dtype", C.c_int32),
+        ("steps", C.c_int32),
+        ("coefficients", C.c_double * 3),
+        ("eps", C.c_double),
+        ("stride", C.c_int64 * 2),
+    ]
+
+
 # name -> (restype, argtypes); must match include/nca_b200.h
 _P = C.c_void_p
 _I = C.c_int32
@@ -259,6 +272,8 @@ SIGNATURES = {
     "nca_b200_gated_scan_saved_bytes": (_I, [C.POINTER(NcaScanDesc), C.POINTER(C.c_size_t)]),
     "nca_b200_gated_scan_workspace": (_I, [C.POINTER(NcaScanDesc), _I, C.POINTER(C.c_size_t)]),
     "nca_b200_gated_scan": (_I, [C.POINTER(NcaScanDesc), *[_P] * 8, C.c_size_t, _P]),
+    "nca_b200_orthogonalize_workspace": (_I, [C.POINTER(NcaOrthoDesc), C.POINTER(C.c_size_t)]),
+    "nca_b200_orthogonalize": (_I, [C.POINTER(NcaOrthoDesc), _P, _P, _P, C.c_size_t, _P, _I, _P]),
     "nca_b200_gated_scan_backward": (_I, [C.POINTER(NcaScanDesc), *[_P] * 11, C.c_size_t, _P]),
 }
 

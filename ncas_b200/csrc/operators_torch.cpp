@@ -11,7 +11,9 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <array>
+#include <cmath>
 #include <cstdlib>
 #include <mutex>
 #include <optional>
@@ -775,6 +777,49 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& x, const Tensor& gate, const
   return {y, last};
 }
 
+// -------------------------------------------------------------------------------- orthogonalised update
+Tensor orthogonalize(const Tensor& matrix, int64_t steps, at::ArrayRef<double> coefficients, double eps) {
+  constexpr const char* op = "orthogonalize";
+  on_cuda(matrix, op, "matrix");
+  no_tangent(matrix, op, "matrix");
+  TORCH_CHECK_VALUE(!matrix.requires_grad() || !at::GradMode::is_enabled(), op, ": matrix gets no gradient: detach it");
+  TORCH_CHECK_TYPE(matrix.scalar_type() == at::kBFloat16 || matrix.scalar_type() == at::kHalf, op,
+                   ": matrix must be bfloat16 or float16, not ", matrix.scalar_type());
+  TORCH_CHECK_VALUE(matrix.dim() >= 2, op, ": matrix must be (..., rows, cols), not ", matrix.sizes());
+  TORCH_CHECK_VALUE(steps >= 1 && steps <= 1000, op, ": steps must lie between 1 and 1000, not ", steps);
+  TORCH_CHECK_VALUE(coefficients.size() == 3, op, ": coefficients must be three numbers");
+  TORCH_CHECK_VALUE(eps >= 0 && std::isfinite(eps), op, ": eps must be finite and not negative, not ", eps);
+  NcaOrthoDesc d{};
+  d.rows = matrix.size(-2);
+  d.cols = matrix.size(-1);
+  d.dtype = matrix.scalar_type() == at::kBFloat16 ? NCA_BF16 : NCA_F16;
+  d.steps = (int32_t)steps;
+  std::copy(coefficients.begin(), coefficients.end(), d.coefficients);
+  d.eps = eps;
+  Tensor m = matrix;
+  const auto view = [&] {
+    return (d.cols <= 1 || m.stride(-1) == 1) && collapse(m, 0, m.dim() - 2, &d.batch, &d.stride[0]);
+  };
+  if (!view()) {
+    m = matrix.contiguous();
+    view();
+  }
+  d.stride[1] = m.stride(-2);
+  const c10::cuda::CUDAGuard guard(matrix.device());
+  size_t bytes = 0;
+  const int32_t st = nca_b200_orthogonalize_workspace(&d, &bytes);
+  TORCH_CHECK_VALUE(st != NCA_ERR_INVALID, op, ": coefficients must be finite");
+  TORCH_CHECK_VALUE(st != NCA_ERR_UNSUPPORTED, op, ": the coefficients let a singular value grow beyond 2 within ", steps,
+                    " steps (or a size is above 2^30)");
+  check(st, "nca_b200_orthogonalize_workspace");
+  Tensor out = at::empty(matrix.sizes(), matrix.options().memory_format(at::MemoryFormat::Contiguous));
+  Tensor ws = scratch(bytes, matrix), ctrl = control_words(matrix.device());
+  check(nca_b200_orthogonalize(&d, ptr(m), mptr(out), mptr(ws), bytes_of(ws), static_cast<int32_t*>(mptr(ctrl)),
+                               timeout_ms(), stream_of(matrix)),
+        "nca_b200_orthogonalize");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(nca_b200, m) {
@@ -791,5 +836,6 @@ TORCH_LIBRARY_FRAGMENT(nca_b200, m) {
         &distill_loss_and_grad);
   m.def("gated_scan(Tensor x, Tensor gate, Tensor? state, int dim, bool reverse, Tensor? mask) -> (Tensor, Tensor)",
         &gated_scan);
+  m.def("orthogonalize(Tensor matrix, int steps, float[] coefficients, float eps) -> Tensor", &orthogonalize);
   m.def("operators_status(Tensor like) -> int[]", &operators_status);
 }

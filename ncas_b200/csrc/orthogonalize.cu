@@ -1,0 +1,711 @@
+// orthogonalize.cu -- the orthogonalised update of a matrix by Newton-Schulz products
+// (nca_b200_orthogonalize): X = M / (|M|_F + eps), then `steps` times
+//
+//   A = X X^T,  B = b A + c A^2,  X = a X + B X        (of a tall matrix A = X^T X, X = a X + X B)
+//
+// which brings the singular values of M towards 1.  The products run on the tensor cores with fp16 operands
+// and fp32 sums, for bf16 input too: powers of two keep every operand in fp16's range (|X| <= 2 is checked
+// for the coefficients), and its 11 bits leave an eighth of the error that bf16 operands would.  X is kept
+// as hi + lo, two fp16 values of 22 bits together: a X amplifies what is left in the small singular
+// directions by a at every step, and with X in 11 bits that would be rounding noise (6 % of the result
+// for a matrix of rank 1).  The products read hi alone: their errors appear only beside large singular values,
+// which nothing amplifies.
+//
+// A and A^2 are symmetric: tiles above the diagonal are computed, and stored twice.
+//
+// One product kernel, built as gemm.cuh's: a persistent CTA or CTA pair (cta_group::2) a multiprocessor, warp 0
+// loads tiles by TMA, warp 1 issues the MMAs, warps 4-11 take the accumulators out, add the terms that they load by
+// TMA and store by TMA; two accumulators in tensor memory.  Matrices of a batch are the third dimension of
+// the tensor maps, so that a tile reaches over its own matrix's edge into zeros and writes nothing there.
+#include "gemm.cuh"
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+using namespace nca;
+
+namespace {
+
+#define NCA_TRY(call)                    \
+  do {                                   \
+    const int32_t st_ = (call);          \
+    if (st_ != NCA_OK) return st_;       \
+  } while (0)
+
+inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+inline long long pad8(long long v) { return (v + 7) / 8 * 8; }
+constexpr int kMaxDevices = 64;
+
+// X is stored times 2^12: |X| <= 2 stays below 2^13, and the entries of a normalised matrix of 2^24 and more values
+// are still normal fp16 numbers.  A, |A| <= 4, is stored times 2^10.
+constexpr float kScaleX = 4096.f, kScaleA = 1024.f;
+
+enum OrthoStep {
+  STEP_POWER = 0,  // out = alpha D + beta src: A, and B
+  STEP_UPDATE = 1  // X: alpha D + beta (hi + lo), stored as hi + lo, or as the result
+};
+
+struct OrthoParams {
+  CUtensorMap a, b;
+  CUtensorMap src[2];  // boxes of 32 rows of 64 bytes: what the epilogue reads
+  CUtensorMap out[2];
+  int m, n;  // of D
+  int m_tiles, n_tiles, batch, kb;
+  int symmetric;
+  int terms;  // matrices in src
+  int last;   // STEP_UPDATE: out[0] is the result
+  int out_bf16, plain_c;
+  float alpha, beta, scale;
+  uint16_t* c;  // the result, where its rows lie on no 16-byte boundaries
+  long long ldc;
+  int* ctrl;
+  unsigned long long timeout_ns;
+};
+
+template <int CG>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  if constexpr (CG == 1)
+    tma_load_3d(dst, map, bar, x, y, z);
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+        "%5}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// A lane's 32 values as a column of a place: row c of the place holds column c of the warp's 32 rows.
+__device__ __forceinline__ void put_column(uint32_t place, int lane, const float (&f)[32]) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const uint32_t at = place + 64 * c + ((16 * (lane >> 3)) ^ (16 * ((c >> 1) & 3))) + 2 * (lane & 7);
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(__half_as_ushort(__float2half_rn(f[c]))) : "memory");
+  }
+}
+__device__ __forceinline__ void unpack_half(const uint4 (&q)[4], float (&f)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = __half22float2(reinterpret_cast<const __half2&>(w[j]));
+      f[8 * i + 2 * j] = t.x;
+      f[8 * i + 2 * j + 1] = t.y;
+    }
+  }
+}
+
+struct OrthoTile {
+  int m0, n0, z;
+};
+// Symmetric: of tile row i the tiles from the diagonal on.
+__host__ __device__ __forceinline__ int tiles_of(const OrthoParams& p, int tm, int tn) {
+  if (!p.symmetric) return p.m_tiles * p.n_tiles;
+  return p.m_tiles * p.n_tiles - (tm / tn) * (p.m_tiles * (p.m_tiles - 1) / 2);
+}
+template <int TM, int TN>
+__device__ __forceinline__ OrthoTile tile_at(const OrthoParams& p, int per, int t) {
+  OrthoTile r;
+  r.z = t / per;
+  int i = t - r.z * per;
+  if (p.symmetric) {
+    int row = 0;
+    for (int left = p.n_tiles; i >= left; left -= TM / TN) {
+      i -= left;
+      ++row;
+    }
+    r.m0 = row * TM;
+    r.n0 = (row * (TM / TN) + i) * TN;
+  } else {  // groups of 8 tile rows, columns within: tiles that run together share operands in L2
+    const int group = 8 * p.n_tiles, g = i / group, rows = min(8, p.m_tiles - g * 8);
+    i -= g * group;
+    r.m0 = (g * 8 + i % rows) * TM;
+    r.n0 = (i / rows) * TN;
+  }
+  return r;
+}
+
+template <int CG, int BN>
+using OrthoShape = GemmShape<CG, BN, EPI_DGATE>;  // four places an epilogue warp
+
+template <int CG, int BN, bool A_MN, bool B_MN, int STEP>
+__global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_constant__ OrthoParams p) {
+  using S = OrthoShape<CG, BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::kBars);
+  uint64_t* empty = full + S::kStages;
+  uint64_t* acc_full = empty + S::kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drained = acc_empty + 2;
+  uint64_t* loaded = drained + 1;  // the terms of each epilogue warp
+  uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(loaded + kEpilogueWarps);
+  volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_base_s + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 1 ? 0 : cta_rank_in_cluster();
+  const FailState fs{p.ctrl, abort_s, 0, p.timeout_ns, true};
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], kEpilogueWarps * CG);
+    }
+    mbar_init(drained, 1);
+    for (int i = 0; i < kEpilogueWarps; ++i) mbar_init(&loaded[i], 1);
+    *abort_s = 0;
+    fence_mbar_init();
+  }
+  if (warp == 2) tc_alloc<CG>(tmem_base_s, S::kTmemCols);
+  may_start_next();
+  after_previous();
+  tc_fence_before();
+  if constexpr (CG == 2) cluster_sync_all();
+  else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_base_s;
+
+  const int per = tiles_of(p, kBM * CG, BN), tiles = per * p.batch;
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      long long issued = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        const OrthoTile tl = tile_at<kBM * CG, BN>(p, per, t);
+        const int am = tl.m0 + (int)rank * kBM, bn = tl.n0 + (int)rank * S::kBNc;
+        for (int kb = 0; kb < p.kb; ++kb) {
+          if (!mbar_wait(&empty[s], ph ^ 1, fs, 111)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], S::kStageBytes * CG);
+          const uint32_t bar = CG == 1 ? smem_u32(&full[s]) : map_to_rank(smem_u32(&full[s]), 0);
+          const uint32_t sa = smem_u32(smem + s * S::kStageBytes), sb = sa + S::kABytes;
+          const int k0 = kb * kBK;
+          if constexpr (A_MN) {
+#pragma unroll
+            for (int i = 0; i < kBM / 64; ++i) load_tile<CG>(sa + i * 8192, &p.a, bar, am + 64 * i, k0, tl.z);
+          } else {
+            load_tile<CG>(sa, &p.a, bar, k0, am, tl.z);
+          }
+          if constexpr (B_MN) {
+#pragma unroll
+            for (int i = 0; i < S::kBNc / 64; ++i) load_tile<CG>(sb + i * 8192, &p.b, bar, bn + 64 * i, k0, tl.z);
+          } else {
+            load_tile<CG>(sb, &p.b, bar, k0, bn, tl.z);
+          }
+          ++issued;
+          if (++s == S::kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+      if (rank == 0) {  // loads in flight land before this CTA leaves, whichever warp gave up (bounded)
+        for (long long i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
+          for (int tries = 0; tries < 64 && !mbar_try_wait(&full[i % S::kStages], (i / S::kStages) & 1); ++tries) {
+          }
+      }
+    }
+  } else if (warp == 1 && rank == 0) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
+                                 ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM * CG >> 4) << 24);  // fp16, fp32 sums
+      constexpr uint32_t a_step = (A_MN ? 2048 : 32) >> 4, b_step = (B_MN ? 2048 : 32) >> 4;
+      int s = 0, buf = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        if (!mbar_wait(&acc_empty[buf], acc_ph ^ 1, fs, 112)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + buf * BN;
+        for (int kb = 0; kb < p.kb; ++kb) {
+          if (!mbar_wait(&full[s], ph, fs, 113)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * S::kStageBytes), sb = sa + S::kABytes;
+          const uint64_t da = smem_desc(sa, A_MN ? 8192 : 16, 1024);
+          const uint64_t db = smem_desc(sb, B_MN ? 8192 : 16, 1024);
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k) umma_ss<CG>(d, da + k * a_step, db + k * b_step, idesc, kb > 0 || k > 0);
+          tc_commit<CG>(&empty[s]);
+          if (++s == S::kStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+        if (!ok) break;
+        tc_commit<CG>(&acc_full[buf]);
+        buf ^= 1;
+        if (buf == 0) acc_ph ^= 1;
+      }
+      // the MMAs in flight end before the tensor memory is freed, also when only the epilogue gave up (bounded)
+      umma_commit_local<CG>(drained);
+      for (int tries = 0; tries < 64 && !mbar_try_wait(drained, 0); ++tries) {
+      }
+    }
+  } else if (warp >= 4) {
+    const int q = (warp - 4) & 3, turn = (warp - 4) >> 2;  // tensor memory lanes 32 q .. 32 q + 31
+    // places: 0 and 3 stored from, 1 and 2 loaded to
+    const uint32_t place = smem_u32(smem + S::kPlacesAt) + (warp - 4) * S::kPlaces * kPlace;
+    uint64_t* mine = &loaded[warp - 4];
+    uint32_t load_ph = 0, ph = 0;
+    int buf = 0;
+    bool ok = true, pending = false;  // pending: terms asked for and not yet waited for
+    for (int t = first; t < tiles && ok; t += step) {
+      const OrthoTile tl = tile_at<kBM * CG, BN>(p, per, t);
+      const int row0 = tl.m0 + (int)rank * kBM + 32 * q, cols = min(BN, p.n - tl.n0);
+      const bool rows = row0 < p.m;
+      const bool mirror = STEP == STEP_POWER && p.symmetric && tl.n0 >= tl.m0 + kBM * CG;
+      const auto ask = [&](int c) {
+        pending = true;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(mine, p.terms * kPlace);
+          for (int i = 0; i < p.terms; ++i) tma_load_3d(place + (1 + i) * kPlace, &p.src[i], smem_u32(mine), tl.n0 + c, row0, tl.z);
+        }
+      };
+      const bool asks = p.terms > 0 && rows;
+      if (asks && 32 * turn < cols) ask(32 * turn);
+      ok = mbar_wait_warp(&acc_full[buf], ph, fs, 114);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * BN + ((uint32_t)(32 * q) << 16);
+      for (int c = 32 * turn; c < cols && rows; c += 64) {
+        const int col = tl.n0 + c;
+        float f[32];
+        if (asks) {
+          ok = mbar_wait_warp(mine, load_ph, fs, 115);
+          if (!ok) break;
+          load_ph ^= 1;
+          pending = false;
+          uint4 k0[4], k1[4];
+          take_row(place + kPlace, lane, k0);
+          if (STEP == STEP_UPDATE) take_row(place + 2 * kPlace, lane, k1);
+          // every lane's reads come before the copy that overwrites them
+          fence_async_proxy();
+          __syncwarp();
+          if (c + 64 < cols) ask(c + 64);
+          unpack_half(k0, f);
+          if (STEP == STEP_UPDATE) {
+            float lo[32];
+            unpack_half(k1, lo);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] += lo[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = 0.f;
+        }
+        uint32_t r[32];
+        tmem_take32(acc + c, r);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = fmaf(p.alpha, __uint_as_float(r[i]), p.beta * f[i]);
+        uint4 v[4];
+        if (STEP == STEP_UPDATE && p.last) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] *= p.scale;
+          if (p.out_bf16) pack_row<__nv_bfloat16>(f, v);
+          else pack_row<__half>(f, v);
+        } else {
+          pack_row<__half>(f, v);
+        }
+        if (lane == 0) bulk_wait_read<0>();  // the places have been read
+        __syncwarp();
+        put_row(place, lane, v);
+        if (STEP == STEP_UPDATE && p.last && p.plain_c) {
+          __syncwarp();
+          store_plain(place, lane, p.c + ((long long)tl.z * p.m + row0) * p.ldc + col, p.ldc, min(32, p.m - row0),
+                      min(32, cols - c));
+          __syncwarp();
+          continue;
+        }
+        if (STEP == STEP_UPDATE && !p.last) {  // what hi leaves
+          float hi[32];
+          unpack_half(v, hi);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] -= hi[i];
+          pack_row<__half>(f, v);
+          put_row(place + 3 * kPlace, lane, v);
+        }
+        if (mirror) put_column(place + 3 * kPlace, lane, f);
+        fence_async_proxy();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(&p.out[0], place, col, row0, tl.z);
+          if (mirror) tma_store_3d(&p.out[0], place + 3 * kPlace, row0, col, tl.z);
+          if (STEP == STEP_UPDATE && !p.last) tma_store_3d(&p.out[1], place + 3 * kPlace, col, row0, tl.z);
+          bulk_commit();
+        }
+      }
+      if (!ok) break;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2) mbar_arrive_cluster_relaxed(map_to_rank(smem_u32(&acc_empty[buf]), 0));
+        else mbar_arrive_relaxed(&acc_empty[buf]);
+      }
+      buf ^= 1;
+      if (buf == 0) ph ^= 1;
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the stores are done
+    if (pending)  // after a wait that ran out: the load in flight lands before this CTA leaves (bounded)
+      for (int tries = 0; tries < 64 && !mbar_try_wait(mine, load_ph); ++tries) {
+      }
+  }
+  __syncwarp();
+  tc_fence_before();
+  if constexpr (CG == 2) cluster_sync_all();
+  else __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tc_dealloc<CG>(tmem, S::kTmemCols);
+}
+
+// ------------------------------------------------------------------------- the norm and the first X
+struct StartParams {
+  const void* m;
+  long long rows, cols, batch_stride, row_stride, pitch;
+  double* part;  // [batch][parts]
+  int parts;
+  double eps;
+  __half *hi, *lo;  // [batch][rows][pitch]
+};
+// Sums of squares in 64 bits: squares of bf16 values leave the range of fp32.  One block a part: rows in turn.
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(256) ortho_norm_kernel(const __grid_constant__ StartParams p) {
+  may_start_next();
+  after_previous();
+  constexpr int V = WIDE ? 8 : 1;
+  const long long z = blockIdx.y, per = (p.cols + V - 1) / V, count = p.rows * per;
+  const T* m = static_cast<const T*>(p.m) + z * p.batch_stride;
+  double s = 0;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) {
+    const long long r = i / per, c = (i - r * per) * V;
+    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(m + r * p.row_stride + c);
+    double t = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const double d = to_f32<T>(v.v[j]);
+      t = fma(d, d, t);
+    }
+    s += t;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  __shared__ double red[8];
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int i = 1; i < 8; ++i) s += red[i];
+  p.part[z * p.parts + blockIdx.x] = s;
+}
+// X_0 = M / (|M|_F + eps).
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(256) ortho_start_kernel(const __grid_constant__ StartParams p) {
+  may_start_next();
+  after_previous();
+  constexpr int V = WIDE ? 8 : 1;
+  __shared__ double scale_s;
+  const long long z = blockIdx.y;
+  if (threadIdx.x < 32) {  // every block adds the parts up in the same order
+    double s = 0;
+    for (int i = threadIdx.x; i < p.parts; i += 32) s += p.part[z * p.parts + i];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x == 0) scale_s = kScaleX / (sqrt(s) + p.eps);
+  }
+  __syncthreads();
+  const double scale = scale_s;
+  const float small = (float)scale;
+  const bool fits = small >= 0x1p-120f && small <= 0x1p120f;  // else (norms at the ends of bf16) the product in 64 bits
+  const long long per = p.cols / V, count = p.rows * per;
+  const T* m = static_cast<const T*>(p.m) + z * p.batch_stride;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) {
+    const long long r = i / per, c = (i - r * per) * V, at = (z * p.rows + r) * p.pitch + c;
+    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(m + r * p.row_stride + c);
+    Vec<__half, V> hi, lo;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float x = to_f32<T>(v.v[j]), f = fits ? x * small : (float)(x * scale);
+      hi.v[j] = __float2half_rn(f);
+      lo.v[j] = __float2half_rn(f - __half2float(hi.v[j]));
+    }
+    *reinterpret_cast<Vec<__half, V>*>(p.hi + at) = hi;
+    *reinterpret_cast<Vec<__half, V>*>(p.lo + at) = lo;
+  }
+}
+
+// --------------------------------------------------------------------------------------- host side
+int sm_count() {
+  static std::atomic<int> kept[kMaxDevices];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  n = kept[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    kept[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static std::atomic<EncodeFn> kept{nullptr};
+  EncodeFn f = kept.load(std::memory_order_acquire);
+  if (!f) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    f = reinterpret_cast<EncodeFn>(p);
+    kept.store(f, std::memory_order_release);
+  }
+  return f;
+}
+
+// A stack of 16-bit matrices, rows `ld` values apart.
+struct Stack {
+  const void* p;
+  long long rows, cols, ld, batch;
+};
+// Boxes of `box_cols` x `box_rows` of one matrix; outside reads as zero and is not written.
+bool encode(CUtensorMap* map, const Stack& m, CUtensorMapDataType type, int box_cols, int box_rows) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.batch};
+  const cuuint64_t strides[2] = {(cuuint64_t)m.ld * 2, (cuuint64_t)(m.ld * m.rows) * 2};
+  const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+  const cuuint32_t one[3] = {1, 1, 1};
+  return fn(map, type, 3, const_cast<void*>(m.p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool encode_operand(CUtensorMap* map, const Stack& m, bool mn, int rows) {
+  return encode(map, m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 64, mn ? 64 : rows);
+}
+bool encode_places(CUtensorMap* map, const Stack& m, bool bf16 = false) {
+  return encode(map, m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 32, 32);
+}
+
+template <int CG, int BN, bool A_MN, bool B_MN, int STEP>
+int32_t launch(OrthoParams& p, const Stack& a, const Stack& b, cudaStream_t s) {
+  using S = OrthoShape<CG, BN>;
+  auto* kernel = ortho_kernel<CG, BN, A_MN, B_MN, STEP>;
+  static std::atomic<uint64_t> ready{0};  // a bit for each device whose shared-memory limit is set
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
+  if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess)
+      return launch_status() == NCA_OK ? NCA_ERR_CUDA : NCA_ERR_DEVICE;
+    ready.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  if (!encode_operand(&p.a, a, A_MN, kBM) || !encode_operand(&p.b, b, B_MN, S::kBNc)) return NCA_ERR_CUDA;
+  p.m_tiles = (int)ceil_div(p.m, kBM * CG);
+  // symmetric: whole blocks on the diagonal, the last of whose tiles may be empty
+  p.n_tiles = p.symmetric ? p.m_tiles * (kBM * CG / BN) : (int)ceil_div(p.n, BN);
+  if ((long long)p.m_tiles * p.n_tiles > (1ll << 31) - 1024) return NCA_ERR_UNSUPPORTED;
+  const long long tiles = (long long)tiles_of(p, kBM * CG, BN) * p.batch;
+  if (tiles > (1ll << 31) - 1024) return NCA_ERR_UNSUPPORTED;
+  const long long room = sm_count() / CG;
+  return launch_after(kernel, dim3((unsigned)((tiles < room ? tiles : room) * CG)), dim3(kGemmThreads), S::kSmem, s, CG, p);
+}
+
+// The tile of a product by the cost of its waves, as the gated block's: a k block costs a 256 x 256 tile of a pair of
+// multiprocessors 0.28 us, a 256 x 128 tile 0.24 and a 128 x 128 tile of one 0.25, a wave 3 us besides.
+template <bool A_MN, bool B_MN, int STEP>
+int32_t product(OrthoParams& p, const Stack& a, const Stack& b, cudaStream_t s) {
+  static const struct {
+    int cg, bn;
+    double us;
+  } kinds[] = {{2, 256, 0.28}, {2, 128, 0.24}, {1, 128, 0.25}};
+  int best = 0;
+  double least = 1e30;
+  for (int i = 0; i < 3; ++i) {
+    const long long tm = 128 * kinds[i].cg, mt = ceil_div(p.m, tm);
+    long long tiles = mt * ceil_div(p.n, kinds[i].bn);
+    if (p.symmetric) tiles = (tm / kinds[i].bn) * (mt * (mt + 1) / 2);
+    const double us = (double)ceil_div(tiles * p.batch, sm_count() / kinds[i].cg) * (p.kb * kinds[i].us + 3.0);
+    if (us < least) {
+      least = us;
+      best = i;
+    }
+  }
+  if (best == 0) return launch<2, 256, A_MN, B_MN, STEP>(p, a, b, s);
+  return best == 1 ? launch<2, 128, A_MN, B_MN, STEP>(p, a, b, s) : launch<1, 128, A_MN, B_MN, STEP>(p, a, b, s);
+}
+
+int32_t check_desc(const NcaOrthoDesc* d) {
+  if (!d || d->batch < 0 || d->rows < 0 || d->cols < 0 || d->steps < 1) return NCA_ERR_INVALID;
+  if (!(d->eps >= 0) || !std::isfinite(d->eps)) return NCA_ERR_INVALID;
+  for (int i = 0; i < 3; ++i)
+    if (!std::isfinite(d->coefficients[i])) return NCA_ERR_INVALID;
+  if (d->dtype != NCA_BF16 && d->dtype != NCA_F16) return dtype_ok(d->dtype) ? NCA_ERR_UNSUPPORTED : NCA_ERR_INVALID;
+  const long long most = 1ll << 30;
+  if (d->rows > most || d->cols > most || d->batch > most) return NCA_ERR_UNSUPPORTED;
+  if (d->steps > 1000 || d->batch > 65535) return NCA_ERR_UNSUPPORTED;
+  // the largest singular value after every step, from [0, 1]: x (a + b x^2 + c x^4) is largest at the end of the range
+  // or where a + 3 b x^2 + 5 c x^4 = 0
+  const double a = d->coefficients[0], b = d->coefficients[1], c = d->coefficients[2];
+  const auto image = [&](double x) { return std::fabs(x * (a + x * x * (b + x * x * c))); };
+  const double root = std::sqrt(std::max(0.0, 9 * b * b - 20 * a * c));
+  const double inner[3] = {(-3 * b + root) / (10 * c), (-3 * b - root) / (10 * c), -a / (3 * b)};  // x^2; the last for c = 0
+  double range = 1.0;
+  for (int k = 0; k < d->steps; ++k) {
+    double most = image(range);
+    for (double x2 : inner)
+      if (x2 > 0 && x2 < range * range) most = std::max(most, image(std::sqrt(x2)));
+    if (!(most <= 2.0)) return NCA_ERR_UNSUPPORTED;
+    range = most;
+  }
+  return NCA_OK;
+}
+
+struct Plan {
+  long long small, pitch, small_pitch;
+  bool tall;
+  size_t x[2][2], a, b, part, total;  // x[buffer][hi, lo]
+  int parts;
+};
+Plan plan_of(const NcaOrthoDesc& d) {
+  Plan p{};
+  p.tall = d.rows > d.cols;
+  p.small = std::min(d.rows, d.cols);
+  p.pitch = pad8(d.cols);
+  p.small_pitch = pad8(p.small);
+  size_t at = 0;
+  const size_t x = align256((size_t)d.batch * d.rows * p.pitch * 2), a = align256((size_t)d.batch * p.small * p.small_pitch * 2);
+  for (auto& buffer : p.x)
+    for (size_t& part : buffer) {
+      part = at;
+      at += x;
+    }
+  p.a = at;
+  at += a;
+  p.b = at;
+  at += a;
+  p.part = at;
+  p.parts = (int)std::max<long long>(1, std::min<long long>(ceil_div(d.rows * d.cols, 4096), ceil_div(592, d.batch ? d.batch : 1)));
+  at += align256((size_t)d.batch * p.parts * sizeof(double));
+  p.total = at + 256;
+  return p;
+}
+
+template <class T, bool WIDE>
+int32_t start(const StartParams& p, long long batch, cudaStream_t s) {
+  if (batch > 65535) return NCA_ERR_UNSUPPORTED;
+  NCA_TRY(launch_after(ortho_norm_kernel<T, WIDE>, dim3(p.parts, (unsigned)batch), dim3(256), 0, s, 1, p));
+  const long long blocks = std::min<long long>(ceil_div(p.rows * p.cols, WIDE ? 4096 : 1024), 148 * 8);
+  return launch_after(ortho_start_kernel<T, WIDE>, dim3((unsigned)blocks, (unsigned)batch), dim3(256), 0, s, 1, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t nca_b200_orthogonalize_workspace(const NcaOrthoDesc* d, size_t* bytes) {
+  const int32_t st = check_desc(d);
+  if (st != NCA_OK || !bytes) return st != NCA_OK ? st : NCA_ERR_INVALID;
+  *bytes = d->batch && d->rows && d->cols ? plan_of(*d).total : 0;
+  return NCA_OK;
+}
+
+int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* out, void* workspace,
+                               size_t workspace_bytes, int32_t* ctrl, int32_t timeout_ms, void* stream) {
+  NCA_TRY(check_desc(d));
+  if (d->batch == 0 || d->rows == 0 || d->cols == 0) return NCA_OK;
+  const Plan pl = plan_of(*d);
+  if (!matrix || !out || !ctrl) return NCA_ERR_INVALID;
+  if (!workspace || workspace_bytes < pl.total) return NCA_ERR_SCRATCH;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255);
+  const auto x_of = [&](int buffer, int part) { return Stack{ws + pl.x[buffer][part], d->rows, d->cols, pl.pitch, d->batch}; };
+  const Stack a_of{ws + pl.a, pl.small, pl.small, pl.small_pitch, d->batch}, b_of{ws + pl.b, pl.small, pl.small, pl.small_pitch, d->batch};
+
+  StartParams sp{};
+  sp.m = matrix;
+  sp.rows = d->rows;
+  sp.cols = d->cols;
+  sp.batch_stride = d->stride[0];
+  sp.row_stride = d->stride[1];
+  sp.pitch = pl.pitch;
+  sp.part = reinterpret_cast<double*>(ws + pl.part);
+  sp.parts = pl.parts;
+  sp.eps = d->eps;
+  sp.hi = reinterpret_cast<__half*>(ws + pl.x[0][0]);
+  sp.lo = reinterpret_cast<__half*>(ws + pl.x[0][1]);
+  const bool wide = d->cols % 8 == 0 && (d->rows == 1 || d->stride[1] % 8 == 0) && (d->batch == 1 || d->stride[0] % 8 == 0) &&
+                    reinterpret_cast<uintptr_t>(matrix) % 16 == 0;
+  if (d->dtype == NCA_BF16)
+    NCA_TRY((wide ? start<__nv_bfloat16, true>(sp, d->batch, s) : start<__nv_bfloat16, false>(sp, d->batch, s)));
+  else
+    NCA_TRY((wide ? start<__half, true>(sp, d->batch, s) : start<__half, false>(sp, d->batch, s)));
+
+  const double c0 = d->coefficients[0], c1 = d->coefficients[1], c2 = d->coefficients[2];
+  // |B| <= 4 |b| + 16 |c|: times the largest power of two, 2^10 at most, that leaves it below 2^15
+  double scale_b = kScaleA;
+  while (scale_b * (4 * std::fabs(c1) + 16 * std::fabs(c2)) > 32768.0) scale_b /= 2;
+  OrthoParams p{};
+  p.batch = (int)d->batch;
+  p.ctrl = ctrl;
+  p.timeout_ns = (unsigned long long)(timeout_ms > 0 ? timeout_ms : 10000) * 1000000ull;
+  p.out_bf16 = d->dtype == NCA_BF16;
+  for (int k = 0; k < d->steps; ++k) {
+    const Stack hi = x_of(k & 1, 0), lo = x_of(k & 1, 1);
+    const bool last = k + 1 == d->steps;
+    p.m = p.n = (int)pl.small;
+    p.symmetric = 1;
+    p.kb = (int)ceil_div(std::max(d->rows, d->cols), kBK);
+    p.terms = 0;
+    p.last = 0;
+    p.alpha = kScaleA / (kScaleX * kScaleX);
+    p.beta = 0.f;
+    if (!encode_places(&p.out[0], a_of)) return NCA_ERR_CUDA;
+    NCA_TRY((pl.tall ? product<true, true, STEP_POWER>(p, hi, hi, s) : product<false, false, STEP_POWER>(p, hi, hi, s)));
+
+    p.kb = (int)ceil_div(pl.small, kBK);
+    p.terms = 1;
+    p.alpha = (float)(c2 * scale_b / ((double)kScaleA * kScaleA));
+    p.beta = (float)(c1 * scale_b / kScaleA);
+    if (!encode_places(&p.src[0], a_of) || !encode_places(&p.out[0], b_of)) return NCA_ERR_CUDA;
+    NCA_TRY((product<false, false, STEP_POWER>(p, a_of, a_of, s)));
+
+    p.m = (int)d->rows;
+    p.n = (int)d->cols;
+    p.symmetric = 0;
+    p.terms = 2;
+    p.last = last;
+    p.alpha = (float)(1.0 / scale_b);
+    p.beta = (float)c0;
+    p.scale = 1.f / kScaleX;
+    p.c = static_cast<uint16_t*>(out);
+    p.ldc = d->cols;
+    p.plain_c = d->cols % 8 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0;
+    if (!encode_places(&p.src[0], hi) || !encode_places(&p.src[1], lo)) return NCA_ERR_CUDA;
+    if (!last) {
+      if (!encode_places(&p.out[0], x_of(~k & 1, 0)) || !encode_places(&p.out[1], x_of(~k & 1, 1))) return NCA_ERR_CUDA;
+    } else if (!p.plain_c && !encode_places(&p.out[0], Stack{out, d->rows, d->cols, d->cols, d->batch}, p.out_bf16)) {
+      return NCA_ERR_CUDA;
+    }
+    NCA_TRY((pl.tall ? product<false, false, STEP_UPDATE>(p, hi, b_of, s) : product<false, true, STEP_UPDATE>(p, b_of, hi, s)));
+  }
+  return NCA_OK;
+}
+
+}  // extern "C"

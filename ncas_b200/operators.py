@@ -92,6 +92,18 @@ def gated_scan(x, gate, state=None, *, dim=-2, reverse=False, mask=None):
     return _op("gated_scan")(x, gate, state, dim, reverse, mask)
 
 
+def orthogonalize(matrix, *, steps=5, coefficients=(3.4445, -4.775, 2.0315), eps=1e-7):
+    """matrix (..., rows, cols) with its singular values brought towards 1 by Newton-Schulz products: X = M / (|M|_F + eps),
+    then `steps` times X = a X + (b A + c A^2) X, A = X X^T, with coefficients (a, b, c).
+
+    bfloat16 or float16, any strides (adjacent columns are read in place, others copied); the result is contiguous and
+    of the same type.  Products are summed in fp32 over fp16 operands, X keeps 22 bits between the steps, and the
+    result is rounded once.  Coefficients that let a singular value grow beyond 2 are refused.  Not differentiable: for
+    the update of an optimiser.  The first call on a device makes its control words: it must precede a stream capture.
+    """
+    return _op("orthogonalize")(matrix, steps, coefficients, eps)
+
+
 def check(device="cuda") -> None:
     """Synchronises the current stream and raises NcaError when a kernel's bounded wait ran out since this
     thread's last call (at first: since it began to use the operators).

@@ -1,0 +1,151 @@
+"""orthogonalize on the GPU against the 64-bit oracle.
+
+The kernels round to fp16 in documented places (operands of the products; X to 22 bits) and sum in fp32.  The oracle
+can make the same roundings, everything else exact: its distance r from the exact result is what they cost.  The
+kernels' roundings fall on values that differ in the last place of fp32, so their errors are of the same size and
+otherwise independent: in the Frobenius norm, of n values, within a factor 1 + 6 / sqrt(n) of each other, and 4 for
+the smallest matrices here, whose few roundings do not average.  Sums of k <= 4096 products in fp32 add
+2^-24 sqrt(k) < 2^-18 of a norm, amplified like r, which is made of roundings of 2^-12: covered by the factor 4 too.
+The result adds half a step of its type in every value."""
+
+import pytest
+import torch
+
+import oracle.cell_operators as O
+from ncas_b200 import operators as ops
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+UNIT = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+TYPES = [torch.bfloat16, torch.float16]
+
+
+def matrix(shape, dtype, seed=0, scale=0.02):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype)
+
+
+def check(m, steps=5, put=lambda t: t.to(DEV), **kw):
+    got = ops.orthogonalize(put(m), steps=steps, **kw)
+    ops.check()
+    assert got.shape == m.shape and got.dtype == m.dtype and got.is_contiguous()
+    flat = lambda t: t.double().cpu().reshape(-1, *m.shape[-2:])  # noqa: E731
+    want, near = flat(O.orthogonalize(m, steps, **kw)), flat(O.orthogonalize(m, steps, rounded=True, **kw))
+    for g, w, r in zip(flat(got), want, near):
+        tol = 4 * (r - w).norm() + UNIT[m.dtype] * w.norm() + 2.0**-25 * w.numel() ** 0.5
+        assert (g - w).norm() <= tol, (float((g - w).norm()), float(tol), float((r - w).norm()))
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [
+    (1, 1), (1, 9), (9, 1), (8, 8), (5, 70), (64, 64), (64, 256), (256, 64), (256, 256), (129, 130), (100, 1000),
+    (1000, 100), (257, 600), (513, 300), (385, 385), (640, 1288), (1001, 730)])
+def test_against_the_oracle(rows, cols, dtype):
+    check(matrix((rows, cols), dtype, seed=rows))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(3, 40, 24), (2, 2, 130, 300), (5, 257, 129), (40, 64, 72), (3, 300, 300)])
+def test_stacks(shape, dtype):
+    m = matrix(shape, dtype, seed=1)
+    got = check(m)
+    alone = ops.orthogonalize(m.reshape(-1, *shape[-2:])[-1].to(DEV))
+    # a matrix of a stack does not see the others: at most the tiles' shapes differ, and with them nothing in a sum's order
+    assert torch.equal(alone, got.reshape(-1, *shape[-2:])[-1])
+
+
+def test_a_bad_matrix_stays_alone():
+    m = matrix((4, 100, 260), torch.bfloat16, seed=2).to(DEV)
+    want = ops.orthogonalize(m)
+    for bad in (float("nan"), float("inf")):
+        b = m.clone()
+        b[1, 50, 3] = bad
+        got = ops.orthogonalize(b)
+        assert torch.equal(got[[0, 2, 3]], want[[0, 2, 3]]) and got[1].isnan().any()
+    z = m.clone()
+    z[2] = 0
+    got = ops.orthogonalize(z)
+    assert (got[2] == 0).all() and torch.equal(got[[0, 1, 3]], want[[0, 1, 3]])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rank", [1, 3])
+def test_low_rank(dtype, rank):
+    # what a is left in the small directions is amplified by a at every step: X must not be rounded to 11 bits
+    g = torch.Generator().manual_seed(3)
+    u, v = torch.randint(-3, 4, (300, rank), generator=g), torch.randint(-3, 4, (rank, 520), generator=g)
+    m = (u @ v).to(dtype)  # exact in the type: rank `rank`
+    got = check(m)
+    s = torch.linalg.svdvals(got.double().cpu())
+    # five steps bring the large ones to 0.68 to 1.21; nothing but the result's rounding may appear in the others
+    assert (s[:rank] > 0.6).all() and (s[:rank] < 1.25).all()
+    assert s[rank] <= UNIT[dtype] * 1.25 * rank**0.5 + 4 * float((O.orthogonalize(m, rounded=True) - O.orthogonalize(m)).norm())
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-9, 1e30, 3e37])
+def test_norms_at_the_ends_of_the_range(scale):
+    m = matrix((70, 90), torch.bfloat16, seed=4, scale=scale)
+    check(m, eps=1e-7 if scale > 1 else 0.0)
+    if scale < 1e-8:  # the norm counts for little beside eps
+        check(m.clone(), eps=1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_alignment(dtype):
+    m = matrix((3, 80, 136), dtype, seed=5)
+    for put in (lambda t: t.to(DEV).transpose(1, 2).contiguous().transpose(1, 2),  # copied
+                lambda t: torch.cat([t, t], 2).to(DEV)[..., :136],
+                lambda t: torch.cat([t[..., :1], t], 2).to(DEV)[..., 1:],  # odd starts and rows
+                lambda t: t.to(DEV).transpose(0, 1).contiguous().transpose(0, 1)):
+        check(m, put=put)
+    check(m[:1].expand(3, 80, 136))
+
+
+def test_steps_and_coefficients():
+    m = matrix((90, 200), torch.float16, seed=6)
+    check(m, steps=1)
+    check(m, steps=12)
+    check(m, steps=8, coefficients=(1.5, -0.5, 0.0))
+    check(m, steps=3, coefficients=(1.875, -1.25, 0.375))
+    check(m, steps=2, coefficients=(1.0, 0.0, 0.0), eps=0.0)
+
+
+@pytest.mark.parametrize("shape", [(0, 4), (4, 0), (0, 4, 4), (3, 0, 5)])
+def test_sizes_of_zero(shape):
+    assert ops.orthogonalize(torch.zeros(shape, device=DEV, dtype=torch.bfloat16)).shape == shape
+
+
+def test_repeats_bit_for_bit_on_other_streams_and_in_a_graph():
+    m = matrix((600, 1000), torch.bfloat16, seed=7).to(DEV)
+    want = ops.orthogonalize(m)
+    torch.cuda.synchronize()
+    got, streams = [], [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(ops.orthogonalize(m))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.orthogonalize(m)
+    m.neg_()
+    graph.replay()
+    assert torch.equal(y, -want)
+    ops.check()
+
+
+def test_refusals():
+    m = torch.zeros((4, 8), device=DEV, dtype=torch.bfloat16)
+    cases = [(ValueError, "CUDA", m.cpu(), {}), (TypeError, "matrix", m.float(), {}), (ValueError, "matrix", m[0], {}),
+             (ValueError, "steps", m, dict(steps=0)), (ValueError, "steps", m, dict(steps=1001)),
+             (ValueError, "three", m, dict(coefficients=(1.0, 2.0))),
+             (ValueError, "finite", m, dict(coefficients=(float("nan"), 0.0, 0.0))),
+             (ValueError, "grow", m, dict(coefficients=(3.0, 0.0, 0.0))),
+             (ValueError, "grow", m, dict(coefficients=(3.4445, -4.775, 3.0))),
+             (ValueError, "eps", m, dict(eps=-1.0)), (ValueError, "eps", m, dict(eps=float("inf"))),
+             (ValueError, "gradient", m.clone().requires_grad_(), {})]
+    for kind, match, t, kw in cases:
+        with pytest.raises(kind, match=match):
+            ops.orthogonalize(t, **kw)
