@@ -477,6 +477,25 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
                                void* workspace, size_t workspace_bytes, int32_t* ctrl,
                                int32_t timeout_ms, void* stream);
 
+/* Classes drawn from rows of logits.  w_i = exp((z_i - max z) / temperature); classes in the order of z, largest first,
+ * equal ones by index.  Kept are the first top_k (0: all); of those, the ones before which less than top_p of their mass
+ * lies; of those, the ones with w_i >= min_p.  tokens[r][k] is the first kept class, by index, at which the sum of the
+ * kept w exceeds uniforms[r][k] times the whole (the last kept one where there is none), probs[r][k] (may be NULL) its share
+ * of the kept mass.  NaN counts as -inf; +inf beats every finite logit; a row of -inf alone gives -1 and 0.  temperature 0: the first
+ * of the largest. */
+typedef struct NcaSampleDesc {
+  int64_t rows, classes, draws;
+  int64_t logits_stride;        /* of rows; classes are adjacent */
+  int32_t dtype;                /* NcaDtype of the logits */
+  int32_t reserved;
+  int64_t top_k;
+  double temperature;           /* 0, or 1e-30 to 1e30 */
+  double top_p, min_p;          /* (0, 1], [0, 1] */
+} NcaSampleDesc;
+
+int32_t nca_b200_sample(const NcaSampleDesc* d, const void* logits, const float* uniforms,
+                        int64_t* tokens, float* probs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

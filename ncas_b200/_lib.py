@@ -200,6 +200,21 @@ class NcaOrthoDesc(C.Structure):
     ]
 
 
+class NcaSampleDesc(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64),
+        ("classes", C.c_int64),
+        ("draws", C.c_int64),
+        ("logits_stride", C.c_int64),
+        ("dtype", C.c_int32),
+        ("reserved", C.c_int32),
+        ("top_k", C.c_int64),
+        ("temperature", C.c_double),
+        ("top_p", C.c_double),
+        ("min_p", C.c_double),
+    ]
+
+
 # name -> (restype, argtypes); must match include/nca_b200.h
 _P = C.c_void_p
 _I = C.c_int32
@@ -272,6 +287,7 @@ SIGNATURES = {
     "nca_b200_gated_scan_saved_bytes": (_I, [C.POINTER(NcaScanDesc), C.POINTER(C.c_size_t)]),
     "nca_b200_gated_scan_workspace": (_I, [C.POINTER(NcaScanDesc), _I, C.POINTER(C.c_size_t)]),
     "nca_b200_gated_scan": (_I, [C.POINTER(NcaScanDesc), *[_P] * 8, C.c_size_t, _P]),
+    "nca_b200_sample": (_I, [C.POINTER(NcaSampleDesc), *[_P] * 5]),
     "nca_b200_orthogonalize_workspace": (_I, [C.POINTER(NcaOrthoDesc), C.POINTER(C.c_size_t)]),
     "nca_b200_orthogonalize": (_I, [C.POINTER(NcaOrthoDesc), _P, _P, _P, C.c_size_t, _P, _I, _P]),
     "nca_b200_gated_scan_backward": (_I, [C.POINTER(NcaScanDesc), *[_P] * 11, C.c_size_t, _P]),

@@ -20,7 +20,8 @@ SOURCES = [CSRC / "api.cu", CSRC / "steps_64_256.cu", CSRC / "steps_32_128.cu",
            CSRC / "steps_16_128.cu", CSRC / "steps_32_256.cu",
            CSRC / "norm.cu", CSRC / "norm_held_forward.cu", CSRC / "norm_held_backward.cu",
            CSRC / "gated.cu", CSRC / "distill.cu",
-           CSRC / "scan.cu", CSRC / "orthogonalize.cu"]  # the cell-training operators
+           CSRC / "scan.cu", CSRC / "orthogonalize.cu",
+           CSRC / "sample.cu"]  # the cell-training operators
 HEADERS = [CSRC / "ptx.cuh", CSRC / "step_kernel.cuh", CSRC / "launch.cuh", CSRC / "cell_ops.cuh",
            CSRC / "gemm.cuh", CSRC / "gemm_rows.cuh", CSRC / "norm.cuh",
            CSRC / "norm_held.cuh",

@@ -820,6 +820,48 @@ Tensor orthogonalize(const Tensor& matrix, int64_t steps, at::ArrayRef<double> c
   return out;
 }
 
+// -------------------------------------------------------------------------------- sampled classes
+std::tuple<Tensor, Tensor> sample(const Tensor& logits, const Tensor& uniforms, double temperature, int64_t top_k,
+                                  double top_p, double min_p) {
+  constexpr const char* op = "sample";
+  on_cuda(logits, op, "logits");
+  no_tangent(logits, op, "logits");
+  NcaSampleDesc d{};
+  d.dtype = dtype_of(logits, op, "logits");
+  TORCH_CHECK_VALUE(!logits.requires_grad() || !at::GradMode::is_enabled(), op, ": logits gets no gradient: detach it");
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0 && logits.size(-1) <= 1 << 30, op,
+                    ": logits must be (..., classes) with 1 to 2^30 classes, not ", logits.sizes());
+  same_device(uniforms, logits, op, "uniforms");
+  TORCH_CHECK_TYPE(uniforms.scalar_type() == at::kFloat, op, ": uniforms must be float32, not ", uniforms.scalar_type());
+  const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+  const bool one = uniforms.dim() == logits.dim() - 1;
+  TORCH_CHECK_VALUE((one || uniforms.dim() == logits.dim()) && uniforms.sizes().slice(0, lead.size()) == lead, op,
+                    ": uniforms must be ", lead, " or these with a number of draws, not ", uniforms.sizes());
+  TORCH_CHECK_VALUE(temperature == 0 || (temperature >= 1e-30 && temperature <= 1e30), op,
+                    ": temperature must be 0 or lie between 1e-30 and 1e30, not ", temperature);
+  TORCH_CHECK_VALUE(top_k >= 0, op, ": top_k must not be negative, not ", top_k);
+  TORCH_CHECK_VALUE(top_p > 0 && top_p <= 1, op, ": top_p must lie above 0 and not above 1, not ", top_p);
+  TORCH_CHECK_VALUE(min_p >= 0 && min_p <= 1, op, ": min_p must lie between 0 and 1, not ", min_p);
+  d.rows = 1;
+  for (const int64_t n : lead) d.rows *= n;
+  d.classes = logits.size(-1);
+  d.draws = one ? 1 : uniforms.size(-1);
+  d.top_k = top_k;
+  d.temperature = temperature;
+  d.top_p = top_p;
+  d.min_p = min_p;
+  const Tensor rows = d.rows ? rows_of(logits, d.classes) : logits;
+  d.logits_stride = d.rows > 1 ? rows.stride(0) : d.classes;
+  const Tensor u = uniforms.contiguous();
+  const c10::cuda::CUDAGuard guard(logits.device());
+  Tensor tokens = at::empty(uniforms.sizes(), logits.options().dtype(at::kLong));
+  Tensor probs = at::empty(uniforms.sizes(), logits.options().dtype(at::kFloat));
+  check(nca_b200_sample(&d, ptr(rows), static_cast<const float*>(ptr(u)), static_cast<int64_t*>(mptr(tokens)),
+                        static_cast<float*>(mptr(probs)), stream_of(logits)),
+        "nca_b200_sample");
+  return {tokens, probs};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(nca_b200, m) {
@@ -837,5 +879,8 @@ TORCH_LIBRARY_FRAGMENT(nca_b200, m) {
   m.def("gated_scan(Tensor x, Tensor gate, Tensor? state, int dim, bool reverse, Tensor? mask) -> (Tensor, Tensor)",
         &gated_scan);
   m.def("orthogonalize(Tensor matrix, int steps, float[] coefficients, float eps) -> Tensor", &orthogonalize);
+  m.def("sample(Tensor logits, Tensor uniforms, float temperature, int top_k, float top_p, float min_p) -> "
+        "(Tensor, Tensor)",
+        &sample);
   m.def("operators_status(Tensor like) -> int[]", &operators_status);
 }

@@ -104,6 +104,20 @@ def orthogonalize(matrix, *, steps=5, coefficients=(3.4445, -4.775, 2.0315), eps
     return _op("orthogonalize")(matrix, steps, coefficients, eps)
 
 
+def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(classes, probabilities) drawn from each row of logits (..., classes) with the given uniform numbers of [0, 1):
+    uniforms (..., draws), or (...) for one draw; both results have its shape (int64, float32).
+
+    Classes in the order of their logits, the lower index first among equals.  Kept are the first top_k (0: all); of
+    those, the ones before which less than top_p of their mass exp(logit / temperature) lies; of those, the ones of at
+    least min_p times the largest one's mass.  A draw is the first kept class, by index, at which the sum of the kept
+    masses exceeds the uniform number times the whole; its probability is its share of it.  Weights and sums are
+    in 64 bits.  logits: float32, bfloat16 or float16, any strides; NaN counts as -inf; +inf beats every finite logit; a row
+    that is -inf alone gives -1 and 0.  temperature 0: the first of the largest.  Not differentiable.
+    """
+    return _op("sample")(logits, uniforms, temperature, top_k, top_p, min_p)
+
+
 def check(device="cuda") -> None:
     """Synchronises the current stream and raises NcaError when a kernel's bounded wait ran out since this
     thread's last call (at first: since it began to use the operators).

@@ -151,3 +151,40 @@ def orthogonalize(m, steps=5, coefficients=(3.4445, -4.775, 2.0315), eps=1e-7, r
             x = a * x + q @ hi
         out.append(x.T if m.shape[-2] > m.shape[-1] else x)
     return torch.stack(out).reshape(m.shape)
+
+
+def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(classes, probabilities, nearest) of rows x classes and rows x draws: `nearest` is the least distance of a
+    draw, or of the cut by top_p, from a border, as a share of the mass.  A loop over rows."""
+    rows, classes = logits.shape
+    tokens = torch.full(uniforms.shape, -1, dtype=torch.int64)
+    probs = torch.zeros(uniforms.shape, dtype=torch.float64)
+    nearest = 1.0
+    for r in range(rows):
+        z = logits[r].double()
+        z = torch.where(z.isnan(), -math.inf, z)
+        top = z.max()
+        if top == -math.inf:
+            continue
+        w = torch.where(z == top, 1.0, torch.exp((z - top) / (temperature or 1.0)))
+        order = torch.argsort(-z, stable=True)
+        kept = order[z[order] > -math.inf]
+        if temperature == 0 or top_k:
+            kept = kept[: 1 if temperature == 0 else top_k]
+        if top_p < 1:
+            ends = w[kept].cumsum(0)
+            before = ends - w[kept]
+            target = top_p * ends[-1]
+            nearest = min(nearest, float((before - target).abs().min() / ends[-1]))
+            kept = kept[before < target]
+        kept = kept[w[kept] >= min_p].sort().values
+        c = w[kept].cumsum(0)
+        for k, u in enumerate(uniforms[r].double().tolist()):
+            t = (u if u > 0 else 0.0) * c[-1]  # NaN: the first
+            at = min(int((c <= t).sum()), len(kept) - 1)
+            if 0 < u < 1:
+                nearest = min(nearest, float((c - t).abs().min() / c[-1]))
+            while w[kept[at]] == 0:  # u = 1: the last that can be drawn
+                at -= 1
+            tokens[r, k], probs[r, k] = kept[at], w[kept[at]] / c[-1]
+    return tokens, probs, nearest
