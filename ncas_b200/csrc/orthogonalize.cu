@@ -9,7 +9,9 @@
 // as hi + lo, two fp16 values of 22 bits together: a X amplifies what is left in the small singular
 // directions by a at every step, and with X in 11 bits that would be rounding noise (6 % of the result
 // for a matrix of rank 1).  The products read hi alone: their errors appear only beside large singular values,
-// which nothing amplifies.
+// which nothing amplifies, and later steps mend most of what earlier ones leave.  A bf16 result has 1.1 to 1.25 times the
+// error of its rounding alone; a fp16 result would have 8 times, so there the operands of the last three steps' products
+// have 22 bits, hi hi + hi lo + lo hi (2.2 times the operations, and an error of 1.05 times the rounding's).
 //
 // A and A^2 are symmetric: tiles above the diagonal are computed, and stored twice.
 //
@@ -43,16 +45,19 @@ constexpr int kMaxDevices = 64;
 constexpr float kScaleX = 4096.f, kScaleA = 1024.f;
 
 enum OrthoStep {
-  STEP_POWER = 0,  // out = alpha D + beta src: A, and B
-  STEP_UPDATE = 1  // X: alpha D + beta (hi + lo), stored as hi + lo, or as the result
+  STEP_POWER = 0,  // A, and B
+  STEP_UPDATE = 1  // X, or the result
 };
 
+// alpha D + beta (src[0] + src[1]), stored as a value or as hi + lo.
 struct OrthoParams {
-  CUtensorMap a, b;
+  CUtensorMap a[2], b[2];  // hi and, where there are three passes, lo
   CUtensorMap src[2];  // boxes of 32 rows of 64 bytes: what the epilogue reads
   CUtensorMap out[2];
   int m, n;  // of D
   int m_tiles, n_tiles, batch, kb;
+  int passes;  // over the k axis: 1, or 3 (hi hi, hi lo, lo hi)
+  int pair;    // the output as hi + lo
   int symmetric;
   int terms;  // matrices in src
   int last;   // STEP_UPDATE: out[0] is the result
@@ -183,7 +188,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
       for (int t = first; t < tiles && ok; t += step) {
         const OrthoTile tl = tile_at<kBM * CG, BN>(p, per, t);
         const int am = tl.m0 + (int)rank * kBM, bn = tl.n0 + (int)rank * S::kBNc;
-        for (int kb = 0; kb < p.kb; ++kb) {
+        for (int kb = 0, pass = 0; pass < p.passes; kb + 1 < p.kb ? ++kb : (kb = 0, ++pass)) {
+          const CUtensorMap *ma = &p.a[pass == 2], *mb = &p.b[pass == 1];
           if (!mbar_wait(&empty[s], ph ^ 1, fs, 111)) {
             ok = false;
             break;
@@ -194,15 +200,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
           const int k0 = kb * kBK;
           if constexpr (A_MN) {
 #pragma unroll
-            for (int i = 0; i < kBM / 64; ++i) load_tile<CG>(sa + i * 8192, &p.a, bar, am + 64 * i, k0, tl.z);
+            for (int i = 0; i < kBM / 64; ++i) load_tile<CG>(sa + i * 8192, ma, bar, am + 64 * i, k0, tl.z);
           } else {
-            load_tile<CG>(sa, &p.a, bar, k0, am, tl.z);
+            load_tile<CG>(sa, ma, bar, k0, am, tl.z);
           }
           if constexpr (B_MN) {
 #pragma unroll
-            for (int i = 0; i < S::kBNc / 64; ++i) load_tile<CG>(sb + i * 8192, &p.b, bar, bn + 64 * i, k0, tl.z);
+            for (int i = 0; i < S::kBNc / 64; ++i) load_tile<CG>(sb + i * 8192, mb, bar, bn + 64 * i, k0, tl.z);
           } else {
-            load_tile<CG>(sb, &p.b, bar, k0, bn, tl.z);
+            load_tile<CG>(sb, mb, bar, k0, bn, tl.z);
           }
           ++issued;
           if (++s == S::kStages) {
@@ -232,7 +238,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
         }
         tc_fence_after();
         const uint32_t d = tmem + buf * BN;
-        for (int kb = 0; kb < p.kb; ++kb) {
+        for (int kb = 0; kb < p.kb * p.passes; ++kb) {
           if (!mbar_wait(&full[s], ph, fs, 113)) {
             ok = false;
             break;
@@ -295,13 +301,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
           pending = false;
           uint4 k0[4], k1[4];
           take_row(place + kPlace, lane, k0);
-          if (STEP == STEP_UPDATE) take_row(place + 2 * kPlace, lane, k1);
+          if (p.terms == 2) take_row(place + 2 * kPlace, lane, k1);
           // every lane's reads come before the copy that overwrites them
           fence_async_proxy();
           __syncwarp();
           if (c + 64 < cols) ask(c + 64);
           unpack_half(k0, f);
-          if (STEP == STEP_UPDATE) {
+          if (p.terms == 2) {
             float lo[32];
             unpack_half(k1, lo);
 #pragma unroll
@@ -334,22 +340,31 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
           __syncwarp();
           continue;
         }
-        if (STEP == STEP_UPDATE && !p.last) {  // what hi leaves
+        if (mirror) put_column(place + 3 * kPlace, lane, f);
+        const auto store = [&](const CUtensorMap* out, uint32_t from) {
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(out, from, col, row0, tl.z);
+            if (mirror) tma_store_3d(out, place + 3 * kPlace, row0, col, tl.z);
+            bulk_commit();
+          }
+        };
+        store(&p.out[0], place);
+        if (p.pair) {  // what hi leaves
           float hi[32];
           unpack_half(v, hi);
 #pragma unroll
           for (int i = 0; i < 32; ++i) f[i] -= hi[i];
           pack_row<__half>(f, v);
-          put_row(place + 3 * kPlace, lane, v);
-        }
-        if (mirror) put_column(place + 3 * kPlace, lane, f);
-        fence_async_proxy();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_3d(&p.out[0], place, col, row0, tl.z);
-          if (mirror) tma_store_3d(&p.out[0], place + 3 * kPlace, row0, col, tl.z);
-          if (STEP == STEP_UPDATE && !p.last) tma_store_3d(&p.out[1], place + 3 * kPlace, col, row0, tl.z);
-          bulk_commit();
+          const uint32_t second = mirror ? place : place + 3 * kPlace;
+          if (mirror) {  // both places are in use
+            if (lane == 0) bulk_wait_read<0>();
+            __syncwarp();
+            put_column(place + 3 * kPlace, lane, f);
+          }
+          put_row(second, lane, v);
+          store(&p.out[1], second);
         }
       }
       if (!ok) break;
@@ -505,7 +520,7 @@ bool encode_places(CUtensorMap* map, const Stack& m, bool bf16 = false) {
 }
 
 template <int CG, int BN, bool A_MN, bool B_MN, int STEP>
-int32_t launch(OrthoParams& p, const Stack& a, const Stack& b, cudaStream_t s) {
+int32_t launch(OrthoParams& p, const Stack (&a)[2], const Stack (&b)[2], cudaStream_t s) {
   using S = OrthoShape<CG, BN>;
   auto* kernel = ortho_kernel<CG, BN, A_MN, B_MN, STEP>;
   static std::atomic<uint64_t> ready{0};  // a bit for each device whose shared-memory limit is set
@@ -516,7 +531,8 @@ int32_t launch(OrthoParams& p, const Stack& a, const Stack& b, cudaStream_t s) {
       return launch_status() == NCA_OK ? NCA_ERR_CUDA : NCA_ERR_DEVICE;
     ready.fetch_or(1ull << dev, std::memory_order_release);
   }
-  if (!encode_operand(&p.a, a, A_MN, kBM) || !encode_operand(&p.b, b, B_MN, S::kBNc)) return NCA_ERR_CUDA;
+  for (int i = 0; i < (p.passes == 1 ? 1 : 2); ++i)
+    if (!encode_operand(&p.a[i], a[i], A_MN, kBM) || !encode_operand(&p.b[i], b[i], B_MN, S::kBNc)) return NCA_ERR_CUDA;
   p.m_tiles = (int)ceil_div(p.m, kBM * CG);
   // symmetric: whole blocks on the diagonal, the last of whose tiles may be empty
   p.n_tiles = p.symmetric ? p.m_tiles * (kBM * CG / BN) : (int)ceil_div(p.n, BN);
@@ -530,7 +546,7 @@ int32_t launch(OrthoParams& p, const Stack& a, const Stack& b, cudaStream_t s) {
 // The tile of a product by the cost of its waves, as the gated block's: a k block costs a 256 x 256 tile of a pair of
 // multiprocessors 0.28 us, a 256 x 128 tile 0.24 and a 128 x 128 tile of one 0.25, a wave 3 us besides.
 template <bool A_MN, bool B_MN, int STEP>
-int32_t product(OrthoParams& p, const Stack& a, const Stack& b, cudaStream_t s) {
+int32_t product(OrthoParams& p, const Stack (&a)[2], const Stack (&b)[2], cudaStream_t s) {
   static const struct {
     int cg, bn;
     double us;
@@ -541,7 +557,7 @@ int32_t product(OrthoParams& p, const Stack& a, const Stack& b, cudaStream_t s) 
     const long long tm = 128 * kinds[i].cg, mt = ceil_div(p.m, tm);
     long long tiles = mt * ceil_div(p.n, kinds[i].bn);
     if (p.symmetric) tiles = (tm / kinds[i].bn) * (mt * (mt + 1) / 2);
-    const double us = (double)ceil_div(tiles * p.batch, sm_count() / kinds[i].cg) * (p.kb * kinds[i].us + 3.0);
+    const double us = (double)ceil_div(tiles * p.batch, sm_count() / kinds[i].cg) * (p.kb * p.passes * kinds[i].us + 3.0);
     if (us < least) {
       least = us;
       best = i;
@@ -580,7 +596,7 @@ int32_t check_desc(const NcaOrthoDesc* d) {
 struct Plan {
   long long small, pitch, small_pitch;
   bool tall;
-  size_t x[2][2], a, b, part, total;  // x[buffer][hi, lo]
+  size_t x[2][2], a[2], b[2], part, total;  // x[buffer][hi, lo]; a, b: hi, lo
   int parts;
 };
 Plan plan_of(const NcaOrthoDesc& d) {
@@ -596,10 +612,11 @@ Plan plan_of(const NcaOrthoDesc& d) {
       part = at;
       at += x;
     }
-  p.a = at;
-  at += a;
-  p.b = at;
-  at += a;
+  for (int i = 0; i < 2; ++i) {
+    p.a[i] = at;
+    p.b[i] = at + a;
+    if (i == 0 || d.dtype == NCA_F16) at += 2 * a;
+  }
   p.part = at;
   p.parts = (int)std::max<long long>(1, std::min<long long>(ceil_div(d.rows * d.cols, 4096), ceil_div(592, d.batch ? d.batch : 1)));
   at += align256((size_t)d.batch * p.parts * sizeof(double));
@@ -636,7 +653,8 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255);
   const auto x_of = [&](int buffer, int part) { return Stack{ws + pl.x[buffer][part], d->rows, d->cols, pl.pitch, d->batch}; };
-  const Stack a_of{ws + pl.a, pl.small, pl.small, pl.small_pitch, d->batch}, b_of{ws + pl.b, pl.small, pl.small, pl.small_pitch, d->batch};
+  const auto square = [&](size_t at) { return Stack{ws + at, pl.small, pl.small, pl.small_pitch, d->batch}; };
+  const Stack a_of[2] = {square(pl.a[0]), square(pl.a[1])}, b_of[2] = {square(pl.b[0]), square(pl.b[1])};
 
   StartParams sp{};
   sp.m = matrix;
@@ -667,8 +685,10 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
   p.timeout_ns = (unsigned long long)(timeout_ms > 0 ? timeout_ms : 10000) * 1000000ull;
   p.out_bf16 = d->dtype == NCA_BF16;
   for (int k = 0; k < d->steps; ++k) {
-    const Stack hi = x_of(k & 1, 0), lo = x_of(k & 1, 1);
-    const bool last = k + 1 == d->steps;
+    const Stack x[2] = {x_of(k & 1, 0), x_of(k & 1, 1)};
+    const bool last = k + 1 == d->steps, precise = d->dtype == NCA_F16 && k + 3 >= d->steps;
+    p.passes = precise ? 3 : 1;
+    p.pair = precise;
     p.m = p.n = (int)pl.small;
     p.symmetric = 1;
     p.kb = (int)ceil_div(std::max(d->rows, d->cols), kBK);
@@ -676,20 +696,23 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
     p.last = 0;
     p.alpha = kScaleA / (kScaleX * kScaleX);
     p.beta = 0.f;
-    if (!encode_places(&p.out[0], a_of)) return NCA_ERR_CUDA;
-    NCA_TRY((pl.tall ? product<true, true, STEP_POWER>(p, hi, hi, s) : product<false, false, STEP_POWER>(p, hi, hi, s)));
+    for (int i = 0; i <= p.pair; ++i)
+      if (!encode_places(&p.out[i], a_of[i])) return NCA_ERR_CUDA;
+    NCA_TRY((pl.tall ? product<true, true, STEP_POWER>(p, x, x, s) : product<false, false, STEP_POWER>(p, x, x, s)));
 
     p.kb = (int)ceil_div(pl.small, kBK);
-    p.terms = 1;
+    p.terms = 1 + p.pair;
     p.alpha = (float)(c2 * scale_b / ((double)kScaleA * kScaleA));
     p.beta = (float)(c1 * scale_b / kScaleA);
-    if (!encode_places(&p.src[0], a_of) || !encode_places(&p.out[0], b_of)) return NCA_ERR_CUDA;
+    for (int i = 0; i <= p.pair; ++i)
+      if (!encode_places(&p.src[i], a_of[i]) || !encode_places(&p.out[i], b_of[i])) return NCA_ERR_CUDA;
     NCA_TRY((product<false, false, STEP_POWER>(p, a_of, a_of, s)));
 
     p.m = (int)d->rows;
     p.n = (int)d->cols;
     p.symmetric = 0;
     p.terms = 2;
+    p.pair = !last;
     p.last = last;
     p.alpha = (float)(1.0 / scale_b);
     p.beta = (float)c0;
@@ -697,13 +720,13 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
     p.c = static_cast<uint16_t*>(out);
     p.ldc = d->cols;
     p.plain_c = d->cols % 8 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0;
-    if (!encode_places(&p.src[0], hi) || !encode_places(&p.src[1], lo)) return NCA_ERR_CUDA;
+    if (!encode_places(&p.src[0], x[0]) || !encode_places(&p.src[1], x[1])) return NCA_ERR_CUDA;
     if (!last) {
       if (!encode_places(&p.out[0], x_of(~k & 1, 0)) || !encode_places(&p.out[1], x_of(~k & 1, 1))) return NCA_ERR_CUDA;
     } else if (!p.plain_c && !encode_places(&p.out[0], Stack{out, d->rows, d->cols, d->cols, d->batch}, p.out_bf16)) {
       return NCA_ERR_CUDA;
     }
-    NCA_TRY((pl.tall ? product<false, false, STEP_UPDATE>(p, hi, b_of, s) : product<false, true, STEP_UPDATE>(p, b_of, hi, s)));
+    NCA_TRY((pl.tall ? product<false, false, STEP_UPDATE>(p, x, b_of, s) : product<false, true, STEP_UPDATE>(p, b_of, x, s)));
   }
   return NCA_OK;
 }

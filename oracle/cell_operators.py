@@ -135,20 +135,21 @@ def gated_scan(x, gate, state=None, dim=-2, reverse=False, mask=None, dy=None, d
 
 def orthogonalize(m, steps=5, coefficients=(3.4445, -4.775, 2.0315), eps=1e-7, rounded=False):
     """Newton-Schulz steps of a stack of matrices.  rounded: with the roundings to fp16 that the library's
-    kernels document (operands X 2^12, A 2^10, B 2^10; X itself as two fp16 values), everything else exact."""
+    kernels document (operands X 2^12, A 2^10, B 2^10; X itself, and of fp16 matrices the operands of the last three
+    steps, as two fp16 values), everything else exact."""
     a, b, c = coefficients
-    half = lambda t, s: (t * s).half().double() / s if rounded else t  # noqa: E731
+    once = lambda t, s: (t * s).half().double() / s if rounded else t  # noqa: E731
+    twice = lambda t, s: once(t, s) + once(t - once(t, s), s) if rounded else t  # noqa: E731
     out = []
     for x in m.double().reshape(-1, *m.shape[-2:]):
         x = x / (x.square().sum().sqrt() + eps)
         if x.shape[0] > x.shape[1]:
             x = x.T
         for k in range(steps):
-            hi = half(x, 4096.0)
-            x = hi + half(x - hi, 4096.0) if rounded else x
-            p = half(hi @ hi.T, 1024.0)
-            q = half(b * p + c * (p @ p), 1024.0)
-            x = a * x + q @ hi
+            operand = twice if m.dtype == torch.float16 and k + 3 >= steps else once
+            y, x = operand(x, 4096.0), twice(x, 4096.0)
+            p = operand(y @ y.T, 1024.0)
+            x = a * x + operand(b * p + c * (p @ p), 1024.0) @ y
         out.append(x.T if m.shape[-2] > m.shape[-1] else x)
     return torch.stack(out).reshape(m.shape)
 
