@@ -8,13 +8,18 @@
 // The answers are whole numbers, and a row of 131072 classes has a border every 1e-5 of its mass: weights are computed in
 // 64 bits, so that an answer other than the exact one takes a u within about 1e-13 of a border.  Sums are in fixed
 // point: they do not depend on an order, and a class of no mass is never drawn.  The exponential is table-driven
-// (Tang, ACM TOMS 15, 1989): 2^(j / 64) from a table, e^r of |r| < 0.0055 by four terms, 9 operations in 64 bits.
+// (Tang, ACM TOMS 15, 1989): 2^(j / 256) from a table, e^r of |r| < 0.00136 by three terms, 10 operations in 64 bits with
+// the conversion to fixed point.
 //
-// Up to 32 classes a row is a group of lanes, a class a lane, and ranks are counted.  Longer rows are a block's: the kept
-// set is always "above a threshold (z, index)".  A small top_k: the least of k groups' maxima bounds the k-th largest
-// from below, the few entries above it are listed and sorted.  Else histograms over the ordered bits of z (counts, masses)
-// until the entries of the bin with the border can be listed.
-// Segments of 256 entries, a warp each, then sum the kept weights, and a draw looks through one segment.
+// Up to 32 classes a row is a group of lanes, a class a lane, and ranks are counted.  Longer rows are a block's.  All three
+// cuts keep a prefix of the order, so the kept set is always "from a place (z, index) on".
+//   min_p: the least z of enough weight, by search.
+//   a small top_k: the least of k groups' maxima bounds the k-th largest from below; the few entries above it are listed
+//     and sorted, and everything else happens in the list (as for all rows that fit it).
+//   top_p alone: a histogram of counts over (top - z) / T bounds the mass before every bin within 0.3 %; one pass then
+//     computes all weights, adds up those surely kept by segment and lists those about the border, which decide.
+//   else: histograms over the ordered bits of z until the entries of the bin with the border can be listed.
+// Segments of entries, a warp each, hold the sums of the kept weights; a draw looks through one segment.
 #include "cell_ops.cuh"
 
 #include <algorithm>
@@ -115,7 +120,10 @@ __global__ void __launch_bounds__(256) sample_few_kernel(const __grid_constant__
 }
 
 // ------------------------------------------------------------------------------------ longer rows
-constexpr int kBins = 2048;
+constexpr int kBins = 2048;       // of the ordered bits
+constexpr int kMassBins = 8192;   // of (top - z) / T
+constexpr float kPerBin = 200.f;  // the last holds all beyond 40.9, whose weights are below 2^-58
+constexpr int kSubBins = 256;
 constexpr int kMostSegments = 1024;
 
 // Floats in their order as whole numbers.
@@ -127,19 +135,32 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 // Its place in the order: larger first, then the lower index.
 __device__ __forceinline__ uint64_t place_of(uint32_t key, int i) { return (uint64_t)key << 32 | (0xffffffffu - (uint32_t)i); }
 __device__ __forceinline__ int index_of(uint64_t place) { return (int)(0xffffffffu - (uint32_t)place); }
+__device__ __forceinline__ float value_of(uint64_t place) { return of_key((uint32_t)(place >> 32)); }
+constexpr uint64_t kPossible = 0x00800000ull << 32;  // the places above -inf
 
+// Blocks of 128 threads serve rows that the list holds whole.
 template <int THREADS>
 struct RowShared {
-  static constexpr int kList = THREADS >= 512 ? 2048 : 1024;
-  double table[64];
-  uint64_t sums[kMostSegments];
+  static constexpr bool kLong = THREADS > 128;
+  static constexpr int kList = kLong ? 2048 : 1024;      // entries with their masses
+  static constexpr int kRegion = kLong ? 4096 : 1024;    // entries alone
+  static constexpr int kSegments = kLong ? kMostSegments : 64;
+  double table[256];
+  uint64_t sums[kSegments];
   uint64_t warp_sums[32];
-  uint64_t list[kList];
   union {
-    uint64_t masses[kList];
-    uint32_t counts[kBins];
+    uint64_t list[kRegion];
+    struct {
+      uint64_t list_[kList];
+      uint64_t masses[kList];
+    };
+    struct {
+      uint32_t counts[kLong ? kBins : 1];
+      uint32_t low[kLong ? kBins : 1], high[kLong ? kBins : 1];  // masses of the bins
+    };
+    uint32_t mass_counts[kLong ? kMassBins : 1];
   };
-  uint32_t low[kBins], high[kBins];  // masses of the bins, in fixed point
+  uint32_t sub_low[kLong ? kSubBins : 1], sub_high[kLong ? kSubBins : 1];
   float reds[64];
   uint32_t keys[64];
   int listed, found;
@@ -147,84 +168,164 @@ struct RowShared {
   long long amount;
 };
 
+// Adds to a 64-bit sum of two words.
+__device__ __forceinline__ void add_to(uint32_t* low, uint32_t* high, uint64_t m) {
+  const uint32_t l = (uint32_t)m, old = atomicAdd(low, l);
+  const uint32_t h = (uint32_t)(m >> 32) + (old + l < old ? 1u : 0u);
+  if (h) atomicAdd(high, h);
+}
+__device__ __forceinline__ uint64_t warp_sum(uint64_t s) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+template <class S>
+__device__ __forceinline__ S warp_running(S s, int lane) {  // with this lane's own
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const S below = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += below;
+  }
+  return s;
+}
+
+// 16 bytes of a row: 8 entries, or 4 of fp32.
+template <class T>
+struct Entries {
+  static constexpr int kV = 16 / sizeof(T);
+  uint4 q;
+  __device__ __forceinline__ float at(int j) const {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+    if constexpr (__is_same(T, __nv_bfloat16)) return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+    else return __half2float(__ushort_as_half((unsigned short)(j & 1 ? w[j / 2] >> 16 : w[j / 2])));
+  }
+  __device__ __forceinline__ void set(int j, T v) { reinterpret_cast<T*>(&q)[j] = v; }
+  // the largest, NaN aside: of two, then of all
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4) {
+      return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    } else if constexpr (__is_same(T, __nv_bfloat16)) {
+      const __nv_bfloat162 m = __hmax2(reinterpret_cast<__nv_bfloat162&>(a), reinterpret_cast<__nv_bfloat162&>(b));
+      return reinterpret_cast<const uint32_t&>(m);
+    } else {
+      const __half2 m = __hmax2(reinterpret_cast<__half2&>(a), reinterpret_cast<__half2&>(b));
+      return reinterpret_cast<const uint32_t&>(m);
+    }
+  }
+  __device__ __forceinline__ uint32_t most() const { return max2(max2(q.x, q.y), max2(q.z, q.w)); }
+  static __device__ __forceinline__ float value(uint32_t most) {
+    if constexpr (sizeof(T) == 4) return clean(__uint_as_float(most));
+    Entries e;
+    e.q.x = most;
+    return fmaxf(clean(e.at(0)), clean(e.at(1)));
+  }
+};
+
 template <class T, int THREADS>
 struct Row {
   using Sh = RowShared<THREADS>;
-  static constexpr int kWarps = THREADS / 32;
+  using E = Entries<T>;
+  static constexpr int kWarps = THREADS / 32, kV = E::kV, kChunk = 32 * kV;
   const SampleParams& p;
   Sh& sh;
   const T* z;
-  int n, shift, chunks, per_segment, segments;  // chunks of 256 entries; of a segment
-  float top;
-  uint64_t limit;  // places from here on up are kept
+  int n, shift, chunks, per_segment, segments;  // chunks of a warp's vectors; of a segment
+  float top, lowest;      // of the entries; what lies below `lowest` has no mass
+  double steep, offset;   // v steep + offset = 256 log2(e) (v - top) / T
+  bool far;               // ... but for a top whose offset 64 bits round
+  uint64_t limit;         // places from here on are kept
   int warp, lane;
 
   __device__ __forceinline__ Row(const SampleParams& p_, Sh& sh_, long long row) : p(p_), sh(sh_) {
     z = static_cast<const T*>(p.logits) + row * p.stride;
     n = p.classes;
     shift = (int)(reinterpret_cast<uintptr_t>(z) % 16 / sizeof(T));  // chunks start on 16-byte boundaries
-    chunks = (n + shift + 255) / 256;
-    per_segment = (chunks + kMostSegments - 1) / kMostSegments;
+    chunks = (n + shift + kChunk - 1) / kChunk;
+    per_segment = (chunks + Sh::kSegments - 1) / Sh::kSegments;
     segments = (chunks + per_segment - 1) / per_segment;
-    limit = 0;
+    limit = kPossible;
     warp = threadIdx.x / 32;
     lane = threadIdx.x % 32;
+    // a weight of 1 is p.one: sums are in fixed point
+    for (int i = threadIdx.x; i < 256; i += THREADS) sh.table[i] = exp2(i / 256.0) * p.one;
   }
-  // This lane's 8 entries of a chunk, from entry `first` on; entries outside of the row are -inf.
-  __device__ __forceinline__ int fetch(int chunk, float (&v)[8]) const {
-    const int first = chunk * 256 + lane * 8 - shift;
-    if (first >= 0 && first + 8 <= n) {
-      constexpr int V = 16 / sizeof(T);
-#pragma unroll
-      for (int k = 0; k < 8 / V; ++k) {
-        const Vec<T, V> q = *reinterpret_cast<const Vec<T, V>*>(z + first + k * V);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[k * V + j] = clean(to_f32<T>(q.v[j]));
-      }
+  __device__ __forceinline__ void set_top(float t) {
+    top = t;
+    steep = p.inverse_t * 369.32993046757463;
+    offset = -(double)top * steep;
+    far = !(fabs(offset) < 262144.0);
+    lowest = (float)((double)top - 42.0 / p.inverse_t);  // e^-42 < 2^-60
+  }
+  // This lane's entries of a chunk, from entry `first` on; entries outside of the row are -inf.
+  __device__ __forceinline__ int fetch(int chunk, E& e) const {
+    const int first = chunk * kChunk + lane * kV - shift;
+    if (first >= 0 && first + kV <= n) {
+      e.q = *reinterpret_cast<const uint4*>(z + first);
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = first + j >= 0 && first + j < n ? clean(to_f32<T>(z[first + j])) : __int_as_float(0xff800000);
+      for (int j = 0; j < kV; ++j)
+        e.set(j, first + j >= 0 && first + j < n ? z[first + j] : from_f32<T>(__int_as_float(0xff800000)));
     }
     return first;
   }
-  // exp((v - top) / T) of a possible v
-  __device__ __forceinline__ double weight(float v) const {
-    if (v == top) return 1.0;
-    constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52: the sum's low bits are the nearest whole number
-    const double x = ((double)v - (double)top) * (p.inverse_t * 92.332482616893656770);  // 64 log2(e)
-    if (!(x > -64.0 * 1000)) return 0.0;
+  // fn(first, entries): chunks in turn over the warps; the next one's load is on its way while one is worked on.
+  template <class F>
+  __device__ __forceinline__ void each_chunk(F fn) const {
+    E next;
+    int at = 0;
+    if (warp < chunks) at = fetch(warp, next);
+    for (int c = warp; c < chunks; c += kWarps) {
+      const E e = next;
+      const int first = at;
+      if (c + kWarps < chunks) at = fetch(c + kWarps, next);
+      fn(first, e);
+    }
+  }
+  // fn(segment, fn of its chunks): segments in turn over the warps.
+  template <class F>
+  __device__ __forceinline__ uint64_t segment(int s, F fn) const {
+    const int end = min((s + 1) * per_segment, chunks);
+    uint64_t sum = 0;
+    for (int c = s * per_segment; c < end; ++c) {
+      E e;
+      const int first = fetch(c, e);
+      sum += fn(first, e);
+    }
+    return warp_sum(sum);
+  }
+  __device__ __forceinline__ bool kept(float v, int i) const { return place_of(key_of(v), i) >= limit; }  // of a clean v
+
+  // exp((v - top) / T) times p.one
+  template <bool FAR>
+  __device__ __forceinline__ double weight_of(float v) const {
+    constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52: the low bits of a sum with it are the nearest whole number
+    double x;
+    if constexpr (!FAR) {
+      x = fma((double)fmaxf(v, lowest), steep, offset);
+    } else {
+      if (v == top) return p.one;  // also of infinities
+      x = ((double)v - (double)top) * steep;
+      if (!(x > -16000.0)) return 0.0;
+    }
     const double m = x + kMagic;
     const int k = __double2loint(m);
     const double r = x - (m - kMagic);
-    constexpr double c = 0.010830424696249145;  // ln(2) / 64
-    const double q = r * (c + r * (c * c / 2 + r * (c * c * c / 6 + r * (c * c * c * c / 24))));
-    const double t = sh.table[k & 63];
-    const double e = fma(t, q, t);
-    return __hiloint2double(__double2hiint(e) + ((k >> 6) << 20), __double2loint(e));
+    constexpr double c = 0.0027076061740622863;  // ln(2) / 256
+    const double q = r * (c + r * (c * c / 2 + r * (c * c * c / 6)));
+    const double t = sh.table[k & 255], e = fma(t, q, t);
+    return __hiloint2double(__double2hiint(e) + ((k & ~255) << 12), __double2loint(e));
   }
-  __device__ __forceinline__ bool kept(float v, int i) const { return possible(v) && place_of(key_of(v), i) >= limit; }
+  __device__ __forceinline__ double weight(float v) const { return far ? weight_of<true>(v) : weight_of<false>(v); }
+  __device__ __forceinline__ uint64_t mass(float v) const { return fixed(weight(v), 1.0); }
+  __device__ __forceinline__ uint64_t near_mass(float v) const { return fixed(weight_of<false>(v), 1.0); }
 
-  template <class F>
-  __device__ __forceinline__ void each_chunk(F fn) const {
-    for (int c = warp; c < chunks; c += kWarps) {
-      float v[8];
-      const int first = fetch(c, v);
-      fn(first, v);
-    }
-  }
-  __device__ __forceinline__ uint64_t mass(float v) const { return fixed(weight(v), p.one); }
   // Running sums of a[0 .. count) in place; returns the whole.
   __device__ __forceinline__ uint64_t scan(uint64_t* a, int count) {
     uint64_t carry = 0;
     for (int b = 0; b < count; b += THREADS) {
       const int i = b + threadIdx.x;
-      uint64_t s = i < count ? a[i] : 0;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t below = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += below;
-      }
+      uint64_t s = warp_running(i < count ? a[i] : 0, lane);
       __syncthreads();
       if (lane == 31) sh.warp_sums[warp] = s;
       __syncthreads();
@@ -238,6 +339,15 @@ struct Row {
     __syncthreads();
     return carry;
   }
+  // The sum of a value of each warp.
+  __device__ __forceinline__ uint64_t block_sum(uint64_t s) {
+    __syncthreads();
+    if (lane == 0) sh.warp_sums[warp] = s;
+    __syncthreads();
+    s = 0;
+    for (int w = 0; w < kWarps; ++w) s += sh.warp_sums[w];
+    return s;
+  }
   // The first of count running sums above t.
   __device__ __forceinline__ int above(const uint64_t* a, int count, uint64_t t) const {
     int lo = 0, hi = count - 1;
@@ -248,8 +358,11 @@ struct Row {
     }
     return lo;
   }
-  // list[0 .. size), size a power of two, to descending order
-  __device__ __forceinline__ void sort(int size) {
+  // The list, filled up to a power of two, to descending order.
+  __device__ __forceinline__ void sort(int count) {
+    int size = 2;
+    while (size < count) size <<= 1;
+    for (int i = count + threadIdx.x; i < size; i += THREADS) sh.list[i] = 0;
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j; j >>= 1) {
         __syncthreads();
@@ -261,25 +374,36 @@ struct Row {
       }
     __syncthreads();
   }
-  __device__ __forceinline__ int padded() {  // the list filled up with places below all others
-    const int c = sh.listed;
-    int size = 2;
-    while (size < c) size <<= 1;
-    for (int i = c + threadIdx.x; i < size; i += THREADS) sh.list[i] = 0;
-    return size;
+  // All lanes of a warp call it.
+  __device__ __forceinline__ int room_for(bool mine) {
+    const unsigned who = __ballot_sync(0xffffffffu, mine);
+    if (!who) return 0;
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&sh.listed, __popc(who));
+    return __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1));
   }
-  __device__ __forceinline__ void append(uint64_t place) {
-    const int at = atomicAdd(&sh.listed, 1);
-    if (at < Sh::kList) sh.list[at] = place;
+  __device__ __forceinline__ void append(bool mine, uint64_t place, int room) {
+    const int at = room_for(mine);
+    if (mine && at < room) sh.list[at] = place;
+  }
+  __device__ __forceinline__ void append(bool mine, float v, int i, int room) {
+    const int at = room_for(mine);
+    if (mine && at < room) sh.list[at] = place_of(key_of(clean(v)), i);
+  }
+  __device__ __forceinline__ void start_list() {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
   }
 
   // The largest entry; with `groups` (a power of two, at most THREADS) also a bound that so many entries reach.
   __device__ __forceinline__ float largest(int groups, float& bound) {
-    float m = __int_as_float(0xff800000);
-    each_chunk([&](int, const float (&v)[8]) {
+    E none;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = fmaxf(m, v[j]);
-    });
+    for (int j = 0; j < kV; ++j) none.set(j, from_f32<T>(__int_as_float(0xff800000)));
+    uint32_t most = none.q.x;
+    each_chunk([&](int, const E& e) { most = E::max2(most, e.most()); });
+    float m = E::value(most);
     const int wide = THREADS / groups;  // threads of a group
     for (int o = 1; o < min(wide, 32); o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float least = m;
@@ -296,146 +420,37 @@ struct Row {
     const int warps = max(wide / 32, 1);  // of a group
     bound = __int_as_float(0x7f800000);
     for (int g = 0; g < kWarps; g += warps) {
-      float most = __int_as_float(0xff800000);
-      if (warps == 1) most = sh.reds[32 + g];
+      float first = __int_as_float(0xff800000);
+      if (warps == 1) first = sh.reds[32 + g];
       else
-        for (int w = 0; w < warps; ++w) most = fmaxf(most, sh.reds[g + w]);
-      bound = fminf(bound, most);
+        for (int w = 0; w < warps; ++w) first = fmaxf(first, sh.reds[g + w]);
+      bound = fminf(bound, first);
     }
     m = sh.reds[0];
     for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh.reds[w]);
     return m;
   }
 
-  // The first `need` of the entries from `limit` on (BY_MASS: those before which less than `share` of their mass lies) by
-  // histograms over their keys: the new limit.
-  template <bool BY_MASS>
-  __device__ __forceinline__ void narrow(long long need, double share) {
-    uint32_t lo, hi;
-    {  // the range of the keys
-      uint32_t a = 0xffffffffu, b = 0;
-      each_chunk([&](int first, const float (&v)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (kept(v[j], first + j)) a = min(a, key_of(v[j])), b = max(b, key_of(v[j]));
-      });
-      a = __reduce_min_sync(0xffffffffu, a);
-      b = __reduce_max_sync(0xffffffffu, b);
-      __syncthreads();
-      if (lane == 0) sh.keys[warp] = a, sh.keys[32 + warp] = b;
-      __syncthreads();
-      lo = sh.keys[0], hi = sh.keys[32];
-      for (int w = 1; w < kWarps; ++w) lo = min(lo, sh.keys[w]), hi = max(hi, sh.keys[32 + w]);
+  // The least place of a weight of min_p, by a search of 32 keys at a time (every warp for itself).
+  __device__ __forceinline__ uint64_t limit_of_weight(double min_p) const {
+    const double least = min_p * p.one;
+    uint32_t lo = (uint32_t)(kPossible >> 32), hi = key_of(top);  // hi is heavy enough
+    while (lo < hi) {
+      const uint32_t step = (hi - lo + 30) / 31, at = min(lo + lane * step, hi);
+      const float v = of_key(at);
+      const int first = __ffs(__ballot_sync(0xffffffffu, weight(v) >= least || at == hi)) - 1;  // of the 32
+      const uint32_t found = __shfl_sync(0xffffffffu, at, first);
+      lo = first == 0 ? lo : __shfl_sync(0xffffffffu, at, first - 1) + 1;
+      hi = found;
     }
-    uint64_t above_mass = 0, target = 0;
-    long long above_count = 0;
-    bool have_target = !BY_MASS;
-    for (;;) {
-      int bin_bits = 0;
-      while ((hi - lo) >> bin_bits >= kBins) ++bin_bits;
-      __syncthreads();
-      for (int i = threadIdx.x; i < kBins; i += THREADS) sh.counts[i] = sh.low[i] = sh.high[i] = 0;
-      __syncthreads();
-      each_chunk([&](int first, const float (&v)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t key = key_of(v[j]);
-          if (key < lo || key > hi || !kept(v[j], first + j)) continue;
-          const uint32_t b = (key - lo) >> bin_bits;
-          atomicAdd(&sh.counts[b], 1u);
-          if (BY_MASS) {
-            const uint64_t m = mass(v[j]);
-            const uint32_t l = (uint32_t)m;
-            uint32_t h = (uint32_t)(m >> 32);
-            const uint32_t old = atomicAdd(&sh.low[b], l);
-            if (old + l < old) ++h;  // the carry
-            if (h) atomicAdd(&sh.high[b], h);
-          }
-        }
-      });
-      __syncthreads();
-      // from the largest bin down: the one with the border (a thread; the loops over the row cost far more)
-      if (warp == 0) {
-        const auto mass_of = [&](int b) { return (uint64_t)sh.high[b] << 32 | sh.low[b]; };
-        constexpr int kPer = kBins / 32;
-        uint64_t ms = 0;
-        uint32_t cs = 0;
-        for (int i = 0; i < kPer; ++i) {  // lane 0: the largest bins
-          const int b = kBins - 1 - (lane * kPer + i);
-          cs += sh.counts[b];
-          if (BY_MASS) ms += mass_of(b);
-        }
-        uint64_t m_before = 0, m_all = 0;
-        uint32_t c_before = 0;
-        for (int w = 0; w < 32; ++w) {
-          const uint64_t mw = __shfl_sync(0xffffffffu, ms, w);
-          const uint32_t cw = __shfl_sync(0xffffffffu, cs, w);
-          m_all += mw;
-          if (w < lane) m_before += mw, c_before += cw;
-        }
-        if (!have_target) target = (uint64_t)__double2ull_ru(share * (double)m_all);
-        // the border lies in the bin at which the sum reaches what is asked for; in the last that holds anything otherwise
-        int at = -1;
-        uint64_t m = above_mass + m_before;
-        long long c = above_count + c_before;
-        for (int i = 0; i < kPer && at < 0; ++i) {
-          const int b = kBins - 1 - (lane * kPer + i);
-          const uint32_t count = sh.counts[b];
-          if (count && (BY_MASS ? m < target && m + mass_of(b) >= target : c < need && c + count >= need)) at = b;
-          else m += BY_MASS ? mass_of(b) : 0, c += count;
-        }
-        const unsigned who = __ballot_sync(0xffffffffu, at >= 0);
-        if (who ? lane == __ffs(who) - 1 : lane == 0) {
-          sh.found = at;
-          sh.limit = m;
-          sh.amount = c;
-        }
-        if (lane == 0) sh.keys[0] = (uint32_t)target, sh.keys[1] = (uint32_t)(target >> 32);
-      }
-      __syncthreads();
-      const int bin = sh.found;
-      if (BY_MASS) target = (uint64_t)sh.keys[1] << 32 | sh.keys[0];
-      have_target = true;
-      if (bin < 0) return;  // everything
-      above_mass = sh.limit;
-      above_count = sh.amount;
-      const uint32_t in_bin = sh.counts[bin];
-      lo += (uint32_t)bin << bin_bits;
-      hi = bin_bits ? min(hi, lo + ((1u << bin_bits) - 1)) : lo;
-      __syncthreads();
-      if (in_bin <= Sh::kList) break;
-      if (lo == hi) {  // so many ties: the first by index
-        const uint64_t m = mass(of_key(lo));
-        long long ties = need - above_count;
-        if (BY_MASS) ties = m ? (long long)((target - above_mass + m - 1) / m) : in_bin;
-        nth_tie(lo, ties);
-        return;
-      }
-    }
-    // the entries of the bin with the border, sorted
-    if (threadIdx.x == 0) sh.listed = 0;
-    __syncthreads();
-    each_chunk([&](int first, const float (&v)[8]) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t key = key_of(v[j]);
-        if (key >= lo && key <= hi && kept(v[j], first + j)) append(place_of(key, first + j));
-      }
-    });
-    __syncthreads();
-    const int count = sh.listed;
-    sort(padded());
+    return (uint64_t)lo << 32;
+  }
+  // The place at which the sorted list's masses, from `m` on, reach the target.
+  __device__ __forceinline__ uint64_t limit_of_list(int count, uint64_t m, uint64_t target) {
     if (warp == 0) {
-      int taken = BY_MASS ? 0 : (int)min((long long)count, need - above_count);
-      uint64_t m = above_mass;
-      for (int b = 0; BY_MASS && b < count; b += 32) {
-        const uint64_t own = b + lane < count ? mass(of_key((uint32_t)(sh.list[b + lane] >> 32))) : 0;
-        uint64_t up = own;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint64_t below = __shfl_up_sync(0xffffffffu, up, o);
-          if (lane >= o) up += below;
-        }
+      int taken = 0;
+      for (int b = 0; b < count; b += 32) {
+        const uint64_t own = b + lane < count ? mass(value_of(sh.list[b + lane])) : 0, up = warp_running(own, lane);
         const unsigned in = __ballot_sync(0xffffffffu, b + lane < count && m + up - own < target);
         taken += __popc(in);
         m += __shfl_sync(0xffffffffu, up, 31);
@@ -444,20 +459,303 @@ struct Row {
       if (lane == 0) sh.limit = sh.list[max(taken, 1) - 1];
     }
     __syncthreads();
-    limit = sh.limit;
+    const uint64_t l = sh.limit;
     __syncthreads();
+    return l;
+  }
+
+  // top_p alone.  `least`: the limit by min_p.  Returns kCut where the limit is found, kSummed where sh.sums also holds the
+  // segments' kept sums, kNot where the entries about the border do not fit the list.
+  enum { kNot, kCut, kSummed };
+  __device__ __forceinline__ int cut_mass(uint64_t least) {
+    if constexpr (Sh::kLong) {
+      const float scale = kPerBin * (float)p.inverse_t;
+      for (int i = threadIdx.x; i < kMassBins; i += THREADS) sh.mass_counts[i] = 0;
+      for (int i = threadIdx.x; i < kSubBins; i += THREADS) sh.sub_low[i] = sh.sub_high[i] = 0;
+      if (threadIdx.x < 8) sh.keys[threadIdx.x] = kMassBins - 1;
+      __syncthreads();
+      each_chunk([&](int, const E& e) {
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {  // to nearest, by the bits of a sum with 2^23; NaN to the last
+          const uint32_t b = __float_as_uint(fmaf(top - e.at(j), scale, 8388608.f)) - 0x4b000000u;
+          atomicAdd(&sh.mass_counts[min(b, (uint32_t)kMassBins - 1)], 1u);
+        }
+      });
+      __syncthreads();
+      // bin b lies at (b -+ 0.501) / 200 (roundings: 8192 2^-23 of a bin): bounds of the masses up to every bin
+      constexpr int kPer = kMassBins / THREADS;
+      constexpr float kLog = -1.4426950408889634f / kPerBin;
+      float lower = 0.f, upper = 0.f;
+      int count = 0;
+      for (int i = 0; i < kPer; ++i) {
+        const int b = threadIdx.x * kPer + i, c = b + 1 < kMassBins ? sh.mass_counts[b] : 0;
+        count += c;
+        lower += c * ex2((b + 0.501f) * kLog);
+        upper += c * ex2((b - 0.501f) * kLog);
+      }
+      const float l_up = warp_running(lower, lane), u_up = warp_running(upper, lane);
+      const int c_up = warp_running(count, lane);
+      if (lane == 31) {
+        sh.reds[warp] = l_up;
+        sh.reds[32 + warp] = u_up;
+        sh.keys[32 + warp] = c_up;
+      }
+      __syncthreads();
+      float l = l_up - lower, u = u_up - upper, l_all = 0.f, u_all = 0.f;
+      int c = c_up - count;
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) l += sh.reds[w], u += sh.reds[32 + w], c += sh.keys[32 + w];
+        l_all += sh.reds[w], u_all += sh.reds[32 + w];
+      }
+      // the first bins at which the border may have been reached, is likely to be, and must have been (fp32 sums of 8192
+      // terms, in three levels: 2^-17 of themselves)
+      const float may = (float)p.top_p * l_all * 0.9999f, must = (float)p.top_p * u_all * 1.0001f;
+      const float likely = (float)p.top_p * 0.5f * (l_all + u_all);
+      const int before = c;
+      {
+        uint32_t first[3] = {kMassBins - 1, kMassBins - 1, kMassBins - 1}, at_likely = 0;
+        for (int i = 0; i < kPer; ++i) {
+          const int b = threadIdx.x * kPer + i, here = b + 1 < kMassBins ? sh.mass_counts[b] : 0;
+          l += here * ex2((b + 0.501f) * kLog);
+          u += here * ex2((b - 0.501f) * kLog);
+          if (u >= may) first[0] = min(first[0], b);
+          if (0.5f * (l + u) >= likely && b < first[1]) first[1] = b, at_likely = c;
+          if (l >= must) first[2] = min(first[2], b);
+          c += here;
+        }
+        const uint32_t mid = __reduce_min_sync(0xffffffffu, first[1]);
+        for (int i = 0; i < 3; ++i) {
+          const uint32_t f = __reduce_min_sync(0xffffffffu, first[i]);
+          if (lane == 0) atomicMin(&sh.keys[i], f);
+        }
+        __syncthreads();
+        if (first[1] == sh.keys[1] && mid == first[1]) sh.amount = at_likely;
+      }
+      __syncthreads();
+      uint32_t from = sh.keys[0], to = sh.keys[2];
+      const float sure = top - (from - 0.501f) / scale;  // the border lies below
+      if (value_of(least) > sure) {
+        limit = least;
+        __syncthreads();
+        return kCut;
+      }
+      // as many entries about the likely one as the list holds
+      const int room = Sh::kRegion / 2 - 64, centre = (int)sh.amount;
+      c = before;
+      uint32_t low_bin = kMassBins - 1, high_bin = 0;
+      for (int i = 0; i < kPer; ++i) {
+        const uint32_t b = threadIdx.x * kPer + i;
+        const int here = b + 1 < kMassBins ? sh.mass_counts[b] : 0;
+        if (c >= centre - room) low_bin = min(low_bin, b);
+        if (c + here <= centre + room) high_bin = max(high_bin, b);
+        c += here;
+      }
+      low_bin = __reduce_min_sync(0xffffffffu, low_bin);
+      high_bin = __reduce_max_sync(0xffffffffu, high_bin);
+      if (threadIdx.x == 0) sh.keys[4] = 0;
+      __syncthreads();
+      if (lane == 0) {
+        atomicMin(&sh.keys[3], low_bin);
+        atomicMax(&sh.keys[4], high_bin);
+      }
+      start_list();
+      from = max(from, sh.keys[3]);
+      to = min(to, sh.keys[4]);
+      if (from > to || to >= kMassBins - 1) return kNot;
+      const float high = top - (from - 0.5f) / scale, low = top - (to + 0.5f) / scale;  // the list: low < v <= high
+      __syncthreads();  // the list takes the counts' place
+      uint64_t sure_sum = 0, all = 0;
+      for (int s = warp; s < segments; s += kWarps) {
+        const uint64_t sum = segment(s, [&](int first, const E& e) {
+          uint64_t some = 0;
+#pragma unroll
+          for (int j = 0; j < kV; ++j) {
+            const float v = e.at(j);
+            const uint64_t m = near_mass(v);
+            all += m;
+            some += v > high ? m : 0;
+            append(v <= high && v > low, v, first + j, Sh::kRegion);
+          }
+          return some;
+        });
+        sure_sum += sum;
+        if (lane == 0) sh.sums[s] = sum;
+      }
+      sure_sum = block_sum(sure_sum);
+      all = block_sum(warp_sum(all));
+      const int listed = sh.listed;
+      if (listed > Sh::kRegion) return kNot;
+      const uint64_t target = (uint64_t)__double2ull_ru(p.top_p * (double)all);
+      // the list by 256 bins of their own, then the border's
+      const float fine = low < high ? kSubBins / (high - low) : 0.f;
+      const auto sub_of = [&](float v) { return min(max((int)((high - v) * fine), 0), kSubBins - 1); };
+      constexpr int kOwn = Sh::kRegion / THREADS;
+      uint64_t own[kOwn], masses[kOwn];
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const int at = threadIdx.x + i * THREADS;
+        own[i] = at < listed ? sh.list[at] : 0;
+        masses[i] = 0;
+        if (own[i]) {
+          masses[i] = mass(value_of(own[i]));
+          const int b = sub_of(value_of(own[i]));
+          add_to(&sh.sub_low[b], &sh.sub_high[b], masses[i]);
+        }
+      }
+      start_list();
+      if (warp == 0) {
+        uint64_t m = sure_sum;
+        int border = -1;
+        for (int b = 0; b < kSubBins && border < 0 && m < target; b += 32) {
+          const uint64_t here = (uint64_t)sh.sub_high[b + lane] << 32 | sh.sub_low[b + lane], up = warp_running(here, lane);
+          const unsigned reached = __ballot_sync(0xffffffffu, m + up >= target);
+          const int at = reached ? __ffs(reached) - 1 : 31;
+          if (reached) border = b + at;
+          m += __shfl_sync(0xffffffffu, reached ? up - here : up, at);
+        }
+        if (lane == 0) {
+          sh.found = border;
+          sh.limit = m;
+        }
+      }
+      __syncthreads();
+      const int border = sh.found;
+      const uint64_t reached = sh.limit;
+      if (border < 0) return kNot;  // not about the likely place
+      const int per = kChunk * per_segment;
+      const auto join = [&](uint64_t place, uint64_t m) {
+        if (place >= least)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sums[(index_of(place) + shift) / per]), (unsigned long long)m);
+      };
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const int b = own[i] ? sub_of(value_of(own[i])) : kSubBins;
+        if (b < border) join(own[i], masses[i]);
+        append(b == border, own[i], Sh::kRegion);
+      }
+      __syncthreads();
+      const int last = sh.listed;
+      sort(last);
+      const uint64_t at = limit_of_list(last, reached, target);
+      for (int i = threadIdx.x; i < last; i += THREADS)
+        if (sh.list[i] >= at) join(sh.list[i], mass(value_of(sh.list[i])));
+      limit = max(at, least);
+      __syncthreads();
+      return kSummed;
+    } else {
+      return kNot;
+    }
+  }
+
+  // The first `need` of the entries from `limit` on (BY_MASS: those before which less than `share` of their mass lies) by
+  // histograms over their keys: the new limit.
+  template <bool BY_MASS>
+  __device__ __forceinline__ void narrow(long long need, double share) {
+    if constexpr (Sh::kLong) {
+      uint32_t lo = (uint32_t)(limit >> 32), hi = key_of(top);
+      uint64_t above_mass = 0, target = 0;
+      long long above_count = 0;
+      bool have_target = !BY_MASS;
+      for (;;) {
+        int bin_bits = 0;
+        while ((hi - lo) >> bin_bits >= kBins) ++bin_bits;
+        __syncthreads();
+        for (int i = threadIdx.x; i < kBins; i += THREADS) sh.counts[i] = sh.low[i] = sh.high[i] = 0;
+        __syncthreads();
+        const float bottom = of_key(lo), ceiling = of_key(hi);
+        each_chunk([&](int first, const E& e) {
+          if (!(E::value(e.most()) >= bottom)) return;
+#pragma unroll
+          for (int j = 0; j < kV; ++j) {
+            const float v = clean(e.at(j));
+            if (!(v >= bottom && v <= ceiling) || !kept(v, first + j)) continue;
+            const uint32_t b = (key_of(v) - lo) >> bin_bits;
+            atomicAdd(&sh.counts[b], 1u);
+            if (BY_MASS) add_to(&sh.low[b], &sh.high[b], mass(v));
+          }
+        });
+        __syncthreads();
+        // from the largest bin down: the one with the border
+        if (warp == 0) {
+          const auto mass_of = [&](int b) { return (uint64_t)sh.high[b] << 32 | sh.low[b]; };
+          constexpr int kPer = kBins / 32;
+          uint64_t ms = 0;
+          long long cs = 0;
+          for (int i = 0; i < kPer; ++i) {  // lane 0: the largest bins
+            const int b = kBins - 1 - (lane * kPer + i);
+            cs += sh.counts[b];
+            if (BY_MASS) ms += mass_of(b);
+          }
+          const uint64_t m_up = warp_running(ms, lane);
+          if (!have_target) target = (uint64_t)__double2ull_ru(share * (double)__shfl_sync(0xffffffffu, m_up, 31));
+          // the border lies in the bin at which the sum reaches what is asked for
+          int at = -1;
+          uint64_t m = above_mass + m_up - ms;
+          long long c = above_count + warp_running(cs, lane) - cs;
+          for (int i = 0; i < kPer && at < 0; ++i) {
+            const int b = kBins - 1 - (lane * kPer + i);
+            const uint32_t count = sh.counts[b];
+            if (count && (BY_MASS ? m < target && m + mass_of(b) >= target : c < need && c + count >= need)) at = b;
+            else m += BY_MASS ? mass_of(b) : 0, c += count;
+          }
+          const unsigned who = __ballot_sync(0xffffffffu, at >= 0);
+          if (who ? lane == __ffs(who) - 1 : lane == 0) {
+            sh.found = at;
+            sh.limit = m;
+            sh.amount = c;
+          }
+          if (lane == 0) sh.keys[0] = (uint32_t)target, sh.keys[1] = (uint32_t)(target >> 32);
+        }
+        __syncthreads();
+        const int bin = sh.found;
+        if (BY_MASS) target = (uint64_t)sh.keys[1] << 32 | sh.keys[0];
+        have_target = true;
+        if (bin < 0) return;  // everything
+        above_mass = sh.limit;
+        above_count = sh.amount;
+        const uint32_t in_bin = sh.counts[bin];
+        lo += (uint32_t)bin << bin_bits;
+        hi = bin_bits ? min(hi, lo + ((1u << bin_bits) - 1)) : lo;
+        if (in_bin <= Sh::kRegion) break;
+        if (lo == hi) {  // so many ties: the first by index
+          const uint64_t m = mass(of_key(lo));
+          long long ties = need - above_count;
+          if (BY_MASS) ties = m ? (long long)((target - above_mass + m - 1) / m) : in_bin;
+          nth_tie(lo, ties);
+          return;
+        }
+      }
+      // the entries of the bin with the border, sorted
+      start_list();
+      const float bottom = of_key(lo), ceiling = of_key(hi);
+      each_chunk([&](int first, const E& e) {
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+          const float v = clean(e.at(j));
+          append(v >= bottom && v <= ceiling && kept(v, first + j), v, first + j, Sh::kRegion);
+        }
+      });
+      __syncthreads();
+      const int count = sh.listed;
+      sort(count);
+      if (BY_MASS) limit = limit_of_list(count, above_mass, target);
+      else limit = sh.list[max(1, (int)min((long long)count, need - above_count)) - 1];
+      __syncthreads();
+    }
   }
   // The limit that keeps the first `ties` entries of a key (and all larger ones).
   __device__ __forceinline__ void nth_tie(uint32_t key, long long ties) {
-    for (int s = warp; s < segments; s += kWarps) {
-      int count = 0;
-      for (int c = s * per_segment; c < min((s + 1) * per_segment, chunks); ++c) {
-        float v[8];
-        const int first = fetch(c, v);
+    const auto count_in = [&](int first, const E& e) {
+      uint64_t count = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) count += key_of(v[j]) == key && kept(v[j], first + j);
+      for (int j = 0; j < kV; ++j) {
+        const float v = clean(e.at(j));
+        count += key_of(v) == key && kept(v, first + j);
       }
-      count = __reduce_add_sync(0xffffffffu, count);
+      return count;
+    };
+    for (int s = warp; s < segments; s += kWarps) {
+      const uint64_t count = segment(s, count_in);
       if (lane == 0) sh.sums[s] = count;
     }
     __syncthreads();
@@ -467,26 +765,19 @@ struct Row {
       while (s < segments - 1 && (long long)sh.sums[s] < left) left -= (long long)sh.sums[s++];
       int at = -1;
       for (int c = s * per_segment; c < min((s + 1) * per_segment, chunks) && at < 0; ++c) {
-        float v[8];
-        const int first = fetch(c, v);
-        int mine = 0;
+        E e;
+        const int first = fetch(c, e);
+        const int mine = (int)count_in(first, e), up = warp_running(mine, lane);
+        if (up - mine < left && up >= left) {
+          long long k = left - (up - mine);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mine += key_of(v[j]) == key && kept(v[j], first + j);
-        int sum = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int below = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += below;
-        }
-        const int all = __shfl_sync(0xffffffffu, sum, 31);
-        if (sum - mine < left && sum >= left) {
-          long long k = left - (sum - mine);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (key_of(v[j]) == key && kept(v[j], first + j) && --k == 0) at = first + j;
+          for (int j = 0; j < kV; ++j) {
+            const float v = clean(e.at(j));
+            if (key_of(v) == key && kept(v, first + j) && --k == 0) at = first + j;
+          }
         }
         at = __reduce_max_sync(0xffffffffu, at);
-        left -= all;
+        left -= __shfl_sync(0xffffffffu, up, 31);
       }
       if (lane == 0) sh.limit = place_of(key, at < 0 ? n : at);
     }
@@ -501,27 +792,26 @@ struct Row {
       if (p.probs) p.probs[row * p.draws + d] = 0.f;
     }
   }
-  // The kept entries are in the list: by rank, cut by top-p and min-p, then by index.
-  __device__ __forceinline__ void draw_listed(long long row) {
-    const int count = min(sh.listed, p.top_k);
-    sort(padded());
+  // The list holds the first top_k entries and maybe others: by rank, cut by top-p and min-p, then by index.
+  __device__ __forceinline__ void draw_listed(long long row, uint64_t least) {
+    const int listed = sh.listed, count = min(listed, p.top_k);
+    sort(listed);
     int m = count;
     if (p.top_p < 1.0) {
-      for (int i = threadIdx.x; i < count; i += THREADS) sh.masses[i] = mass(of_key((uint32_t)(sh.list[i] >> 32)));
+      for (int i = threadIdx.x; i < count; i += THREADS) sh.masses[i] = mass(value_of(sh.list[i]));
       __syncthreads();
       const uint64_t all = scan(sh.masses, count), target = (uint64_t)__double2ull_ru(p.top_p * (double)all);
       m = above(sh.masses, count, target - 1) + 1;  // the first sum that reaches the target is the last one kept
     }
     for (int i = threadIdx.x; i < m; i += THREADS) {  // by index from the lowest: descending again
       const uint64_t place = sh.list[i];
-      sh.list[i] = (uint64_t)(uint32_t)place << 32 | (uint32_t)(place >> 32);
+      sh.list[i] = place << 32 | place >> 32;
     }
-    if (threadIdx.x == 0) sh.listed = m;
     __syncthreads();
-    sort(padded());
+    sort(m);
     for (int i = threadIdx.x; i < m; i += THREADS) {
-      const double w = weight(of_key((uint32_t)sh.list[i]));
-      sh.masses[i] = w >= p.min_p ? fixed(w, p.one) : 0;
+      const uint64_t place = sh.list[i] << 32 | sh.list[i] >> 32;
+      sh.masses[i] = place >= least ? mass(value_of(place)) : 0;
     }
     __syncthreads();
     const uint64_t total = scan(sh.masses, m);
@@ -532,49 +822,48 @@ struct Row {
       if (p.probs) p.probs[at] = (float)((double)(sh.masses[i] - (i ? sh.masses[i - 1] : 0)) / (double)total);
     }
   }
-  // The kept entries are those from `limit` on: sums of segments, then a look through the segment of each draw.
-  __device__ __forceinline__ void draw_row(long long row) {
-    const auto share = [&](float v, int i) -> uint64_t {
-      if (!kept(v, i)) return 0;
-      const double w = weight(v);
-      return w >= p.min_p ? fixed(w, p.one) : 0;
-    };
-    for (int s = warp; s < segments; s += kWarps) {
-      uint64_t sum = 0;
-      for (int c = s * per_segment; c < min((s + 1) * per_segment, chunks); ++c) {
-        float v[8];
-        const int first = fetch(c, v);
+  // The kept entries are those from `limit` on: sums of segments (unless they are there), then a look through the
+  // segment of each draw.
+  __device__ __forceinline__ void draw_row(long long row, bool summed) {
+    const float least = value_of(limit);
+    const bool all = limit == kPossible;
+    if (!summed)
+      for (int s = warp; s < segments; s += kWarps) {
+        const uint64_t sum = segment(s, [&](int first, const E& e) {
+          uint64_t some = 0;
+          if (all || E::value(e.most()) >= least) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += share(v[j], first + j);
+            for (int j = 0; j < kV; ++j) {
+              const float v = e.at(j);
+              if (all || (v >= least && kept(clean(v), first + j))) some += mass(v);
+            }
+          }
+          return some;
+        });
+        if (lane == 0) sh.sums[s] = sum;
       }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) sh.sums[s] = sum;
-    }
     __syncthreads();
     const uint64_t total = scan(sh.sums, segments);
     for (int d = warp; d < p.draws; d += kWarps) {
       const long long at = row * p.draws + d;
       const uint64_t t = threshold(p.uniforms[at], total);
-      const int s = above(sh.sums, segments, t);
+      const int s = above(sh.sums, segments, t), end = min((s + 1) * per_segment, chunks);
       uint64_t sum = s ? sh.sums[s - 1] : 0;
-      for (int c = s * per_segment; c < min((s + 1) * per_segment, chunks); ++c) {
-        float v[8];
-        const int first = fetch(c, v);
-        uint64_t own[8], up = 0;
+      for (int c = s * per_segment; c < end && sum <= t; ++c) {
+        E e;
+        const int first = fetch(c, e);
+        uint64_t own[kV], mine = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) up += own[j] = share(v[j], first + j);
-        const uint64_t mine = up;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint64_t below = __shfl_up_sync(0xffffffffu, up, o);
-          if (lane >= o) up += below;
+        for (int j = 0; j < kV; ++j) {
+          const float v = clean(e.at(j));
+          mine += own[j] = kept(v, first + j) ? mass(v) : 0;
         }
+        const uint64_t up = warp_running(mine, lane);
         uint64_t run = sum + up - mine;
         sum += __shfl_sync(0xffffffffu, up, 31);
         if (run <= t && t < run + mine) {  // one lane
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
+          for (int j = 0; j < kV; ++j) {
             if (run <= t && t < run + own[j]) {
               p.tokens[at] = first + j;
               if (p.probs) p.probs[at] = (float)((double)own[j] / (double)total);
@@ -582,7 +871,6 @@ struct Row {
             run += own[j];
           }
         }
-        if (sum > t) break;
       }
     }
   }
@@ -592,43 +880,50 @@ struct Row {
 constexpr int kSmallK = 256;
 
 template <class T, int THREADS>
-__global__ void __launch_bounds__(THREADS) sample_row_kernel(const __grid_constant__ SampleParams p) {
+__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 2) sample_row_kernel(const __grid_constant__ SampleParams p) {
   may_start_next();
   after_previous();
   extern __shared__ __align__(16) uint8_t smem[];
   auto& sh = *reinterpret_cast<RowShared<THREADS>*>(smem);
   using R = Row<T, THREADS>;
-  if (threadIdx.x < 64) sh.table[threadIdx.x] = exp2(threadIdx.x / 64.0);
-  if (threadIdx.x == 0) sh.listed = 0;
   R r(p, sh, blockIdx.x);
   const bool cut_k = p.top_k < p.classes, cut_p = p.top_p < 1.0;
-  const bool short_list = cut_k && p.top_k <= min(kSmallK, THREADS);
+  const bool small_k = cut_k && p.top_k <= min(kSmallK, THREADS);
   int groups = 1;
-  while (short_list && groups < p.top_k) groups <<= 1;
+  while (small_k && groups < p.top_k) groups <<= 1;
   float bound;
-  r.top = r.largest(groups, bound);
-  if (!possible(r.top)) {
+  const float top = r.largest(groups, bound);
+  if (!possible(top)) {
     r.none(blockIdx.x);
     return;
   }
-  __syncthreads();
-  const bool whole = (cut_k || cut_p) && p.classes <= R::Sh::kList;  // all of the row in the list
-  if (short_list || whole) {
-    const float least = short_list ? bound : __int_as_float(0xff800000);
-    r.each_chunk([&](int first, const float (&v)[8]) {
+  r.set_top(top);
+  const uint64_t least = p.min_p > 0.0 ? r.limit_of_weight(p.min_p) : kPossible;
+  if (small_k || ((cut_k || cut_p) && p.classes <= R::Sh::kList)) {
+    if (!small_k) bound = __int_as_float(0xff800000);
+    r.start_list();
+    r.each_chunk([&](int first, const typename R::E& e) {
+      if (!__any_sync(0xffffffffu, R::E::value(e.most()) >= bound)) return;  // most vectors hold none
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (v[j] >= least && possible(v[j])) r.append(place_of(key_of(v[j]), first + j));
+      for (int j = 0; j < R::kV; ++j) {
+        const float v = clean(e.at(j));
+        r.append(v >= bound && possible(v), v, first + j, R::Sh::kList);
+      }
     });
     __syncthreads();
     if (sh.listed <= R::Sh::kList) {
-      r.draw_listed(blockIdx.x);
+      r.draw_listed(blockIdx.x, least);
       return;
     }
   }
   if (cut_k) r.template narrow<false>(p.top_k, 1.0);
-  if (cut_p) r.template narrow<true>(0, p.top_p);
-  r.draw_row(blockIdx.x);
+  int cut = R::kNot;
+  if (cut_p) {
+    if (!cut_k && !r.far) cut = r.cut_mass(least);
+    if (cut == R::kNot) r.template narrow<true>(0, p.top_p);
+  }
+  r.limit = max(r.limit, least);
+  r.draw_row(blockIdx.x, cut == R::kSummed);
 }
 
 // --------------------------------------------------------------------------------------- host side
@@ -692,6 +987,6 @@ extern "C" int32_t nca_b200_sample(const NcaSampleDesc* d, const void* logits, c
     if (p.classes <= 8) return few<T, 8>(p, s);
     if (p.classes <= 16) return few<T, 16>(p, s);
     if (p.classes <= 32) return few<T, 32>(p, s);
-    return p.classes <= 4096 ? row_blocks<T, 128>(p, s) : row_blocks<T, 512>(p, s);
+    return p.classes <= RowShared<128>::kList ? row_blocks<T, 128>(p, s) : row_blocks<T, 512>(p, s);
   });
 }
