@@ -8,14 +8,15 @@
 // The answers are whole numbers, and a row of 131072 classes has a border every 1e-5 of its mass: weights are computed in
 // 64 bits, so that an answer other than the exact one takes a u within about 1e-13 of a border.  Sums are in fixed
 // point: they do not depend on an order, and a class of no mass is never drawn.  The exponential is table-driven
-// (Tang, ACM TOMS 15, 1989): 2^(j / 256) from a table, e^r of |r| < 0.00136 by three terms, 10 operations in 64 bits with
-// the conversion to fixed point.
+// (Tang, ACM TOMS 15, 1989): 2^(j / 32) from a table, e^r of |r| < 0.0109 by five terms, 12 operations in 64 bits with
+// the conversion to fixed point.  A table of 256 saves two of them and loses more by conflicts of banks (1024 x 131072 without
+// cuts: XXX against YYY us).
 //
 // Up to 32 classes a row is a group of lanes, a class a lane, and ranks are counted.  Longer rows are a block's.  All three
 // cuts keep a prefix of the order, so the kept set is always "from a place (z, index) on".
 //   min_p: the least z of enough weight, by search.
-//   a small top_k: the least of k groups' maxima bounds the k-th largest from below; the few entries above it are listed
-//     and sorted, and everything else happens in the list (as for all rows that fit it).
+//   a small top_k: the k-th largest of 2 k groups' maxima bounds the k-th largest entry from below; the few entries above it
+//     are listed and sorted, and everything else happens in the list (as for all rows that fit it).
 //   top_p alone: a histogram of counts over (top - z) / T bounds the mass before every bin within 0.3 %; one pass then
 //     computes all weights, adds up those surely kept by segment and lists those about the border, which decide.
 //   else: histograms over the ordered bits of z until the entries of the bin with the border can be listed.
@@ -124,7 +125,9 @@ constexpr int kBins = 2048;       // of the ordered bits
 constexpr int kMassBins = 8192;   // of (top - z) / T
 constexpr float kPerBin = 200.f;  // the last holds all beyond 40.9, whose weights are below 2^-58
 constexpr int kSubBins = 256;
+constexpr int kTableBits = 5, kTable = 1 << kTableBits;  // parts of an octave: two addresses a bank
 constexpr int kMostSegments = 1024;
+constexpr int kMostTops = 2048;
 
 // Floats in their order as whole numbers.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -145,7 +148,7 @@ struct RowShared {
   static constexpr int kList = kLong ? 2048 : 1024;      // entries with their masses
   static constexpr int kRegion = kLong ? 4096 : 1024;    // entries alone
   static constexpr int kSegments = kLong ? kMostSegments : 64;
-  double table[256];
+  double table[kTable];
   uint64_t sums[kSegments];
   uint64_t warp_sums[32];
   union {
@@ -162,12 +165,19 @@ struct RowShared {
   };
   uint32_t sub_low[kLong ? kSubBins : 1], sub_high[kLong ? kSubBins : 1];
   float reds[64];
+  float groups[THREADS];                      // their largest entries
+  float chunk_tops[kLong ? kMostTops : 1];    // of the chunks, where there are not more
   uint32_t keys[64];
   int listed, found;
   uint64_t limit;
   long long amount;
 };
 
+__device__ __forceinline__ float warp_max(float v) {  // NaN aside
+  float m;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
 // Adds to a 64-bit sum of two words.
 __device__ __forceinline__ void add_to(uint32_t* low, uint32_t* high, uint64_t m) {
   const uint32_t l = (uint32_t)m, old = atomicAdd(low, l);
@@ -230,9 +240,10 @@ struct Row {
   const SampleParams& p;
   Sh& sh;
   const T* z;
+  const uint4* base;  // this lane's 16 bytes of chunk 0
   int n, shift, chunks, per_segment, segments;  // chunks of a warp's vectors; of a segment
   float top, lowest;      // of the entries; what lies below `lowest` has no mass
-  double steep, offset;   // v steep + offset = 256 log2(e) (v - top) / T
+  double steep, offset;   // v steep + offset = kTable log2(e) (v - top) / T
   bool far;               // ... but for a top whose offset 64 bits round
   uint64_t limit;         // places from here on are kept
   int warp, lane;
@@ -247,52 +258,70 @@ struct Row {
     limit = kPossible;
     warp = threadIdx.x / 32;
     lane = threadIdx.x % 32;
+    base = reinterpret_cast<const uint4*>(z - shift) + lane;
     // a weight of 1 is p.one: sums are in fixed point
-    for (int i = threadIdx.x; i < 256; i += THREADS) sh.table[i] = exp2(i / 256.0) * p.one;
+    if (threadIdx.x < kTable) sh.table[threadIdx.x] = exp2(threadIdx.x / (double)kTable) * p.one;
   }
   __device__ __forceinline__ void set_top(float t) {
     top = t;
-    steep = p.inverse_t * 369.32993046757463;
+    steep = p.inverse_t * (kTable * 1.4426950408889634074);
     offset = -(double)top * steep;
-    far = !(fabs(offset) < 262144.0);
+    far = !(fabs(offset) < 1024.0 * kTable);
     lowest = (float)((double)top - 42.0 / p.inverse_t);  // e^-42 < 2^-60
   }
-  // This lane's entries of a chunk, from entry `first` on; entries outside of the row are -inf.
-  __device__ __forceinline__ int fetch(int chunk, E& e) const {
-    const int first = chunk * kChunk + lane * kV - shift;
-    if (first >= 0 && first + kV <= n) {
-      e.q = *reinterpret_cast<const uint4*>(z + first);
+  // This lane's entries of a chunk; entries outside of the row (in the first and last chunk) are -inf.
+  __device__ __forceinline__ E fetch(int chunk) const {
+    E e;
+    if (chunk > 0 && chunk + 1 < chunks) {
+      e.q = base[chunk * 32];
     } else {
+      const int first = first_of(chunk);
+      if (first >= 0 && first + kV <= n) {
+        e.q = base[chunk * 32];
+      } else {
 #pragma unroll
-      for (int j = 0; j < kV; ++j)
-        e.set(j, first + j >= 0 && first + j < n ? z[first + j] : from_f32<T>(__int_as_float(0xff800000)));
+        for (int j = 0; j < kV; ++j)
+          e.set(j, first + j >= 0 && first + j < n ? z[first + j] : from_f32<T>(__int_as_float(0xff800000)));
+      }
     }
-    return first;
+    return e;
   }
-  // fn(first, entries): chunks in turn over the warps; the next one's load is on its way while one is worked on.
-  template <class F>
+  __device__ __forceinline__ int first_of(int chunk) const { return chunk * kChunk + lane * kV - shift; }
+  // fn(chunk, entries): chunks in turn over the warps, AHEAD of them on their way.
+  template <int AHEAD, class F>
   __device__ __forceinline__ void each_chunk(F fn) const {
-    E next;
-    int at = 0;
-    if (warp < chunks) at = fetch(warp, next);
-    for (int c = warp; c < chunks; c += kWarps) {
-      const E e = next;
-      const int first = at;
-      if (c + kWarps < chunks) at = fetch(c + kWarps, next);
-      fn(first, e);
+    E next[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (warp + i * kWarps < chunks) next[i] = fetch(warp + i * kWarps);
+    for (int c = warp; c < chunks;) {
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        if (c >= chunks) break;
+        const E e = next[i];
+        if (c + AHEAD * kWarps < chunks) next[i] = fetch(c + AHEAD * kWarps);
+        fn(c, e);
+        c += kWarps;
+      }
     }
   }
-  // fn(segment, fn of its chunks): segments in turn over the warps.
-  template <class F>
-  __device__ __forceinline__ uint64_t segment(int s, F fn) const {
-    const int end = min((s + 1) * per_segment, chunks);
-    uint64_t sum = 0;
-    for (int c = s * per_segment; c < end; ++c) {
-      E e;
-      const int first = fetch(c, e);
-      sum += fn(first, e);
+  // Segments in turn over the warps: fn(chunk, entries), and after a segment's chunks done(segment).
+  template <class F, class D>
+  __device__ __forceinline__ void each_segment(F fn, D done) const {
+    if (warp >= segments) return;
+    int s = warp, c = s * per_segment;
+    E next = fetch(c);
+    while (s < segments) {
+      const E e = next;
+      const int here = c, segment = s;
+      if (++c >= min((s + 1) * per_segment, chunks)) {
+        s += kWarps;
+        c = s * per_segment;
+      }
+      if (s < segments) next = fetch(c);
+      fn(here, e);
+      if (s != segment) done(segment);
     }
-    return warp_sum(sum);
   }
   __device__ __forceinline__ bool kept(float v, int i) const { return place_of(key_of(v), i) >= limit; }  // of a clean v
 
@@ -306,15 +335,17 @@ struct Row {
     } else {
       if (v == top) return p.one;  // also of infinities
       x = ((double)v - (double)top) * steep;
-      if (!(x > -16000.0)) return 0.0;
+      if (!(x > -62.0 * kTable)) return 0.0;
     }
     const double m = x + kMagic;
     const int k = __double2loint(m);
     const double r = x - (m - kMagic);
-    constexpr double c = 0.0027076061740622863;  // ln(2) / 256
-    const double q = r * (c + r * (c * c / 2 + r * (c * c * c / 6)));
-    const double t = sh.table[k & 255], e = fma(t, q, t);
-    return __hiloint2double(__double2hiint(e) + ((k & ~255) << 12), __double2loint(e));
+    // e^(c r) - 1 of |c r| < 0.0109, to 3e-15
+    constexpr double c = 0.69314718055994530942 / kTable;
+    constexpr double c2 = c * c / 2, c3 = c2 * c / 3, c4 = c3 * c / 4, c5 = c4 * c / 5;
+    const double q = r * (c + r * (c2 + r * (c3 + r * (c4 + r * c5))));
+    const double t = sh.table[k & (kTable - 1)], e = fma(t, q, t);
+    return __hiloint2double(__double2hiint(e) + (k >> kTableBits << 20), __double2loint(e));
   }
   __device__ __forceinline__ double weight(float v) const { return far ? weight_of<true>(v) : weight_of<false>(v); }
   __device__ __forceinline__ uint64_t mass(float v) const { return fixed(weight(v), 1.0); }
@@ -358,8 +389,20 @@ struct Row {
     }
     return lo;
   }
-  // The list, filled up to a power of two, to descending order.
+  // The list to descending order: a few entries by counting the larger ones, else filled up to a power of two.
   __device__ __forceinline__ void sort(int count) {
+    if (count <= min(THREADS, 256)) {
+      uint64_t mine = 0;
+      int rank = 0;
+      if (threadIdx.x < (count + 31) / 32 * 32) {
+        mine = threadIdx.x < count ? sh.list[threadIdx.x] : 0;
+        for (int i = 0; i < count; ++i) rank += sh.list[i] > mine;
+      }
+      __syncthreads();
+      if (threadIdx.x < count) sh.list[rank] = mine;
+      __syncthreads();
+      return;
+    }
     int size = 2;
     while (size < count) size <<= 1;
     for (int i = count + threadIdx.x; i < size; i += THREADS) sh.list[i] = 0;
@@ -396,39 +439,60 @@ struct Row {
     __syncthreads();
   }
 
-  // The largest entry; with `groups` (a power of two, at most THREADS) also a bound that so many entries reach.
-  __device__ __forceinline__ float largest(int groups, float& bound) {
+  // The largest entry, and those of the chunks.  k > 0: also a bound that k entries reach, the k-th largest of the largest
+  // entries of `groups` groups (a power of two, at most THREADS, and at least k).
+  __device__ __forceinline__ float largest(int k, int groups, float& bound) {
+    const float least = __int_as_float(0xff800000);
     E none;
 #pragma unroll
-    for (int j = 0; j < kV; ++j) none.set(j, from_f32<T>(__int_as_float(0xff800000)));
+    for (int j = 0; j < kV; ++j) none.set(j, from_f32<T>(least));
     uint32_t most = none.q.x;
-    each_chunk([&](int, const E& e) { most = E::max2(most, e.most()); });
+    each_chunk<4>([&](int chunk, const E& e) {
+      const uint32_t m = e.most();
+      most = E::max2(most, m);
+      if (Sh::kLong) {
+        const float t = warp_max(E::value(m));
+        if (lane == 0 && chunk < kMostTops) sh.chunk_tops[chunk] = t;
+      }
+    });
     float m = E::value(most);
     const int wide = THREADS / groups;  // threads of a group
     for (int o = 1; o < min(wide, 32); o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float least = m;
-    for (int o = min(wide, 32); o < 32; o <<= 1) {
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
-    }
+    sh.groups[threadIdx.x] = m;
+    m = warp_max(m);
+    if (lane == 0) sh.reds[warp] = m;
     __syncthreads();
-    if (lane == 0) {
-      sh.reds[warp] = m;
-      sh.reds[32 + warp] = least;
-    }
-    __syncthreads();
-    const int warps = max(wide / 32, 1);  // of a group
-    bound = __int_as_float(0x7f800000);
-    for (int g = 0; g < kWarps; g += warps) {
-      float first = __int_as_float(0xff800000);
-      if (warps == 1) first = sh.reds[32 + g];
-      else
-        for (int w = 0; w < warps; ++w) first = fmaxf(first, sh.reds[g + w]);
-      bound = fminf(bound, first);
-    }
     m = sh.reds[0];
     for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh.reds[w]);
+    if (k > 0) {
+      if (threadIdx.x < groups) {
+        const auto of_group = [&](int g) {
+          float f = sh.groups[g * wide];
+          for (int i = 32; i < wide; i += 32) f = fmaxf(f, sh.groups[g * wide + i]);
+          return f;
+        };
+        const float mine = of_group(threadIdx.x);
+        int before = 0;  // in the order of the groups
+        for (int g = 0; g < groups; ++g) {
+          const float f = of_group(g);
+          before += f > mine || (f == mine && g < threadIdx.x);
+        }
+        if (before == k - 1) sh.reds[32] = mine;
+      }
+      __syncthreads();
+      bound = sh.reds[32];
+    }
     return m;
+  }
+  // Whether a chunk can hold entries from `least` on.
+  __device__ __forceinline__ bool reaches(int chunk, float least) const {
+    return !Sh::kLong || chunk >= kMostTops || sh.chunk_tops[chunk] >= least;
+  }
+  // fn(chunk, entries) of those chunks, in turn over the warps.
+  template <class F>
+  __device__ __forceinline__ void each_reaching(float least, F fn) const {
+    for (int c = warp; c < chunks; c += kWarps)
+      if (reaches(c, least)) fn(c, fetch(c));
   }
 
   // The least place of a weight of min_p, by a search of 32 keys at a time (every warp for itself).
@@ -474,7 +538,7 @@ struct Row {
       for (int i = threadIdx.x; i < kSubBins; i += THREADS) sh.sub_low[i] = sh.sub_high[i] = 0;
       if (threadIdx.x < 8) sh.keys[threadIdx.x] = kMassBins - 1;
       __syncthreads();
-      each_chunk([&](int, const E& e) {
+      each_chunk<2>([&](int, const E& e) {
 #pragma unroll
         for (int j = 0; j < kV; ++j) {  // to nearest, by the bits of a sum with 2^23; NaN to the last
           const uint32_t b = __float_as_uint(fmaf(top - e.at(j), scale, 8388608.f)) - 0x4b000000u;
@@ -539,8 +603,8 @@ struct Row {
         __syncthreads();
         return kCut;
       }
-      // as many entries about the likely one as the list holds
-      const int room = Sh::kRegion / 2 - 64, centre = (int)sh.amount;
+      // so many entries about the likely one
+      const int room = Sh::kRegion / 4, centre = (int)sh.amount;
       c = before;
       uint32_t low_bin = kMassBins - 1, high_bin = 0;
       for (int i = 0; i < kPer; ++i) {
@@ -564,23 +628,30 @@ struct Row {
       if (from > to || to >= kMassBins - 1) return kNot;
       const float high = top - (from - 0.5f) / scale, low = top - (to + 0.5f) / scale;  // the list: low < v <= high
       __syncthreads();  // the list takes the counts' place
-      uint64_t sure_sum = 0, all = 0;
-      for (int s = warp; s < segments; s += kWarps) {
-        const uint64_t sum = segment(s, [&](int first, const E& e) {
-          uint64_t some = 0;
+      uint64_t sure_sum = 0, all = 0, some = 0;
+      each_segment(
+          [&](int chunk, const E& e) {
+            unsigned about = 0;
 #pragma unroll
-          for (int j = 0; j < kV; ++j) {
-            const float v = e.at(j);
-            const uint64_t m = near_mass(v);
-            all += m;
-            some += v > high ? m : 0;
-            append(v <= high && v > low, v, first + j, Sh::kRegion);
-          }
-          return some;
-        });
-        sure_sum += sum;
-        if (lane == 0) sh.sums[s] = sum;
-      }
+            for (int j = 0; j < kV; ++j) {
+              const float v = e.at(j);
+              const uint64_t m = near_mass(v);
+              all += m;
+              if (v > high) some += m;
+              else if (v > low) about |= 1u << j;
+            }
+            while (__any_sync(0xffffffffu, about)) {  // few lanes, and of those the most have one
+              const int i = first_of(chunk) + __ffs(about) - 1;
+              append(about != 0, about ? to_f32<T>(z[i]) : 0.f, i, Sh::kRegion);
+              about &= about - 1;
+            }
+          },
+          [&](int s) {
+            some = warp_sum(some);
+            sure_sum += some;
+            if (lane == 0) sh.sums[s] = some;
+            some = 0;
+          });
       sure_sum = block_sum(sure_sum);
       all = block_sum(warp_sum(all));
       const int listed = sh.listed;
@@ -622,10 +693,9 @@ struct Row {
       const int border = sh.found;
       const uint64_t reached = sh.limit;
       if (border < 0) return kNot;  // not about the likely place
-      const int per = kChunk * per_segment;
       const auto join = [&](uint64_t place, uint64_t m) {
-        if (place >= least)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sums[(index_of(place) + shift) / per]), (unsigned long long)m);
+        const unsigned chunk = (unsigned)(index_of(place) + shift) / kChunk, s = per_segment == 1 ? chunk : chunk / per_segment;
+        if (place >= least) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sums[s]), (unsigned long long)m);
       };
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
@@ -663,8 +733,8 @@ struct Row {
         for (int i = threadIdx.x; i < kBins; i += THREADS) sh.counts[i] = sh.low[i] = sh.high[i] = 0;
         __syncthreads();
         const float bottom = of_key(lo), ceiling = of_key(hi);
-        each_chunk([&](int first, const E& e) {
-          if (!(E::value(e.most()) >= bottom)) return;
+        each_reaching(bottom, [&](int chunk, const E& e) {
+          const int first = first_of(chunk);
 #pragma unroll
           for (int j = 0; j < kV; ++j) {
             const float v = clean(e.at(j));
@@ -728,7 +798,8 @@ struct Row {
       // the entries of the bin with the border, sorted
       start_list();
       const float bottom = of_key(lo), ceiling = of_key(hi);
-      each_chunk([&](int first, const E& e) {
+      each_reaching(bottom, [&](int chunk, const E& e) {
+        const int first = first_of(chunk);
 #pragma unroll
         for (int j = 0; j < kV; ++j) {
           const float v = clean(e.at(j));
@@ -746,7 +817,7 @@ struct Row {
   // The limit that keeps the first `ties` entries of a key (and all larger ones).
   __device__ __forceinline__ void nth_tie(uint32_t key, long long ties) {
     const auto count_in = [&](int first, const E& e) {
-      uint64_t count = 0;
+      int count = 0;
 #pragma unroll
       for (int j = 0; j < kV; ++j) {
         const float v = clean(e.at(j));
@@ -754,10 +825,13 @@ struct Row {
       }
       return count;
     };
-    for (int s = warp; s < segments; s += kWarps) {
-      const uint64_t count = segment(s, count_in);
-      if (lane == 0) sh.sums[s] = count;
-    }
+    uint64_t some = 0;
+    each_segment([&](int chunk, const E& e) { some += count_in(first_of(chunk), e); },
+                 [&](int s) {
+                   some = warp_sum(some);
+                   if (lane == 0) sh.sums[s] = some;
+                   some = 0;
+                 });
     __syncthreads();
     if (warp == 0) {
       long long left = ties;
@@ -765,9 +839,9 @@ struct Row {
       while (s < segments - 1 && (long long)sh.sums[s] < left) left -= (long long)sh.sums[s++];
       int at = -1;
       for (int c = s * per_segment; c < min((s + 1) * per_segment, chunks) && at < 0; ++c) {
-        E e;
-        const int first = fetch(c, e);
-        const int mine = (int)count_in(first, e), up = warp_running(mine, lane);
+        const E e = fetch(c);
+        const int first = first_of(c);
+        const int mine = count_in(first, e), up = warp_running(mine, lane);
         if (up - mine < left && up >= left) {
           long long k = left - (up - mine);
 #pragma unroll
@@ -827,20 +901,31 @@ struct Row {
   __device__ __forceinline__ void draw_row(long long row, bool summed) {
     const float least = value_of(limit);
     const bool all = limit == kPossible;
-    if (!summed)
-      for (int s = warp; s < segments; s += kWarps) {
-        const uint64_t sum = segment(s, [&](int first, const E& e) {
-          uint64_t some = 0;
-          if (all || E::value(e.most()) >= least) {
+    uint64_t some = 0;
+    const auto done = [&](int s) {
+      some = warp_sum(some);
+      if (lane == 0) sh.sums[s] = some;
+      some = 0;
+    };
+    if (!summed && all && !far)
+      each_segment(
+          [&](int, const E& e) {
 #pragma unroll
-            for (int j = 0; j < kV; ++j) {
-              const float v = e.at(j);
-              if (all || (v >= least && kept(clean(v), first + j))) some += mass(v);
-            }
+            for (int j = 0; j < kV; ++j) some += near_mass(e.at(j));
+          },
+          done);
+    else if (!summed)
+      for (int s = warp; s < segments; s += kWarps) {
+        for (int c = s * per_segment; c < min((s + 1) * per_segment, chunks); ++c) {
+          if (!reaches(c, least)) continue;
+          const E e = fetch(c);
+#pragma unroll
+          for (int j = 0; j < kV; ++j) {
+            const float v = clean(e.at(j));
+            if (v >= least && kept(v, first_of(c) + j)) some += mass(v);
           }
-          return some;
-        });
-        if (lane == 0) sh.sums[s] = sum;
+        }
+        done(s);
       }
     __syncthreads();
     const uint64_t total = scan(sh.sums, segments);
@@ -850,8 +935,8 @@ struct Row {
       const int s = above(sh.sums, segments, t), end = min((s + 1) * per_segment, chunks);
       uint64_t sum = s ? sh.sums[s - 1] : 0;
       for (int c = s * per_segment; c < end && sum <= t; ++c) {
-        E e;
-        const int first = fetch(c, e);
+        const E e = fetch(c);
+        const int first = first_of(c);
         uint64_t own[kV], mine = 0;
 #pragma unroll
         for (int j = 0; j < kV; ++j) {
@@ -876,7 +961,7 @@ struct Row {
   }
 };
 
-// A k up to this is found through the groups' maxima: k groups leave about k ln k entries.
+// A k up to this is found through groups: the k-th largest of 2 k maxima or more leaves about 1.4 k entries.
 constexpr int kSmallK = 256;
 
 template <class T, int THREADS>
@@ -888,11 +973,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 2) sample_row_ke
   using R = Row<T, THREADS>;
   R r(p, sh, blockIdx.x);
   const bool cut_k = p.top_k < p.classes, cut_p = p.top_p < 1.0;
-  const bool small_k = cut_k && p.top_k <= min(kSmallK, THREADS);
+  const bool small_k = cut_k && p.top_k <= min(kSmallK, THREADS / 2);
   int groups = 1;
-  while (small_k && groups < p.top_k) groups <<= 1;
-  float bound;
-  const float top = r.largest(groups, bound);
+  while (small_k && groups < 2 * p.top_k) groups <<= 1;
+  float bound = __int_as_float(0xff800000);
+  const float top = r.largest(small_k ? p.top_k : 0, groups, bound);
   if (!possible(top)) {
     r.none(blockIdx.x);
     return;
@@ -900,10 +985,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 2) sample_row_ke
   r.set_top(top);
   const uint64_t least = p.min_p > 0.0 ? r.limit_of_weight(p.min_p) : kPossible;
   if (small_k || ((cut_k || cut_p) && p.classes <= R::Sh::kList)) {
-    if (!small_k) bound = __int_as_float(0xff800000);
     r.start_list();
-    r.each_chunk([&](int first, const typename R::E& e) {
-      if (!__any_sync(0xffffffffu, R::E::value(e.most()) >= bound)) return;  // most vectors hold none
+    r.each_reaching(bound, [&](int chunk, const typename R::E& e) {
+      const int first = r.first_of(chunk);
 #pragma unroll
       for (int j = 0; j < R::kV; ++j) {
         const float v = clean(e.at(j));
