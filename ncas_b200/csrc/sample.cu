@@ -10,7 +10,7 @@
 // point: they do not depend on an order, and a class of no mass is never drawn.  The exponential is table-driven
 // (Tang, ACM TOMS 15, 1989): 2^(j / 32) from a table, e^r of |r| < 0.0109 by five terms, 12 operations in 64 bits with
 // the conversion to fixed point.  A table of 256 saves two of them and loses more by conflicts of banks (1024 x 131072 without
-// cuts: XXX against YYY us).
+// cuts: 232 against 216 us).
 //
 // Up to 32 classes a row is a group of lanes, a class a lane, and ranks are counted.  Longer rows are a block's.  All three
 // cuts keep a prefix of the order, so the kept set is always "from a place (z, index) on".
@@ -139,6 +139,15 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 __device__ __forceinline__ uint64_t place_of(uint32_t key, int i) { return (uint64_t)key << 32 | (0xffffffffu - (uint32_t)i); }
 __device__ __forceinline__ int index_of(uint64_t place) { return (int)(0xffffffffu - (uint32_t)place); }
 __device__ __forceinline__ float value_of(uint64_t place) { return of_key((uint32_t)(place >> 32)); }
+// 2^(j / kTable)
+__constant__ double kPowers[kTable] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484,
+    1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407,
+    1.5759808451078865, 1.6104903319492543, 1.645755478153965, 1.681792830507429, 1.718619298122478,
+    1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474,
+    1.9571441241754002};
 constexpr uint64_t kPossible = 0x00800000ull << 32;  // the places above -inf
 
 // Blocks of 128 threads serve rows that the list holds whole.
@@ -260,7 +269,7 @@ struct Row {
     lane = threadIdx.x % 32;
     base = reinterpret_cast<const uint4*>(z - shift) + lane;
     // a weight of 1 is p.one: sums are in fixed point
-    if (threadIdx.x < kTable) sh.table[threadIdx.x] = exp2(threadIdx.x / (double)kTable) * p.one;
+    if (threadIdx.x < kTable) sh.table[threadIdx.x] = kPowers[threadIdx.x] * p.one;
   }
   __device__ __forceinline__ void set_top(float t) {
     top = t;
@@ -488,11 +497,22 @@ struct Row {
   __device__ __forceinline__ bool reaches(int chunk, float least) const {
     return !Sh::kLong || chunk >= kMostTops || sh.chunk_tops[chunk] >= least;
   }
-  // fn(chunk, entries) of those chunks, in turn over the warps.
+  // fn(chunk, entries) of those chunks, in turn over the warps; the next one is on its way.
   template <class F>
   __device__ __forceinline__ void each_reaching(float least, F fn) const {
-    for (int c = warp; c < chunks; c += kWarps)
-      if (reaches(c, least)) fn(c, fetch(c));
+    for (int c0 = warp; c0 < chunks; c0 += 32 * kWarps) {
+      const int mine = c0 + lane * kWarps;
+      unsigned which = __ballot_sync(0xffffffffu, mine < chunks && reaches(mine, least));
+      if (!which) continue;
+      E next = fetch(c0 + (__ffs(which) - 1) * kWarps);
+      while (which) {
+        const E e = next;
+        const int c = c0 + (__ffs(which) - 1) * kWarps;
+        which &= which - 1;
+        if (which) next = fetch(c0 + (__ffs(which) - 1) * kWarps);
+        fn(c, e);
+      }
+    }
   }
 
   // The least place of a weight of min_p, by a search of 32 keys at a time (every warp for itself).
@@ -965,7 +985,7 @@ struct Row {
 constexpr int kSmallK = 256;
 
 template <class T, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 128 ? 8 : 2) sample_row_kernel(const __grid_constant__ SampleParams p) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_row_kernel(const __grid_constant__ SampleParams p) {
   may_start_next();
   after_previous();
   extern __shared__ __align__(16) uint8_t smem[];
@@ -1071,6 +1091,10 @@ extern "C" int32_t nca_b200_sample(const NcaSampleDesc* d, const void* logits, c
     if (p.classes <= 8) return few<T, 8>(p, s);
     if (p.classes <= 16) return few<T, 16>(p, s);
     if (p.classes <= 32) return few<T, 32>(p, s);
-    return p.classes <= RowShared<128>::kList ? row_blocks<T, 128>(p, s) : row_blocks<T, 512>(p, s);
+    // Smaller blocks, more rows at once, hide each other's short steps (2047 x 32003 fp16, top-k 50: 101 against 141 us); top-p
+    // alone has few of them and works through its list faster in large ones (348 against 432 us, top-p 0.95).
+    if (p.classes <= RowShared<128>::kList) return row_blocks<T, 128>(p, s);
+    const bool by_mass = p.top_p < 1.0 && p.top_k == p.classes;
+    return p.classes <= 65536 && !by_mass ? row_blocks<T, 256>(p, s) : row_blocks<T, 512>(p, s);
   });
 }
