@@ -9,9 +9,11 @@
 // as hi + lo, two fp16 values of 22 bits together: a X amplifies what is left in the small singular
 // directions by a at every step, and with X in 11 bits that would be rounding noise (6 % of the result
 // for a matrix of rank 1).  The products read hi alone: their errors appear only beside large singular values,
-// which nothing amplifies, and later steps mend most of what earlier ones leave.  A bf16 result has 1.1 to 1.25 times the
-// error of its rounding alone; a fp16 result would have 8 times, so there the operands of the last three steps' products
-// have 22 bits, hi hi + hi lo + lo hi (2.2 times the operations, and an error of 1.05 times the rounding's).
+// which nothing amplifies.  What a step leaves once the singular values have arrived stays, though: 1.0e-3 to 1.5e-3 of
+// the result's norm a step, beside the 1.7e-3 of its own rounding to bf16 (2e-4 to fp16).  They have arrived
+// about log(sqrt(rows)) / log(a) steps from the start, so of a bf16 matrix the steps beyond the first three from there on (5
+// steps: matrices of fewer than 140 rows) read B and X in 22 bits in the largest product, hi hi + hi lo + lo hi, and of a
+// fp16 matrix all of them in all three products.  Errors are then 1.0 to 1.4 times the rounding's.
 //
 // A and A^2 are symmetric: tiles above the diagonal are computed, and stored twice.
 //
@@ -593,6 +595,14 @@ int32_t check_desc(const NcaOrthoDesc* d) {
   return NCA_OK;
 }
 
+// How many of the last steps take operands of 22 bits.
+int precise_steps(const NcaOrthoDesc& d) {
+  const double small = (double)std::max<int64_t>(1, std::min(d.rows, d.cols)), a = std::fabs(d.coefficients[0]);
+  const double arrived = a > 1.05 ? std::max(0.0, d.steps - 0.5 * std::log(small) / std::log(a)) : d.steps;
+  if (d.dtype == NCA_F16) return (int)std::min<double>(d.steps, std::ceil(arrived));
+  return arrived <= 3.0 ? 0 : (int)std::ceil(arrived - 1.2);
+}
+
 struct Plan {
   long long small, pitch, small_pitch;
   bool tall;
@@ -615,7 +625,7 @@ Plan plan_of(const NcaOrthoDesc& d) {
   for (int i = 0; i < 2; ++i) {
     p.a[i] = at;
     p.b[i] = at + a;
-    if (i == 0 || d.dtype == NCA_F16) at += 2 * a;
+    if (i == 0 || precise_steps(d) > 0) at += 2 * a;
   }
   p.part = at;
   p.parts = (int)std::max<long long>(1, std::min<long long>(ceil_div(d.rows * d.cols, 4096), ceil_div(592, d.batch ? d.batch : 1)));
@@ -686,9 +696,9 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
   p.out_bf16 = d->dtype == NCA_BF16;
   for (int k = 0; k < d->steps; ++k) {
     const Stack x[2] = {x_of(k & 1, 0), x_of(k & 1, 1)};
-    const bool last = k + 1 == d->steps, precise = d->dtype == NCA_F16 && k + 3 >= d->steps;
-    p.passes = precise ? 3 : 1;
-    p.pair = precise;
+    const bool last = k + 1 == d->steps, precise = k + precise_steps(*d) >= d->steps, all = precise && d->dtype == NCA_F16;
+    p.passes = all ? 3 : 1;
+    p.pair = all;
     p.m = p.n = (int)pl.small;
     p.symmetric = 1;
     p.kb = (int)ceil_div(std::max(d->rows, d->cols), kBK);
@@ -701,16 +711,19 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
     NCA_TRY((pl.tall ? product<true, true, STEP_POWER>(p, x, x, s) : product<false, false, STEP_POWER>(p, x, x, s)));
 
     p.kb = (int)ceil_div(pl.small, kBK);
-    p.terms = 1 + p.pair;
+    p.terms = 1 + all;
+    p.pair = precise;
     p.alpha = (float)(c2 * scale_b / ((double)kScaleA * kScaleA));
     p.beta = (float)(c1 * scale_b / kScaleA);
-    for (int i = 0; i <= p.pair; ++i)
-      if (!encode_places(&p.src[i], a_of[i]) || !encode_places(&p.out[i], b_of[i])) return NCA_ERR_CUDA;
+    for (int i = 0; i < 2; ++i)
+      if ((i < p.terms && !encode_places(&p.src[i], a_of[i])) || (i <= p.pair && !encode_places(&p.out[i], b_of[i])))
+        return NCA_ERR_CUDA;
     NCA_TRY((product<false, false, STEP_POWER>(p, a_of, a_of, s)));
 
     p.m = (int)d->rows;
     p.n = (int)d->cols;
     p.symmetric = 0;
+    p.passes = precise ? 3 : 1;
     p.terms = 2;
     p.pair = !last;
     p.last = last;

@@ -135,21 +135,26 @@ def gated_scan(x, gate, state=None, dim=-2, reverse=False, mask=None, dy=None, d
 
 def orthogonalize(m, steps=5, coefficients=(3.4445, -4.775, 2.0315), eps=1e-7, rounded=False):
     """Newton-Schulz steps of a stack of matrices.  rounded: with the roundings to fp16 that the library's
-    kernels document (operands X 2^12, A 2^10, B 2^10; X itself, and of fp16 matrices the operands of the last three
-    steps, as two fp16 values), everything else exact."""
+    kernels document (operands X 2^12, A 2^10, B 2^10; X itself, and the operands of the last steps, as two fp16 values),
+    everything else exact."""
     a, b, c = coefficients
     once = lambda t, s: (t * s).half().double() / s if rounded else t  # noqa: E731
     twice = lambda t, s: once(t, s) + once(t - once(t, s), s) if rounded else t  # noqa: E731
+    full = m.dtype == torch.float16
+    arrived = max(0.0, steps - 0.5 * math.log(max(1, min(m.shape[-2:]))) / math.log(abs(a))) if abs(a) > 1.05 else steps
+    precise = min(steps, math.ceil(arrived)) if full else 0 if arrived <= 3 else math.ceil(arrived - 1.2)
     out = []
     for x in m.double().reshape(-1, *m.shape[-2:]):
         x = x / (x.square().sum().sqrt() + eps)
         if x.shape[0] > x.shape[1]:
             x = x.T
         for k in range(steps):
-            operand = twice if m.dtype == torch.float16 and k + 3 >= steps else once
-            y, x = operand(x, 4096.0), twice(x, 4096.0)
-            p = operand(y @ y.T, 1024.0)
-            x = a * x + operand(b * p + c * (p @ p), 1024.0) @ y
+            late = k + precise >= steps
+            early = twice if late and full else once
+            y, x = early(x, 4096.0), twice(x, 4096.0)
+            p = early(y @ y.T, 1024.0)
+            q = (twice if late else once)(b * p + c * (p @ p), 1024.0)
+            x = a * x + q @ (x if late else y)
         out.append(x.T if m.shape[-2] > m.shape[-1] else x)
     return torch.stack(out).reshape(m.shape)
 
