@@ -15,7 +15,9 @@
 // steps: matrices of fewer than 140 rows) read B and X in 22 bits in the largest product, hi hi + hi lo + lo hi, and of a
 // fp16 matrix all of them in all three products.  Errors are then 1.0 to 1.4 times the rounding's.
 //
-// A and A^2 are symmetric: tiles above the diagonal are computed, and stored twice.
+// A and A^2 are symmetric: tiles above the diagonal are computed, and stored twice.  Where a product has few tiles, a
+// cluster of 2 or 4 CTAs shares the k axis of each: every CTA adds up a share of the tile's columns through distributed
+// shared memory and stores it.
 //
 // One product kernel, built as gemm.cuh's: a persistent CTA or CTA pair (cta_group::2) a multiprocessor, warp 0
 // loads tiles by TMA, warp 1 issues the MMAs, warps 4-11 take the accumulators out, add the terms that they load by
@@ -58,6 +60,7 @@ struct OrthoParams {
   CUtensorMap out[2];
   int m, n;  // of D
   int m_tiles, n_tiles, batch, kb;
+  int slices;  // SPLIT: CTAs that share a tile's k axis, 2 or 4
   int passes;  // over the k axis: 1, or 3 (hi hi, hi lo, lo hi)
   int pair;    // the output as hi + lo
   int symmetric;
@@ -134,10 +137,21 @@ __device__ __forceinline__ OrthoTile tile_at(const OrthoParams& p, int per, int 
   return r;
 }
 
+// A lane's row of a place (put_row's layout) in another block's shared memory.
+__device__ __forceinline__ void put_remote(uint32_t place, int lane, const uint4 (&v)[4]) {
+  const uint32_t row = place + 64 * lane, x = 16 * ((lane >> 1) & 3);
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((16 * j) ^ x)), "r"(v[j].x), "r"(v[j].y),
+                 "r"(v[j].z), "r"(v[j].w)
+                 : "memory");
+}
+
 template <int CG, int BN>
 using OrthoShape = GemmShape<CG, BN, EPI_DGATE>;  // four places an epilogue warp
 
-template <int CG, int BN, bool A_MN, bool B_MN, int STEP>
+// SPLIT (CG = 1): a cluster of p.slices CTAs works on one tile.
+template <int CG, int BN, bool A_MN, bool B_MN, int STEP, bool SPLIT>
 __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_constant__ OrthoParams p) {
   using S = OrthoShape<CG, BN>;
   extern __shared__ uint8_t smem_raw[];
@@ -152,7 +166,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
   volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_base_s + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 1 ? 0 : cta_rank_in_cluster();
+  const uint32_t rank = CG == 1 ? 0 : cta_rank_in_cluster(), slice = SPLIT ? cta_rank_in_cluster() : 0;
   const FailState fs{p.ctrl, abort_s, 0, p.timeout_ns, true};
 
   if (threadIdx.x == 0) {
@@ -170,6 +184,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
     fence_mbar_init();
   }
   if (warp == 2) tc_alloc<CG>(tmem_base_s, S::kTmemCols);
+  if (warp == 3 && lane < 8) {  // the maps come while the kernel before ends
+    const CUtensorMap* map = lane < 2 ? &p.a[lane] : lane < 4 ? &p.b[lane - 2] : lane < 6 ? &p.src[lane - 4] : &p.out[lane - 6];
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  }
   may_start_next();
   after_previous();
   tc_fence_before();
@@ -179,7 +197,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
   const uint32_t tmem = *tmem_base_s;
 
   const int per = tiles_of(p, kBM * CG, BN), tiles = per * p.batch;
-  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int width = SPLIT ? p.slices : CG, first = blockIdx.x / width, step = gridDim.x / width;
+  // this CTA's part of the k axis
+  const int blocks = p.kb * p.passes, from = SPLIT ? blocks * (int)slice / p.slices : 0;
+  const int to = SPLIT ? blocks * ((int)slice + 1) / p.slices : blocks;
+
+  // SPLIT: two meetings of the cluster.  After the first all MMAs have ended and the rings are free, after the second the
+  // shares have arrived.  Every warp comes to both, whatever failed.
+  const int share = SPLIT ? BN / p.slices : BN;
+  const uint32_t ring = smem_u32(smem);
+  bool first_met = false, met = false;
+  const auto meet = [&] {
+    __syncwarp();
+    cluster_started_arrive();
+    cluster_started_wait();
+    first_met = true;
+  };
+  const auto part_of = [&](int from_slice, int q, int c) { return (from_slice * 4 + q) * (share / 16) + c / 16; };
 
   if (warp == 0) {
     if (lane == 0) {
@@ -190,7 +224,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
       for (int t = first; t < tiles && ok; t += step) {
         const OrthoTile tl = tile_at<kBM * CG, BN>(p, per, t);
         const int am = tl.m0 + (int)rank * kBM, bn = tl.n0 + (int)rank * S::kBNc;
-        for (int kb = 0, pass = 0; pass < p.passes; kb + 1 < p.kb ? ++kb : (kb = 0, ++pass)) {
+        for (int i = from, pass = from / p.kb, kb = from - pass * p.kb; i < to; ++i, kb + 1 < p.kb ? ++kb : (kb = 0, ++pass)) {
           const CUtensorMap *ma = &p.a[pass == 2], *mb = &p.b[pass == 1];
           if (!mbar_wait(&empty[s], ph ^ 1, fs, 111)) {
             ok = false;
@@ -202,13 +236,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
           const int k0 = kb * kBK;
           if constexpr (A_MN) {
 #pragma unroll
-            for (int i = 0; i < kBM / 64; ++i) load_tile<CG>(sa + i * 8192, ma, bar, am + 64 * i, k0, tl.z);
+            for (int j = 0; j < kBM / 64; ++j) load_tile<CG>(sa + j * 8192, ma, bar, am + 64 * j, k0, tl.z);
           } else {
             load_tile<CG>(sa, ma, bar, k0, am, tl.z);
           }
           if constexpr (B_MN) {
 #pragma unroll
-            for (int i = 0; i < S::kBNc / 64; ++i) load_tile<CG>(sb + i * 8192, mb, bar, bn + 64 * i, k0, tl.z);
+            for (int j = 0; j < S::kBNc / 64; ++j) load_tile<CG>(sb + j * 8192, mb, bar, bn + 64 * j, k0, tl.z);
           } else {
             load_tile<CG>(sb, mb, bar, k0, bn, tl.z);
           }
@@ -240,7 +274,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
         }
         tc_fence_after();
         const uint32_t d = tmem + buf * BN;
-        for (int kb = 0; kb < p.kb * p.passes; ++kb) {
+        for (int kb = from; kb < to; ++kb) {
           if (!mbar_wait(&full[s], ph, fs, 113)) {
             ok = false;
             break;
@@ -250,7 +284,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
           const uint64_t da = smem_desc(sa, A_MN ? 8192 : 16, 1024);
           const uint64_t db = smem_desc(sb, B_MN ? 8192 : 16, 1024);
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) umma_ss<CG>(d, da + k * a_step, db + k * b_step, idesc, kb > 0 || k > 0);
+          for (int k = 0; k < kBK / 16; ++k) umma_ss<CG>(d, da + k * a_step, db + k * b_step, idesc, kb > from || k > 0);
           tc_commit<CG>(&empty[s]);
           if (++s == S::kStages) {
             s = 0;
@@ -288,12 +322,28 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
         }
       };
       const bool asks = p.terms > 0 && rows;
-      if (asks && 32 * turn < cols) ask(32 * turn);
+      const int asked = (SPLIT ? slice * share : 0) + 32 * turn, end = SPLIT ? min(cols, (int)slice * share + share) : cols;
+      if (asks && asked < end) ask(asked);
       ok = mbar_wait_warp(&acc_full[buf], ph, fs, 114);
       if (!ok) break;
       tc_fence_after();
       const uint32_t acc = tmem + buf * BN + ((uint32_t)(32 * q) << 16);
-      for (int c = 32 * turn; c < cols && rows; c += 64) {
+      if constexpr (SPLIT) {  // the others' shares of the columns to them, 16 columns a place, into their rings
+        meet();
+        for (int c = 16 * turn; c < BN; c += 32) {
+          const uint32_t owner = c / share;
+          if (owner == slice) continue;
+          uint32_t r[16];
+          tmem_take16(acc + c, r);
+          uint4 v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+          put_remote(map_to_rank(ring + part_of(slice, q, c - owner * share) * kPlace, owner), lane, v);
+        }
+        cluster_sync_all();
+        met = true;
+      }
+      for (int c = asked; c < end && rows; c += 64) {
         const int col = tl.n0 + c;
         float f[32];
         if (asks) {
@@ -307,7 +357,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
           // every lane's reads come before the copy that overwrites them
           fence_async_proxy();
           __syncwarp();
-          if (c + 64 < cols) ask(c + 64);
+          if (c + 64 < end) ask(c + 64);
           unpack_half(k0, f);
           if (p.terms == 2) {
             float lo[32];
@@ -321,6 +371,21 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
         }
         uint32_t r[32];
         tmem_take32(acc + c, r);
+        if constexpr (SPLIT) {
+          for (int from_slice = 0; from_slice < p.slices; ++from_slice) {  // in the order of the slices
+            if (from_slice == (int)slice) continue;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint4 v[4];
+              take_row(ring + part_of(from_slice, q, c + 16 * half - (int)slice * share) * kPlace, lane, v);
+              const uint32_t w[16] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w,
+                                      v[2].x, v[2].y, v[2].z, v[2].w, v[3].x, v[3].y, v[3].z, v[3].w};
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                r[16 * half + i] = __float_as_uint(__uint_as_float(r[16 * half + i]) + __uint_as_float(w[i]));
+            }
+          }
+        }
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] = fmaf(p.alpha, __uint_as_float(r[i]), p.beta * f[i]);
         uint4 v[4];
@@ -383,6 +448,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
     if (pending)  // after a wait that ran out: the load in flight lands before this CTA leaves (bounded)
       for (int tries = 0; tries < 64 && !mbar_try_wait(mine, load_ph); ++tries) {
       }
+  }
+  if constexpr (SPLIT) {
+    if (!first_met) meet();
+    if (!met) {
+      __syncwarp();
+      cluster_sync_all();
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -521,10 +593,11 @@ bool encode_places(CUtensorMap* map, const Stack& m, bool bf16 = false) {
   return encode(map, m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 32, 32);
 }
 
-template <int CG, int BN, bool A_MN, bool B_MN, int STEP>
+template <int CG, int BN, bool A_MN, bool B_MN, int STEP, bool SPLIT = false>
 int32_t launch(OrthoParams& p, const Stack (&a)[2], const Stack (&b)[2], cudaStream_t s) {
   using S = OrthoShape<CG, BN>;
-  auto* kernel = ortho_kernel<CG, BN, A_MN, B_MN, STEP>;
+  auto* kernel = ortho_kernel<CG, BN, A_MN, B_MN, STEP, SPLIT>;
+  static_assert(!SPLIT || (CG == 1 && BN == 128 && S::kStages * S::kStageBytes >= 32 * kPlace), "the ring holds a tile in fp32");
   static std::atomic<uint64_t> ready{0};  // a bit for each device whose shared-memory limit is set
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
@@ -541,30 +614,42 @@ int32_t launch(OrthoParams& p, const Stack (&a)[2], const Stack (&b)[2], cudaStr
   if ((long long)p.m_tiles * p.n_tiles > (1ll << 31) - 1024) return NCA_ERR_UNSUPPORTED;
   const long long tiles = (long long)tiles_of(p, kBM * CG, BN) * p.batch;
   if (tiles > (1ll << 31) - 1024) return NCA_ERR_UNSUPPORTED;
+  if (SPLIT) return launch_after(kernel, dim3((unsigned)(tiles * p.slices)), dim3(kGemmThreads), S::kSmem, s, p.slices, p);
   const long long room = sm_count() / CG;
   return launch_after(kernel, dim3((unsigned)((tiles < room ? tiles : room) * CG)), dim3(kGemmThreads), S::kSmem, s, CG, p);
 }
 
 // The tile of a product by the cost of its waves, as the gated block's: a k block costs a 256 x 256 tile of a pair of
-// multiprocessors 0.28 us, a 256 x 128 tile 0.24 and a 128 x 128 tile of one 0.25, a wave 3 us besides.
+// multiprocessors 0.28 us, a 256 x 128 tile 0.24 and a 128 x 128 tile of one 0.25, a wave 6, 5 or 4 us besides (epilogue, ramps); CTAs
+// that share the k axis 2 us more.
 template <bool A_MN, bool B_MN, int STEP>
 int32_t product(OrthoParams& p, const Stack (&a)[2], const Stack (&b)[2], cudaStream_t s) {
   static const struct {
     int cg, bn;
-    double us;
-  } kinds[] = {{2, 256, 0.28}, {2, 128, 0.24}, {1, 128, 0.25}};
-  int best = 0;
+    double us, wave;
+  } kinds[] = {{2, 256, 0.28, 6.0}, {2, 128, 0.24, 5.0}, {1, 128, 0.25, 4.0}};
+  const long long blocks = (long long)p.kb * p.passes;
+  int best = 0, slices = 1;
   double least = 1e30;
   for (int i = 0; i < 3; ++i) {
     const long long tm = 128 * kinds[i].cg, mt = ceil_div(p.m, tm);
     long long tiles = mt * ceil_div(p.n, kinds[i].bn);
     if (p.symmetric) tiles = (tm / kinds[i].bn) * (mt * (mt + 1) / 2);
-    const double us = (double)ceil_div(tiles * p.batch, sm_count() / kinds[i].cg) * (p.kb * p.passes * kinds[i].us + 3.0);
-    if (us < least) {
-      least = us;
-      best = i;
+    tiles *= p.batch;
+    for (int z = 1; z <= (kinds[i].cg == 1 ? 4 : 1); z *= 2) {
+      // clusters of 2 and 4 leave some multiprocessors of a processing cluster out
+      if (z > 1 && (tiles * z > sm_count() * (z == 2 ? 88 : 80) / 100 || blocks < 4 * z)) break;
+      const double us = (double)ceil_div(tiles * z, sm_count() / kinds[i].cg) * (ceil_div(blocks, z) * kinds[i].us + kinds[i].wave) +
+                        (z > 1 ? 2.0 : 0.0);
+      if (us < least) {
+        least = us;
+        best = i;
+        slices = z;
+      }
     }
   }
+  p.slices = slices;
+  if (slices > 1) return launch<1, 128, A_MN, B_MN, STEP, true>(p, a, b, s);
   if (best == 0) return launch<2, 256, A_MN, B_MN, STEP>(p, a, b, s);
   return best == 1 ? launch<2, 128, A_MN, B_MN, STEP>(p, a, b, s) : launch<1, 128, A_MN, B_MN, STEP>(p, a, b, s);
 }
