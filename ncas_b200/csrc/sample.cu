@@ -56,12 +56,111 @@ __device__ __forceinline__ uint64_t threshold(float u, uint64_t total) {
   return t < (double)total ? min((uint64_t)t, total - 1) : total - 1;
 }
 
+// 2^(j / kTable)
+constexpr int kTableBits = 5, kTable = 1 << kTableBits;  // parts of an octave: two addresses a bank
+__constant__ double kPowers[kTable] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
+    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484,
+    1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407,
+    1.5759808451078865, 1.6104903319492543, 1.645755478153965, 1.681792830507429, 1.718619298122478,
+    1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474,
+    1.9571441241754002};
+// e^(c r) - 1 of c = ln(2) / kTable and |r| <= 1/2, to 3e-15
+__device__ __forceinline__ double power_rest(double r) {
+  constexpr double c = 0.69314718055994530942 / kTable;
+  constexpr double c2 = c * c / 2, c3 = c2 * c / 3, c4 = c3 * c / 4, c5 = c4 * c / 5;
+  return r * (c + r * (c2 + r * (c3 + r * (c4 + r * c5))));
+}
+constexpr double kNearest = 6755399441055744.0;  // 1.5 2^52: the low bits of a sum with it are the nearest whole number
+// exp((v - top) / T) times table[0], from a table of kPowers times that; kTable log2(e) / T in `steep`.
+__device__ __forceinline__ double weight_below(float v, float top, double steep, const double* table) {
+  if (v == top) return table[0];  // also of infinities
+  const double x = ((double)v - (double)top) * steep;
+  if (!(x > -62.0 * kTable)) return 0.0;
+  const double m = x + kNearest;
+  const int k = __double2loint(m);
+  const double t = table[k & (kTable - 1)], e = fma(t, power_rest(x - (m - kNearest)), t);
+  return __hiloint2double(__double2hiint(e) + (k >> kTableBits << 20), __double2loint(e));
+}
+
 // ------------------------------------------------------------------------------- up to 32 classes
+// Up to 4 classes and 4 draws: a row a thread, everything in registers (900000 rows of 2 bf16 classes: 11 us, with two
+// lanes a row 17).
+template <class T, int C>
+__global__ void __launch_bounds__(256) sample_tiny_kernel(const __grid_constant__ SampleParams p) {
+  may_start_next();
+  after_previous();
+  __shared__ double table[kTable];
+  if (threadIdx.x < kTable) table[threadIdx.x] = kPowers[threadIdx.x] * p.one;
+  __syncthreads();
+  const long long row = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (row >= p.rows) return;
+  const T* z = static_cast<const T*>(p.logits) + row * p.stride;
+  float v[C];
+  float top = __int_as_float(0xff800000);
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    v[i] = i < p.classes ? clean(to_f32<T>(z[i])) : __int_as_float(0xff800000);
+    top = fmaxf(top, v[i]);
+  }
+  const double steep = p.inverse_t * (kTable * 1.4426950408889634074), least = p.min_p * p.one;
+  uint64_t w[C], mass = 0;
+  bool heavy[C];
+  int rank[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const double e = possible(v[i]) ? weight_below(v[i], top, steep, table) : 0.0;
+    w[i] = fixed(e, 1.0);
+    heavy[i] = e >= least;
+    rank[i] = 0;
+#pragma unroll
+    for (int j = 0; j < C; ++j) rank[i] += v[j] > v[i] || (v[j] == v[i] && j < i);
+    if (rank[i] < p.top_k) mass += w[i];
+  }
+  uint64_t c[C], total = 0;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    bool keep = rank[i] < p.top_k && heavy[i];
+    if (p.top_p < 1.0) {
+      uint64_t before = 0;
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        if (rank[j] < rank[i]) before += w[j];
+      keep = keep && (double)before < p.top_p * (double)mass;
+    }
+    total += keep ? w[i] : 0;
+    c[i] = total;
+  }
+  for (int d = 0; d < p.draws; ++d) {
+    const long long at = row * p.draws + d;
+    int token = -1;
+    float prob = 0.f;
+    if (total) {
+      const uint64_t t = threshold(p.uniforms[at], total);
+      uint64_t below = 0, own = 0;
+      token = 0;
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const bool over = c[i] > t;
+        if (!over) token = i + 1, below = c[i];
+        if (over && !own) own = c[i] - below;
+      }
+      prob = (float)((double)own / (double)total);
+    }
+    p.tokens[at] = token;
+    if (p.probs) p.probs[at] = prob;
+  }
+}
+
 template <class T, int G>
 __global__ void __launch_bounds__(256) sample_few_kernel(const __grid_constant__ SampleParams p) {
   may_start_next();
   after_previous();
   __shared__ uint64_t sums[256];
+  __shared__ double table[kTable];
+  if (threadIdx.x < kTable) table[threadIdx.x] = kPowers[threadIdx.x] * p.one;
+  __syncthreads();
   const int lane = threadIdx.x % G, base = threadIdx.x - lane;
   const long long row = (long long)blockIdx.x * (256 / G) + threadIdx.x / G;
   const bool here = row < p.rows && lane < p.classes;
@@ -70,9 +169,8 @@ __global__ void __launch_bounds__(256) sample_few_kernel(const __grid_constant__
   float top = v;
 #pragma unroll
   for (int o = G / 2; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(all, top, o));
-  double weight = v == top ? 1.0 : exp(((double)v - (double)top) * p.inverse_t);
-  if (!possible(v)) weight = 0.0;
-  uint64_t w = fixed(weight, p.one);
+  const double weight = possible(v) ? weight_below(v, top, p.inverse_t * (kTable * 1.4426950408889634074), table) : 0.0;
+  uint64_t w = fixed(weight, 1.0);
   // its place in the order, and the mass before it
   int rank = 0;
   uint64_t before = 0;
@@ -92,7 +190,7 @@ __global__ void __launch_bounds__(256) sample_few_kernel(const __grid_constant__
     for (int o = G / 2; o; o >>= 1) mass += __shfl_xor_sync(all, mass, o);
     if (!((double)before < p.top_p * (double)mass)) w = 0;
   }
-  if (!(weight >= p.min_p)) w = 0;
+  if (!(weight >= p.min_p * p.one)) w = 0;
   uint64_t c = w;  // sums in the order of the classes
 #pragma unroll
   for (int o = 1; o < G; o <<= 1) {
@@ -125,7 +223,6 @@ constexpr int kBins = 2048;       // of the ordered bits
 constexpr int kMassBins = 8192;   // of (top - z) / T
 constexpr float kPerBin = 200.f;  // the last holds all beyond 40.9, whose weights are below 2^-58
 constexpr int kSubBins = 256;
-constexpr int kTableBits = 5, kTable = 1 << kTableBits;  // parts of an octave: two addresses a bank
 constexpr int kMostSegments = 1024;
 constexpr int kMostTops = 2048;
 
@@ -139,15 +236,6 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 __device__ __forceinline__ uint64_t place_of(uint32_t key, int i) { return (uint64_t)key << 32 | (0xffffffffu - (uint32_t)i); }
 __device__ __forceinline__ int index_of(uint64_t place) { return (int)(0xffffffffu - (uint32_t)place); }
 __device__ __forceinline__ float value_of(uint64_t place) { return of_key((uint32_t)(place >> 32)); }
-// 2^(j / kTable)
-__constant__ double kPowers[kTable] = {
-    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924,
-    1.1387886347566916, 1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484,
-    1.2690509571917332, 1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
-    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228, 1.5422108254079407,
-    1.5759808451078865, 1.6104903319492543, 1.645755478153965, 1.681792830507429, 1.718619298122478,
-    1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474,
-    1.9571441241754002};
 constexpr uint64_t kPossible = 0x00800000ull << 32;  // the places above -inf
 
 // Blocks of 128 threads serve rows that the list holds whole.
@@ -337,24 +425,14 @@ struct Row {
   // exp((v - top) / T) times p.one
   template <bool FAR>
   __device__ __forceinline__ double weight_of(float v) const {
-    constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52: the low bits of a sum with it are the nearest whole number
-    double x;
-    if constexpr (!FAR) {
-      x = fma((double)fmaxf(v, lowest), steep, offset);
+    if constexpr (FAR) {
+      return weight_below(v, top, steep, sh.table);
     } else {
-      if (v == top) return p.one;  // also of infinities
-      x = ((double)v - (double)top) * steep;
-      if (!(x > -62.0 * kTable)) return 0.0;
+      const double x = fma((double)fmaxf(v, lowest), steep, offset), m = x + kNearest;
+      const int k = __double2loint(m);
+      const double t = sh.table[k & (kTable - 1)], e = fma(t, power_rest(x - (m - kNearest)), t);
+      return __hiloint2double(__double2hiint(e) + (k >> kTableBits << 20), __double2loint(e));
     }
-    const double m = x + kMagic;
-    const int k = __double2loint(m);
-    const double r = x - (m - kMagic);
-    // e^(c r) - 1 of |c r| < 0.0109, to 3e-15
-    constexpr double c = 0.69314718055994530942 / kTable;
-    constexpr double c2 = c * c / 2, c3 = c2 * c / 3, c4 = c3 * c / 4, c5 = c4 * c / 5;
-    const double q = r * (c + r * (c2 + r * (c3 + r * (c4 + r * c5))));
-    const double t = sh.table[k & (kTable - 1)], e = fma(t, q, t);
-    return __hiloint2double(__double2hiint(e) + (k >> kTableBits << 20), __double2loint(e));
   }
   __device__ __forceinline__ double weight(float v) const { return far ? weight_of<true>(v) : weight_of<false>(v); }
   __device__ __forceinline__ uint64_t mass(float v) const { return fixed(weight(v), 1.0); }
@@ -1039,6 +1117,12 @@ int32_t few(const SampleParams& p, cudaStream_t s) {
   if (blocks > (1ll << 31) - 1) return NCA_ERR_UNSUPPORTED;
   return launch_after(sample_few_kernel<T, G>, dim3((unsigned)blocks), dim3(256), 0, s, 1, p);
 }
+template <class T, int C>
+int32_t tiny(const SampleParams& p, cudaStream_t s) {
+  const long long blocks = ceil_div(p.rows, 256);
+  if (blocks > (1ll << 31) - 1) return NCA_ERR_UNSUPPORTED;
+  return launch_after(sample_tiny_kernel<T, C>, dim3((unsigned)blocks), dim3(256), 0, s, 1, p);
+}
 template <class T, int THREADS>
 int32_t row_blocks(const SampleParams& p, cudaStream_t s) {
   if (p.rows > (1ll << 31) - 1) return NCA_ERR_UNSUPPORTED;
@@ -1086,6 +1170,7 @@ extern "C" int32_t nca_b200_sample(const NcaSampleDesc* d, const void* logits, c
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return with_dtype(d->dtype, [&](auto t) -> int32_t {
     using T = decltype(t);
+    if (p.classes <= 4 && p.draws <= 4) return p.classes <= 2 ? tiny<T, 2>(p, s) : tiny<T, 4>(p, s);
     if (p.classes <= 2) return few<T, 2>(p, s);
     if (p.classes <= 4) return few<T, 4>(p, s);
     if (p.classes <= 8) return few<T, 8>(p, s);
