@@ -17,7 +17,8 @@
 //   min_p: the least z of enough weight, by search.
 //   a small top_k: the k-th largest of 2 k groups' maxima bounds the k-th largest entry from below; the few entries above it
 //     are listed and sorted, and everything else happens in the list (as for all rows that fit it).
-//   top_p alone: a histogram of counts over (top - z) / T bounds the mass before every bin within 0.3 %; one pass then
+//   a larger top_k, of 1536 at most: its place in a histogram of counts over (top - z) / T, and the list likewise.
+//   top_p alone: such a histogram bounds the mass before every bin within 0.5 %; one pass then
 //     computes all weights, adds up those surely kept by segment and lists those about the border, which decide.
 //   else: histograms over the ordered bits of z until the entries of the bin with the border can be listed.
 // Segments of entries, a warp each, hold the sums of the kept weights; a draw looks through one segment.
@@ -220,8 +221,8 @@ __global__ void __launch_bounds__(256) sample_few_kernel(const __grid_constant__
 
 // ------------------------------------------------------------------------------------ longer rows
 constexpr int kBins = 2048;       // of the ordered bits
-constexpr int kMassBins = 8192;   // of (top - z) / T
-constexpr float kPerBin = 200.f;  // the last holds all beyond 40.9, whose weights are below 2^-58
+constexpr int kMassBins = 4096;   // of (top - z) / T
+constexpr float kPerBin = 100.f;  // the last holds all beyond 40.9, whose weights are below 2^-58
 constexpr int kSubBins = 256;
 constexpr int kMostSegments = 1024;
 constexpr int kMostTops = 2048;
@@ -243,7 +244,7 @@ template <int THREADS>
 struct RowShared {
   static constexpr bool kLong = THREADS > 128;
   static constexpr int kList = kLong ? 2048 : 1024;      // entries with their masses
-  static constexpr int kRegion = kLong ? 4096 : 1024;    // entries alone
+  static constexpr int kRegion = kLong ? 2048 : 1024;    // entries alone
   static constexpr int kSegments = kLong ? kMostSegments : 64;
   double table[kTable];
   uint64_t sums[kSegments];
@@ -626,25 +627,56 @@ struct Row {
     return l;
   }
 
+  // How many entries lie at each (top - v) scale, to nearest; all beyond the bins, and NaN, in the last.
+  __device__ __forceinline__ void count_bins(float scale) {
+    for (int i = threadIdx.x; i < kMassBins; i += THREADS) sh.mass_counts[i] = 0;
+    __syncthreads();
+    each_chunk<2>([&](int, const E& e) {
+#pragma unroll
+      for (int j = 0; j < kV; ++j) {  // by the bits of a sum with 2^23
+        const uint32_t b = __float_as_uint(fmaf(top - e.at(j), scale, 8388608.f)) - 0x4b000000u;
+        atomicAdd(&sh.mass_counts[min(b, (uint32_t)kMassBins - 1)], 1u);
+      }
+    });
+    __syncthreads();
+  }
+  // What k entries reach, but for roundings at the edge of a bin; -inf where it lies in the last.
+  __device__ __forceinline__ float bound_by_count(int k) {
+    if constexpr (Sh::kLong) {
+      const float scale = kPerBin * (float)p.inverse_t;
+      if (threadIdx.x == 0) sh.keys[0] = kMassBins - 1;
+      count_bins(scale);
+      constexpr int kPer = kMassBins / THREADS;
+      int count = 0;
+      for (int i = 0; i < kPer; ++i) count += sh.mass_counts[threadIdx.x * kPer + i];
+      const int up = warp_running(count, lane);
+      if (lane == 31) sh.keys[32 + warp] = up;
+      __syncthreads();
+      int before = up - count;
+      for (int w = 0; w < warp; ++w) before += sh.keys[32 + w];
+      for (int i = 0; i < kPer; ++i) {
+        const int here = sh.mass_counts[threadIdx.x * kPer + i];
+        if (before < k && before + here >= k) sh.keys[0] = threadIdx.x * kPer + i;  // one thread
+        before += here;
+      }
+      __syncthreads();
+      const uint32_t b = sh.keys[0];
+      __syncthreads();
+      if (b < kMassBins - 1) return top - (b + 0.51f) / scale;
+    }
+    return __int_as_float(0xff800000);
+  }
+
   // top_p alone.  `least`: the limit by min_p.  Returns kCut where the limit is found, kSummed where sh.sums also holds the
   // segments' kept sums, kNot where the entries about the border do not fit the list.
   enum { kNot, kCut, kSummed };
   __device__ __forceinline__ int cut_mass(uint64_t least) {
     if constexpr (Sh::kLong) {
       const float scale = kPerBin * (float)p.inverse_t;
-      for (int i = threadIdx.x; i < kMassBins; i += THREADS) sh.mass_counts[i] = 0;
       for (int i = threadIdx.x; i < kSubBins; i += THREADS) sh.sub_low[i] = sh.sub_high[i] = 0;
       if (threadIdx.x < 8) sh.keys[threadIdx.x] = kMassBins - 1;
-      __syncthreads();
-      each_chunk<2>([&](int, const E& e) {
-#pragma unroll
-        for (int j = 0; j < kV; ++j) {  // to nearest, by the bits of a sum with 2^23; NaN to the last
-          const uint32_t b = __float_as_uint(fmaf(top - e.at(j), scale, 8388608.f)) - 0x4b000000u;
-          atomicAdd(&sh.mass_counts[min(b, (uint32_t)kMassBins - 1)], 1u);
-        }
-      });
-      __syncthreads();
-      // bin b lies at (b -+ 0.501) / 200 (roundings: 8192 2^-23 of a bin): bounds of the masses up to every bin
+      count_bins(scale);
+      // bin b lies at (b -+ 0.501) / 100 (roundings: 4096 2^-23 of a bin): bounds of the masses up to every bin
       constexpr int kPer = kMassBins / THREADS;
       constexpr float kLog = -1.4426950408889634f / kPerBin;
       float lower = 0.f, upper = 0.f;
@@ -669,7 +701,7 @@ struct Row {
         if (w < warp) l += sh.reds[w], u += sh.reds[32 + w], c += sh.keys[32 + w];
         l_all += sh.reds[w], u_all += sh.reds[32 + w];
       }
-      // the first bins at which the border may have been reached, is likely to be, and must have been (fp32 sums of 8192
+      // the first bins at which the border may have been reached, is likely to be, and must have been (fp32 sums of 4096
       // terms, in three levels: 2^-17 of themselves)
       const float may = (float)p.top_p * l_all * 0.9999f, must = (float)p.top_p * u_all * 1.0001f;
       const float likely = (float)p.top_p * 0.5f * (l_all + u_all);
@@ -702,7 +734,7 @@ struct Row {
         return kCut;
       }
       // so many entries about the likely one
-      const int room = Sh::kRegion / 4, centre = (int)sh.amount;
+      const int room = Sh::kRegion * 3 / 8, centre = (int)sh.amount;
       c = before;
       uint32_t low_bin = kMassBins - 1, high_bin = 0;
       for (int i = 0; i < kPer; ++i) {
@@ -793,7 +825,8 @@ struct Row {
       if (border < 0) return kNot;  // not about the likely place
       const auto join = [&](uint64_t place, uint64_t m) {
         const unsigned chunk = (unsigned)(index_of(place) + shift) / kChunk, s = per_segment == 1 ? chunk : chunk / per_segment;
-        if (place >= least) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sums[s]), (unsigned long long)m);
+        uint32_t* sum = reinterpret_cast<uint32_t*>(&sh.sums[s]);
+        if (place >= least) add_to(sum, sum + 1, m);
       };
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) {
@@ -1082,7 +1115,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_row_kernel(con
   }
   r.set_top(top);
   const uint64_t least = p.min_p > 0.0 ? r.limit_of_weight(p.min_p) : kPossible;
-  if (small_k || ((cut_k || cut_p) && p.classes <= R::Sh::kList)) {
+  const bool middle_k = cut_k && !small_k && p.classes > R::Sh::kList && p.top_k <= R::Sh::kList * 3 / 4 &&
+                        top < __int_as_float(0x7f800000);
+  if (middle_k) bound = r.bound_by_count(p.top_k);
+  if (small_k || possible(bound) || ((cut_k || cut_p) && p.classes <= R::Sh::kList)) {
     r.start_list();
     r.each_reaching(bound, [&](int chunk, const typename R::E& e) {
       const int first = r.first_of(chunk);
@@ -1093,7 +1129,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_row_kernel(con
       }
     });
     __syncthreads();
-    if (sh.listed <= R::Sh::kList) {
+    if (sh.listed <= R::Sh::kList && (!middle_k || sh.listed >= p.top_k)) {
       r.draw_listed(blockIdx.x, least);
       return;
     }

@@ -175,3 +175,54 @@ def test_refusals():
             ops.sample(a, b, **kw)
     with fwd.dual_level(), pytest.raises(ValueError, match="tangent"):
         ops.sample(fwd.make_dual(z, z), u)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes", [2049, 30000])
+@pytest.mark.parametrize("shape", ["peaked", "flat", "two levels", "steps", "far", "tail"])
+def test_rows_of_many_shapes(shape, classes, dtype):
+    # rows for which the counts over the weights estimate the cut badly: one class with almost all mass, differences below
+    # a bin, ties across the border, values far from zero, half of the classes impossible
+    g = torch.Generator().manual_seed(11)
+    z = torch.randn((2, classes), generator=g)
+    if shape == "peaked":
+        z[:, classes // 3] = 14.0
+    elif shape == "flat":
+        z = 3.0 + z * 1e-3
+    elif shape == "two levels":
+        z = (z > 0.5).float() * 2.0
+    elif shape == "steps":
+        z = torch.floor(z * 2.0)
+    elif shape == "far":
+        z = z * 3.0 + 900.0
+    else:
+        z = torch.where(z > 0, -z * 20, -float("inf"))
+        z[:, 7] = 0.0
+    z = z.to(dtype)
+    u = torch.rand((2, 3), generator=g)
+    for cut in (dict(top_p=0.95003), dict(top_p=0.30007, temperature=0.2), dict(top_p=0.99931, temperature=3.0),
+                dict(top_p=0.01031), dict(top_p=0.77003, min_p=0.031), dict(top_k=700), dict(top_k=1501, top_p=0.61),
+                dict(top_k=1900, min_p=0.2), dict(top_p=0.87004, temperature=1e6)):
+        check(z, u, **cut)
+
+
+@pytest.mark.parametrize("cut", [dict(top_p=0.95), dict(top_k=50, top_p=0.9), dict(top_k=900), dict(min_p=0.02), dict()])
+def test_many_rows_at_once(cut):
+    z, u = inputs(1500, 2500, 2, torch.bfloat16, seed=12)
+    want, _ = ops.sample(z.to(DEV), u.to(DEV), **cut)
+    some = torch.arange(0, 1500, 149)
+    assert torch.equal(want.cpu()[some], O.sample(z[some], u[some], **cut)[0])
+    again, _ = ops.sample(z.to(DEV)[700:], u.to(DEV)[700:], **cut)
+    assert torch.equal(again, want[700:])
+
+
+def test_offsets_beyond_32_bits():
+    free, _ = torch.cuda.mem_get_info()
+    if free < 16 << 30:
+        pytest.skip("needs 16 GB")
+    big = torch.empty(2**31 + 2**13, dtype=torch.bfloat16, device=DEV)
+    z = big.as_strided((2, 3000), (2**31, 1))
+    v, u = inputs(2, 3000, 4, torch.bfloat16, seed=13)
+    z.copy_(v)
+    for cut in (dict(), dict(top_k=40), dict(top_p=0.8)):
+        assert torch.equal(ops.sample(z, u.to(DEV), **cut)[0], ops.sample(v.to(DEV), u.to(DEV), **cut)[0])
