@@ -19,7 +19,11 @@
 // cluster of 2 or 4 CTAs shares the k axis of each: every CTA adds up a share of the tile's columns through distributed
 // shared memory and stores it.
 //
-// One product kernel, built as gemm.cuh's: a persistent CTA or CTA pair (cta_group::2) a multiprocessor, warp 0
+// Matrices of up to 128 x 256 (and 256 x 256 where no step takes operands of 22 bits) run in one launch: a CTA (or a pair,
+// cta_group::2) holds X as MMA operands in shared memory and in fp32 in tensor memory, beside the accumulator, for all
+// steps.  256 x 256, 5 steps: HH us, as 17 launches 98.
+//
+// Else one product kernel, built as gemm.cuh's: a persistent CTA or CTA pair (cta_group::2) a multiprocessor, warp 0
 // loads tiles by TMA, warp 1 issues the MMAs, warps 4-11 take the accumulators out, add the terms that they load by
 // TMA and store by TMA; two accumulators in tensor memory.  Matrices of a batch are the third dimension of
 // the tensor maps, so that a tile reaches over its own matrix's edge into zeros and writes nothing there.
@@ -538,6 +542,296 @@ __global__ void __launch_bounds__(256) ortho_start_kernel(const __grid_constant_
   }
 }
 
+// ------------------------------------------------------------------------ small matrices in one launch
+struct HeldParams {
+  const uint16_t* m;
+  uint16_t* out;
+  long long batch_stride, si, sj;  // X[i][j] = m[i si + j sj]: X is the wide one of the matrix and its transpose
+  long long out_batch, oi, oj;
+  int small, large, steps;
+  int bf16;         // type of the matrix and the result
+  int wide_loads, wide_stores;  // 16 bytes at a time along j
+  int precise, all; // steps with operands of 22 bits in the largest product; in all products
+  float a, a_scale, b_acc, b_src, inverse_b;
+  double eps;
+  int* ctrl;
+  unsigned long long timeout_ns;
+};
+
+// Operands in shared memory: blocks of 64 columns, rows of 128 bytes, 16-byte pieces at j ^ (row & 7).
+//   CG = 1: X hi, X lo (256 columns each), A or B hi, lo (128 columns)
+//   CG = 2: this CTA's 128 rows of X, its 128 columns of X (of all rows), its rows of A or B (256 columns)
+template <int CG>
+struct HeldShape {
+  static constexpr int kX = 65536;
+  static constexpr int kSecond = kX;       // X lo, or the columns
+  static constexpr int kSquare = 2 * kX;   // A, then B
+  static constexpr int kSquareLo = kSquare + 32768;
+  static constexpr int kRest = 3 * kX;
+  static constexpr int kSmem = kRest + 512 + 1024;
+  static constexpr int kSquareCols = 128 * CG;
+};
+constexpr int kHeldThreads = 288;
+
+__device__ __forceinline__ uint32_t piece_at(uint32_t base, int rows, int row, int col) {  // of 8 columns from col on
+  return base + (col >> 6) * rows * 128 + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ void put_piece(uint32_t at, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 take_piece(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+
+template <int CG>
+__global__ void __launch_bounds__(kHeldThreads, 1) ortho_held_kernel(const __grid_constant__ HeldParams p) {
+  using S = HeldShape<CG>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* done = reinterpret_cast<uint64_t*>(smem + S::kRest);
+  double* sums = reinterpret_cast<double*>(done + 1);  // of the warps, then of the CTAs
+  uint32_t* tmem_base_s = reinterpret_cast<uint32_t*>(sums + 10);
+  volatile int* abort_s = reinterpret_cast<volatile int*>(tmem_base_s + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 1 ? 0 : cta_rank_in_cluster();
+  const FailState fs{p.ctrl, abort_s, 0, p.timeout_ns, true};
+  if (threadIdx.x == 0) {
+    mbar_init(done, 1);
+    *abort_s = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) tc_alloc<CG>(tmem_base_s, 512);
+  cluster_started_arrive();
+  may_start_next();
+  after_previous();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  cluster_started_wait();
+  const uint32_t tmem = *tmem_base_s, base = smem_u32(smem);
+  // a phase's results to the next phase's MMAs, in both CTAs
+  const auto meet = [&] {
+    tc_fence_before();
+    asm volatile("fence.proxy.async;" ::: "memory");
+    __syncwarp();
+    cluster_sync_all();
+    asm volatile("fence.proxy.async;" ::: "memory");
+    tc_fence_after();
+  };
+
+  const int q = warp & 3, half = warp >> 2, row = 32 * q + lane, i = (int)rank * 128 + row;  // warps 0 to 7: a lane a row of X
+  const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16), held = acc + 256;  // the accumulator, X in fp32
+  const uint16_t* m = p.m + (blockIdx.x / CG) * p.batch_stride;
+  const auto value = [&](uint32_t bits) {
+    return p.bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits));
+  };
+  const auto keep = [&](int c, const float (&f)[32]) {  // 32 columns of X in fp32
+    uint32_t r[16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(f[16 * h + j]);
+      tmem_st16(held + c + 16 * h, r);
+    }
+    tc_wait_st();
+  };
+  // the same as operands of the next products
+  const auto spread = [&](int c, float (&f)[32], bool low) {
+    uint4 v[4];
+    pack_row<__half>(f, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) put_piece(piece_at(base, 128, row, c + 8 * j), v[j]);
+    if constexpr (CG == 2) {
+      const uint32_t to = map_to_rank(base + S::kSecond, c >> 7);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at(to, 256, i, (c & 127) + 8 * j)), "r"(v[j].x),
+                     "r"(v[j].y), "r"(v[j].z), "r"(v[j].w)
+                     : "memory");
+    } else if (low) {
+      float hi[32];
+      unpack_half(v, hi);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] -= hi[j];
+      pack_row<__half>(f, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) put_piece(piece_at(base + S::kSecond, 128, row, c + 8 * j), v[j]);
+    }
+  };
+  const auto precise_at = [&](int k) { return k + p.precise >= p.steps; };
+
+  double sum = 0;
+  if (warp < 8) {
+    for (int c = 128 * half; c < min(p.large, 128 * half + 128); c += 32) {
+      float f[32];
+      if (p.wide_loads && i < p.small && c + 32 <= p.large) {
+        const uint4* from = reinterpret_cast<const uint4*>(m + i * p.si + c);
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = from[j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+          for (int t = 0; t < 4; ++t) f[8 * j + 2 * t] = value(w[t] & 0xffffu), f[8 * j + 2 * t + 1] = value(w[t] >> 16);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] = i < p.small && c + j < p.large ? value(m[i * p.si + (c + j) * p.sj]) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) sum = fma((double)f[j], (double)f[j], sum);
+      keep(c, f);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sums[warp] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0;
+    for (int w = 0; w < 8; ++w) sum += sums[w];
+    for (uint32_t r = 0; r < CG; ++r)
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(map_to_rank(smem_u32(sums + 8 + rank), r)), "d"(sum) : "memory");
+  }
+  meet();
+  if (warp < 8) {
+    const double scale = kScaleX / (sqrt(CG == 2 ? sums[8] + sums[9] : sums[8]) + p.eps);
+    const float one = (float)scale;
+    const bool fits = one >= 0x1p-120f && one <= 0x1p120f;
+    for (int c = 128 * half; c < min(p.large, 128 * half + 128); c += 32) {
+      uint32_t r[32];
+      float f[32];
+      tmem_take32(held + c, r);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float x = __uint_as_float(r[j]);
+        f[j] = fits ? x * one : (float)(x * scale);
+      }
+      keep(c, f);
+      spread(c, f, precise_at(0));
+    }
+  }
+  meet();
+
+  bool ok = true;
+  uint32_t ph = 0;
+  // D = a b^T over `blocks` of 16 k; b MN-major for the last product
+  const auto multiply = [&](uint32_t a, uint32_t b, int blocks, bool mn, int n, bool more) {
+    const uint32_t idesc = (1u << 4) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
+    for (int k = 0; k < blocks; ++k) {
+      const uint64_t da = smem_desc(a + (k >> 2) * 16384, 16, 1024) + (k & 3) * 2;
+      const uint64_t db = mn ? smem_desc(b, CG == 2 ? 32768 : 16384, 1024) + (uint64_t)k * 128
+                             : smem_desc(b + (k >> 2) * 16384, 16, 1024) + (k & 3) * 2;
+      umma_ss<CG>(tmem, da, db, idesc, more || k > 0);
+    }
+  };
+  const bool issues = warp == 8 && lane == 0 && rank == 0;
+  const uint32_t x = base, x_lo = base + S::kSecond, columns = CG == 2 ? base + S::kSecond : base;
+  const uint32_t square = base + S::kSquare, square_lo = base + S::kSquareLo;
+  const int small_blocks = (p.small + 15) / 16, large_blocks = (p.large + 15) / 16;
+  for (int k = 0; k < p.steps; ++k) {
+    const bool last = k + 1 == p.steps, precise = CG == 1 && precise_at(k), all = precise && p.all;
+    for (int phase = 0; phase < 3; ++phase) {
+      const bool three = phase < 2 ? all : precise;
+      if (issues) {
+        const uint32_t a = phase == 0 ? x : square, b = phase == 0 ? x : phase == 1 ? square : columns;
+        const int blocks = phase == 0 ? large_blocks : small_blocks, n = phase < 2 ? S::kSquareCols : 256;
+        multiply(a, b, blocks, phase == 2, n, false);
+        if (three) {
+          const uint32_t al = phase == 0 ? x_lo : square_lo, bl = phase == 1 ? square_lo : x_lo;
+          multiply(a, bl, blocks, phase == 2, n, true);
+          multiply(al, b, blocks, phase == 2, n, true);
+        }
+        tc_commit<CG>(done);
+      }
+      __syncwarp();
+      if (ok) ok = mbar_wait_warp(done, ph, fs, 121 + phase);
+      ph ^= 1;
+      tc_fence_after();
+      if (warp < 8 && ok) {
+        const int width = phase < 2 ? S::kSquareCols / 2 : 128, from = half * width;
+        const int to = min(from + width, phase < 2 ? p.small : p.large);
+        for (int c = from; c < to; c += 32) {
+          uint32_t r[32];
+          float f[32];
+          tmem_take32(acc + c, r);
+          if (phase < 2) {
+            if (phase == 0) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[j] = p.a_scale * __uint_as_float(r[j]);
+            } else {
+              uint4 v[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] = take_piece(piece_at(square, 128, row, c + 8 * j));
+              unpack_half(v, f);
+              if (all) {
+                float lo[32];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = take_piece(piece_at(square_lo, 128, row, c + 8 * j));
+                unpack_half(v, lo);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) f[j] += lo[j];
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[j] = fmaf(p.b_acc, __uint_as_float(r[j]), p.b_src * f[j]);
+            }
+            uint4 v[4];
+            pack_row<__half>(f, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) put_piece(piece_at(square, 128, row, c + 8 * j), v[j]);
+            if (phase == 0 ? all : precise) {
+              float hi[32];
+              unpack_half(v, hi);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[j] -= hi[j];
+              pack_row<__half>(f, v);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) put_piece(piece_at(square_lo, 128, row, c + 8 * j), v[j]);
+            }
+          } else {
+            uint32_t h[32];
+            tmem_take32(held + c, h);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = fmaf(p.inverse_b, __uint_as_float(r[j]), p.a * __uint_as_float(h[j]));
+            if (!last) {
+              keep(c, f);
+              spread(c, f, precise_at(k + 1));
+            } else if (i < p.small) {
+              uint16_t* to_row = p.out + (blockIdx.x / CG) * p.out_batch + i * p.oi;
+              uint4 v[4];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[j] *= 1.f / kScaleX;
+              if (p.bf16) pack_row<__nv_bfloat16>(f, v);
+              else pack_row<__half>(f, v);
+              const uint32_t w[16] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w,
+                                      v[2].x, v[2].y, v[2].z, v[2].w, v[3].x, v[3].y, v[3].z, v[3].w};
+              if (p.wide_stores && c + 32 <= p.large) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) reinterpret_cast<uint4*>(to_row + c)[j] = v[j];
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (c + j < p.large) to_row[(c + j) * p.oj] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+              }
+            }
+          }
+        }
+      }
+      meet();
+    }
+  }
+  // after a wait that ran out: the MMAs in flight end before the tensor memory is freed (bounded)
+  if (issues && !ok)
+    for (int tries = 0; tries < 64 && !mbar_try_wait(done, ph ^ 1); ++tries) {
+    }
+  __syncwarp();
+  cluster_sync_all();
+  if (warp == 8) tc_dealloc<CG>(tmem, 512);
+}
+
 // --------------------------------------------------------------------------------------- host side
 int sm_count() {
   static std::atomic<int> kept[kMaxDevices];
@@ -688,6 +982,13 @@ int precise_steps(const NcaOrthoDesc& d) {
   return arrived <= 3.0 ? 0 : (int)std::ceil(arrived - 1.2);
 }
 
+// CTAs that hold a matrix in one launch; 0: it goes through the products.
+int held_by(const NcaOrthoDesc& d) {
+  const int64_t small = std::min(d.rows, d.cols), large = std::max(d.rows, d.cols);
+  if (large > 256) return 0;
+  return small <= 128 ? 1 : precise_steps(d) == 0 ? 2 : 0;
+}
+
 struct Plan {
   long long small, pitch, small_pitch;
   bool tall;
@@ -727,6 +1028,58 @@ int32_t start(const StartParams& p, long long batch, cudaStream_t s) {
   return launch_after(ortho_start_kernel<T, WIDE>, dim3((unsigned)blocks, (unsigned)batch), dim3(256), 0, s, 1, p);
 }
 
+// |B| <= 4 |b| + 16 |c|: times the largest power of two, 2^10 at most, that leaves it below 2^15
+double scale_of_b(const NcaOrthoDesc& d) {
+  double scale = kScaleA;
+  while (scale * (4 * std::fabs(d.coefficients[1]) + 16 * std::fabs(d.coefficients[2])) > 32768.0) scale /= 2;
+  return scale;
+}
+
+template <int CG>
+int32_t held_launch(const HeldParams& p, long long batch, cudaStream_t s) {
+  auto* kernel = ortho_held_kernel<CG>;
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return NCA_ERR_DEVICE;
+  if (!(ready.load(std::memory_order_acquire) >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, HeldShape<CG>::kSmem) != cudaSuccess)
+      return launch_status() == NCA_OK ? NCA_ERR_CUDA : NCA_ERR_DEVICE;
+    ready.fetch_or(1ull << dev, std::memory_order_release);
+  }
+  return launch_after(kernel, dim3((unsigned)(batch * CG)), dim3(kHeldThreads), HeldShape<CG>::kSmem, s, CG, p);
+}
+int32_t held(const NcaOrthoDesc& d, const void* matrix, void* out, int32_t* ctrl, int32_t timeout_ms, cudaStream_t s) {
+  HeldParams p{};
+  const bool tall = d.rows > d.cols;
+  p.m = static_cast<const uint16_t*>(matrix);
+  p.out = static_cast<uint16_t*>(out);
+  p.batch_stride = d.stride[0];
+  p.si = tall ? 1 : d.stride[1];
+  p.sj = tall ? d.stride[1] : 1;
+  p.out_batch = d.rows * d.cols;
+  p.oi = tall ? 1 : d.cols;
+  p.oj = tall ? d.cols : 1;
+  p.small = (int)std::min(d.rows, d.cols);
+  p.large = (int)std::max(d.rows, d.cols);
+  p.steps = d.steps;
+  p.bf16 = d.dtype == NCA_BF16;
+  p.wide_loads = !tall && (d.rows == 1 || d.stride[1] % 8 == 0) && (d.batch == 1 || d.stride[0] % 8 == 0) &&
+                 reinterpret_cast<uintptr_t>(matrix) % 16 == 0;
+  p.wide_stores = !tall && d.cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  p.precise = precise_steps(d);
+  p.all = d.dtype == NCA_F16;
+  const double scale_b = scale_of_b(d);
+  p.a = (float)d.coefficients[0];
+  p.a_scale = kScaleA / (kScaleX * kScaleX);
+  p.b_acc = (float)(d.coefficients[2] * scale_b / ((double)kScaleA * kScaleA));
+  p.b_src = (float)(d.coefficients[1] * scale_b / kScaleA);
+  p.inverse_b = (float)(1.0 / scale_b);
+  p.eps = d.eps;
+  p.ctrl = ctrl;
+  p.timeout_ns = (unsigned long long)(timeout_ms > 0 ? timeout_ms : 10000) * 1000000ull;
+  return held_by(d) == 1 ? held_launch<1>(p, d.batch, s) : held_launch<2>(p, d.batch, s);
+}
+
 }  // namespace
 
 extern "C" {
@@ -734,7 +1087,7 @@ extern "C" {
 int32_t nca_b200_orthogonalize_workspace(const NcaOrthoDesc* d, size_t* bytes) {
   const int32_t st = check_desc(d);
   if (st != NCA_OK || !bytes) return st != NCA_OK ? st : NCA_ERR_INVALID;
-  *bytes = d->batch && d->rows && d->cols ? plan_of(*d).total : 0;
+  *bytes = d->batch && d->rows && d->cols && !held_by(*d) ? plan_of(*d).total : 0;
   return NCA_OK;
 }
 
@@ -742,8 +1095,9 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
                                size_t workspace_bytes, int32_t* ctrl, int32_t timeout_ms, void* stream) {
   NCA_TRY(check_desc(d));
   if (d->batch == 0 || d->rows == 0 || d->cols == 0) return NCA_OK;
-  const Plan pl = plan_of(*d);
   if (!matrix || !out || !ctrl) return NCA_ERR_INVALID;
+  if (held_by(*d)) return held(*d, matrix, out, ctrl, timeout_ms, static_cast<cudaStream_t>(stream));
+  const Plan pl = plan_of(*d);
   if (!workspace || workspace_bytes < pl.total) return NCA_ERR_SCRATCH;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* ws = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~(uintptr_t)255);
@@ -771,9 +1125,7 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
     NCA_TRY((wide ? start<__half, true>(sp, d->batch, s) : start<__half, false>(sp, d->batch, s)));
 
   const double c0 = d->coefficients[0], c1 = d->coefficients[1], c2 = d->coefficients[2];
-  // |B| <= 4 |b| + 16 |c|: times the largest power of two, 2^10 at most, that leaves it below 2^15
-  double scale_b = kScaleA;
-  while (scale_b * (4 * std::fabs(c1) + 16 * std::fabs(c2)) > 32768.0) scale_b /= 2;
+  const double scale_b = scale_of_b(*d);
   OrthoParams p{};
   p.batch = (int)d->batch;
   p.ctrl = ctrl;
