@@ -21,7 +21,8 @@
 //
 // Matrices of up to 128 x 256 (and 256 x 256 where no step takes operands of 22 bits) run in one launch: a CTA (or a pair,
 // cta_group::2) holds X as MMA operands in shared memory and in fp32 in tensor memory, beside the accumulator, for all
-// steps.  256 x 256, 5 steps: HH us, as 17 launches 98.
+// steps.  256 x 256, 5 steps: 59 us, as 17 launches 98; with twice the epilogue warps the same (the phases are bound by the
+// latencies of MMA, commit, tensor memory and cluster barrier).
 //
 // Else one product kernel, built as gemm.cuh's: a persistent CTA or CTA pair (cta_group::2) a multiprocessor, warp 0
 // loads tiles by TMA, warp 1 issues the MMAs, warps 4-11 take the accumulators out, add the terms that they load by
