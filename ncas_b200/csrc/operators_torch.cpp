@@ -1,5 +1,6 @@
-// operators_torch.cpp -- the cell-training operators of libnca_b200 as differentiable torch
-// operators (torch.ops.nca_b200.group_norm_act, gated_ffn, distill_loss, distill_loss_and_grad).
+// operators_torch.cpp -- the cell-training operators of libnca_b200 as torch operators, differentiable where a
+// gradient exists (torch.ops.nca_b200.group_norm_act, gated_ffn, distill_loss, distill_loss_and_grad, gated_scan,
+// orthogonalize, sample).
 //
 // Each operator checks its arguments (ValueError / TypeError with the argument's name), allocates
 // outputs and workspace from torch's caching allocator, and enqueues on torch's current stream of
@@ -805,6 +806,7 @@ Tensor orthogonalize(const Tensor& matrix, int64_t steps, at::ArrayRef<double> c
     view();
   }
   d.stride[1] = m.stride(-2);
+  TORCH_CHECK_VALUE(d.batch <= 65535, op, ": at most 65535 matrices, not ", d.batch);
   const c10::cuda::CUDAGuard guard(matrix.device());
   size_t bytes = 0;
   const int32_t st = nca_b200_orthogonalize_workspace(&d, &bytes);

@@ -8,10 +8,13 @@ the smallest matrices here, whose few roundings do not average.  Sums of k <= 40
 2^-24 sqrt(k) < 2^-18 of a norm, amplified like r, which is made of roundings of 2^-12: covered by the factor 4 too.
 The result adds half a step of its type in every value."""
 
+import ctypes as C
+
 import pytest
 import torch
 
 import oracle.cell_operators as O
+from ncas_b200 import _lib as L
 from ncas_b200 import operators as ops
 
 pytestmark = pytest.mark.gpu
@@ -53,6 +56,15 @@ def test_stacks(shape, dtype):
     alone = ops.orthogonalize(m.reshape(-1, *shape[-2:])[-1].to(DEV))
     # a matrix of a stack does not see the others: at most the tiles' shapes differ, and with them nothing in a sum's order
     assert torch.equal(alone, got.reshape(-1, *shape[-2:])[-1])
+
+
+# about the sizes from which a matrix takes one launch, and from which its last steps take operands of 22 bits
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,steps", [
+    (128, 256, 5), (128, 257, 5), (129, 256, 5), (256, 129, 5), (256, 257, 5), (140, 200, 5), (200, 141, 5), (17, 33, 7),
+    (128, 128, 1), (250, 250, 2), (250, 250, 3), (300, 310, 8), (255, 255, 6), (1, 256, 12)])
+def test_about_the_borders(rows, cols, steps, dtype):
+    check(matrix((rows, cols), dtype, seed=rows + cols), steps=steps)
 
 
 def test_a_bad_matrix_stays_alone():
@@ -149,3 +161,64 @@ def test_refusals():
     for kind, match, t, kw in cases:
         with pytest.raises(kind, match=match):
             ops.orthogonalize(t, **kw)
+
+
+def test_a_failure_that_nobody_has_read_does_not_end_it():
+    """The C ABI on one row of 2^27 values with control words that an earlier call has set, which end nothing and stay for
+    whoever asks."""
+    lib = L.lib()
+    wide = 1 << 27
+    m = torch.ones((1, wide), device=DEV, dtype=torch.bfloat16)
+    out = torch.zeros_like(m)
+    d = L.NcaOrthoDesc(batch=1, rows=1, cols=wide, dtype=1, steps=2, eps=0.0)
+    d.coefficients[:] = [1.5, -0.5, 0.0]
+    d.stride[:] = [wide, wide]
+    size = C.c_size_t(0)
+    assert lib.nca_b200_orthogonalize_workspace(C.byref(d), C.byref(size)) == 0
+    ws = torch.empty(size.value, device=DEV, dtype=torch.uint8)
+    ctrl = torch.tensor([4, 77, 0, 1], device=DEV, dtype=torch.int32)
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    detail = C.c_int32(0)
+    st = lib.nca_b200_orthogonalize(C.byref(d), p(m), p(out), p(ws), ws.numel(), p(ctrl), 20000, stream)
+    assert st == 0
+    assert lib.nca_b200_ctrl_status(p(ctrl), C.byref(detail), stream) == 4 and detail.value == 77
+    # the one singular value is 1, a fixed point of 1.5 x - 0.5 x^3, and each entry 2^-13.5.  A is off by 2^-8 at most, X by
+    # half of that in each step; operands and result round by 2^-8 at most
+    assert ((out.float() * 2.0**13.5 - 1).abs() <= 2.0**-7).all()
+
+
+# sums of more terms than one product adds up, of one sign on A's diagonal and (equal rows) everywhere
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(3, 200001), (200001, 3), (150, 70000), (65600, 300), (2, 40, 131072 + 8), (2, 65537, 130)])
+def test_long_sums(shape, dtype):
+    m = matrix(shape, dtype, seed=12)
+    check(m)
+    m = m.abs()
+    m[..., : m.shape[-2] // 2, :] = 0.02
+    check(m)
+
+
+def test_a_very_long_row():
+    for dtype in TYPES:
+        got = ops.orthogonalize(torch.full((1, 1 << 22), 3.0, device=DEV, dtype=dtype), steps=3, coefficients=(1.5, -0.5, 0.0), eps=0.0)
+        ops.check()
+        # as above; the 256 products lose 3e-4 at most, in each step half of it, and the values round
+        assert ((got.double() * 2.0**11 - 1).abs() <= 3 * 1.5e-4 + UNIT[dtype]).all()
+
+
+def test_a_backward_pass_elsewhere_does_not_disturb_it():
+    # orthogonalize under a graph of autograd: its input is detached, and nothing is recorded
+    w = torch.randn((40, 60), device=DEV).to(torch.bfloat16).requires_grad_()
+    loss = (w.float() ** 2).sum()
+    with torch.no_grad():
+        u = ops.orthogonalize(w)
+    assert not u.requires_grad
+    loss.backward()
+    assert torch.equal(w.grad, (2 * w.detach().float()).to(torch.bfloat16))
+    assert torch.equal(ops.orthogonalize(w.detach()), u)
+
+
+def test_more_matrices_than_a_launch_takes_are_refused():
+    with pytest.raises(ValueError, match="65535"):
+        ops.orthogonalize(torch.zeros((65536, 2, 2), device=DEV, dtype=torch.bfloat16))
