@@ -309,9 +309,10 @@ int32_t nca_b200_run_steps_static(const NcaModelDesc* m, const NcaBatchDesc* b,
                                   void* stream);
 
 /* ---- cell-training operators -------------------------------------------------------------- */
-/* Group norm with an activation (channels last), the gated feed-forward block, and distillation
- * from a teacher's top logits, each with its gradient: what a normalised, gated cell
- * (NCAConfig.norm_groups, update "swiglu") and its training need beside the rollout.
+/* Group norm with an activation (channels last), the gated feed-forward block, distillation
+ * from a teacher's top logits and the gated scan along lines, each with its gradient: what a normalised, gated cell
+ * (NCAConfig.norm_groups, update "swiglu") and its training need beside the rollout; the orthogonalised update of
+ * its matrices; and classes drawn from its readout.
  *
  * Strides are in elements and may be any size_t-addressable value; every product of indexes and
  * strides is formed in 64 bits.  Outputs are contiguous.  Zero sizes are valid: nothing is read,

@@ -1,5 +1,5 @@
-// cell_ops.cuh -- what the cell-training operators (norm.cu, gated.cu, distill.cu) share: element
-// types, 16-byte vectors of them, and the activations with their derivatives.
+// cell_ops.cuh -- what the cell-training operators (norm.cu, gated.cu, distill.cu, scan.cu, orthogonalize.cu, sample.cu)
+// share: element types, 16-byte vectors of them, and the activations with their derivatives.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -2,8 +2,11 @@
 
     group_norm_act          group norm with an activation, channels last
     gated_ffn               gated feed-forward block: (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd
+    gated_scan              gated linear recurrence along the lines of boards or long sequences
     distill_loss            distillation from a teacher's top logits
     distill_loss_and_grad   the same with its gradient in one pass over the logits
+    orthogonalize           an optimiser's update with its singular values brought towards 1
+    sample                  classes drawn from logits with temperature, top-k, top-p and min-p
 
 The reference's cells have the first two as `norm_groups` and `update="swiglu"`
 (src/nca/model.py:48-137, 440-455), which the rollout kernels do not run.  The functions take CUDA
@@ -122,7 +125,7 @@ def check(device="cuda") -> None:
     """Synchronises the current stream and raises NcaError when a kernel's bounded wait ran out since this
     thread's last call (at first: since it began to use the operators).
 
-    A gated_ffn whose wait ran out leaves its outputs unfinished; later calls are not affected.  The
+    A gated_ffn or orthogonalize whose wait ran out leaves its outputs unfinished; later calls are not affected.  The
     record is the device's: every thread that uses the operators is told once, whichever of them ran
     the call and whichever asks first."""
     status, site = _op("operators_status")(torch.empty(0, device=device))
