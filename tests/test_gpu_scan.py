@@ -270,6 +270,40 @@ def test_captured_and_replayed():
     assert torch.equal(y, -want[0]) and torch.equal(last, -want[1])
 
 
+def test_a_training_pass_captured_and_replayed():
+    x, gate, h, m, dy, dlast = inputs((6, 70, 12), 1, torch.bfloat16, seed=10, mask=0.8)
+    x, gate, h, m, dy, dlast = (t.to(DEV) for t in (x, gate, h, m, dy, dlast))
+
+    def once():
+        leaves = [t.detach().requires_grad_() for t in (x, gate, h)]  # fresh: no graph outlives the pass
+        outs = ops.gated_scan(*leaves, dim=1, mask=m)
+        return [t.detach() for t in outs] + list(torch.autograd.grad(outs, leaves, [dy, dlast]))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once()
+    x.mul_(0.5)
+    dy.neg_()
+    graph.replay()
+    for a, b in zip(got, once()):
+        assert torch.equal(a, b)
+
+
+def test_the_same_tensor_twice():
+    x = torch.randn((3, 40, 6), generator=torch.Generator().manual_seed(11))
+    dy, dlast = torch.randn((3, 40, 6)), torch.zeros((3, 6))
+    want, bound = bounds(x, x, None, 1, False, None, dy, dlast)
+    leaf = x.to(DEV).requires_grad_()
+    y, _ = ops.gated_scan(leaf, leaf, dim=1)
+    (g,) = torch.autograd.grad(y, leaf, dy.to(DEV))
+    tol = 4 * (bound["x"] + bound["gate"]) + 3 * E * (want["x"].abs() + want["gate"].abs()) + 2.0**-126
+    assert ((g.cpu().double() - want["x"] - want["gate"]).abs() <= tol).all()
+
+
 def test_offsets_beyond_32_bits():
     # rows 2^31 elements and more apart: two lines of 3 steps in a view of a large buffer
     free, _ = torch.cuda.mem_get_info()
