@@ -159,7 +159,8 @@ def ortho_desc(**kw):
 def test_orthogonalize_descriptor_checks(lib):
     n = C.c_size_t(0)
     ask = lambda **kw: lib.nca_b200_orthogonalize_workspace(C.byref(ortho_desc(**kw)), C.byref(n))  # noqa: E731
-    assert ask() == 0 and n.value >= 2 * 4 * 30 * 56 * 2  # X twice, each as two planes
+    assert ask() == 0 and n.value == 0  # one launch, which holds everything itself
+    assert ask(cols=300) == 0 and n.value >= 2 * 4 * 30 * 304 * 2  # X twice, each as two planes
     assert ask(batch=0) == 0 and n.value == 0
     for bad in (dict(batch=-1), dict(rows=-1), dict(cols=-1), dict(steps=0), dict(dtype=5), dict(eps=-1.0),
                 dict(eps=float("nan")), dict(coefficients=[float("inf"), 0, 0])):
