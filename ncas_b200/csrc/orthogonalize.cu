@@ -48,7 +48,7 @@ namespace {
 
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-inline long long pad8(long long v) { return (v + 7) / 8 * 8; }
+inline long long pad64(long long v) { return (v + 63) / 64 * 64; }
 constexpr int kMaxDevices = 64;
 
 // X is stored times 2^12: |X| <= 2 stays below 2^13, and the entries of a normalised matrix of 2^24 and more values
@@ -1009,8 +1009,8 @@ Plan plan_of(const NcaOrthoDesc& d) {
   p.tall = d.rows > d.cols;
   p.small = std::min(d.rows, d.cols);
   p.large = std::max(d.rows, d.cols);
-  p.pitch = pad8(d.cols);
-  p.small_pitch = pad8(p.small);
+  p.pitch = pad64(d.cols);
+  p.small_pitch = pad64(p.small);
   size_t at = 0;
   const size_t x = align256((size_t)d.batch * d.rows * p.pitch * 2), a = align256((size_t)d.batch * p.small * p.small_pitch * 2);
   for (auto& buffer : p.x)
