@@ -6,7 +6,8 @@
 //
 // Steps compose as maps h -> P h + H (P the product of the a), so a line can be cut anywhere.  A thread
 // owns two adjacent 16-bit channels (or one channel) of kSub adjacent steps, all of which it holds in
-// registers.  Where lines and channels fill the GPU, a thread walks along its line alone.  Else the
+// registers.  Where lines and channels fill the GPU, a thread walks along its line alone.  If they are that many and short, it
+// takes 16 bytes of every row instead (8 backward): the work a row and a line costs besides is shared by more channels.  Else the
 // threads of a block's warps split a stretch of the line: each builds its steps' maps from the identity on, the
 // warps exchange the last through shared memory, and y_t = P_t h + H_t from the state h before the thread's
 // steps.  Blocks walk along the line and load the next stretch while they work on this one.  Where that does not fill
@@ -15,10 +16,10 @@
 // from the end; the states come again from the inputs, from the state that the forward pass stored before
 // each kSub steps (4 bytes for kSub elements).
 //
-// Instructions bound it beside HBM: 72000 lines of 9 steps, 64 channels, bf16 take 65 us forward (47 % of the DRAM cycles,
-// 80 % of the issue slots) and 119 backward (43 %, 62 %); one line of 100001 steps, 1024 channels 198 us forward (80 of
-// them for the pieces' maps) and 282 backward (83), at 59 to 66 % of the DRAM cycles and 53 to 62 % of the issue slots.
-// 16 steps a thread there: 217 and 331 us, for their registers.
+// 72000 lines of 9 steps, 64 channels, bf16 take 43 us forward and 89 backward (90 and 75 % of the HBM rate; 62 and 115 with two
+// channels a thread), 100000 single steps of 504 channels 90 and 208 (389 and 690).  One line of 100001 steps, 1024 channels
+// takes 198 us forward (80 of them for the pieces' maps) and 282 backward (83), at 59 to 66 % of the DRAM cycles and 53 to 62 %
+// of the issue slots; with 16 steps a thread 217 and 331, for their registers.
 #include "cell_ops.cuh"
 
 #include <algorithm>
@@ -516,6 +517,202 @@ __global__ void __launch_bounds__(kThreads, kBlocksBack) scan_backward_kernel(co
   if (p.dstate && me.on && me.sub == 0 && blockIdx.y == 0) store_edge<V>(p.dstate, me.line * p.channels + me.c, run);
 }
 
+// ------------------------------------------------------------------------------- many or short lines
+// A thread takes WORDS words of a row, up to 16 bytes, of S steps at a time, alone along its line.  PLAIN: the compiler orders
+// loads and places (4 steps: backward 55 against 68 us; of 8 steps it would keep 276 bytes outside of the registers).
+template <class T, int WORDS, int S, bool PLAIN>
+struct Wide {
+  static constexpr int kV = sizeof(T) == 2 ? 2 : 1, kChannels = WORDS * kV;  // of a word; of a thread
+  using C = Ch<kV>;
+  using F = typename C::F;
+  struct __align__(4 * WORDS) Row {
+    uint32_t w[WORDS];
+  };
+  static __device__ __forceinline__ uint32_t pack(F f) {
+    if constexpr (kV == 2) {
+      const Vec<T, 2> v = from_pairs<T, 2>({f});
+      return reinterpret_cast<const uint32_t&>(v);
+    } else {
+      return __float_as_uint(f);
+    }
+  }
+  // The rows of the steps that count; others are 0.
+  static __device__ __forceinline__ void load(Row (&q)[S], const T* from, long long step, uint32_t on) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+#pragma unroll
+      for (uint32_t& w : q[i].w) w = 0;
+      if constexpr (PLAIN) {
+        if (on >> i & 1) q[i] = *reinterpret_cast<const Row*>(from + i * step);
+        continue;
+      }
+      if (on >> i & 1) {
+        if constexpr (WORDS == 4)
+          asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(q[i].w[0]), "=r"(q[i].w[1]), "=r"(q[i].w[2]), "=r"(q[i].w[3])
+                       : "l"(from));
+        else
+          asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(q[i].w[0]), "=r"(q[i].w[1]) : "l"(from));
+      }
+      advance(from, step);
+    }
+  }
+  static __device__ __forceinline__ void store(T* to, long long step, const Row (&q)[S], uint32_t in, uint32_t on) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      if (in >> i & 1) *reinterpret_cast<Row*>(PLAIN ? to + i * step : to) = on >> i & 1 ? q[i] : Row{};
+      if constexpr (!PLAIN) advance(to, step);
+    }
+  }
+  // Asks for S steps from t0 on in L2.
+  static __device__ __forceinline__ void soon(const T* line, long long t0, long long step, long long steps) {
+    const long long t = t0 + threadIdx.x % S;
+    if (t >= 0 && t < steps) asm volatile("prefetch.global.L2 [%0];" ::"l"(line + t * step));
+  }
+  // fp32 states, on any 4-byte boundary
+  static __device__ __forceinline__ void load_states(F (&f)[WORDS], const float* p, long long at) {
+    float v[kChannels];
+    if (!p) {
+#pragma unroll
+      for (float& t : v) t = 0.f;
+    } else if (kChannels % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < kChannels / 4; ++i) {
+        const float4 t = reinterpret_cast<const float4*>(p + at)[i];
+        v[4 * i] = t.x, v[4 * i + 1] = t.y, v[4 * i + 2] = t.z, v[4 * i + 3] = t.w;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kChannels; ++i) v[i] = p[at + i];
+    }
+#pragma unroll
+    for (int u = 0; u < WORDS; ++u) {
+      if constexpr (kV == 2) f[u] = make_float2(v[2 * u], v[2 * u + 1]);
+      else f[u] = v[u];
+    }
+  }
+  static __device__ __forceinline__ void store_states(float* p, long long at, const F (&f)[WORDS]) {
+    float v[kChannels];
+#pragma unroll
+    for (int u = 0; u < WORDS; ++u) {
+      if constexpr (kV == 2) v[2 * u] = f[u].x, v[2 * u + 1] = f[u].y;
+      else v[u] = f[u];
+    }
+    if (kChannels % 4 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < kChannels / 4; ++i)
+        reinterpret_cast<float4*>(p + at)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kChannels; ++i) p[at + i] = v[i];
+    }
+  }
+};
+
+constexpr int kShort = 4;  // steps at a time
+// ONCE: lines that end there.
+template <class T, bool ONCE>
+__global__ void __launch_bounds__(kThreads, ONCE ? 8 : 6) scan_wide_forward_kernel(const __grid_constant__ ScanParams p) {
+  using W = Wide<T, 4, kShort, ONCE>;
+  using C = typename W::C;
+  may_start_next();
+  after_previous();
+  const Place<W::kChannels> me(p);
+  if (!me.on) return;
+  const T* x = static_cast<const T*>(p.x) + me.at(p.xs) + me.c;
+  const T* g = static_cast<const T*>(p.gate) + me.at(p.gs) + me.c;
+  T* y = static_cast<T*>(p.y) + me.at(p.ys) + me.c;
+  const long long edge = me.line * p.channels + me.c;
+  typename W::F run[4];
+  W::load_states(run, p.state, edge);
+  for (long long t0 = 0; t0 < p.steps; t0 += kShort) {
+    const uint32_t in = me.inside(p, t0) & ((1u << kShort) - 1), on = me.kept(p, t0, in);
+    typename W::Row xs[kShort], gs[kShort];
+    W::load(xs, x + t0 * p.xs[2], p.xs[2], on);
+    W::load(gs, g + t0 * p.gs[2], p.gs[2], on);
+    if constexpr (!ONCE) {
+      W::soon(x, t0 + kShort, p.xs[2], p.steps);
+      W::soon(g, t0 + kShort, p.gs[2], p.steps);
+    }
+    if (!ONCE && p.saved && t0 && t0 % kSub == 0) W::store_states(p.saved, (me.line * p.marks + t0 / kSub - 1) * p.channels + me.c, run);
+#pragma unroll
+    for (int i = 0; i < kShort; ++i)
+      if (on >> i & 1) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          typename W::F keep, a;
+          coefficients<T, W::kV>(take<T, W::kV>(gs[i].w[u]), keep, a);
+          run[u] = C::fma(a, run[u], C::mul(keep, take<T, W::kV>(xs[i].w[u])));
+          xs[i].w[u] = W::pack(run[u]);
+        }
+      }
+    W::store(y + t0 * p.ys[2], p.ys[2], xs, in, on);
+    if (ONCE) break;
+  }
+  W::store_states(p.last, edge, run);
+}
+
+// As scan_backward_kernel, a word after the other.  S: kShort for lines that end there, else kSub, from the stored states.
+template <class T, int WORDS, int S>
+__global__ void __launch_bounds__(kThreads, 4) scan_wide_backward_kernel(const __grid_constant__ ScanParams p) {
+  using W = Wide<T, WORDS, S, S == kShort>;
+  using C = typename W::C;
+  using F = typename W::F;
+  may_start_next();
+  after_previous();
+  const Place<W::kChannels> me(p);
+  if (!me.on) return;
+  const T* x = static_cast<const T*>(p.x) + me.at(p.xs) + me.c;
+  const T* g = static_cast<const T*>(p.gate) + me.at(p.gs) + me.c;
+  const T* dy = static_cast<const T*>(p.dy) + me.at(p.ds) + me.c;
+  T* dx = static_cast<T*>(p.dx) + me.at(p.ys) + me.c;
+  T* dg = static_cast<T*>(p.dgate) + me.at(p.ys) + me.c;
+  const long long edge = me.line * p.channels + me.c;
+  F h[WORDS], r[WORDS];
+  W::load_states(r, p.dlast, edge);
+  for (long long t0 = S == kShort ? 0 : p.marks * S; t0 >= 0; t0 -= S) {
+    const uint32_t in = me.inside(p, t0), on = me.kept(p, t0, in);
+    typename W::Row xs[S], gs[S], ds[S];
+    W::load(xs, x + t0 * p.xs[2], p.xs[2], on);
+    W::load(gs, g + t0 * p.gs[2], p.gs[2], on);
+    W::load(ds, dy + t0 * p.ds[2], p.ds[2], on);
+    const long long mark = t0 / S - 1;
+    if (S == kShort || mark < 0) W::load_states(h, p.state, edge);
+    else W::load_states(h, p.saved, (me.line * p.marks + mark) * p.channels + me.c);
+    if (S != kShort) {
+      W::soon(x, t0 - S, p.xs[2], p.steps);
+      W::soon(g, t0 - S, p.gs[2], p.steps);
+      W::soon(dy, t0 - S, p.ds[2], p.steps);
+    }
+#pragma unroll
+    for (int u = 0; u < WORDS; ++u) {
+      F keeps[S], w[S], as[W::kV == 1 ? S : 1];
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        if (on >> i & 1) {
+          F a;
+          coefficients<T, W::kV>(take<T, W::kV>(gs[i].w[u]), keeps[i], a);
+          const F xi = take<T, W::kV>(xs[i].w[u]);
+          w[i] = C::mul(a, C::fma(xi, C::of(-1.f), h[u]));
+          h[u] = C::fma(a, h[u], C::mul(keeps[i], xi));
+          if constexpr (W::kV == 1) as[i] = a;
+        }
+#pragma unroll
+      for (int i = S - 1; i >= 0; --i)
+        if (on >> i & 1) {
+          const F G = C::add(take<T, W::kV>(ds[i].w[u]), r[u]), ox = C::mul(keeps[i], G);
+          if constexpr (W::kV == 1) r[u] = C::mul(as[i], G);
+          else r[u] = C::fma(C::mul(keeps[i], C::of(-1.f)), G, G);
+          xs[i].w[u] = W::pack(ox);
+          gs[i].w[u] = W::pack(C::mul(w[i], ox));
+        }
+    }
+    if (p.dx) W::store(dx + t0 * p.ys[2], p.ys[2], xs, in, on);
+    if (p.dgate) W::store(dg + t0 * p.ys[2], p.ys[2], gs, in, on);
+  }
+  if (p.dstate) W::store_states(p.dstate, edge, r);
+}
+
 // --------------------------------------------------------------------------------------- host side
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
@@ -569,6 +766,26 @@ const void* first(const void* p, const int64_t (&s)[3], const NcaScanDesc& d, si
   return p && d.reverse && d.steps ? static_cast<const uint8_t*>(p) + (d.steps - 1) * s[2] * (int64_t)size : p;
 }
 bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 != 0; }
+
+// Lines that a thread with 8 channels walks along are fewer threads than with 2, and each waits for its own loads: worth it
+// for up to 64 steps (250 x 59 x 59, 32 channels, masked: 34 against 44 us forward; 800 lines of 200 steps, 512 channels, 98
+// against 87), of as many lines as fill a quarter of the GPU.
+constexpr long long kWideColumns = 148 * 256, kWideSteps = 64;
+bool on(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+// Whether a thread can take `bytes` of every row (the tensors' bases aside); if so, the plan for it.
+bool take_wide(ScanParams& p, const NcaScanDesc& d, int bytes, bool backward) {
+  const long long channels = bytes / (long long)dtype_size(d.dtype);
+  if (d.channels % channels != 0) return false;
+  for (int i = 0; i < 3; ++i)
+    if ((d.x_stride[i] | d.gate_stride[i] | d.y_stride[i] | (backward ? d.dy_stride[i] : 0)) % channels != 0) return false;
+  const long long columns = p.lines * (d.channels / channels);
+  if (d.steps > kShort && (columns < kWideColumns || d.steps > kWideSteps)) return false;
+  p.per_line = (int)(d.channels / channels);
+  p.columns = columns;
+  p.subs = p.pieces = 1;
+  p.block_columns = kThreads;
+  return true;
+}
 
 template <class F>
 int32_t with_kind(int dtype, bool pairs, F fn) {
@@ -648,10 +865,18 @@ int32_t nca_b200_gated_scan(const NcaScanDesc* d, const void* x, const void* gat
   p.saved = p.marks ? saved : nullptr;
   p.agg_p = static_cast<float*>(workspace);
   p.agg_h = p.agg_p + (size_t)p.pieces * p.lines * p.channels;
+  const bool pairs = two_wide(p), wide = on(p.x, 16) && on(p.gate, 16) && on(p.y, 16) && take_wide(p, *d, 16, false);
   const long long groups = ceil_div(p.columns, p.block_columns);
   if (groups > (1ll << 31) - 1) return NCA_ERR_UNSUPPORTED;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return with_kind(d->dtype, two_wide(p), [&](auto t, auto v) -> int32_t {
+  if (wide)
+    return with_dtype(d->dtype, [&](auto t) -> int32_t {
+      using T = decltype(t);
+      const dim3 grid((unsigned)groups), block(kThreads);
+      return p.steps <= kShort ? launch_after(scan_wide_forward_kernel<T, true>, grid, block, 0, s, 1, p)
+                               : launch_after(scan_wide_forward_kernel<T, false>, grid, block, 0, s, 1, p);
+    });
+  return with_kind(d->dtype, pairs, [&](auto t, auto v) -> int32_t {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
     return p.subs > 1 ? run_forward<T, V, kThreads / kLanes>(p, groups, s) : run_forward<T, V, 1>(p, groups, s);
@@ -689,10 +914,21 @@ int32_t nca_b200_gated_scan_backward(const NcaScanDesc* d, const void* x, const 
   p.saved = const_cast<float*>(saved);
   p.agg_p = static_cast<float*>(workspace);
   p.agg_h = p.agg_p + (size_t)p.pieces * p.lines * p.channels;
+  const bool pairs = two_wide(p);
+  const int bytes = d->steps > kShort ? 8 : 16;
+  const bool wide = on(p.x, bytes) && on(p.gate, bytes) && on(p.dy, bytes) && on(p.dx, bytes) && on(p.dgate, bytes) &&
+                    take_wide(p, *d, bytes, true);
   const long long groups = ceil_div(p.columns, p.block_columns);
   if (groups > (1ll << 31) - 1) return NCA_ERR_UNSUPPORTED;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return with_kind(d->dtype, two_wide(p), [&](auto t, auto v) -> int32_t {
+  if (wide)
+    return with_dtype(d->dtype, [&](auto t) -> int32_t {
+      using T = decltype(t);
+      const dim3 grid((unsigned)groups), block(kThreads);
+      return bytes == 16 ? launch_after(scan_wide_backward_kernel<T, 4, kShort>, grid, block, 0, s, 1, p)
+                         : launch_after(scan_wide_backward_kernel<T, 2, kSub>, grid, block, 0, s, 1, p);
+    });
+  return with_kind(d->dtype, pairs, [&](auto t, auto v) -> int32_t {
     using T = decltype(t);
     constexpr int V = decltype(v)::value;
     return p.subs > 1 ? run_backward<T, V, kThreads / kLanes>(p, groups, s) : run_backward<T, V, 1>(p, groups, s);

@@ -120,8 +120,35 @@ def test_axes(shape, dim, dtype):
     check(x, gate, None, None, dy, dlast, dim, True)
 
 
+# a few steps, whose rows a thread takes 16 bytes at a time where they lie on such places
+@pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,t,c", [(5, 9, 32), (2, 300, 16), (1, 3000, 6)])
+@pytest.mark.parametrize("n,t,m,c", [(1, 1, 1, 8), (130, 1, 1, 40), (7, 2, 3, 16), (3, 3, 50, 4), (5, 4, 9, 24), (2, 5, 4, 8), (4, 4, 4, 12)])
+def test_a_few_steps(n, t, m, c, dtype, reverse):
+    for dim, shape in ((1, (n, t, m, c)), (2, (n, m, t, c))):
+        x, gate, h, mask, dy, dlast = inputs(shape, dim, dtype, seed=n + t, mask=0.6)
+        check(x, gate, h, mask, dy, dlast, dim, reverse)
+        check(x, gate, None, None, dy, dlast, dim, reverse)
+        # the state on a 4-byte boundary; rows on 16 bytes in a wider tensor; rows off them
+        off = lambda t: torch.cat((torch.zeros(1), t.reshape(-1)))[1:].view(t.shape) if t.dim() == 3 and t.dtype == torch.float32 else t  # noqa: E731
+        padded = lambda k: lambda t: torch.cat((t, t[..., :1].expand(*t.shape[:-1], k)), -1).to(DEV)[..., : t.shape[-1]] if t.dim() == 4 and t.is_floating_point() else off(t).to(DEV)  # noqa: E731
+        check(x, gate, h, mask, dy, dlast, dim, reverse, put=padded(8))
+        check(x, gate, h, mask, dy, dlast, dim, reverse, put=padded(1))
+
+
+# many lines of up to 64 steps: a thread a line with several channels, in the backward alone or in both directions
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,t,m,c", [(300, 9, 9, 64), (700, 9, 9, 64), (2500, 5, 2, 64), (1300, 8, 30, 8), (1, 16, 5000, 72),
+                                     (90, 64, 7, 512), (5000, 33, 1, 64), (1200, 65, 1, 256)])
+def test_many_lines(n, t, m, c, dtype):
+    for dim, shape, reverse in ((1, (n, t, m, c), False), (2, (n, m, t, c), True)):
+        x, gate, h, mask, dy, dlast = inputs(shape, dim, dtype, seed=t, mask=0.8)
+        check(x, gate, None, None, dy, dlast, dim, reverse)
+        check(x, gate, h, mask, dy, dlast, dim, reverse)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,t,c", [(5, 9, 32), (300, 3, 16), (2, 300, 16), (1, 3000, 6)])
 def test_masked_steps_hold_anything(n, t, c, dtype):
     x, gate, h, m, dy, dlast = inputs((n, t, c), 1, dtype, seed=1, mask=0.6)
     want = check(x, gate, h, m, dy, dlast, 1, True)
