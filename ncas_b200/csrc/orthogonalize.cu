@@ -21,8 +21,8 @@
 //
 // Matrices of up to 128 x 256 (and 256 x 256 where no step takes operands of 22 bits) run in one launch: a CTA (or a pair,
 // cta_group::2) holds X as MMA operands in shared memory and in fp32 in tensor memory, beside the accumulator, for all
-// steps.  256 x 256, 5 steps: 59 us, as 17 launches 98; with twice the epilogue warps the same (the phases are bound by the
-// latencies of MMA, commit, tensor memory and cluster barrier).
+// steps.  256 x 256, 5 steps: 57 us, as 17 launches 98; a phase is about 2400 cycles of MMAs, 1400 to 3100 of epilogue and 1300 of
+// cluster barrier (with twice the epilogue warps the same time), and 7 us pass before the first.
 //
 // Else one product kernel, built as gemm.cuh's: a persistent CTA or CTA pair (cta_group::2) a multiprocessor, warp 0
 // loads tiles by TMA, warp 1 issues the MMAs, warps 4-11 take the accumulators out, add the terms that they load by
@@ -668,25 +668,55 @@ __global__ void __launch_bounds__(kHeldThreads, 1) ortho_held_kernel(const __gri
 
   double sum = 0;
   if (warp < 8) {
-    for (int c = 128 * half; c < min(p.large, 128 * half + 128); c += 32) {
-      float f[32];
+    const int end = min(p.large, 128 * half + 128);
+    uint4 v[4][4];  // all loads come first
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int c = 128 * half + 32 * t;
       if (p.wide_loads && i < p.small && c + 32 <= p.large) {
         const uint4* from = reinterpret_cast<const uint4*>(m + i * p.si + c);
-        uint4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = from[j];
+        for (int j = 0; j < 4; ++j) v[t][j] = from[j];
+      } else if (c < end) {
+        uint32_t w[16];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-          for (int t = 0; t < 4; ++t) f[8 * j + 2 * t] = value(w[t] & 0xffffu), f[8 * j + 2 * t + 1] = value(w[t] >> 16);
+        for (int j = 0; j < 16; ++j) {
+          const int at = c + 2 * j;
+          const uint32_t low = i < p.small && at < p.large ? m[i * p.si + at * p.sj] : 0;
+          w[j] = low | (uint32_t)(i < p.small && at + 1 < p.large ? m[i * p.si + (at + 1) * p.sj] : 0) << 16;
         }
-      } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = i < p.small && c + j < p.large ? value(m[i * p.si + (c + j) * p.sj]) : 0.f;
+        for (int j = 0; j < 4; ++j) v[t][j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
       }
+    }
 #pragma unroll
-      for (int j = 0; j < 32; ++j) sum = fma((double)f[j], (double)f[j], sum);
+    for (int t = 0; t < 4; ++t) {
+      const int c = 128 * half + 32 * t;
+      if (c >= end) break;
+      float f[32];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w[4] = {v[t][j].x, v[t][j].y, v[t][j].z, v[t][j].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[8 * j + 2 * k] = value(w[k] & 0xffffu), f[8 * j + 2 * k + 1] = value(w[k] >> 16);
+      }
+      // squares of bf16 values leave the range of fp32: 32 of them add up in it where none is large and some is not small
+      float most = 0.f, near = 0.f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        most = fmaxf(most, fabsf(f[j]));
+        near = fmaf(f[j], f[j], near);
+      }
+      if ((most >= 0x1p-50f && most <= 0x1p60f) || most == 0.f) {
+        sum += near;
+      } else {
+#pragma unroll 1
+        for (int j = 0; j < 32; ++j) {
+          if (i >= p.small || c + j >= p.large) break;
+          const double d = value(m[i * p.si + (c + j) * p.sj]);
+          sum = fma(d, d, sum);
+        }
+      }
       keep(c, f);
     }
 #pragma unroll
@@ -704,19 +734,20 @@ __global__ void __launch_bounds__(kHeldThreads, 1) ortho_held_kernel(const __gri
   if (warp < 8) {
     const double scale = kScaleX / (sqrt(CG == 2 ? sums[8] + sums[9] : sums[8]) + p.eps);
     const float one = (float)scale;
-    const bool fits = one >= 0x1p-120f && one <= 0x1p120f;
-    for (int c = 128 * half; c < min(p.large, 128 * half + 128); c += 32) {
-      uint32_t r[32];
-      float f[32];
-      tmem_take32(held + c, r);
+    const auto scaled = [&](auto times) {
+#pragma unroll 1
+      for (int c = 128 * half; c < min(p.large, 128 * half + 128); c += 32) {
+        uint32_t r[32];
+        float f[32];
+        tmem_take32(held + c, r);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float x = __uint_as_float(r[j]);
-        f[j] = fits ? x * one : (float)(x * scale);
+        for (int j = 0; j < 32; ++j) f[j] = times(__uint_as_float(r[j]));
+        keep(c, f);
+        spread(c, f, precise_at(0));
       }
-      keep(c, f);
-      spread(c, f, precise_at(0));
-    }
+    };
+    if (one >= 0x1p-120f && one <= 0x1p120f) scaled([&](float x) { return x * one; });
+    else scaled([&](float x) { return (float)(x * scale); });
   }
   meet();
 
@@ -725,11 +756,13 @@ __global__ void __launch_bounds__(kHeldThreads, 1) ortho_held_kernel(const __gri
   // D = a b^T over `blocks` of 16 k; b MN-major for the last product
   const auto multiply = [&](uint32_t a, uint32_t b, int blocks, bool mn, int n, bool more) {
     const uint32_t idesc = (1u << 4) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
-    for (int k = 0; k < blocks; ++k) {
-      const uint64_t da = smem_desc(a + (k >> 2) * 16384, 16, 1024) + (k & 3) * 2;
-      const uint64_t db = mn ? smem_desc(b, CG == 2 ? 32768 : 16384, 1024) + (uint64_t)k * 128
-                             : smem_desc(b + (k >> 2) * 16384, 16, 1024) + (k & 3) * 2;
-      umma_ss<CG>(tmem, da, db, idesc, more || k > 0);
+    // the one thread that issues them: few operations for each
+    uint64_t da = smem_desc(a, 16, 1024), db = mn ? smem_desc(b, CG == 2 ? 32768 : 16384, 1024) : smem_desc(b, 16, 1024);
+    const uint32_t step = mn ? 128 : 2;
+    for (int k = 0; k < blocks; k += 4, da += 1024, db += mn ? 512 : 1024) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k + j < blocks) umma_ss<CG>(tmem, da + 2 * j, db + step * j, idesc, more || k + j > 0);
     }
   };
   const bool issues = warp == 8 && lane == 0 && rank == 0;
