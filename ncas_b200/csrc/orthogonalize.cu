@@ -481,25 +481,64 @@ struct StartParams {
   double eps;
   __half *hi, *lo;  // [batch][rows][pitch]
 };
-// Sums of squares in 64 bits: squares of bf16 values leave the range of fp32.  One block a part: rows in turn.
+// Eight values of a row at once: WIDE, where all rows start on 16 bytes and end with a whole eight, in one load.
+struct Eights {
+  long long per, count;  // of a row, of the matrix
+  bool narrow;           // 64-bit divisions cost more than the values
+  __device__ __forceinline__ Eights(const StartParams& p) : per((p.cols + 7) / 8), count(p.rows * per), narrow(count < 1ll << 31) {}
+  __device__ __forceinline__ void at(long long i, long long& row, long long& col) const {
+    row = narrow ? (long long)((unsigned)i / (unsigned)per) : i / per;
+    col = (i - row * per) * 8;
+  }
+};
+template <class T, bool WIDE>
+__device__ __forceinline__ Vec<T, 8> eight(const T* row, long long col, long long cols) {
+  if constexpr (WIDE) return *reinterpret_cast<const Vec<T, 8>*>(row + col);
+  Vec<T, 8> v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v.v[j] = col + j < cols ? row[col + j] : from_f32<T>(0.f);
+  return v;
+}
+constexpr int kInFlight = 4;  // eights of a thread
+// One block a part.  Sums of squares in 64 bits: squares of bf16 values leave the range of fp32, in which eight of them add
+// up where none is large and some is not small.
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(256) ortho_norm_kernel(const __grid_constant__ StartParams p) {
   may_start_next();
   after_previous();
-  constexpr int V = WIDE ? 8 : 1;
-  const long long z = blockIdx.y, per = (p.cols + V - 1) / V, count = p.rows * per;
+  const long long z = blockIdx.y, step = (long long)gridDim.x * 256;
+  const Eights all(p);
   const T* m = static_cast<const T*>(p.m) + z * p.batch_stride;
   double s = 0;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) {
-    const long long r = i / per, c = (i - r * per) * V;
-    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(m + r * p.row_stride + c);
-    double t = 0;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all.count; i += kInFlight * step) {
+    Vec<T, 8> v[kInFlight];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const double d = to_f32<T>(v.v[j]);
-      t = fma(d, d, t);
+    for (int k = 0; k < kInFlight; ++k) {
+      if (i + k * step >= all.count) break;
+      long long row, col;
+      all.at(i + k * step, row, col);
+      v[k] = eight<T, WIDE>(m + row * p.row_stride, col, p.cols);
     }
-    s += t;
+#pragma unroll
+    for (int k = 0; k < kInFlight; ++k) {
+      if (i + k * step >= all.count) break;
+      float most = 0.f, near = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = to_f32<T>(v[k].v[j]);
+        most = fmaxf(most, fabsf(d));
+        near = fmaf(d, d, near);
+      }
+      if ((most >= 0x1p-50f && most <= 0x1p60f) || most == 0.f) {
+        s += near;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const double d = to_f32<T>(v[k].v[j]);
+          s = fma(d, d, s);
+        }
+      }
+    }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -510,14 +549,13 @@ __global__ void __launch_bounds__(256) ortho_norm_kernel(const __grid_constant__
   for (int i = 1; i < 8; ++i) s += red[i];
   p.part[z * p.parts + blockIdx.x] = s;
 }
-// X_0 = M / (|M|_F + eps).
+// X_0 = M / (|M|_F + eps).  Rows of X have room for whole eights.
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(256) ortho_start_kernel(const __grid_constant__ StartParams p) {
   may_start_next();
   after_previous();
-  constexpr int V = WIDE ? 8 : 1;
   __shared__ double scale_s;
-  const long long z = blockIdx.y;
+  const long long z = blockIdx.y, step = (long long)gridDim.x * 256;
   if (threadIdx.x < 32) {  // every block adds the parts up in the same order
     double s = 0;
     for (int i = threadIdx.x; i < p.parts; i += 32) s += p.part[z * p.parts + i];
@@ -528,22 +566,28 @@ __global__ void __launch_bounds__(256) ortho_start_kernel(const __grid_constant_
   __syncthreads();
   const double scale = scale_s;
   const float small = (float)scale;
-  const bool fits = small >= 0x1p-120f && small <= 0x1p120f;  // else (norms at the ends of bf16) the product in 64 bits
-  const long long per = p.cols / V, count = p.rows * per;
+  const Eights all(p);
   const T* m = static_cast<const T*>(p.m) + z * p.batch_stride;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) {
-    const long long r = i / per, c = (i - r * per) * V, at = (z * p.rows + r) * p.pitch + c;
-    const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(m + r * p.row_stride + c);
-    Vec<__half, V> hi, lo;
+  const auto scaled = [&](auto times) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all.count; i += step) {
+      long long row, col;
+      all.at(i, row, col);
+      const Vec<T, 8> v = eight<T, WIDE>(m + row * p.row_stride, col, p.cols);
+      const long long at = (z * p.rows + row) * p.pitch + col;
+      Vec<__half, 8> hi, lo;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float x = to_f32<T>(v.v[j]), f = fits ? x * small : (float)(x * scale);
-      hi.v[j] = __float2half_rn(f);
-      lo.v[j] = __float2half_rn(f - __half2float(hi.v[j]));
+      for (int j = 0; j < 8; ++j) {
+        const float f = times(to_f32<T>(v.v[j]));
+        hi.v[j] = __float2half_rn(f);
+        lo.v[j] = __float2half_rn(f - __half2float(hi.v[j]));
+      }
+      *reinterpret_cast<Vec<__half, 8>*>(p.hi + at) = hi;
+      *reinterpret_cast<Vec<__half, 8>*>(p.lo + at) = lo;
     }
-    *reinterpret_cast<Vec<__half, V>*>(p.hi + at) = hi;
-    *reinterpret_cast<Vec<__half, V>*>(p.lo + at) = lo;
-  }
+  };
+  // norms at the ends of bf16: the product in 64 bits
+  if (small >= 0x1p-120f && small <= 0x1p120f) scaled([&](float x) { return x * small; });
+  else scaled([&](float x) { return (float)(x * scale); });
 }
 
 // ------------------------------------------------------------------------ small matrices in one launch
@@ -1067,7 +1111,7 @@ template <class T, bool WIDE>
 int32_t start(const StartParams& p, long long batch, cudaStream_t s) {
   if (batch > 65535) return NCA_ERR_UNSUPPORTED;
   NCA_TRY(launch_after(ortho_norm_kernel<T, WIDE>, dim3(p.parts, (unsigned)batch), dim3(256), 0, s, 1, p));
-  const long long blocks = std::min<long long>(ceil_div(p.rows * p.cols, WIDE ? 4096 : 1024), 148 * 8);
+  const long long blocks = std::min<long long>(ceil_div(p.rows * ceil_div(p.cols, 8), 512), 148 * 8);
   return launch_after(ortho_start_kernel<T, WIDE>, dim3((unsigned)blocks, (unsigned)batch), dim3(256), 0, s, 1, p);
 }
 
