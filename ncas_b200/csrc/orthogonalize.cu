@@ -67,6 +67,7 @@ struct OrthoParams {
   CUtensorMap out[2];
   int m, n;  // of D
   int m_tiles, n_tiles, batch, kb;
+  int pieces;  // of the k axis, kb blocks each: matrix z / pieces, and results for every z
   int slices;  // SPLIT: CTAs that share a tile's k axis, 2 or 4
   int passes;  // over the k axis: 1, or 3 (hi lo, lo hi, hi hi: additions to a small sum lose less)
   int pair;    // the output as hi + lo
@@ -232,6 +233,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
       for (int t = first; t < tiles && ok; t += step) {
         const OrthoTile tl = tile_at<kBM * CG, BN>(p, per, t);
         const int am = tl.m0 + (int)rank * kBM, bn = tl.n0 + (int)rank * S::kBNc;
+        const int z = tl.z / p.pieces, k_from = (tl.z - z * p.pieces) * p.kb;
         for (int i = from, pass = from / p.kb, kb = from - pass * p.kb; i < to; ++i, kb + 1 < p.kb ? ++kb : (kb = 0, ++pass)) {
           const CUtensorMap *ma = &p.a[low && pass == 1], *mb = &p.b[low && pass == 0];
           if (!mbar_wait(&empty[s], ph ^ 1, fs, 111)) {
@@ -241,18 +243,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ortho_kernel(const __grid_con
           if (rank == 0) mbar_arrive_expect_tx(&full[s], S::kStageBytes * CG);
           const uint32_t bar = CG == 1 ? smem_u32(&full[s]) : map_to_rank(smem_u32(&full[s]), 0);
           const uint32_t sa = smem_u32(smem + s * S::kStageBytes), sb = sa + S::kABytes;
-          const int k0 = kb * kBK;
+          const int k0 = (k_from + kb) * kBK;  // beyond the axis: zeros
           if constexpr (A_MN) {
 #pragma unroll
-            for (int j = 0; j < kBM / 64; ++j) load_tile<CG>(sa + j * 8192, ma, bar, am + 64 * j, k0, tl.z);
+            for (int j = 0; j < kBM / 64; ++j) load_tile<CG>(sa + j * 8192, ma, bar, am + 64 * j, k0, z);
           } else {
-            load_tile<CG>(sa, ma, bar, k0, am, tl.z);
+            load_tile<CG>(sa, ma, bar, k0, am, z);
           }
           if constexpr (B_MN) {
 #pragma unroll
-            for (int j = 0; j < S::kBNc / 64; ++j) load_tile<CG>(sb + j * 8192, mb, bar, bn + 64 * j, k0, tl.z);
+            for (int j = 0; j < S::kBNc / 64; ++j) load_tile<CG>(sb + j * 8192, mb, bar, bn + 64 * j, k0, z);
           } else {
-            load_tile<CG>(sb, mb, bar, k0, bn, tl.z);
+            load_tile<CG>(sb, mb, bar, k0, bn, z);
           }
           ++issued;
           if (++s == S::kStages) {
@@ -588,6 +590,39 @@ __global__ void __launch_bounds__(256) ortho_start_kernel(const __grid_constant_
   // norms at the ends of bf16: the product in 64 bits
   if (small >= 0x1p-120f && small <= 0x1p120f) scaled([&](float x) { return x * small; });
   else scaled([&](float x) { return (float)(x * scale); });
+}
+
+// A from its pieces (values in 22 bits), in their order.
+struct JoinParams {
+  const __half *hi, *lo;  // [batch][pieces][rows][pitch]
+  __half *to_hi, *to_lo;  // [batch][rows][pitch]; to_lo: null where one value is enough
+  long long eights;       // of a matrix
+  int pieces;
+};
+__global__ void __launch_bounds__(256) ortho_join_kernel(const __grid_constant__ JoinParams p) {
+  may_start_next();
+  after_previous();
+  using Eight = Vec<__half, 8>;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.eights) return;
+  const long long z = blockIdx.y;
+  const Eight* hi = reinterpret_cast<const Eight*>(p.hi) + z * p.pieces * p.eights + i;
+  const Eight* lo = reinterpret_cast<const Eight*>(p.lo) + z * p.pieces * p.eights + i;
+  float sum[8] = {};
+#pragma unroll 4
+  for (int k = 0; k < p.pieces; ++k) {
+    const Eight a = hi[k * p.eights], b = lo[k * p.eights];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] += __half2float(a.v[j]) + __half2float(b.v[j]);
+  }
+  Eight a, b;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    a.v[j] = __float2half_rn(sum[j]);
+    b.v[j] = __float2half_rn(sum[j] - __half2float(a.v[j]));
+  }
+  reinterpret_cast<Eight*>(p.to_hi)[z * p.eights + i] = a;
+  if (p.to_lo) reinterpret_cast<Eight*>(p.to_lo)[z * p.eights + i] = b;
 }
 
 // ------------------------------------------------------------------------ small matrices in one launch
@@ -1071,14 +1106,24 @@ int held_by(const NcaOrthoDesc& d) {
   return small <= 128 ? 1 : precise_steps(d) == 0 ? 2 : 0;
 }
 
-// Terms that one product adds up.  The accumulators lose 7.6e-8 of a sum of equal signs with every 16 terms, 16 % of 2^25;
-// A over a longer axis is brought together from products of this many (8e-5 at most), in 22 bits.
-constexpr long long kLongest = 16384;
+// Blocks of the k axis that one product adds up.  The accumulators lose 7.6e-8 of a sum of equal signs with every 16 terms, 16 %
+// of 2^25; A over a longer axis is brought together from pieces of it (8e-5 at most), in fp32 from 22 bits.
+constexpr long long kLongest = 16384 / kBK;
+// Pieces of the long axis: also where A has so few tiles that clusters of 4 leave most of the GPU idle, for as many CTAs as there
+// are, where what they save (a block of the axis takes 0.25 us) is more than the second kernel's 4 us (64 x 16384: 240 to 195 us).
+long long pieces_of(const NcaOrthoDesc& d, int passes) {
+  const long long small = std::min(d.rows, d.cols), blocks = ceil_div(std::max(d.rows, d.cols), kBK);
+  const long long side = ceil_div(small, 128), tiles = side * (side + 1) / 2 * d.batch;
+  const long long want = std::min(sm_count() / std::max(tiles, 1ll), blocks * passes / 8);
+  const bool worth = want > 4 && 0.25 * blocks * passes * (0.25 - 1.0 / want) > 4.0;
+  const long long pieces = std::max(worth ? want : 1, ceil_div(blocks, kLongest));
+  return ceil_div(blocks, ceil_div(blocks, pieces));  // no empty ones
+}
 
 struct Plan {
   long long small, large, pitch, small_pitch;
   bool tall;
-  size_t x[2][2], a[2], b[2], part, total;  // x[buffer][hi, lo]; a, b: hi, lo
+  size_t x[2][2], a[2], b[2], pieces[2], part, total;  // x[buffer][hi, lo]; a, b, pieces: hi, lo
   int parts;
 };
 Plan plan_of(const NcaOrthoDesc& d) {
@@ -1098,7 +1143,12 @@ Plan plan_of(const NcaOrthoDesc& d) {
   for (int i = 0; i < 2; ++i) {
     p.a[i] = at;
     p.b[i] = at + a;
-    if (i == 0 || precise_steps(d) > 0 || std::max(d.rows, d.cols) > kLongest) at += 2 * a;
+    if (i == 0 || precise_steps(d) > 0) at += 2 * a;
+  }
+  const long long pieces = std::max(pieces_of(d, 1), pieces_of(d, 3));
+  for (size_t& part : p.pieces) {
+    part = at;
+    if (pieces > 1) at += align256((size_t)d.batch * pieces * p.small * p.small_pitch * 2);
   }
   p.part = at;
   p.parts = (int)std::max<long long>(1, std::min<long long>(ceil_div(d.rows * d.cols, 4096), ceil_div(592, d.batch ? d.batch : 1)));
@@ -1225,23 +1275,32 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
     p.m = p.n = (int)pl.small;
     p.symmetric = 1;
     p.last = 0;
+    p.terms = 0;
     p.alpha = kScaleA / (kScaleX * kScaleX);
-    p.beta = 1.f;
-    for (long long from = 0; from < pl.large; from += kLongest) {
-      const long long len = std::min(kLongest, pl.large - from);
-      Stack part[2] = {x[0], x[1]};
-      for (Stack& t : part) {
-        (pl.tall ? t.rows : t.cols) = len;
-        t.p = static_cast<const uint16_t*>(t.p) + from * (pl.tall ? t.ld : 1);
-      }
-      p.kb = (int)ceil_div(len, kBK);
-      p.terms = from ? 2 : 0;  // the sum so far: a warp reads what it then stores, and nobody else does
-      p.pair = all || from + len < pl.large;
-      for (int i = 0; i < 2; ++i)
-        if ((i < p.terms && !encode_places(&p.src[i], a_of[i])) || (i <= p.pair && !encode_places(&p.out[i], a_of[i])))
-          return NCA_ERR_CUDA;
-      NCA_TRY((pl.tall ? product<true, true, STEP_POWER>(p, part, part, s) : product<false, false, STEP_POWER>(p, part, part, s)));
+    p.beta = 0.f;
+    const long long blocks = ceil_div(pl.large, kBK);
+    p.pieces = (int)pieces_of(*d, p.passes);
+    p.kb = (int)ceil_div(blocks, p.pieces);
+    p.batch = (int)d->batch * p.pieces;
+    p.pair = all || p.pieces > 1;
+    for (int i = 0; i <= p.pair; ++i) {
+      Stack to = p.pieces > 1 ? square(pl.pieces[i]) : a_of[i];
+      to.batch = p.batch;
+      if (!encode_places(&p.out[i], to)) return NCA_ERR_CUDA;
     }
+    NCA_TRY((pl.tall ? product<true, true, STEP_POWER>(p, x, x, s) : product<false, false, STEP_POWER>(p, x, x, s)));
+    if (p.pieces > 1) {
+      JoinParams j{};
+      j.hi = reinterpret_cast<const __half*>(ws + pl.pieces[0]);
+      j.lo = reinterpret_cast<const __half*>(ws + pl.pieces[1]);
+      j.to_hi = reinterpret_cast<__half*>(ws + pl.a[0]);
+      j.to_lo = all ? reinterpret_cast<__half*>(ws + pl.a[1]) : nullptr;
+      j.eights = pl.small * pl.small_pitch / 8;
+      j.pieces = p.pieces;
+      NCA_TRY(launch_after(ortho_join_kernel, dim3((unsigned)ceil_div(j.eights, 256), (unsigned)d->batch), dim3(256), 0, s, 1, j));
+    }
+    p.pieces = 1;
+    p.batch = (int)d->batch;
 
     p.kb = (int)ceil_div(pl.small, kBK);
     p.terms = 1 + all;
