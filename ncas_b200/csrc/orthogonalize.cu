@@ -1030,6 +1030,9 @@ int32_t launch(OrthoParams& p, const Stack (&a)[2], const Stack (&b)[2], cudaStr
   return launch_after(kernel, dim3((unsigned)((tiles < room ? tiles : room) * CG)), dim3(kGemmThreads), S::kSmem, s, CG, p);
 }
 
+// Clusters of 2 and 4 leave some multiprocessors of a processing cluster out: the share in percent that runs at once.
+constexpr int kClusters2 = 88, kClusters4 = 80;
+
 // The tile of a product by the cost of its waves, as the gated block's: a k block costs a 256 x 256 tile of a pair of
 // multiprocessors 0.28 us, a 256 x 128 tile 0.24 and a 128 x 128 tile of one 0.25, a wave 6, 5 or 4 us besides (epilogue, ramps); CTAs
 // that share the k axis 2 us more.
@@ -1048,8 +1051,7 @@ int32_t product(OrthoParams& p, const Stack (&a)[2], const Stack (&b)[2], cudaSt
     if (p.symmetric) tiles = (tm / kinds[i].bn) * (mt * (mt + 1) / 2);
     tiles *= p.batch;
     for (int z = 1; z <= (kinds[i].cg == 1 ? 4 : 1); z *= 2) {
-      // clusters of 2 and 4 leave some multiprocessors of a processing cluster out
-      if (z > 1 && (tiles * z > sm_count() * (z == 2 ? 88 : 80) / 100 || blocks < 4 * z)) break;
+      if (z > 1 && (tiles * z > sm_count() * (z == 2 ? kClusters2 : kClusters4) / 100 || blocks < 4 * z)) break;
       const double us = (double)ceil_div(tiles * z, sm_count() / kinds[i].cg) * (ceil_div(blocks, z) * kinds[i].us + kinds[i].wave) +
                         (z > 1 ? 2.0 : 0.0);
       if (us < least) {
@@ -1109,14 +1111,15 @@ int held_by(const NcaOrthoDesc& d) {
 // Blocks of the k axis that one product adds up.  The accumulators lose 7.6e-8 of a sum of equal signs with every 16 terms, 16 %
 // of 2^25; A over a longer axis is brought together from pieces of it (8e-5 at most), in fp32 from 22 bits.
 constexpr long long kLongest = 16384 / kBK;
-// Pieces of the long axis: also where A has so few tiles that clusters of 4 leave most of the GPU idle, for as many CTAs as there
+// Pieces of the long axis: also where A has so few tiles that its clusters leave much of the GPU idle, for as many CTAs as there
 // are, where what they save (a block of the axis takes 0.25 us) is more than the second kernel's 4 us (64 x 16384, 5 steps:
-// bf16 178 to 127 us, fp16 305 to 195).
+// bf16 178 to 127 us, fp16 305 to 195; 2730 x 1001 fp16 291 to 274).
 long long pieces_of(const NcaOrthoDesc& d, int passes) {
   const long long small = std::min(d.rows, d.cols), blocks = ceil_div(std::max(d.rows, d.cols), kBK);
   const long long side = ceil_div(small, 128), tiles = side * (side + 1) / 2 * d.batch;
   const long long want = std::min(sm_count() / std::max(tiles, 1ll), blocks * passes / 8);
-  const bool worth = want > 4 && 0.25 * blocks * passes * (0.25 - 1.0 / want) > 4.0;
+  const int slices = tiles * 4 <= kClusters4 * sm_count() / 100 ? 4 : tiles * 2 <= kClusters2 * sm_count() / 100 ? 2 : 1;
+  const bool worth = want > slices && 0.25 * blocks * passes * (1.0 / slices - 1.0 / want) > 4.0;
   const long long pieces = std::max(worth ? want : 1, ceil_div(blocks, kLongest));
   return ceil_div(blocks, ceil_div(blocks, pieces));  // no empty ones
 }

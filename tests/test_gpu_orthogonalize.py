@@ -191,7 +191,7 @@ def test_a_failure_that_nobody_has_read_does_not_end_it():
 # sums of more terms than one product adds up, or of pieces for more CTAs, of one sign on A's diagonal and (equal rows) everywhere
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(3, 200001), (200001, 3), (150, 70000), (65600, 300), (2, 40, 131072 + 8), (2, 65537, 130),
-                                   (64, 16384), (16385, 100), (300, 8190), (5, 30, 2500), (2, 3001, 9), (270, 5000)])
+                                   (64, 16384), (16385, 100), (300, 8190), (5, 30, 2500), (2, 3001, 9), (270, 5000), (1000, 4100), (2730, 1001)])
 def test_long_sums(shape, dtype):
     m = matrix(shape, dtype, seed=12)
     check(m)
