@@ -223,3 +223,27 @@ def test_a_backward_pass_elsewhere_does_not_disturb_it():
 def test_more_matrices_than_a_launch_takes_are_refused():
     with pytest.raises(ValueError, match="65535"):
         ops.orthogonalize(torch.zeros((65536, 2, 2), device=DEV, dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("shape", [(64, 9000), (100, 200), (2, 200, 180)])
+def test_two_graphs_in_turn_and_another_stream(shape):
+    # each graph has its own workspace: replays of one between those of the other change nothing
+    a, b = (matrix(shape, torch.bfloat16, seed=s).to(DEV) for s in (20, 21))
+    want = [ops.orthogonalize(t) for t in (a, b)]
+    graphs, got = [], []
+    for t in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(ops.orthogonalize(t))
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        graphs[0].replay()
+        graphs[1].replay()
+        with torch.cuda.stream(side):  # beside them
+            beside = ops.orthogonalize(a)
+        graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(beside, want[0])
+    ops.check()

@@ -130,8 +130,13 @@ def test_a_few_steps(n, t, m, c, dtype, reverse):
         check(x, gate, h, mask, dy, dlast, dim, reverse)
         check(x, gate, None, None, dy, dlast, dim, reverse)
         # the state on a 4-byte boundary; rows on 16 bytes in a wider tensor; rows off them
-        off = lambda t: torch.cat((torch.zeros(1), t.reshape(-1)))[1:].view(t.shape) if t.dim() == 3 and t.dtype == torch.float32 else t  # noqa: E731
-        padded = lambda k: lambda t: torch.cat((t, t[..., :1].expand(*t.shape[:-1], k)), -1).to(DEV)[..., : t.shape[-1]] if t.dim() == 4 and t.is_floating_point() else off(t).to(DEV)  # noqa: E731
+        def padded(k):
+            def put(t):
+                if t.dim() == 3 and t.dtype == torch.float32:
+                    return torch.cat((torch.zeros(1), t.reshape(-1))).to(DEV)[1:].view(t.shape)
+                return torch.cat((t, t[..., :1].expand(*t.shape[:-1], k)), -1).to(DEV)[..., : t.shape[-1]] if t.dim() == 4 else t.to(DEV)
+            return put
+
         check(x, gate, h, mask, dy, dlast, dim, reverse, put=padded(8))
         check(x, gate, h, mask, dy, dlast, dim, reverse, put=padded(1))
 
