@@ -842,7 +842,8 @@ struct Row {
         if (sh.list[i] >= at) join(sh.list[i], mass(value_of(sh.list[i])));
       limit = max(at, least);
       __syncthreads();
-      return kSummed;
+      // the sums hold all above the list: where min_p cuts some of those too, they come again
+      return value_of(least) > high ? kCut : kSummed;
     } else {
       return kNot;
     }
@@ -1065,6 +1066,9 @@ struct Row {
       const uint64_t t = threshold(p.uniforms[at], total);
       const int s = above(sh.sums, segments, t), end = min((s + 1) * per_segment, chunks);
       uint64_t sum = s ? sh.sums[s - 1] : 0;
+      int last = -1;  // the last class of the walk that can be drawn
+      uint64_t last_mass = 0;
+      bool drawn = false;
       for (int c = s * per_segment; c < end && sum <= t; ++c) {
         const E e = fetch(c);
         const int first = first_of(c);
@@ -1073,11 +1077,13 @@ struct Row {
         for (int j = 0; j < kV; ++j) {
           const float v = clean(e.at(j));
           mine += own[j] = kept(v, first + j) ? mass(v) : 0;
+          if (own[j]) last = first + j, last_mass = own[j];
         }
         const uint64_t up = warp_running(mine, lane);
         uint64_t run = sum + up - mine;
         sum += __shfl_sync(0xffffffffu, up, 31);
         if (run <= t && t < run + mine) {  // one lane
+          drawn = true;
 #pragma unroll
           for (int j = 0; j < kV; ++j) {
             if (run <= t && t < run + own[j]) {
@@ -1086,6 +1092,14 @@ struct Row {
             }
             run += own[j];
           }
+        }
+      }
+      // the walk ends with a class, as its sums are the segment's; no output stays unwritten if one were off
+      if (!__any_sync(0xffffffffu, drawn)) {
+        const int best = __reduce_max_sync(0xffffffffu, last);
+        if (last == best && (best >= 0 || lane == 0)) {
+          p.tokens[at] = best;
+          if (p.probs) p.probs[at] = (float)((double)last_mass / (double)total);
         }
       }
     }

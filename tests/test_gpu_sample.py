@@ -5,11 +5,15 @@ the histograms 2^-44 of the largest at these sizes; sums of n <= 2^17 of them at
 1e-11 of the mass of a border, which each test checks, the classes have to be equal.  Probabilities are rounded to
 fp32 once: 2^-24 of themselves and the 1e-11."""
 
+import ctypes as C
+import math
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
 import oracle.cell_operators as O
+from ncas_b200 import _lib as L
 from ncas_b200 import operators as ops
 
 pytestmark = pytest.mark.gpu
@@ -226,3 +230,41 @@ def test_offsets_beyond_32_bits():
     z.copy_(v)
     for cut in (dict(), dict(top_k=40), dict(top_p=0.8)):
         assert torch.equal(ops.sample(z, u.to(DEV), **cut)[0], ops.sample(v.to(DEV), u.to(DEV), **cut)[0])
+
+
+def near_cuts(z, top_p, temperature, bins):
+    """The min_p whose border lies `bins` hundredths of an exponent above that of top_p."""
+    w = torch.exp((z.double() - z.double().max()) / temperature).sort(descending=True).values
+    border = w[int((w.cumsum(0) < top_p * w.sum()).sum())]
+    min_p = min(1.0, float(border) * math.exp(0.01 * bins))
+    assert ((w / min_p - 1).abs() > 1e-11).all()  # no class within rounding of it
+    return min_p
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("classes,scale,top_p,temperature", [(131072, 0.8, 0.95, 1.0), (131072, 0.3, 0.9, 0.7), (65536, 1.0, 0.95, 1.5),
+                                                             (40000, 0.56, 0.7, 1.0), (2500, 0.5, 0.9, 1.0)])
+def test_min_p_beside_the_border_of_top_p(classes, scale, top_p, temperature, dtype):
+    for seed in range(3):
+        z, u = inputs(1, classes, 12, dtype, seed=100 + seed, scale=scale)
+        for bins in (-1.37, 0.23, 0.71, 1.37, 2.41, 3.7, 6.1, 9.3, 14.7):
+            check(z, u, temperature=temperature, top_p=top_p, min_p=near_cuts(z[0], top_p, temperature, bins))
+
+
+@pytest.mark.parametrize("classes,scale,min_p,dtype", [(131072, 0.8, 0.02003, torch.bfloat16), (131072, 0.56, 0.05003, torch.float32),
+                                                       (65536, 0.8, 0.02003, torch.float16)])
+def test_every_output_is_written(classes, scale, min_p, dtype):
+    # through the C ABI into buffers that hold what no draw gives
+    z, u = inputs(60, classes, 6, dtype, seed=21, scale=scale)
+    zd, ud = z.to(DEV), u.to(DEV)
+    tokens, probs = torch.full(u.shape, -7, dtype=torch.int64, device=DEV), torch.full(u.shape, -7.0, device=DEV)
+    d = L.NcaSampleDesc(rows=60, classes=classes, draws=6, logits_stride=classes, dtype=TYPES.index(dtype), top_k=0, temperature=1.0,
+                        top_p=0.95, min_p=min_p)
+    p = lambda t: C.c_void_p(t.data_ptr())  # noqa: E731
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert L.lib().nca_b200_sample(C.byref(d), p(zd), p(ud), p(tokens), p(probs), stream) == 0
+    assert (tokens >= 0).all() and (probs > 0).all()
+    want, share, nearest = O.sample(z, u, top_p=0.95, min_p=min_p)
+    assert nearest > 1e-11
+    assert torch.equal(tokens.cpu(), want)
+    assert ((probs.cpu().double() - share).abs() <= share * 2.0**-24 + 1e-10).all()
