@@ -1,8 +1,9 @@
 // scan.cu -- the gated scan h_t = a_t h_{t-1} + (1 - a_t) x_t, a = sigmoid(gate), along one axis, forward
 // and backward (nca_b200_gated_scan*).
 //
-// With e = exp(gate), 1 - a is 1 / (1 + e) and a is e / (1 + e): both with full relative precision.  States,
-// products and sums are fp32.
+// With e = exp(gate), 1 - a is 1 / (1 + e), and a is e / (1 + e) up to 1/2 and 1 less the former from there on: both with full
+// relative precision, and a the nearest fp32 where the former is small, so that open gates hold a state.  States, products
+// and sums are fp32.
 //
 // Steps compose as maps h -> P h + H (P the product of the a), so a line can be cut anywhere.  A thread
 // owns two adjacent 16-bit channels (or one channel) of kSub adjacent steps, all of which it holds in
@@ -72,6 +73,8 @@ struct Ch<1> {
   static __device__ __forceinline__ F fma(F a, F b, F c) { return fmaf(a, b, c); }
   template <class O>
   static __device__ __forceinline__ F each(F a, O o) { return o(a); }
+  // b where g is not negative (its sign bit), else c
+  static __device__ __forceinline__ F pick(F g, F b, F c) { return __float_as_int(g) >= 0 ? b : c; }
 };
 template <>
 struct Ch<2> {
@@ -82,6 +85,7 @@ struct Ch<2> {
   static __device__ __forceinline__ F fma(F a, F b, F c) { return fma2(a, b, c); }
   template <class O>
   static __device__ __forceinline__ F each(F a, O o) { return make_float2(o(a.x), o(a.y)); }
+  static __device__ __forceinline__ F pick(F g, F b, F c) { return make_float2(Ch<1>::pick(g.x, b.x, c.x), Ch<1>::pick(g.y, b.y, c.y)); }
 };
 
 template <class T, int V>
@@ -110,7 +114,8 @@ __device__ __forceinline__ void coefficients(typename Ch<V>::F gate, typename Ch
     e = C::fma(e, C::mul(rest, C::of(0.6931471805599453f)), e);
   }
   keep = C::each(C::add(e, C::of(1.f)), [](float v) { return rcp(v); });
-  a = C::mul(e, keep);
+  // beside 1 the rounded 1 - keep: the product's own roundings would take 2^-24 off a held state at every step
+  a = C::pick(g, C::fma(keep, C::of(-1.f), C::of(1.f)), C::mul(e, keep));
 }
 // Of a step that counts only where `live`: else a = 1, so that the state stays.
 template <class T, int V, bool WHOLE>

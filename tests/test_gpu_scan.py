@@ -371,3 +371,24 @@ def test_refusals():
         torch.autograd.grad(y.sum(), leaf, create_graph=True)
     with fwd.dual_level(), pytest.raises(ValueError, match="tangent"):
         ops.gated_scan(fwd.make_dual(x, x), x, dim=1)
+
+
+# a line's warps and pieces, a thread a line, 16 bytes of a row a thread
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,t,c", [(1, 100001, 32), (3, 40, 64), (800, 200, 512), (1200, 60, 512), (7, 3, 64)])
+def test_open_gates_hold_the_state(n, t, c, dtype):
+    # 1 - sigmoid(gate) below 2^-25: the nearest fp32 of sigmoid(gate) is 1, so that a state without input stays as it is; the
+    # formula's own decay, of t (1 - a) of it at most, is all that it is off by.  `want` itself is rounded in 64 bits: an exponential
+    # near 1 within 2^-52 and its product with h within 2^-53 of it, below 2^-50
+    gate = torch.linspace(17.5, 30.0, c).to(dtype)
+    share = torch.sigmoid(-gate.double())
+    assert (share < 2.0**-25).all()
+    h = torch.randn((n, c), generator=torch.Generator().manual_seed(0))
+    x = torch.zeros((1, 1, c), dtype=dtype, device=DEV).expand(n, t, c).contiguous()
+    gates = gate.to(DEV).expand(n, t, c).contiguous()
+    y, last = ops.gated_scan(x, gates, h.to(DEV), dim=1)
+    want = h.double() * torch.exp(t * torch.log1p(-share))
+    off = (last.cpu().double() - want).abs()
+    tol = (t * share + 2.0**-50) * h.double().abs()
+    assert (off <= tol).all(), float((off / tol).max())
+    assert torch.equal(y[:, -1], last.to(dtype))
