@@ -481,7 +481,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksBack) scan_backward_kernel(co
     }
     const auto work = [&](auto all) {
       constexpr bool W = decltype(all)::value != 0;
-      F keeps[kSub], w[kSub], as[V == 1 ? kSub : 1];
+      // Two channels of a thread alone along its line: one row for a and 1 - a, the smaller of them, as the gate's sign tells,
+      // since the other is 1 less that.  Two rows do not fit the registers (800 lines of 200 steps, 512 channels bf16: 180 us; at 3
+      // blocks a multiprocessor 175; folded 172).  1 - a alone (163) would lose a beside 1 - a of nearly 1.
+      constexpr bool kFold = V == 2 && SUBS == 1;
+      F keeps[kSub], w[kSub], as[kFold ? 1 : kSub];
       F P = C::of(1.f), H = C::of(0.f);
       // in the order of the line: the states again, w = a (h before - x), and the stretch's map of r = a G
 #pragma unroll
@@ -496,19 +500,28 @@ __global__ void __launch_bounds__(kThreads, kBlocksBack) scan_backward_kernel(co
           P = C::mul(P, a);
           H = C::fma(P, take<T, V>(raw[2].v[i]), H);
         }
-        keeps[i] = keep;
-        if constexpr (V == 1) as[i] = a;
+        if constexpr (kFold) {
+          keeps[i] = C::pick(take<T, V>(raw[1].v[i]), keep, a);
+        } else {
+          keeps[i] = keep;
+          as[i] = a;
+        }
       }
       if constexpr (SUBS > 1) r = exchange.template go<true>(k & 1, me.sub, me.lane, P, H, run);
-      // from its end: dx = (1 - a) G, dgate = w dx, r = a G.  Two channels: r = G - (1 - a) G in one rounding, since a third
-      // row of registers would cost blocks; beside 16-bit outputs its error of 2^-24 G is nothing.
+      // from its end: dx = (1 - a) G, dgate = w dx, r = a G
       long long to = (t0 + kSub - 1) * ystep;
 #pragma unroll
       for (int i = kSub - 1; i >= 0; --i) {
         if (W || i < st.end) {
-          const F G = C::add(take<T, V>(raw[2].v[i]), r), ox = C::mul(keeps[i], G);
-          if constexpr (V == 1) r = C::mul(as[i], G);
-          else r = C::fma(C::mul(keeps[i], C::of(-1.f)), G, G);
+          const F G = C::add(take<T, V>(raw[2].v[i]), r);
+          F ox = C::mul(keeps[i], G);
+          if constexpr (kFold) {
+            const F rest = C::fma(ox, C::of(-1.f), G), gate = take<T, V>(raw[1].v[i]);
+            r = C::pick(gate, rest, ox);
+            ox = C::pick(gate, ox, rest);
+          } else {
+            r = C::mul(as[i], G);
+          }
           if (p.dx) put<T, V, W>(dx + to, ox, st, i);
           if (p.dgate) put<T, V, W>(dg + to, C::mul(w[i], ox), st, i);
         }
@@ -691,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_wide_backward_kernel(const _
     }
 #pragma unroll
     for (int u = 0; u < WORDS; ++u) {
-      F keeps[S], w[S], as[W::kV == 1 ? S : 1];
+      F keeps[S], w[S], as[S];
 #pragma unroll
       for (int i = 0; i < S; ++i)
         if (on >> i & 1) {
@@ -700,14 +713,13 @@ __global__ void __launch_bounds__(kThreads, 4) scan_wide_backward_kernel(const _
           const F xi = take<T, W::kV>(xs[i].w[u]);
           w[i] = C::mul(a, C::fma(xi, C::of(-1.f), h[u]));
           h[u] = C::fma(a, h[u], C::mul(keeps[i], xi));
-          if constexpr (W::kV == 1) as[i] = a;
+          as[i] = a;
         }
 #pragma unroll
       for (int i = S - 1; i >= 0; --i)
         if (on >> i & 1) {
           const F G = C::add(take<T, W::kV>(ds[i].w[u]), r[u]), ox = C::mul(keeps[i], G);
-          if constexpr (W::kV == 1) r[u] = C::mul(as[i], G);
-          else r[u] = C::fma(C::mul(keeps[i], C::of(-1.f)), G, G);
+          r[u] = C::mul(as[i], G);
           xs[i].w[u] = W::pack(ox);
           gs[i].w[u] = W::pack(C::mul(w[i], ox));
         }

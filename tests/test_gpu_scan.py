@@ -392,3 +392,23 @@ def test_open_gates_hold_the_state(n, t, c, dtype):
     tol = (t * share + 2.0**-50) * h.double().abs()
     assert (off <= tol).all(), float((off / tol).max())
     assert torch.equal(y[:, -1], last.to(dtype))
+
+
+# 16 bytes of a row a thread (once, walking), a thread a line, a line's warps, its pieces
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,t,c", [(5, 4, 64), (600, 9, 512), (300, 40, 260), (40, 16, 10), (2, 100, 32), (1, 3000, 6)])
+def test_gradients_through_closed_gates_keep_their_precision(n, t, c, dtype):
+    # a gradient from `last` alone passes closed gates, a of 4e-8 to 3e-4: what is left keeps a relative error.  The bounds of
+    # fp32 data (r = a G off by k a |G|) for all types
+    x, gate, h, _, dy, dlast = inputs((n, t, c), 1, dtype, seed=t)
+    g = torch.Generator().manual_seed(t + 1)
+    closed = torch.rand((n, t, c), generator=g) < min(0.3, 3 / t)
+    shut = (-8 - 9 * torch.rand((n, t, c), generator=g)).to(dtype)
+    gate = torch.where(closed, shut, gate)
+    dy = torch.zeros_like(dy)
+    want, bound = bounds(x.float(), gate.float(), h, 1, False, None, dy.float(), dlast)
+    leaves = [v.to(DEV).requires_grad_() for v in (x, gate, h)]
+    y, last = ops.gated_scan(*leaves, dim=1)
+    grads = torch.autograd.grad([last], leaves, [dlast.to(DEV)])
+    for name, got in zip(("x", "gate", "state"), grads):
+        close(got, want[name], bound[name], name)
