@@ -123,11 +123,14 @@ class Muon(torch.optim.Optimizer):
     float16 matrices; momenta are float32."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, steps: int = 5):
-        params = list(params)
-        for p in params:
-            if p.dim() != 2 or p.dtype not in (torch.bfloat16, torch.float16):
-                raise ValueError(f"Muon takes bfloat16 and float16 matrices, not {p.dtype} {tuple(p.shape)}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, steps=steps))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2 or p.dtype not in (torch.bfloat16, torch.float16):
+                self.param_groups.pop()
+                raise ValueError(f"Muon takes bfloat16 and float16 matrices, not {p.dtype} {tuple(p.shape)}")
 
     @torch.no_grad()
     def step(self, closure=None):

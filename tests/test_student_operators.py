@@ -11,6 +11,7 @@ import oracle.cell_operators as O
 from ncas_b200 import _lib as L
 from ncas_b200 import operators as ops
 from ncas_b200.build import build
+from ncas_b200.student import Muon
 
 
 @pytest.fixture(scope="module")
@@ -83,6 +84,20 @@ def test_oracle_sample_is_the_definition():
     assert pick(0.7, temperature=0.0) == 1 and pick(1.0) == 4 and pick(1.0, top_k=3) == 3
     tokens, probs, _ = O.sample(torch.full((1, 3), -math.inf), torch.tensor([[0.5, 0.1]]))
     assert tokens.tolist() == [[-1, -1]] and probs.tolist() == [[0.0, 0.0]]
+
+
+# ------------------------------------------------------------------------------- the optimiser
+def test_muon_takes_parameter_groups():
+    matrix = lambda: torch.nn.Parameter(torch.zeros(4, 6, dtype=torch.bfloat16))  # noqa: E731
+    opt = Muon([{"params": [matrix()], "lr": 0.1}, {"params": [matrix(), matrix()], "momentum": 0.5}], lr=0.02)
+    assert [(g["lr"], g["momentum"], len(g["params"])) for g in opt.param_groups] == [(0.1, 0.95, 1), (0.02, 0.5, 2)]
+    opt.add_param_group({"params": matrix(), "steps": 3})
+    for bad in (torch.zeros(4, dtype=torch.bfloat16), torch.zeros(4, 4)):
+        with pytest.raises(ValueError, match="Muon"):
+            opt.add_param_group({"params": [matrix(), torch.nn.Parameter(bad)]})
+        with pytest.raises(ValueError, match="Muon"):
+            Muon([{"params": [torch.nn.Parameter(bad)]}])
+    assert len(opt.param_groups) == 3 and opt.param_groups[2]["steps"] == 3
 
 
 # ------------------------------------------------------------------------------- refusals
