@@ -132,6 +132,15 @@ class Muon(torch.optim.Optimizer):
                 self.param_groups.pop()
                 raise ValueError(f"Muon takes bfloat16 and float16 matrices, not {p.dtype} {tuple(p.shape)}")
 
+    def load_state_dict(self, state_dict):
+        """Momenta stay float32 (the base class casts them to the type of their matrices), copies of the given ones."""
+        super().load_state_dict(state_dict)
+        names = [n for group in state_dict["param_groups"] for n in group["params"]]
+        for name, p in zip(names, (p for group in self.param_groups for p in group["params"])):
+            if "momentum" in state_dict["state"].get(name, {}):
+                momentum = state_dict["state"][name]["momentum"]
+                self.state[p]["momentum"] = momentum.to(device=p.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

@@ -100,6 +100,52 @@ def test_muon_takes_parameter_groups():
     assert len(opt.param_groups) == 3 and opt.param_groups[2]["steps"] == 3
 
 
+@pytest.fixture
+def plain_orthogonalize(monkeypatch):
+    """Muon on the CPU: the operator's formula in 64 bits in its place."""
+    monkeypatch.setattr(ops, "orthogonalize", lambda m, **kw: O.orthogonalize(m, **kw).to(m.dtype))
+
+
+def gradients(params, seed):
+    for i, p in enumerate(params):
+        p.grad = rand(*p.shape, seed=seed + i).to(p.dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_resumed_muon_goes_on_as_if_never_stopped(plain_orthogonalize, dtype, tmp_path):
+    def fresh():
+        params = [torch.nn.Parameter(rand(6, 9, seed=i).to(dtype)) for i in range(3)]
+        return params, Muon([{"params": params[:2], "lr": 0.1}, {"params": params[2:]}], lr=0.05)
+
+    one, opt = fresh()
+    for step in range(4):
+        gradients(one, 10 * step)
+        opt.step()
+        if step == 1:
+            torch.save((one, opt.state_dict()), tmp_path / "at_two")
+            kept = opt.state_dict()
+    two, resumed = fresh()
+    weights, state = torch.load(tmp_path / "at_two", weights_only=False)
+    resumed.load_state_dict(state)
+    for p, w in zip(two, weights):
+        p.data.copy_(w.data)
+        assert resumed.state[p]["momentum"].dtype == torch.float32
+    for step in (2, 3):
+        gradients(two, 10 * step)
+        resumed.step()
+    for a, b in zip(one, two):
+        assert torch.equal(a, b) and torch.equal(opt.state[a]["momentum"], resumed.state[b]["momentum"])
+    assert resumed.param_groups[0]["lr"] == 0.1 and resumed.param_groups[1]["lr"] == 0.05
+    # the dict that was given is not the resumed optimiser's own state; a state without momenta is one of no steps
+    live = kept["state"][0]["momentum"].clone()
+    resumed.load_state_dict(kept)
+    gradients(two, 50)
+    resumed.step()
+    assert torch.equal(kept["state"][0]["momentum"], live)
+    resumed.load_state_dict(fresh()[1].state_dict())
+    assert not resumed.state
+
+
 # ------------------------------------------------------------------------------- refusals
 def test_cpu_tensors_are_refused():
     x = torch.zeros(2, 3, 4)
