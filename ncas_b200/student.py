@@ -117,6 +117,17 @@ def teacher_top(engine, inputs, given, top: int, steps: int, p_fire: float = 0.5
     return values.contiguous(), index.to(torch.int32).contiguous()
 
 
+def near_one(matrices: torch.Tensor) -> torch.Tensor:
+    """float32 matrices (..., rows, cols), each times the power of two that brings its largest entry to [1/2, 1).  What is
+    orthogonalised does not depend on its size, but fp16 holds no more than 65504 and little below 6e-8."""
+    if matrices.numel() == 0:
+        return matrices
+    exponent = torch.frexp(matrices.abs().amax((-2, -1), keepdim=True)).exponent
+    half = torch.div(exponent, 2, rounding_mode="floor")  # two factors: 2^149 is no float32
+    power = lambda n: ((n + 127) << 23).view(torch.float32)  # noqa: E731  exact
+    return matrices * power(-half) * power(half - exponent)
+
+
 class Muon(torch.optim.Optimizer):
     """Momentum whose matrices are orthogonalised before they are added: an update of w (out, in) has all its singular
     values near 1, times lr sqrt(max(1, out / in)).  Matrices of one shape are orthogonalised in one call.  Takes bfloat16 and
@@ -158,10 +169,11 @@ class Muon(torch.optim.Optimizer):
                 m = state["momentum"]
                 m.mul_(group["momentum"]).add_(p.grad)
                 update = p.grad.float().add(m, alpha=group["momentum"]) if group["nesterov"] else m
-                shapes.setdefault((p.shape, p.dtype, p.device), []).append((p, update.to(p.dtype)))
-            for (shape, _, _), pairs in shapes.items():
+                shapes.setdefault((p.shape, p.dtype, p.device), []).append((p, update))
+            for (shape, dtype, _), pairs in shapes.items():
                 rates = -group["lr"] * max(1.0, shape[0] / shape[1]) ** 0.5
-                for (p, _), u in zip(pairs, ops.orthogonalize(torch.stack([u for _, u in pairs]), steps=group["steps"])):
+                updates = near_one(torch.stack([u for _, u in pairs])).to(dtype)
+                for (p, _), u in zip(pairs, ops.orthogonalize(updates, steps=group["steps"])):
                     p.add_(u, alpha=rates)
         return loss
 

@@ -118,6 +118,24 @@ def test_muon_adds_orthogonalised_momenta():
             Muon([torch.nn.Parameter(bad)])
 
 
+@pytest.mark.parametrize("size,steps", [(3e4, 20), (1e-7, 1)])
+def test_muon_of_fp16_matrices_at_the_ends_of_their_range(size, steps):
+    # momenta beyond 65504, and updates of one or two steps of fp16: as the same gradients of about 1 move them
+    g = torch.Generator(device=DEV).manual_seed(4)
+    sign = (torch.rand((48, 64), generator=g, device=DEV) < 0.5).half() * 2 - 1
+    params = [torch.nn.Parameter(torch.zeros(48, 64, device=DEV, dtype=torch.float16)) for _ in range(2)]
+    opts = [Muon([p], lr=0.5) for p in params]
+    for p, opt, scale in zip(params, opts, (size, 1.0)):
+        p.grad = sign * scale
+        for _ in range(steps):
+            p.data.zero_()
+            opt.step()
+    ops.check()
+    assert params[1].abs().max() > 0.01
+    # entries of one size: after the scaling both are the same matrix, but for the rounding of 20 sums of fp32
+    assert (params[0].double() - params[1].double()).norm() <= 2.0**-10 * params[1].double().norm()
+
+
 def test_every_parameter_has_an_optimizer():
     student = Student(10, 32, 64, 9, scan=True)
     for name in ("adam", "muon"):

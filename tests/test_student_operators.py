@@ -11,7 +11,7 @@ import oracle.cell_operators as O
 from ncas_b200 import _lib as L
 from ncas_b200 import operators as ops
 from ncas_b200.build import build
-from ncas_b200.student import Muon
+from ncas_b200.student import Muon, near_one
 
 
 @pytest.fixture(scope="module")
@@ -144,6 +144,53 @@ def test_a_resumed_muon_goes_on_as_if_never_stopped(plain_orthogonalize, dtype, 
     assert torch.equal(kept["state"][0]["momentum"], live)
     resumed.load_state_dict(fresh()[1].state_dict())
     assert not resumed.state
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [1e-7, 1e-30, 3e4, 1e36])
+def test_an_update_does_not_depend_on_the_size_of_its_gradients(plain_orthogonalize, size, dtype):
+    # the same gradients times a power of two give the same bits, but for eps = 1e-7 of the smaller one's norm, which the
+    # largest entry's scale keeps near 1; the optimiser's grad is of the matrix's type, whose range the sizes stay in
+    exponent = math.floor(math.log2(size if dtype == torch.bfloat16 else min(max(size, 2.0**-11), 3e4)))
+
+    def run(scale):
+        p = torch.nn.Parameter(torch.zeros(5, 7, dtype=dtype))
+        opt = Muon([p], lr=1.0)
+        for seed in range(3):
+            p.grad = ((rand(5, 7, seed=seed).clamp(-1, 1) * 64).round() / 64 * scale).to(dtype)
+            opt.step()
+        return p.detach()
+
+    got, want = run(2.0**exponent), run(1.0)
+    assert want.abs().max() > 0.1 and torch.equal(got, want)
+
+
+def test_tiny_and_huge_fp16_momenta(plain_orthogonalize):
+    # gradients at the ends of fp16: the momentum of many of 3e4 passes 65504, the update of one of 6e-8 is one step of the type
+    for size, steps in ((3e4, 20), (6e-8, 1)):
+        p = torch.nn.Parameter(torch.zeros(4, 4, dtype=torch.float16))
+        opt = Muon([p], lr=0.5, nesterov=False)
+        p.grad = (torch.eye(4) * size).half()
+        for _ in range(steps):
+            p.data.zero_()
+            opt.step()
+        # singular values of a multiple of the identity: 0.5 to begin with, then five steps of the polynomial
+        want = -0.5 * O.orthogonalize(torch.eye(4))
+        assert (p.double() - want).abs().max() <= 2.0**-10
+    zero = torch.nn.Parameter(torch.ones(3, 4, dtype=torch.float16))
+    zero.grad = torch.zeros_like(zero)
+    Muon([zero]).step()
+    assert (zero == 1).all()
+
+
+def test_near_one_multiplies_by_powers_of_two():
+    ends = torch.tensor([2.0**-149, -(2.0**-126), 3.0, 3.4e38, -1.0, 0.5, 0.0])
+    got = near_one(ends[:, None, None] * torch.tensor([[1.0, 0.5]]))
+    top = got.abs().amax((-2, -1))
+    assert ((top >= 0.5) & (top < 1))[:-1].all() and (got[-1] == 0).all()
+    assert (torch.frexp(got[:-1, 0, 0].abs()).mantissa == torch.frexp(ends[:-1].abs()).mantissa).all()
+    assert torch.equal(got[1:, 0, 1], got[1:, 0, 0] / 2)
+    assert near_one(torch.zeros(2, 0, 4)).shape == (2, 0, 4)
 
 
 # ------------------------------------------------------------------------------- refusals
