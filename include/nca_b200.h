@@ -482,7 +482,8 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
  * equal ones by index.  Kept are the first top_k (0: all); of those, the ones before which less than top_p of their mass
  * lies; of those, the ones with w_i >= min_p.  tokens[r][k] is the first kept class, by index, at which the sum of the
  * kept w exceeds uniforms[r][k] times the whole (the last kept one where there is none), probs[r][k] (may be NULL) its share
- * of the kept mass.  NaN counts as -inf; +inf beats every finite logit; a row of -inf alone gives -1 and 0.  temperature 0: the first
+ * of the kept mass.  w are whole multiples of 2^-bits, 51 bits up to 2048 classes and one less for every doubling up to 2^19;
+ * beyond, 62 less those of the row's sum of w, 51 at most.  NaN counts as -inf; +inf beats every finite logit; a row of -inf alone gives -1 and 0.  temperature 0: the first
  * of the largest. */
 typedef struct NcaSampleDesc {
   int64_t rows, classes, draws;

@@ -6,8 +6,12 @@
 // the first class, by index, at which the sum of the kept w exceeds u times the whole.
 //
 // The answers are whole numbers, and a row of 131072 classes has a border every 1e-5 of its mass: weights are computed in
-// 64 bits, so that an answer other than the exact one takes a u within about 1e-13 of a border.  Sums are in fixed
-// point: they do not depend on an order, and a class of no mass is never drawn.  The exponential is table-driven
+// 64 bits, to 1e-14 of themselves.  Sums are in fixed point: they do not depend on an order.  The largest weight is 2^bits of
+// its units: 51 bits up to 2048 classes, one less for every doubling to 43 at 2^19, so that a row of nothing but large weights
+// still adds up within 2^62.  A weight is off by half a unit at most and one below that has no mass, so a border is off by
+// classes 2^-(bits + 1) of the largest weight at most: 5e-13 at 2048 classes, 2e-9 at 131072, 3e-8 at 2^19, half the spacing of
+// uniform numbers beside 1.  Beyond, where that would be 12 % at 2^30, another pass bounds the row's sum first and the bits
+// follow from it (62 less its own): classes 2^-52 of the sum at most, 2e-7 at 2^30.  The exponential is table-driven
 // (Tang, ACM TOMS 15, 1989): 2^(j / 32) from a table, e^r of |r| < 0.0109 by five terms, 12 operations in 64 bits with
 // the conversion to fixed point.  A table of 256 saves two of them and loses more by conflicts of banks (1024 x 131072 without
 // cuts: 232 against 216 us).
@@ -40,7 +44,7 @@ struct SampleParams {
   int classes, draws;
   int top_k;               // classes: all
   double inverse_t, top_p, min_p;
-  double one;              // a weight of 1 in fixed point
+  double one;              // a weight of 1 in fixed point (up to kKnown classes)
 };
 
 // -inf for NaN (drawn as little as -inf), 0 for -0.
@@ -226,6 +230,7 @@ constexpr float kPerBin = 100.f;  // the last holds all beyond 40.9, whose weigh
 constexpr int kSubBins = 256;
 constexpr int kMostSegments = 1024;
 constexpr int kMostTops = 2048;
+constexpr int kKnown = 1 << 19;   // classes up to which their number alone gives the fixed point
 
 // Floats in their order as whole numbers.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -341,6 +346,7 @@ struct Row {
   const uint4* base;  // this lane's 16 bytes of chunk 0
   int n, shift, chunks, per_segment, segments;  // chunks of a warp's vectors; of a segment
   float top, lowest;      // of the entries; what lies below `lowest` has no mass
+  double one;             // a weight of 1 in fixed point
   double steep, offset;   // v steep + offset = kTable log2(e) (v - top) / T
   bool far;               // ... but for a top whose offset 64 bits round
   uint64_t limit;         // places from here on are kept
@@ -357,8 +363,37 @@ struct Row {
     warp = threadIdx.x / 32;
     lane = threadIdx.x % 32;
     base = reinterpret_cast<const uint4*>(z - shift) + lane;
-    // a weight of 1 is p.one: sums are in fixed point
-    if (threadIdx.x < kTable) sh.table[threadIdx.x] = kPowers[threadIdx.x] * p.one;
+    set_one(p.one);
+  }
+  __device__ __forceinline__ void set_one(double o) {
+    one = o;
+    if (threadIdx.x < kTable) sh.table[threadIdx.x] = kPowers[threadIdx.x] * one;
+  }
+  // The fixed point of a row of many classes, from a bound of its sum of weights: 8 exponentials at a time add up in fp32, all in 64
+  // bits, each within 2e-5 (roundings of the exponent, 2^-23 of 60 octaves, and the exponential's).
+  __device__ __forceinline__ void fit_one() {
+    const float scale = (float)(p.inverse_t * 1.4426950408889634074);
+    double sum = 0;
+    each_chunk<2>([&](int, const E& e) {
+      float some = 0.f;
+#pragma unroll
+      for (int j = 0; j < kV; ++j) {
+        const float v = clean(e.at(j));
+        some += v == top ? 1.f : ex2((v - top) * scale);
+      }
+      sum += some;
+    });
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
+    if (lane == 0) sh.warp_sums[warp] = (uint64_t)__double_as_longlong(sum);
+    __syncthreads();
+    sum = 0;
+    for (int w = 0; w < kWarps; ++w) sum += __longlong_as_double((long long)sh.warp_sums[w]);
+    int bits = 51;
+    while (bits > 32 && 1.001 * sum > (double)(1ll << (62 - bits))) --bits;
+    set_one((double)(1ll << bits));
+    __syncthreads();
   }
   __device__ __forceinline__ void set_top(float t) {
     top = t;
@@ -423,7 +458,7 @@ struct Row {
   }
   __device__ __forceinline__ bool kept(float v, int i) const { return place_of(key_of(v), i) >= limit; }  // of a clean v
 
-  // exp((v - top) / T) times p.one
+  // exp((v - top) / T) times `one`
   template <bool FAR>
   __device__ __forceinline__ double weight_of(float v) const {
     if constexpr (FAR) {
@@ -596,7 +631,7 @@ struct Row {
 
   // The least place of a weight of min_p, by a search of 32 keys at a time (every warp for itself).
   __device__ __forceinline__ uint64_t limit_of_weight(double min_p) const {
-    const double least = min_p * p.one;
+    const double least = min_p * one;
     uint32_t lo = (uint32_t)(kPossible >> 32), hi = key_of(top);  // hi is heavy enough
     while (lo < hi) {
       const uint32_t step = (hi - lo + 30) / 31, at = min(lo + lane * step, hi);
@@ -1128,6 +1163,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) sample_row_kernel(con
     return;
   }
   r.set_top(top);
+  if (R::Sh::kLong && p.classes > kKnown) r.fit_one();
   const uint64_t least = p.min_p > 0.0 ? r.limit_of_weight(p.min_p) : kPossible;
   const bool middle_k = cut_k && !small_k && p.classes > R::Sh::kList && p.top_k <= R::Sh::kList * 3 / 4 &&
                         top < __int_as_float(0x7f800000);
@@ -1214,8 +1250,8 @@ extern "C" int32_t nca_b200_sample(const NcaSampleDesc* d, const void* logits, c
   p.inverse_t = d->temperature == 0 ? 1.0 : 1.0 / d->temperature;
   p.top_p = d->top_p;
   p.min_p = d->min_p;
-  int bits = 51;  // the sum of all weights stays below 2^62
-  while (d->classes > (1ll << (62 - bits))) --bits;
+  int bits = 51;  // the sum of all weights stays below 2^62; beyond kKnown classes the rows' own sums decide
+  while (std::min<int64_t>(d->classes, kKnown) > (1ll << (62 - bits))) --bits;
   p.one = (double)(1ll << bits);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return with_dtype(d->dtype, [&](auto t) -> int32_t {

@@ -114,9 +114,11 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     Classes in the order of their logits, the lower index first among equals.  Kept are the first top_k (0: all); of
     those, the ones before which less than top_p of their mass exp(logit / temperature) lies; of those, the ones of at
     least min_p times the largest one's mass.  A draw is the first kept class, by index, at which the sum of the kept
-    masses exceeds the uniform number times the whole; its probability is its share of it.  Weights and sums are
-    in 64 bits.  logits: float32, bfloat16 or float16, any strides; NaN counts as -inf; +inf beats every finite logit; a row
-    that is -inf alone gives -1 and 0.  temperature 0: the first of the largest.  Not differentiable.
+    masses exceeds the uniform number times the whole; its probability is its share of it.  Masses are computed in
+    64 bits and added up in fixed point: a border between two classes is off by 5e-13 of the largest mass at most up to 2048
+    classes, by 2e-9 at 131072 and 3e-8 at 2^19, and beyond by classes 2^-52 of the whole.  logits: float32, bfloat16 or
+    float16, any strides; NaN counts as -inf; +inf beats every finite logit; a row that is -inf alone gives -1 and 0.
+    temperature 0: the first of the largest.  Not differentiable.
     """
     return _op("sample")(logits, uniforms, temperature, top_k, top_p, min_p)
 

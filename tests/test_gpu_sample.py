@@ -268,3 +268,31 @@ def test_every_output_is_written(classes, scale, min_p, dtype):
     assert nearest > 1e-11
     assert torch.equal(tokens.cpu(), want)
     assert ((probs.cpu().double() - share).abs() <= share * 2.0**-24 + 1e-10).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("classes,tail", [(131072, 46.03), (131072, 45.51), (2**19, 44.1), (2**19 + 3, 44.1), (2**20 + 1, 43.2), (2**23, 40.6),
+                                          (2**23 + 7, 30.2), (2**23, 3.0)])
+def test_one_class_above_a_long_tail_of_equal_ones(classes, tail, dtype):
+    # a peak of weight 1 and the others at 2^-tail, about half a unit of the fixed point that so many heavy classes would need.
+    # Weights are rounded to 2^-bits of the largest: 62 bits less those of the number of classes (51 at most), from 2^19 classes on
+    # less those of the weights' sum.  A draw is off by half a unit of every class at most.
+    low = torch.tensor(-tail * math.log(2.0)).to(dtype)
+    w = math.exp(float(low))
+    total = 1 + (classes - 1) * w
+    bits = 62 - math.ceil(math.log2(classes if classes <= 2**19 else 2 * total))
+    slack = classes * 2.0 ** -(min(bits, 51) + 1) + 1e-13 * total
+    peak = classes // 3
+    z = torch.full((1, classes), float(low))
+    z[0, peak] = 0.0
+    inner = (torch.arange(1, 40, dtype=torch.float64) / 40 * (peak * w)) / total
+    outer = 1 - (torch.arange(1, 40, dtype=torch.float64) / 40 * ((classes - 1 - peak) * w)) / total
+    u = torch.cat([inner, outer, torch.linspace(0, 1, 40, dtype=torch.float64)[:-1]]).float()
+    tokens, probs = ops.sample(z.to(dtype).to(DEV), u[None].to(DEV))
+    at = tokens[0].cpu().double()
+    before = at * w + torch.where(at > peak, 1 - w, 0.0)  # the mass before the class that was drawn
+    own = torch.where(at == peak, 1.0, w)
+    t = u.double() * total
+    assert ((at >= 0) & (at < classes)).all()
+    assert (before - slack <= t).all() and (t < before + own + slack).all()
+    assert ((probs[0].cpu().double() - own / total).abs() <= own / total * 2.0**-24 + slack / total).all()
