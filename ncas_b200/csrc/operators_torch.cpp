@@ -718,7 +718,8 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
     const int64_t dim = ctx->saved_data["dim"].toInt();
     for (const Tensor& g : grads) no_tangent(g, "gated_scan", "the gradient");
     Scan a(x, gate, state, dim, ctx->saved_data["reverse"].toBool(), saved[3]);
-    const Tensor dy = grads[0].defined() ? grads[0] : at::zeros({1}, x.options()).expand(x.sizes());  // only `last` was used
+    // only `last` was used: one row of zeros, read in place
+    const Tensor dy = grads[0].defined() ? grads[0] : at::zeros({x.size(-1)}, x.options()).expand(x.sizes());
     a.set_dy(dy, dim);
     const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
     const Needs needs(ctx, {x, gate, state, saved[3]});

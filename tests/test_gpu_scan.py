@@ -412,3 +412,18 @@ def test_gradients_through_closed_gates_keep_their_precision(n, t, c, dtype):
     grads = torch.autograd.grad([last], leaves, [dlast.to(DEV)])
     for name, got in zip(("x", "gate", "state"), grads):
         close(got, want[name], bound[name], name)
+
+
+def test_a_gradient_of_last_alone_takes_no_copy():
+    # dx, dgate and the states of every 8 steps (held already), no third tensor of x's size
+    x = torch.randn((4, 4000, 512), device=DEV, dtype=torch.bfloat16).requires_grad_()
+    gate = torch.randn_like(x).requires_grad_()
+    last = ops.gated_scan(x, gate, dim=1)[1]
+    size = x.numel() * x.element_size()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(last, [x, gate], torch.ones_like(last))
+    assert torch.cuda.max_memory_allocated() - held <= 2.5 * size
+    y, last = ops.gated_scan(x, gate, dim=1)
+    full = torch.autograd.grad([y, last], [x, gate], [torch.zeros_like(y), torch.ones_like(last)])
+    assert all(torch.equal(a, b) for a, b in zip(grads, full))
