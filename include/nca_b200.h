@@ -445,7 +445,8 @@ typedef struct NcaScanDesc {
   int64_t mask_stride[3];
 } NcaScanDesc;
 
-/* Bytes of the buffer `saved` that a training forward fills for the backward call: states along the line. */
+/* Bytes of the buffer `saved` that a training forward fills for the backward call: states along the line.  It and the workspace
+ * start on 8 bytes at least. */
 int32_t nca_b200_gated_scan_saved_bytes(const NcaScanDesc* d, size_t* bytes);
 int32_t nca_b200_gated_scan_workspace(const NcaScanDesc* d, int32_t backward, size_t* bytes);
 /* state (before the first step; NULL: zeros) and last (after the last): device [n][m][channels] fp32. */

@@ -782,7 +782,9 @@ void strides(long long (&to)[3], const int64_t (&from)[3], const NcaScanDesc& d)
 const void* first(const void* p, const int64_t (&s)[3], const NcaScanDesc& d, size_t size) {
   return p && d.reverse && d.steps ? static_cast<const uint8_t*>(p) + (d.steps - 1) * s[2] * (int64_t)size : p;
 }
-bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 != 0; }
+bool misaligned(const void* p, int bytes = 4) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+// States in `saved` and maps in the workspace are read and written in pairs.
+constexpr int kPairBytes = 8;
 
 // Lines that a thread with 8 channels walks along are fewer threads than with 2, and each waits for its own loads: worth it
 // for up to 64 steps (250 x 59 x 59, 32 channels, masked: 34 against 44 us forward; 800 lines of 200 steps, 512 channels, 98
@@ -866,8 +868,10 @@ int32_t nca_b200_gated_scan(const NcaScanDesc* d, const void* x, const void* gat
   if (p.columns == 0) return NCA_OK;
   if (!last || (d->steps && (!x || !gate || !y)) || (d->masked && d->steps && !mask)) return NCA_ERR_INVALID;
   if (two_wide(p) && (misaligned(x) || misaligned(gate) || misaligned(y))) return NCA_ERR_INVALID;
+  if (p.marks && misaligned(saved, kPairBytes)) return NCA_ERR_INVALID;
   const size_t need = workspace_of(p);
   if (need && (!workspace || workspace_bytes < need)) return NCA_ERR_SCRATCH;
+  if (need && misaligned(workspace, kPairBytes)) return NCA_ERR_INVALID;
   const size_t size = dtype_size(d->dtype);
   p.x = first(x, d->x_stride, *d, size);
   p.gate = first(gate, d->gate_stride, *d, size);
@@ -911,8 +915,10 @@ int32_t nca_b200_gated_scan_backward(const NcaScanDesc* d, const void* x, const 
   if ((d->steps && (!x || !gate || !dy)) || (p.marks && !saved) || (d->masked && d->steps && !mask)) return NCA_ERR_INVALID;
   if (two_wide(p) && (misaligned(x) || misaligned(gate) || misaligned(dy) || misaligned(dx) || misaligned(dgate)))
     return NCA_ERR_INVALID;
+  if (p.marks && misaligned(saved, kPairBytes)) return NCA_ERR_INVALID;
   const size_t need = workspace_of(p);
   if (need && (!workspace || workspace_bytes < need)) return NCA_ERR_SCRATCH;
+  if (need && misaligned(workspace, kPairBytes)) return NCA_ERR_INVALID;
   const size_t size = dtype_size(d->dtype);
   p.x = first(x, d->x_stride, *d, size);
   p.gate = first(gate, d->gate_stride, *d, size);

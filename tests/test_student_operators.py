@@ -252,6 +252,19 @@ def test_scan_pointers_and_workspace_are_checked_before_a_launch(lib):
     assert call(d) == 1
 
 
+def test_scan_buffers_of_pairs_start_on_8_bytes(lib):
+    # an address that nothing reads: the checks come before a launch; without room for the maps even a right call ends there
+    d = scan_desc(n=1, m=1, steps=100000)
+    p = 1 << 20
+    forward = lambda saved, ws, size: lib.nca_b200_gated_scan(C.byref(d), p, p, None, None, p, p, saved, ws, size, None)  # noqa: E731
+    backward = lambda saved, ws, size: lib.nca_b200_gated_scan_backward(  # noqa: E731
+        C.byref(d), p, p, None, None, saved, p, None, p, p, None, ws, size, None)
+    for call in (forward, backward):
+        assert call(p + 4, p, 8) == 1
+        assert call(p, p + 4, 1 << 30) == 1
+        assert call(p, p, 8) == call(p, None, 1 << 30) == 7
+
+
 def ortho_desc(**kw):
     d = L.NcaOrthoDesc(batch=2, rows=30, cols=50, dtype=1, steps=5, eps=1e-7)
     d.coefficients[:] = [3.4445, -4.775, 2.0315]
