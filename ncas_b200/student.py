@@ -171,7 +171,7 @@ class Muon(torch.optim.Optimizer):
                 update = p.grad.float().add(m, alpha=group["momentum"]) if group["nesterov"] else m
                 shapes.setdefault((p.shape, p.dtype, p.device), []).append((p, update))
             for (shape, dtype, _), pairs in shapes.items():
-                rates = -group["lr"] * max(1.0, shape[0] / shape[1]) ** 0.5
+                rates = -group["lr"] * max(1.0, shape[0] / max(1, shape[1])) ** 0.5
                 updates = near_one(torch.stack([u for _, u in pairs])).to(dtype)
                 for (p, _), u in zip(pairs, ops.orthogonalize(updates, steps=group["steps"])):
                     p.add_(u, alpha=rates)

@@ -183,6 +183,14 @@ def test_tiny_and_huge_fp16_momenta(plain_orthogonalize):
     assert (zero == 1).all()
 
 
+@pytest.mark.parametrize("shape", [(0, 4), (4, 0)])
+def test_muon_of_empty_matrices(monkeypatch, shape):
+    monkeypatch.setattr(ops, "orthogonalize", lambda m, **kw: m)
+    p = torch.nn.Parameter(torch.zeros(shape, dtype=torch.bfloat16))
+    p.grad = torch.zeros_like(p)
+    Muon([p]).step()
+
+
 def test_near_one_multiplies_by_powers_of_two():
     ends = torch.tensor([2.0**-149, -(2.0**-126), 3.0, 3.4e38, -1.0, 0.5, 0.0])
     got = near_one(ends[:, None, None] * torch.tensor([[1.0, 0.5]]))
