@@ -13,7 +13,11 @@
 // the result's norm a step, beside the 1.7e-3 of its own rounding to bf16 (2e-4 to fp16).  They have arrived
 // about log(sqrt(rows)) / log(a) steps from the start, so of a bf16 matrix the steps beyond the first three from there on (5
 // steps: matrices of fewer than 140 rows) read B and X in 22 bits in the largest product, hi hi + hi lo + lo hi, and of a
-// fp16 matrix all of them in all three products.  Errors are then 1.0 to 1.4 times the rounding's.
+// fp16 matrix all of them in all three products.  Of matrices of fewer than 64 rows all steps
+// do so in all products, whichever the type: nothing averages the few roundings of a small matrix, and beside a norm of sqrt(rows) an
+// error of a strong direction weighs more (16 x 24 fp16, 6 steps: up to 4.6 times the rounding's without, 8 x 12
+// bf16 3.5; 48 x 240 takes 36 us without and 48 with them in bf16, 45 and 48 in fp16).  Errors are
+// then 1.0 to 1.5 times the rounding's.
 //
 // A and A^2 are symmetric: tiles above the diagonal are computed, and stored twice.  Where a product has few tiles, a
 // cluster of 2 or 4 CTAs shares the k axis of each: every CTA adds up a share of the tile's columns through distributed
@@ -21,7 +25,8 @@
 //
 // Matrices of up to 128 x 256 (and 256 x 256 where no step takes operands of 22 bits) run in one launch: a CTA (or a pair,
 // cta_group::2) holds X as MMA operands in shared memory and in fp32 in tensor memory, beside the accumulator, for all
-// steps.  256 x 256, 5 steps: 57 us, as 17 launches 98; a phase is about 2400 cycles of MMAs, 1400 to 3100 of epilogue and 1300 of
+// steps.  256 x 256, 5 steps: 57 us, as 17 launches 98 (fp16 125 and 6 steps of bf16 128,
+// which have no such form); a phase is about 2400 cycles of MMAs, 1400 to 3100 of epilogue and 1300 of
 // cluster barrier (with twice the epilogue warps the same time), and 7 us pass before the first.
 //
 // Else one product kernel, built as gemm.cuh's: a persistent CTA or CTA pair (cta_group::2) a multiprocessor, warp 0
@@ -1093,9 +1098,14 @@ int32_t check_desc(const NcaOrthoDesc* d) {
   return NCA_OK;
 }
 
+// Whether a step with operands of 22 bits has them in all three products.
+constexpr int64_t kFewRows = 64;
+bool few_rows(const NcaOrthoDesc& d) { return std::min(d.rows, d.cols) < kFewRows; }
+bool all_products(const NcaOrthoDesc& d) { return d.dtype == NCA_F16 || few_rows(d); }
 // How many of the last steps take operands of 22 bits.
 int precise_steps(const NcaOrthoDesc& d) {
-  const double small = (double)std::max<int64_t>(1, std::min(d.rows, d.cols)), a = std::fabs(d.coefficients[0]);
+  if (few_rows(d)) return d.steps;
+  const double small = (double)std::min(d.rows, d.cols), a = std::fabs(d.coefficients[0]);
   const double arrived = a > 1.05 ? std::max(0.0, d.steps - 0.5 * std::log(small) / std::log(a)) : d.steps;
   if (d.dtype == NCA_F16) return (int)std::min<double>(d.steps, std::ceil(arrived));
   return arrived <= 3.0 ? 0 : (int)std::ceil(arrived - 1.2);
@@ -1208,7 +1218,7 @@ int32_t held(const NcaOrthoDesc& d, const void* matrix, void* out, int32_t* ctrl
                  reinterpret_cast<uintptr_t>(matrix) % 16 == 0;
   p.wide_stores = !tall && d.cols % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   p.precise = precise_steps(d);
-  p.all = d.dtype == NCA_F16;
+  p.all = all_products(d);
   const double scale_b = scale_of_b(d);
   p.a = (float)d.coefficients[0];
   p.a_scale = kScaleA / (kScaleX * kScaleX);
@@ -1274,7 +1284,7 @@ int32_t nca_b200_orthogonalize(const NcaOrthoDesc* d, const void* matrix, void* 
   p.out_bf16 = d->dtype == NCA_BF16;
   for (int k = 0; k < d->steps; ++k) {
     const Stack x[2] = {x_of(k & 1, 0), x_of(k & 1, 1)};
-    const bool last = k + 1 == d->steps, precise = k + precise_steps(*d) >= d->steps, all = precise && d->dtype == NCA_F16;
+    const bool last = k + 1 == d->steps, precise = k + precise_steps(*d) >= d->steps, all = precise && all_products(*d);
     p.passes = all ? 3 : 1;
     p.m = p.n = (int)pl.small;
     p.symmetric = 1;

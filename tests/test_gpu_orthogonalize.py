@@ -247,3 +247,25 @@ def test_two_graphs_in_turn_and_another_stream(shape):
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(beside, want[0])
     ops.check()
+
+
+def strong_and_weak(rows, cols, dtype, seed):
+    """A strong direction over noise, as a momentum."""
+    g = torch.Generator().manual_seed(seed)
+    return ((torch.randn((rows, 1), generator=g) @ torch.randn((1, cols), generator=g) + 0.5 * torch.randn((rows, cols), generator=g)) * 0.01).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols,steps", [(16, 24, 6), (24, 16, 5), (13, 19, 6), (8, 12, 6), (8, 300, 5), (40, 400, 6), (63, 90, 5)])
+def test_small_matrices_are_as_exact_as_their_type(rows, cols, steps, dtype):
+    # all operands have 22 bits: what is left is the result's own rounding, whose norm over n values is within a factor
+    # 1 + 6 / sqrt(n) of that of the exact result, and the roundings that the oracle can make (factor 4, above).  A whole stack at
+    # once: some of its matrices were off by 2 to 4 times the rounding with 11 bits in the first step
+    m = torch.stack([strong_and_weak(rows, cols, dtype, seed) for seed in range(20)] +
+                    [matrix((rows, cols), dtype, seed=seed) for seed in range(20)])
+    got = ops.orthogonalize(m.to(DEV), steps=steps).double().cpu()
+    ops.check()
+    want, near = O.orthogonalize(m, steps), O.orthogonalize(m, steps, rounded=True)
+    norm = lambda t: t.flatten(1).norm(dim=1)  # noqa: E731
+    tol = (1 + 6 / (rows * cols) ** 0.5) * norm(want.to(dtype).double() - want) + 4 * norm(near - want) + 2.0**-25 * (rows * cols) ** 0.5
+    assert (norm(got - want) <= tol).all(), float((norm(got - want) / tol).max())
