@@ -14,7 +14,7 @@
 // follow from it (62 less its own): classes 2^-52 of the sum at most, 2e-7 at 2^30.  The exponential is table-driven
 // (Tang, ACM TOMS 15, 1989): 2^(j / 32) from a table, e^r of |r| < 0.0109 by five terms, 12 operations in 64 bits with
 // the conversion to fixed point.  A table of 256 saves two of them and loses more by conflicts of banks (1024 x 131072 without
-// cuts: 232 against 216 us).
+// cuts: 7 % slower than the 190 us of now).
 //
 // Up to 32 classes a row is a group of lanes, a class a lane, and ranks are counted.  Longer rows are a block's.  All three
 // cuts keep a prefix of the order, so the kept set is always "from a place (z, index) on".
@@ -877,7 +877,8 @@ struct Row {
         if (sh.list[i] >= at) join(sh.list[i], mass(value_of(sh.list[i])));
       limit = max(at, least);
       __syncthreads();
-      // the sums hold all above the list: where min_p cuts some of those too, they come again
+      // the sums hold all above the list: where min_p cuts some of those too, they come again (in few rows: 1024 x 131072 bf16, top-p
+      // 0.95 and min-p 0.02 take 196 us)
       return value_of(least) > high ? kCut : kSummed;
     } else {
       return kNot;
@@ -1262,8 +1263,10 @@ extern "C" int32_t nca_b200_sample(const NcaSampleDesc* d, const void* logits, c
     if (p.classes <= 8) return few<T, 8>(p, s);
     if (p.classes <= 16) return few<T, 16>(p, s);
     if (p.classes <= 32) return few<T, 32>(p, s);
-    // Smaller blocks, more rows at once, hide each other's short steps (2047 x 32003 fp16, top-k 50: 101 against 141 us); top-p
-    // alone has few of them and works through its list faster in large ones (348 against 432 us, top-p 0.95).
+    // Smaller blocks, more rows at once, hide each other's short steps (2047 x 32003 fp16, top-k 50: 93 against 127 us, without cuts 104
+    // against 122); top-p alone has few of them and works through its list faster in large ones (1024 x 20000 bf16, top-p 0.95: 110
+    // against 121, 1024 x 131072 365 against 387), as longer rows do (131072 without cuts 190 against 199, min-p alone 126 against 134;
+    // top-k 50 is the exception, 117 against 110).
     if (p.classes <= RowShared<128>::kList) return row_blocks<T, 128>(p, s);
     const bool by_mass = p.top_p < 1.0 && p.top_k == p.classes;
     return p.classes <= 65536 && !by_mass ? row_blocks<T, 256>(p, s) : row_blocks<T, 512>(p, s);

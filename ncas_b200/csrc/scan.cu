@@ -17,10 +17,13 @@
 // from the end; the states come again from the inputs, from the state that the forward pass stored before
 // each kSub steps (4 bytes for kSub elements).
 //
-// 72000 lines of 9 steps, 64 channels, bf16 take 43 us forward and 89 backward (90 and 75 % of the HBM rate; 62 and 115 with two
-// channels a thread), 100000 single steps of 504 channels 90 and 208 (389 and 690).  One line of 100001 steps, 1024 channels
-// takes 198 us forward (80 of them for the pieces' maps) and 282 backward (83), at 59 to 66 % of the DRAM cycles and 53 to 62 %
-// of the issue slots; with 16 steps a thread 217 and 331, for their registers.
+// 72000 lines of 9 steps, 64 channels, bf16 take 44 us forward and 94 backward (87 and 67 % of the HBM rate; with two channels
+// a thread 62 and 115 where these took 43 and 89, before `a` had its present form), 100000 single steps of 504 channels 93 and 217
+// (two channels: 389 and 690).  One line of 100001 steps, 1024 channels takes 203 us forward (87 of them for the pieces' maps) and 289
+// backward (88), at 55 to 62 % of the DRAM cycles and 57 to 67 % of the issue slots; with 16 steps a thread 217 and 331, for their
+// registers.  Passes in a row take 580 to 595 in all, 80 to 100 more than the two alone: a kernel that starts while the one before
+// ends settles on the multiprocessors that are free first, up to 8 blocks on one, and its grid holds no more than 5 for each (510 to
+// 530 where every kernel waits for the one before).
 #include "cell_ops.cuh"
 
 #include <algorithm>
@@ -537,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksBack) scan_backward_kernel(co
 
 // ------------------------------------------------------------------------------- many or short lines
 // A thread takes WORDS words of a row, up to 16 bytes, of S steps at a time, alone along its line.  PLAIN: the compiler orders
-// loads and places (4 steps: backward 55 against 68 us; of 8 steps it would keep 276 bytes outside of the registers).
+// loads and places (4 steps: backward 55 against 68 us when it was chosen; of 8 steps it would keep 276 bytes outside of the registers).
 template <class T, int WORDS, int S, bool PLAIN>
 struct Wide {
   static constexpr int kV = sizeof(T) == 2 ? 2 : 1, kChannels = WORDS * kV;  // of a word; of a thread

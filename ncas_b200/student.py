@@ -179,7 +179,7 @@ class Muon(torch.optim.Optimizer):
 
 
 def make_optimizers(student: Student, name: str = "adam", lr: float = 3e-3) -> list[torch.optim.Optimizer]:
-    """"adam": Adam for all; "muon": Muon for the cell's matrices, Adam for the rest."""
+    """"adam": Adam for all; "muon": Muon for the cell's matrices (with its own lr), Adam for the rest.  lr: Adam's."""
     if name == "adam":
         return [torch.optim.Adam(student.parameters(), lr=lr)]
     if name != "muon":
