@@ -836,7 +836,7 @@ __global__ void __launch_bounds__(kHeldThreads, 1) ortho_held_kernel(const __gri
   meet();
 
   bool ok = true;
-  uint32_t ph = 0;
+  uint32_t ph = 0, issued = 0;  // issued: the parity of the last phase whose MMAs were issued
   // D = a b^T over `blocks` of 16 k; b MN-major for the last product
   const auto multiply = [&](uint32_t a, uint32_t b, int blocks, bool mn, int n, bool more) {
     const uint32_t idesc = (1u << 4) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
@@ -857,7 +857,7 @@ __global__ void __launch_bounds__(kHeldThreads, 1) ortho_held_kernel(const __gri
     const bool last = k + 1 == p.steps, precise = CG == 1 && precise_at(k), all = precise && p.all;
     for (int phase = 0; phase < 3; ++phase) {
       const bool three = phase < 2 ? all : precise;
-      if (issues) {
+      if (issues && ok) {  // after a wait that ran out no more: one phase at most is in flight at the end
         const uint32_t a = phase == 0 ? x : square, b = phase == 0 ? x : phase == 1 ? square : columns;
         const int blocks = phase == 0 ? large_blocks : small_blocks, n = phase < 2 ? S::kSquareCols : 256;
         multiply(a, b, blocks, phase == 2, n, false);
@@ -867,6 +867,7 @@ __global__ void __launch_bounds__(kHeldThreads, 1) ortho_held_kernel(const __gri
           multiply(al, b, blocks, phase == 2, n, true);
         }
         tc_commit<CG>(done);
+        issued = ph;
       }
       __syncwarp();
       if (ok) ok = mbar_wait_warp(done, ph, fs, 121 + phase);
@@ -946,7 +947,7 @@ __global__ void __launch_bounds__(kHeldThreads, 1) ortho_held_kernel(const __gri
   }
   // after a wait that ran out: the MMAs in flight end before the tensor memory is freed (bounded)
   if (issues && !ok)
-    for (int tries = 0; tries < 64 && !mbar_try_wait(done, ph ^ 1); ++tries) {
+    for (int tries = 0; tries < 64 && !mbar_try_wait(done, issued); ++tries) {
     }
   __syncwarp();
   cluster_sync_all();

@@ -84,3 +84,15 @@ def test_copies_and_products_in_flight_end_before_a_block_leaves():
     body = dict(kernels())["gemm_rows.cuh:gemm_rows_kernel"]
     assert "\n      for (int j = i > S::kStages ? i - S::kStages : 0; j < i; ++j)" in body
     assert body.count("mbar_try_wait(done, 0)") == 1
+
+
+def test_the_held_matrices_issue_no_products_after_a_failure():
+    # MMAs of several phases in flight could not be told apart by the parity of one barrier: after a wait that ran out none
+    # are issued, and the last ones that were are waited for before the tensor memory is freed
+    body = dict(kernels())["orthogonalize.cu:ortho_held_kernel"]
+    issue = body.index("if (issues && ok)")
+    commit = body.index("tc_commit<CG>(done);", issue)
+    assert body.count("tc_commit<CG>(done)") == 1 and "if (issues)" not in body
+    kept = body.index("issued = ph;", commit)
+    assert kept < body.index("ph ^= 1;", kept)
+    assert body.index("mbar_try_wait(done, issued)") < body.index("tc_dealloc<CG>(")
