@@ -16,8 +16,9 @@
 // fp16 matrix all of them in all three products.  Of matrices of fewer than 64 rows all steps
 // do so in all products, whichever the type: nothing averages the few roundings of a small matrix, and beside a norm of sqrt(rows) an
 // error of a strong direction weighs more (16 x 24 fp16, 6 steps: up to 4.6 times the rounding's without, 8 x 12
-// bf16 3.5; 48 x 240 takes 36 us without and 48 with them in bf16, 45 and 48 in fp16).  Errors are
-// then 1.0 to 1.5 times the rounding's.
+// bf16 3.5; 48 x 240 takes 36 us without and 48 with them in bf16, 45 and 48 in fp16).  One or two
+// steps of a fp16 matrix do too, for a strong direction has arrived before the first (with nearly all of the norm in it, 1 step: up
+// to 4.6 times the rounding's without; 1001 x 2730, 2 steps, 90 us without and 135 with them).  Errors of 1 to 8 steps are then 1.0 to 1.4 times the rounding's on average, 1.9 at most (bf16, 8 steps).
 //
 // A and A^2 are symmetric: tiles above the diagonal are computed, and stored twice.  Where a product has few tiles, a
 // cluster of 2 or 4 CTAs shares the k axis of each: every CTA adds up a share of the tile's columns through distributed
@@ -1101,11 +1102,12 @@ int32_t check_desc(const NcaOrthoDesc* d) {
 
 // Whether a step with operands of 22 bits has them in all three products.
 constexpr int64_t kFewRows = 64;
+constexpr int kFewSteps = 2;
 bool few_rows(const NcaOrthoDesc& d) { return std::min(d.rows, d.cols) < kFewRows; }
 bool all_products(const NcaOrthoDesc& d) { return d.dtype == NCA_F16 || few_rows(d); }
 // How many of the last steps take operands of 22 bits.
 int precise_steps(const NcaOrthoDesc& d) {
-  if (few_rows(d)) return d.steps;
+  if (few_rows(d) || (d.dtype == NCA_F16 && d.steps <= kFewSteps)) return d.steps;
   const double small = (double)std::min(d.rows, d.cols), a = std::fabs(d.coefficients[0]);
   const double arrived = a > 1.05 ? std::max(0.0, d.steps - 0.5 * std::log(small) / std::log(a)) : d.steps;
   if (d.dtype == NCA_F16) return (int)std::min<double>(d.steps, std::ceil(arrived));

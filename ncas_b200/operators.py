@@ -101,9 +101,9 @@ def orthogonalize(matrix, *, steps=5, coefficients=(3.4445, -4.775, 2.0315), eps
 
     bfloat16 or float16, any strides (adjacent columns are read in place, others copied); the result is contiguous and
     of the same type.  Products are summed in fp32 over fp16 operands, X keeps 22 bits between the steps, and the
-    result is rounded once: its error is 1.0 to 1.5 times that rounding.  Coefficients that let a singular value grow beyond
-    2 are refused.  A norm below a millionth of eps leaves X, and the result (then below 1e-3), fewer bits than its type has.
-    Not differentiable: for the update of an optimiser.  The first call on a device makes its control words: it must precede a stream capture.
+    result is rounded once: its error is 1.0 to 1.4 times that rounding on average, 1.9 at most (of up to 8 steps).
+    Coefficients that let a singular value grow beyond 2 are refused.  A norm below a millionth of eps leaves X, and the
+    result (then below 1e-3), fewer bits than its type has.  Not differentiable: for the update of an optimiser.  The first call on a device makes its control words: it must precede a stream capture.
     """
     return _op("orthogonalize")(matrix, steps, coefficients, eps)
 

@@ -140,7 +140,7 @@ def orthogonalize(m, steps=5, coefficients=(3.4445, -4.775, 2.0315), eps=1e-7, r
     a, b, c = coefficients
     once = lambda t, s: (t * s).half().double() / s if rounded else t  # noqa: E731
     twice = lambda t, s: once(t, s) + once(t - once(t, s), s) if rounded else t  # noqa: E731
-    few = min(m.shape[-2:]) < 64
+    few = min(m.shape[-2:]) < 64 or (m.dtype == torch.float16 and steps <= 2)
     full = m.dtype == torch.float16 or few
     arrived = max(0.0, steps - 0.5 * math.log(max(1, min(m.shape[-2:]))) / math.log(abs(a))) if abs(a) > 1.05 else steps
     precise = steps if few else min(steps, math.ceil(arrived)) if full else 0 if arrived <= 3 else math.ceil(arrived - 1.2)

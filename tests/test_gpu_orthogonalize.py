@@ -269,3 +269,18 @@ def test_small_matrices_are_as_exact_as_their_type(rows, cols, steps, dtype):
     norm = lambda t: t.flatten(1).norm(dim=1)  # noqa: E731
     tol = (1 + 6 / (rows * cols) ** 0.5) * norm(want.to(dtype).double() - want) + 4 * norm(near - want) + 2.0**-25 * (rows * cols) ** 0.5
     assert (norm(got - want) <= tol).all(), float((norm(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("steps", [1, 2])
+@pytest.mark.parametrize("rows,cols", [(64, 141), (425, 274), (100, 3000)])
+def test_few_steps_of_a_strong_direction(rows, cols, steps):
+    # fp16, a direction with nearly all of the norm: as above, all operands have 22 bits
+    noise = matrix((5, rows, cols), torch.float32, seed=rows, scale=0.005)
+    g = torch.Generator().manual_seed(cols)
+    m = (noise + 0.2 * torch.randn((5, rows, 1), generator=g) @ torch.randn((5, 1, cols), generator=g)).half()
+    got = ops.orthogonalize(m.to(DEV), steps=steps).double().cpu()
+    ops.check()
+    want, near = O.orthogonalize(m, steps), O.orthogonalize(m, steps, rounded=True)
+    norm = lambda t: t.flatten(1).norm(dim=1)  # noqa: E731
+    tol = (1 + 6 / (rows * cols) ** 0.5) * norm(want.half().double() - want) + 4 * norm(near - want) + 2.0**-25 * norm(want)
+    assert (norm(got - want) <= tol).all(), float((norm(got - want) / tol).max())
