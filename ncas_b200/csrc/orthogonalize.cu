@@ -18,7 +18,8 @@
 // error of a strong direction weighs more (16 x 24 fp16, 6 steps: up to 4.6 times the rounding's without, 8 x 12
 // bf16 3.5; 48 x 240 takes 36 us without and 48 with them in bf16, 45 and 48 in fp16).  One or two
 // steps of a fp16 matrix do too, for a strong direction has arrived before the first (with nearly all of the norm in it, 1 step: up
-// to 4.6 times the rounding's without; 1001 x 2730, 2 steps, 90 us without and 135 with them).  Errors of 1 to 8 steps are then 1.0 to 1.4 times the rounding's on average, 1.9 at most (bf16, 8 steps).
+// to 4.6 times the rounding's without; 1001 x 2730, 2 steps, 90 us without and 135 with them).  Errors of 1 to 8
+// steps are then 1.0 to 1.4 times the rounding's on average, 1.9 at most (bf16, 8 steps).
 //
 // A and A^2 are symmetric: tiles above the diagonal are computed, and stored twice.  Where a product has few tiles, a
 // cluster of 2 or 4 CTAs shares the k axis of each: every CTA adds up a share of the tile's columns through distributed
@@ -26,9 +27,9 @@
 //
 // Matrices of up to 128 x 256 (and 256 x 256 where no step takes operands of 22 bits) run in one launch: a CTA (or a pair,
 // cta_group::2) holds X as MMA operands in shared memory and in fp32 in tensor memory, beside the accumulator, for all
-// steps.  256 x 256, 5 steps: 57 us, as 17 launches 98 (fp16 125 and 6 steps of bf16 128,
-// which have no such form); a phase is about 2400 cycles of MMAs, 1400 to 3100 of epilogue and 1300 of
-// cluster barrier (with twice the epilogue warps the same time), and 7 us pass before the first.
+// steps.  256 x 256, 5 steps: 57 us, as 17 launches 98 (fp16 125 and 6 steps of bf16 128, which have no such form); a phase is
+// about 2400 cycles of MMAs, 1400 to 3100 of epilogue and 1300 of cluster barrier (with twice the epilogue warps the same time), and
+// 7 us pass before the first.
 //
 // Else one product kernel, built as gemm.cuh's: a persistent CTA or CTA pair (cta_group::2) a multiprocessor, warp 0
 // loads tiles by TMA, warp 1 issues the MMAs, warps 4-11 take the accumulators out, add the terms that they load by
